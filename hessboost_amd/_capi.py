@@ -23,6 +23,7 @@ OBJ_SQUARED_ERROR, OBJ_LOGISTIC, OBJ_SOFTMAX, OBJ_LOGITRAW = 0, 1, 2, 3
 GROW_DEPTHWISE, GROW_LOSSGUIDE = 0, 1
 SCAN_EMPTY, SCAN_REPLAY, SCAN_NUMERIC, SCAN_CATEGORICAL = 0, 1, 2, 3
 FALLBACK_NUMERIC_SCORE, FALLBACK_CATEGORICAL_ORDER, FALLBACK_CATEGORICAL_SCORE, FALLBACK_NEAR_TIE = 1, 2, 3, 4
+F32, BF16 = 0, 1
 TRANSFORM_SIGMOID, TRANSFORM_SOFTMAX, TRANSFORM_CLASS_INDEX = 1, 2, 3
 
 P = C.POINTER
@@ -116,6 +117,27 @@ class ForestDesc(C.Structure):
                 ("n_categories", C.c_uint64)]
 
 
+class Lookup(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("n_columns", C.c_uint32),
+                ("pad", C.c_uint32), ("table_rows", C.c_uint64), ("table_stride", C.c_uint64),
+                ("ids_stride", C.c_uint64), ("out_stride", C.c_uint64), ("ids", C.c_void_p), ("offset", C.c_void_p),
+                ("scale", C.c_void_p)]
+
+
+class Softmax(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("n_classes", C.c_uint32),
+                ("grad_scale", C.c_float), ("h_stride", C.c_uint64), ("w_stride", C.c_uint64),
+                ("dh_stride", C.c_uint64), ("dw_stride", C.c_uint64), ("h", C.c_void_p), ("w", C.c_void_p),
+                ("bias", C.c_void_p), ("labels", C.c_void_p), ("weight", C.c_void_p), ("loss", C.c_void_p),
+                ("lse", C.c_void_p), ("best", C.c_void_p), ("dh", C.c_void_p), ("dw", C.c_void_p),
+                ("db", C.c_void_p)]
+
+
+class Tensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("len", C.c_uint64), ("dtype", C.c_uint32),
+                ("pad", C.c_uint32)]
+
+
 # name -> (restype, argtypes); every entry point include/hessboost_rocm.h declares
 SIGNATURES = {
     "hbr_last_error": (C.c_size_t, [C.c_char_p, C.c_size_t]),
@@ -199,6 +221,16 @@ SIGNATURES = {
     "hbr_pred_transform": (C.c_int, [C.c_int, C.c_void_p, C.c_uint64, C.c_uint32]),
     "hbr_forest_set_profiling": (C.c_int, [C.c_void_p, C.c_int, C.c_char_p]),
     "hbr_forest_kernel_stats": (C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t]),
+    "hbr_leaf_embedding": (C.c_int, [C.c_int, P(Lookup), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "hbr_leaf_embedding_grad_workspace": (C.c_int, [P(Lookup), P(C.c_uint64)]),
+    "hbr_leaf_embedding_grad": (C.c_int, [C.c_int, P(Lookup), C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64,
+                                          C.c_void_p]),
+    "hbr_softmax_head_workspace": (C.c_int, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+                                             P(C.c_uint64)]),
+    "hbr_softmax_head": (C.c_int, [C.c_int, P(Softmax), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "hbr_clip_gradients_workspace": (C.c_int, [C.c_uint64, P(C.c_uint64)]),
+    "hbr_clip_gradients": (C.c_int, [C.c_int, P(Tensor), C.c_uint64, C.c_double, C.c_void_p, C.c_void_p, C.c_uint64,
+                                     C.c_void_p]),
     "hbr_device_alloc": (C.c_int, [C.c_int, C.c_uint64, P(C.c_void_p)]),
     "hbr_device_free": (C.c_int, [C.c_int, C.c_void_p]),
     "hbr_device_upload": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_uint64]),

@@ -1051,4 +1051,153 @@ struct PredictArgs {
 };
 constexpr uint32_t kPredCategorical = 1u << 29;
 
+// ---- operators over leaves and many classes --------------------------------------
+
+// Element types of the operators' arrays (HBR_F32, HBR_BF16).
+constexpr uint32_t kF32 = 0;
+constexpr uint32_t kBf16 = 1;
+
+// hbr_leaf_embed_*: out[r] = sum over columns t of scale[t] * table[offset[t] + ids[r][t]].
+struct EmbedArgs {
+    const void *table;
+    const int32_t *ids;
+    const int32_t *offset;  // per column, or null
+    const float *scale;     // per column, or null
+    void *out;
+    uint64_t n_rows;
+    uint64_t table_rows;
+    uint64_t table_stride;  // elements
+    uint64_t ids_stride;
+    uint64_t out_stride;
+    uint32_t columns;
+    uint32_t dim;
+    uint32_t vecs;            // vectors a row
+    uint32_t rows_per_block;
+};
+
+// Entries of one sort tile (hbr_sort_*): 256 threads x 16.
+constexpr uint32_t kSortTile = 4096;
+constexpr uint32_t kSortBits = 8;
+constexpr uint32_t kSortDigits = 1u << kSortBits;
+
+// The table gradient: the ids' entries (r, t) sorted by table row, stable.
+struct LookupSortArgs {
+    const int32_t *ids;
+    const int32_t *offset;
+    uint64_t ids_stride;
+    uint64_t table_rows;
+    uint32_t columns;
+    uint32_t n;               // entries: rows x columns
+    uint32_t tiles;
+    uint32_t shift;           // the pass's digit
+    const uint32_t *keys_in;  // null: the first pass, keys from the ids
+    const uint32_t *vals_in;
+    uint32_t *keys_out;
+    uint32_t *vals_out;
+    uint32_t *hist;           // [digit][tile]
+    uint32_t *total;          // [digit]
+};
+
+// The sorted entries' rows of dout summed per table row. An id that adds
+// nothing has the key table_rows, behind every other.
+struct LookupSumArgs {
+    const uint32_t *keys;
+    const uint32_t *vals;     // entry: r * columns + t
+    const void *dout;
+    const float *scale;
+    void *dtable;
+    uint32_t *start;          // table_rows + 1: each table row's first entry
+    float *part;              // [chunk][2][dim]
+    uint64_t table_rows;
+    uint64_t dout_stride;
+    uint64_t dtable_stride;
+    uint32_t n;
+    uint32_t columns;
+    uint32_t dim;
+    uint32_t vecs;
+    uint32_t chunk;           // entries a wave
+    uint32_t chunks;
+};
+
+// Rows x classes of one tile of the head's products.
+constexpr uint32_t kHeadTile = 64;
+
+// One product of the softmax head, C[m][n] = sum_k A(m, k) B(n, k), each
+// operand with its own element strides, and what its epilogue needs.
+struct HeadArgs {
+    const void *a;
+    const void *b;
+    uint64_t a_m, a_k, b_n, b_k;  // strides, elements
+    uint64_t m, n, k;
+    const int32_t *skip;          // per k: rows whose label is below 0 are not read (or null)
+    // scores: m rows, n classes from class `first` on
+    uint64_t first;
+    const float *bias;
+    const int32_t *labels;
+    float *part_max;              // [class tile][rows]
+    float *part_sum;
+    int32_t *part_best;           // or null
+    float *label_margin;          // [rows]
+    uint64_t rows;
+    // pairs: g[m][n] from the scores
+    const float *lse;
+    const float *weight;
+    float grad_scale;
+    uint32_t accumulate;          // add to c instead of overwriting it
+    void *g;
+    uint64_t g_stride;
+    float *part_db;               // [row tile][n]
+    // plain
+    void *c;
+    uint64_t c_stride;
+};
+
+struct HeadFinishArgs {
+    const float *part_max;
+    const float *part_sum;
+    const int32_t *part_best;
+    const float *label_margin;
+    const int32_t *labels;
+    const float *weight;
+    float *lse;
+    float *loss;      // or null
+    int32_t *best;    // or null
+    uint64_t rows;
+    uint64_t classes;
+    uint32_t tiles;
+    uint32_t pad;
+};
+
+// dst[i] = sum over parts of part[p][i], rounded to the type.
+struct HeadSumArgs {
+    const float *part;
+    void *dst;
+    uint64_t rows, cols, dst_stride;
+    uint64_t part_stride;
+    uint32_t parts;
+    uint32_t pad;
+};
+
+// hbr_clip_*: up to kClipTensors tensors a launch.
+constexpr uint32_t kClipTensors = 96;
+constexpr uint32_t kClipBlocks = 2048;  // workgroups, and partial sums, a launch at most
+constexpr uint32_t kClipElems = 8192;   // elements of one block
+struct ClipTensor {
+    const void *data;
+    void *out;
+    uint64_t len;
+    uint32_t block;  // the tensor's first block of the launch
+    uint32_t dtype;
+};
+struct ClipArgs {
+    ClipTensor t[kClipTensors];
+    uint32_t tensors;
+    uint32_t blocks;      // blocks of elements in the launch
+    uint32_t first_part;  // where the launch's partial sums begin
+    uint32_t parts;
+    double *part;
+    float *norm;          // or null
+    double max_norm;
+};
+
 }  // namespace hbr

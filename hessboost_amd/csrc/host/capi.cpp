@@ -10,6 +10,7 @@
 #include "cuts.h"
 #include "engine.h"
 #include "forest.h"
+#include "leafops.h"
 #include "noalloc.h"
 #include "split_math.h"
 #include "hessboost_rocm.h"
@@ -1022,6 +1023,59 @@ int hbr_forest_set_profiling(hbr_forest *h, int on, const char *prefix) {
 
 int hbr_forest_kernel_stats(hbr_forest *h, char *buf, size_t len) {
     return with_forest(h, [&](Forest &f) { copy_string(stats_string(f.dev()), buf, len); });
+}
+
+// ---- operators over leaves and many classes --------------------------------------------
+
+int hbr_leaf_embedding(int ordinal, const hbr_lookup *p, const void *table, void *out, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "leaf embedding: null argument");
+        leaf_embedding(ordinal, stream, *p, table, out);
+    });
+}
+
+int hbr_leaf_embedding_grad_workspace(const hbr_lookup *p, uint64_t *bytes) {
+    return guard([&] {
+        if (!p || !bytes) fail(kInvalid, "leaf embedding gradient: null argument");
+        *bytes = leaf_embedding_grad_workspace(*p);
+    });
+}
+
+int hbr_leaf_embedding_grad(int ordinal, const hbr_lookup *p, const void *dout, void *dtable, void *workspace,
+                            uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "leaf embedding gradient: null argument");
+        leaf_embedding_grad(ordinal, stream, *p, dout, dtable, workspace, workspace_bytes);
+    });
+}
+
+int hbr_softmax_head_workspace(uint64_t n_rows, uint32_t n_classes, uint32_t dim, uint32_t dtype, int gradient,
+                               uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail(kInvalid, "softmax head: null argument");
+        *bytes = softmax_head_workspace(n_rows, n_classes, dim, dtype, gradient != 0);
+    });
+}
+
+int hbr_softmax_head(int ordinal, const hbr_softmax *p, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "softmax head: null argument");
+        softmax_head(ordinal, stream, *p, workspace, workspace_bytes);
+    });
+}
+
+int hbr_clip_gradients_workspace(uint64_t n_tensors, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail(kInvalid, "clip gradients: null argument");
+        *bytes = clip_gradients_workspace(n_tensors);
+    });
+}
+
+int hbr_clip_gradients(int ordinal, const hbr_tensor *tensors, uint64_t n_tensors, double max_norm, float *norm,
+                       void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        clip_gradients(ordinal, stream, tensors, n_tensors, max_norm, norm, workspace, workspace_bytes);
+    });
 }
 
 int hbr_device_alloc(int ordinal, uint64_t bytes, void **out) {

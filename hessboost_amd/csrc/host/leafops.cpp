@@ -1,0 +1,485 @@
+#include "leafops.h"
+
+#include <algorithm>
+#include <string>
+
+#include "../abi.h"
+
+namespace hbr {
+
+namespace {
+
+uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+// A workspace handed out from its start, 256 bytes apart. Without memory it
+// only counts.
+struct Arena {
+    char *base;
+    uint64_t used = 0;
+    explicit Arena(void *p) : base(static_cast<char *>(p)) {}
+    template <typename T>
+    T *take(uint64_t n) {
+        T *p = base ? reinterpret_cast<T *>(base + used) : nullptr;
+        used += up(n * sizeof(T), 256);
+        return p;
+    }
+};
+
+// The caller's stream, with its device current while the call runs and the
+// thread's own device current again behind it.
+class Queue {
+public:
+    Queue(int ordinal, void *stream) : stream_(static_cast<hipStream_t>(stream)) {
+        if (hipGetDevice(&before_) != hipSuccess) before_ = -1;
+        try {
+            device_ = &device(ordinal);
+            hipDevice_t of = ordinal;
+            if (stream_) HBR_HIP(hipStreamGetDevice(stream_, &of));
+            if (of != ordinal) fail(kInvalid, "the stream is not one of device " + std::to_string(ordinal));
+        } catch (...) {
+            restore();
+            throw;
+        }
+    }
+    ~Queue() { restore(); }
+    Queue(const Queue &) = delete;
+    Queue &operator=(const Queue &) = delete;
+    template <typename Args>
+    void launch(const char *kernel, dim3 grid, dim3 block, const Args &args, uint32_t lds_bytes = 0) {
+        device_->launch_on(stream_, kernel, grid, block, args, lds_bytes);
+    }
+
+private:
+    void restore() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    int before_ = -1;
+    Device *device_ = nullptr;
+    hipStream_t stream_;
+};
+
+uint64_t size_of(uint32_t dtype, const char *what) {
+    if (dtype == HBR_F32) return 4;
+    if (dtype == HBR_BF16) return 2;
+    fail(kInvalid, std::string(what) + ": the type is neither HBR_F32 nor HBR_BF16");
+}
+
+void check_workspace(const void *p, uint64_t have, uint64_t need, const char *what) {
+    if (need == 0) return;
+    if (!p || have < need)
+        fail(kInvalid, std::string(what) + ": the workspace holds " + std::to_string(p ? have : 0) + " bytes of " +
+                           std::to_string(need));
+    if (reinterpret_cast<uint64_t>(p) % 16)
+        fail(kInvalid, std::string(what) + ": the workspace is not aligned to 16 bytes");
+}
+
+void check_aligned(const void *p, uint64_t size, const char *what) {
+    if (reinterpret_cast<uint64_t>(p) % size)
+        fail(kInvalid, std::string(what) + ": an array is not aligned to its elements");
+}
+
+// The widest vector (elements, at most 16 bytes) that divides every row
+// length, stride and address.
+uint32_t vector_width(uint64_t size, std::initializer_list<uint64_t> lengths, std::initializer_list<const void *> ptrs) {
+    uint32_t v = (uint32_t)(16 / size);
+    for (; v > 1; v /= 2) {
+        bool ok = true;
+        for (uint64_t n : lengths) ok = ok && n % v == 0;
+        for (const void *p : ptrs) ok = ok && reinterpret_cast<uint64_t>(p) % (v * size) == 0;
+        if (ok) break;
+    }
+    return v;
+}
+
+const char *name_of(uint32_t dtype) { return dtype == HBR_F32 ? "f32" : "bf16"; }
+
+// ---- leaf vectors ------------------------------------------------------------------
+
+void check_lookup(const hbr_lookup &p, const char *what) {
+    size_of(p.dtype, what);
+    if (p.dim == 0) fail(kInvalid, std::string(what) + ": vectors of no elements");
+    if (p.n_rows && p.n_columns && !p.ids) fail(kInvalid, std::string(what) + ": null ids");
+    if (p.n_rows > 1 && p.ids_stride < p.n_columns) fail(kInvalid, std::string(what) + ": the rows of ids overlap");
+    if (p.table_rows > 1 && p.table_stride < p.dim) fail(kInvalid, std::string(what) + ": the table's rows overlap");
+    if (p.n_rows > 1 && p.out_stride < p.dim) fail(kInvalid, std::string(what) + ": the rows' vectors overlap");
+    check_aligned(p.ids, 4, what);
+    check_aligned(p.offset, 4, what);
+    check_aligned(p.scale, 4, what);
+    if (p.table_rows > 0x7fffffffull || p.n_rows > 0x7fffffffull)
+        fail(kRefused, std::string(what) + ": more than 2^31 - 1 rows");
+}
+
+}  // namespace
+
+void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *table, void *out) {
+    const char *what = "leaf embedding";
+    check_lookup(p, what);
+    const uint64_t size = size_of(p.dtype, what);
+    if (p.n_rows == 0) return;
+    if (!out || (!table && p.table_rows)) fail(kInvalid, std::string(what) + ": null argument");
+    check_aligned(table, size, what);
+    check_aligned(out, size, what);
+    Queue queue(ordinal, stream);
+    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {table, out});
+    EmbedArgs a{};
+    a.table = table;
+    a.ids = p.ids;
+    a.offset = p.offset;
+    a.scale = p.scale;
+    a.out = out;
+    a.n_rows = p.n_rows;
+    a.table_rows = p.table_rows;
+    a.table_stride = p.table_stride;
+    a.ids_stride = p.ids_stride;
+    a.out_stride = p.out_stride;
+    a.columns = p.table_rows ? p.n_columns : 0;
+    a.dim = p.dim;
+    a.vecs = p.dim / v;
+    a.rows_per_block = std::max(1u, 256 / a.vecs);
+    const uint64_t blocks = (p.n_rows + a.rows_per_block - 1) / a.rows_per_block;
+    const std::string k = std::string("hbr_leaf_embed_") + name_of(p.dtype) + "_" + std::to_string(v);
+    queue.launch(k.c_str(), dim3((uint32_t)std::min<uint64_t>(blocks, 1u << 20)), dim3(256), a);
+}
+
+namespace {
+
+struct LookupPlan {
+    uint64_t n;  // entries
+    uint32_t tiles, passes, chunk, chunks;
+    uint32_t *key[2], *val[2], *hist, *total, *start;
+    float *part;
+    uint64_t bytes;
+};
+
+LookupPlan lookup_plan(const hbr_lookup &p, void *workspace) {
+    LookupPlan q{};
+    if (p.n_columns && p.n_rows > 0x7fffffffull / p.n_columns)
+        fail(kRefused, "leaf embedding gradient: more than 2^31 - 1 ids");
+    q.n = p.n_rows * p.n_columns;
+    q.tiles = (uint32_t)((q.n + kSortTile - 1) / kSortTile);
+    // keys run from 0 to table_rows
+    uint32_t bits = 1;
+    while (bits < 32 && (p.table_rows >> bits)) bits++;
+    q.passes = (bits + kSortBits - 1) / kSortBits;
+    // about 8,192 waves, 32 to 512 entries each
+    q.chunk = (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(32, up(q.n / 8192, 32)));
+    q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
+    Arena w(workspace);
+    for (int b = 0; b < 2; b++) {
+        q.key[b] = w.take<uint32_t>(q.n);
+        q.val[b] = w.take<uint32_t>(q.n);
+    }
+    q.hist = w.take<uint32_t>((uint64_t)kSortDigits * q.tiles);
+    q.total = w.take<uint32_t>(kSortDigits);
+    q.start = w.take<uint32_t>(p.table_rows + 1);
+    q.part = w.take<float>((uint64_t)q.chunks * 2 * p.dim);
+    q.bytes = w.used;
+    return q;
+}
+
+}  // namespace
+
+uint64_t leaf_embedding_grad_workspace(const hbr_lookup &p) {
+    check_lookup(p, "leaf embedding gradient");
+    return lookup_plan(p, nullptr).bytes;
+}
+
+void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const void *dout, void *dtable,
+                         void *workspace, uint64_t workspace_bytes) {
+    const char *what = "leaf embedding gradient";
+    check_lookup(p, what);
+    const uint64_t size = size_of(p.dtype, what);
+    if (p.table_rows == 0) return;
+    if (!dtable || (!dout && p.n_rows)) fail(kInvalid, std::string(what) + ": null argument");
+    check_aligned(dout, size, what);
+    check_aligned(dtable, size, what);
+    const LookupPlan q = lookup_plan(p, workspace);
+    check_workspace(workspace, workspace_bytes, q.bytes, what);
+    Queue queue(ordinal, stream);
+    int from = 0;
+    for (uint32_t pass = 0; pass < q.passes && q.n; pass++) {
+        LookupSortArgs a{};
+        a.ids = p.ids;
+        a.offset = p.offset;
+        a.ids_stride = p.ids_stride;
+        a.table_rows = p.table_rows;
+        a.columns = p.n_columns;
+        a.n = (uint32_t)q.n;
+        a.tiles = q.tiles;
+        a.shift = pass * kSortBits;
+        a.keys_in = pass ? q.key[from] : nullptr;
+        a.vals_in = pass ? q.val[from] : nullptr;
+        a.keys_out = q.key[from ^ 1];
+        a.vals_out = q.val[from ^ 1];
+        a.hist = q.hist;
+        a.total = q.total;
+        queue.launch("hbr_sort_count", dim3(q.tiles), dim3(256), a);
+        queue.launch("hbr_sort_scan", dim3(kSortDigits), dim3(256), a);
+        queue.launch("hbr_sort_scatter", dim3(q.tiles), dim3(256), a);
+        from ^= 1;
+    }
+    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
+    LookupSumArgs a{};
+    a.keys = q.key[from];
+    a.vals = q.val[from];
+    a.dout = dout;
+    a.scale = p.scale;
+    a.dtable = dtable;
+    a.start = q.start;
+    a.part = q.part;
+    a.table_rows = p.table_rows;
+    a.dout_stride = p.out_stride;
+    a.dtable_stride = p.table_stride;
+    a.n = (uint32_t)q.n;
+    a.columns = p.n_columns;
+    a.dim = p.dim;
+    a.vecs = p.dim / v;
+    a.chunk = q.chunk;
+    a.chunks = q.chunks;
+    auto blocks = [](uint64_t threads) { return dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16)); };
+    const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
+    queue.launch("hbr_lookup_starts", blocks(p.table_rows + 1), dim3(256), a);
+    queue.launch(("hbr_lookup_sum_" + suffix).c_str(), dim3((q.chunks + 3) / 4), dim3(256), a);
+    queue.launch(("hbr_lookup_finish_" + suffix).c_str(), blocks(p.table_rows * a.vecs), dim3(256), a);
+}
+
+// ---- the softmax head ------------------------------------------------------------------
+
+namespace {
+
+// The scores' gradients of one piece of the classes are held at a time, in
+// about this many bytes.
+constexpr uint64_t kPieceBytes = 256ull << 20;
+
+struct HeadPlan {
+    uint64_t class_tiles, row_tiles, piece;
+    float *part_max, *part_sum, *label_margin, *lse, *part_db, *dh;
+    int32_t *part_best;
+    void *g;
+    uint64_t bytes;
+};
+
+HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, bool gradient, void *workspace) {
+    const uint64_t size = size_of(dtype, "softmax head");
+    if (classes == 0 || dim == 0) fail(kInvalid, "softmax head: no classes, or inputs of no elements");
+    if (classes > 0x7fffffffull || n > 0x7fffffffull) fail(kRefused, "softmax head: more than 2^31 - 1 rows or classes");
+    HeadPlan q{};
+    q.class_tiles = (classes + kHeadTile - 1) / kHeadTile;
+    q.row_tiles = (n + kHeadTile - 1) / kHeadTile;
+    if (q.class_tiles > 65535 || dim > 65535 * (uint64_t)kHeadTile)
+        fail(kRefused, "softmax head: more than 4,194,240 classes or elements");
+    Arena w(workspace);
+    q.part_max = w.take<float>(q.class_tiles * n);
+    q.part_sum = w.take<float>(q.class_tiles * n);
+    q.part_best = w.take<int32_t>(q.class_tiles * n);
+    q.label_margin = w.take<float>(n);
+    q.lse = w.take<float>(n);
+    if (gradient) {
+        const uint64_t fits = kPieceBytes / (std::max<uint64_t>(n, 1) * size) / kHeadTile * kHeadTile;
+        q.piece = std::min(up(classes, kHeadTile), std::max<uint64_t>(fits, kHeadTile));
+        q.g = w.take<char>(n * q.piece * size);
+        q.part_db = w.take<float>(q.row_tiles * q.piece);
+        q.dh = w.take<float>(n * dim);
+    }
+    q.bytes = w.used;
+    return q;
+}
+
+}  // namespace
+
+uint64_t softmax_head_workspace(uint64_t n_rows, uint32_t n_classes, uint32_t dim, uint32_t dtype, bool gradient) {
+    return head_plan(n_rows, n_classes, dim, dtype, gradient, nullptr).bytes;
+}
+
+void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspace, uint64_t workspace_bytes) {
+    const char *what = "softmax head";
+    const bool gradient = p.dh || p.dw || p.db;
+    const uint64_t size = size_of(p.dtype, what), n = p.n_rows, classes = p.n_classes, dim = p.dim;
+    const HeadPlan q = head_plan(n, classes, dim, p.dtype, gradient, workspace);
+    if (!p.w || (n && !p.h)) fail(kInvalid, std::string(what) + ": null inputs or weights");
+    if (gradient && !p.labels && n) fail(kInvalid, std::string(what) + ": gradients need labels");
+    if ((n > 1 && p.h_stride < dim) || (classes > 1 && p.w_stride < dim) || (p.dh && n > 1 && p.dh_stride < dim) ||
+        (p.dw && classes > 1 && p.dw_stride < dim))
+        fail(kInvalid, std::string(what) + ": rows overlap");
+    for (const void *x : {p.h, p.w, (const void *)p.dh, (const void *)p.dw}) check_aligned(x, size, what);
+    for (const void *x : {(const void *)p.bias, (const void *)p.labels, (const void *)p.weight, (const void *)p.loss,
+                          (const void *)p.lse, (const void *)p.best, (const void *)p.db})
+        check_aligned(x, 4, what);
+    check_workspace(workspace, workspace_bytes, q.bytes, what);
+    Queue queue(ordinal, stream);
+    const std::string suffix = name_of(p.dtype);
+    float *lse = p.lse ? p.lse : q.lse;
+    auto grid = [](uint64_t m, uint64_t c) {
+        return dim3((uint32_t)((m + kHeadTile - 1) / kHeadTile), (uint32_t)((c + kHeadTile - 1) / kHeadTile));
+    };
+    HeadArgs z{};  // scores
+    z.a = p.h;
+    z.b = p.w;
+    z.a_m = p.h_stride;
+    z.b_n = p.w_stride;
+    z.a_k = z.b_k = 1;
+    z.m = z.rows = n;
+    z.n = classes;
+    z.k = dim;
+    z.bias = p.bias;
+    z.labels = p.labels;
+    z.part_max = q.part_max;
+    z.part_sum = q.part_sum;
+    z.part_best = p.best ? q.part_best : nullptr;
+    z.label_margin = q.label_margin;
+    z.lse = lse;
+    z.weight = p.weight;
+    z.grad_scale = p.grad_scale;
+    if (n) {
+        queue.launch(("hbr_head_scores_" + suffix).c_str(), grid(n, classes), dim3(256), z);
+        HeadFinishArgs f{};
+        f.part_max = q.part_max;
+        f.part_sum = q.part_sum;
+        f.part_best = z.part_best;
+        f.label_margin = q.label_margin;
+        f.labels = p.labels;
+        f.weight = p.weight;
+        f.lse = lse;
+        f.loss = p.loss;
+        f.best = p.best;
+        f.rows = n;
+        f.classes = classes;
+        f.tiles = (uint32_t)q.class_tiles;
+        queue.launch("hbr_head_finish", dim3((uint32_t)((n + 63) / 64)), dim3(1024), f);
+    }
+    if (!gradient) return;
+    auto sum_grid = [](uint64_t cells) { return dim3((uint32_t)std::min<uint64_t>((cells + 255) / 256, 1u << 16)); };
+    for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
+        const uint64_t kc = std::min(q.piece, classes - k0);
+        HeadArgs g = z;
+        g.b = static_cast<const char *>(p.w) + k0 * p.w_stride * size;
+        g.n = kc;
+        g.first = k0;
+        g.g = q.g;
+        g.g_stride = q.piece;
+        g.part_db = q.part_db;
+        if (n) queue.launch(("hbr_head_pairs_" + suffix).c_str(), grid(n, kc), dim3(256), g);
+        if (p.db) {
+            HeadSumArgs b{};
+            b.part = q.part_db;
+            b.dst = p.db + k0;
+            b.rows = 1;
+            b.cols = b.dst_stride = b.part_stride = kc;
+            b.parts = (uint32_t)q.row_tiles;
+            queue.launch("hbr_head_sum_f32", sum_grid(kc), dim3(256), b);
+        }
+        if (p.dw) {
+            HeadArgs w{};
+            w.a = q.g;
+            w.a_m = 1;
+            w.a_k = q.piece;
+            w.b = p.h;
+            w.b_n = 1;
+            w.b_k = p.h_stride;
+            w.skip = p.labels;
+            w.m = kc;
+            w.n = dim;
+            w.k = n;
+            w.c = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
+            w.c_stride = p.dw_stride;
+            queue.launch(("hbr_head_out_" + suffix).c_str(), grid(kc, dim), dim3(256), w);
+        }
+        if (p.dh && n) {
+            HeadArgs h{};
+            h.a = q.g;
+            h.a_m = q.piece;
+            h.a_k = 1;
+            h.b = g.b;
+            h.b_n = 1;
+            h.b_k = p.w_stride;
+            h.m = n;
+            h.n = dim;
+            h.k = kc;
+            h.c = q.dh;
+            h.c_stride = dim;
+            h.accumulate = k0 != 0;
+            queue.launch(("hbr_head_add_" + suffix).c_str(), grid(n, dim), dim3(256), h);
+        }
+    }
+    if (p.dh && n) {
+        HeadSumArgs h{};
+        h.part = q.dh;
+        h.dst = p.dh;
+        h.rows = n;
+        h.cols = dim;
+        h.dst_stride = p.dh_stride;
+        h.parts = 1;
+        queue.launch(("hbr_head_sum_" + suffix).c_str(), sum_grid(n * dim), dim3(256), h);
+    }
+}
+
+// ---- clipping ----------------------------------------------------------------------------
+
+namespace {
+
+// The launches of one pass over the tensors: kClipTensors of them at a time.
+uint64_t clip_launches(uint64_t n) { return (n + kClipTensors - 1) / kClipTensors; }
+
+}  // namespace
+
+uint64_t clip_gradients_workspace(uint64_t n_tensors) {
+    if (n_tensors > (1u << 20)) fail(kRefused, "clip gradients: more than 1,048,576 tensors");
+    return clip_launches(n_tensors) * kClipBlocks * sizeof(double);
+}
+
+void clip_gradients(int ordinal, void *stream, const hbr_tensor *tensors, uint64_t n, double max_norm, float *norm,
+                    void *workspace, uint64_t workspace_bytes) {
+    const char *what = "clip gradients";
+    if (n && !tensors) fail(kInvalid, std::string(what) + ": null tensors");
+    if (!(max_norm >= 0.0)) fail(kInvalid, std::string(what) + ": the largest norm is negative or no number");
+    check_aligned(norm, 4, what);
+    check_workspace(workspace, workspace_bytes, clip_gradients_workspace(n), what);
+    uint64_t blocks = 0;  // of a launch
+    for (uint64_t i = 0; i < n; i++) {
+        const uint64_t size = size_of(tensors[i].dtype, what);
+        if (tensors[i].len && (!tensors[i].data || !tensors[i].out)) fail(kInvalid, std::string(what) + ": null tensor");
+        if (tensors[i].len > (1ull << 42)) fail(kRefused, std::string(what) + ": a tensor of more than 2^42 elements");
+        check_aligned(tensors[i].data, size, what);
+        check_aligned(tensors[i].out, size, what);
+        blocks = (i % kClipTensors ? blocks : 0) + (tensors[i].len + kClipElems - 1) / kClipElems;
+        if (blocks > 0x7fffffffull) fail(kRefused, std::string(what) + ": too many elements");
+    }
+    Queue queue(ordinal, stream);
+    const uint64_t launches = std::max<uint64_t>(1, clip_launches(n));
+    auto fill = [&](uint64_t l, ClipArgs &a) {
+        a = ClipArgs{};
+        uint64_t block = 0;
+        for (uint64_t i = l * kClipTensors; i < std::min(n, (l + 1) * kClipTensors); i++) {
+            if (tensors[i].len == 0) continue;
+            ClipTensor &t = a.t[a.tensors++];
+            t.data = tensors[i].data;
+            t.out = tensors[i].out;
+            t.len = tensors[i].len;
+            t.dtype = tensors[i].dtype;
+            t.block = (uint32_t)block;
+            block += (t.len + kClipElems - 1) / kClipElems;
+        }
+        a.blocks = (uint32_t)block;
+        a.part = static_cast<double *>(workspace);
+        a.norm = norm;
+        a.max_norm = max_norm;
+    };
+    ClipArgs a;
+    uint32_t parts = 0;
+    for (uint64_t l = 0; l < launches; l++) {
+        fill(l, a);
+        a.first_part = parts;
+        const uint32_t groups = std::min(a.blocks, kClipBlocks);
+        if (groups) queue.launch("hbr_clip_norm", dim3(groups), dim3(256), a);
+        parts += groups;
+    }
+    for (uint64_t l = 0; l < launches; l++) {
+        fill(l, a);
+        a.parts = parts;
+        a.first_part = (uint32_t)l;  // the first launch gives the norm
+        const uint32_t groups = std::min(a.blocks, kClipBlocks);
+        if (groups || l == 0) queue.launch("hbr_clip_scale", dim3(std::max(groups, 1u)), dim3(256), a);
+    }
+}
+
+}  // namespace hbr

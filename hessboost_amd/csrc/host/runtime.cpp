@@ -125,6 +125,14 @@ void Device::launch_raw(const char *kernel, dim3 grid, dim3 block, const void *a
     pending_.push_back(ev);
 }
 
+void Device::launch_raw_on(hipStream_t s, const char *kernel, dim3 grid, dim3 block, const void *args,
+                           uint32_t lds_bytes) {
+    if (grid.x == 0 || grid.y == 0 || grid.z == 0) return;
+    void *params[] = {const_cast<void *>(args)};
+    HBR_HIP(hipModuleLaunchKernel(function(kernel), grid.x, grid.y, grid.z, block.x, block.y, block.z, lds_bytes, s,
+                                  params, nullptr));
+}
+
 hipEvent_t Device::take_event() {
     if (!event_pool_.empty()) {
         hipEvent_t e = event_pool_.back();

@@ -51,6 +51,11 @@ public:
     void launch(const char *kernel, dim3 grid, dim3 block, const Args &args, uint32_t lds_bytes = 0) {
         launch_raw(kernel, grid, block, &args, lds_bytes);
     }
+    // The same on a caller's stream (of this device; untimed).
+    template <typename Args>
+    void launch_on(hipStream_t s, const char *kernel, dim3 grid, dim3 block, const Args &args, uint32_t lds_bytes = 0) {
+        launch_raw_on(s, kernel, grid, block, &args, lds_bytes);
+    }
     void sync();
 
     // Kernel timing with HIP events on this device's stream (off by default):
@@ -91,6 +96,7 @@ public:
 
 private:
     void launch_raw(const char *kernel, dim3 grid, dim3 block, const void *args, uint32_t lds_bytes);
+    void launch_raw_on(hipStream_t s, const char *kernel, dim3 grid, dim3 block, const void *args, uint32_t lds_bytes);
     hipFunction_t function(const char *kernel);
     void drain_events();
 

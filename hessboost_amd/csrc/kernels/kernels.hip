@@ -6,6 +6,9 @@
 #include "split.hip"
 #include "grow.hip"
 #include "predict.hip"
+#include "leaf_lookup.hip"
+#include "softmax_head.hip"
+#include "clip.hip"
 
 // The abi.h checksum this code object was built with (checked by the host
 // library at module load).

@@ -49,6 +49,9 @@ pub const HBR_TRANSFORM_SIGMOID: c_int = 1;
 pub const HBR_TRANSFORM_SOFTMAX: c_int = 2;
 pub const HBR_TRANSFORM_CLASS_INDEX: c_int = 3;
 
+pub const HBR_F32: u32 = 0;
+pub const HBR_BF16: u32 = 1;
+
 // Opaque handles.
 #[repr(C)]
 pub struct hbr_cuts {
@@ -247,6 +250,53 @@ pub struct hbr_forest_desc {
     pub n_categories: u64,
 }
 
+#[repr(C)]
+pub struct hbr_lookup {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub n_columns: u32,
+    pub pad: u32,
+    pub table_rows: u64,
+    pub table_stride: u64,
+    pub ids_stride: u64,
+    pub out_stride: u64,
+    pub ids: *const i32,
+    pub offset: *const i32,
+    pub scale: *const f32,
+}
+#[repr(C)]
+pub struct hbr_softmax {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub n_classes: u32,
+    pub grad_scale: f32,
+    pub h_stride: u64,
+    pub w_stride: u64,
+    pub dh_stride: u64,
+    pub dw_stride: u64,
+    pub h: *const c_void,
+    pub w: *const c_void,
+    pub bias: *const f32,
+    pub labels: *const i32,
+    pub weight: *const f32,
+    pub loss: *mut f32,
+    pub lse: *mut f32,
+    pub best: *mut i32,
+    pub dh: *mut c_void,
+    pub dw: *mut c_void,
+    pub db: *mut f32,
+}
+#[repr(C)]
+pub struct hbr_tensor {
+    pub data: *const c_void,
+    pub out: *mut c_void,
+    pub len: u64,
+    pub dtype: u32,
+    pub pad: u32,
+}
+
 extern "C" {
     pub fn hbr_last_error(buf: *mut c_char, len: usize) -> usize;
     pub fn hbr_device_count(count: *mut c_int) -> c_int;
@@ -353,6 +403,19 @@ extern "C" {
     pub fn hbr_forest_set_profiling(f: *mut hbr_forest, on: c_int, kernel_prefix: *const c_char) -> c_int;
     pub fn hbr_forest_kernel_stats(f: *mut hbr_forest, buf: *mut c_char, len: usize) -> c_int;
     pub fn hbr_pred_transform(kind: c_int, values: *mut f32, n_rows: u64, n_outputs: u32) -> c_int;
+    pub fn hbr_leaf_embedding(ordinal: c_int, p: *const hbr_lookup, table: *const c_void, out: *mut c_void,
+                              stream: *mut c_void) -> c_int;
+    pub fn hbr_leaf_embedding_grad_workspace(p: *const hbr_lookup, bytes: *mut u64) -> c_int;
+    pub fn hbr_leaf_embedding_grad(ordinal: c_int, p: *const hbr_lookup, dout: *const c_void, dtable: *mut c_void,
+                                   workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn hbr_softmax_head_workspace(n_rows: u64, n_classes: u32, dim: u32, dtype: u32, gradient: c_int,
+                                      bytes: *mut u64) -> c_int;
+    pub fn hbr_softmax_head(ordinal: c_int, p: *const hbr_softmax, workspace: *mut c_void, workspace_bytes: u64,
+                            stream: *mut c_void) -> c_int;
+    pub fn hbr_clip_gradients_workspace(n_tensors: u64, bytes: *mut u64) -> c_int;
+    pub fn hbr_clip_gradients(ordinal: c_int, tensors: *const hbr_tensor, n_tensors: u64, max_norm: f64,
+                              norm: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
+                              stream: *mut c_void) -> c_int;
     pub fn hbr_device_alloc(ordinal: c_int, bytes: u64, out: *mut *mut c_void) -> c_int;
     pub fn hbr_device_free(ordinal: c_int, p: *mut c_void) -> c_int;
     pub fn hbr_device_upload(ordinal: c_int, dst: *mut c_void, src: *const c_void, bytes: u64) -> c_int;

@@ -636,6 +636,118 @@ int hbr_forest_kernel_stats(hbr_forest *f, char *buf, size_t len);
 #define HBR_TRANSFORM_CLASS_INDEX 3
 int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outputs);
 
+/* ------------------------------------------------------------------------- */
+/* Operators over leaves and many classes.                                    */
+/* ------------------------------------------------------------------------- */
+
+/* No counterpart in the reference: a model on a forest's leaves. A forest
+ * grows one tree per class and round, so hundreds of classes and more are
+ * modelled over its leaf ids (hbr_predict_leaf, hbr_predict_margin_device)
+ * instead: each leaf has a vector (hbr_leaf_embedding), the sum of a row's
+ * vectors is scored against every class (hbr_softmax_head), and the tables
+ * step by clipped gradients (hbr_clip_gradients).
+ *
+ * These calls take device memory of device `ordinal` throughout, and a
+ * stream of that device: a hipStream_t, NULL for the device's default
+ * stream. They queue their work on it and return; nothing is allocated,
+ * copied to the host or waited for, so they can be captured into a graph (a
+ * process's first call on a device loads the kernels and is made outside a
+ * capture). The current device of the calling thread is left as it was.
+ * Results do not depend on how the work was spread: the same call gives the
+ * same bits. What a call needs meanwhile lies in the caller's workspace
+ * (16-byte aligned, of at least the bytes that the operator's _workspace
+ * call names for the same sizes): two calls that may run at the same time
+ * need one each, and so do two graphs that may be replayed at the same time.
+ * Outputs overlap no input, except where said. Arrays have rows of
+ * contiguous elements, `_stride` elements apart. */
+#define HBR_F32 0
+#define HBR_BF16 1
+
+/* A look-up of n_rows x n_columns ids in a table of table_rows vectors of
+ * dim elements. Column t's id i means table row offset[t] + i (a tree's first
+ * node; NULL: 0) and counts scale[t] times (a tree's weight; NULL: 1). An id
+ * below 0, or one that leads out of the table, adds nothing. */
+typedef struct hbr_lookup {
+    uint32_t dtype;           /* of the table and the vectors */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint32_t n_columns;
+    uint32_t pad;
+    uint64_t table_rows;
+    uint64_t table_stride;    /* of the table, or of its gradient */
+    uint64_t ids_stride;
+    uint64_t out_stride;      /* of the rows' vectors, or of their gradient */
+    const int32_t *ids;
+    const int32_t *offset;    /* n_columns, or NULL */
+    const float *scale;       /* n_columns, or NULL */
+} hbr_lookup;
+
+/* out[r] = sum over t of scale[t] * table[offset[t] + ids[r][t]], summed in
+ * f32 in the order of the columns and rounded once. One column is a plain
+ * scaled look-up. */
+int hbr_leaf_embedding(int ordinal, const hbr_lookup *p, const void *table, void *out, void *stream);
+/* dtable[v] = sum over every (r, t) that leads to row v of scale[t] *
+ * dout[r], in f32, rounded once; rows that no id leads to are zeros. At most
+ * 2^31 - 1 ids (HBR_REFUSED beyond). */
+int hbr_leaf_embedding_grad_workspace(const hbr_lookup *p, uint64_t *bytes);
+int hbr_leaf_embedding_grad(int ordinal, const hbr_lookup *p, const void *dout, void *dtable, void *workspace,
+                            uint64_t workspace_bytes, void *stream);
+
+/* The softmax cross entropy of a linear layer over n_classes classes. With
+ * z[r][k] = <h[r], w[k]> + bias[k] (f32):
+ *   lse[r]  = log sum over k of exp z[r][k];
+ *   loss[r] = weight[r] * (lse[r] - z[r][labels[r]]); 0 for a label below 0,
+ *             whose row takes no part (whatever its inputs hold); without
+ *             labels lse[r] less the row's largest z;
+ *   best[r] = the first class of the largest z;
+ *   dh, dw, db = the gradients of grad_scale * (sum over r of loss[r]), in h,
+ *             w and bias.
+ * A label of n_classes or more makes its row's lse and loss, and the
+ * gradients, NaN. A bias of -infinity shuts a class; a row whose classes are
+ * all shut has an lse of -infinity, and a loss and gradients that are NaN
+ * unless its label is below 0. The scores are made in tiles and not kept:
+ * the gradients hold those of one piece of the classes at a time. */
+typedef struct hbr_softmax {
+    uint32_t dtype;           /* of h, w, dh and dw */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint32_t n_classes;
+    float grad_scale;
+    uint64_t h_stride;
+    uint64_t w_stride;
+    uint64_t dh_stride;
+    uint64_t dw_stride;
+    const void *h;
+    const void *w;
+    const float *bias;        /* n_classes, or NULL */
+    const int32_t *labels;    /* n_rows; NULL without gradients */
+    const float *weight;      /* n_rows, or NULL: 1 */
+    float *loss;              /* the outputs: n_rows each, or NULL */
+    float *lse;
+    int32_t *best;
+    void *dh;                 /* NULL where not wanted */
+    void *dw;
+    float *db;
+} hbr_softmax;
+int hbr_softmax_head_workspace(uint64_t n_rows, uint32_t n_classes, uint32_t dim, uint32_t dtype, int gradient,
+                               uint64_t *bytes);
+int hbr_softmax_head(int ordinal, const hbr_softmax *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* A set of tensors scaled to a largest 2-norm: norm = the square root of the
+ * sum of every element's square (f64, rounded to f32), out = data * min(1,
+ * max_norm / (norm + 1e-6)). A norm that is no number makes every element
+ * none. out may be data itself. */
+typedef struct hbr_tensor {
+    const void *data;
+    void *out;
+    uint64_t len;
+    uint32_t dtype;
+    uint32_t pad;
+} hbr_tensor;
+int hbr_clip_gradients_workspace(uint64_t n_tensors, uint64_t *bytes);
+int hbr_clip_gradients(int ordinal, const hbr_tensor *tensors, uint64_t n_tensors, double max_norm, float *norm,
+                       void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* Device memory for callers that keep inputs resident (bytes on device
  * `ordinal`). */
 int hbr_device_alloc(int ordinal, uint64_t bytes, void **out);

@@ -1,0 +1,703 @@
+"""The operators over leaves and many classes against their plain forms in
+64 bits, at the sizes, masks and layouts where they can go wrong."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+import hessboost_amd as hb
+import leaf_reference as R
+from hessboost_amd import _capi as A
+from hessboost_amd.leafops import DeviceArray
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ("float32", "bfloat16")
+_BITS = {"float32": np.uint32, "bfloat16": np.uint16, "int32": np.uint32, "uint8": np.uint8}
+
+
+def dev(values, dtype, pad=0, lead=0):
+    """The values on the device, rows `pad` elements apart beyond their own,
+    `lead` elements into the buffer; the gaps hold NaN bits."""
+    v = np.asarray(values)
+    if dtype == "bfloat16":
+        bits = R.to_bf16(v)
+    elif dtype == "float32":
+        bits = np.ascontiguousarray(v, np.float32).view(np.uint32)
+    else:
+        bits = np.ascontiguousarray(v, np.int32).view(np.uint32)
+    rows, cols = (1, v.shape[0]) if v.ndim == 1 else v.shape
+    stride = cols + pad
+    whole = np.full(lead + rows * stride, 0x7FC0 if dtype == "bfloat16" else 0x7FC00000, _BITS[dtype])
+    for r in range(rows):
+        whole[lead + r * stride: lead + r * stride + cols] = bits.reshape(rows, cols)[r]
+    buf = hb.DeviceBuffer(max(16, whole.nbytes))
+    if whole.nbytes:
+        buf.upload(whole)
+    size = whole.itemsize
+    a = DeviceArray(buf, dtype, v.shape, stride=stride if v.ndim == 2 else None, byte_offset=lead * size)
+    a.lead, a.pad = lead, pad
+    return a
+
+
+def like(shape, dtype, pad=0, lead=0):
+    """An output array: every element, and the gaps, NaN bits."""
+    a = dev(np.full(shape, np.nan) if dtype != "int32" else np.full(shape, 0x7FC00000), dtype, pad, lead)
+    return a
+
+
+def back(a):
+    """The array's values (f64, or int32); the gaps must still hold their bits."""
+    bits = _BITS[a.dtype]
+    whole = a.buffer.download(bits, a.buffer.nbytes // np.dtype(bits).itemsize)
+    rows, cols = (1, a.shape[0]) if len(a.shape) == 1 else a.shape
+    stride = cols + a.pad
+    body = whole[a.lead: a.lead + rows * stride].reshape(rows, stride)
+    gap = 0x7FC0 if a.dtype == "bfloat16" else 0x7FC00000
+    assert np.all(whole[:a.lead] == gap) and np.all(body[:, cols:] == gap), "written outside the array"
+    v = np.ascontiguousarray(body[:, :cols]).reshape(a.shape)
+    if a.dtype == "bfloat16":
+        return R.from_bf16(v).astype(np.float64)
+    if a.dtype == "float32":
+        return v.view(np.float32).astype(np.float64)
+    return v.view(np.int32)
+
+
+def work(nbytes):
+    """A workspace of just the bytes asked for, full of NaN bits."""
+    buf = hb.DeviceBuffer(max(16, nbytes))
+    buf.upload(np.full(max(16, nbytes) // 4 + 1, 0x7FC00001, np.uint32).view(np.uint8)[:max(16, nbytes)])
+    return DeviceArray(buf, "uint8", nbytes)
+
+
+def close(got, want, what=""):
+    value, bound = want
+    both = np.isnan(value) & np.isnan(got)
+    same = (got == value) | both  # infinities
+    with np.errstate(invalid="ignore"):
+        off = np.where(same, 0.0, np.abs(got - value))
+    worst = np.max(np.where(same, 0.0, off / bound)) if off.size else 0.0
+    assert np.all(same | (off <= bound)), f"{what}: {worst} times the bound"
+
+
+# ---- leaf vectors ------------------------------------------------------------------
+
+# rows, columns, table rows a column, dim, dtype, offsets, scale, padded share, stride gaps, lead
+LOOKUPS = [
+    (1, 1, 1, 1, "float32", False, False, 0.0, 0, 0),
+    (1, 1, 5, 8, "bfloat16", False, True, 0.0, 0, 0),
+    (3, 2, 7, 5, "float32", True, True, 0.3, 3, 1),
+    (3, 2, 7, 5, "bfloat16", True, True, 0.3, 2, 1),
+    (33, 9, 15, 16, "float32", True, True, 0.0, 0, 0),
+    (257, 17, 31, 50, "float32", True, False, 0.1, 0, 0),
+    (257, 17, 31, 50, "bfloat16", True, False, 0.1, 0, 0),
+    (1000, 100, 127, 64, "bfloat16", True, True, 0.0, 0, 0),
+    (1000, 23, 127, 32, "float32", True, True, 0.0, 8, 4),
+    (4097, 3, 511, 24, "bfloat16", True, True, 0.5, 8, 8),
+    (5000, 1, 9001, 96, "bfloat16", False, True, 0.02, 0, 0),
+    (300, 1, 70_001, 257, "float32", False, True, 0.02, 0, 0),
+    (130, 2, 40, 1030, "bfloat16", True, False, 0.0, 2, 0),
+    (64, 5, 12, 3, "float32", True, True, 1.0, 0, 0),        # nothing adds
+    (20_000, 4, 3, 8, "float32", True, True, 0.0, 0, 0),     # a few rows hold every id
+    (9000, 1, 2, 40, "bfloat16", False, False, 0.0, 0, 0),
+    (0, 3, 4, 8, "float32", True, True, 0.0, 0, 0),
+    (5, 0, 4, 8, "float32", False, False, 0.0, 0, 0),
+]
+
+
+def lookup_case(case, seed=0):
+    n, columns, rows, dim, dtype, offsets, scaled, padded, gap, lead = case
+    rng = np.random.default_rng([seed, n, columns, dim])
+    table_rows = rows * max(1, columns) if offsets else rows
+    ids = np.minimum((rng.random((n, columns)) ** 2 * rows).astype(np.int32), rows - 1)
+    drop = rng.random((n, columns)) < padded
+    # ids that add nothing: negative ones, and ones past the table's end
+    ids = np.where(drop, np.where(rng.random((n, columns)) < 0.5, -1 - ids, 2_000_000_000 + ids), ids).astype(np.int32)
+    off = (np.arange(columns) * rows).astype(np.int32) if offsets else None
+    s = (rng.random(columns) + 0.5).astype(np.float32) if scaled else None
+    return dict(n=n, columns=columns, table_rows=table_rows, dim=dim, dtype=dtype, ids=ids, offset=off, scale=s,
+                gap=gap, lead=lead, rng=rng)
+
+
+def vec(v, dtype):
+    return None if v is None else dev(v, dtype)
+
+
+@pytest.mark.parametrize("case", LOOKUPS)
+def test_leaf_embedding_sums_the_rows_of_its_ids(case):
+    c = lookup_case(case)
+    table = R.rounded(c["rng"].standard_normal((c["table_rows"], c["dim"])), c["dtype"])
+    out = like((c["n"], c["dim"]), c["dtype"], c["gap"], c["lead"])
+    hb.leaf_embedding(dev(table, c["dtype"], c["gap"], c["lead"]), dev(c["ids"], "int32", c["gap"]), out,
+                      offset=vec(c["offset"], "int32"), scale=vec(c["scale"], "float32"))
+    close(back(out), R.embedding(table, c["ids"], c["offset"], c["scale"], c["dtype"]), "out")
+
+
+@pytest.mark.parametrize("case", LOOKUPS)
+def test_leaf_embedding_grad_sums_the_rows_that_lead_to_each_place(case):
+    c = lookup_case(case, 1)
+    dout = R.rounded(c["rng"].standard_normal((c["n"], c["dim"])), c["dtype"])
+    dtable = like((c["table_rows"], c["dim"]), c["dtype"], c["gap"], c["lead"])
+    args = (dev(dout, c["dtype"], c["gap"], c["lead"]), dev(c["ids"], "int32", c["gap"]), dtable)
+    kw = dict(offset=vec(c["offset"], "int32"), scale=vec(c["scale"], "float32"),
+              workspace=work(hb.leaf_embedding_grad_workspace(c["n"], c["columns"], c["table_rows"], c["dim"],
+                                                              c["dtype"])))
+    hb.leaf_embedding_grad(*args, **kw)
+    got = back(dtable)
+    want = R.embedding_grad(dout, c["ids"], c["offset"], c["scale"], c["table_rows"], c["dtype"])
+    close(got, want, "dtable")
+    assert np.all(got[want[0].any(1) == 0] == 0)
+    hb.leaf_embedding_grad(*args, **kw)  # the same bits on a used workspace
+    assert np.array_equal(back(dtable), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_columns_that_share_table_rows_add_up(dtype):
+    """Overlapping offsets, negative ones among them, and the same id twice in a row."""
+    rng = np.random.default_rng(3)
+    n, columns, rows, dim = 700, 6, 50, 12
+    ids = rng.integers(-3, 40, (n, columns)).astype(np.int32)
+    off = np.array([0, 0, 5, -7, 30, 0], np.int32)
+    s = rng.standard_normal(columns).astype(np.float32)
+    table = R.rounded(rng.standard_normal((rows, dim)), dtype)
+    out, dtable = like((n, dim), dtype), like((rows, dim), dtype)
+    d = dict(offset=dev(off, "int32"), scale=dev(s, "float32"))
+    hb.leaf_embedding(dev(table, dtype), dev(ids, "int32"), out, **d)
+    close(back(out), R.embedding(table, ids, off, s, dtype))
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable,
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, columns, rows, dim, dtype)), **d)
+    close(back(dtable), R.embedding_grad(dout, ids, off, s, rows, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_what_no_id_leads_to_is_not_read(dtype):
+    """NaN and infinities in table rows, or in rows of dout, that no id leads
+    to or from; a NaN that one leads to reaches its sums alone."""
+    rng = np.random.default_rng(4)
+    n, rows, dim = 300, 20, 10
+    ids = (2 * rng.integers(0, rows // 2, (n, 3))).astype(np.int32)
+    ids[5] = -1
+    ids[7] = [4, -2, rows]
+    table = R.rounded(rng.standard_normal((rows, dim)), dtype)
+    table[1::2] = np.nan
+    table[3] = np.inf
+    out = like((n, dim), dtype)
+    hb.leaf_embedding(dev(table, dtype), dev(ids, "int32"), out)
+    clean = np.where(np.isfinite(table), table, 0.0)
+    close(back(out), R.embedding(clean, ids, None, None, dtype))
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    dout[5] = np.nan
+    dout[7] = np.inf
+    dtable = like((rows, dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable,
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, 3, rows, dim, dtype)))
+    got, rest = back(dtable), ids.copy()
+    assert np.all(np.isinf(got[4]))
+    rest[7] = -1
+    want, bound = R.embedding_grad(np.where(np.isfinite(dout), dout, 0.0), rest, None, None, rows, dtype)
+    keep = np.arange(rows) != 4
+    close(got[keep], (want[keep], bound[keep]))
+
+
+def test_an_embedding_gradient_is_the_differences_of_its_sum():
+    """<out, dout> is linear in the table: a step along any direction changes
+    it by <dtable, direction>, up to both sides' rounding bounds."""
+    c = lookup_case((500, 7, 31, 20, "float32", True, True, 0.1, 0, 0), 2)
+    rng = c["rng"]
+    table = R.rounded(rng.standard_normal((c["table_rows"], c["dim"])), "float32")
+    step = R.rounded(rng.standard_normal(table.shape), "float32")
+    dout = R.rounded(rng.standard_normal((c["n"], c["dim"])), "float32")
+    d = dict(offset=dev(c["offset"], "int32"), scale=dev(c["scale"], "float32"))
+    ids, sums, slack = dev(c["ids"], "int32"), [], 0.0
+    for t in (R.rounded(table + step, "float32"), R.rounded(table - step, "float32")):
+        out = like((c["n"], c["dim"]), "float32")
+        hb.leaf_embedding(dev(t, "float32"), ids, out, **d)
+        sums.append(np.sum(back(out) * dout))
+        slack += np.sum(R.embedding(t, c["ids"], c["offset"], c["scale"], "float32")[1] * np.abs(dout))
+    moved = R.rounded(table + step, "float32") - R.rounded(table - step, "float32")
+    dtable = like(table.shape, "float32")
+    hb.leaf_embedding_grad(dev(dout, "float32"), ids, dtable, **d,
+                           workspace=work(hb.leaf_embedding_grad_workspace(c["n"], c["columns"], c["table_rows"],
+                                                                           c["dim"], "float32")))
+    slack += np.sum(R.embedding_grad(dout, c["ids"], c["offset"], c["scale"], c["table_rows"], "float32")[1]
+                    * np.abs(moved))
+    assert abs((sums[0] - sums[1]) - np.sum(back(dtable) * moved)) <= slack
+
+
+def test_leaf_ids_of_a_forest_are_looked_up_where_they_lie():
+    """The ids that a forest writes on the device, with its trees' offsets and
+    weights and the leaf values as vectors of one element: its margins."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((3_000, 6)).astype(np.float32)
+    b = hb.train({"objective": "reg:squarederror", "max_depth": 5}, hb.DMatrix(x, label=x[:, 0] * x[:, 1]), 12)
+    f = b.forest()
+    dx, margins = hb.DeviceBuffer(x.nbytes), hb.DeviceBuffer(4 * len(x))
+    leaves = hb.DeviceBuffer(4 * len(x) * f.n_trees)
+    dx.upload(x)
+    f.predict_margin_device(dx.ptr, len(x), x.shape[1], margins.ptr, leaves.ptr)
+    values = f.arrs["leaf_value"].astype(np.float64)[:, None]
+    out = like((len(x), 1), "float32")
+    ids = DeviceArray(leaves, "int32", (len(x), f.n_trees))
+    offset = f.arrs["tree_offset"][:-1].astype(np.int32)
+    hb.leaf_embedding(dev(values, "float32"), ids, out, offset=dev(offset, "int32"))
+    host_ids = leaves.download(np.int32, len(x) * f.n_trees).reshape(len(x), -1)
+    want, bound = R.embedding(values, host_ids, offset, None, "float32")
+    close(back(out), (want, bound))
+    m = margins.download(np.float32, len(x)).astype(np.float64)
+    base = float(b.base_score[0])
+    assert np.all(np.abs(back(out)[:, 0] + base - m) <= 2 * bound[:, 0] + (f.n_trees + 2) * R.EPS32 * (np.abs(m) + abs(base)) * 2)
+
+
+# ---- the softmax head ---------------------------------------------------------------------
+
+# rows, classes, dim, ignored share, weights, bias, stride gap, lead
+HEADS = [
+    (1, 1, 1, 0.0, False, False, 0, 0),
+    (1, 2, 3, 0.0, False, True, 1, 1),
+    (5, 7, 8, 0.0, True, True, 0, 0),
+    (64, 10, 50, 0.1, True, True, 0, 0),
+    (129, 65, 33, 0.0, False, True, 3, 1),
+    (300, 16, 64, 0.0, True, False, 0, 0),
+    (257, 17, 40, 0.2, True, True, 0, 0),
+    (70, 300, 128, 0.1, True, True, 8, 8),
+    (513, 513, 96, 0.0, False, True, 0, 0),
+    (33, 1000, 257, 0.5, True, True, 0, 0),
+    (1025, 129, 72, 0.0, True, True, 16, 0),
+    (40, 90, 20, 1.0, True, True, 0, 0),      # no row takes part
+    (600, 31, 1, 0.0, False, True, 0, 0),
+    (2000, 3, 12, 0.1, True, True, 0, 0),
+    (0, 5, 8, 0.0, True, True, 0, 0),
+]
+
+
+def head_case(case, dtype, seed=0):
+    n, classes, dim, ignored, weighted, biased, gap, lead = case
+    rng = np.random.default_rng([seed, n, classes, dim])
+    w = R.rounded(rng.standard_normal((classes, dim)) * 2 / np.sqrt(dim), dtype)
+    h = R.rounded(rng.standard_normal((n, dim)), dtype)
+    bias = R.rounded(rng.standard_normal(classes) * 0.5, "float32") if biased else None
+    labels = rng.integers(0, classes, n).astype(np.int32)
+    labels[rng.random(n) < ignored] = -1 - rng.integers(0, 3)
+    weight = R.rounded(rng.random(n) + 0.5, "float32") if weighted else None
+    return dict(n=n, classes=classes, dim=dim, w=w, h=h, bias=bias, labels=labels, weight=weight, gap=gap, lead=lead,
+                dtype=dtype, scale=float(np.float32(1.0 / max(1, n))))
+
+
+def run_head(c, outputs=("loss", "lse", "best", "dh", "dw", "db"), labels=True, workspace=None):
+    n, classes, dim, dtype = c["n"], c["classes"], c["dim"], c["dtype"]
+    shapes = dict(loss=((n,), "float32"), lse=((n,), "float32"), best=((n,), "int32"), dh=((n, dim), dtype),
+                  dw=((classes, dim), dtype), db=((classes,), "float32"))
+    out = {k: like(*shapes[k], *((c["gap"], c["lead"]) if k in ("dh", "dw") else ())) for k in outputs}
+    gradient = any(k in out for k in ("dh", "dw", "db"))
+    if workspace is None:
+        workspace = work(hb.softmax_head_workspace(n, classes, dim, dtype, gradient))
+    hb.softmax_head(dev(c["h"], dtype, c["gap"], c["lead"]), dev(c["w"], dtype, c["gap"], c["lead"]),
+                    bias=vec(c["bias"], "float32"), labels=vec(c["labels"], "int32") if labels else None,
+                    weight=vec(c["weight"], "float32"), grad_scale=c["scale"], workspace=workspace, **out)
+    return {k: back(v) for k, v in out.items()}
+
+
+def check_head(got, want, h_dim=None):
+    for k, v in got.items():
+        if k != "best":
+            close(v, want[k], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", HEADS)
+def test_softmax_head_and_its_gradients(case, dtype):
+    c = head_case(case, dtype)
+    got = run_head(c)
+    if c["n"] == 0:
+        assert not got["dw"].any() and not got["db"].any()
+        return
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    check_head(got, want)
+    z = c["h"] @ c["w"].T + (0 if c["bias"] is None else c["bias"])
+    second = np.sort(z, 1)[:, -2] if c["classes"] > 1 else np.full(c["n"], -np.inf)
+    clear = z.max(1) - second > 2 * (c["dim"] + 4) * R.EPS32 * (np.abs(c["h"]) @ np.abs(c["w"].T) + 2).max(1)
+    assert np.array_equal(got["best"][clear], want["best"][0][clear])
+    again = run_head(c)
+    assert all(np.array_equal(got[k], again[k]) for k in got)
+    for k in got:  # each alone
+        assert np.array_equal(run_head(c, (k,))[k], got[k]), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, classes, dim", [(1, 5, 16), (1, 4099, 64), (7, 1000, 33), (16, 70_000, 24), (50, 257, 512)])
+def test_rows_answered_without_labels(n, classes, dim, dtype):
+    c = head_case((n, classes, dim, 0.0, False, True, 0, 0), dtype, 1)
+    got = run_head(c, ("loss", "lse", "best"), labels=False)
+    want = R.head(c["h"], c["w"], c["bias"], None, None, 1.0, dtype)
+    check_head(got, want)
+    z = c["h"] @ c["w"].T + c["bias"]
+    assert np.all(z[np.arange(n), got["best"]] >= z.max(1) - 2 * (dim + 4) * R.EPS32 * (
+        np.abs(c["h"]) @ np.abs(c["w"].T) + np.abs(c["bias"])).max(1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, classes", [(70, 9), (5, 3000), (200, 700)])
+def test_the_first_of_equal_classes_is_the_best(n, classes, dtype):
+    """Every class alike, and a later pair above the others."""
+    c = head_case((n, classes, 16, 0.0, False, False, 0, 0), dtype, 2)
+    c["w"][:] = c["w"][0]
+    assert np.all(run_head(c, ("best",), labels=False)["best"] == 0)
+    c["bias"] = np.zeros(classes)
+    c["bias"][[classes - 1, classes // 2]] = 3.0
+    assert np.all(run_head(c, ("best",), labels=False)["best"] == classes // 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, classes, dim", [(90, 12, 20), (90, 300, 64)])
+def test_shut_classes_and_rows_that_take_no_part(n, classes, dim, dtype):
+    """Biases of -infinity; NaN, infinities and a NaN weight in rows whose
+    label is below 0: the others' results are those without them."""
+    c = head_case((n, classes, dim, 0.3, True, True, 0, 0), dtype, 3)
+    c["bias"][::3] = -np.inf
+    open_ = np.flatnonzero(np.isfinite(c["bias"]))
+    live = c["labels"] >= 0
+    c["labels"][live] = open_[c["labels"][live] % len(open_)]
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    dead = np.flatnonzero(~live)
+    c["h"][dead[0]] = np.nan
+    c["h"][dead[1]] = np.inf
+    c["h"][dead[2], 0] = -np.inf
+    c["weight"][dead[3]] = np.nan
+    got = run_head(c)
+    assert not got["dh"][dead].any() and not got["loss"][dead].any()
+    assert not got["dw"][::3].any() and not got["db"][::3].any()
+    for k in ("loss", "dh", "lse"):
+        close(got[k][live], (want[k][0][live], want[k][1][live]), k)
+    for k in ("dw", "db"):
+        close(got[k], want[k], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [6, 200])
+def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dtype):
+    c = head_case((40, classes, 24, 0.0, False, True, 0, 0), dtype, 4)
+    c["bias"][0] = -np.inf
+    c["labels"][:] = np.maximum(c["labels"], 1)
+    c["labels"][3] = 0
+    got = run_head(c)
+    assert np.isposinf(got["loss"][3]) and np.isfinite(np.delete(got["loss"], 3)).all()
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], None, c["scale"], dtype)
+    for k in ("dh", "dw", "db"):
+        close(got[k], want[k], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [4, 130])
+def test_rows_with_no_open_class_and_labels_that_are_no_class(classes, dtype):
+    c = head_case((30, classes, 8, 0.0, False, True, 0, 0), dtype, 5)
+    shut = dict(c, bias=np.full(classes, -np.inf))
+    got = run_head(shut, ("loss", "lse"))
+    assert np.all(np.isneginf(got["lse"])) and np.all(np.isnan(got["loss"]))
+    shut["labels"] = np.full(30, -1, np.int32)
+    got = run_head(shut)
+    assert not got["loss"].any() and not got["dh"].any() and not got["dw"].any() and not got["db"].any()
+    c["labels"][4] = classes
+    got = run_head(c)
+    assert np.isnan(got["loss"][4]) and np.isnan(got["lse"][4]) and np.isnan(got["dh"][4]).all()
+    assert np.isfinite(np.delete(got["loss"], 4)).all() and np.isnan(got["dw"]).all()
+
+
+@pytest.mark.parametrize("classes", [5, 150])
+def test_scores_far_from_zero_keep_their_loss(classes):
+    """Scores of thousands: exponentials are taken of differences alone."""
+    c = head_case((50, classes, 16, 0.0, False, True, 0, 0), "float32", 6)
+    c["h"] = R.rounded(c["h"] * 1000, "float32")
+    c["bias"] = R.rounded(c["bias"] - 5e4, "float32")
+    got = run_head(c)
+    check_head(got, R.head(c["h"], c["w"], c["bias"], c["labels"], None, c["scale"], "float32"))
+
+
+@pytest.mark.parametrize("n, classes, dim", [(6, 5, 8), (20, 150, 12)])
+def test_head_gradients_are_the_differences_of_the_loss(n, classes, dim):
+    """A central difference along a direction in h, w and bias at once. With
+    step e the difference is off by e^2/6 times the loss's third derivative
+    (a third moment of the scores' slopes u_k and, through the product of
+    the two moving factors, of their bends) and by the loss's bound over e."""
+    c = head_case((n, classes, dim, 0.0, True, True, 0, 0), "float32", 7)
+    rng = np.random.default_rng(8)
+    e = 2.0 ** -7
+    g = run_head(c, ("dh", "dw", "db"))
+    total, slack, moved = [], 0.0, []
+    sides = []
+    dh, dw, db = (rng.standard_normal(c[k].shape) for k in ("h", "w", "bias"))
+    for sign in (1, -1):
+        s = dict(c, h=R.rounded(c["h"] + sign * e * dh, "float32"), w=R.rounded(c["w"] + sign * e * dw, "float32"),
+                 bias=R.rounded(c["bias"] + sign * e * db, "float32"))
+        loss = run_head(s, ("loss",))["loss"]
+        want = R.head(s["h"], s["w"], s["bias"], s["labels"], s["weight"], 1.0, "float32")["loss"]
+        total.append(loss.sum())
+        slack += want[1].sum()
+        sides.append(s)
+    moved = {k: sides[0][k] - sides[1][k] for k in ("h", "w", "bias")}
+    slope = np.sum(g["dh"] * moved["h"]) + np.sum(g["dw"] * moved["w"]) + np.sum(g["db"] * moved["bias"])
+    # z(t) = z + t u + t^2 v: the third derivative of lse is the third central
+    # moment of u plus three times the covariance of u and 2 v
+    u = dh @ c["w"].T + c["h"] @ dw.T + db
+    v = dh @ dw.T
+    span_u = np.ptp(np.abs(u) + 2 * e * np.abs(v), axis=1) + 2 * (np.abs(u) + 2 * e * np.abs(v)).max(1)
+    span_v = 2 * np.abs(2 * v).max(1)
+    third = span_u ** 3 + 3 * span_u * span_v
+    slack += np.sum(c["weight"] * third) * e ** 3 / 3
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], c["scale"], "float32")
+    slack += sum(np.sum(want[k][1] * np.abs(moved[m])) for k, m in (("dh", "h"), ("dw", "w"), ("db", "bias"))) / c["scale"]
+    slack += 1e-12 * abs(total[0]) + 1e-5 * e  # the sides' own rounding of the step
+    assert abs((total[0] - total[1]) - slope / c["scale"]) <= slack
+
+
+# ---- clipping ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [[1], [0], [], [7, 0, 8192, 8193], [5] * 97, [100_003, 3, 16_384 * 3 + 5],
+                                   [1] * 300 + [5_000_001]])
+def test_clipping_scales_a_set_to_its_largest_norm(sizes, dtype):
+    rng = np.random.default_rng(len(sizes))
+    grads = [R.rounded(rng.standard_normal(s), dtype) for s in sizes]
+    true = np.sqrt(sum(float(np.sum(g * g)) for g in grads))
+    for most in (0.0, 0.25 * true, 4.0 * true + 1.0, np.inf):
+        arrays = [dev(g, dtype, lead=i % 3) for i, g in enumerate(grads)]
+        outs = [like(g.shape, dtype, lead=(i // 2) % 3) for i, g in enumerate(grads)]
+        norm = like((1,), "float32")
+        kw = dict(norm=norm, workspace=work(hb.clip_gradients_workspace(len(grads))))
+        hb.clip_gradients(arrays, most, out=outs, **kw)
+        # f64 sums, one rounding of the norm
+        assert abs(back(norm)[0] - true) <= true * (2 * R.EPS32)
+        by = min(1.0, most / (true + 1e-6))
+        for g, o, a in zip(grads, outs, arrays):
+            want = g * by
+            close(back(o), (want, (4 * R.EPS32 + R.HALF[dtype]) * np.abs(want) + 1e-38))
+            assert np.array_equal(back(a), g)
+        hb.clip_gradients(arrays, most, **kw)  # in place
+        for o, a in zip(outs, arrays):
+            assert np.array_equal(back(o), back(a))
+
+
+def test_clipping_of_mixed_types_and_huge_values():
+    a, b = np.array([1e30, -3e38], np.float32).astype(np.float64), R.rounded(np.array([2e38, 1.0]), "bfloat16")
+    x, y, norm = dev(a, "float32"), dev(b, "bfloat16"), like((1,), "float32")
+    w = work(hb.clip_gradients_workspace(2))
+    hb.clip_gradients([x, y], 1.0, norm=norm, workspace=w)
+    # the norm is past f32's range, the factor is not
+    true = np.sqrt(np.sum(a * a) + np.sum(b * b))
+    assert np.isposinf(back(norm)[0])
+    # each factor is a denormal f32 here: half its smallest step
+    close(back(x), (a / true, np.abs(a) * (2.0 ** -150 + 4 * R.EPS32 / true)))
+    close(back(y), (b / true, np.abs(b) * (2.0 ** -150 + 4 * R.EPS32 / true) + R.HALF["bfloat16"] * np.abs(b / true) + 1e-40))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_norm_that_is_none_shows_in_every_tensor(bad):
+    x, y, norm = dev(np.array([1.0, bad]), "float32"), dev(np.ones(5), "float32"), like((1,), "float32")
+    hb.clip_gradients([x, y], 1.0, norm=norm, workspace=work(hb.clip_gradients_workspace(2)))
+    if np.isnan(bad):
+        assert np.isnan(back(norm)[0]) and np.isnan(back(x)).all() and np.isnan(back(y)).all()
+    else:  # 1 / infinity: zeros, and infinity times zero
+        assert np.isposinf(back(norm)[0]) and not back(y).any() and back(x)[0] == 0 and np.isnan(back(x)[1])
+
+
+# ---- together, on streams and in graphs ---------------------------------------------------------
+
+class Step:
+    """One training step of a model on leaves: look-up, head, gradients, clip."""
+
+    def __init__(self, dtype, seed, n=700, columns=12, rows=31, dim=40, classes=130):
+        rng = np.random.default_rng(seed)
+        self.dtype, self.n, self.dim, self.classes, self.rows = dtype, n, dim, classes, rows * columns
+        self.ids_v = rng.integers(0, rows, (n, columns)).astype(np.int32)
+        self.off_v = (np.arange(columns) * rows).astype(np.int32)
+        self.s_v = R.rounded(rng.random(columns) + 0.5, "float32")
+        self.table_v = R.rounded(rng.standard_normal((self.rows, dim)) * 0.3, dtype)
+        self.w_v = R.rounded(rng.standard_normal((classes, dim)) * 0.2, dtype)
+        self.b_v = R.rounded(rng.standard_normal(classes) * 0.1, "float32")
+        self.y_v = rng.integers(-1, classes, n).astype(np.int32)
+        self.ids, self.off, self.s = dev(self.ids_v, "int32"), dev(self.off_v, "int32"), dev(self.s_v, "float32")
+        self.table, self.w, self.b = dev(self.table_v, dtype), dev(self.w_v, dtype), dev(self.b_v, "float32")
+        self.y = dev(self.y_v, "int32")
+        self.h, self.dh = like((n, dim), dtype), like((n, dim), dtype)
+        self.loss, self.norm = like((n,), "float32"), like((1,), "float32")
+        self.grads = [like((self.rows, dim), dtype), like((classes, dim), dtype), like((classes,), "float32")]
+        self.ws = [work(b) for b in (hb.softmax_head_workspace(n, classes, dim, dtype),
+                                     hb.leaf_embedding_grad_workspace(n, columns, self.rows, dim, dtype),
+                                     hb.clip_gradients_workspace(3))]
+
+    def run(self, stream=None):
+        kw = dict(offset=self.off, scale=self.s, stream=stream)
+        hb.leaf_embedding(self.table, self.ids, self.h, **kw)
+        hb.softmax_head(self.h, self.w, bias=self.b, labels=self.y, loss=self.loss, dh=self.dh, dw=self.grads[1],
+                        db=self.grads[2], grad_scale=1.0 / self.n, workspace=self.ws[0], stream=stream)
+        hb.leaf_embedding_grad(self.dh, self.ids, self.grads[0], workspace=self.ws[1], **kw)
+        hb.clip_gradients(self.grads, 0.01, norm=self.norm, workspace=self.ws[2], stream=stream)
+
+    def outputs(self):
+        return [back(a) for a in (self.h, self.loss, self.norm, *self.grads)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_training_step_runs_through_all_of_them(dtype):
+    s = Step(dtype, 11)
+    s.run()
+    h, loss, norm, *grads = s.outputs()
+    close(h, R.embedding(s.table_v, s.ids_v, s.off_v, s.s_v, dtype))
+    want = R.head(h, s.w_v, s.b_v, s.y_v, None, float(np.float32(1 / s.n)), dtype)
+    close(loss, want["loss"])
+    dh = back(s.dh)
+    close(dh, want["dh"])
+    full = [R.embedding_grad(dh, s.ids_v, s.off_v, s.s_v, s.rows, dtype), want["dw"], want["db"]]
+    true = np.sqrt(sum(np.sum(v * v) for v, _ in full))
+    slack = np.sqrt(sum(np.sum(e * e) for _, e in full))
+    assert abs(norm[0] - true) <= slack + 2 * R.EPS32 * true and true > 0.01
+    by = 0.01 / (true + 1e-6)
+    for g, (v, e), t in zip(grads, full, (dtype, dtype, "float32")):
+        close(g, (v * by, (e + np.abs(v) * (slack / true + 6 * R.EPS32)) * by * 1.01 + R.HALF[t] * 1.01 * (np.abs(v) + e) * by + 1e-38))
+
+
+def hip():
+    L = C.CDLL("libamdhip64.so.7")
+    for name in ("hipStreamCreateWithFlags", "hipStreamBeginCapture", "hipStreamEndCapture", "hipGraphInstantiate",
+                 "hipGraphLaunch", "hipStreamSynchronize", "hipDeviceSynchronize", "hipGetDevice", "hipStreamDestroy",
+                 "hipGraphExecDestroy", "hipGraphDestroy"):
+        getattr(L, name).restype = C.c_int
+    return L
+
+
+def ok(status):
+    assert status == 0, f"HIP error {status}"
+
+
+def test_steps_on_several_streams_give_the_same_bits():
+    L = hip()
+    steps = [Step("bfloat16", 21), Step("bfloat16", 22), Step("float32", 23)]
+    want = []
+    for s in steps:
+        s.run()
+        want.append(s.outputs())
+    streams = []
+    for _ in steps:
+        st = C.c_void_p()
+        ok(L.hipStreamCreateWithFlags(C.byref(st), 1))
+        streams.append(st)
+    again = [Step("bfloat16", 21), Step("bfloat16", 22), Step("float32", 23)]
+    for _ in range(3):
+        for s, st in zip(again, streams):
+            s.run(st.value)
+    ok(L.hipDeviceSynchronize())
+    for s, w in zip(again, want):
+        for a, b in zip(s.outputs(), w):
+            assert np.array_equal(a, b)
+    for st in streams:
+        ok(L.hipStreamDestroy(st))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_captured_step_replays_with_the_eager_bits(dtype):
+    """Captured once; replayed on other inputs with eager work between."""
+    L = hip()
+    st = C.c_void_p()
+    ok(L.hipStreamCreateWithFlags(C.byref(st), 1))
+    s = Step(dtype, 31)
+    other = Step(dtype, 32)
+    other.run()
+    ok(L.hipStreamBeginCapture(st, 2))
+    s.run(st.value)
+    graph, run = C.c_void_p(), C.c_void_p()
+    ok(L.hipStreamEndCapture(st, C.byref(graph)))
+    ok(L.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)))
+    for seed in (31, 41, 42, 31):
+        t = Step(dtype, seed)
+        for mine, its in ((s.ids, t.ids), (s.table, t.table), (s.w, t.w), (s.b, t.b), (s.y, t.y), (s.s, t.s)):
+            mine.buffer.copy_from(its.buffer)
+        ok(L.hipDeviceSynchronize())
+        ok(L.hipGraphLaunch(run, st))
+        ok(L.hipStreamSynchronize(st))
+        got = s.outputs()
+        t.run()
+        for a, b in zip(got, t.outputs()):
+            assert np.array_equal(a, b)
+        other.run()
+    ok(L.hipGraphExecDestroy(run))
+    ok(L.hipGraphDestroy(graph))
+    ok(L.hipStreamDestroy(st))
+
+
+def test_a_stream_of_no_such_device_is_invalid():
+    s = Step("float32", 1, n=5)
+    p = A.Lookup(A.F32, 4, 1, 1, 0, 1, 4, 1, 4, s.ids.data_ptr(), None, None)
+    n = C.c_int()
+    A.check(A.lib().hbr_device_count(C.byref(n)))
+    assert A.lib().hbr_leaf_embedding(n.value, C.byref(p), s.table.data_ptr(), s.h.data_ptr(), None) == A.INVALID
+
+
+TORCH = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import numpy as np
+import torch
+import hessboost_amd as hb
+import leaf_reference as R
+
+torch.manual_seed(0)
+n, t, rows, dim, classes = 500, 6, 15, 48, 300
+for dtype, name in ((torch.float32, "float32"), (torch.bfloat16, "bfloat16")):
+    table = torch.randn(rows * t, dim, device="cuda").to(dtype)
+    ids = torch.randint(0, rows, (n, t), device="cuda", dtype=torch.int32)
+    off = (torch.arange(t, device="cuda") * rows).int()
+    w = torch.randn(classes, dim, device="cuda").mul_(0.2).to(dtype)
+    y = torch.randint(-1, classes, (n,), device="cuda", dtype=torch.int32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # the tensors' stream by default: torch's current one
+        wide = torch.full((n, 2 * dim), float("nan"), device="cuda", dtype=dtype)
+        h = wide[:, :dim]
+        hb.leaf_embedding(table, ids, h, offset=off)
+        loss = torch.empty(n, device="cuda")
+        dh, dw = torch.empty(n, dim, device="cuda", dtype=dtype), torch.empty_like(w)
+        ws = torch.empty(hb.softmax_head_workspace(n, classes, dim, dtype), dtype=torch.uint8, device="cuda")
+        hb.softmax_head(h, w, labels=y, loss=loss, dh=dh, dw=dw, grad_scale=0.5, workspace=ws)
+        dt = torch.empty_like(table)
+        ws = torch.empty(hb.leaf_embedding_grad_workspace(n, t, rows * t, dim, dtype), dtype=torch.uint8, device="cuda")
+        hb.leaf_embedding_grad(dh, ids, dt, offset=off, workspace=ws)
+        norm = torch.empty(1, device="cuda")
+        ws = torch.empty(hb.clip_gradients_workspace(2), dtype=torch.uint8, device="cuda")
+        clipped = [torch.empty_like(dt), torch.empty_like(dw)]
+        hb.clip_gradients([dt, dw], 1.0, norm=norm, out=clipped, workspace=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    v = lambda x: x.detach().cpu().double().numpy()
+    assert torch.isnan(wide[:, dim:]).all()
+
+    def close(got, want):
+        assert np.all(np.abs(v(got) - want[0]) <= want[1])
+    close(h, R.embedding(v(table), ids.cpu().numpy(), off.cpu().numpy(), None, name))
+    want = R.head(v(h), v(w), None, y.cpu().numpy(), None, 0.5, name)
+    close(loss, want["loss"]); close(dh, want["dh"]); close(dw, want["dw"])
+    close(dt, R.embedding_grad(v(dh), ids.cpu().numpy(), off.cpu().numpy(), None, rows * t, name))
+    true = np.sqrt(np.sum(v(dt) ** 2) + np.sum(v(dw) ** 2))
+    assert abs(v(norm)[0] - true) <= 2 * R.EPS32 * true and true > 1
+    for a, b in zip(clipped, (dt, dw)):
+        close(a, (v(b) / (true + 1e-6), (R.HALF[name] + 4 * R.EPS32) * np.abs(v(b)) / true))
+for bad in (lambda: hb.leaf_embedding(table.cpu(), ids, h, offset=off),
+            lambda: hb.leaf_embedding(table.half(), ids, h, offset=off),
+            lambda: hb.leaf_embedding(table, ids.long(), h, offset=off),
+            lambda: hb.leaf_embedding(table.t(), ids, h, offset=off)):
+    try:
+        bad()
+    except ValueError:
+        continue
+    raise AssertionError("not refused")
+print("torch ok", flush=True)
+"""
+
+
+def test_torch_tensors_are_taken_on_their_stream():
+    """In a process of its own: torch brings its own HIP runtime."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = TORCH.format(root=os.path.dirname(here), tests=here)
+    r = subprocess.run([sys.executable, "-u", "-c", code], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "torch ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]

@@ -1,0 +1,166 @@
+"""The operators over leaves and many classes refuse what they cannot run,
+before they touch a device."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import hessboost_amd as hb
+from hessboost_amd import _capi as A
+from hessboost_amd.leafops import DeviceArray
+
+
+class Memory:
+    """Stands for a DeviceBuffer: an address that nothing reads."""
+
+    def __init__(self, nbytes=1 << 20, ptr=1 << 20, ordinal=0):
+        self.ptr, self.nbytes, self.ordinal = ptr, nbytes, ordinal
+
+
+def arr(dtype, *shape, **kw):
+    mem = {k: kw.pop(k) for k in ("ptr", "ordinal") if k in kw}
+    return DeviceArray(Memory(**mem), dtype, shape, **kw)
+
+
+def lookup(**kw):
+    p = dict(dtype=A.F32, dim=4, n_rows=3, n_columns=2, pad=0, table_rows=5, table_stride=4, ids_stride=2, out_stride=4,
+             ids=1 << 20, offset=None, scale=None)
+    p.update(kw)
+    return A.Lookup(**p)
+
+
+@pytest.mark.parametrize("bad, said", [
+    (dict(dtype=7), "type"), (dict(dim=0), "no elements"), (dict(ids=None), "null ids"),
+    (dict(ids_stride=1), "overlap"), (dict(table_stride=3), "overlap"), (dict(out_stride=3), "overlap"),
+    (dict(ids=(1 << 20) + 2), "aligned"), (dict(scale=(1 << 20) + 1), "aligned")])
+def test_lookups_with_malformed_records_are_invalid(bad, said):
+    p, n = lookup(**bad), C.c_uint64()
+    ok = 1 << 20
+    assert A.lib().hbr_leaf_embedding(0, C.byref(p), ok, ok, None) == A.INVALID and said in A.last_error()
+    assert A.lib().hbr_leaf_embedding_grad(0, C.byref(p), ok, ok, ok, ok, None) == A.INVALID and said in A.last_error()
+    assert A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.INVALID
+
+
+def test_lookups_of_null_and_misaligned_arrays_are_invalid():
+    p, ok = lookup(), 1 << 20
+    L = A.lib()
+    assert L.hbr_leaf_embedding(0, None, ok, ok, None) == A.INVALID
+    for t, o in ((None, ok), (ok, None), (ok + 1, ok), (ok, ok + 2)):
+        assert L.hbr_leaf_embedding(0, C.byref(p), t, o, None) == A.INVALID
+        assert L.hbr_leaf_embedding_grad(0, C.byref(p), t, o, ok, 1 << 30, None) == A.INVALID
+
+
+def test_lookups_past_the_index_range_are_refused():
+    n = C.c_uint64()
+    for big in (dict(table_rows=1 << 31), dict(n_rows=1 << 31), dict(n_rows=1 << 24, n_columns=1 << 7, ids_stride=1 << 7)):
+        p = lookup(**big)
+        assert A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.REFUSED
+    p = lookup(n_rows=(1 << 24) - 1, n_columns=1 << 7, ids_stride=1 << 7)
+    assert A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.OK and n.value > 1 << 31
+
+
+def softmax(**kw):
+    ok = 1 << 20
+    p = dict(dtype=A.BF16, dim=8, n_rows=3, n_classes=5, grad_scale=1.0, h_stride=8, w_stride=8, dh_stride=8,
+             dw_stride=8, h=ok, w=ok, bias=None, labels=ok, weight=None, loss=ok, lse=None, best=None, dh=ok, dw=ok,
+             db=ok)
+    p.update(kw)
+    return A.Softmax(**p)
+
+
+@pytest.mark.parametrize("bad, said", [
+    (dict(dtype=2), "type"), (dict(dim=0), "no classes"), (dict(n_classes=0), "no classes"), (dict(h=None), "null"),
+    (dict(w=None), "null"), (dict(labels=None), "labels"), (dict(h_stride=7), "overlap"), (dict(w_stride=7), "overlap"),
+    (dict(dh_stride=7), "overlap"), (dict(dw_stride=7), "overlap"), (dict(h=(1 << 20) + 1), "aligned"),
+    (dict(dw=(1 << 20) + 1), "aligned"), (dict(bias=(1 << 20) + 2), "aligned"), (dict(best=(1 << 20) + 1), "aligned")])
+def test_heads_with_malformed_records_are_invalid(bad, said):
+    p = softmax(**bad)
+    assert A.lib().hbr_softmax_head(0, C.byref(p), 1 << 20, 1 << 40, None) == A.INVALID and said in A.last_error()
+
+
+def test_a_workspace_that_is_missing_short_or_misaligned_is_invalid():
+    L, ok = A.lib(), 1 << 20
+    need = hb.softmax_head_workspace(3, 5, 8, "bfloat16")
+    p, q = softmax(), lookup()
+    for w, size in ((None, need), (ok, need - 1), (ok + 8, need)):
+        assert L.hbr_softmax_head(0, C.byref(p), w, size, None) == A.INVALID and "workspace" in A.last_error()
+    need = hb.leaf_embedding_grad_workspace(3, 2, 5, 4, "float32")
+    for w, size in ((None, need), (ok, need - 1), (ok + 4, need)):
+        assert L.hbr_leaf_embedding_grad(0, C.byref(q), ok, ok, w, size, None) == A.INVALID
+    need = hb.clip_gradients_workspace(1)
+    t = A.Tensor(ok, ok, 4, A.F32, 0)
+    for w, size in ((None, need), (ok, need - 1), (ok + 4, need)):
+        assert L.hbr_clip_gradients(0, C.byref(t), 1, 1.0, None, w, size, None) == A.INVALID
+
+
+def test_clipping_refuses_malformed_sets():
+    L, ok, big = A.lib(), 1 << 20, 1 << 40
+    t = A.Tensor(ok, ok, 4, A.F32, 0)
+    for norm in (-1.0, float("nan")):
+        assert L.hbr_clip_gradients(0, C.byref(t), 1, norm, None, ok, big, None) == A.INVALID
+    assert L.hbr_clip_gradients(0, None, 1, 1.0, None, ok, big, None) == A.INVALID
+    for bad in (A.Tensor(None, ok, 4, A.F32, 0), A.Tensor(ok, None, 4, A.F32, 0), A.Tensor(ok, ok, 4, 5, 0),
+                A.Tensor(ok + 2, ok, 4, A.F32, 0), A.Tensor(ok, ok + 1, 4, A.BF16, 0)):
+        assert L.hbr_clip_gradients(0, C.byref(bad), 1, 1.0, None, ok, big, None) == A.INVALID
+    huge = A.Tensor(ok, ok, (1 << 42) + 1, A.BF16, 0)
+    assert L.hbr_clip_gradients(0, C.byref(huge), 1, 1.0, None, ok, big, None) == A.REFUSED
+    many = (A.Tensor * 9)(*[A.Tensor(ok, ok, 1 << 42, A.BF16, 0)] * 9)
+    assert L.hbr_clip_gradients(0, many, 9, 1.0, None, ok, big, None) == A.REFUSED
+    n = C.c_uint64()
+    assert L.hbr_clip_gradients_workspace((1 << 20) + 1, C.byref(n)) == A.REFUSED
+
+
+def test_python_arrays_are_checked():
+    f, i = "float32", "int32"
+    table, ids, out = arr(f, 10, 4), arr(i, 6, 3), arr(f, 6, 4)
+    bad = [
+        dict(table=arr(i, 10, 4)), dict(table=arr(f, 40)), dict(out=arr(f, 6, 5)), dict(out=arr("bfloat16", 6, 4)),
+        dict(out=arr(f, 5, 4)), dict(ids=arr(f, 6, 3)), dict(ids=arr(i, 6)), dict(offset=arr(i, 4)),
+        dict(scale=arr(i, 3)), dict(out=arr(f, 6, 4, ordinal=1)), dict(table=arr(f, 10, 4, stride=3)),
+    ]
+    for kw in bad:
+        a = dict(table=table, ids=ids, out=out)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            hb.leaf_embedding(a.pop("table"), a.pop("ids"), a.pop("out"), **a)
+    h, w = arr(f, 6, 4), arr(f, 7, 4)
+    for kw in (dict(bias=arr(f, 6)), dict(labels=arr(f, 6)), dict(labels=arr(i, 7)), dict(weight=arr(f, 7)),
+               dict(dh=arr(f, 7, 4)), dict(dw=arr(f, 6, 4)), dict(db=arr(f, 6)), dict(best=arr(f, 6)),
+               dict(loss=arr("bfloat16", 6))):
+        with pytest.raises(ValueError):
+            hb.softmax_head(h, w, **kw)
+    with pytest.raises(ValueError):
+        hb.softmax_head(h, arr(f, 7, 5))
+    with pytest.raises(ValueError):
+        hb.softmax_head(h, arr("bfloat16", 7, 4))
+    with pytest.raises(hb.HbrError, match="labels"):
+        hb.softmax_head(h, w, db=arr(f, 7))
+    with pytest.raises(ValueError):
+        hb.clip_gradients([h], 1.0, out=[arr(f, 23)])
+    with pytest.raises(ValueError):
+        hb.clip_gradients([h], 1.0, out=[])
+    with pytest.raises(ValueError):
+        hb.clip_gradients([arr(f, 6, 4, stride=5)], 1.0)
+    with pytest.raises(ValueError):
+        hb.clip_gradients([arr(i, 6)], 1.0)
+    with pytest.raises(ValueError):
+        hb.softmax_head_workspace(3, 5, 8, "float16")
+
+
+def test_a_device_array_fits_its_buffer():
+    m = Memory(nbytes=100)
+    DeviceArray(m, "float32", (5, 5))
+    DeviceArray(m, "bfloat16", (5, 4), stride=11)
+    DeviceArray(m, "uint8", 100)
+    for bad in (dict(dtype="float32", shape=(5, 5), byte_offset=4), dict(dtype="float32", shape=26),
+                dict(dtype="bfloat16", shape=(5, 5), stride=12), dict(dtype="float32", shape=4, byte_offset=-4),
+                dict(dtype="float32", shape=(2, 2, 2)), dict(dtype="float64", shape=2)):
+        with pytest.raises(ValueError):
+            DeviceArray(m, **bad)
+
+
+def test_the_reference_rounds_to_bf16_as_numpy_can_check():
+    from leaf_reference import from_bf16, to_bf16
+    x = np.array([1.0, 1.00390625, 1.01171875, -3.4e38, 1e-40, np.inf], np.float32)
+    assert to_bf16(x).tolist() == [0x3F80, 0x3F80, 0x3F82, 0xFF80, 0x0001, 0x7F80]
+    assert np.isnan(from_bf16(to_bf16(np.array([np.nan], np.float32))))[0]
