@@ -1119,37 +1119,58 @@ struct LookupSumArgs {
     uint32_t chunks;
 };
 
-// Rows x classes of one tile of the head's products.
-constexpr uint32_t kHeadTile = 64;
-
-// One product of the softmax head, C[m][n] = sum_k A(m, k) B(n, k), each
-// operand with its own element strides, and what its epilogue needs.
+// The head's products C[m][n] = sum_k A(m, k) B(n, k) of bf16 operands, in
+// tiles of kHeadM x kHeadN, kHeadK products a step. An operand lies [m][k]
+// (k contiguous) or, transposed, [k][m]; f32 operands lie in three bf16 parts
+// whose sum they are, and a product of two is summed over the six pairs of
+// parts that reach f32's precision, one segment of steps each.
+constexpr uint32_t kHeadM = 256;
+constexpr uint32_t kHeadN = 128;
+constexpr uint32_t kHeadK = 32;
 struct HeadArgs {
-    const void *a;
-    const void *b;
-    uint64_t a_m, a_k, b_n, b_k;  // strides, elements
-    uint64_t m, n, k;
-    const int32_t *skip;          // per k: rows whose label is below 0 are not read (or null)
-    // scores: m rows, n classes from class `first` on
-    uint64_t first;
-    const float *bias;
+    const void *a, *b;
+    uint64_t a_stride, b_stride;  // elements
+    uint64_t a_part, b_part;      // elements from one part to the next
+    uint32_t m, n, k;
+    uint32_t m_tiles, n_tiles;
+    uint32_t splits;              // shares of the steps, each a workgroup's
+    uint32_t segments;            // 1, or 6
+    uint32_t rows;
+    const uint32_t *keep;         // bit r: row r of the reduction is read (or null: all)
+    // scores (m: classes, n: rows) and pairs (m: rows, n: classes)
+    const float *bias;            // of the first class
     const int32_t *labels;
-    float *part_max;              // [class tile][rows]
+    float *part_max;              // [class tile][rows], in units of log2
     float *part_sum;
     int32_t *part_best;           // or null
     float *label_margin;          // [rows]
-    uint64_t rows;
-    // pairs: g[m][n] from the scores
-    const float *lse;
+    const float *lse2;
     const float *weight;
+    uint64_t first;               // the first class
     float grad_scale;
-    uint32_t accumulate;          // add to c instead of overwriting it
-    void *g;
-    uint64_t g_stride;
-    float *part_db;               // [row tile][n]
-    // plain
+    uint32_t pad;
+    void *g;                      // [part][rows][g_stride]
+    uint64_t g_stride, g_part;
+    float *part_db;               // [row tile][g_stride]
+    // sums: c in f32, [split][m][c_stride], or the rounded result
     void *c;
-    uint64_t c_stride;
+    uint64_t c_stride, c_split;
+    uint32_t accumulate;          // add to c
+    uint32_t pad2;
+};
+
+// src as bf16 parts with rows of dst_stride elements (zeros past cols).
+struct HeadPartsArgs {
+    const void *src;
+    uint16_t *dst;
+    uint64_t rows, src_stride, dst_stride, part;
+    uint32_t cols, pad;
+};
+
+struct HeadKeepArgs {
+    const int32_t *labels;
+    uint32_t *keep;
+    uint64_t rows;
 };
 
 struct HeadFinishArgs {
@@ -1159,7 +1180,8 @@ struct HeadFinishArgs {
     const float *label_margin;
     const int32_t *labels;
     const float *weight;
-    float *lse;
+    float *lse2;      // in units of log2, for the pairs
+    float *lse;       // or null
     float *loss;      // or null
     int32_t *best;    // or null
     uint64_t rows;

@@ -247,39 +247,76 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
 
 namespace {
 
-// The scores' gradients of one piece of the classes are held at a time, in
-// about this many bytes.
-constexpr uint64_t kPieceBytes = 256ull << 20;
+// The scores' gradients of one piece of the classes are held at a time, in at
+// most about this many bytes.
+constexpr uint64_t kPieceBytes = 1ull << 30;
+// Workgroups that run at once: two on each of 256 CUs.
+constexpr uint64_t kHeadSlots = 512;
+
+uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
+
+// Shares of a product's steps: where its tiles are fewer than the device
+// runs at once, enough of them to fill it, of 16 steps at least.
+uint32_t head_splits(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t t = tiles(m, kHeadM) * tiles(n, kHeadN), steps = tiles(k, kHeadK) * segments;
+    return (uint32_t)std::max<uint64_t>(1, std::min(kHeadSlots / std::max<uint64_t>(t, 1), steps / 16));
+}
 
 struct HeadPlan {
-    uint64_t class_tiles, row_tiles, piece;
-    float *part_max, *part_sum, *label_margin, *lse, *part_db, *dh;
+    uint64_t parts, segments, dim8;
+    bool copy_h, copy_w;
+    uint64_t piece, pieces;
+    uint32_t splits_h, splits_w;
+    bool sum_h;  // dh is summed from f32 parts
+    float *part_max, *part_sum, *label_margin, *lse2, *part_db, *dh, *dw;
     int32_t *part_best;
-    void *g;
+    uint16_t *h, *w, *g;
+    uint32_t *keep;
     uint64_t bytes;
 };
 
+// What the products read in place: bf16 rows of whole 16-byte pieces, near
+// enough to each other for a tile's 32-bit offsets.
+bool head_in_place(const void *p, uint64_t stride, const hbr_softmax &a) {
+    return a.dtype == HBR_BF16 && a.dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 22) &&
+           reinterpret_cast<uint64_t>(p) % 16 == 0;
+}
+
 HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, bool gradient, void *workspace) {
-    const uint64_t size = size_of(dtype, "softmax head");
+    size_of(dtype, "softmax head");
     if (classes == 0 || dim == 0) fail(kInvalid, "softmax head: no classes, or inputs of no elements");
     if (classes > 0x7fffffffull || n > 0x7fffffffull) fail(kRefused, "softmax head: more than 2^31 - 1 rows or classes");
+    if (dim >= (1u << 21)) fail(kRefused, "softmax head: inputs of 2,097,152 elements or more");
     HeadPlan q{};
-    q.class_tiles = (classes + kHeadTile - 1) / kHeadTile;
-    q.row_tiles = (n + kHeadTile - 1) / kHeadTile;
-    if (q.class_tiles > 65535 || dim > 65535 * (uint64_t)kHeadTile)
-        fail(kRefused, "softmax head: more than 4,194,240 classes or elements");
+    q.parts = dtype == HBR_F32 ? 3 : 1;
+    q.segments = dtype == HBR_F32 ? 6 : 1;
+    q.dim8 = up(dim, 8);
+    const uint64_t class_tiles = tiles(classes, kHeadM);
     Arena w(workspace);
-    q.part_max = w.take<float>(q.class_tiles * n);
-    q.part_sum = w.take<float>(q.class_tiles * n);
-    q.part_best = w.take<int32_t>(q.class_tiles * n);
+    q.part_max = w.take<float>(class_tiles * n);
+    q.part_sum = w.take<float>(class_tiles * n);
+    q.part_best = w.take<int32_t>(class_tiles * n);
     q.label_margin = w.take<float>(n);
-    q.lse = w.take<float>(n);
+    q.lse2 = w.take<float>(n);
+    q.h = w.take<uint16_t>(q.parts * n * q.dim8);
+    q.w = w.take<uint16_t>(q.parts * classes * q.dim8);
     if (gradient) {
-        const uint64_t fits = kPieceBytes / (std::max<uint64_t>(n, 1) * size) / kHeadTile * kHeadTile;
-        q.piece = std::min(up(classes, kHeadTile), std::max<uint64_t>(fits, kHeadTile));
-        q.g = w.take<char>(n * q.piece * size);
-        q.part_db = w.take<float>(q.row_tiles * q.piece);
-        q.dh = w.take<float>(n * dim);
+        // the pieces as even as whole tiles allow, each of enough tiles of
+        // dw to fill the device where that many classes fit
+        const uint64_t row_bytes = std::max<uint64_t>(n, 1) * 2 * q.parts;
+        const uint64_t fits = std::max<uint64_t>(kHeadM, kPieceBytes / row_bytes / kHeadM * kHeadM);
+        const uint64_t fills = tiles(kHeadSlots, tiles(dim, kHeadN)) * kHeadM;
+        q.pieces = tiles(classes, std::min(fits, std::max<uint64_t>(fills, kHeadM)));
+        q.piece = up(tiles(classes, q.pieces), kHeadM);
+        q.pieces = tiles(classes, q.piece);
+        q.splits_h = head_splits(n, dim, q.piece, q.segments);
+        q.splits_w = head_splits(q.piece, dim, n, q.segments);
+        q.sum_h = q.splits_h > 1 || q.pieces > 1;
+        q.g = w.take<uint16_t>(q.parts * n * q.piece);
+        q.part_db = w.take<float>(tiles(n, kHeadM) * q.piece);
+        if (q.sum_h) q.dh = w.take<float>(q.splits_h * n * dim);
+        if (q.splits_w > 1) q.dw = w.take<float>(q.splits_w * q.piece * dim);
+        q.keep = w.take<uint32_t>(tiles(n, 64) * 2);
     }
     q.bytes = w.used;
     return q;
@@ -301,6 +338,8 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     if ((n > 1 && p.h_stride < dim) || (classes > 1 && p.w_stride < dim) || (p.dh && n > 1 && p.dh_stride < dim) ||
         (p.dw && classes > 1 && p.dw_stride < dim))
         fail(kInvalid, std::string(what) + ": rows overlap");
+    if (p.dh_stride >= (1u << 21) || p.dw_stride >= (1u << 21))
+        fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
     for (const void *x : {p.h, p.w, (const void *)p.dh, (const void *)p.dw}) check_aligned(x, size, what);
     for (const void *x : {(const void *)p.bias, (const void *)p.labels, (const void *)p.weight, (const void *)p.loss,
                           (const void *)p.lse, (const void *)p.best, (const void *)p.db})
@@ -308,109 +347,165 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     check_workspace(workspace, workspace_bytes, q.bytes, what);
     Queue queue(ordinal, stream);
     const std::string suffix = name_of(p.dtype);
-    float *lse = p.lse ? p.lse : q.lse;
-    auto grid = [](uint64_t m, uint64_t c) {
-        return dim3((uint32_t)((m + kHeadTile - 1) / kHeadTile), (uint32_t)((c + kHeadTile - 1) / kHeadTile));
+    const dim3 threads(256);
+    auto cells = [](uint64_t n) { return dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 16)); };
+    auto sum = [&](const char *kernel, const float *part, uint64_t parts, uint64_t part_stride, void *dst, uint64_t rows,
+                   uint64_t cols, uint64_t dst_stride) {
+        HeadSumArgs a{};
+        a.part = part;
+        a.parts = (uint32_t)parts;
+        a.part_stride = part_stride;
+        a.dst = dst;
+        a.rows = rows;
+        a.cols = cols;
+        a.dst_stride = dst_stride;
+        queue.launch(kernel, cells(rows * cols), threads, a);
     };
-    HeadArgs z{};  // scores
-    z.a = p.h;
-    z.b = p.w;
-    z.a_m = p.h_stride;
-    z.b_n = p.w_stride;
-    z.a_k = z.b_k = 1;
-    z.m = z.rows = n;
-    z.n = classes;
-    z.k = dim;
+    const std::string sum_kernel = "hbr_head_sum_" + suffix;
+    if (n == 0) {  // sums over no rows
+        if (p.dw) sum(sum_kernel.c_str(), nullptr, 0, 0, p.dw, classes, dim, p.dw_stride);
+        if (p.db) sum("hbr_head_sum_f32", nullptr, 0, 0, p.db, 1, classes, classes);
+        return;
+    }
+    // the operands of the products: h, and w from class k on
+    auto parts = [&](const void *src, uint64_t stride, uint64_t rows, uint16_t *to) {
+        HeadPartsArgs a{};
+        a.src = src;
+        a.dst = to;
+        a.rows = rows;
+        a.src_stride = stride;
+        a.dst_stride = q.dim8;
+        a.part = rows * q.dim8;
+        a.cols = (uint32_t)dim;
+        queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.dim8 / 8), threads, a);
+    };
+    const uint16_t *h = static_cast<const uint16_t *>(p.h), *w = static_cast<const uint16_t *>(p.w);
+    uint64_t h_stride = n > 1 ? p.h_stride : q.dim8, w_stride = classes > 1 ? p.w_stride : q.dim8;
+    if (!head_in_place(h, h_stride, p)) {
+        parts(p.h, p.h_stride, n, q.h);
+        h = q.h;
+        h_stride = q.dim8;
+    }
+    if (!head_in_place(w, w_stride, p)) {
+        parts(p.w, p.w_stride, classes, q.w);
+        w = q.w;
+        w_stride = q.dim8;
+    }
+    const uint64_t h_part = n * q.dim8, w_part = classes * q.dim8;
+    auto product = [&](const char *kernel, HeadArgs a) {
+        a.m_tiles = (uint32_t)tiles(a.m, kHeadM);
+        a.n_tiles = (uint32_t)tiles(a.n, kHeadN);
+        a.segments = (uint32_t)q.segments;
+        queue.launch(kernel, dim3(a.m_tiles * a.n_tiles * a.splits), threads, a);
+    };
+    HeadArgs z{};
+    z.a = w;
+    z.b = h;
+    z.a_stride = w_stride;
+    z.b_stride = h_stride;
+    z.a_part = w_part;
+    z.b_part = h_part;
+    z.m = (uint32_t)classes;
+    z.n = (uint32_t)n;
+    z.k = (uint32_t)q.dim8;
+    z.splits = 1;
     z.bias = p.bias;
     z.labels = p.labels;
     z.part_max = q.part_max;
     z.part_sum = q.part_sum;
     z.part_best = p.best ? q.part_best : nullptr;
     z.label_margin = q.label_margin;
-    z.lse = lse;
-    z.weight = p.weight;
-    z.grad_scale = p.grad_scale;
-    if (n) {
-        queue.launch(("hbr_head_scores_" + suffix).c_str(), grid(n, classes), dim3(256), z);
-        HeadFinishArgs f{};
-        f.part_max = q.part_max;
-        f.part_sum = q.part_sum;
-        f.part_best = z.part_best;
-        f.label_margin = q.label_margin;
-        f.labels = p.labels;
-        f.weight = p.weight;
-        f.lse = lse;
-        f.loss = p.loss;
-        f.best = p.best;
-        f.rows = n;
-        f.classes = classes;
-        f.tiles = (uint32_t)q.class_tiles;
-        queue.launch("hbr_head_finish", dim3((uint32_t)((n + 63) / 64)), dim3(1024), f);
-    }
+    product("hbr_head_scores", z);
+    HeadFinishArgs f{};
+    f.part_max = q.part_max;
+    f.part_sum = q.part_sum;
+    f.part_best = z.part_best;
+    f.label_margin = q.label_margin;
+    f.labels = p.labels;
+    f.weight = p.weight;
+    f.lse2 = q.lse2;
+    f.lse = p.lse;
+    f.loss = p.loss;
+    f.best = p.best;
+    f.rows = n;
+    f.classes = classes;
+    f.tiles = (uint32_t)tiles(classes, kHeadM);
+    queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, 64)), dim3(1024), f);
     if (!gradient) return;
-    auto sum_grid = [](uint64_t cells) { return dim3((uint32_t)std::min<uint64_t>((cells + 255) / 256, 1u << 16)); };
+    if (p.dw) {
+        HeadKeepArgs k{};
+        k.labels = p.labels;
+        k.keep = q.keep;
+        k.rows = n;
+        queue.launch("hbr_head_keep", dim3((uint32_t)tiles(n, 256)), threads, k);
+    }
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
         const uint64_t kc = std::min(q.piece, classes - k0);
-        HeadArgs g = z;
-        g.b = static_cast<const char *>(p.w) + k0 * p.w_stride * size;
-        g.n = kc;
+        HeadArgs g{};
+        g.a = h;
+        g.b = w + k0 * w_stride;
+        g.a_stride = h_stride;
+        g.b_stride = w_stride;
+        g.a_part = h_part;
+        g.b_part = w_part;
+        g.m = (uint32_t)n;
+        g.n = (uint32_t)kc;
+        g.k = (uint32_t)q.dim8;
+        g.splits = 1;
+        g.bias = p.bias ? p.bias + k0 : nullptr;
+        g.labels = p.labels;
+        g.lse2 = q.lse2;
+        g.weight = p.weight;
         g.first = k0;
+        g.grad_scale = p.grad_scale;
         g.g = q.g;
         g.g_stride = q.piece;
+        g.g_part = n * q.piece;
         g.part_db = q.part_db;
-        if (n) queue.launch(("hbr_head_pairs_" + suffix).c_str(), grid(n, kc), dim3(256), g);
-        if (p.db) {
-            HeadSumArgs b{};
-            b.part = q.part_db;
-            b.dst = p.db + k0;
-            b.rows = 1;
-            b.cols = b.dst_stride = b.part_stride = kc;
-            b.parts = (uint32_t)q.row_tiles;
-            queue.launch("hbr_head_sum_f32", sum_grid(kc), dim3(256), b);
-        }
+        product(("hbr_head_pairs_" + suffix).c_str(), g);
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kHeadM), q.piece, p.db + k0, 1, kc, kc);
         if (p.dw) {
-            HeadArgs w{};
-            w.a = q.g;
-            w.a_m = 1;
-            w.a_k = q.piece;
-            w.b = p.h;
-            w.b_n = 1;
-            w.b_k = p.h_stride;
-            w.skip = p.labels;
-            w.m = kc;
-            w.n = dim;
-            w.k = n;
-            w.c = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
-            w.c_stride = p.dw_stride;
-            queue.launch(("hbr_head_out_" + suffix).c_str(), grid(kc, dim), dim3(256), w);
+            HeadArgs c{};
+            c.a = q.g;
+            c.b = h;
+            c.a_stride = q.piece;
+            c.b_stride = h_stride;
+            c.a_part = g.g_part;
+            c.b_part = h_part;
+            c.m = (uint32_t)up(kc, 8);
+            c.rows = (uint32_t)kc;
+            c.n = (uint32_t)dim;
+            c.k = (uint32_t)n;
+            c.splits = q.splits_w;
+            c.keep = q.keep;
+            char *to = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
+            const bool direct = q.splits_w == 1;
+            c.c = direct ? (void *)to : q.dw;
+            c.c_stride = direct ? p.dw_stride : dim;
+            c.c_split = q.piece * dim;
+            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", c);
+            if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, p.dw_stride);
         }
-        if (p.dh && n) {
-            HeadArgs h{};
-            h.a = q.g;
-            h.a_m = q.piece;
-            h.a_k = 1;
-            h.b = g.b;
-            h.b_n = 1;
-            h.b_k = p.w_stride;
-            h.m = n;
-            h.n = dim;
-            h.k = kc;
-            h.c = q.dh;
-            h.c_stride = dim;
-            h.accumulate = k0 != 0;
-            queue.launch(("hbr_head_add_" + suffix).c_str(), grid(n, dim), dim3(256), h);
+        if (p.dh) {
+            HeadArgs c{};
+            c.a = q.g;
+            c.b = g.b;
+            c.a_stride = q.piece;
+            c.b_stride = w_stride;
+            c.a_part = g.g_part;
+            c.b_part = w_part;
+            c.m = c.rows = (uint32_t)n;
+            c.n = (uint32_t)dim;
+            c.k = (uint32_t)kc;
+            c.splits = q.splits_h;
+            c.c = q.sum_h ? q.dh : p.dh;
+            c.c_stride = q.sum_h ? dim : p.dh_stride;
+            c.c_split = n * dim;
+            c.accumulate = k0 != 0;
+            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", c);
         }
     }
-    if (p.dh && n) {
-        HeadSumArgs h{};
-        h.part = q.dh;
-        h.dst = p.dh;
-        h.rows = n;
-        h.cols = dim;
-        h.dst_stride = p.dh_stride;
-        h.parts = 1;
-        queue.launch(("hbr_head_sum_" + suffix).c_str(), sum_grid(n * dim), dim3(256), h);
-    }
+    if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);
 }
 
 // ---- clipping ----------------------------------------------------------------------------

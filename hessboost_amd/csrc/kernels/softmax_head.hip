@@ -3,154 +3,435 @@
 //
 //   z = h W^T + b; lse = log sum exp z; loss = a (lse - z_y)
 //   g = c a (exp(z - lse) - [k = y]); dh = g W; dW = g^T h; db = sum g
+//
+// Scores are held in units of log2 (z log2 e), so that an exponential is one
+// v_exp_f32.
 #include "common.h"
 
 namespace hbr {
 
-constexpr uint32_t kHeadDepth = 16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+#define HBR_LDS __attribute__((address_space(3)))
 
-// One 64 x 64 tile of C[m][n] = sum_k A(m, k) B(n, k): 256 threads of 4 x 4
-// sums in f32, the operands staged in LDS as f32. A product's k that `skip`
-// marks is taken as zero on both sides, whatever stands there.
-template <typename E>
-__device__ __forceinline__ void head_tile(const HeadArgs &a, uint64_t m0, uint64_t n0, float (&acc)[4][4]) {
-    using T = typename E::type;
-    __shared__ float sa[kHeadDepth][kHeadTile + 4], sb[kHeadDepth][kHeadTile + 4];
-    const uint32_t tm = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0.0f;
-    for (uint64_t k0 = 0; k0 < a.k; k0 += kHeadDepth) {
-        for (uint32_t q = threadIdx.x; q < kHeadTile * kHeadDepth; q += 256) {
-            // along the axis that is contiguous in memory
-            const uint32_t am = a.a_k == 1 ? q / kHeadDepth : q % kHeadTile, ak = a.a_k == 1 ? q % kHeadDepth : q / kHeadTile;
-            const uint32_t bn = a.b_k == 1 ? q / kHeadDepth : q % kHeadTile, bk = a.b_k == 1 ? q % kHeadDepth : q / kHeadTile;
-            const uint64_t m = m0 + am, n = n0 + bn, ka = k0 + ak, kb = k0 + bk;
-            float va = 0.0f, vb = 0.0f;
-            if (m < a.m && ka < a.k && (!a.skip || a.skip[ka] >= 0))
-                va = E::up(static_cast<const T *>(a.a)[m * a.a_m + ka * a.a_k]);
-            if (n < a.n && kb < a.k && (!a.skip || a.skip[kb] >= 0))
-                vb = E::up(static_cast<const T *>(a.b)[n * a.b_n + kb * a.b_k]);
-            sa[ak][am] = va;
-            sb[bk][bn] = vb;
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t k = 0; k < kHeadDepth; k++) {
-            float va[4], vb[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) va[i] = sa[k][tm + i], vb[i] = sb[k][tn + i];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __builtin_fmaf(va[i], vb[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-}
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr uint32_t kNowhere = 0x80000000u;  // past every buffer: reads as zero
+
+__device__ __forceinline__ int32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane((int32_t)v); }
 
 // A running maximum's shift: a tile with no open class sums to zero.
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-__device__ __forceinline__ float exp_f32(float x) { return expf(x); }
-
-template <typename E>
-__device__ __forceinline__ void head_scores(const HeadArgs &a) {
-    const uint64_t m0 = (uint64_t)blockIdx.x * kHeadTile, n0 = (uint64_t)blockIdx.y * kHeadTile;
-    float acc[4][4];
-    head_tile<E>(a, m0, n0, acc);
-    const uint32_t tm = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint64_t r = m0 + tm + i;
-        const int32_t y = a.labels && r < a.m ? a.labels[r] : -1;
-        float top = -INFINITY;
-        int32_t best = (int32_t)n0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint64_t k = n0 + tn + j;
-            float z = acc[i][j] + (a.bias && k < a.n ? a.bias[k] : 0.0f);
-            if (k >= a.n) z = -INFINITY;
-            acc[i][j] = z;
-            if (y >= 0 && (uint64_t)y == k && k < a.n) a.label_margin[r] = z;
-            if (z > top) top = z, best = (int32_t)k;
-        }
-        for (int d = 1; d < 16; d <<= 1) {
-            const float t = __shfl_xor(top, d, kWave);
-            const int32_t b = __shfl_xor(best, d, kWave);
-            if (t > top || (t == top && b < best)) top = t, best = b;
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) sum += exp_f32(acc[i][j] - shift_of(top));
-        for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d, kWave);
-        if (threadIdx.x % 16 == 0 && r < a.m) {
-            const uint64_t at = (uint64_t)blockIdx.y * a.rows + r;
-            a.part_max[at] = top;
-            a.part_sum[at] = sum;
-            if (a.part_best) a.part_best[at] = best;
-        }
-    }
+__device__ __forceinline__ uint16_t to_bf16(float v) {
+    const __bf16 b = (__bf16)v;
+    return __builtin_bit_cast(uint16_t, b);
 }
 
-template <typename E>
-__device__ __forceinline__ void head_pairs(const HeadArgs &a) {
-    using T = typename E::type;
-    __shared__ float column[16][kHeadTile];
-    const uint64_t m0 = (uint64_t)blockIdx.x * kHeadTile, n0 = (uint64_t)blockIdx.y * kHeadTile;
-    float acc[4][4];
-    head_tile<E>(a, m0, n0, acc);
-    const uint32_t tm = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
-    float db[4] = {};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint64_t r = m0 + tm + i;
-        if (r >= a.m) continue;
-        const int32_t y = a.labels[r];
-        const float by = a.grad_scale * (a.weight ? a.weight[r] : 1.0f), lse = a.lse[r];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint64_t k = n0 + tn + j;
-            if (k >= a.n) continue;
-            const float z = acc[i][j] + (a.bias ? a.bias[a.first + k] : 0.0f);
-            float g = exp_f32(z - lse) - ((uint64_t)(int64_t)y == a.first + k ? 1.0f : 0.0f);
-            g = y < 0 ? 0.0f : g * by;
-            static_cast<T *>(a.g)[r * a.g_stride + k] = E::down(g);
-            db[j] += g;
+// An f32 as the sum of three bf16 values, exactly: each takes the next eight
+// bits of what is left. One that is not finite, or rounds to infinity, is not
+// split.
+__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
+    p[0] = to_bf16(v);
+    if ((p[0] & 0x7f80u) == 0x7f80u) {
+        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) {
+            p[1] = p[2] = 0;
+            return;
         }
+        p[0] = (uint16_t)(__float_as_uint(v) >> 16);
     }
-#pragma unroll
-    for (int j = 0; j < 4; j++) column[threadIdx.x / 16][tn + j] = db[j];
-    __syncthreads();
-    if (threadIdx.x < kHeadTile && n0 + threadIdx.x < a.n) {
-        float s = 0.0f;
-        for (int i = 0; i < 16; i++) s += column[i][threadIdx.x];
-        a.part_db[(uint64_t)blockIdx.x * a.n + n0 + threadIdx.x] = s;
-    }
+    const float rest = v - bf16_f32(p[0]);
+    p[1] = to_bf16(rest);
+    p[2] = to_bf16(rest - bf16_f32(p[1]));
 }
 
-// c in f32, or rounded to the type.
-template <typename E, bool Sum>
-__device__ __forceinline__ void head_product(const HeadArgs &a) {
-    using T = typename E::type;
-    const uint64_t m0 = (uint64_t)blockIdx.x * kHeadTile, n0 = (uint64_t)blockIdx.y * kHeadTile;
-    float acc[4][4];
-    head_tile<E>(a, m0, n0, acc);
-    const uint32_t tm = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
+// ---- one operand's tile in LDS ---------------------------------------------------------
+//
+// A tile is E rows x kHeadK (or kHeadK x E, transposed) bf16, filled by
+// 16-byte loads that go to LDS without registers: a wave's load fills 1 KiB
+// in lane order, so the layout is that of the loads, and the 16-byte pieces
+// of a row are exchanged by their source addresses instead (a piece's place
+// is xored with its row's low bits), which spreads the reads of a fragment
+// over the banks.
+template <bool T, int E>
+struct Operand {
+    static constexpr int kLoads = E / 64;                        // a wave's, a step
+    static constexpr int kBytes = E * kHeadK * 2;
+    static constexpr int kLanesRow = T ? E / 8 : kHeadK / 8;     // lanes of a row of the tile
+    static constexpr int kRowsLoad = 64 / kLanesRow;
+    const char *base;
+    uint32_t off[kLoads];  // a lane's source, bytes from base
+    uint32_t k_at[kLoads]; // and its first k within the step
+
+    // first: the tile's first row (m or n); size: how many there are
+    __device__ __forceinline__ void init(const void *p, uint64_t stride, uint64_t first, uint32_t size,
+                                         const int32_t *labels) {
+        const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
+        base = static_cast<const char *>(p) + (T ? first * 2 : first * stride * 2);
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            const uint32_t row = (wave * kLoads + j) * kRowsLoad + lane / kLanesRow, at = lane % kLanesRow;
+            if (T) {
+                const uint32_t piece = (((at >> 1) ^ (row & 3u)) << 1) | (at & 1u);
+                off[j] = first + piece * 8 < size ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
+                k_at[j] = row;
+            } else {
+                const uint32_t piece = at ^ ((row >> 1) & 3u);
+                const bool in = first + row < size && (!labels || labels[first + row] >= 0);
+                off[j] = in ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
+                k_at[j] = piece * 8;
+            }
+        }
+    }
+    // The step whose first k is k0 (k of them in all), from base + at bytes.
+    // The loads are not the compiler's: it would wait for them before any
+    // read of LDS, and the pipeline's own waits know which stage they fill.
+    __device__ __forceinline__ void load(uint32_t lds, uint64_t at, uint32_t k0, uint32_t k, uint32_t keep) const {
+        const uint64_t from = reinterpret_cast<uint64_t>(base) + at;
+        const i32x4 r = {uniform((uint32_t)from), uniform((uint32_t)(from >> 32)) & 0xffff, 0x7fffffff, 0x00020000};
+        const uint32_t to = uniform(lds + threadIdx.x / kWave * (kLoads * 1024));
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            const bool in = k0 + k_at[j] < k && (!T || (keep >> (k_at[j] & 31u)) & 1u);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(to + j * 1024), "v"(in ? off[j] : kNowhere), "s"(r)
+                         : "memory");
+        }
+    }
+    // Rows [row, row + 32) and products [16 kk, 16 kk + 16) of the tile: a
+    // lane's row is lane % 32, its products the eight from 8 (lane / 32) on.
+    static __device__ __forceinline__ bf16x8 fragment(const char *lds, uint32_t row, uint32_t kk) {
+        const uint32_t lane = lane_id();
+        if (T) {
+            // two transposing reads of four products: sixteen lanes read four
+            // rows of the tile, four elements each, and get a column each
+            const uint32_t k = kk * 16 + lane / 32 * 8 + lane % 16 / 4;
+            const uint32_t col = row + lane / 16 % 2 * 16;
+            const char *p = lds + k * (E * 2) + (((col >> 4) ^ (k & 3u)) << 5) + lane % 4 * 8;
+            union {
+                s16x4 h[2];
+                bf16x8 v;
+            } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)p);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)(p + 4 * E * 2));
+            return u.v;
+        }
+        const uint32_t m = row + lane % 32, piece = (kk * 2 + lane / 32) ^ ((m >> 1) & 3u);
+        return *reinterpret_cast<const bf16x8 *>(lds + m * (kHeadK * 2) + piece * 16);
+    }
+};
+
+// The pairs of parts of a product of two f32 operands, smallest first: (2, 0),
+// (0, 2), (1, 1), (1, 0), (0, 1), (0, 0), two bits a segment.
+constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+
+constexpr int kHeadThreads = 256;  // four waves, 2 x 2, of 128 x 64 each
+constexpr int kStages = 3;
+constexpr int kStageBytes = (kHeadM + kHeadN) * kHeadK * 2;
+
+struct HeadTile {
+    uint32_t m0, n0, split;  // the tile's first row and column, and its share of the steps
+    f32x16 acc[4][2];
+    // element e of acc[i][j]: row wave_m + 32 i + row_of(e), column wave_n + 32 j + lane % 32
+    uint32_t wave_m, wave_n;
+};
+
+__device__ __forceinline__ uint32_t row_of(int e) { return 8 * (e / 4) + 4 * (lane_id() / 32) + e % 4; }
+
+// A workgroup's tile: neighbours in the launch go to different XCDs, so each
+// XCD takes a contiguous share of the tiles, in groups of eight rows of tiles
+// whose operands its L2 holds.
+__device__ __forceinline__ void head_place(const HeadArgs &a, HeadTile &t) {
+    const uint32_t all = gridDim.x, per = all / 8, rest = all % 8, xcd = blockIdx.x % 8;
+    uint32_t id = xcd * per + min(xcd, rest) + blockIdx.x / 8;
+    const uint32_t tiles = a.m_tiles * a.n_tiles;
+    t.split = id / tiles;
+    id -= t.split * tiles;
+    constexpr uint32_t kGroup = 8;
+    const uint32_t group = id / (kGroup * a.n_tiles), first = group * kGroup;
+    const uint32_t rows = min(kGroup, a.m_tiles - first), in = id - group * kGroup * a.n_tiles;
+    t.m0 = (first + in % rows) * kHeadM;
+    t.n0 = in / rows * kHeadN;
+    const uint32_t wave = threadIdx.x / kWave;
+    t.wave_m = wave / 2 * 128;
+    t.wave_n = wave % 2 * 64;
+}
+
+template <bool AT, bool BT>
+__device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, HeadTile &t, const int32_t *a_labels = nullptr) {
+    Operand<AT, kHeadM> oa;
+    Operand<BT, kHeadN> ob;
+    oa.init(a.a, a.a_stride, t.m0, a.m, a_labels);
+    ob.init(a.b, a.b_stride, t.n0, a.n, nullptr);
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint64_t m = m0 + tm + i, n = n0 + tn + j;
-            if (m >= a.m || n >= a.n) continue;
-            if (Sum) {
-                float *c = static_cast<float *>(a.c) + m * a.c_stride + n;
-                *c = a.accumulate ? *c + acc[i][j] : acc[i][j];
-            } else {
-                static_cast<T *>(a.c)[m * a.c_stride + n] = E::down(acc[i][j]);
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) t.acc[i][j][e] = 0.0f;
+    const uint32_t per = (a.k + kHeadK - 1) / kHeadK, steps = per * a.segments;
+    const uint32_t s0 = (uint32_t)((uint64_t)steps * t.split / a.splits),
+                   s1 = (uint32_t)((uint64_t)steps * (t.split + 1) / a.splits);
+    // the loads run two steps ahead; past the end they read nothing
+    uint32_t seg = s0 / per, at = s0 % per;
+    auto load = [&](uint32_t s) {
+        const uint32_t k0 = s < s1 ? at * kHeadK : a.k;
+        const uint32_t of = a.segments == 1 ? 10 : 2 * min(seg, 5u);
+        const uint64_t pa = (kPartA >> of & 3u) * a.a_part, pb = (kPartB >> of & 3u) * a.b_part;
+        const uint32_t keep = (AT || BT) && a.keep && s < s1 ? a.keep[at] : 0xffffffffu;
+        const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % kStages * kStageBytes;
+        oa.load(to, (pa + (uint64_t)at * kHeadK * (AT ? a.a_stride : 1)) * 2, k0, a.k, keep);
+        ob.load(to + Operand<AT, kHeadM>::kBytes, (pb + (uint64_t)at * kHeadK * (BT ? a.b_stride : 1)) * 2, k0, a.k, keep);
+        if (++at == per) at = 0, seg++;
+    };
+    load(s0);
+    load(s0 + 1);
+    for (uint32_t s = s0; s < s1; s++) {
+        // this step's loads are in: those of the next are the last six
+        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load(s + 2);
+        const char *from = lds + s % kStages * kStageBytes;
+        const char *from_b = from + Operand<AT, kHeadM>::kBytes;
+#pragma unroll
+        for (uint32_t kk = 0; kk < kHeadK / 16; kk++) {
+            bf16x8 fa[4], fb[2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) fa[i] = Operand<AT, kHeadM>::fragment(from, t.wave_m + 32 * i, kk);
+#pragma unroll
+            for (int j = 0; j < 2; j++) fb[j] = Operand<BT, kHeadN>::fragment(from_b, t.wave_n + 32 * j, kk);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
+        }
+    }
+    // the loads ahead have landed before the LDS or the workgroup ends
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// ---- the scores' maxima and sums -----------------------------------------------------------
+
+// m: classes, n: rows. A lane holds 64 classes of two rows: maxima and sums
+// stay in its registers but for the other half of the wave and the other
+// wave of the same rows.
+__device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
+    __shared__ float bias[kHeadM];
+    __shared__ float top_of[2][kHeadN], sum_of[2][kHeadN];
+    __shared__ int32_t best_of[2][kHeadN];
+    HeadTile t;
+    head_place(a, t);
+    {
+        const uint32_t c = t.m0 + threadIdx.x;
+        bias[threadIdx.x] = c >= a.m ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+    }
+    head_product<false, false>(a, lds, t);
+    const uint32_t lane = lane_id(), wm = t.wave_m / 128;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint32_t in = t.wave_n + 32 * j + lane % 32, r = t.n0 + in;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float z = __builtin_fmaf(t.acc[i][j][e], kLog2e, bias[t.wave_m + 32 * i + row_of(e)]);
+                t.acc[i][j][e] = z;
+                top = fmaxf(top, z);
+            }
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float shift = shift_of(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(t.acc[i][j][e] - shift);
+        sum += __shfl_xor(sum, 32, kWave);
+        // the label's class, where it is one of the wave's
+        const int64_t y = a.labels && r < a.n ? (int64_t)a.labels[r] - t.m0 - t.wave_m : -1;
+        if (__ballot(y >= 0 && y < 128)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (y == 32 * i + row_of(e) && t.m0 + t.wave_m + y < a.m) a.label_margin[r] = t.acc[i][j][e];
+        }
+        int32_t best = 0x7fffffff;
+        if (a.part_best) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (t.acc[i][j][e] == top) best = min(best, (int32_t)(t.m0 + t.wave_m + 32 * i + row_of(e)));
+            best = min(best, __shfl_xor(best, 32, kWave));
+        }
+        if (lane < 32) {
+            top_of[wm][in] = top;
+            sum_of[wm][in] = sum;
+            best_of[wm][in] = best;
+        }
+    }
+    __syncthreads();
+    const uint32_t in = threadIdx.x, r = t.n0 + in;
+    if (in >= kHeadN || r >= a.n) return;
+    const float t0 = top_of[0][in], t1 = top_of[1][in], top = fmaxf(t0, t1), shift = shift_of(top);
+    const uint64_t at = (uint64_t)(t.m0 / kHeadM) * a.n + r;
+    a.part_max[at] = top;
+    a.part_sum[at] = sum_of[0][in] * __builtin_amdgcn_exp2f(t0 - shift) + sum_of[1][in] * __builtin_amdgcn_exp2f(t1 - shift);
+    if (a.part_best) a.part_best[at] = best_of[t1 > t0 ? 1 : 0][in];
+}
+
+// ---- the scores' gradients --------------------------------------------------------------------
+
+// m: rows, n: classes. A lane holds 64 rows of two classes, so a class's sum
+// over the rows stays in its registers; a row whose label is below 0 is read
+// as zeros and has no gradient. Past the classes g is zero up to its stride.
+template <int Parts>
+__device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
+    __shared__ float lse_of[kHeadM], by_of[kHeadM];
+    __shared__ int32_t label_of[kHeadM];
+    __shared__ float db_of[2][kHeadN];
+    HeadTile t;
+    head_place(a, t);
+    {
+        const uint32_t r = t.m0 + threadIdx.x;
+        const int32_t y = r < a.m ? a.labels[r] : -1;
+        const bool live = y >= 0;
+        lse_of[threadIdx.x] = live ? a.lse2[r] : INFINITY;
+        by_of[threadIdx.x] = live ? a.grad_scale * (a.weight ? a.weight[r] : 1.0f) : 0.0f;
+        const int64_t in = (int64_t)y - (int64_t)a.first - t.n0;
+        label_of[threadIdx.x] = live && in >= 0 && in < (int64_t)kHeadN ? (int32_t)in : -1;
+    }
+    head_product<false, false>(a, lds, t, a.labels);
+    const uint32_t lane = lane_id(), wm = t.wave_m / 128;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint32_t in = t.wave_n + 32 * j + lane % 32, c = t.n0 + in;
+        const float bias = c >= a.n ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+        float db = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            __builtin_amdgcn_sched_barrier(0);  // the rows' values of one i at a time in registers
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const uint32_t m = t.wave_m + 32 * i + row_of(e);
+                const float z = __builtin_fmaf(t.acc[i][j][e], kLog2e, bias);
+                float p = __builtin_amdgcn_exp2f(z - lse_of[m]);
+                if (label_of[m] == (int32_t)in) p -= 1.0f;
+                const float v = p * by_of[m];
+                db += v;
+                t.acc[i][j][e] = v;
             }
         }
+        db += __shfl_xor(db, 32, kWave);
+        if (lane < 32) db_of[wm][in] = db;
+    }
+    // through LDS to stores of 16 bytes: bf16 whole, f32 in two halves of the
+    // rows, split on the way out. A row of LDS is 16 bytes longer than the
+    // tile's, so that the wave's two rows of a write meet different banks.
+    constexpr int kHalves = Parts == 1 ? 1 : 2, kSize = Parts == 1 ? 2 : 4, kI = 4 / kHalves;
+    constexpr uint32_t kRow = kHeadN * kSize + 16, kRows = kHeadM / kHalves;
+    static_assert(kRows * kRow <= kStages * kStageBytes, "the pairs fit the stages");
+#pragma unroll
+    for (int half = 0; half < kHalves; half++) {
+        if (half) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kI; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    char *to = lds + (t.wave_m / kHalves + 32 * i + row_of(e)) * kRow + (t.wave_n + 32 * j + lane % 32) * kSize;
+                    const float v = t.acc[half * kI + i][j][e];
+                    if constexpr (Parts == 1) *reinterpret_cast<uint16_t *>(to) = to_bf16(v);
+                    else *reinterpret_cast<float *>(to) = v;
+                }
+        }
+        __syncthreads();
+        const uint32_t col = threadIdx.x % 16 * 8;
+        uint16_t *g = static_cast<uint16_t *>(a.g) + t.n0 + col;
+        for (uint32_t m = threadIdx.x / 16; m < kRows; m += kHeadThreads / 16) {
+            // the wave of rows from 128 on holds the second half of LDS's rows
+            const uint64_t r = t.m0 + (Parts == 1 ? m : m / 64 * 128 + half * 64 + m % 64);
+            if (r >= a.m) continue;
+            if constexpr (Parts == 1) {
+                *reinterpret_cast<i32x4 *>(g + r * a.g_stride) = *reinterpret_cast<const i32x4 *>(lds + m * kRow + col * 2);
+            } else {
+                Vec<float, 4> v[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    v[k] = *reinterpret_cast<const Vec<float, 4> *>(lds + m * kRow + (col + 4 * k) * 4);
+                Vec<uint16_t, 8> out[3];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    uint16_t s[3];
+                    split3(v[k / 4].v[k % 4], s);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) out[q].v[k] = s[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(g + q * a.g_part + r * a.g_stride) = out[q];
+            }
+        }
+    }
+    const uint32_t c = t.n0 + threadIdx.x;
+    if (threadIdx.x < kHeadN && c < a.n)
+        a.part_db[(uint64_t)(t.m0 / kHeadM) * a.g_stride + c] = db_of[0][threadIdx.x] + db_of[1][threadIdx.x];
+}
+
+// ---- the products with the gradients ---------------------------------------------------------------
+
+// E: what c holds: f32 sums (a share's, added to or not) or the result.
+template <typename E, bool AT>
+__device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
+    using T = typename E::type;
+    HeadTile t;
+    head_place(a, t);
+    head_product<AT, true>(a, lds, t);
+    const uint32_t lane = lane_id();
+    // the tile's rows as a buffer that ends with its last: what lies past the
+    // rows or the columns is neither read nor written
+    const uint64_t from = reinterpret_cast<uint64_t>(static_cast<T *>(a.c) + t.split * a.c_split + t.m0 * a.c_stride + t.n0);
+    const uint32_t stride = (uint32_t)a.c_stride * sizeof(T);
+    const uint32_t rows = min(a.rows > t.m0 ? a.rows - t.m0 : 0u, kHeadM);
+    const uint32_t size = rows ? (rows - 1) * stride + min(a.n - t.n0, kHeadN) * (uint32_t)sizeof(T) : 0u;
+    __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(from), 0, size, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint32_t n = t.wave_n + 32 * j + lane % 32;
+        const uint32_t at = t.n0 + n < a.n ? (t.wave_m + lane / 32 * 4) * stride + n * (uint32_t)sizeof(T) : kNowhere;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) {
+                if (a.accumulate) {
+                    float before[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        before[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                            c, at + (32 * i + 8 * (e / 4) + e % 4) * stride, 0, 0));
+#pragma unroll
+                    for (int e = 0; e < 16; e++) t.acc[i][j][e] += before[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const uint32_t to = at + (32 * i + 8 * (e / 4) + e % 4) * stride;
+                if constexpr (sizeof(T) == 4)
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(t.acc[i][j][e]), c, to, 0, 0);
+                else
+                    __builtin_amdgcn_raw_buffer_store_b16(to_bf16(t.acc[i][j][e]), c, to, 0, 0);
+            }
+        }
+    }
 }
 
 template <typename E>
@@ -164,18 +445,63 @@ __device__ __forceinline__ void head_sum(const HeadSumArgs &a) {
     }
 }
 
+// Eight elements of a row a thread.
+template <typename E, int Parts>
+__device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
+    using T = typename E::type;
+    const uint64_t wide = a.dst_stride / 8, cells = a.rows * wide;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t r = i / wide;
+        const uint32_t c = (uint32_t)(i - r * wide) * 8;
+        const T *src = static_cast<const T *>(a.src) + r * a.src_stride + c;
+        Vec<uint16_t, 8> out[Parts];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const T v = c + k < a.cols ? src[k] : (T)0;
+            if (Parts == 1) {
+                out[0].v[k] = (uint16_t)v;
+            } else {
+                uint16_t s[3];
+                split3(E::up(v), s);
+#pragma unroll
+                for (int q = 0; q < Parts; q++) out[q].v[k] = s[q];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < Parts; q++)
+            *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + q * a.part + r * a.dst_stride + c) = out[q];
+    }
+}
+
 }  // namespace hbr
 
 using namespace hbr;
 
-#define HBR_HEAD(suffix, E)                                                                                       \
-    extern "C" __global__ __launch_bounds__(256) void hbr_head_scores_##suffix(HeadArgs a) { head_scores<E>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void hbr_head_pairs_##suffix(HeadArgs a) { head_pairs<E>(a); }   \
-    extern "C" __global__ __launch_bounds__(256) void hbr_head_add_##suffix(HeadArgs a) { head_product<E, true>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void hbr_head_out_##suffix(HeadArgs a) { head_product<E, false>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void hbr_head_sum_##suffix(HeadSumArgs a) { head_sum<E>(a); }
-HBR_HEAD(f32, F32)
-HBR_HEAD(bf16, Bf16)
+#define HBR_HEAD(name, body)                                                            \
+    extern "C" __global__ __launch_bounds__(kHeadThreads, 2) void name(HeadArgs a) {    \
+        __shared__ __align__(1024) char lds[kStages * kStageBytes];                     \
+        body(a, lds);                                                                   \
+    }
+HBR_HEAD(hbr_head_scores, head_scores)
+HBR_HEAD(hbr_head_pairs_bf16, head_pairs<1>)
+HBR_HEAD(hbr_head_pairs_f32, head_pairs<3>)
+#define HBR_COMMA ,
+HBR_HEAD(hbr_head_dh_part, head_sums<F32 HBR_COMMA false>)
+HBR_HEAD(hbr_head_dh_bf16, head_sums<Bf16 HBR_COMMA false>)
+HBR_HEAD(hbr_head_dw_part, head_sums<F32 HBR_COMMA true>)
+HBR_HEAD(hbr_head_dw_bf16, head_sums<Bf16 HBR_COMMA true>)
+
+extern "C" __global__ __launch_bounds__(256) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_f32(HeadPartsArgs a) { head_parts<F32, 3>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_bf16(HeadPartsArgs a) { head_parts<Bf16, 1>(a); }
+
+// Bit r: row r has a label (of 64 rows a wave, two words).
+extern "C" __global__ __launch_bounds__(256) void hbr_head_keep(HeadKeepArgs a) {
+    const uint64_t r = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t bits = __ballot(r < a.rows && a.labels[r] >= 0);
+    if (lane_id() < 2 && (r - lane_id()) < a.rows) a.keep[(r - lane_id()) / 32 + lane_id()] = (uint32_t)(bits >> (32 * lane_id()));
+}
 
 // A row's tiles joined: 64 rows a workgroup, its 16 waves a share of the
 // class tiles each, in order within a wave and over the waves.
@@ -187,47 +513,33 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
     const uint64_t r = (uint64_t)blockIdx.x * kWave + lane;
     const uint32_t share = (a.tiles + kWaves - 1) / kWaves;
     float top = -INFINITY, sum = 0.0f;
-    int32_t best = 0;
-    bool any = false;
-    if (r < a.rows) {
-        for (uint32_t t = wave * share; t < min(a.tiles, (wave + 1) * share); t++) {
-            const float m = a.part_max[t * a.rows + r], s = a.part_sum[t * a.rows + r];
-            if (!any || m > top) {
-                sum = sum * exp_f32(top - shift_of(m)) + s;
-                top = m;
-                if (a.part_best) best = a.part_best[t * a.rows + r];
-            } else {
-                sum += s * exp_f32(m - shift_of(top));
-            }
-            any = true;
-        }
-    }
-    top_of[wave][lane] = any ? top : -INFINITY;
+    int32_t best = 0x7fffffff;
+    auto join = [&](float m, float s, int32_t b) {
+        const float both = fmaxf(top, m), shift = shift_of(both);
+        sum = sum * __builtin_amdgcn_exp2f(top - shift) + s * __builtin_amdgcn_exp2f(m - shift);
+        best = m > top ? b : m == top ? min(best, b) : best;
+        top = both;
+    };
+    if (r < a.rows)
+        for (uint32_t t = wave * share; t < min(a.tiles, (wave + 1) * share); t++)
+            join(a.part_max[t * a.rows + r], a.part_sum[t * a.rows + r], a.part_best ? a.part_best[t * a.rows + r] : 0);
+    top_of[wave][lane] = top;
     sum_of[wave][lane] = sum;
     best_of[wave][lane] = best;
     __syncthreads();
     if (wave != 0 || r >= a.rows) return;
-    for (uint32_t w = 1; w < kWaves; w++) {
-        if (w * share >= a.tiles) break;
-        const float m = top_of[w][lane], s = sum_of[w][lane];
-        if (m > top) {
-            sum = sum * exp_f32(top - shift_of(m)) + s;
-            top = m;
-            best = best_of[w][lane];
-        } else {
-            sum += s * exp_f32(m - shift_of(top));
-        }
-    }
+    for (uint32_t w = 1; w < kWaves && w * share < a.tiles; w++) join(top_of[w][lane], sum_of[w][lane], best_of[w][lane]);
     const int32_t y = a.labels ? a.labels[r] : -1;
     // a label that is no class: neither a loss nor a gradient
-    const float lse = y >= 0 && (uint64_t)y >= a.classes ? NAN : shift_of(top) + logf(sum);
-    a.lse[r] = lse;
-    if (a.best) a.best[r] = best;
+    const float lse2 = y >= 0 && (uint64_t)y >= a.classes ? NAN : shift_of(top) + __builtin_amdgcn_logf(sum);
+    a.lse2[r] = lse2;
+    if (a.lse) a.lse[r] = lse2 * kLn2;
+    if (a.best) a.best[r] = best == 0x7fffffff ? 0 : best;  // a row of NaN has none
     if (!a.loss) return;
     if (!a.labels) {
-        a.loss[r] = lse - top;
+        a.loss[r] = (lse2 - top) * kLn2;
         return;
     }
     const float by = a.weight ? a.weight[r] : 1.0f;
-    a.loss[r] = y < 0 ? 0.0f : (uint64_t)y >= a.classes ? NAN : by * (lse - a.label_margin[r]);
+    a.loss[r] = y < 0 ? 0.0f : (uint64_t)y >= a.classes ? NAN : by * ((lse2 - a.label_margin[r]) * kLn2);
 }
