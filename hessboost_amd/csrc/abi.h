@@ -1071,8 +1071,34 @@ struct EmbedArgs {
     uint64_t out_stride;
     uint32_t columns;
     uint32_t dim;
-    uint32_t vecs;            // vectors a row
+    uint32_t vecs;              // vectors a row
     uint32_t rows_per_block;
+    uint32_t columns_per_pass;  // a multiple of 8; with the rows at most 4,096 ids
+    uint32_t pad;
+};
+
+// hbr_lookup_columns_*: rows of a block at most, and elements of a slice.
+constexpr uint32_t kColumnBlock = 16384;
+constexpr uint32_t kColumnSlice = 128;
+struct LookupColumnArgs {
+    const int32_t *ids;
+    const int32_t *offset;
+    const float *scale;
+    const void *dout;
+    void *dtable;
+    float *part;              // [block][table row][part_stride], where there are several blocks
+    uint64_t ids_stride;
+    uint64_t dout_stride;
+    uint64_t dtable_stride;
+    uint64_t part_stride;
+    uint64_t table_rows;
+    uint64_t n_rows;
+    uint32_t columns;
+    uint32_t vecs;
+    uint32_t block_rows;
+    uint32_t blocks;
+    uint32_t slices;
+    uint32_t slice_vecs;
 };
 
 // Entries of one sort tile (hbr_sort_*): 256 threads x 16.

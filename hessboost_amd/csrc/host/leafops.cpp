@@ -9,6 +9,8 @@ namespace hbr {
 
 namespace {
 
+constexpr uint32_t kWaveLanes = 64;
+
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // A workspace handed out from its start, 256 bytes apart. Without memory it
@@ -136,14 +138,20 @@ void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *
     a.dim = p.dim;
     a.vecs = p.dim / v;
     a.rows_per_block = std::max(1u, 256 / a.vecs);
+    a.columns_per_pass = (uint32_t)std::min<uint64_t>(up(std::max(a.columns, 1u), 8), 4096 / a.rows_per_block / 8 * 8);
     const uint64_t blocks = (p.n_rows + a.rows_per_block - 1) / a.rows_per_block;
-    const std::string k = std::string("hbr_leaf_embed_") + name_of(p.dtype) + "_" + std::to_string(v);
+    const bool far = p.table_rows * p.table_stride * size >= (1ull << 31);
+    const std::string k = std::string(far ? "hbr_leaf_embed_far_" : "hbr_leaf_embed_") + name_of(p.dtype) + "_" + std::to_string(v);
     queue.launch(k.c_str(), dim3((uint32_t)std::min<uint64_t>(blocks, 1u << 20)), dim3(256), a);
 }
 
 namespace {
 
 struct LookupPlan {
+    // a column at a time
+    bool columns;
+    uint32_t blocks, block_rows;
+    // by sorting
     uint64_t n;  // entries
     uint32_t tiles, passes, chunk, chunks;
     uint32_t *key[2], *val[2], *hist, *total, *start;
@@ -151,11 +159,29 @@ struct LookupPlan {
     uint64_t bytes;
 };
 
-LookupPlan lookup_plan(const hbr_lookup &p, void *workspace) {
+LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     LookupPlan q{};
     if (p.n_columns && p.n_rows > 0x7fffffffull / p.n_columns)
         fail(kRefused, "leaf embedding gradient: more than 2^31 - 1 ids");
     q.n = p.n_rows * p.n_columns;
+    Arena w(workspace);
+    // Columns of their own table rows (one column, or offsets), where a table
+    // row has many ids and a column few enough rows for LDS, are summed a
+    // column at a time, in blocks of rows: enough for the device, of which
+    // each reads at least as many vectors as it writes sums.
+    q.columns = q.n && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows && p.table_rows / p.n_columns <= 2048;
+    if (q.columns) {
+        const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
+        const uint64_t most = std::max<uint64_t>(1, q.n / (8 * p.table_rows));
+        const uint64_t fills = (1024 + p.n_columns * slices - 1) / (p.n_columns * slices);
+        uint64_t blocks = std::max((p.n_rows + kColumnBlock - 1) / kColumnBlock, std::min({most, fills, (p.n_rows + 511) / 512}));
+        if (blocks > 4) blocks = up(blocks, 8);
+        q.blocks = (uint32_t)blocks;
+        q.block_rows = (uint32_t)((p.n_rows + blocks - 1) / blocks);
+        if (blocks > 1) q.part = w.take<float>(blocks * p.table_rows * up(p.dim, 4));
+        q.bytes = w.used;
+        return q;
+    }
     q.tiles = (uint32_t)((q.n + kSortTile - 1) / kSortTile);
     // keys run from 0 to table_rows
     uint32_t bits = 1;
@@ -164,7 +190,6 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace) {
     // about 8,192 waves, 32 to 512 entries each
     q.chunk = (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(32, up(q.n / 8192, 32)));
     q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
-    Arena w(workspace);
     for (int b = 0; b < 2; b++) {
         q.key[b] = w.take<uint32_t>(q.n);
         q.val[b] = w.take<uint32_t>(q.n);
@@ -180,8 +205,12 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace) {
 }  // namespace
 
 uint64_t leaf_embedding_grad_workspace(const hbr_lookup &p) {
-    check_lookup(p, "leaf embedding gradient");
-    return lookup_plan(p, nullptr).bytes;
+    hbr_lookup q = p;
+    q.ids = reinterpret_cast<const int32_t *>(16);  // sizes alone count
+    q.offset = nullptr;
+    q.scale = nullptr;
+    check_lookup(q, "leaf embedding gradient");
+    return std::max(lookup_plan(p, nullptr, false).bytes, lookup_plan(p, nullptr, true).bytes);
 }
 
 void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const void *dout, void *dtable,
@@ -193,9 +222,36 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     if (!dtable || (!dout && p.n_rows)) fail(kInvalid, std::string(what) + ": null argument");
     check_aligned(dout, size, what);
     check_aligned(dtable, size, what);
-    const LookupPlan q = lookup_plan(p, workspace);
+    const LookupPlan q = lookup_plan(p, workspace, p.offset != nullptr);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
     Queue queue(ordinal, stream);
+    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
+    const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
+    auto blocks = [](uint64_t threads) { return dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16)); };
+    if (q.columns) {
+        LookupColumnArgs a{};
+        a.ids = p.ids;
+        a.offset = p.offset;
+        a.scale = p.scale;
+        a.dout = dout;
+        a.dtable = dtable;
+        a.part = q.part;
+        a.ids_stride = p.ids_stride;
+        a.dout_stride = p.out_stride;
+        a.dtable_stride = p.table_stride;
+        a.part_stride = up(p.dim, 4);
+        a.table_rows = p.table_rows;
+        a.n_rows = p.n_rows;
+        a.columns = p.n_columns;
+        a.vecs = p.dim / v;
+        a.block_rows = q.block_rows;
+        a.blocks = q.blocks;
+        a.slice_vecs = std::min<uint32_t>(kColumnSlice / v, kWaveLanes);
+        a.slices = (a.vecs + a.slice_vecs - 1) / a.slice_vecs;
+        queue.launch(("hbr_lookup_columns_" + suffix).c_str(), dim3(q.blocks * a.columns * a.slices), dim3(1024), a);
+        if (q.blocks > 1) queue.launch(("hbr_lookup_join_" + suffix).c_str(), blocks(p.table_rows * a.vecs), dim3(256), a);
+        return;
+    }
     int from = 0;
     for (uint32_t pass = 0; pass < q.passes && q.n; pass++) {
         LookupSortArgs a{};
@@ -218,7 +274,6 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
         queue.launch("hbr_sort_scatter", dim3(q.tiles), dim3(256), a);
         from ^= 1;
     }
-    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
     LookupSumArgs a{};
     a.keys = q.key[from];
     a.vals = q.val[from];
@@ -236,8 +291,6 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     a.vecs = p.dim / v;
     a.chunk = q.chunk;
     a.chunks = q.chunks;
-    auto blocks = [](uint64_t threads) { return dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16)); };
-    const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
     queue.launch("hbr_lookup_starts", blocks(p.table_rows + 1), dim3(256), a);
     queue.launch(("hbr_lookup_sum_" + suffix).c_str(), dim3((q.chunks + 3) / 4), dim3(256), a);
     queue.launch(("hbr_lookup_finish_" + suffix).c_str(), blocks(p.table_rows * a.vecs), dim3(256), a);

@@ -25,56 +25,318 @@ struct Bf16 {
 };
 
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
+struct alignas(sizeof(T) * V <= 16 ? sizeof(T) * V : 16) Vec {
     T v[V];
 };
 
-// The table row of an id of column t; at or past table_rows when it adds
-// nothing (a negative id, or one that leads out of the table).
-__device__ __forceinline__ uint64_t table_row(int32_t id, const int32_t *offset, uint32_t t, uint64_t table_rows) {
-    const int64_t row = (int64_t)id + (offset ? offset[t] : 0);
-    return id < 0 || row < 0 || (uint64_t)row >= table_rows ? table_rows : (uint64_t)row;
+// A vector from a buffer at a byte offset; zeros past its end.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> buffer_vec(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    if constexpr (sizeof(T) * V == 16) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+    else if constexpr (sizeof(T) * V == 8) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0));
+    else if constexpr (sizeof(T) * V == 4) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+    else return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
 }
 
-// A thread holds one vector of one row's sum and walks the columns in order,
-// kAhead look-ups in flight.
-template <typename E, int V>
+// The table row of an id of column t; table_rows when it adds nothing (a
+// negative id, or one that leads out of the column's rows). With offsets
+// column t holds the rows from offset[t] up to the next column's, the last
+// up to the table's end.
+__device__ __forceinline__ uint64_t table_row(int32_t id, const int32_t *offset, uint32_t t, uint32_t columns,
+                                              uint64_t table_rows) {
+    int64_t row = id, end = (int64_t)table_rows;
+    if (offset) {
+        row += offset[t];
+        if (t + 1 < columns) end = min(end, (int64_t)offset[t + 1]);
+    }
+    return id < 0 || row < 0 || row >= end ? table_rows : (uint64_t)row;
+}
+
+__device__ __forceinline__ uint32_t nowhere() { return 0x80000000u; }  // past every buffer: reads as zero
+
+// A workgroup takes rows_per_block rows and places their ids in LDS as the
+// byte offsets of their table rows, kPlaces at a time; a thread then holds one
+// vector of one row's sum and walks the columns in order, eight look-ups in
+// flight. What an id costs (its check, its address) is paid once and not by
+// every vector of its row, and an id that adds nothing reads past the
+// buffer's end, as zeros. Far: tables of 2 GiB and more hold row numbers
+// there, and the addresses are made in 64 bits.
+//
+// Bound by the vectors that the L2 gives to the CUs.
+constexpr uint32_t kPlaces = 4096;
+template <typename E, int V, bool Far>
 __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
     using T = typename E::type;
     constexpr uint32_t kAhead = 8;
+    __shared__ __align__(16) uint32_t place[kPlaces];
+    __shared__ __align__(16) float scale[kPlaces];
     const uint64_t blocks = (a.n_rows + a.rows_per_block - 1) / a.rows_per_block;
-    const uint32_t cells = a.rows_per_block * a.vecs;
+    const uint32_t cells = a.rows_per_block * a.vecs, wide = a.columns_per_pass;
+    __amdgpu_buffer_rsrc_t table = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(a.table), 0, 0x7fffffff, 0x00020000);
     for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-        for (uint32_t i = threadIdx.x; i < cells; i += 256) {
-            const uint64_t r = b * a.rows_per_block + i / a.vecs;
-            const uint32_t c = i % a.vecs * V;
-            if (r >= a.n_rows) break;
-            const int32_t *ids = a.ids + r * a.ids_stride;
-            const T *table = static_cast<const T *>(a.table) + c;
+        const uint64_t r0 = b * a.rows_per_block;
+        for (uint32_t i0 = 0; i0 < cells; i0 += 256) {
+            const uint32_t i = i0 + threadIdx.x, in = i / a.vecs, c = i % a.vecs * V;
+            const bool live = i < cells && r0 + in < a.n_rows;
             float acc[V] = {};
-            for (uint32_t t0 = 0; t0 < a.columns; t0 += kAhead) {
-                uint64_t row[kAhead];
-                Vec<T, V> v[kAhead];
+            for (uint32_t t0 = 0; t0 < a.columns; t0 += wide) {
+                if (t0 || i0 || b != blockIdx.x) __syncthreads();
+                for (uint32_t q = threadIdx.x; q < wide; q += 256)
+                    scale[q] = t0 + q >= a.columns ? 0.0f : a.scale ? a.scale[t0 + q] : 1.0f;
+                for (uint32_t q = threadIdx.x; q < wide * a.rows_per_block; q += 256) {
+                    const uint32_t row = q / wide, t = t0 + q - row * wide;
+                    uint64_t v = a.table_rows;
+                    if (t < a.columns && r0 + row < a.n_rows)
+                        v = table_row(a.ids[(r0 + row) * a.ids_stride + t], a.offset, t, a.columns, a.table_rows);
+                    place[q] = v >= a.table_rows ? nowhere() : (uint32_t)(Far ? v : v * a.table_stride * sizeof(T));
+                }
+                __syncthreads();
+                if (!live) continue;
+                const uint32_t here = min(wide, (a.columns - t0 + kAhead - 1) / kAhead * kAhead);
+                for (uint32_t t = 0; t < here; t += kAhead) {
+                    uint32_t at[kAhead];
+                    Vec<T, V> v[kAhead];
 #pragma unroll
-                for (uint32_t j = 0; j < kAhead; j++)
-                    row[j] = t0 + j < a.columns ? table_row(ids[t0 + j], a.offset, t0 + j, a.table_rows) : a.table_rows;
+                    for (uint32_t j = 0; j < kAhead; j++) at[j] = place[in * wide + t + j];
 #pragma unroll
-                for (uint32_t j = 0; j < kAhead; j++)
-                    if (row[j] < a.table_rows)
-                        v[j] = *reinterpret_cast<const Vec<T, V> *>(table + row[j] * a.table_stride);
+                    for (uint32_t j = 0; j < kAhead; j++) {
+                        if constexpr (Far) {
+                            if (at[j] != nowhere())
+                                v[j] = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(a.table) +
+                                                                             at[j] * a.table_stride + c);
+                            else
+                                v[j] = Vec<T, V>{};
+                        } else {
+                            v[j] = buffer_vec<T, V>(table, at[j] + c * (uint32_t)sizeof(T));
+                        }
+                    }
 #pragma unroll
-                for (uint32_t j = 0; j < kAhead; j++) {
-                    if (row[j] >= a.table_rows) continue;
-                    const float s = a.scale ? a.scale[t0 + j] : 1.0f;
+                    for (uint32_t j = 0; j < kAhead; j++) {
+                        const float s = at[j] == nowhere() ? 0.0f : scale[t + j];
 #pragma unroll
-                    for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s, E::up(v[j].v[k]), acc[k]);
+                        for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s, E::up(v[j].v[k]), acc[k]);
+                    }
                 }
             }
+            if (!live) continue;
             Vec<T, V> out;
 #pragma unroll
             for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
-            *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.out) + r * a.out_stride + c) = out;
+            *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.out) + (r0 + in) * a.out_stride + c) = out;
         }
+    }
+}
+
+// ---- the gradient, a column at a time ----------------------------------------------------
+
+// A workgroup takes one column, one block of rows and one slice of the
+// vectors. Its ids are sorted in LDS, in order within a key: a wave holds
+// consecutive rows, a lane's rank among the wave's rows of its
+// key is a count of matching ballots behind the wave's count so far, and the
+// counts of (key, wave) are joined by one scan. The waves then sum even
+// shares of the sorted rows as lookup_sum does; a key that reaches over
+// shares is joined from LDS. Keys are taken kColumnKeys at a time.
+//
+// No id is written to memory, and the rows of dout that a block gathers stay
+// in the L2 of the XCD that has the block.
+constexpr uint32_t kColumnThreads = 1024, kColumnWaves = kColumnThreads / kWave;
+constexpr uint32_t kColumnSteps = kColumnBlock / kColumnThreads;
+constexpr uint32_t kColumnKeys = 512;
+
+template <typename E, int V>
+__device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
+    using T = typename E::type;
+    __shared__ uint32_t count[kColumnWaves][kColumnKeys];  // then the shares' edges
+    __shared__ uint16_t list[kColumnBlock];
+    __shared__ uint32_t start[kColumnKeys + 1];
+    float(*edge)[2][kColumnSlice] = reinterpret_cast<float(*)[2][kColumnSlice]>(&count[0][0]);
+    static_assert(sizeof(float) * 2 * kColumnSlice <= sizeof(uint32_t) * kColumnKeys, "a wave's edges fit its counts");
+    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
+    // a block's columns and slices on one XCD, one block after the other
+    const uint32_t each = a.columns * a.slices;
+    uint32_t block = blockIdx.x / each, in = blockIdx.x % each;
+    if (a.blocks % 8 == 0) {
+        in = blockIdx.x / 8;
+        block = in / each * 8 + blockIdx.x % 8;
+        in %= each;
+    }
+    const uint32_t t = in / a.slices, slice = in % a.slices;
+    const uint64_t r0 = (uint64_t)block * a.block_rows;
+    const uint32_t m = r0 < a.n_rows ? (uint32_t)min((uint64_t)a.block_rows, a.n_rows - r0) : 0;
+    // the column's table rows; the first column's begin with the table
+    int64_t lo = 0, hi = (int64_t)a.table_rows, off = 0;
+    if (a.offset) {
+        off = a.offset[t];
+        if (t) lo = max(off, (int64_t)0);
+        if (t + 1 < a.columns) hi = min(hi, (int64_t)a.offset[t + 1]);
+    }
+    const float scale = a.scale ? a.scale[t] : 1.0f;
+    // the slice's vectors on the lanes of a group
+    const uint32_t v0 = slice * a.slice_vecs, vecs = min(a.slice_vecs, a.vecs - v0);
+    uint32_t wide = 1;
+    while (wide < vecs) wide <<= 1;
+    const uint32_t groups = kWave / wide, group = lane / wide, c = lane & (wide - 1);
+    const bool live = c < vecs;
+    const T *dout = static_cast<const T *>(a.dout) + r0 * a.dout_stride + (v0 + c) * V;
+    auto write = [&](uint64_t row, const float(&acc)[V]) {
+        if (a.blocks == 1) {
+            Vec<T, V> out;
+#pragma unroll
+            for (int k = 0; k < V; k++) out.v[k] = E::down(scale * acc[k]);
+            *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + row * a.dtable_stride + (v0 + c) * V) = out;
+        } else {
+            Vec<float, V> out;
+#pragma unroll
+            for (int k = 0; k < V; k++) out.v[k] = scale * acc[k];
+            *reinterpret_cast<Vec<float, V> *>(a.part + ((uint64_t)block * a.table_rows + row) * a.part_stride + (v0 + c) * V) = out;
+        }
+    };
+    for (int64_t k0 = lo; k0 < hi; k0 += kColumnKeys) {
+        const uint32_t keys = (uint32_t)min((int64_t)kColumnKeys, hi - k0);
+        for (uint32_t i = threadIdx.x; i < kColumnWaves * kColumnKeys; i += kColumnThreads) (&count[0][0])[i] = 0;
+        __syncthreads();
+        const uint32_t wave_rows = (a.block_rows + kColumnThreads - 1) / kColumnThreads * kWave;
+        uint32_t held[kColumnSteps];  // the key, and the rank in the upper half
+        uint32_t bits = 0;
+        while ((1u << bits) < keys) bits++;
+#pragma unroll
+        for (uint32_t j = 0; j < kColumnSteps; j++) {
+            const uint32_t i = wave * wave_rows + j * kWave + lane;
+            held[j] = 0xffffffffu;
+            if (j * kWave < wave_rows && i < m) {
+                const int32_t id = a.ids[(r0 + i) * a.ids_stride + t];
+                const int64_t key = off + id - k0;
+                if (id >= 0 && key >= 0 && key < keys) held[j] = (uint32_t)key;
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kColumnSteps; j++) {
+            if (j * kWave >= wave_rows) continue;
+            const bool ok = held[j] != 0xffffffffu;
+            const uint32_t key = ok ? held[j] : 0;
+            uint64_t same = __ballot(ok);
+            for (uint32_t bit = 0; bit < bits; bit++) {
+                const uint64_t set = __ballot(ok && ((key >> bit) & 1u));
+                same &= (key >> bit) & 1u ? set : ~set;
+            }
+            const uint64_t below = same & ((1ull << lane) - 1);
+            volatile uint32_t *mine = &count[wave][key];
+            const uint32_t before = *mine;
+            __builtin_amdgcn_wave_barrier();
+            if (ok && below == 0) *mine = before + (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+            if (ok) held[j] = key | (before + (uint32_t)__popcll(below)) << 16;
+        }
+        __syncthreads();
+        uint32_t total = 0, all;
+        if (threadIdx.x < kColumnKeys)
+            for (uint32_t w = 0; w < kColumnWaves; w++) total += count[w][threadIdx.x];
+        uint32_t at = block_exclusive_scan<kColumnThreads>(total, &all);
+        if (threadIdx.x < kColumnKeys) {
+            start[threadIdx.x] = at;
+            for (uint32_t w = 0; w < kColumnWaves; w++) {
+                const uint32_t n = count[w][threadIdx.x];
+                count[w][threadIdx.x] = at;
+                at += n;
+            }
+        }
+        if (threadIdx.x == 0) start[kColumnKeys] = all;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kColumnSteps; j++)
+            if (held[j] != 0xffffffffu)
+                list[count[wave][held[j] & 0xffffu] + (held[j] >> 16)] =
+                    (uint16_t)(wave * wave_rows + j * kWave + lane);
+        __syncthreads();
+        const uint32_t a0 = (uint32_t)((uint64_t)all * wave / kColumnWaves), a1 = (uint32_t)((uint64_t)all * (wave + 1) / kColumnWaves);
+        uint32_t key = 0;
+        if (a0 < a1) {  // the key of the share's first row: the last that begins at or before it
+            uint32_t low = 0, high = keys;
+            while (high - low > 1) {
+                const uint32_t mid = (low + high) / 2;
+                if (start[mid] <= a0) low = mid;
+                else high = mid;
+            }
+            key = low;
+        }
+        uint32_t tail = kColumnKeys;  // the key that goes on past the share, if it began in it
+        for (uint32_t i = a0; i < a1; key++) {
+            const uint32_t s = start[key], end = start[key + 1], e = min(end, a1);
+            if (s == end) continue;
+            float acc[V] = {};
+            if (live) {
+                constexpr uint32_t kAhead = 4;
+                for (uint32_t j = i + group; j < e; j += kAhead * groups) {
+                    Vec<T, V> v[kAhead];
+#pragma unroll
+                    for (uint32_t u = 0; u < kAhead; u++) {
+                        const uint32_t p = j + u * groups;
+                        v[u] = Vec<T, V>{};
+                        if (p < e) v[u] = *reinterpret_cast<const Vec<T, V> *>(dout + list[p] * a.dout_stride);
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < kAhead; u++)
+#pragma unroll
+                        for (int k = 0; k < V; k++) acc[k] += E::up(v[u].v[k]);
+                }
+            }
+            for (uint32_t d = wide; d < (uint32_t)kWave; d <<= 1)
+#pragma unroll
+                for (int k = 0; k < V; k++) acc[k] += __shfl_xor(acc[k], d, kWave);
+            if (group == 0 && live) {
+                if (s >= a0 && end <= a1) {
+                    write((uint64_t)(k0 + key), acc);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; k++) edge[wave][s < a0 ? 0 : 1][c * V + k] = acc[k];
+                }
+            }
+            if (s >= a0 && end > a1) tail = key;
+            i = e;
+        }
+        __syncthreads();
+        if (tail < kColumnKeys && group == 0 && live) {
+            float acc[V];
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[k] = edge[wave][1][c * V + k];
+            for (uint32_t w = wave + 1; w < kColumnWaves; w++) {
+                const uint32_t b0 = (uint32_t)((uint64_t)all * w / kColumnWaves), b1 = (uint32_t)((uint64_t)all * (w + 1) / kColumnWaves);
+                if (b0 >= start[tail + 1]) break;
+                if (b0 == b1) continue;
+#pragma unroll
+                for (int k = 0; k < V; k++) acc[k] += edge[w][0][c * V + k];
+            }
+            write((uint64_t)(k0 + tail), acc);
+        }
+        // rows that nothing leads to
+        for (uint32_t k = threadIdx.x / wide; k < keys; k += kColumnThreads / wide) {
+            if (start[k] != start[k + 1] || !live) continue;
+            const float none[V] = {};
+            write((uint64_t)(k0 + k), none);
+        }
+        __syncthreads();
+    }
+}
+
+// The blocks' sums of each table row, in order.
+template <typename E, int V>
+__device__ __forceinline__ void lookup_join(const LookupColumnArgs &a) {
+    using T = typename E::type;
+    const uint64_t cells = a.table_rows * a.vecs;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / a.vecs;
+        const uint32_t c = (uint32_t)(i - row * a.vecs) * V;
+        const float *p = a.part + row * a.part_stride + c;
+        float acc[V] = {};
+        for (uint32_t b = 0; b < a.blocks; b++, p += a.table_rows * a.part_stride) {
+            const Vec<float, V> v = *reinterpret_cast<const Vec<float, V> *>(p);
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[k] += v.v[k];
+        }
+        Vec<T, V> out;
+#pragma unroll
+        for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
+        *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + row * a.dtable_stride + c) = out;
     }
 }
 
@@ -84,22 +346,33 @@ __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
 __device__ __forceinline__ uint32_t sort_key(const LookupSortArgs &a, uint32_t i) {
     if (a.keys_in) return a.keys_in[i];
     const uint32_t r = i / a.columns, t = i - r * a.columns;
-    return (uint32_t)table_row(a.ids[(uint64_t)r * a.ids_stride + t], a.offset, t, a.table_rows);
+    return (uint32_t)table_row(a.ids[(uint64_t)r * a.ids_stride + t], a.offset, t, a.columns, a.table_rows);
 }
 
 }  // namespace hbr
 
 using namespace hbr;
 
-#define HBR_EMBED(name, E, V) \
-    extern "C" __global__ __launch_bounds__(256) void name(EmbedArgs a) { leaf_embed<E, V>(a); }
-HBR_EMBED(hbr_leaf_embed_f32_4, F32, 4)
-HBR_EMBED(hbr_leaf_embed_f32_2, F32, 2)
-HBR_EMBED(hbr_leaf_embed_f32_1, F32, 1)
-HBR_EMBED(hbr_leaf_embed_bf16_8, Bf16, 8)
-HBR_EMBED(hbr_leaf_embed_bf16_4, Bf16, 4)
-HBR_EMBED(hbr_leaf_embed_bf16_2, Bf16, 2)
-HBR_EMBED(hbr_leaf_embed_bf16_1, Bf16, 1)
+#define HBR_EMBED(suffix, E, V)                                                                               \
+    extern "C" __global__ __launch_bounds__(256) void hbr_leaf_embed_##suffix(EmbedArgs a) {                  \
+        leaf_embed<E, V, false>(a);                                                                           \
+    }                                                                                                         \
+    extern "C" __global__ __launch_bounds__(256) void hbr_leaf_embed_far_##suffix(EmbedArgs a) {              \
+        leaf_embed<E, V, true>(a);                                                                            \
+    }                                                                                                         \
+    extern "C" __global__ __launch_bounds__(kColumnThreads) void hbr_lookup_columns_##suffix(LookupColumnArgs a) { \
+        lookup_columns<E, V>(a);                                                                              \
+    }                                                                                                         \
+    extern "C" __global__ __launch_bounds__(256) void hbr_lookup_join_##suffix(LookupColumnArgs a) {          \
+        lookup_join<E, V>(a);                                                                                 \
+    }
+HBR_EMBED(f32_4, F32, 4)
+HBR_EMBED(f32_2, F32, 2)
+HBR_EMBED(f32_1, F32, 1)
+HBR_EMBED(bf16_8, Bf16, 8)
+HBR_EMBED(bf16_4, Bf16, 4)
+HBR_EMBED(bf16_2, Bf16, 2)
+HBR_EMBED(bf16_1, Bf16, 1)
 
 // A tile's entries counted by the pass's digit (integer counts: any order).
 extern "C" __global__ __launch_bounds__(256) void hbr_sort_count(LookupSortArgs a) {

@@ -166,10 +166,12 @@ def leaf_embedding(table, ids, out, *, offset=None, scale=None, stream=None):
     """out[r] = sum over columns t of scale[t] * table[offset[t] + ids[r, t]].
 
     ``table`` [rows, dim] and ``out`` [n, dim] are float32 or bfloat16 alike,
-    ``ids`` [n, columns] int32, ``offset`` int32 (each tree's first table row;
-    None: 0) and ``scale`` float32 (None: 1) one entry a column. An id below
-    0, or one that leads out of the table, adds nothing. Sums are float32, in
-    the order of the columns."""
+    ``ids`` [n, columns] int32, ``offset`` int32 and ``scale`` float32 (None:
+    1) one entry a column. ``offset`` (each tree's first table row, ascending)
+    gives every column its own rows, up to the next column's; with None every
+    column has the whole table. An id below 0, or one that leads out of its
+    column's rows, adds nothing. Sums are float32, in the order of the
+    columns."""
     call = _Call()
     tp, (rows, dim), ts = call.array(table, "table", 2, _FLOATS)
     dtype = _dtype(table.dtype)
@@ -181,7 +183,7 @@ def leaf_embedding(table, ids, out, *, offset=None, scale=None, stream=None):
 def leaf_embedding_grad_workspace(n, columns, table_rows, dim, dtype):
     """The bytes leaf_embedding_grad needs for n x columns ids."""
     out = C.c_uint64()
-    p = A.Lookup(_CODE[_dtype(dtype)], dim, n, columns, 0, table_rows, dim, columns, dim, 16, None, None)
+    p = A.Lookup(_CODE[_dtype(dtype)], dim, n, columns, 0, table_rows, dim, columns, dim, None, None, None)
     A.check(A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(out)))
     return out.value
 

@@ -664,9 +664,11 @@ int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outp
 #define HBR_BF16 1
 
 /* A look-up of n_rows x n_columns ids in a table of table_rows vectors of
- * dim elements. Column t's id i means table row offset[t] + i (a tree's first
- * node; NULL: 0) and counts scale[t] times (a tree's weight; NULL: 1). An id
- * below 0, or one that leads out of the table, adds nothing. */
+ * dim elements. Column t's id i means table row offset[t] + i and counts
+ * scale[t] times (a tree's weight; NULL: 1). offset (each tree's first node,
+ * ascending) gives each column its own table rows, from its offset up to the
+ * next column's; with NULL every column has the whole table. An id below 0,
+ * or one that leads out of its column's rows, adds nothing. */
 typedef struct hbr_lookup {
     uint32_t dtype;           /* of the table and the vectors */
     uint32_t dim;
@@ -688,7 +690,8 @@ typedef struct hbr_lookup {
 int hbr_leaf_embedding(int ordinal, const hbr_lookup *p, const void *table, void *out, void *stream);
 /* dtable[v] = sum over every (r, t) that leads to row v of scale[t] *
  * dout[r], in f32, rounded once; rows that no id leads to are zeros. At most
- * 2^31 - 1 ids (HBR_REFUSED beyond). */
+ * 2^31 - 1 ids (HBR_REFUSED beyond). The workspace call reads the sizes
+ * alone. */
 int hbr_leaf_embedding_grad_workspace(const hbr_lookup *p, uint64_t *bytes);
 int hbr_leaf_embedding_grad(int ordinal, const hbr_lookup *p, const void *dout, void *dtable, void *workspace,
                             uint64_t workspace_bytes, void *stream);

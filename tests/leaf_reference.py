@@ -27,8 +27,11 @@ def rounded(x, dtype):
 def places(ids, offset, table_rows):
     """Each id's table row, -1 where it adds nothing."""
     ids = np.asarray(ids, np.int64)
-    row = ids if offset is None else ids + np.asarray(offset, np.int64)[None, :]
-    return np.where((ids >= 0) & (row >= 0) & (row < table_rows), row, -1)
+    if offset is None:
+        return np.where((ids >= 0) & (ids < table_rows), ids, -1)
+    row = ids + np.asarray(offset, np.int64)[None, :]
+    end = np.append(np.asarray(offset, np.int64)[1:], table_rows)[None, :]
+    return np.where((ids >= 0) & (row >= 0) & (row < np.minimum(end, table_rows)), row, -1)
 
 
 def embedding(table, ids, offset, scale, dtype):

@@ -154,23 +154,52 @@ def test_leaf_embedding_grad_sums_the_rows_that_lead_to_each_place(case):
     assert np.array_equal(back(dtable), got)
 
 
+# table rows few and many against the ids, so that either way of the gradient runs
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_columns_that_share_table_rows_add_up(dtype):
-    """Overlapping offsets, negative ones among them, and the same id twice in a row."""
+@pytest.mark.parametrize("offsets", [None, (0, 0, 5, 6, 30, 41), (3, 9, 20, 30, 40, 50), (-7, -2, 0, 600, 1000, 1500),
+                                     (0, 100, 200, 300, 400, 5000)])
+@pytest.mark.parametrize("rows", [50, 2000, 40_000])
+def test_columns_hold_the_table_rows_up_to_the_next(offsets, rows, dtype):
+    """Columns that share the table, empty ones, ones that begin before or
+    behind it, ids past a column's end, and the same id twice in a row."""
     rng = np.random.default_rng(3)
-    n, columns, rows, dim = 700, 6, 50, 12
+    n, columns, dim = 700, 6, 12
     ids = rng.integers(-3, 40, (n, columns)).astype(np.int32)
-    off = np.array([0, 0, 5, -7, 30, 0], np.int32)
+    ids[::7] = rng.integers(0, 3000, ids[::7].shape)
+    off = None if offsets is None else np.array(offsets, np.int32)
     s = rng.standard_normal(columns).astype(np.float32)
     table = R.rounded(rng.standard_normal((rows, dim)), dtype)
     out, dtable = like((n, dim), dtype), like((rows, dim), dtype)
-    d = dict(offset=dev(off, "int32"), scale=dev(s, "float32"))
+    d = dict(offset=vec(off, "int32"), scale=dev(s, "float32"))
     hb.leaf_embedding(dev(table, dtype), dev(ids, "int32"), out, **d)
     close(back(out), R.embedding(table, ids, off, s, dtype))
     dout = R.rounded(rng.standard_normal((n, dim)), dtype)
     hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable,
                            workspace=work(hb.leaf_embedding_grad_workspace(n, columns, rows, dim, dtype)), **d)
     close(back(dtable), R.embedding_grad(dout, ids, off, s, rows, dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, rows, columns, dim, few", [
+    (16_384, 512, 1, 8, 512),       # one block, one round of keys
+    (16_385, 513, 1, 24, 513),      # a row more, a key more
+    (40_000, 1200, 1, 130, 3),      # three rounds of keys; three rows hold all ids
+    (5_000, 3, 1, 300, 3),          # fewer rows than waves, several slices
+    (700, 700, 20, 65, 1),          # every id of a column alike
+    (50_001, 31, 7, 20, 31),
+])
+def test_many_ids_a_table_row(n, rows, columns, dim, few, dtype):
+    """Blocks of rows, rounds of keys, slices of the vectors, and keys that
+    reach over several waves' shares."""
+    rng = np.random.default_rng(n)
+    ids = rng.integers(0, few, (n, columns)).astype(np.int32)
+    off = (np.arange(columns) * rows).astype(np.int32) if columns > 1 else None
+    total = rows * columns
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    dtable = like((total, dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable, offset=vec(off, "int32"),
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, columns, total, dim, dtype)))
+    close(back(dtable), R.embedding_grad(dout, ids, off, None, total, dtype))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
