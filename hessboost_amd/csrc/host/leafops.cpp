@@ -169,7 +169,9 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     // row has many ids and a column few enough rows for LDS, are summed a
     // column at a time, in blocks of rows: enough for the device, of which
     // each reads at least as many vectors as it writes sums.
-    q.columns = q.n && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows && p.table_rows / p.n_columns <= 2048;
+    // (A block's rows lie within 2 GiB of dout and of the ids.)
+    q.columns = q.n && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows &&
+                p.table_rows / p.n_columns <= 2048 && std::max(p.out_stride, p.ids_stride) < 32768;
     if (q.columns) {
         const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
         const uint64_t most = std::max<uint64_t>(1, q.n / (8 * p.table_rows));

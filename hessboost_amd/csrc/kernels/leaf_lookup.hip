@@ -149,9 +149,9 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
     __shared__ uint32_t count[kColumnWaves][kColumnKeys];  // then the shares' edges
     __shared__ uint16_t list[kColumnBlock];
     __shared__ uint32_t start[kColumnKeys + 1];
+    __shared__ uint32_t wave_total[kColumnWaves];
     float(*edge)[2][kColumnSlice] = reinterpret_cast<float(*)[2][kColumnSlice]>(&count[0][0]);
     static_assert(sizeof(float) * 2 * kColumnSlice <= sizeof(uint32_t) * kColumnKeys, "a wave's edges fit its counts");
-    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
     // a block's columns and slices on one XCD, one block after the other
     const uint32_t each = a.columns * a.slices;
     uint32_t block = blockIdx.x / each, in = blockIdx.x % each;
@@ -175,9 +175,15 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
     const uint32_t v0 = slice * a.slice_vecs, vecs = min(a.slice_vecs, a.vecs - v0);
     uint32_t wide = 1;
     while (wide < vecs) wide <<= 1;
-    const uint32_t groups = kWave / wide, group = lane / wide, c = lane & (wide - 1);
+    const uint32_t groups = kWave / wide, group = lane_id() / wide, c = lane_id() & (wide - 1);
     const bool live = c < vecs;
-    const T *dout = static_cast<const T *>(a.dout) + r0 * a.dout_stride + (v0 + c) * V;
+    // a block's rows lie within 2 GiB
+    __amdgpu_buffer_rsrc_t dout = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T *>(static_cast<const T *>(a.dout) + r0 * a.dout_stride), 0, 0x7fffffff, 0x00020000);
+    __amdgpu_buffer_rsrc_t ids = __builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t *>(a.ids + r0 * a.ids_stride + t), 0,
+                                                                   0x7fffffff, 0x00020000);
+    const uint32_t dout_stride = (uint32_t)(a.dout_stride * sizeof(T)), ids_stride = (uint32_t)(a.ids_stride * 4);
+    const uint32_t dout_at = (v0 + c) * (uint32_t)(V * sizeof(T));
     auto write = [&](uint64_t row, const float(&acc)[V]) {
         if (a.blocks == 1) {
             Vec<T, V> out;
@@ -192,8 +198,14 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
         }
     };
     for (int64_t k0 = lo; k0 < hi; k0 += kColumnKeys) {
+        // made anew each round: what a compiler would keep of them over the
+        // rounds does not fit the registers
+        uint32_t thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        const uint32_t lane = thread % kWave, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(thread / kWave));
         const uint32_t keys = (uint32_t)min((int64_t)kColumnKeys, hi - k0);
-        for (uint32_t i = threadIdx.x; i < kColumnWaves * kColumnKeys; i += kColumnThreads) (&count[0][0])[i] = 0;
+#pragma unroll 1
+        for (uint32_t i = thread; i < kColumnWaves * kColumnKeys; i += kColumnThreads) (&count[0][0])[i] = 0;
         __syncthreads();
         const uint32_t wave_rows = (a.block_rows + kColumnThreads - 1) / kColumnThreads * kWave;
         uint32_t held[kColumnSteps];  // the key, and the rank in the upper half
@@ -203,11 +215,12 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
         for (uint32_t j = 0; j < kColumnSteps; j++) {
             const uint32_t i = wave * wave_rows + j * kWave + lane;
             held[j] = 0xffffffffu;
-            if (j * kWave < wave_rows && i < m) {
-                const int32_t id = a.ids[(r0 + i) * a.ids_stride + t];
-                const int64_t key = off + id - k0;
-                if (id >= 0 && key >= 0 && key < keys) held[j] = (uint32_t)key;
-            }
+            if (j * kWave < wave_rows && i < m) held[j] = __builtin_amdgcn_raw_buffer_load_b32(ids, i * ids_stride, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kColumnSteps; j++) {
+            const int64_t key = off + (int32_t)held[j] - k0;
+            held[j] = (int32_t)held[j] >= 0 && key >= 0 && key < keys ? (uint32_t)key : 0xffffffffu;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kColumnSteps; j++) {
@@ -215,6 +228,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
             const bool ok = held[j] != 0xffffffffu;
             const uint32_t key = ok ? held[j] : 0;
             uint64_t same = __ballot(ok);
+#pragma unroll 1
             for (uint32_t bit = 0; bit < bits; bit++) {
                 const uint64_t set = __ballot(ok && ((key >> bit) & 1u));
                 same &= (key >> bit) & 1u ? set : ~set;
@@ -228,19 +242,35 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
             if (ok) held[j] = key | (before + (uint32_t)__popcll(below)) << 16;
         }
         __syncthreads();
-        uint32_t total = 0, all;
-        if (threadIdx.x < kColumnKeys)
-            for (uint32_t w = 0; w < kColumnWaves; w++) total += count[w][threadIdx.x];
-        uint32_t at = block_exclusive_scan<kColumnThreads>(total, &all);
-        if (threadIdx.x < kColumnKeys) {
-            start[threadIdx.x] = at;
+        // each key's total over the waves, their scan, and the waves' places
+        uint32_t total = 0;
+        if (thread < kColumnKeys)
+#pragma unroll 4
+            for (uint32_t w = 0; w < kColumnWaves; w++) total += count[w][thread];
+        uint32_t upto = total;
+#pragma unroll 1
+        for (uint32_t d = 1; d < (uint32_t)kWave; d <<= 1) {
+            const uint32_t other = __shfl_up(upto, d, kWave);
+            if (lane >= d) upto += other;
+        }
+        if (lane == kWave - 1) wave_total[wave] = upto;
+        __syncthreads();
+        uint32_t at = upto - total, all = 0;
+#pragma unroll 1
+        for (uint32_t w = 0; w < kColumnWaves; w++) {
+            if (w == wave) at += all;
+            all += wave_total[w];
+        }
+        if (thread < kColumnKeys) {
+            start[thread] = at;
+#pragma unroll 1
             for (uint32_t w = 0; w < kColumnWaves; w++) {
-                const uint32_t n = count[w][threadIdx.x];
-                count[w][threadIdx.x] = at;
+                const uint32_t n = count[w][thread];
+                count[w][thread] = at;
                 at += n;
             }
         }
-        if (threadIdx.x == 0) start[kColumnKeys] = all;
+        if (thread == 0) start[kColumnKeys] = all;
         __syncthreads();
 #pragma unroll
         for (uint32_t j = 0; j < kColumnSteps; j++)
@@ -271,8 +301,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
 #pragma unroll
                     for (uint32_t u = 0; u < kAhead; u++) {
                         const uint32_t p = j + u * groups;
-                        v[u] = Vec<T, V>{};
-                        if (p < e) v[u] = *reinterpret_cast<const Vec<T, V> *>(dout + list[p] * a.dout_stride);
+                        v[u] = buffer_vec<T, V>(dout, p < e ? list[p] * dout_stride + dout_at : nowhere());
                     }
 #pragma unroll
                     for (uint32_t u = 0; u < kAhead; u++)
@@ -299,6 +328,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
             float acc[V];
 #pragma unroll
             for (int k = 0; k < V; k++) acc[k] = edge[wave][1][c * V + k];
+#pragma unroll 1
             for (uint32_t w = wave + 1; w < kColumnWaves; w++) {
                 const uint32_t b0 = (uint32_t)((uint64_t)all * w / kColumnWaves), b1 = (uint32_t)((uint64_t)all * (w + 1) / kColumnWaves);
                 if (b0 >= start[tail + 1]) break;
@@ -309,7 +339,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
             write((uint64_t)(k0 + tail), acc);
         }
         // rows that nothing leads to
-        for (uint32_t k = threadIdx.x / wide; k < keys; k += kColumnThreads / wide) {
+        for (uint32_t k = thread / wide; k < keys; k += kColumnThreads / wide) {
             if (start[k] != start[k + 1] || !live) continue;
             const float none[V] = {};
             write((uint64_t)(k0 + k), none);
@@ -360,7 +390,7 @@ using namespace hbr;
     extern "C" __global__ __launch_bounds__(256) void hbr_leaf_embed_far_##suffix(EmbedArgs a) {              \
         leaf_embed<E, V, true>(a);                                                                            \
     }                                                                                                         \
-    extern "C" __global__ __launch_bounds__(kColumnThreads) void hbr_lookup_columns_##suffix(LookupColumnArgs a) { \
+    extern "C" __global__ __launch_bounds__(kColumnThreads, 8) void hbr_lookup_columns_##suffix(LookupColumnArgs a) { \
         lookup_columns<E, V>(a);                                                                              \
     }                                                                                                         \
     extern "C" __global__ __launch_bounds__(256) void hbr_lookup_join_##suffix(LookupColumnArgs a) {          \
