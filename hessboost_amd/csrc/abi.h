@@ -1185,6 +1185,31 @@ struct HeadArgs {
     uint32_t pad2;
 };
 
+// The head over at most kFewClasses classes (hbr_few_*).
+constexpr uint32_t kFewClasses = 64;
+struct FewArgs {
+    const void *h, *w;
+    uint64_t h_stride, w_stride;
+    uint64_t rows;
+    uint32_t classes, dim;
+    const float *bias;
+    const int32_t *labels;
+    const float *weight;
+    float *loss, *lse;      // or null
+    int32_t *best;          // or null
+    float grad_scale;
+    uint32_t chunks;        // the products' shares of the rows
+    void *g;                // [rows][g_stride], or null: no gradient
+    uint64_t g_stride;      // a multiple of 16
+    uint32_t *keep;         // per 32 rows: which have a label
+    float *part_db;         // [wave][classes]
+    float *part_dw;         // [chunk][classes][dim]
+    void *dh;               // or null
+    uint64_t dh_stride;
+    uint32_t col_tiles;     // of 32 elements of dim
+    uint32_t dw;            // whether dw is wanted
+};
+
 // src as bf16 parts with rows of dst_stride elements (zeros past cols).
 struct HeadPartsArgs {
     const void *src;
@@ -1223,7 +1248,7 @@ struct HeadSumArgs {
     uint64_t rows, cols, dst_stride;
     uint64_t part_stride;
     uint32_t parts;
-    uint32_t pad;
+    uint32_t shares;  // of the parts, a wave each: 1, 4 or 16
 };
 
 // hbr_clip_*: up to kClipTensors tensors a launch.

@@ -318,6 +318,9 @@ uint32_t head_splits(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
 }
 
 struct HeadPlan {
+    bool few;  // few classes: rows, chunks and the pairs of their own kernels
+    uint32_t score_blocks, chunks;
+    uint64_t g_stride;
     uint64_t parts, segments, dim8;
     bool copy_h, copy_w;
     uint64_t piece, pieces;
@@ -348,6 +351,22 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.dim8 = up(dim, 8);
     const uint64_t class_tiles = tiles(classes, kHeadM);
     Arena w(workspace);
+    q.few = classes <= kFewClasses;
+    if (q.few) {
+        // up to sixteen waves on each of 256 CUs
+        const uint64_t groups = tiles(n, 32), cols = tiles(dim, 32);
+        q.score_blocks = (uint32_t)std::min<uint64_t>(tiles(groups, 4), 1024);
+        q.chunks = (uint32_t)std::max<uint64_t>(1, std::min(groups, tiles(4096, cols)));
+        q.g_stride = up(classes, 16);
+        if (gradient) {
+            q.g = w.take<uint16_t>(n * q.g_stride * (dtype == HBR_F32 ? 2 : 1));
+            q.keep = w.take<uint32_t>(groups);
+            q.part_db = w.take<float>(q.score_blocks * 4ull * classes);
+            q.dw = w.take<float>(q.chunks * classes * dim);
+        }
+        q.bytes = w.used;
+        return q;
+    }
     q.part_max = w.take<float>(class_tiles * n);
     q.part_sum = w.take<float>(class_tiles * n);
     q.part_best = w.take<int32_t>(class_tiles * n);
@@ -414,12 +433,51 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         a.rows = rows;
         a.cols = cols;
         a.dst_stride = dst_stride;
-        queue.launch(kernel, cells(rows * cols), threads, a);
+        // few cells of many parts: a workgroup's waves share the parts
+        a.shares = parts >= 64 ? 16 : parts >= 8 ? 4 : 1;
+        const uint32_t waves = a.shares == 16 ? 16 : 4;
+        const uint64_t each = waves / a.shares * 64;
+        queue.launch(kernel, dim3((uint32_t)std::min<uint64_t>(tiles(rows * cols, each), 1u << 16)), dim3(waves * 64), a);
     };
     const std::string sum_kernel = "hbr_head_sum_" + suffix;
     if (n == 0) {  // sums over no rows
         if (p.dw) sum(sum_kernel.c_str(), nullptr, 0, 0, p.dw, classes, dim, p.dw_stride);
         if (p.db) sum("hbr_head_sum_f32", nullptr, 0, 0, p.db, 1, classes, classes);
+        return;
+    }
+    if (q.few) {
+        FewArgs f{};
+        f.h = p.h;
+        f.w = p.w;
+        f.h_stride = p.h_stride;
+        f.w_stride = p.w_stride;
+        f.rows = n;
+        f.classes = (uint32_t)classes;
+        f.dim = (uint32_t)dim;
+        f.bias = p.bias;
+        f.labels = p.labels;
+        f.weight = p.weight;
+        f.loss = p.loss;
+        f.lse = p.lse;
+        f.best = p.best;
+        f.grad_scale = p.grad_scale;
+        f.chunks = q.chunks;
+        f.g = q.g;
+        f.g_stride = q.g_stride;
+        f.keep = q.keep;
+        f.part_db = q.part_db;
+        f.part_dw = q.dw;
+        f.dh = p.dh;
+        f.dh_stride = p.dh_stride;
+        f.col_tiles = (uint32_t)tiles(dim, 32);
+        f.dw = p.dw != nullptr;
+        const std::string few = suffix + (classes > 32 ? "_2" : "_1");
+        queue.launch(("hbr_few_scores_" + few).c_str(), dim3(q.score_blocks), threads, f);
+        if (!gradient) return;
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, q.score_blocks * 4ull, classes, p.db, 1, classes, classes);
+        if (!p.dh && !p.dw) return;
+        queue.launch(("hbr_few_products_" + few).c_str(), dim3((uint32_t)tiles((uint64_t)q.chunks * f.col_tiles, 4)), threads, f);
+        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.chunks, classes * dim, p.dw, classes, dim, p.dw_stride);
         return;
     }
     // the operands of the products: h, and w from class k on

@@ -8,6 +8,7 @@
 #include "predict.hip"
 #include "leaf_lookup.hip"
 #include "softmax_head.hip"
+#include "softmax_few.hip"
 #include "clip.hip"
 
 // The abi.h checksum this code object was built with (checked by the host

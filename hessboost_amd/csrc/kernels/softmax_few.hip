@@ -1,0 +1,238 @@
+// The softmax head over few classes (kFewClasses at most): a row's scores fit
+// the lanes' registers, so one pass over the rows gives loss and pairs, and a
+// second the products with them. Both passes are bound by the rows' traffic:
+// h is read twice and dh written once, w and the pairs are small. No LDS: a
+// fragment is what its lanes load, 16 bytes of a row each or an element of a
+// column each, and the L1 serves what waves of a workgroup share.
+//
+// f32 is multiplied as f32 (v_mfma_f32_32x32x2_f32), whose rate the traffic
+// does not reach.
+#include "common.h"
+
+namespace hbr {
+
+// The products' operands by type: a fragment of kStep products holds kEach of
+// them a lane, those from kEach (lane / 32) on.
+struct FewF32 {
+    using E = F32;
+    static constexpr int kStep = 8, kEach = 4;
+    using Frag = Vec<float, 4>;
+    static __device__ __forceinline__ f32x16 mul(const Frag &a, const Frag &b, f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
+        return c;
+    }
+};
+struct FewBf16 {
+    using E = Bf16;
+    static constexpr int kStep = 16, kEach = 8;
+    using Frag = Vec<uint16_t, 8>;
+    static __device__ __forceinline__ f32x16 mul(const Frag &a, const Frag &b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+
+// kEach elements of a row from k on, zeros past the row's dim. Vectors need
+// no more than their elements' alignment.
+template <typename F>
+__device__ __forceinline__ typename F::Frag few_row(const typename F::E::type *row, uint32_t k, uint32_t dim) {
+    typename F::Frag f{};
+    if (k + F::kEach <= dim) {
+        __builtin_memcpy(&f, row + k, sizeof f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < F::kEach; i++)
+            if (k + i < dim) f.v[i] = row[k + i];
+    }
+    return f;
+}
+
+// A wave takes 32 rows at a time; a lane holds its row's classes 32 kt +
+// row_of(e), the lane of the other half of the wave the row's others.
+template <typename F, int KT>
+__device__ __forceinline__ void few_scores(const FewArgs &a) {
+    using T = typename F::E::type;
+    __shared__ __align__(16) float bias[32 * KT];
+    if (threadIdx.x < 32 * KT)
+        bias[threadIdx.x] = threadIdx.x >= a.classes ? -INFINITY : a.bias ? a.bias[threadIdx.x] * kLog2e : 0.0f;
+    __syncthreads();
+    const uint32_t lane = lane_id(), wave = blockIdx.x * 4 + threadIdx.x / kWave, waves = gridDim.x * 4;
+    const uint32_t groups = (uint32_t)((a.rows + 31) / 32);
+    const T *w[KT];
+#pragma unroll
+    for (int t = 0; t < KT; t++) w[t] = static_cast<const T *>(a.w) + min(32 * t + lane % 32, a.classes - 1) * a.w_stride;
+    float db[KT][16] = {};
+    for (uint32_t g = wave; g < groups; g += waves) {
+        const uint64_t r = (uint64_t)g * 32 + lane % 32;
+        const bool in = r < a.rows;
+        const T *h = static_cast<const T *>(a.h) + min(r, a.rows - 1) * a.h_stride;
+        f32x16 acc[KT];
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+#pragma unroll 4
+        for (uint32_t k0 = 0; k0 < a.dim; k0 += F::kStep) {
+            const uint32_t k = k0 + lane / 32 * F::kEach;
+            const typename F::Frag fh = few_row<F>(h, k, a.dim);
+#pragma unroll
+            for (int t = 0; t < KT; t++) acc[t] = F::mul(few_row<F>(w[t], k, a.dim), fh, acc[t]);
+        }
+        const int32_t y = a.labels && in ? a.labels[r] : -1;
+        float top = -INFINITY, at_label = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const uint32_t c = 32 * t + row_of(e);
+                const float z = c < a.classes ? __builtin_fmaf(acc[t][e], kLog2e, bias[c]) : -INFINITY;
+                acc[t][e] = z;
+                top = fmaxf(top, z);
+                if (y == (int32_t)c) at_label = z;
+            }
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float shift = shift_of(top);
+        float sum = 0.0f;
+        int32_t best = 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                sum += __builtin_amdgcn_exp2f(acc[t][e] - shift);
+                if (acc[t][e] == top) best = min(best, (int32_t)(32 * t + row_of(e)));
+            }
+        sum += __shfl_xor(sum, 32, kWave);
+        at_label += __shfl_xor(at_label, 32, kWave);
+        best = min(best, __shfl_xor(best, 32, kWave));
+        // a label that is no class: neither a loss nor a gradient
+        const bool no_class = y >= 0 && (uint32_t)y >= a.classes;
+        const float lse2 = no_class ? NAN : shift + __builtin_amdgcn_logf(sum);
+        const float weight = in && a.weight ? a.weight[r] : 1.0f;
+        if (in && lane < 32) {
+            if (a.lse) a.lse[r] = lse2 * kLn2;
+            if (a.best) a.best[r] = best < (int32_t)a.classes ? best : 0;
+            if (a.loss)
+                a.loss[r] = !a.labels ? (lse2 - top) * kLn2 : y < 0 ? 0.0f : no_class ? NAN : weight * ((lse2 - at_label) * kLn2);
+        }
+        if (!a.g) continue;
+        const uint64_t kept = __ballot(y >= 0);
+        if (lane == 0) a.keep[g] = (uint32_t)kept;
+        const float by = a.grad_scale * weight;
+        T *out = static_cast<T *>(a.g) + r * a.g_stride;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                Vec<T, 4> v;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = 4 * q + i;
+                    float p = __builtin_amdgcn_exp2f(acc[t][e] - lse2);
+                    if (y == (int32_t)(32 * t + row_of(e))) p -= 1.0f;
+                    p = y < 0 ? 0.0f : p * by;
+                    db[t][e] += p;
+                    v.v[i] = F::E::down(p);
+                }
+                const uint32_t c = 32 * t + 8 * q + 4 * (lane / 32);
+                if (in && c < a.g_stride) *reinterpret_cast<Vec<T, 4> *>(out + c) = v;
+            }
+    }
+    if (!a.g) return;
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            float s = db[t][e];
+            for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor(s, d, kWave);
+            const uint32_t c = 32 * t + row_of(e);
+            if (lane % 32 == 0 && c < a.classes) a.part_db[(uint64_t)wave * a.classes + c] = s;
+        }
+}
+
+// A wave takes 32 columns of h and every chunks-th group of 32 rows: dh = g w
+// with its part of w in registers throughout, dw = g^T h summed in registers
+// over its rows.
+template <typename F, int KT>
+__device__ __forceinline__ void few_products(const FewArgs &a) {
+    using T = typename F::E::type;
+    using Frag = typename F::Frag;
+    constexpr int kSteps = 32 * KT / F::kStep, kRowSteps = 32 / F::kStep;
+    const uint32_t lane = lane_id(), wave = blockIdx.x * 4 + threadIdx.x / kWave, half = lane / 32;
+    const uint32_t chunk = wave / a.col_tiles, d = wave % a.col_tiles * 32 + lane % 32;
+    if (chunk >= a.chunks) return;
+    const uint32_t groups = (uint32_t)((a.rows + 31) / 32), dd = min(d, a.dim - 1);
+    Frag w[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; s++)
+#pragma unroll
+        for (int i = 0; i < F::kEach; i++) {
+            const uint32_t k = s * F::kStep + half * F::kEach + i;
+            w[s].v[i] = k < a.classes ? static_cast<const T *>(a.w)[k * a.w_stride + dd] : (T)0;
+        }
+    f32x16 dw[KT];
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) dw[t][e] = 0.0f;
+    for (uint32_t g = chunk; g < groups; g += a.chunks) {
+        const uint64_t r0 = (uint64_t)g * 32;
+        const uint32_t m = (uint32_t)min((uint64_t)32, a.rows - r0);
+        const T *pairs = static_cast<const T *>(a.g) + r0 * a.g_stride;
+        if (a.dw) {
+            const uint32_t kept = a.keep[g];
+            const T *h = static_cast<const T *>(a.h) + r0 * a.h_stride + dd;
+#pragma unroll
+            for (int s = 0; s < kRowSteps; s++) {
+                Frag fh, fg[KT];
+#pragma unroll
+                for (int i = 0; i < F::kEach; i++) {
+                    const uint32_t r = s * F::kStep + half * F::kEach + i;
+                    const bool in = (kept >> r) & 1u;  // a row past the last is not kept
+                    fh.v[i] = in ? h[r * a.h_stride] : (T)0;
+#pragma unroll
+                    for (int t = 0; t < KT; t++) {
+                        const uint32_t c = 32 * t + lane % 32;
+                        fg[t].v[i] = in && c < a.g_stride ? pairs[r * a.g_stride + c] : (T)0;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < KT; t++) dw[t] = F::mul(fg[t], fh, dw[t]);
+            }
+        }
+        if (a.dh) {
+            f32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+            const T *row = pairs + min(lane % 32, m - 1) * a.g_stride;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+                if ((uint32_t)(s * F::kStep) < a.g_stride) acc = F::mul(few_row<F>(row, s * F::kStep + half * F::kEach, a.g_stride), w[s], acc);
+            T *out = static_cast<T *>(a.dh) + r0 * a.dh_stride + d;
+            if (d < a.dim) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (row_of(e) < m) out[row_of(e) * a.dh_stride] = F::E::down(acc[e]);
+            }
+        }
+    }
+    if (!a.dw || d >= a.dim) return;
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const uint32_t c = 32 * t + row_of(e);
+            if (c < a.classes) a.part_dw[((uint64_t)chunk * a.classes + c) * a.dim + d] = dw[t][e];
+        }
+}
+
+}  // namespace hbr
+
+using namespace hbr;
+
+#define HBR_FEW(suffix, F, KT)                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void hbr_few_scores_##suffix(FewArgs a) { few_scores<F, KT>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void hbr_few_products_##suffix(FewArgs a) { few_products<F, KT>(a); }
+HBR_FEW(f32_1, FewF32, 1)
+HBR_FEW(f32_2, FewF32, 2)
+HBR_FEW(bf16_1, FewBf16, 1)
+HBR_FEW(bf16_2, FewBf16, 2)

@@ -434,12 +434,31 @@ __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
     }
 }
 
+// A workgroup sums 64 cells a wave; with several shares its waves take shares
+// of the same cells' parts, joined in order.
 template <typename E>
 __device__ __forceinline__ void head_sum(const HeadSumArgs &a) {
+    __shared__ float sum_of[16][kWave];
     const uint64_t cells = a.rows * a.cols;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
+    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const uint32_t share = wave % a.shares, each = waves / a.shares;
+    const uint32_t p0 = (uint32_t)((uint64_t)a.parts * share / a.shares), p1 = (uint32_t)((uint64_t)a.parts * (share + 1) / a.shares);
+    for (uint64_t at = (uint64_t)blockIdx.x * each * kWave; at < cells; at += (uint64_t)gridDim.x * each * kWave) {
+        const uint64_t i = at + wave / a.shares * kWave + lane;
         float s = 0.0f;
-        for (uint32_t p = 0; p < a.parts; p++) s += a.part[p * a.part_stride + i];
+        if (i < cells) {
+            const float *part = a.part + i;
+#pragma unroll 8
+            for (uint32_t p = p0; p < p1; p++) s += part[p * a.part_stride];
+        }
+        if (a.shares > 1) {
+            __syncthreads();
+            sum_of[wave][lane] = s;
+            __syncthreads();
+            if (share) continue;
+            for (uint32_t w = 1; w < a.shares; w++) s += sum_of[wave + w][lane];
+        }
+        if (i >= cells) continue;
         const uint64_t r = i / a.cols;
         static_cast<typename E::type *>(a.dst)[r * a.dst_stride + (i - r * a.cols)] = E::down(s);
     }
@@ -491,8 +510,8 @@ HBR_HEAD(hbr_head_dh_bf16, head_sums<Bf16 HBR_COMMA false>)
 HBR_HEAD(hbr_head_dw_part, head_sums<F32 HBR_COMMA true>)
 HBR_HEAD(hbr_head_dw_bf16, head_sums<Bf16 HBR_COMMA true>)
 
-extern "C" __global__ __launch_bounds__(256) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
-extern "C" __global__ __launch_bounds__(256) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
+extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
+extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_f32(HeadPartsArgs a) { head_parts<F32, 3>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_bf16(HeadPartsArgs a) { head_parts<Bf16, 1>(a); }
 
