@@ -1146,13 +1146,15 @@ struct LookupSumArgs {
 };
 
 // The head's products C[m][n] = sum_k A(m, k) B(n, k) of bf16 operands, in
-// tiles of kHeadM x kHeadN, kHeadK products a step. An operand lies [m][k]
+// tiles of kBigM x kBigN or kMidM x kMidN, kHeadK products a step. An operand lies [m][k]
 // (k contiguous) or, transposed, [k][m]; f32 operands lie in three bf16 parts
 // whose sum they are, and a product of two is summed over the six pairs of
 // parts that reach f32's precision, one segment of steps each.
-constexpr uint32_t kHeadM = 256;
-constexpr uint32_t kHeadN = 128;
-constexpr uint32_t kHeadK = 32;
+constexpr uint32_t kBigM = 256;
+constexpr uint32_t kBigN = 256;
+constexpr uint32_t kMidM = 128;
+constexpr uint32_t kMidN = 128;
+constexpr uint32_t kHeadK = 64;
 struct HeadArgs {
     const void *a, *b;
     uint64_t a_stride, b_stride;  // elements
@@ -1162,7 +1164,7 @@ struct HeadArgs {
     uint32_t splits;              // shares of the steps, each a workgroup's
     uint32_t segments;            // 1, or 6
     uint32_t rows;
-    const uint32_t *keep;         // bit r: row r of the reduction is read (or null: all)
+    const uint64_t *keep;         // bit r: row r of the reduction is read (or null: all)
     // scores (m: classes, n: rows) and pairs (m: rows, n: classes)
     const float *bias;            // of the first class
     const int32_t *labels;
@@ -1220,7 +1222,7 @@ struct HeadPartsArgs {
 
 struct HeadKeepArgs {
     const int32_t *labels;
-    uint32_t *keep;
+    uint64_t *keep;
     uint64_t rows;
 };
 

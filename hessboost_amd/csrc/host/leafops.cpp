@@ -305,16 +305,35 @@ namespace {
 // The scores' gradients of one piece of the classes are held at a time, in at
 // most about this many bytes.
 constexpr uint64_t kPieceBytes = 1ull << 30;
-// Workgroups that run at once: two on each of 256 CUs.
-constexpr uint64_t kHeadSlots = 512;
+// A product's tiles, and the workgroups of them that run at once.
+struct HeadTiling {
+    uint64_t m, n, threads, slots;
+    const char *name;
+};
+constexpr HeadTiling kBig{kBigM, kBigN, 512, 256, "_big"}, kMid{kMidM, kMidN, 256, 512, "_mid"};
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
 // Shares of a product's steps: where its tiles are fewer than the device
-// runs at once, enough of them to fill it, of 16 steps at least.
-uint32_t head_splits(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t t = tiles(m, kHeadM) * tiles(n, kHeadN), steps = tiles(k, kHeadK) * segments;
-    return (uint32_t)std::max<uint64_t>(1, std::min(kHeadSlots / std::max<uint64_t>(t, 1), steps / 16));
+// runs at once, enough of them to fill it, of 8 steps at least.
+uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t all = tiles(m, t.m) * tiles(n, t.n), steps = tiles(k, kHeadK) * segments;
+    return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 8));
+}
+
+// The tiles that take fewer rounds of the device, a round of the middle ones
+// at 0.58 of the big ones' time: a quarter of the area each, twice as many
+// at once, and 0.86 of the rate (512 x 128 x 128 x 16,384 bf16 against
+// 256 x 256 x 256 x 16,384: 1,085 and 1,190 TFLOP/s at their best). Whole
+// products show both sides: 16,384 x 16,384 x 1,024 scores 269 us with big
+// tiles and 305 with middle ones, 4,096 x 5,003 x 256 ones of f32 90 and 74.
+const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments, bool split) {
+    const uint64_t steps = tiles(k, kHeadK) * segments;
+    auto cost = [&](const HeadTiling &t, double round) {
+        const uint64_t shares = split ? head_splits(t, m, n, k, segments) : 1;
+        return (double)(tiles(tiles(m, t.m) * tiles(n, t.n) * shares, t.slots) * tiles(steps, shares)) * round;
+    };
+    return cost(kBig, 1.0) <= cost(kMid, 0.58) ? kBig : kMid;
 }
 
 struct HeadPlan {
@@ -324,12 +343,14 @@ struct HeadPlan {
     uint64_t parts, segments, dim8;
     bool copy_h, copy_w;
     uint64_t piece, pieces;
+    const HeadTiling *scores, *pairs, *by_h, *by_w;  // the tiles of each product
     uint32_t splits_h, splits_w;
     bool sum_h;  // dh is summed from f32 parts
     float *part_max, *part_sum, *label_margin, *lse2, *part_db, *dh, *dw;
     int32_t *part_best;
     uint16_t *h, *w, *g;
-    uint32_t *keep;
+    uint64_t *keep;
+    uint32_t *few_keep;
     uint64_t bytes;
 };
 
@@ -349,7 +370,8 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
     q.dim8 = up(dim, 8);
-    const uint64_t class_tiles = tiles(classes, kHeadM);
+    q.scores = &head_tiling(classes, n, dim, q.segments, false);
+    const uint64_t class_tiles = tiles(classes, q.scores->m);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
@@ -360,7 +382,7 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
         q.g_stride = up(classes, 16);
         if (gradient) {
             q.g = w.take<uint16_t>(n * q.g_stride * (dtype == HBR_F32 ? 2 : 1));
-            q.keep = w.take<uint32_t>(groups);
+            q.few_keep = w.take<uint32_t>(groups);
             q.part_db = w.take<float>(q.score_blocks * 4ull * classes);
             q.dw = w.take<float>(q.chunks * classes * dim);
         }
@@ -375,22 +397,22 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.h = w.take<uint16_t>(q.parts * n * q.dim8);
     q.w = w.take<uint16_t>(q.parts * classes * q.dim8);
     if (gradient) {
-        // the pieces as even as whole tiles allow, each of enough tiles of
-        // dw to fill the device where that many classes fit
+        // the pieces as even as whole tiles allow
         const uint64_t row_bytes = std::max<uint64_t>(n, 1) * 2 * q.parts;
-        const uint64_t fits = std::max<uint64_t>(kHeadM, kPieceBytes / row_bytes / kHeadM * kHeadM);
-        const uint64_t fills = tiles(kHeadSlots, tiles(dim, kHeadN)) * kHeadM;
-        q.pieces = tiles(classes, std::min(fits, std::max<uint64_t>(fills, kHeadM)));
-        q.piece = up(tiles(classes, q.pieces), kHeadM);
+        q.pieces = tiles(classes, std::max<uint64_t>(kBigM, kPieceBytes / row_bytes / kBigM * kBigM));
+        q.piece = up(tiles(classes, q.pieces), kMidM);
         q.pieces = tiles(classes, q.piece);
-        q.splits_h = head_splits(n, dim, q.piece, q.segments);
-        q.splits_w = head_splits(q.piece, dim, n, q.segments);
+        q.pairs = &head_tiling(n, q.piece, dim, q.segments, false);
+        q.by_h = &head_tiling(n, dim, q.piece, q.segments, true);
+        q.by_w = &head_tiling(q.piece, dim, n, q.segments, true);
+        q.splits_h = head_splits(*q.by_h, n, dim, q.piece, q.segments);
+        q.splits_w = head_splits(*q.by_w, q.piece, dim, n, q.segments);
         q.sum_h = q.splits_h > 1 || q.pieces > 1;
         q.g = w.take<uint16_t>(q.parts * n * q.piece);
-        q.part_db = w.take<float>(tiles(n, kHeadM) * q.piece);
+        q.part_db = w.take<float>(tiles(n, q.pairs->m) * q.piece);
         if (q.sum_h) q.dh = w.take<float>(q.splits_h * n * dim);
         if (q.splits_w > 1) q.dw = w.take<float>(q.splits_w * q.piece * dim);
-        q.keep = w.take<uint32_t>(tiles(n, 64) * 2);
+        q.keep = w.take<uint64_t>(tiles(n, 64));
     }
     q.bytes = w.used;
     return q;
@@ -464,7 +486,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         f.chunks = q.chunks;
         f.g = q.g;
         f.g_stride = q.g_stride;
-        f.keep = q.keep;
+        f.keep = q.few_keep;
         f.part_db = q.part_db;
         f.part_dw = q.dw;
         f.dh = p.dh;
@@ -505,11 +527,11 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         w_stride = q.dim8;
     }
     const uint64_t h_part = n * q.dim8, w_part = classes * q.dim8;
-    auto product = [&](const char *kernel, HeadArgs a) {
-        a.m_tiles = (uint32_t)tiles(a.m, kHeadM);
-        a.n_tiles = (uint32_t)tiles(a.n, kHeadN);
+    auto product = [&](const std::string &kernel, const HeadTiling &t, HeadArgs a) {
+        a.m_tiles = (uint32_t)tiles(a.m, t.m);
+        a.n_tiles = (uint32_t)tiles(a.n, t.n);
         a.segments = (uint32_t)q.segments;
-        queue.launch(kernel, dim3(a.m_tiles * a.n_tiles * a.splits), threads, a);
+        queue.launch((kernel + t.name).c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), dim3((uint32_t)t.threads), a);
     };
     HeadArgs z{};
     z.a = w;
@@ -528,7 +550,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     z.part_sum = q.part_sum;
     z.part_best = p.best ? q.part_best : nullptr;
     z.label_margin = q.label_margin;
-    product("hbr_head_scores", z);
+    product("hbr_head_scores", *q.scores, z);
     HeadFinishArgs f{};
     f.part_max = q.part_max;
     f.part_sum = q.part_sum;
@@ -542,7 +564,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     f.best = p.best;
     f.rows = n;
     f.classes = classes;
-    f.tiles = (uint32_t)tiles(classes, kHeadM);
+    f.tiles = (uint32_t)tiles(classes, q.scores->m);
     queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, 64)), dim3(1024), f);
     if (!gradient) return;
     if (p.dw) {
@@ -575,8 +597,8 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         g.g_stride = q.piece;
         g.g_part = n * q.piece;
         g.part_db = q.part_db;
-        product(("hbr_head_pairs_" + suffix).c_str(), g);
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kHeadM), q.piece, p.db + k0, 1, kc, kc);
+        product("hbr_head_pairs_" + suffix, *q.pairs, g);
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, q.pairs->m), q.piece, p.db + k0, 1, kc, kc);
         if (p.dw) {
             HeadArgs c{};
             c.a = q.g;
@@ -596,7 +618,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c = direct ? (void *)to : q.dw;
             c.c_stride = direct ? p.dw_stride : dim;
             c.c_split = q.piece * dim;
-            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", c);
+            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", *q.by_w, c);
             if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, p.dw_stride);
         }
         if (p.dh) {
@@ -615,7 +637,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c_stride = q.sum_h ? dim : p.dh_stride;
             c.c_split = n * dim;
             c.accumulate = k0 != 0;
-            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", c);
+            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", *q.by_h, c);
         }
     }
     if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);

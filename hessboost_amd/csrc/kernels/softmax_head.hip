@@ -18,6 +18,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
+constexpr int kPairsMore = 4096;  // LDS of the pairs beyond the stages
 constexpr uint32_t kNowhere = 0x80000000u;  // past every buffer: reads as zero
 
 __device__ __forceinline__ int32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane((int32_t)v); }
@@ -52,33 +53,34 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
 // A tile is E rows x kHeadK (or kHeadK x E, transposed) bf16, filled by
 // 16-byte loads that go to LDS without registers: a wave's load fills 1 KiB
 // in lane order, so the layout is that of the loads, and the 16-byte pieces
-// of a row are exchanged by their source addresses instead (a piece's place
-// is xored with its row's low bits), which spreads the reads of a fragment
-// over the banks.
-template <bool T, int E>
+// of a row are exchanged by their source addresses instead: a piece's place
+// is xored with its row's low bits, so that the lanes that LDS serves at once
+// (16 of a 16-byte read, 32 of a transposing one) meet all 64 banks.
+template <bool T, int E, int Waves>
 struct Operand {
-    static constexpr int kLoads = E / 64;                        // a wave's, a step
     static constexpr int kBytes = E * kHeadK * 2;
+    static constexpr int kLoads = kBytes / 1024 / Waves;         // a wave's, a step
     static constexpr int kLanesRow = T ? E / 8 : kHeadK / 8;     // lanes of a row of the tile
     static constexpr int kRowsLoad = 64 / kLanesRow;
+    static_assert(kLoads * Waves * 1024 == kBytes, "whole loads");
     const char *base;
     uint32_t off[kLoads];  // a lane's source, bytes from base
     uint32_t k_at[kLoads]; // and its first k within the step
 
     // first: the tile's first row (m or n); size: how many there are
-    __device__ __forceinline__ void init(const void *p, uint64_t stride, uint64_t first, uint32_t size,
+    __device__ __forceinline__ void init(const void *p, uint64_t stride, uint32_t first, uint32_t size,
                                          const int32_t *labels) {
         const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
-        base = static_cast<const char *>(p) + (T ? first * 2 : first * stride * 2);
+        base = static_cast<const char *>(p) + (T ? (uint64_t)first * 2 : first * stride * 2);
 #pragma unroll
         for (int j = 0; j < kLoads; j++) {
             const uint32_t row = (wave * kLoads + j) * kRowsLoad + lane / kLanesRow, at = lane % kLanesRow;
             if (T) {
-                const uint32_t piece = (((at >> 1) ^ (row & 3u)) << 1) | (at & 1u);
+                const uint32_t piece = at ^ ((row & 3u) << 2);
                 off[j] = first + piece * 8 < size ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
                 k_at[j] = row;
             } else {
-                const uint32_t piece = at ^ ((row >> 1) & 3u);
+                const uint32_t piece = at ^ ((row >> 1) & 7u);
                 const bool in = first + row < size && (!labels || labels[first + row] >= 0);
                 off[j] = in ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
                 k_at[j] = piece * 8;
@@ -88,13 +90,13 @@ struct Operand {
     // The step whose first k is k0 (k of them in all), from base + at bytes.
     // The loads are not the compiler's: it would wait for them before any
     // read of LDS, and the pipeline's own waits know which stage they fill.
-    __device__ __forceinline__ void load(uint32_t lds, uint64_t at, uint32_t k0, uint32_t k, uint32_t keep) const {
+    __device__ __forceinline__ void load(uint32_t lds, uint64_t at, uint32_t k0, uint32_t k, uint64_t keep) const {
         const uint64_t from = reinterpret_cast<uint64_t>(base) + at;
         const i32x4 r = {uniform((uint32_t)from), uniform((uint32_t)(from >> 32)) & 0xffff, 0x7fffffff, 0x00020000};
         const uint32_t to = uniform(lds + threadIdx.x / kWave * (kLoads * 1024));
 #pragma unroll
         for (int j = 0; j < kLoads; j++) {
-            const bool in = k0 + k_at[j] < k && (!T || (keep >> (k_at[j] & 31u)) & 1u);
+            const bool in = k0 + k_at[j] < k && (!T || (keep >> k_at[j]) & 1u);
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(to + j * 1024), "v"(in ? off[j] : kNowhere), "s"(r)
@@ -110,7 +112,7 @@ struct Operand {
             // rows of the tile, four elements each, and get a column each
             const uint32_t k = kk * 16 + lane / 32 * 8 + lane % 16 / 4;
             const uint32_t col = row + lane / 16 % 2 * 16;
-            const char *p = lds + k * (E * 2) + (((col >> 4) ^ (k & 3u)) << 5) + lane % 4 * 8;
+            const char *p = lds + k * (E * 2) + (((col >> 4) ^ ((k & 3u) << 1)) << 5) + lane % 4 * 8;
             union {
                 s16x4 h[2];
                 bf16x8 v;
@@ -119,7 +121,7 @@ struct Operand {
             u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)(p + 4 * E * 2));
             return u.v;
         }
-        const uint32_t m = row + lane % 32, piece = (kk * 2 + lane / 32) ^ ((m >> 1) & 3u);
+        const uint32_t m = row + lane % 32, piece = (kk * 2 + lane / 32) ^ ((m >> 1) & 7u);
         return *reinterpret_cast<const bf16x8 *>(lds + m * (kHeadK * 2) + piece * 16);
     }
 };
@@ -129,23 +131,28 @@ struct Operand {
 constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
 constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
-constexpr int kHeadThreads = 256;  // four waves, 2 x 2, of 128 x 64 each
-constexpr int kStages = 3;
-constexpr int kStageBytes = (kHeadM + kHeadN) * kHeadK * 2;
-
+// A workgroup's tile: M x N of the product, WM x WN waves of equal parts, the
+// operands of two steps in LDS.
+template <int M, int N, int WM, int WN>
 struct HeadTile {
+    static constexpr int kM = M, kN = N, kWavesM = WM, kWavesN = WN, kWaves = WM * WN, kThreads = kWaves * kWave;
+    static constexpr int kWaveM = M / WM, kWaveN = N / WN, kI = kWaveM / 32, kJ = kWaveN / 32;
+    static constexpr int kStage = (M + N) * kHeadK * 2, kLds = 2 * kStage;
     uint32_t m0, n0, split;  // the tile's first row and column, and its share of the steps
-    f32x16 acc[4][2];
     // element e of acc[i][j]: row wave_m + 32 i + row_of(e), column wave_n + 32 j + lane % 32
+    f32x16 acc[kI][kJ];
     uint32_t wave_m, wave_n;
 };
+using BigTile = HeadTile<kBigM, kBigN, 2, 4>;
+using MidTile = HeadTile<kMidM, kMidN, 2, 2>;
 
 __device__ __forceinline__ uint32_t row_of(int e) { return 8 * (e / 4) + 4 * (lane_id() / 32) + e % 4; }
 
 // A workgroup's tile: neighbours in the launch go to different XCDs, so each
 // XCD takes a contiguous share of the tiles, in groups of eight rows of tiles
 // whose operands its L2 holds.
-__device__ __forceinline__ void head_place(const HeadArgs &a, HeadTile &t) {
+template <typename Tile>
+__device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
     const uint32_t all = gridDim.x, per = all / 8, rest = all % 8, xcd = blockIdx.x % 8;
     uint32_t id = xcd * per + min(xcd, rest) + blockIdx.x / 8;
     const uint32_t tiles = a.m_tiles * a.n_tiles;
@@ -154,93 +161,114 @@ __device__ __forceinline__ void head_place(const HeadArgs &a, HeadTile &t) {
     constexpr uint32_t kGroup = 8;
     const uint32_t group = id / (kGroup * a.n_tiles), first = group * kGroup;
     const uint32_t rows = min(kGroup, a.m_tiles - first), in = id - group * kGroup * a.n_tiles;
-    t.m0 = (first + in % rows) * kHeadM;
-    t.n0 = in / rows * kHeadN;
+    t.m0 = (first + in % rows) * Tile::kM;
+    t.n0 = in / rows * Tile::kN;
     const uint32_t wave = threadIdx.x / kWave;
-    t.wave_m = wave / 2 * 128;
-    t.wave_n = wave % 2 * 64;
+    t.wave_m = wave / Tile::kWavesN * Tile::kWaveM;
+    t.wave_n = wave % Tile::kWavesN * Tile::kWaveN;
 }
 
-template <bool AT, bool BT>
-__device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, HeadTile &t, const int32_t *a_labels = nullptr) {
-    Operand<AT, kHeadM> oa;
-    Operand<BT, kHeadN> ob;
+// The tile's products. A step's fragments are read one sixteenth of products
+// ahead of the matrix instructions that use them, across the steps too: the
+// last sixteenth's are in registers when the waves meet, so that the next
+// step's loads may overwrite its stage and its first fragments be read
+// behind the meeting, both under the last sixteenth's products.
+template <bool AT, bool BT, typename Tile>
+__device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile &t, const int32_t *a_labels = nullptr) {
+    using A = Operand<AT, Tile::kM, Tile::kWaves>;
+    using B = Operand<BT, Tile::kN, Tile::kWaves>;
+    constexpr int kI = Tile::kI, kJ = Tile::kJ, kSixteenths = kHeadK / 16;
+    A oa;
+    B ob;
     oa.init(a.a, a.a_stride, t.m0, a.m, a_labels);
     ob.init(a.b, a.b_stride, t.n0, a.n, nullptr);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < kI; i++)
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < kJ; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) t.acc[i][j][e] = 0.0f;
     const uint32_t per = (a.k + kHeadK - 1) / kHeadK, steps = per * a.segments;
     const uint32_t s0 = (uint32_t)((uint64_t)steps * t.split / a.splits),
                    s1 = (uint32_t)((uint64_t)steps * (t.split + 1) / a.splits);
-    // the loads run two steps ahead; past the end they read nothing
+    // past the last step the loads read nothing
     uint32_t seg = s0 / per, at = s0 % per;
     auto load = [&](uint32_t s) {
         const uint32_t k0 = s < s1 ? at * kHeadK : a.k;
         const uint32_t of = a.segments == 1 ? 10 : 2 * min(seg, 5u);
         const uint64_t pa = (kPartA >> of & 3u) * a.a_part, pb = (kPartB >> of & 3u) * a.b_part;
-        const uint32_t keep = (AT || BT) && a.keep && s < s1 ? a.keep[at] : 0xffffffffu;
-        const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % kStages * kStageBytes;
+        const uint64_t keep = (AT || BT) && a.keep && s < s1 ? a.keep[at] : ~0ull;
+        const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % 2 * Tile::kStage;
         oa.load(to, (pa + (uint64_t)at * kHeadK * (AT ? a.a_stride : 1)) * 2, k0, a.k, keep);
-        ob.load(to + Operand<AT, kHeadM>::kBytes, (pb + (uint64_t)at * kHeadK * (BT ? a.b_stride : 1)) * 2, k0, a.k, keep);
+        ob.load(to + A::kBytes, (pb + (uint64_t)at * kHeadK * (BT ? a.b_stride : 1)) * 2, k0, a.k, keep);
         if (++at == per) at = 0, seg++;
     };
-    load(s0);
-    load(s0 + 1);
-    for (uint32_t s = s0; s < s1; s++) {
-        // this step's loads are in: those of the next are the last six
-        asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    bf16x8 fa[2][kI], fb[2][kJ];
+    auto read = [&](int set, uint32_t s, uint32_t kk) {
+        const char *from = lds + s % 2 * Tile::kStage;
+#pragma unroll
+        for (int i = 0; i < kI; i++) fa[set][i] = A::fragment(from, t.wave_m + 32 * i, kk);
+#pragma unroll
+        for (int j = 0; j < kJ; j++) fb[set][j] = B::fragment(from + A::kBytes, t.wave_n + 32 * j, kk);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](int set) {
+        __builtin_amdgcn_s_setprio(1);  // before the other waves' reads and addresses
+#pragma unroll
+        for (int i = 0; i < kI; i++)
+#pragma unroll
+            for (int j = 0; j < kJ; j++)
+                t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[set][i], fb[set][j], t.acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto meet = [&] {  // the wave's loads have landed and its reads are in registers; so have all others'
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load(s + 2);
-        const char *from = lds + s % kStages * kStageBytes;
-        const char *from_b = from + Operand<AT, kHeadM>::kBytes;
+    };
+    load(s0);
+    meet();
+    load(s0 + 1);
+    read(0, s0, 0);
+    for (uint32_t s = s0; s < s1; s++) {
 #pragma unroll
-        for (uint32_t kk = 0; kk < kHeadK / 16; kk++) {
-            bf16x8 fa[4], fb[2];
-#pragma unroll
-            for (int i = 0; i < 4; i++) fa[i] = Operand<AT, kHeadM>::fragment(from, t.wave_m + 32 * i, kk);
-#pragma unroll
-            for (int j = 0; j < 2; j++) fb[j] = Operand<BT, kHeadN>::fragment(from_b, t.wave_n + 32 * j, kk);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
+        for (int kk = 0; kk + 1 < kSixteenths; kk++) {
+            read((kk + 1) & 1, s, kk + 1);
+            multiply(kk & 1);
         }
+        meet();
+        load(s + 2);
+        read(kSixteenths & 1, s + 1, 0);
+        multiply((kSixteenths - 1) & 1);
     }
-    // the loads ahead have landed before the LDS or the workgroup ends
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    meet();  // the loads ahead have landed before the LDS or the workgroup ends
 }
 
 // ---- the scores' maxima and sums -----------------------------------------------------------
 
-// m: classes, n: rows. A lane holds 64 classes of two rows: maxima and sums
-// stay in its registers but for the other half of the wave and the other
-// wave of the same rows.
+// m: classes, n: rows. A lane holds its wave's classes of kJ rows: maxima and
+// sums stay in its registers but for the other half of the wave and the other
+// waves of the same rows.
+template <typename Tile>
 __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
-    __shared__ float bias[kHeadM];
-    __shared__ float top_of[2][kHeadN], sum_of[2][kHeadN];
-    __shared__ int32_t best_of[2][kHeadN];
-    HeadTile t;
+    __shared__ float bias[Tile::kM];
+    __shared__ float top_of[Tile::kWavesM][Tile::kN], sum_of[Tile::kWavesM][Tile::kN];
+    __shared__ int32_t best_of[Tile::kWavesM][Tile::kN];
+    Tile t;
     head_place(a, t);
-    {
-        const uint32_t c = t.m0 + threadIdx.x;
-        bias[threadIdx.x] = c >= a.m ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+    for (uint32_t i = threadIdx.x; i < Tile::kM; i += Tile::kThreads) {
+        const uint32_t c = t.m0 + i;
+        bias[i] = c >= a.m ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
     }
     head_product<false, false>(a, lds, t);
-    const uint32_t lane = lane_id(), wm = t.wave_m / 128;
+    const uint32_t lane = lane_id(), wm = t.wave_m / Tile::kWaveM;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < Tile::kJ; j++) {
         const uint32_t in = t.wave_n + 32 * j + lane % 32, r = t.n0 + in;
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const float z = __builtin_fmaf(t.acc[i][j][e], kLog2e, bias[t.wave_m + 32 * i + row_of(e)]);
@@ -251,15 +279,15 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
         const float shift = shift_of(top);
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(t.acc[i][j][e] - shift);
         sum += __shfl_xor(sum, 32, kWave);
         // the label's class, where it is one of the wave's
         const int64_t y = a.labels && r < a.n ? (int64_t)a.labels[r] - t.m0 - t.wave_m : -1;
-        if (__ballot(y >= 0 && y < 128)) {
+        if (__ballot(y >= 0 && y < Tile::kWaveM)) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (y == 32 * i + row_of(e) && t.m0 + t.wave_m + y < a.m) a.label_margin[r] = t.acc[i][j][e];
@@ -267,7 +295,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
         int32_t best = 0x7fffffff;
         if (a.part_best) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (t.acc[i][j][e] == top) best = min(best, (int32_t)(t.m0 + t.wave_m + 32 * i + row_of(e)));
@@ -281,9 +309,10 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     }
     __syncthreads();
     const uint32_t in = threadIdx.x, r = t.n0 + in;
-    if (in >= kHeadN || r >= a.n) return;
+    if (in >= Tile::kN || r >= a.n) return;
+    static_assert(Tile::kN <= Tile::kThreads && Tile::kWavesM == 2, "a thread a row, two waves of its classes");
     const float t0 = top_of[0][in], t1 = top_of[1][in], top = fmaxf(t0, t1), shift = shift_of(top);
-    const uint64_t at = (uint64_t)(t.m0 / kHeadM) * a.n + r;
+    const uint64_t at = (uint64_t)(t.m0 / Tile::kM) * a.n + r;
     a.part_max[at] = top;
     a.part_sum[at] = sum_of[0][in] * __builtin_amdgcn_exp2f(t0 - shift) + sum_of[1][in] * __builtin_amdgcn_exp2f(t1 - shift);
     if (a.part_best) a.part_best[at] = best_of[t1 > t0 ? 1 : 0][in];
@@ -291,55 +320,77 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
 
 // ---- the scores' gradients --------------------------------------------------------------------
 
-// m: rows, n: classes. A lane holds 64 rows of two classes, so a class's sum
-// over the rows stays in its registers; a row whose label is below 0 is read
-// as zeros and has no gradient. Past the classes g is zero up to its stride.
-template <int Parts>
+// m: rows, n: classes. A lane holds its wave's rows of kJ classes, so a
+// class's sum over the rows stays in its registers; a row whose label is below
+// 0 is read as zeros and has no gradient. Past the classes g is zero up to its
+// stride.
+template <typename Tile, int Parts>
 __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
-    __shared__ float lse_of[kHeadM], by_of[kHeadM];
-    __shared__ int32_t label_of[kHeadM];
-    __shared__ float db_of[2][kHeadN];
-    HeadTile t;
+    __shared__ float lse_of[Tile::kM], by_of[Tile::kM];
+    __shared__ int32_t label_of[Tile::kM];
+    __shared__ float db_of[Tile::kWavesM][Tile::kN];
+    Tile t;
     head_place(a, t);
-    {
-        const uint32_t r = t.m0 + threadIdx.x;
+    for (uint32_t i = threadIdx.x; i < Tile::kM; i += Tile::kThreads) {
+        const uint32_t r = t.m0 + i;
         const int32_t y = r < a.m ? a.labels[r] : -1;
         const bool live = y >= 0;
-        lse_of[threadIdx.x] = live ? a.lse2[r] : INFINITY;
-        by_of[threadIdx.x] = live ? a.grad_scale * (a.weight ? a.weight[r] : 1.0f) : 0.0f;
+        lse_of[i] = live ? a.lse2[r] : INFINITY;
+        by_of[i] = live ? a.grad_scale * (a.weight ? a.weight[r] : 1.0f) : 0.0f;
         const int64_t in = (int64_t)y - (int64_t)a.first - t.n0;
-        label_of[threadIdx.x] = live && in >= 0 && in < (int64_t)kHeadN ? (int32_t)in : -1;
+        label_of[i] = live && in >= 0 && in < (int64_t)Tile::kN ? (int32_t)in : -0x10000;
     }
     head_product<false, false>(a, lds, t, a.labels);
-    const uint32_t lane = lane_id(), wm = t.wave_m / 128;
+    const uint32_t lane = lane_id(), wm = t.wave_m / Tile::kWaveM;
+    float bias[Tile::kJ], db[Tile::kJ];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const uint32_t in = t.wave_n + 32 * j + lane % 32, c = t.n0 + in;
-        const float bias = c >= a.n ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
-        float db = 0.0f;
+    for (int j = 0; j < Tile::kJ; j++) {
+        const uint32_t c = t.n0 + t.wave_n + 32 * j + lane % 32;
+        bias[j] = c >= a.n ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+        db[j] = 0.0f;
+    }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            __builtin_amdgcn_sched_barrier(0);  // the rows' values of one i at a time in registers
+    for (int i = 0; i < Tile::kI; i++) {
+        __builtin_amdgcn_sched_barrier(0);  // the rows' values of one i at a time in registers
+        // does a row of these 32 have its label among the wave's classes?
+        const uint32_t y = (uint32_t)label_of[t.wave_m + 32 * i + lane % 32] - t.wave_n;
+        const bool labelled = __ballot(y < (uint32_t)Tile::kWaveN) != 0;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const uint32_t m = t.wave_m + 32 * i + row_of(e);
+            const float lse = lse_of[m], by = by_of[m];
+#pragma unroll
+            for (int j = 0; j < Tile::kJ; j++)
+                t.acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][e], kLog2e, bias[j]) - lse) * by;
+        }
+        if (labelled) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const uint32_t m = t.wave_m + 32 * i + row_of(e);
-                const float z = __builtin_fmaf(t.acc[i][j][e], kLog2e, bias);
-                float p = __builtin_amdgcn_exp2f(z - lse_of[m]);
-                if (label_of[m] == (int32_t)in) p -= 1.0f;
-                const float v = p * by_of[m];
-                db += v;
-                t.acc[i][j][e] = v;
+                const int32_t at = label_of[m] - (int32_t)(t.wave_n + lane % 32);
+                const float by = by_of[m];
+#pragma unroll
+                for (int j = 0; j < Tile::kJ; j++)
+                    if (at == 32 * j) t.acc[i][j][e] -= by;
             }
         }
-        db += __shfl_xor(db, 32, kWave);
-        if (lane < 32) db_of[wm][in] = db;
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+#pragma unroll
+            for (int j = 0; j < Tile::kJ; j++) db[j] += t.acc[i][j][e];
     }
-    // through LDS to stores of 16 bytes: bf16 whole, f32 in two halves of the
-    // rows, split on the way out. A row of LDS is 16 bytes longer than the
-    // tile's, so that the wave's two rows of a write meet different banks.
-    constexpr int kHalves = Parts == 1 ? 1 : 2, kSize = Parts == 1 ? 2 : 4, kI = 4 / kHalves;
-    constexpr uint32_t kRow = kHeadN * kSize + 16, kRows = kHeadM / kHalves;
-    static_assert(kRows * kRow <= kStages * kStageBytes, "the pairs fit the stages");
+#pragma unroll
+    for (int j = 0; j < Tile::kJ; j++) {
+        db[j] += __shfl_xor(db[j], 32, kWave);
+        if (lane < 32) db_of[wm][t.wave_n + 32 * j + lane % 32] = db[j];
+    }
+    // through LDS to stores of 16 bytes: bf16 whole, f32 in two halves of each
+    // wave's rows, split on the way out. A row of LDS is 16 bytes longer than
+    // the tile's, so that the wave's two rows of a write meet different banks.
+    constexpr int kHalves = Parts == 1 ? 1 : 2, kSize = Parts == 1 ? 2 : 4, kI = Tile::kI / kHalves;
+    constexpr uint32_t kRow = Tile::kN * kSize + 16, kRows = Tile::kM / kHalves, kWaveRows = Tile::kWaveM / kHalves;
+    constexpr uint32_t kLanes = Tile::kN / 8;  // threads of a row
+    static_assert(kRows * kRow <= Tile::kLds + kPairsMore, "the pairs fit the stages");
 #pragma unroll
     for (int half = 0; half < kHalves; half++) {
         if (half) __syncthreads();
@@ -349,20 +400,19 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
 #pragma unroll
             for (int e = 0; e < 16; e++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    char *to = lds + (t.wave_m / kHalves + 32 * i + row_of(e)) * kRow + (t.wave_n + 32 * j + lane % 32) * kSize;
+                for (int j = 0; j < Tile::kJ; j++) {
+                    char *to = lds + (wm * kWaveRows + 32 * i + row_of(e)) * kRow + (t.wave_n + 32 * j + lane % 32) * kSize;
                     const float v = t.acc[half * kI + i][j][e];
                     if constexpr (Parts == 1) *reinterpret_cast<uint16_t *>(to) = to_bf16(v);
                     else *reinterpret_cast<float *>(to) = v;
                 }
         }
         __syncthreads();
-        const uint32_t col = threadIdx.x % 16 * 8;
+        const uint32_t col = threadIdx.x % kLanes * 8;
         uint16_t *g = static_cast<uint16_t *>(a.g) + t.n0 + col;
-        for (uint32_t m = threadIdx.x / 16; m < kRows; m += kHeadThreads / 16) {
-            // the wave of rows from 128 on holds the second half of LDS's rows
-            const uint64_t r = t.m0 + (Parts == 1 ? m : m / 64 * 128 + half * 64 + m % 64);
-            if (r >= a.m) continue;
+        for (uint32_t m = threadIdx.x / kLanes; m < kRows; m += Tile::kThreads / kLanes) {
+            const uint64_t r = t.m0 + m / kWaveRows * Tile::kWaveM + half * kWaveRows + m % kWaveRows;
+            if (r >= a.m || t.n0 + col >= a.g_stride) continue;
             if constexpr (Parts == 1) {
                 *reinterpret_cast<i32x4 *>(g + r * a.g_stride) = *reinterpret_cast<const i32x4 *>(lds + m * kRow + col * 2);
             } else {
@@ -384,17 +434,20 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
         }
     }
     const uint32_t c = t.n0 + threadIdx.x;
-    if (threadIdx.x < kHeadN && c < a.n)
-        a.part_db[(uint64_t)(t.m0 / kHeadM) * a.g_stride + c] = db_of[0][threadIdx.x] + db_of[1][threadIdx.x];
+    if (threadIdx.x < Tile::kN && c < a.n) {
+        float sum = 0.0f;
+        for (int w = 0; w < Tile::kWavesM; w++) sum += db_of[w][threadIdx.x];
+        a.part_db[(uint64_t)(t.m0 / Tile::kM) * a.g_stride + c] = sum;
+    }
 }
 
 // ---- the products with the gradients ---------------------------------------------------------------
 
 // E: what c holds: f32 sums (a share's, added to or not) or the result.
-template <typename E, bool AT>
+template <typename Tile, typename E, bool AT>
 __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
     using T = typename E::type;
-    HeadTile t;
+    Tile t;
     head_place(a, t);
     head_product<AT, true>(a, lds, t);
     const uint32_t lane = lane_id();
@@ -402,15 +455,15 @@ __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
     // rows or the columns is neither read nor written
     const uint64_t from = reinterpret_cast<uint64_t>(static_cast<T *>(a.c) + t.split * a.c_split + t.m0 * a.c_stride + t.n0);
     const uint32_t stride = (uint32_t)a.c_stride * sizeof(T);
-    const uint32_t rows = min(a.rows > t.m0 ? a.rows - t.m0 : 0u, kHeadM);
-    const uint32_t size = rows ? (rows - 1) * stride + min(a.n - t.n0, kHeadN) * (uint32_t)sizeof(T) : 0u;
+    const uint32_t rows = min(a.rows > t.m0 ? a.rows - t.m0 : 0u, (uint32_t)Tile::kM);
+    const uint32_t size = rows ? (rows - 1) * stride + min(a.n - t.n0, (uint32_t)Tile::kN) * (uint32_t)sizeof(T) : 0u;
     __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(from), 0, size, 0x00020000);
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
+    for (int j = 0; j < Tile::kJ; j++) {
         const uint32_t n = t.wave_n + 32 * j + lane % 32;
         const uint32_t at = t.n0 + n < a.n ? (t.wave_m + lane / 32 * 4) * stride + n * (uint32_t)sizeof(T) : kNowhere;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < Tile::kI; i++) {
             if constexpr (sizeof(T) == 4) {
                 if (a.accumulate) {
                     float before[16];
@@ -496,30 +549,32 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
 
 using namespace hbr;
 
-#define HBR_HEAD(name, body)                                                            \
-    extern "C" __global__ __launch_bounds__(kHeadThreads, 2) void name(HeadArgs a) {    \
-        __shared__ __align__(1024) char lds[kStages * kStageBytes];                     \
-        body(a, lds);                                                                   \
+#define HBR_HEAD(name, Tile, more, ...)                                                 \
+    extern "C" __global__ __launch_bounds__(Tile::kThreads, 2) void name(HeadArgs a) {  \
+        __shared__ __align__(1024) char lds[Tile::kLds + more];                         \
+        __VA_ARGS__(a, lds);                                                            \
     }
-HBR_HEAD(hbr_head_scores, head_scores)
-HBR_HEAD(hbr_head_pairs_bf16, head_pairs<1>)
-HBR_HEAD(hbr_head_pairs_f32, head_pairs<3>)
-#define HBR_COMMA ,
-HBR_HEAD(hbr_head_dh_part, head_sums<F32 HBR_COMMA false>)
-HBR_HEAD(hbr_head_dh_bf16, head_sums<Bf16 HBR_COMMA false>)
-HBR_HEAD(hbr_head_dw_part, head_sums<F32 HBR_COMMA true>)
-HBR_HEAD(hbr_head_dw_bf16, head_sums<Bf16 HBR_COMMA true>)
+#define HBR_HEADS(suffix, Tile)                                                         \
+    HBR_HEAD(hbr_head_scores_##suffix, Tile, 0, head_scores<Tile>)                      \
+    HBR_HEAD(hbr_head_pairs_bf16_##suffix, Tile, kPairsMore, head_pairs<Tile, 1>)       \
+    HBR_HEAD(hbr_head_pairs_f32_##suffix, Tile, kPairsMore, head_pairs<Tile, 3>)        \
+    HBR_HEAD(hbr_head_dh_part_##suffix, Tile, 0, head_sums<Tile, F32, false>)           \
+    HBR_HEAD(hbr_head_dh_bf16_##suffix, Tile, 0, head_sums<Tile, Bf16, false>)          \
+    HBR_HEAD(hbr_head_dw_part_##suffix, Tile, 0, head_sums<Tile, F32, true>)            \
+    HBR_HEAD(hbr_head_dw_bf16_##suffix, Tile, 0, head_sums<Tile, Bf16, true>)
+HBR_HEADS(big, BigTile)
+HBR_HEADS(mid, MidTile)
 
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_f32(HeadPartsArgs a) { head_parts<F32, 3>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_bf16(HeadPartsArgs a) { head_parts<Bf16, 1>(a); }
 
-// Bit r: row r has a label (of 64 rows a wave, two words).
+// Bit r: row r has a label.
 extern "C" __global__ __launch_bounds__(256) void hbr_head_keep(HeadKeepArgs a) {
     const uint64_t r = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     const uint64_t bits = __ballot(r < a.rows && a.labels[r] >= 0);
-    if (lane_id() < 2 && (r - lane_id()) < a.rows) a.keep[(r - lane_id()) / 32 + lane_id()] = (uint32_t)(bits >> (32 * lane_id()));
+    if (lane_id() == 0 && r < a.rows) a.keep[r / 64] = bits;
 }
 
 // A row's tiles joined: 64 rows a workgroup, its 16 waves a share of the
