@@ -1146,25 +1146,23 @@ struct LookupSumArgs {
 };
 
 // The head's products C[m][n] = sum_k A(m, k) B(n, k) of bf16 operands, in
-// tiles of kBigM x kBigN or kMidM x kMidN, kHeadK products a step. An operand lies [m][k]
-// (k contiguous) or, transposed, [k][m]; f32 operands lie in three bf16 parts
-// whose sum they are, and a product of two is summed over the six pairs of
-// parts that reach f32's precision, one segment of steps each.
-constexpr uint32_t kBigM = 256;
-constexpr uint32_t kBigN = 256;
-constexpr uint32_t kMidM = 128;
-constexpr uint32_t kMidN = 128;
-constexpr uint32_t kHeadK = 64;
+// tiles of kHeadTile x kHeadTile, kHeadK products a step. An operand lies in
+// rows of m (k across) or, transposed, in rows of k; its columns in chunks of
+// 32. f32 operands lie in three bf16 parts whose sum they are, and a product
+// of two is summed over the six pairs of parts that reach f32's precision,
+// one segment of steps each.
+constexpr uint32_t kHeadTile = 128;
+constexpr uint32_t kHeadK = 32;
 struct HeadArgs {
     const void *a, *b;
-    uint64_t a_stride, b_stride;  // elements
-    uint64_t a_part, b_part;      // elements from one part to the next
+    uint64_t a_row, b_row;        // bytes from row to row
+    uint64_t a_chunk, b_chunk;    // and from chunk to chunk
+    uint64_t a_part, b_part;      // and from part to part
     uint32_t m, n, k;
     uint32_t m_tiles, n_tiles;
     uint32_t splits;              // shares of the steps, each a workgroup's
     uint32_t segments;            // 1, or 6
     uint32_t rows;
-    const uint64_t *keep;         // bit r: row r of the reduction is read (or null: all)
     // scores (m: classes, n: rows) and pairs (m: rows, n: classes)
     const float *bias;            // of the first class
     const int32_t *labels;
@@ -1176,8 +1174,8 @@ struct HeadArgs {
     const float *weight;
     uint64_t first;               // the first class
     float grad_scale;
-    uint32_t pad;
-    void *g;                      // [part][rows][g_stride]
+    uint32_t check;               // rows of m or n may end within a chunk
+    void *g;                      // [part][chunk][rows][32], g_stride columns
     uint64_t g_stride, g_part;
     float *part_db;               // [row tile][g_stride]
     // sums: c in f32, [split][m][c_stride], or the rounded result
@@ -1212,18 +1210,13 @@ struct FewArgs {
     uint32_t dw;            // whether dw is wanted
 };
 
-// src as bf16 parts with rows of dst_stride elements (zeros past cols).
+// src as bf16 parts in chunks of 32 columns (zeros past cols).
 struct HeadPartsArgs {
     const void *src;
+    const int32_t *labels;  // of its rows, or null: elements that are not finite are zeros where it is below 0
     uint16_t *dst;
-    uint64_t rows, src_stride, dst_stride, part;
-    uint32_t cols, pad;
-};
-
-struct HeadKeepArgs {
-    const int32_t *labels;
-    uint64_t *keep;
-    uint64_t rows;
+    uint64_t rows, src_stride, part;
+    uint32_t cols, chunks;
 };
 
 struct HeadFinishArgs {

@@ -305,57 +305,39 @@ namespace {
 // The scores' gradients of one piece of the classes are held at a time, in at
 // most about this many bytes.
 constexpr uint64_t kPieceBytes = 1ull << 30;
-// A product's tiles, and the workgroups of them that run at once.
-struct HeadTiling {
-    uint64_t m, n, threads, slots;
-    const char *name;
-};
-constexpr HeadTiling kBig{kBigM, kBigN, 512, 256, "_big"}, kMid{kMidM, kMidN, 256, 512, "_mid"};
+// Tiles of a product that run at once: four on each of 256 CUs.
+constexpr uint64_t kHeadSlots = 1024;
+// From this many rows on, a call that only scores lays its operands out in
+// chunks too.
+constexpr uint64_t kLayRows = 1024;
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
 // Shares of a product's steps: where its tiles are fewer than the device
-// runs at once, enough of them to fill it, of 8 steps at least.
-uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t all = tiles(m, t.m) * tiles(n, t.n), steps = tiles(k, kHeadK) * segments;
-    return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 8));
-}
-
-// The tiles that take fewer rounds of the device, a round of the middle ones
-// at 0.58 of the big ones' time: a quarter of the area each, twice as many
-// at once, and 0.86 of the rate (512 x 128 x 128 x 16,384 bf16 against
-// 256 x 256 x 256 x 16,384: 1,085 and 1,190 TFLOP/s at their best). Whole
-// products show both sides: 16,384 x 16,384 x 1,024 scores 269 us with big
-// tiles and 305 with middle ones, 4,096 x 5,003 x 256 ones of f32 90 and 74.
-const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments, bool split) {
-    const uint64_t steps = tiles(k, kHeadK) * segments;
-    auto cost = [&](const HeadTiling &t, double round) {
-        const uint64_t shares = split ? head_splits(t, m, n, k, segments) : 1;
-        return (double)(tiles(tiles(m, t.m) * tiles(n, t.n) * shares, t.slots) * tiles(steps, shares)) * round;
-    };
-    return cost(kBig, 1.0) <= cost(kMid, 0.58) ? kBig : kMid;
+// runs at once, enough of them to fill it, of 16 steps at least.
+uint32_t head_splits(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t t = tiles(m, kHeadTile) * tiles(n, kHeadTile), steps = tiles(k, kHeadK) * segments;
+    return (uint32_t)std::max<uint64_t>(1, std::min(kHeadSlots / std::max<uint64_t>(t, 1), steps / 16));
 }
 
 struct HeadPlan {
-    bool few;  // few classes: rows, chunks and the pairs of their own kernels
-    uint32_t score_blocks, chunks;
+    bool few;  // few classes: their own kernels, and the products' shares of the rows
+    uint32_t score_blocks, shares;
     uint64_t g_stride;
-    uint64_t parts, segments, dim8;
-    bool copy_h, copy_w;
+    uint64_t parts, segments, chunks;
+    bool lay;  // h and w are laid out in chunks whatever their rows
     uint64_t piece, pieces;
-    const HeadTiling *scores, *pairs, *by_h, *by_w;  // the tiles of each product
     uint32_t splits_h, splits_w;
     bool sum_h;  // dh is summed from f32 parts
     float *part_max, *part_sum, *label_margin, *lse2, *part_db, *dh, *dw;
     int32_t *part_best;
     uint16_t *h, *w, *g;
-    uint64_t *keep;
-    uint32_t *few_keep;
+    uint32_t *keep;
     uint64_t bytes;
 };
 
-// What the products read in place: bf16 rows of whole 16-byte pieces, near
-// enough to each other for a tile's 32-bit offsets.
+// What the products can read in place: bf16 rows of whole 16-byte pieces,
+// near enough to each other for a tile's 32-bit offsets.
 bool head_in_place(const void *p, uint64_t stride, const hbr_softmax &a) {
     return a.dtype == HBR_BF16 && a.dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 22) &&
            reinterpret_cast<uint64_t>(p) % 16 == 0;
@@ -369,22 +351,22 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     HeadPlan q{};
     q.parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
-    q.dim8 = up(dim, 8);
-    q.scores = &head_tiling(classes, n, dim, q.segments, false);
-    const uint64_t class_tiles = tiles(classes, q.scores->m);
+    q.chunks = tiles(dim, 32);
+    q.lay = dtype == HBR_F32 || n >= kLayRows;
+    const uint64_t class_tiles = tiles(classes, kHeadTile);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
         // up to sixteen waves on each of 256 CUs
         const uint64_t groups = tiles(n, 32), cols = tiles(dim, 32);
         q.score_blocks = (uint32_t)std::min<uint64_t>(tiles(groups, 4), 1024);
-        q.chunks = (uint32_t)std::max<uint64_t>(1, std::min(groups, tiles(4096, cols)));
+        q.shares = (uint32_t)std::max<uint64_t>(1, std::min(groups, tiles(4096, cols)));
         q.g_stride = up(classes, 16);
         if (gradient) {
             q.g = w.take<uint16_t>(n * q.g_stride * (dtype == HBR_F32 ? 2 : 1));
-            q.few_keep = w.take<uint32_t>(groups);
+            q.keep = w.take<uint32_t>(groups);
             q.part_db = w.take<float>(q.score_blocks * 4ull * classes);
-            q.dw = w.take<float>(q.chunks * classes * dim);
+            q.dw = w.take<float>(q.shares * classes * dim);
         }
         q.bytes = w.used;
         return q;
@@ -394,25 +376,21 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.part_best = w.take<int32_t>(class_tiles * n);
     q.label_margin = w.take<float>(n);
     q.lse2 = w.take<float>(n);
-    q.h = w.take<uint16_t>(q.parts * n * q.dim8);
-    q.w = w.take<uint16_t>(q.parts * classes * q.dim8);
+    q.h = w.take<uint16_t>(q.parts * n * q.chunks * 32);
+    q.w = w.take<uint16_t>(q.parts * classes * q.chunks * 32);
     if (gradient) {
         // the pieces as even as whole tiles allow
         const uint64_t row_bytes = std::max<uint64_t>(n, 1) * 2 * q.parts;
-        q.pieces = tiles(classes, std::max<uint64_t>(kBigM, kPieceBytes / row_bytes / kBigM * kBigM));
-        q.piece = up(tiles(classes, q.pieces), kMidM);
+        q.pieces = tiles(classes, std::max<uint64_t>(kHeadTile, kPieceBytes / row_bytes / kHeadTile * kHeadTile));
+        q.piece = up(tiles(classes, q.pieces), kHeadTile);
         q.pieces = tiles(classes, q.piece);
-        q.pairs = &head_tiling(n, q.piece, dim, q.segments, false);
-        q.by_h = &head_tiling(n, dim, q.piece, q.segments, true);
-        q.by_w = &head_tiling(q.piece, dim, n, q.segments, true);
-        q.splits_h = head_splits(*q.by_h, n, dim, q.piece, q.segments);
-        q.splits_w = head_splits(*q.by_w, q.piece, dim, n, q.segments);
+        q.splits_h = head_splits(n, dim, q.piece, q.segments);
+        q.splits_w = head_splits(q.piece, dim, n, q.segments);
         q.sum_h = q.splits_h > 1 || q.pieces > 1;
         q.g = w.take<uint16_t>(q.parts * n * q.piece);
-        q.part_db = w.take<float>(tiles(n, q.pairs->m) * q.piece);
+        q.part_db = w.take<float>(tiles(n, kHeadTile) * q.piece);
         if (q.sum_h) q.dh = w.take<float>(q.splits_h * n * dim);
         if (q.splits_w > 1) q.dw = w.take<float>(q.splits_w * q.piece * dim);
-        q.keep = w.take<uint64_t>(tiles(n, 64));
     }
     q.bytes = w.used;
     return q;
@@ -483,10 +461,10 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         f.lse = p.lse;
         f.best = p.best;
         f.grad_scale = p.grad_scale;
-        f.chunks = q.chunks;
+        f.chunks = q.shares;
         f.g = q.g;
         f.g_stride = q.g_stride;
-        f.keep = q.few_keep;
+        f.keep = q.keep;
         f.part_db = q.part_db;
         f.part_dw = q.dw;
         f.dh = p.dh;
@@ -498,51 +476,49 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         if (!gradient) return;
         if (p.db) sum("hbr_head_sum_f32", q.part_db, q.score_blocks * 4ull, classes, p.db, 1, classes, classes);
         if (!p.dh && !p.dw) return;
-        queue.launch(("hbr_few_products_" + few).c_str(), dim3((uint32_t)tiles((uint64_t)q.chunks * f.col_tiles, 4)), threads, f);
-        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.chunks, classes * dim, p.dw, classes, dim, p.dw_stride);
+        queue.launch(("hbr_few_products_" + few).c_str(), dim3((uint32_t)tiles((uint64_t)q.shares * f.col_tiles, 4)), threads, f);
+        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.shares, classes * dim, p.dw, classes, dim, p.dw_stride);
         return;
     }
-    // the operands of the products: h, and w from class k on
-    auto parts = [&](const void *src, uint64_t stride, uint64_t rows, uint16_t *to) {
+    // the operands of the products
+    struct Laid {
+        const char *p;
+        uint64_t row, chunk, part;
+        uint32_t cols;
+    };
+    auto lay = [&](const void *src, uint64_t stride, uint64_t rows, uint16_t *to, bool always, const int32_t *labels) -> Laid {
+        if (rows == 1) stride = up(dim, 8);
+        if (!always && head_in_place(src, stride, p))
+            return {static_cast<const char *>(src), stride * 2, 64, 0, (uint32_t)dim};
         HeadPartsArgs a{};
         a.src = src;
+        a.labels = labels;
         a.dst = to;
         a.rows = rows;
         a.src_stride = stride;
-        a.dst_stride = q.dim8;
-        a.part = rows * q.dim8;
+        a.part = rows * q.chunks * 32;
         a.cols = (uint32_t)dim;
-        queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.dim8 / 8), threads, a);
+        a.chunks = (uint32_t)q.chunks;
+        queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.chunks * 4), threads, a);
+        return {reinterpret_cast<const char *>(to), 64, rows * 64, a.part * 2, (uint32_t)(q.chunks * 32)};
     };
-    const uint16_t *h = static_cast<const uint16_t *>(p.h), *w = static_cast<const uint16_t *>(p.w);
-    uint64_t h_stride = n > 1 ? p.h_stride : q.dim8, w_stride = classes > 1 ? p.w_stride : q.dim8;
-    if (!head_in_place(h, h_stride, p)) {
-        parts(p.h, p.h_stride, n, q.h);
-        h = q.h;
-        h_stride = q.dim8;
-    }
-    if (!head_in_place(w, w_stride, p)) {
-        parts(p.w, p.w_stride, classes, q.w);
-        w = q.w;
-        w_stride = q.dim8;
-    }
-    const uint64_t h_part = n * q.dim8, w_part = classes * q.dim8;
-    auto product = [&](const std::string &kernel, const HeadTiling &t, HeadArgs a) {
-        a.m_tiles = (uint32_t)tiles(a.m, t.m);
-        a.n_tiles = (uint32_t)tiles(a.n, t.n);
+    const Laid h = lay(p.h, p.h_stride, n, q.h, q.lay || p.dw, p.dw ? p.labels : nullptr);
+    const Laid w = lay(p.w, p.w_stride, classes, q.w, q.lay, nullptr);
+    auto set_a = [](HeadArgs &a, const Laid &o) { a.a = o.p, a.a_row = o.row, a.a_chunk = o.chunk, a.a_part = o.part; };
+    auto set_b = [](HeadArgs &a, const Laid &o) { a.b = o.p, a.b_row = o.row, a.b_chunk = o.chunk, a.b_part = o.part; };
+    auto product = [&](const std::string &kernel, HeadArgs a) {
+        a.m_tiles = (uint32_t)tiles(a.m, kHeadTile);
+        a.n_tiles = (uint32_t)tiles(a.n, kHeadTile);
         a.segments = (uint32_t)q.segments;
-        queue.launch((kernel + t.name).c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), dim3((uint32_t)t.threads), a);
+        queue.launch(kernel.c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), threads, a);
     };
     HeadArgs z{};
-    z.a = w;
-    z.b = h;
-    z.a_stride = w_stride;
-    z.b_stride = h_stride;
-    z.a_part = w_part;
-    z.b_part = h_part;
+    set_a(z, w);
+    set_b(z, h);
     z.m = (uint32_t)classes;
     z.n = (uint32_t)n;
-    z.k = (uint32_t)q.dim8;
+    z.k = std::min(h.cols, w.cols);
+    z.check = z.k % kHeadK != 0;
     z.splits = 1;
     z.bias = p.bias;
     z.labels = p.labels;
@@ -550,7 +526,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     z.part_sum = q.part_sum;
     z.part_best = p.best ? q.part_best : nullptr;
     z.label_margin = q.label_margin;
-    product("hbr_head_scores", *q.scores, z);
+    product("hbr_head_scores", z);
     HeadFinishArgs f{};
     f.part_max = q.part_max;
     f.part_sum = q.part_sum;
@@ -564,28 +540,21 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     f.best = p.best;
     f.rows = n;
     f.classes = classes;
-    f.tiles = (uint32_t)tiles(classes, q.scores->m);
+    f.tiles = (uint32_t)tiles(classes, kHeadTile);
     queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, 64)), dim3(1024), f);
     if (!gradient) return;
-    if (p.dw) {
-        HeadKeepArgs k{};
-        k.labels = p.labels;
-        k.keep = q.keep;
-        k.rows = n;
-        queue.launch("hbr_head_keep", dim3((uint32_t)tiles(n, 256)), threads, k);
-    }
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
         const uint64_t kc = std::min(q.piece, classes - k0);
+        Laid wk = w;  // w from class k0 on, and its scores' gradients
+        wk.p += k0 * w.row;
+        const Laid pairs{reinterpret_cast<const char *>(q.g), 64, n * 64, n * q.piece * 2, (uint32_t)q.piece};
         HeadArgs g{};
-        g.a = h;
-        g.b = w + k0 * w_stride;
-        g.a_stride = h_stride;
-        g.b_stride = w_stride;
-        g.a_part = h_part;
-        g.b_part = w_part;
+        set_a(g, h);
+        set_b(g, wk);
         g.m = (uint32_t)n;
         g.n = (uint32_t)kc;
-        g.k = (uint32_t)q.dim8;
+        g.k = z.k;
+        g.check = z.check;
         g.splits = 1;
         g.bias = p.bias ? p.bias + k0 : nullptr;
         g.labels = p.labels;
@@ -597,38 +566,29 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         g.g_stride = q.piece;
         g.g_part = n * q.piece;
         g.part_db = q.part_db;
-        product("hbr_head_pairs_" + suffix, *q.pairs, g);
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, q.pairs->m), q.piece, p.db + k0, 1, kc, kc);
+        product("hbr_head_pairs_" + suffix, g);
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kHeadTile), q.piece, p.db + k0, 1, kc, kc);
         if (p.dw) {
             HeadArgs c{};
-            c.a = q.g;
-            c.b = h;
-            c.a_stride = q.piece;
-            c.b_stride = h_stride;
-            c.a_part = g.g_part;
-            c.b_part = h_part;
-            c.m = (uint32_t)up(kc, 8);
+            set_a(c, pairs);
+            set_b(c, h);
+            c.m = (uint32_t)up(kc, 32);
             c.rows = (uint32_t)kc;
             c.n = (uint32_t)dim;
             c.k = (uint32_t)n;
             c.splits = q.splits_w;
-            c.keep = q.keep;
             char *to = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
             const bool direct = q.splits_w == 1;
             c.c = direct ? (void *)to : q.dw;
             c.c_stride = direct ? p.dw_stride : dim;
             c.c_split = q.piece * dim;
-            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", *q.by_w, c);
+            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", c);
             if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, p.dw_stride);
         }
         if (p.dh) {
             HeadArgs c{};
-            c.a = q.g;
-            c.b = g.b;
-            c.a_stride = q.piece;
-            c.b_stride = w_stride;
-            c.a_part = g.g_part;
-            c.b_part = w_part;
+            set_a(c, pairs);
+            set_b(c, wk);
             c.m = c.rows = (uint32_t)n;
             c.n = (uint32_t)dim;
             c.k = (uint32_t)kc;
@@ -637,7 +597,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c_stride = q.sum_h ? dim : p.dh_stride;
             c.c_split = n * dim;
             c.accumulate = k0 != 0;
-            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", *q.by_h, c);
+            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", c);
         }
     }
     if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);

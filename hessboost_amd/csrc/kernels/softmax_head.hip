@@ -18,7 +18,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr int kPairsMore = 4096;  // LDS of the pairs beyond the stages
+constexpr int kTile = (int)kHeadTile, kHeadWaves = 4;
+constexpr int kPairsMore = 2048;  // LDS of the pairs beyond the stages
 constexpr uint32_t kNowhere = 0x80000000u;  // past every buffer: reads as zero
 
 __device__ __forceinline__ int32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane((int32_t)v); }
@@ -50,58 +51,74 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
 
 // ---- one operand's tile in LDS ---------------------------------------------------------
 //
-// A tile is E rows x kHeadK (or kHeadK x E, transposed) bf16, filled by
-// 16-byte loads that go to LDS without registers: a wave's load fills 1 KiB
-// in lane order, so the layout is that of the loads, and the 16-byte pieces
-// of a row are exchanged by their source addresses instead: a piece's place
-// is xored with its row's low bits, so that the lanes that LDS serves at once
-// (16 of a 16-byte read, 32 of a transposing one) meet all 64 banks.
-template <bool T, int E, int Waves>
+// An operand lies in chunks of 32 columns: rows row_step bytes apart, chunks
+// chunk_step. What the products read often is laid out so (a chunk's rows of
+// 64 bytes one behind the other), and 16 rows of a chunk are the 1 KiB that
+// one load of a wave fills; plain rows are the same with other steps.
+//
+// A tile is kTile rows x kHeadK, or, transposed, kHeadK rows x kTile in four
+// chunks, filled by 16-byte loads that go to LDS without registers. A wave's
+// load fills LDS in lane order, so the layout is that of the loads. Of a tile
+// read along its rows the 16-byte pieces of a row are exchanged by their
+// source addresses: a piece's place is xored with its row's bits, so that the
+// 16 lanes that LDS serves at once meet all 64 banks. The transposing reads
+// meet them anyway (four rows of 64 bytes).
+template <bool T>
 struct Operand {
-    static constexpr int kBytes = E * kHeadK * 2;
-    static constexpr int kLoads = kBytes / 1024 / Waves;         // a wave's, a step
-    static constexpr int kLanesRow = T ? E / 8 : kHeadK / 8;     // lanes of a row of the tile
-    static constexpr int kRowsLoad = 64 / kLanesRow;
-    static_assert(kLoads * Waves * 1024 == kBytes, "whole loads");
-    const char *base;
-    uint32_t off[kLoads];  // a lane's source, bytes from base
-    uint32_t k_at[kLoads]; // and its first k within the step
+    static constexpr int kBytes = kTile * kHeadK * 2;
+    static constexpr int kLoads = kBytes / 1024 / kHeadWaves;  // a wave's, a step
+    uint64_t at, step;      // where the wave's next step begins, and from step to step
+    uint32_t off[kLoads];   // a lane's source, bytes from there
+    uint32_t k_at[kLoads];  // and its first k within the step (not transposed)
 
-    // first: the tile's first row (m or n); size: how many there are
-    __device__ __forceinline__ void init(const void *p, uint64_t stride, uint32_t first, uint32_t size,
-                                         const int32_t *labels) {
+    // first: the tile's first row (m or n); size: how many there are (to the
+    // end of the last chunk, transposed)
+    __device__ __forceinline__ void init(uint64_t row_step, uint64_t chunk_step, uint32_t first, uint32_t size, const int32_t *labels) {
         const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
-        base = static_cast<const char *>(p) + (T ? (uint64_t)first * 2 : first * stride * 2);
+        step = T ? kHeadK * row_step : chunk_step;
 #pragma unroll
         for (int j = 0; j < kLoads; j++) {
-            const uint32_t row = (wave * kLoads + j) * kRowsLoad + lane / kLanesRow, at = lane % kLanesRow;
-            if (T) {
-                const uint32_t piece = at ^ ((row & 3u) << 2);
-                off[j] = first + piece * 8 < size ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
-                k_at[j] = row;
+            if (T) {  // a wave loads a chunk
+                const uint32_t row = j * 16 + lane / 4, col = wave * 32 + lane % 4 * 8;
+                off[j] = first + col < size ? (uint32_t)(row * row_step) + lane % 4 * 16 : kNowhere;
             } else {
-                const uint32_t piece = at ^ ((row >> 1) & 7u);
+                const uint32_t row = (wave * kLoads + j) * 16 + lane / 4, piece = lane % 4 ^ ((row >> 2) & 3u);
                 const bool in = first + row < size && (!labels || labels[first + row] >= 0);
-                off[j] = in ? (uint32_t)(row * stride * 2) + piece * 16 : kNowhere;
+                off[j] = in ? (uint32_t)(row * row_step) + piece * 16 : kNowhere;
                 k_at[j] = piece * 8;
             }
         }
+        static_assert(kLoads == 2 && kTile == 32 * kHeadWaves, "a wave loads a chunk's 32 rows");
     }
-    // The step whose first k is k0 (k of them in all), from base + at bytes.
-    // The loads are not the compiler's: it would wait for them before any
-    // read of LDS, and the pipeline's own waits know which stage they fill.
-    __device__ __forceinline__ void load(uint32_t lds, uint64_t at, uint32_t k0, uint32_t k, uint64_t keep) const {
-        const uint64_t from = reinterpret_cast<uint64_t>(base) + at;
-        const i32x4 r = {uniform((uint32_t)from), uniform((uint32_t)(from >> 32)) & 0xffff, 0x7fffffff, 0x00020000};
+    // To step s of the operand at p.
+    __device__ __forceinline__ void seek(const void *p, uint64_t row_step, uint64_t chunk_step, uint32_t first, uint32_t s) {
+        const uint32_t wave = uniform(threadIdx.x / kWave);
+        at = reinterpret_cast<uint64_t>(p) + (T ? (first / 32 + wave) * chunk_step : first * row_step) + s * step;
+    }
+    // The next step, of which `left` k are left (0: nothing is read). The
+    // loads are not the compiler's: it would wait for them before any read of
+    // LDS, and the pipeline's own waits know which stage they fill.
+    // Transposed, the buffer ends with the last k; else what lies past it is
+    // zeros, or `check`ed.
+    __device__ __forceinline__ void load(uint32_t lds, uint32_t left, uint64_t row_step, bool check) {
         const uint32_t to = uniform(lds + threadIdx.x / kWave * (kLoads * 1024));
+        const uint32_t size = T ? (left >= kHeadK ? 0x7fffffffu : left * (uint32_t)row_step) : left ? 0x7fffffffu : 0u;
+        const i32x4 r = {uniform((uint32_t)at), uniform((uint32_t)(at >> 32)) & 0xffff, uniform(size), 0x00020000};
+        uint32_t from[kLoads];
 #pragma unroll
-        for (int j = 0; j < kLoads; j++) {
-            const bool in = k0 + k_at[j] < k && (!T || (keep >> k_at[j]) & 1u);
+        for (int j = 0; j < kLoads; j++) from[j] = off[j];
+        if (!T && check && left < kHeadK) {
+#pragma unroll
+            for (int j = 0; j < kLoads; j++)
+                if (k_at[j] >= left) from[j] = kNowhere;
+        }
+#pragma unroll
+        for (int j = 0; j < kLoads; j++)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(to + j * 1024), "v"(in ? off[j] : kNowhere), "s"(r)
+                         : "s"(to + j * 1024), "v"(from[j]), "s"(r)
                          : "memory");
-        }
+        at += step;
     }
     // Rows [row, row + 32) and products [16 kk, 16 kk + 16) of the tile: a
     // lane's row is lane % 32, its products the eight from 8 (lane / 32) on.
@@ -111,17 +128,16 @@ struct Operand {
             // two transposing reads of four products: sixteen lanes read four
             // rows of the tile, four elements each, and get a column each
             const uint32_t k = kk * 16 + lane / 32 * 8 + lane % 16 / 4;
-            const uint32_t col = row + lane / 16 % 2 * 16;
-            const char *p = lds + k * (E * 2) + (((col >> 4) ^ ((k & 3u) << 1)) << 5) + lane % 4 * 8;
+            const char *p = lds + row / 32 * 2048 + k * 64 + lane / 16 % 2 * 32 + lane % 4 * 8;
             union {
                 s16x4 h[2];
                 bf16x8 v;
             } u;
             u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)p);
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)(p + 4 * E * 2));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HBR_LDS s16x4 *)(p + 4 * 64));
             return u.v;
         }
-        const uint32_t m = row + lane % 32, piece = (kk * 2 + lane / 32) ^ ((m >> 1) & 7u);
+        const uint32_t m = row + lane % 32, piece = (kk * 2 + lane / 32) ^ ((m >> 2) & 3u);
         return *reinterpret_cast<const bf16x8 *>(lds + m * (kHeadK * 2) + piece * 16);
     }
 };
@@ -131,27 +147,24 @@ struct Operand {
 constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
 constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
-// A workgroup's tile: M x N of the product, WM x WN waves of equal parts, the
-// operands of two steps in LDS.
-template <int M, int N, int WM, int WN>
+// A workgroup's tile of the product: kTile x kTile, 2 x 2 waves, the operands
+// of two steps in LDS.
 struct HeadTile {
-    static constexpr int kM = M, kN = N, kWavesM = WM, kWavesN = WN, kWaves = WM * WN, kThreads = kWaves * kWave;
-    static constexpr int kWaveM = M / WM, kWaveN = N / WN, kI = kWaveM / 32, kJ = kWaveN / 32;
-    static constexpr int kStage = (M + N) * kHeadK * 2, kLds = 2 * kStage;
+    static constexpr int kM = kTile, kN = kTile, kWavesM = 2, kWavesN = 2, kThreads = kHeadWaves * kWave;
+    static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN, kI = kWaveM / 32, kJ = kWaveN / 32;
+    static constexpr int kStage = (kM + kN) * kHeadK * 2, kLds = 2 * kStage;
     uint32_t m0, n0, split;  // the tile's first row and column, and its share of the steps
     // element e of acc[i][j]: row wave_m + 32 i + row_of(e), column wave_n + 32 j + lane % 32
     f32x16 acc[kI][kJ];
     uint32_t wave_m, wave_n;
 };
-using BigTile = HeadTile<kBigM, kBigN, 2, 4>;
-using MidTile = HeadTile<kMidM, kMidN, 2, 2>;
+using Tile = HeadTile;
 
 __device__ __forceinline__ uint32_t row_of(int e) { return 8 * (e / 4) + 4 * (lane_id() / 32) + e % 4; }
 
 // A workgroup's tile: neighbours in the launch go to different XCDs, so each
 // XCD takes a contiguous share of the tiles, in groups of eight rows of tiles
 // whose operands its L2 holds.
-template <typename Tile>
 __device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
     const uint32_t all = gridDim.x, per = all / 8, rest = all % 8, xcd = blockIdx.x % 8;
     uint32_t id = xcd * per + min(xcd, rest) + blockIdx.x / 8;
@@ -173,15 +186,15 @@ __device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
 // last sixteenth's are in registers when the waves meet, so that the next
 // step's loads may overwrite its stage and its first fragments be read
 // behind the meeting, both under the last sixteenth's products.
-template <bool AT, bool BT, typename Tile>
+template <bool AT, bool BT>
 __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile &t, const int32_t *a_labels = nullptr) {
-    using A = Operand<AT, Tile::kM, Tile::kWaves>;
-    using B = Operand<BT, Tile::kN, Tile::kWaves>;
+    using A = Operand<AT>;
+    using B = Operand<BT>;
     constexpr int kI = Tile::kI, kJ = Tile::kJ, kSixteenths = kHeadK / 16;
     A oa;
     B ob;
-    oa.init(a.a, a.a_stride, t.m0, a.m, a_labels);
-    ob.init(a.b, a.b_stride, t.n0, a.n, nullptr);
+    oa.init(a.a_row, a.a_chunk, t.m0, a.m, a_labels);
+    ob.init(a.b_row, a.b_chunk, t.n0, a.n, nullptr);
 #pragma unroll
     for (int i = 0; i < kI; i++)
 #pragma unroll
@@ -191,17 +204,23 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
     const uint32_t per = (a.k + kHeadK - 1) / kHeadK, steps = per * a.segments;
     const uint32_t s0 = (uint32_t)((uint64_t)steps * t.split / a.splits),
                    s1 = (uint32_t)((uint64_t)steps * (t.split + 1) / a.splits);
-    // past the last step the loads read nothing
     uint32_t seg = s0 / per, at = s0 % per;
-    auto load = [&](uint32_t s) {
-        const uint32_t k0 = s < s1 ? at * kHeadK : a.k;
+    auto seek = [&] {
         const uint32_t of = a.segments == 1 ? 10 : 2 * min(seg, 5u);
-        const uint64_t pa = (kPartA >> of & 3u) * a.a_part, pb = (kPartB >> of & 3u) * a.b_part;
-        const uint64_t keep = (AT || BT) && a.keep && s < s1 ? a.keep[at] : ~0ull;
+        oa.seek(static_cast<const char *>(a.a) + (kPartA >> of & 3u) * a.a_part, a.a_row, a.a_chunk, t.m0, at);
+        ob.seek(static_cast<const char *>(a.b) + (kPartB >> of & 3u) * a.b_part, a.b_row, a.b_chunk, t.n0, at);
+    };
+    seek();
+    // past the last step the loads read nothing
+    auto load = [&](uint32_t s) {
+        const uint32_t left = s < s1 ? a.k - at * kHeadK : 0;
         const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % 2 * Tile::kStage;
-        oa.load(to, (pa + (uint64_t)at * kHeadK * (AT ? a.a_stride : 1)) * 2, k0, a.k, keep);
-        ob.load(to + A::kBytes, (pb + (uint64_t)at * kHeadK * (BT ? a.b_stride : 1)) * 2, k0, a.k, keep);
-        if (++at == per) at = 0, seg++;
+        oa.load(to, left, a.a_row, a.check != 0);
+        ob.load(to + A::kBytes, left, a.b_row, a.check != 0);
+        if (++at == per) {
+            at = 0, seg++;
+            seek();
+        }
     };
     bf16x8 fa[2][kI], fb[2][kJ];
     auto read = [&](int set, uint32_t s, uint32_t kk) {
@@ -250,7 +269,6 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
 // m: classes, n: rows. A lane holds its wave's classes of kJ rows: maxima and
 // sums stay in its registers but for the other half of the wave and the other
 // waves of the same rows.
-template <typename Tile>
 __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     __shared__ float bias[Tile::kM];
     __shared__ float top_of[Tile::kWavesM][Tile::kN], sum_of[Tile::kWavesM][Tile::kN];
@@ -324,7 +342,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
 // class's sum over the rows stays in its registers; a row whose label is below
 // 0 is read as zeros and has no gradient. Past the classes g is zero up to its
 // stride.
-template <typename Tile, int Parts>
+template <int Parts>
 __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
     __shared__ float lse_of[Tile::kM], by_of[Tile::kM];
     __shared__ int32_t label_of[Tile::kM];
@@ -389,7 +407,6 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
     // the tile's, so that the wave's two rows of a write meet different banks.
     constexpr int kHalves = Parts == 1 ? 1 : 2, kSize = Parts == 1 ? 2 : 4, kI = Tile::kI / kHalves;
     constexpr uint32_t kRow = Tile::kN * kSize + 16, kRows = Tile::kM / kHalves, kWaveRows = Tile::kWaveM / kHalves;
-    constexpr uint32_t kLanes = Tile::kN / 8;  // threads of a row
     static_assert(kRows * kRow <= Tile::kLds + kPairsMore, "the pairs fit the stages");
 #pragma unroll
     for (int half = 0; half < kHalves; half++) {
@@ -408,13 +425,14 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
                 }
         }
         __syncthreads();
-        const uint32_t col = threadIdx.x % kLanes * 8;
-        uint16_t *g = static_cast<uint16_t *>(a.g) + t.n0 + col;
-        for (uint32_t m = threadIdx.x / kLanes; m < kRows; m += Tile::kThreads / kLanes) {
+        // a wave writes 16 rows of a chunk at a time
+        for (uint32_t i = threadIdx.x; i < kRows * (Tile::kN / 8); i += Tile::kThreads) {
+            const uint32_t chunk = i / (kRows * 4), m = i / 4 % kRows, col = chunk * 32 + i % 4 * 8;
             const uint64_t r = t.m0 + m / kWaveRows * Tile::kWaveM + half * kWaveRows + m % kWaveRows;
             if (r >= a.m || t.n0 + col >= a.g_stride) continue;
+            uint16_t *g = static_cast<uint16_t *>(a.g) + ((uint64_t)(t.n0 / 32 + chunk) * a.m + r) * 32 + i % 4 * 8;
             if constexpr (Parts == 1) {
-                *reinterpret_cast<i32x4 *>(g + r * a.g_stride) = *reinterpret_cast<const i32x4 *>(lds + m * kRow + col * 2);
+                *reinterpret_cast<i32x4 *>(g) = *reinterpret_cast<const i32x4 *>(lds + m * kRow + col * 2);
             } else {
                 Vec<float, 4> v[2];
 #pragma unroll
@@ -429,7 +447,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
                     for (int q = 0; q < 3; q++) out[q].v[k] = s[q];
                 }
 #pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(g + q * a.g_part + r * a.g_stride) = out[q];
+                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(g + q * a.g_part) = out[q];
             }
         }
     }
@@ -444,7 +462,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
 // ---- the products with the gradients ---------------------------------------------------------------
 
 // E: what c holds: f32 sums (a share's, added to or not) or the result.
-template <typename Tile, typename E, bool AT>
+template <typename E, bool AT>
 __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
     using T = typename E::type;
     Tile t;
@@ -517,31 +535,48 @@ __device__ __forceinline__ void head_sum(const HeadSumArgs &a) {
     }
 }
 
-// Eight elements of a row a thread.
+// Rows into chunks of 32 columns (zeros past the last): eight elements of a
+// row a thread, a wave 16 rows of a chunk.
 template <typename E, int Parts>
 __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
     using T = typename E::type;
-    const uint64_t wide = a.dst_stride / 8, cells = a.rows * wide;
+    const uint64_t cells = a.rows * a.chunks * 4;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = i / wide;
-        const uint32_t c = (uint32_t)(i - r * wide) * 8;
+        // four chunks (256 bytes of a bf16 row) of a row by neighbouring threads
+        const uint64_t block = i / (a.rows * 16);
+        const uint32_t wide = min(4u, a.chunks - (uint32_t)block * 4);
+        const uint64_t in = i - block * a.rows * 16, r = in / (wide * 4);
+        const uint32_t chunk = (uint32_t)block * 4 + (uint32_t)(in % (wide * 4)) / 4, c = chunk * 32 + in % 4 * 8;
         const T *src = static_cast<const T *>(a.src) + r * a.src_stride + c;
+        Vec<T, 8> v{};
+        if (c + 8 <= a.cols) {
+            __builtin_memcpy(&v, src, sizeof v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (c + k < a.cols) v.v[k] = src[k];
+        }
+        // a row that takes no part may hold anything: finite, so that its
+        // gradient of zero adds nothing
+        if (a.labels && a.labels[r] < 0)
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (!(__builtin_fabsf(E::up(v.v[k])) < INFINITY)) v.v[k] = (T)0;
         Vec<uint16_t, 8> out[Parts];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const T v = c + k < a.cols ? src[k] : (T)0;
             if (Parts == 1) {
-                out[0].v[k] = (uint16_t)v;
+                out[0].v[k] = (uint16_t)v.v[k];
             } else {
                 uint16_t s[3];
-                split3(E::up(v), s);
+                split3(E::up(v.v[k]), s);
 #pragma unroll
                 for (int q = 0; q < Parts; q++) out[q].v[k] = s[q];
             }
         }
 #pragma unroll
         for (int q = 0; q < Parts; q++)
-            *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + q * a.part + r * a.dst_stride + c) = out[q];
+            *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + q * a.part + (chunk * a.rows + r) * 32 + in % 4 * 8) = out[q];
     }
 }
 
@@ -549,33 +584,23 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
 
 using namespace hbr;
 
-#define HBR_HEAD(name, Tile, more, ...)                                                 \
-    extern "C" __global__ __launch_bounds__(Tile::kThreads, 2) void name(HeadArgs a) {  \
+#define HBR_HEAD(name, at_once, more, ...)                                                       \
+    extern "C" __global__ __launch_bounds__(Tile::kThreads, at_once) void name(HeadArgs a) {     \
         __shared__ __align__(1024) char lds[Tile::kLds + more];                         \
         __VA_ARGS__(a, lds);                                                            \
     }
-#define HBR_HEADS(suffix, Tile)                                                         \
-    HBR_HEAD(hbr_head_scores_##suffix, Tile, 0, head_scores<Tile>)                      \
-    HBR_HEAD(hbr_head_pairs_bf16_##suffix, Tile, kPairsMore, head_pairs<Tile, 1>)       \
-    HBR_HEAD(hbr_head_pairs_f32_##suffix, Tile, kPairsMore, head_pairs<Tile, 3>)        \
-    HBR_HEAD(hbr_head_dh_part_##suffix, Tile, 0, head_sums<Tile, F32, false>)           \
-    HBR_HEAD(hbr_head_dh_bf16_##suffix, Tile, 0, head_sums<Tile, Bf16, false>)          \
-    HBR_HEAD(hbr_head_dw_part_##suffix, Tile, 0, head_sums<Tile, F32, true>)            \
-    HBR_HEAD(hbr_head_dw_bf16_##suffix, Tile, 0, head_sums<Tile, Bf16, true>)
-HBR_HEADS(big, BigTile)
-HBR_HEADS(mid, MidTile)
+HBR_HEAD(hbr_head_scores, 3, 0, head_scores)
+HBR_HEAD(hbr_head_pairs_bf16, 4, kPairsMore, head_pairs<1>)
+HBR_HEAD(hbr_head_pairs_f32, 4, kPairsMore, head_pairs<3>)
+HBR_HEAD(hbr_head_dh_part, 4, 0, head_sums<F32, false>)
+HBR_HEAD(hbr_head_dh_bf16, 4, 0, head_sums<Bf16, false>)
+HBR_HEAD(hbr_head_dw_part, 4, 0, head_sums<F32, true>)
+HBR_HEAD(hbr_head_dw_bf16, 4, 0, head_sums<Bf16, true>)
 
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_f32(HeadPartsArgs a) { head_parts<F32, 3>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_bf16(HeadPartsArgs a) { head_parts<Bf16, 1>(a); }
-
-// Bit r: row r has a label.
-extern "C" __global__ __launch_bounds__(256) void hbr_head_keep(HeadKeepArgs a) {
-    const uint64_t r = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint64_t bits = __ballot(r < a.rows && a.labels[r] >= 0);
-    if (lane_id() == 0 && r < a.rows) a.keep[r / 64] = bits;
-}
 
 // A row's tiles joined: 64 rows a workgroup, its 16 waves a share of the
 // class tiles each, in order within a wave and over the waves.

@@ -705,6 +705,8 @@ int hbr_leaf_embedding_grad(int ordinal, const hbr_lookup *p, const void *dout, 
  *   best[r] = the first class of the largest z;
  *   dh, dw, db = the gradients of grad_scale * (sum over r of loss[r]), in h,
  *             w and bias.
+ * (The lse of a row that takes no part counts inputs that are not finite as
+ * zeros or not, as it comes.)
  * A label of n_classes or more makes its row's lse and loss, and the
  * gradients, NaN. A bias of -infinity shuts a class; a row whose classes are
  * all shut has an lse of -infinity, and a loss and gradients that are NaN
