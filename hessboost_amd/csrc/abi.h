@@ -1146,12 +1146,11 @@ struct LookupSumArgs {
 };
 
 // The head's products C[m][n] = sum_k A(m, k) B(n, k) of bf16 operands, in
-// tiles of kHeadTile x kHeadTile, kHeadK products a step. An operand lies in
+// tiles of 256 x 256 or 128 x 128, kHeadK products a step. An operand lies in
 // rows of m (k across) or, transposed, in rows of k; its columns in chunks of
 // 32. f32 operands lie in three bf16 parts whose sum they are, and a product
 // of two is summed over the six pairs of parts that reach f32's precision,
 // one segment of steps each.
-constexpr uint32_t kHeadTile = 128;
 constexpr uint32_t kHeadK = 32;
 struct HeadArgs {
     const void *a, *b;
@@ -1176,7 +1175,7 @@ struct HeadArgs {
     float grad_scale;
     uint32_t check;               // rows of m or n may end within a chunk
     void *g;                      // [part][chunk][rows][32], g_stride columns
-    uint64_t g_stride, g_part;
+    uint64_t g_stride, g_chunk, g_part;
     float *part_db;               // [row tile][g_stride]
     // sums: c in f32, [split][m][c_stride], or the rounded result
     void *c;
@@ -1210,12 +1209,23 @@ struct FewArgs {
     uint32_t dw;            // whether dw is wanted
 };
 
+struct FewSumsArgs {
+    const float *part_dw;  // [share][classes][dim], or null
+    const float *part_db;  // [wave][classes], or null
+    void *dw;
+    float *db;
+    uint64_t dw_stride;
+    uint32_t shares, waves, classes, dim;
+    uint32_t dw_blocks;    // the blocks of dw's cells, those of db's behind them
+    uint32_t pad;
+};
+
 // src as bf16 parts in chunks of 32 columns (zeros past cols).
 struct HeadPartsArgs {
     const void *src;
     const int32_t *labels;  // of its rows, or null: elements that are not finite are zeros where it is below 0
     uint16_t *dst;
-    uint64_t rows, src_stride, part;
+    uint64_t rows, src_stride, chunk, part;  // elements from chunk to chunk, and from part to part
     uint32_t cols, chunks;
 };
 

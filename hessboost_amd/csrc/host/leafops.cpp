@@ -170,7 +170,7 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     // column at a time, in blocks of rows: enough for the device, of which
     // each reads at least as many vectors as it writes sums.
     // (A block's rows lie within 2 GiB of dout and of the ids.)
-    q.columns = q.n && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows &&
+    q.columns = q.n && p.table_rows && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows &&
                 p.table_rows / p.n_columns <= 2048 && std::max(p.out_stride, p.ids_stride) < 32768;
     if (q.columns) {
         const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
@@ -305,19 +305,47 @@ namespace {
 // The scores' gradients of one piece of the classes are held at a time, in at
 // most about this many bytes.
 constexpr uint64_t kPieceBytes = 1ull << 30;
-// Tiles of a product that run at once: four on each of 256 CUs.
-constexpr uint64_t kHeadSlots = 1024;
+// Bytes from one chunk of 32 bf16 columns to the next. An odd multiple of
+// 2 KiB: the chunks of a tile, whose steps of 32 rows are 2 KiB each, then
+// begin in different halves of the L2's channels.
+constexpr uint64_t kChunkStep = 2048;
+uint64_t chunk_bytes(uint64_t rows) { return ((rows * 64 + 2 * kChunkStep - 1) / (2 * kChunkStep) * 2 + 1) * kChunkStep; }
+
 // From this many rows on, a call that only scores lays its operands out in
 // chunks too.
 constexpr uint64_t kLayRows = 1024;
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
+// A product's tiles, and how many of them run at once on 256 CUs.
+struct HeadTiling {
+    uint64_t tile, threads, slots;
+    const char *name;
+};
+constexpr HeadTiling kTile256{256, 512, 256, "_256"}, kTile128{128, 256, 1024, "_128"};
+
 // Shares of a product's steps: where its tiles are fewer than the device
 // runs at once, enough of them to fill it, of 16 steps at least.
-uint32_t head_splits(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t t = tiles(m, kHeadTile) * tiles(n, kHeadTile), steps = tiles(k, kHeadK) * segments;
-    return (uint32_t)std::max<uint64_t>(1, std::min(kHeadSlots / std::max<uint64_t>(t, 1), steps / 16));
+uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t all = tiles(m, t.tile) * tiles(n, t.tile), steps = tiles(k, kHeadK) * segments;
+    return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 16));
+}
+
+// The tiles of a product with the gradients: those that take less of the
+// device, a step of 1,024 small tiles at 1.08 times one of 256 large ones.
+// Both at their best: 16,384 x 131,072 x 1,024 products of bf16 take 3.9 ms
+// with large tiles and 4.2 with small ones, 8,191 x 32,768 x 512 ones 0.29
+// and 0.32; 4,096 x 5,003 x 256 ones of f32 70 us either way. (The scores and
+// pairs keep the small ones: four workgroups on a CU hide each other's
+// exponentials and stores. 16,384 x 32,768 pairs of 1,024 take 1.34 ms against
+// 1.35 with large ones, 4,096 x 5,003 ones of 256 in f32 84 us against 119.)
+const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t steps = tiles(k, kHeadK) * segments;
+    auto cost = [&](const HeadTiling &t, double step) {
+        const uint64_t shares = head_splits(t, m, n, k, segments);
+        return (double)(tiles(tiles(m, t.tile) * tiles(n, t.tile) * shares, t.slots) * tiles(steps, shares)) * step;
+    };
+    return cost(kTile256, 1.0) <= cost(kTile128, 1.08) ? kTile256 : kTile128;
 }
 
 struct HeadPlan {
@@ -327,11 +355,12 @@ struct HeadPlan {
     uint64_t parts, segments, chunks;
     bool lay;  // h and w are laid out in chunks whatever their rows
     uint64_t piece, pieces;
+    const HeadTiling *by_h, *by_w;  // the tiles of the products with the gradients
     uint32_t splits_h, splits_w;
     bool sum_h;  // dh is summed from f32 parts
     float *part_max, *part_sum, *label_margin, *lse2, *part_db, *dh, *dw;
     int32_t *part_best;
-    uint16_t *h, *w, *g;
+    char *h, *w, *g;
     uint32_t *keep;
     uint64_t bytes;
 };
@@ -353,17 +382,18 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.segments = dtype == HBR_F32 ? 6 : 1;
     q.chunks = tiles(dim, 32);
     q.lay = dtype == HBR_F32 || n >= kLayRows;
-    const uint64_t class_tiles = tiles(classes, kHeadTile);
+    const uint64_t class_tiles = tiles(classes, kTile128.tile);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
-        // up to sixteen waves on each of 256 CUs
-        const uint64_t groups = tiles(n, 32), cols = tiles(dim, 32);
-        q.score_blocks = (uint32_t)std::min<uint64_t>(tiles(groups, 4), 1024);
-        q.shares = (uint32_t)std::max<uint64_t>(1, std::min(groups, tiles(4096, cols)));
+        // groups of 32 rows, evenly: at most 4,096 waves of scores, and 2,048
+        // of products, which is what their registers let run at once
+        const uint64_t groups = std::max<uint64_t>(1, tiles(n, 32)), cols = tiles(dim, 32);
+        q.score_blocks = (uint32_t)tiles(tiles(groups, tiles(groups, 4096)), 4);
+        q.shares = (uint32_t)tiles(groups, tiles(groups, std::max<uint64_t>(1, 2048 / cols)));
         q.g_stride = up(classes, 16);
         if (gradient) {
-            q.g = w.take<uint16_t>(n * q.g_stride * (dtype == HBR_F32 ? 2 : 1));
+            q.g = w.take<char>(n * q.g_stride * (dtype == HBR_F32 ? 4 : 2));
             q.keep = w.take<uint32_t>(groups);
             q.part_db = w.take<float>(q.score_blocks * 4ull * classes);
             q.dw = w.take<float>(q.shares * classes * dim);
@@ -376,19 +406,21 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.part_best = w.take<int32_t>(class_tiles * n);
     q.label_margin = w.take<float>(n);
     q.lse2 = w.take<float>(n);
-    q.h = w.take<uint16_t>(q.parts * n * q.chunks * 32);
-    q.w = w.take<uint16_t>(q.parts * classes * q.chunks * 32);
+    q.h = w.take<char>(q.parts * q.chunks * chunk_bytes(n));
+    q.w = w.take<char>(q.parts * q.chunks * chunk_bytes(classes));
     if (gradient) {
         // the pieces as even as whole tiles allow
         const uint64_t row_bytes = std::max<uint64_t>(n, 1) * 2 * q.parts;
-        q.pieces = tiles(classes, std::max<uint64_t>(kHeadTile, kPieceBytes / row_bytes / kHeadTile * kHeadTile));
-        q.piece = up(tiles(classes, q.pieces), kHeadTile);
+        q.pieces = tiles(classes, std::max<uint64_t>(256, kPieceBytes / row_bytes / 256 * 256));
+        q.piece = up(tiles(classes, q.pieces), 256);
         q.pieces = tiles(classes, q.piece);
-        q.splits_h = head_splits(n, dim, q.piece, q.segments);
-        q.splits_w = head_splits(q.piece, dim, n, q.segments);
+        q.by_h = &head_tiling(n, dim, q.piece, q.segments);
+        q.by_w = &head_tiling(q.piece, dim, n, q.segments);
+        q.splits_h = head_splits(*q.by_h, n, dim, q.piece, q.segments);
+        q.splits_w = head_splits(*q.by_w, q.piece, dim, n, q.segments);
         q.sum_h = q.splits_h > 1 || q.pieces > 1;
-        q.g = w.take<uint16_t>(q.parts * n * q.piece);
-        q.part_db = w.take<float>(tiles(n, kHeadTile) * q.piece);
+        q.g = w.take<char>(q.parts * (q.piece / 32) * chunk_bytes(n));
+        q.part_db = w.take<float>(tiles(n, kTile128.tile) * q.piece);
         if (q.sum_h) q.dh = w.take<float>(q.splits_h * n * dim);
         if (q.splits_w > 1) q.dw = w.take<float>(q.splits_w * q.piece * dim);
     }
@@ -474,10 +506,22 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         const std::string few = suffix + (classes > 32 ? "_2" : "_1");
         queue.launch(("hbr_few_scores_" + few).c_str(), dim3(q.score_blocks), threads, f);
         if (!gradient) return;
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, q.score_blocks * 4ull, classes, p.db, 1, classes, classes);
-        if (!p.dh && !p.dw) return;
-        queue.launch(("hbr_few_products_" + few).c_str(), dim3((uint32_t)tiles((uint64_t)q.shares * f.col_tiles, 4)), threads, f);
-        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.shares, classes * dim, p.dw, classes, dim, p.dw_stride);
+        if (p.dh || p.dw)
+            queue.launch(("hbr_few_products_" + few).c_str(), dim3((uint32_t)tiles((uint64_t)q.shares * f.col_tiles, 4)), threads, f);
+        if (p.dw || p.db) {
+            FewSumsArgs a{};
+            a.part_dw = p.dw ? q.dw : nullptr;
+            a.part_db = p.db ? q.part_db : nullptr;
+            a.dw = p.dw;
+            a.db = p.db;
+            a.dw_stride = p.dw_stride;
+            a.shares = q.shares;
+            a.waves = q.score_blocks * 4;
+            a.classes = (uint32_t)classes;
+            a.dim = (uint32_t)dim;
+            a.dw_blocks = p.dw ? (uint32_t)tiles(classes * dim, 16) : 0;
+            queue.launch(("hbr_few_sums_" + suffix).c_str(), dim3(a.dw_blocks + (p.db ? (uint32_t)tiles(classes, 16) : 0)), dim3(1024), a);
+        }
         return;
     }
     // the operands of the products
@@ -486,31 +530,32 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         uint64_t row, chunk, part;
         uint32_t cols;
     };
-    auto lay = [&](const void *src, uint64_t stride, uint64_t rows, uint16_t *to, bool always, const int32_t *labels) -> Laid {
+    auto lay = [&](const void *src, uint64_t stride, uint64_t rows, char *to, bool always, const int32_t *labels) -> Laid {
         if (rows == 1) stride = up(dim, 8);
         if (!always && head_in_place(src, stride, p))
             return {static_cast<const char *>(src), stride * 2, 64, 0, (uint32_t)dim};
         HeadPartsArgs a{};
         a.src = src;
         a.labels = labels;
-        a.dst = to;
+        a.dst = reinterpret_cast<uint16_t *>(to);
         a.rows = rows;
         a.src_stride = stride;
-        a.part = rows * q.chunks * 32;
+        a.chunk = chunk_bytes(rows) / 2;
+        a.part = q.chunks * a.chunk;
         a.cols = (uint32_t)dim;
         a.chunks = (uint32_t)q.chunks;
         queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.chunks * 4), threads, a);
-        return {reinterpret_cast<const char *>(to), 64, rows * 64, a.part * 2, (uint32_t)(q.chunks * 32)};
+        return {static_cast<const char *>(to), 64, a.chunk * 2, a.part * 2, (uint32_t)(q.chunks * 32)};
     };
     const Laid h = lay(p.h, p.h_stride, n, q.h, q.lay || p.dw, p.dw ? p.labels : nullptr);
     const Laid w = lay(p.w, p.w_stride, classes, q.w, q.lay, nullptr);
     auto set_a = [](HeadArgs &a, const Laid &o) { a.a = o.p, a.a_row = o.row, a.a_chunk = o.chunk, a.a_part = o.part; };
     auto set_b = [](HeadArgs &a, const Laid &o) { a.b = o.p, a.b_row = o.row, a.b_chunk = o.chunk, a.b_part = o.part; };
-    auto product = [&](const std::string &kernel, HeadArgs a) {
-        a.m_tiles = (uint32_t)tiles(a.m, kHeadTile);
-        a.n_tiles = (uint32_t)tiles(a.n, kHeadTile);
+    auto product = [&](const std::string &kernel, const HeadTiling &t, HeadArgs a) {
+        a.m_tiles = (uint32_t)tiles(a.m, t.tile);
+        a.n_tiles = (uint32_t)tiles(a.n, t.tile);
         a.segments = (uint32_t)q.segments;
-        queue.launch(kernel.c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), threads, a);
+        queue.launch((kernel + t.name).c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), dim3((uint32_t)t.threads), a);
     };
     HeadArgs z{};
     set_a(z, w);
@@ -526,7 +571,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     z.part_sum = q.part_sum;
     z.part_best = p.best ? q.part_best : nullptr;
     z.label_margin = q.label_margin;
-    product("hbr_head_scores", z);
+    product("hbr_head_scores", kTile128, z);
     HeadFinishArgs f{};
     f.part_max = q.part_max;
     f.part_sum = q.part_sum;
@@ -540,14 +585,14 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     f.best = p.best;
     f.rows = n;
     f.classes = classes;
-    f.tiles = (uint32_t)tiles(classes, kHeadTile);
+    f.tiles = (uint32_t)tiles(classes, kTile128.tile);
     queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, 64)), dim3(1024), f);
     if (!gradient) return;
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
         const uint64_t kc = std::min(q.piece, classes - k0);
         Laid wk = w;  // w from class k0 on, and its scores' gradients
         wk.p += k0 * w.row;
-        const Laid pairs{reinterpret_cast<const char *>(q.g), 64, n * 64, n * q.piece * 2, (uint32_t)q.piece};
+        const Laid pairs{static_cast<const char *>(q.g), 64, chunk_bytes(n), chunk_bytes(n) * (q.piece / 32), (uint32_t)q.piece};
         HeadArgs g{};
         set_a(g, h);
         set_b(g, wk);
@@ -564,10 +609,11 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         g.grad_scale = p.grad_scale;
         g.g = q.g;
         g.g_stride = q.piece;
-        g.g_part = n * q.piece;
+        g.g_chunk = pairs.chunk / 2;
+        g.g_part = pairs.part / 2;
         g.part_db = q.part_db;
-        product("hbr_head_pairs_" + suffix, g);
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kHeadTile), q.piece, p.db + k0, 1, kc, kc);
+        product("hbr_head_pairs_" + suffix, kTile128, g);
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kTile128.tile), q.piece, p.db + k0, 1, kc, kc);
         if (p.dw) {
             HeadArgs c{};
             set_a(c, pairs);
@@ -582,7 +628,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c = direct ? (void *)to : q.dw;
             c.c_stride = direct ? p.dw_stride : dim;
             c.c_split = q.piece * dim;
-            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", c);
+            product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", *q.by_w, c);
             if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, p.dw_stride);
         }
         if (p.dh) {
@@ -597,7 +643,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c_stride = q.sum_h ? dim : p.dh_stride;
             c.c_split = n * dim;
             c.accumulate = k0 != 0;
-            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", c);
+            product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", *q.by_h, c);
         }
     }
     if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);

@@ -71,12 +71,20 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
-#pragma unroll 4
-        for (uint32_t k0 = 0; k0 < a.dim; k0 += F::kStep) {
-            const uint32_t k = k0 + lane / 32 * F::kEach;
-            const typename F::Frag fh = few_row<F>(h, k, a.dim);
+        constexpr int kAhead = 4;  // loads of as many steps in flight
+        for (uint32_t k0 = 0; k0 < a.dim; k0 += kAhead * F::kStep) {
+            typename F::Frag fh[kAhead], fw[kAhead][KT];
 #pragma unroll
-            for (int t = 0; t < KT; t++) acc[t] = F::mul(few_row<F>(w[t], k, a.dim), fh, acc[t]);
+            for (int u = 0; u < kAhead; u++) {
+                const uint32_t k = k0 + u * F::kStep + lane / 32 * F::kEach;
+                fh[u] = few_row<F>(h, k, a.dim);
+#pragma unroll
+                for (int t = 0; t < KT; t++) fw[u][t] = few_row<F>(w[t], k, a.dim);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; u++)
+#pragma unroll
+                for (int t = 0; t < KT; t++) acc[t] = F::mul(fw[u][t], fh[u], acc[t]);
         }
         const int32_t y = a.labels && in ? a.labels[r] : -1;
         float top = -INFINITY, at_label = 0.0f;
@@ -225,6 +233,30 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
         }
 }
 
+// dw and db from their parts: a workgroup takes 16 cells, its 64 groups of 16
+// lanes an even share of the parts each, joined in order.
+template <typename E>
+__device__ __forceinline__ void few_sums(const FewSumsArgs &a) {
+    __shared__ float sum_of[64][16];
+    const bool dw = blockIdx.x < a.dw_blocks;
+    const uint32_t lane = threadIdx.x % 16, group = threadIdx.x / 16;
+    const uint32_t cells = dw ? a.classes * a.dim : a.classes, parts = dw ? a.shares : a.waves;
+    const uint32_t i = (dw ? blockIdx.x : blockIdx.x - a.dw_blocks) * 16 + lane;
+    const uint32_t p0 = (uint32_t)((uint64_t)parts * group / 64), p1 = (uint32_t)((uint64_t)parts * (group + 1) / 64);
+    float s = 0.0f;
+    if (i < cells) {
+        const float *part = (dw ? a.part_dw : a.part_db) + i;
+#pragma unroll 8
+        for (uint32_t p = p0; p < p1; p++) s += part[(uint64_t)p * cells];
+    }
+    sum_of[group][lane] = s;
+    __syncthreads();
+    if (group || i >= cells) return;
+    for (int g = 1; g < 64; g++) s += sum_of[g][lane];
+    if (dw) static_cast<typename E::type *>(a.dw)[i / a.dim * a.dw_stride + i % a.dim] = E::down(s);
+    else a.db[i] = s;
+}
+
 }  // namespace hbr
 
 using namespace hbr;
@@ -236,3 +268,5 @@ HBR_FEW(f32_1, FewF32, 1)
 HBR_FEW(f32_2, FewF32, 2)
 HBR_FEW(bf16_1, FewBf16, 1)
 HBR_FEW(bf16_2, FewBf16, 2)
+extern "C" __global__ __launch_bounds__(1024) void hbr_few_sums_f32(FewSumsArgs a) { few_sums<F32>(a); }
+extern "C" __global__ __launch_bounds__(1024) void hbr_few_sums_bf16(FewSumsArgs a) { few_sums<Bf16>(a); }

@@ -18,7 +18,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr int kTile = (int)kHeadTile, kHeadWaves = 4;
 constexpr int kPairsMore = 2048;  // LDS of the pairs beyond the stages
 constexpr uint32_t kNowhere = 0x80000000u;  // past every buffer: reads as zero
 
@@ -56,17 +55,17 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
 // 64 bytes one behind the other), and 16 rows of a chunk are the 1 KiB that
 // one load of a wave fills; plain rows are the same with other steps.
 //
-// A tile is kTile rows x kHeadK, or, transposed, kHeadK rows x kTile in four
-// chunks, filled by 16-byte loads that go to LDS without registers. A wave's
+// A tile is 32 W rows x kHeadK (W waves), or, transposed, kHeadK rows x 32 W
+// in W chunks, filled by 16-byte loads that go to LDS without registers. A wave's
 // load fills LDS in lane order, so the layout is that of the loads. Of a tile
 // read along its rows the 16-byte pieces of a row are exchanged by their
 // source addresses: a piece's place is xored with its row's bits, so that the
 // 16 lanes that LDS serves at once meet all 64 banks. The transposing reads
 // meet them anyway (four rows of 64 bytes).
-template <bool T>
+template <bool T, int W>
 struct Operand {
-    static constexpr int kBytes = kTile * kHeadK * 2;
-    static constexpr int kLoads = kBytes / 1024 / kHeadWaves;  // a wave's, a step
+    static constexpr int kBytes = 32 * W * kHeadK * 2;
+    static constexpr int kLoads = kBytes / 1024 / W;  // a wave's, a step
     uint64_t at, step;      // where the wave's next step begins, and from step to step
     uint32_t off[kLoads];   // a lane's source, bytes from there
     uint32_t k_at[kLoads];  // and its first k within the step (not transposed)
@@ -88,7 +87,7 @@ struct Operand {
                 k_at[j] = piece * 8;
             }
         }
-        static_assert(kLoads == 2 && kTile == 32 * kHeadWaves, "a wave loads a chunk's 32 rows");
+        static_assert(kLoads == 2, "a wave loads a chunk's 32 rows");
     }
     // To step s of the operand at p.
     __device__ __forceinline__ void seek(const void *p, uint64_t row_step, uint64_t chunk_step, uint32_t first, uint32_t s) {
@@ -147,10 +146,11 @@ struct Operand {
 constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
 constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
 
-// A workgroup's tile of the product: kTile x kTile, 2 x 2 waves, the operands
-// of two steps in LDS.
+// A workgroup's tile of the product: 32 W x 32 W of W waves, 2 x W / 2, the
+// operands of two steps in LDS.
+template <int W>
 struct HeadTile {
-    static constexpr int kM = kTile, kN = kTile, kWavesM = 2, kWavesN = 2, kThreads = kHeadWaves * kWave;
+    static constexpr int kW = W, kM = 32 * W, kN = 32 * W, kWavesM = 2, kWavesN = W / 2, kThreads = W * kWave;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN, kI = kWaveM / 32, kJ = kWaveN / 32;
     static constexpr int kStage = (kM + kN) * kHeadK * 2, kLds = 2 * kStage;
     uint32_t m0, n0, split;  // the tile's first row and column, and its share of the steps
@@ -158,13 +158,13 @@ struct HeadTile {
     f32x16 acc[kI][kJ];
     uint32_t wave_m, wave_n;
 };
-using Tile = HeadTile;
 
 __device__ __forceinline__ uint32_t row_of(int e) { return 8 * (e / 4) + 4 * (lane_id() / 32) + e % 4; }
 
 // A workgroup's tile: neighbours in the launch go to different XCDs, so each
 // XCD takes a contiguous share of the tiles, in groups of eight rows of tiles
 // whose operands its L2 holds.
+template <typename Tile>
 __device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
     const uint32_t all = gridDim.x, per = all / 8, rest = all % 8, xcd = blockIdx.x % 8;
     uint32_t id = xcd * per + min(xcd, rest) + blockIdx.x / 8;
@@ -186,10 +186,10 @@ __device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
 // last sixteenth's are in registers when the waves meet, so that the next
 // step's loads may overwrite its stage and its first fragments be read
 // behind the meeting, both under the last sixteenth's products.
-template <bool AT, bool BT>
+template <bool AT, bool BT, typename Tile>
 __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile &t, const int32_t *a_labels = nullptr) {
-    using A = Operand<AT>;
-    using B = Operand<BT>;
+    using A = Operand<AT, Tile::kW>;
+    using B = Operand<BT, Tile::kW>;
     constexpr int kI = Tile::kI, kJ = Tile::kJ, kSixteenths = kHeadK / 16;
     A oa;
     B ob;
@@ -269,6 +269,7 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
 // m: classes, n: rows. A lane holds its wave's classes of kJ rows: maxima and
 // sums stay in its registers but for the other half of the wave and the other
 // waves of the same rows.
+template <typename Tile>
 __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     __shared__ float bias[Tile::kM];
     __shared__ float top_of[Tile::kWavesM][Tile::kN], sum_of[Tile::kWavesM][Tile::kN];
@@ -342,7 +343,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
 // class's sum over the rows stays in its registers; a row whose label is below
 // 0 is read as zeros and has no gradient. Past the classes g is zero up to its
 // stride.
-template <int Parts>
+template <typename Tile, int Parts>
 __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
     __shared__ float lse_of[Tile::kM], by_of[Tile::kM];
     __shared__ int32_t label_of[Tile::kM];
@@ -407,7 +408,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
     // the tile's, so that the wave's two rows of a write meet different banks.
     constexpr int kHalves = Parts == 1 ? 1 : 2, kSize = Parts == 1 ? 2 : 4, kI = Tile::kI / kHalves;
     constexpr uint32_t kRow = Tile::kN * kSize + 16, kRows = Tile::kM / kHalves, kWaveRows = Tile::kWaveM / kHalves;
-    static_assert(kRows * kRow <= Tile::kLds + kPairsMore, "the pairs fit the stages");
+    static_assert(kRows * kRow <= Tile::kLds + kPairsMore, "the pairs fit LDS");
 #pragma unroll
     for (int half = 0; half < kHalves; half++) {
         if (half) __syncthreads();
@@ -430,7 +431,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
             const uint32_t chunk = i / (kRows * 4), m = i / 4 % kRows, col = chunk * 32 + i % 4 * 8;
             const uint64_t r = t.m0 + m / kWaveRows * Tile::kWaveM + half * kWaveRows + m % kWaveRows;
             if (r >= a.m || t.n0 + col >= a.g_stride) continue;
-            uint16_t *g = static_cast<uint16_t *>(a.g) + ((uint64_t)(t.n0 / 32 + chunk) * a.m + r) * 32 + i % 4 * 8;
+            uint16_t *g = static_cast<uint16_t *>(a.g) + (t.n0 / 32 + chunk) * a.g_chunk + r * 32 + i % 4 * 8;
             if constexpr (Parts == 1) {
                 *reinterpret_cast<i32x4 *>(g) = *reinterpret_cast<const i32x4 *>(lds + m * kRow + col * 2);
             } else {
@@ -462,7 +463,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
 // ---- the products with the gradients ---------------------------------------------------------------
 
 // E: what c holds: f32 sums (a share's, added to or not) or the result.
-template <typename E, bool AT>
+template <typename Tile, typename E, bool AT>
 __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
     using T = typename E::type;
     Tile t;
@@ -576,7 +577,7 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
         }
 #pragma unroll
         for (int q = 0; q < Parts; q++)
-            *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + q * a.part + (chunk * a.rows + r) * 32 + in % 4 * 8) = out[q];
+            *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + q * a.part + chunk * a.chunk + r * 32 + in % 4 * 8) = out[q];
     }
 }
 
@@ -584,18 +585,22 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
 
 using namespace hbr;
 
-#define HBR_HEAD(name, at_once, more, ...)                                                       \
-    extern "C" __global__ __launch_bounds__(Tile::kThreads, at_once) void name(HeadArgs a) {     \
-        __shared__ __align__(1024) char lds[Tile::kLds + more];                         \
-        __VA_ARGS__(a, lds);                                                            \
+// waves: a SIMD's, at least
+#define HBR_HEAD(name, W, waves, more, ...)                                                       \
+    extern "C" __global__ __launch_bounds__(HeadTile<W>::kThreads, waves) void name(HeadArgs a) { \
+        __shared__ __align__(1024) char lds[HeadTile<W>::kLds + more];                            \
+        __VA_ARGS__(a, lds);                                                                      \
     }
-HBR_HEAD(hbr_head_scores, 3, 0, head_scores)
-HBR_HEAD(hbr_head_pairs_bf16, 4, kPairsMore, head_pairs<1>)
-HBR_HEAD(hbr_head_pairs_f32, 4, kPairsMore, head_pairs<3>)
-HBR_HEAD(hbr_head_dh_part, 4, 0, head_sums<F32, false>)
-HBR_HEAD(hbr_head_dh_bf16, 4, 0, head_sums<Bf16, false>)
-HBR_HEAD(hbr_head_dw_part, 4, 0, head_sums<F32, true>)
-HBR_HEAD(hbr_head_dw_bf16, 4, 0, head_sums<Bf16, true>)
+#define HBR_HEADS(suffix, W, waves)                                                                 \
+    HBR_HEAD(hbr_head_dh_part_##suffix, W, waves, 0, head_sums<HeadTile<W>, F32, false>)            \
+    HBR_HEAD(hbr_head_dh_bf16_##suffix, W, waves, 0, head_sums<HeadTile<W>, Bf16, false>)           \
+    HBR_HEAD(hbr_head_dw_part_##suffix, W, waves, 0, head_sums<HeadTile<W>, F32, true>)             \
+    HBR_HEAD(hbr_head_dw_bf16_##suffix, W, waves, 0, head_sums<HeadTile<W>, Bf16, true>)
+HBR_HEAD(hbr_head_scores_128, 4, 3, 0, head_scores<HeadTile<4>>)
+HBR_HEAD(hbr_head_pairs_bf16_128, 4, 4, kPairsMore, head_pairs<HeadTile<4>, 1>)
+HBR_HEAD(hbr_head_pairs_f32_128, 4, 4, kPairsMore, head_pairs<HeadTile<4>, 3>)
+HBR_HEADS(256, 8, 2)
+HBR_HEADS(128, 4, 4)
 
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_f32(HeadSumArgs a) { head_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_bf16(HeadSumArgs a) { head_sum<Bf16>(a); }
@@ -619,9 +624,23 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
         best = m > top ? b : m == top ? min(best, b) : best;
         top = both;
     };
+    constexpr uint32_t kAhead = 8;
+    const uint32_t end = min(a.tiles, (wave + 1) * share);
     if (r < a.rows)
-        for (uint32_t t = wave * share; t < min(a.tiles, (wave + 1) * share); t++)
-            join(a.part_max[t * a.rows + r], a.part_sum[t * a.rows + r], a.part_best ? a.part_best[t * a.rows + r] : 0);
+        for (uint32_t t0 = wave * share; t0 < end; t0 += kAhead) {
+            float m[kAhead], s[kAhead];
+            int32_t b[kAhead];
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; u++) {
+                const uint64_t at = min(t0 + u, end - 1) * a.rows + r;
+                m[u] = a.part_max[at];
+                s[u] = a.part_sum[at];
+                b[u] = a.part_best ? a.part_best[at] : 0;
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; u++)
+                if (t0 + u < end) join(m[u], s[u], b[u]);
+        }
     top_of[wave][lane] = top;
     sum_of[wave][lane] = sum;
     best_of[wave][lane] = best;

@@ -80,6 +80,23 @@ def test_heads_with_malformed_records_are_invalid(bad, said):
     assert A.lib().hbr_softmax_head(0, C.byref(p), 1 << 20, 1 << 40, None) == A.INVALID and said in A.last_error()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_workspaces_of_all_sizes_are_named(dtype):
+    """From no rows to the largest, with every count of classes on either
+    side of a tile."""
+    for n in (0, 1, 31, 1023, 1024, 70_000, (1 << 31) - 1):
+        for classes in (1, 2, 64, 65, 128, 129, 131_072):
+            for dim in (1, 7, 64, 1024, 70_000):
+                score = hb.softmax_head_workspace(n, classes, dim, dtype, gradient=False)
+                assert score <= hb.softmax_head_workspace(n, classes, dim, dtype)
+    for n in (0, 1, 16_383, 1 << 20):
+        for columns in (0, 1, 3, 1000):
+            for rows in (0, 1, 512, 1 << 20):
+                assert hb.leaf_embedding_grad_workspace(n, columns, rows, 33, dtype) >= 0
+    for n in (0, 1, 96, 97, 1 << 20):
+        assert hb.clip_gradients_workspace(n) >= 8 * n // 96
+
+
 def test_a_workspace_that_is_missing_short_or_misaligned_is_invalid():
     L, ok = A.lib(), 1 << 20
     need = hb.softmax_head_workspace(3, 5, 8, "bfloat16")
