@@ -1101,9 +1101,9 @@ struct LookupColumnArgs {
     uint32_t slice_vecs;
 };
 
-// Entries of one sort tile (hbr_sort_*): 256 threads x 16.
-constexpr uint32_t kSortTile = 4096;
-constexpr uint32_t kSortBits = 8;
+// The sort's digits, and the most entries that one workgroup sorts by itself.
+constexpr uint32_t kSortBits = 9;
+constexpr uint32_t kSortSmall = 4096;
 constexpr uint32_t kSortDigits = 1u << kSortBits;
 
 // The table gradient: the ids' entries (r, t) sorted by table row, stable.
@@ -1132,7 +1132,6 @@ struct LookupSumArgs {
     const void *dout;
     const float *scale;
     void *dtable;
-    uint32_t *start;          // table_rows + 1: each table row's first entry
     float *part;              // [chunk][2][dim]
     uint64_t table_rows;
     uint64_t dout_stride;
@@ -1141,8 +1140,10 @@ struct LookupSumArgs {
     uint32_t columns;
     uint32_t dim;
     uint32_t vecs;
-    uint32_t chunk;           // entries a wave
+    uint32_t wide;            // lanes a row: a power of two that covers the vectors, at most 64
+    uint32_t chunk;           // entries a group of lanes
     uint32_t chunks;
+    uint32_t row_blocks;      // hbr_lookup_finish: the blocks that write rows of no entries
 };
 
 // The head's products C[m][n] = sum_k A(m, k) B(n, k) of bf16 operands, in

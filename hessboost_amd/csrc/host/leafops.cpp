@@ -153,8 +153,8 @@ struct LookupPlan {
     uint32_t blocks, block_rows;
     // by sorting
     uint64_t n;  // entries
-    uint32_t tiles, passes, chunk, chunks;
-    uint32_t *key[2], *val[2], *hist, *total, *start;
+    uint32_t tile, tiles, passes, chunk, chunks;
+    uint32_t *key[2], *val[2], *hist, *total;
     float *part;
     uint64_t bytes;
 };
@@ -184,13 +184,16 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
         q.bytes = w.used;
         return q;
     }
-    q.tiles = (uint32_t)((q.n + kSortTile - 1) / kSortTile);
+    // small tiles where large ones would be too few for the device
+    q.tile = q.n < (1u << 20) ? 512 : 4096;
+    q.tiles = (uint32_t)((q.n + q.tile - 1) / q.tile);
     // keys run from 0 to table_rows
     uint32_t bits = 1;
     while (bits < 32 && (p.table_rows >> bits)) bits++;
     q.passes = (bits + kSortBits - 1) / kSortBits;
-    // about 8,192 waves, 32 to 512 entries each
-    q.chunk = (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(32, up(q.n / 8192, 32)));
+    // 8 to 64 entries a chunk, for about 4,096 waves of 16-byte vectors
+    const uint64_t waves = (p.dim * (p.dtype == HBR_F32 ? 4 : 2) + 1023) / 1024;
+    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(8, up(q.n * waves / 4096, 8)));
     q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
     for (int b = 0; b < 2; b++) {
         q.key[b] = w.take<uint32_t>(q.n);
@@ -198,7 +201,6 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     }
     q.hist = w.take<uint32_t>((uint64_t)kSortDigits * q.tiles);
     q.total = w.take<uint32_t>(kSortDigits);
-    q.start = w.take<uint32_t>(p.table_rows + 1);
     q.part = w.take<float>((uint64_t)q.chunks * 2 * p.dim);
     q.bytes = w.used;
     return q;
@@ -255,7 +257,9 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
         return;
     }
     int from = 0;
-    for (uint32_t pass = 0; pass < q.passes && q.n; pass++) {
+    const std::string steps = q.tile == 512 ? "_2" : "_16";
+    const bool small = q.n <= kSortSmall;
+    for (uint32_t pass = 0; pass < (small ? 1 : q.passes) && q.n; pass++) {
         LookupSortArgs a{};
         a.ids = p.ids;
         a.offset = p.offset;
@@ -271,10 +275,14 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
         a.vals_out = q.val[from ^ 1];
         a.hist = q.hist;
         a.total = q.total;
-        queue.launch("hbr_sort_count", dim3(q.tiles), dim3(256), a);
-        queue.launch("hbr_sort_scan", dim3(kSortDigits), dim3(256), a);
-        queue.launch("hbr_sort_scatter", dim3(q.tiles), dim3(256), a);
         from ^= 1;
+        if (small) {
+            queue.launch("hbr_sort_small", dim3(1), dim3(1024), a);
+            break;
+        }
+        queue.launch(("hbr_sort_count" + steps).c_str(), dim3(q.tiles), dim3(256), a);
+        queue.launch("hbr_sort_scan", dim3(kSortDigits), dim3(256), a);
+        queue.launch(("hbr_sort_scatter" + steps).c_str(), dim3(q.tiles), dim3(256), a);
     }
     LookupSumArgs a{};
     a.keys = q.key[from];
@@ -282,7 +290,6 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     a.dout = dout;
     a.scale = p.scale;
     a.dtable = dtable;
-    a.start = q.start;
     a.part = q.part;
     a.table_rows = p.table_rows;
     a.dout_stride = p.out_stride;
@@ -291,11 +298,14 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     a.columns = p.n_columns;
     a.dim = p.dim;
     a.vecs = p.dim / v;
+    a.wide = 1;
+    while (a.wide < a.vecs && a.wide < kWaveLanes) a.wide *= 2;
     a.chunk = q.chunk;
     a.chunks = q.chunks;
-    queue.launch("hbr_lookup_starts", blocks(p.table_rows + 1), dim3(256), a);
-    queue.launch(("hbr_lookup_sum_" + suffix).c_str(), dim3((q.chunks + 3) / 4), dim3(256), a);
-    queue.launch(("hbr_lookup_finish_" + suffix).c_str(), blocks(p.table_rows * a.vecs), dim3(256), a);
+    const uint32_t groups = 256 / a.wide, slices = (a.vecs + a.wide - 1) / a.wide;
+    queue.launch(("hbr_lookup_sum_" + suffix).c_str(), dim3((q.chunks + groups - 1) / groups, slices), dim3(256), a);
+    a.row_blocks = (uint32_t)((p.table_rows + 4 * 63 - 1) / (4 * 63));
+    queue.launch(("hbr_lookup_finish_" + suffix).c_str(), dim3(a.row_blocks + (q.chunks + groups - 1) / groups), dim3(256), a);
 }
 
 // ---- the softmax head ------------------------------------------------------------------

@@ -404,53 +404,51 @@ HBR_EMBED(bf16_4, Bf16, 4)
 HBR_EMBED(bf16_2, Bf16, 2)
 HBR_EMBED(bf16_1, Bf16, 1)
 
+namespace hbr {
+
 // A tile's entries counted by the pass's digit (integer counts: any order).
-extern "C" __global__ __launch_bounds__(256) void hbr_sort_count(LookupSortArgs a) {
+template <uint32_t Steps>
+__device__ __forceinline__ void sort_count(const LookupSortArgs &a) {
     __shared__ uint32_t count[kSortDigits];
-    count[threadIdx.x] = 0;
+    for (uint32_t d = threadIdx.x; d < kSortDigits; d += 256) count[d] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * kSortTile;
-    for (uint32_t j = 0; j < kSortTile / 256; j++) {
+    const uint32_t base = blockIdx.x * (Steps * 256);
+#pragma unroll
+    for (uint32_t j = 0; j < Steps; j++) {
         const uint32_t i = base + j * 256 + threadIdx.x;
         if (i < a.n) atomicAdd(&count[(sort_key(a, i) >> a.shift) & (kSortDigits - 1)], 1u);
     }
     __syncthreads();
-    a.hist[(uint64_t)threadIdx.x * a.tiles + blockIdx.x] = count[threadIdx.x];
-}
-
-// One workgroup a digit: its tiles' counts to places, and the digit's total.
-extern "C" __global__ __launch_bounds__(256) void hbr_sort_scan(LookupSortArgs a) {
-    uint32_t *h = a.hist + (uint64_t)blockIdx.x * a.tiles;
-    uint32_t run = 0;
-    for (uint32_t t0 = 0; t0 < a.tiles; t0 += 256) {
-        const uint32_t t = t0 + threadIdx.x;
-        const uint32_t v = t < a.tiles ? h[t] : 0;
-        uint32_t all;
-        const uint32_t at = block_exclusive_scan<256>(v, &all);
-        if (t < a.tiles) h[t] = run + at;
-        run += all;
-    }
-    if (threadIdx.x == 0) a.total[blockIdx.x] = run;
+    for (uint32_t d = threadIdx.x; d < kSortDigits; d += 256) a.hist[(uint64_t)d * a.tiles + blockIdx.x] = count[d];
 }
 
 // A tile's entries to their places, in order within a digit: wave w holds the
 // tile's w-th quarter, 64 entries a step; a lane's rank is the lanes below it
-// with its digit (eight ballots), behind the wave's earlier steps.
-extern "C" __global__ __launch_bounds__(256) void hbr_sort_scatter(LookupSortArgs a) {
-    constexpr uint32_t kWaves = 256 / kWave, kSteps = kSortTile / 256;
+// with its digit (a ballot a bit), behind the wave's earlier steps.
+template <uint32_t Steps>
+__device__ __forceinline__ void sort_scatter(const LookupSortArgs &a) {
+    constexpr uint32_t kWaves = 256 / kWave, kEach = kSortDigits / 256;
     __shared__ uint32_t count[kWaves][kSortDigits];
-    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, d = threadIdx.x;
-    for (uint32_t w = 0; w < kWaves; w++) count[w][d] = 0;
-    uint32_t all;
-    const uint32_t digit_at = block_exclusive_scan<256>(a.total[d], &all) + a.hist[(uint64_t)d * a.tiles + blockIdx.x];
-    __syncthreads();
-    const uint32_t base = blockIdx.x * kSortTile + wave * (kSortTile / kWaves);
-    uint32_t key[kSteps], rank[kSteps];
+    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
+    for (uint32_t i = threadIdx.x; i < kWaves * kSortDigits; i += 256) (&count[0][0])[i] = 0;
+    // where the digits of this thread begin, over all tiles and for this one
+    uint32_t total[kEach], sum = 0, all;
 #pragma unroll
-    for (uint32_t j = 0; j < kSteps; j++) {
+    for (uint32_t q = 0; q < kEach; q++) {
+        total[q] = a.total[threadIdx.x * kEach + q];
+        sum += total[q];
+    }
+    uint32_t digit_at = block_exclusive_scan<256>(sum, &all);
+    const uint32_t base = blockIdx.x * (Steps * 256) + wave * (Steps * kWave);
+    uint32_t key[Steps], rank[Steps];
+#pragma unroll
+    for (uint32_t j = 0; j < Steps; j++) {
         const uint32_t i = base + j * kWave + lane;
-        const bool in = i < a.n;
-        key[j] = in ? sort_key(a, i) : 0;
+        key[j] = i < a.n ? sort_key(a, i) : 0;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < Steps; j++) {
+        const bool in = base + j * kWave + lane < a.n;
         const uint32_t digit = (key[j] >> a.shift) & (kSortDigits - 1);
         uint64_t same = __ballot(in);
 #pragma unroll
@@ -468,15 +466,20 @@ extern "C" __global__ __launch_bounds__(256) void hbr_sort_scatter(LookupSortArg
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    uint32_t at = digit_at;
-    for (uint32_t w = 0; w < kWaves; w++) {
-        const uint32_t c = count[w][d];
-        count[w][d] = at;
-        at += c;
+#pragma unroll
+    for (uint32_t q = 0; q < kEach; q++) {
+        const uint32_t d = threadIdx.x * kEach + q;
+        uint32_t at = digit_at + a.hist[(uint64_t)d * a.tiles + blockIdx.x];
+        digit_at += total[q];
+        for (uint32_t w = 0; w < kWaves; w++) {
+            const uint32_t c = count[w][d];
+            count[w][d] = at;
+            at += c;
+        }
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t j = 0; j < kSteps; j++) {
+    for (uint32_t j = 0; j < Steps; j++) {
         const uint32_t i = base + j * kWave + lane;
         if (i >= a.n) continue;
         const uint32_t p = count[wave][(key[j] >> a.shift) & (kSortDigits - 1)] + rank[j];
@@ -485,100 +488,183 @@ extern "C" __global__ __launch_bounds__(256) void hbr_sort_scatter(LookupSortArg
     }
 }
 
-// Where each table row's entries begin (the first entry whose key is not below it).
-extern "C" __global__ __launch_bounds__(256) void hbr_lookup_starts(LookupSumArgs a) {
-    for (uint64_t v = (uint64_t)blockIdx.x * 256 + threadIdx.x; v <= a.table_rows; v += (uint64_t)gridDim.x * 256) {
-        uint32_t lo = 0, hi = a.n;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (a.keys[mid] < v) lo = mid + 1;
-            else hi = mid;
+}  // namespace hbr
+
+extern "C" __global__ __launch_bounds__(256) void hbr_sort_count_2(LookupSortArgs a) { sort_count<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_sort_count_16(LookupSortArgs a) { sort_count<16>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_sort_scatter_2(LookupSortArgs a) { sort_scatter<2>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_sort_scatter_16(LookupSortArgs a) { sort_scatter<16>(a); }
+
+// One workgroup a digit: its tiles' counts to places, and the digit's total.
+extern "C" __global__ __launch_bounds__(256) void hbr_sort_scan(LookupSortArgs a) {
+    uint32_t *h = a.hist + (uint64_t)blockIdx.x * a.tiles;
+    uint32_t run = 0;
+    for (uint32_t t0 = 0; t0 < a.tiles; t0 += 256) {
+        const uint32_t t = t0 + threadIdx.x;
+        const uint32_t v = t < a.tiles ? h[t] : 0;
+        uint32_t all;
+        const uint32_t at = block_exclusive_scan<256>(v, &all);
+        if (t < a.tiles) h[t] = run + at;
+        run += all;
+    }
+    if (threadIdx.x == 0) a.total[blockIdx.x] = run;
+}
+
+// Few entries, sorted in one workgroup: (key, entry) pairs are all different,
+// so that any sort gives their one order (bitonic).
+extern "C" __global__ __launch_bounds__(1024) void hbr_sort_small(LookupSortArgs a) {
+    __shared__ uint64_t pair[kSortSmall];
+    uint32_t size = 64;
+    while (size < a.n) size <<= 1;
+    for (uint32_t i = threadIdx.x; i < size; i += 1024)
+        pair[i] = i < a.n ? (uint64_t)sort_key(a, i) << 32 | i : ~0ull;
+    for (uint32_t k = 2; k <= size; k <<= 1)
+        for (uint32_t d = k / 2; d; d >>= 1) {
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < size / 2; i += 1024) {
+                const uint32_t low = i / d * 2 * d + i % d, high = low + d;
+                const uint64_t x = pair[low], y = pair[high];
+                if ((x > y) == ((low & k) == 0)) pair[low] = y, pair[high] = x;
+            }
         }
-        a.start[v] = lo;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.n; i += 1024) {
+        a.keys_out[i] = (uint32_t)(pair[i] >> 32);
+        a.vals_out[i] = (uint32_t)pair[i];
     }
 }
 
 namespace hbr {
 
-// One wave a chunk of the sorted entries. A run of equal keys is summed by
-// the wave's lane groups (each a row's vectors wide, every group an entry of
-// its own) and folded over the groups; a run inside the chunk is a table
-// row's whole sum and is written at once, one that reaches the chunk's start
-// or end leaves its part in f32.
+// A chunk of the sorted entries a group of lanes, a vector of the rows a lane:
+// eight entries' rows in flight, added up run by run of equal keys. A run that
+// the chunk holds whole is its table row's sum and is written at once, one
+// that reaches the chunk's start or end leaves its part in f32.
 template <typename E, int V>
 __device__ __forceinline__ void lookup_sum(const LookupSumArgs &a) {
     using T = typename E::type;
-    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
-    const uint32_t chunk = blockIdx.x * (256 / kWave) + wave;
-    if (chunk >= a.chunks) return;
-    const uint32_t valid = a.start[a.table_rows];
-    const uint32_t c0 = chunk * a.chunk;
-    const uint32_t c1 = min(c0 + a.chunk, valid);
-    uint32_t wide = 1;  // lanes a row: the power of two that covers its vectors, at most the wave
-    while (wide < a.vecs && wide < (uint32_t)kWave) wide <<= 1;
-    const uint32_t groups = kWave / wide, group = lane / wide, in_group = lane & (wide - 1);
-    for (uint32_t i = c0; i < c1;) {
-        const uint32_t key = a.keys[i];
-        const uint32_t first = a.start[key], end = a.start[key + 1];
-        const uint32_t e = min(end, c1);
-        const bool whole = first >= c0 && end <= c0 + a.chunk;
-        for (uint32_t c = in_group; c - in_group < a.vecs; c += wide) {
-            float acc[V] = {};
-            if (c < a.vecs) {
-                for (uint32_t j = i + group; j < e; j += groups) {
-                    const uint32_t entry = a.vals[j];
-                    const uint32_t r = entry / a.columns, t = entry - r * a.columns;
-                    const float s = a.scale ? a.scale[t] : 1.0f;
-                    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V> *>(static_cast<const T *>(a.dout) +
-                                                                             r * a.dout_stride + c * V);
+    constexpr uint32_t kAhead = 8, kNone = 0xffffffffu;
+    const uint32_t groups = 256 / a.wide, c = blockIdx.y * a.wide + (threadIdx.x & (a.wide - 1));
+    const uint32_t chunk = blockIdx.x * groups + threadIdx.x / a.wide;
+    if (chunk >= a.chunks || c >= a.vecs) return;
+    const uint32_t c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, a.n);
+    const uint32_t before = c0 ? a.keys[c0 - 1] : kNone, behind = c1 < a.n ? a.keys[c1] : kNone;
+    const T *dout = static_cast<const T *>(a.dout) + c * V;
+    uint32_t run = kNone, first = c0;  // the run's key, and where it begins in the chunk
+    float acc[V] = {};
+    auto flush = [&](uint32_t end) {
+        if (run >= a.table_rows) return;  // none, or the ids that add nothing
+        if ((first > c0 || run != before) && (end < c1 || run != behind)) {
+            Vec<T, V> out;
 #pragma unroll
-                    for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s, E::up(v.v[k]), acc[k]);
-                }
-            }
-            for (uint32_t d = wide; d < (uint32_t)kWave; d <<= 1)
+            for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
+            *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + run * a.dtable_stride + c * V) = out;
+        } else {
+            float *p = a.part + ((uint64_t)chunk * 2 + (first == c0 ? 0 : 1)) * a.dim + c * V;
 #pragma unroll
-                for (int k = 0; k < V; k++) acc[k] += __shfl_xor(acc[k], d, kWave);
-            if (group == 0 && c < a.vecs) {
-                if (whole) {
-                    Vec<T, V> out;
-#pragma unroll
-                    for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
-                    *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + key * a.dtable_stride + c * V) = out;
-                } else {
-                    float *p = a.part + ((uint64_t)chunk * 2 + (i == c0 ? 0 : 1)) * a.dim + c * V;
-#pragma unroll
-                    for (int k = 0; k < V; k++) p[k] = acc[k];
-                }
-            }
+            for (int k = 0; k < V; k++) p[k] = acc[k];
         }
-        i = e;
+    };
+    uint32_t key[kAhead], val[kAhead], next_key[kAhead], next_val[kAhead];
+    auto entries = [&](uint32_t at) {  // the eight from `at` on, one round ahead of their rows
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; u++) {
+            next_key[u] = at + u < c1 ? a.keys[at + u] : kNone;
+            next_val[u] = at + u < c1 ? a.vals[at + u] : 0;
+        }
+    };
+    entries(c0);
+    for (uint32_t i0 = c0; i0 < c1; i0 += kAhead) {
+        float s[kAhead];
+        Vec<T, V> v[kAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; u++) {
+            key[u] = next_key[u];
+            val[u] = next_val[u];
+            v[u] = Vec<T, V>{};
+            s[u] = 1.0f;
+            if (key[u] >= a.table_rows) continue;
+            const uint32_t r = a.columns == 1 ? val[u] : val[u] / a.columns;
+            if (a.scale) s[u] = a.scale[val[u] - r * a.columns];
+            v[u] = *reinterpret_cast<const Vec<T, V> *>(dout + r * a.dout_stride);
+        }
+        entries(i0 + kAhead);
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; u++) {
+            if (i0 + u >= c1) break;
+            if (key[u] != run) {
+                flush(i0 + u);
+                run = key[u];
+                first = i0 + u;
+#pragma unroll
+                for (int k = 0; k < V; k++) acc[k] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s[u], E::up(v[u].v[k]), acc[k]);
+        }
     }
+    flush(c1);
 }
 
-// The table rows that no chunk wrote: zeros where no entry is, the parts in
-// order where the entries lie in several chunks.
+// The first entry whose key is not below `key`.
+__device__ __forceinline__ uint32_t first_entry(const LookupSumArgs &a, uint64_t key) {
+    uint32_t low = 0, high = a.n;
+    while (low < high) {
+        const uint32_t mid = low + (high - low) / 2;
+        if (a.keys[mid] < key) low = mid + 1;
+        else high = mid;
+    }
+    return low;
+}
+
+// The table rows that no chunk wrote. The first blocks write zeros where no
+// entry is: a wave finds where the entries of 64 rows begin, a search a lane,
+// and has the ends of 63. The others join the parts of runs that reach over
+// chunks, in order: a group of lanes a chunk, for the run that begins in it
+// and goes on behind it.
 template <typename E, int V>
 __device__ __forceinline__ void lookup_finish(const LookupSumArgs &a) {
     using T = typename E::type;
-    const uint64_t cells = a.table_rows * a.vecs;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t v = i / a.vecs;
-        const uint32_t c = (uint32_t)(i - v * a.vecs) * V;
-        const uint32_t s = a.start[v], e = a.start[v + 1];
-        float acc[V] = {};
-        if (s < e) {
-            const uint32_t first = s / a.chunk, last = (e - 1) / a.chunk;
-            if (first == last) continue;
-            for (uint32_t q = first; q <= last; q++) {
-                const float *p = a.part + ((uint64_t)q * 2 + (q == first && s != q * a.chunk ? 1 : 0)) * a.dim + c;
+    const uint32_t lane = lane_id(), c0 = lane & (a.wide - 1), groups = kWave / a.wide;
+    T *dtable = static_cast<T *>(a.dtable);
+    if (blockIdx.x < a.row_blocks) {
+        const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + threadIdx.x / kWave) * (kWave - 1);
+        if (r0 >= a.table_rows) return;
+        const uint32_t at = first_entry(a, r0 + lane);
+        const uint32_t rows = (uint32_t)min((uint64_t)(kWave - 1), a.table_rows - r0);
+        const Vec<T, V> none{};
+        for (uint32_t j0 = 0; j0 < rows; j0 += groups) {
+            const uint32_t j = j0 + lane / a.wide;
+            const uint32_t s = __shfl(at, min(j, 63u), kWave), e = __shfl(at, min(j + 1, 63u), kWave);
+            if (j >= rows || s < e) continue;
+            for (uint32_t c = c0; c < a.vecs; c += a.wide)
+                *reinterpret_cast<Vec<T, V> *>(dtable + (r0 + j) * a.dtable_stride + c * V) = none;
+        }
+        return;
+    }
+    const uint32_t chunk = ((blockIdx.x - a.row_blocks) * 4 + threadIdx.x / kWave) * groups + lane / a.wide;
+    if (chunk + 1 >= a.chunks) return;  // nothing goes on behind the last
+    const uint32_t last = (chunk + 1) * a.chunk;  // the chunk is whole, another follows
+    const uint32_t key = a.keys[last - 1];
+    if (key >= a.table_rows || a.keys[last] != key) return;
+    const uint32_t start = first_entry(a, key), to = (first_entry(a, (uint64_t)key + 1) - 1) / a.chunk;
+    if (start < chunk * a.chunk) return;  // it began before
+    const uint32_t slot = start != chunk * a.chunk ? 1 : 0;
+    for (uint32_t c = c0; c < a.vecs; c += a.wide) {
+        float acc[V];
+        const float *p = a.part + ((uint64_t)chunk * 2 + slot) * a.dim + c * V;
 #pragma unroll
-                for (int k = 0; k < V; k++) acc[k] += p[k];
-            }
+        for (int k = 0; k < V; k++) acc[k] = p[k];
+#pragma unroll 8
+        for (uint32_t q = chunk + 1; q <= to; q++) {
+            p = a.part + (uint64_t)q * 2 * a.dim + c * V;
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[k] += p[k];
         }
         Vec<T, V> out;
 #pragma unroll
         for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
-        *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + v * a.dtable_stride + c) = out;
+        *reinterpret_cast<Vec<T, V> *>(dtable + key * a.dtable_stride + c * V) = out;
     }
 }
 
