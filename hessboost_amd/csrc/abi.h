@@ -1244,7 +1244,7 @@ struct HeadFinishArgs {
     uint64_t rows;
     uint64_t classes;
     uint32_t tiles;
-    uint32_t pad;
+    uint32_t wide;    // rows a workgroup
 };
 
 // dst[i] = sum over parts of part[p][i], rounded to the type.

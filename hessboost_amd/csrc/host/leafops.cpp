@@ -596,7 +596,10 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     f.rows = n;
     f.classes = classes;
     f.tiles = (uint32_t)tiles(classes, kTile128.tile);
-    queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, 64)), dim3(1024), f);
+    // fewer rows a workgroup where they would not fill the device
+    f.wide = 64;
+    while (f.wide > 1 && tiles(n, f.wide) < 256) f.wide /= 4;
+    queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, f.wide)), dim3(1024), f);
     if (!gradient) return;
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
         const uint64_t kc = std::min(q.piece, classes - k0);

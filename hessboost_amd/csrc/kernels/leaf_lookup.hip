@@ -204,9 +204,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
         asm volatile("" : "+v"(thread));
         const uint32_t lane = thread % kWave, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(thread / kWave));
         const uint32_t keys = (uint32_t)min((int64_t)kColumnKeys, hi - k0);
-#pragma unroll 1
-        for (uint32_t i = thread; i < kColumnWaves * kColumnKeys; i += kColumnThreads) (&count[0][0])[i] = 0;
-        __syncthreads();
+        for (uint32_t k = lane; k < keys; k += kWave) count[wave][k] = 0;  // its own: before its own counts
         const uint32_t wave_rows = (a.block_rows + kColumnThreads - 1) / kColumnThreads * kWave;
         uint32_t held[kColumnSteps];  // the key, and the rank in the upper half
         uint32_t bits = 0;
@@ -244,8 +242,8 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
         __syncthreads();
         // each key's total over the waves, their scan, and the waves' places
         uint32_t total = 0;
-        if (thread < kColumnKeys)
-#pragma unroll 4
+        if (thread < keys)
+#pragma unroll 8
             for (uint32_t w = 0; w < kColumnWaves; w++) total += count[w][thread];
         uint32_t upto = total;
 #pragma unroll 1
@@ -261,13 +259,18 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
             if (w == wave) at += all;
             all += wave_total[w];
         }
-        if (thread < kColumnKeys) {
-            start[thread] = at;
+        if (thread < kColumnKeys) start[thread] = at;
+        if (thread < keys) {
 #pragma unroll 1
-            for (uint32_t w = 0; w < kColumnWaves; w++) {
-                const uint32_t n = count[w][thread];
-                count[w][thread] = at;
-                at += n;
+            for (uint32_t w = 0; w < kColumnWaves; w += 8) {
+                uint32_t n[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) n[u] = count[w + u][thread];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; u++) {
+                    count[w + u][thread] = at;
+                    at += n[u];
+                }
             }
         }
         if (thread == 0) start[kColumnKeys] = all;

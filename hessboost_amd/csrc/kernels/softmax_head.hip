@@ -607,15 +607,17 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_sum_bf16(HeadSumArgs
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_f32(HeadPartsArgs a) { head_parts<F32, 3>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_head_parts_bf16(HeadPartsArgs a) { head_parts<Bf16, 1>(a); }
 
-// A row's tiles joined: 64 rows a workgroup, its 16 waves a share of the
-// class tiles each, in order within a wave and over the waves.
+// A row's tiles joined: a.wide rows a workgroup (a power of two, 64 at most),
+// a lane of a wave for each, the wave's other lanes and the 16 waves shares of
+// the class tiles, in order within a lane, over the lanes and over the waves.
 extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArgs a) {
     constexpr uint32_t kWaves = 16;
     __shared__ float top_of[kWaves][kWave], sum_of[kWaves][kWave];
     __shared__ int32_t best_of[kWaves][kWave];
-    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave;
-    const uint64_t r = (uint64_t)blockIdx.x * kWave + lane;
-    const uint32_t share = (a.tiles + kWaves - 1) / kWaves;
+    const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, in = lane & (a.wide - 1);
+    const uint64_t r = (uint64_t)blockIdx.x * a.wide + in;
+    const uint32_t lanes = kWave / a.wide, share = (a.tiles + kWaves * lanes - 1) / (kWaves * lanes);
+    const uint32_t first = (wave * lanes + lane / a.wide) * share, end = min(a.tiles, first + share);
     float top = -INFINITY, sum = 0.0f;
     int32_t best = 0x7fffffff;
     auto join = [&](float m, float s, int32_t b) {
@@ -625,9 +627,8 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
         top = both;
     };
     constexpr uint32_t kAhead = 8;
-    const uint32_t end = min(a.tiles, (wave + 1) * share);
     if (r < a.rows)
-        for (uint32_t t0 = wave * share; t0 < end; t0 += kAhead) {
+        for (uint32_t t0 = first; t0 < end; t0 += kAhead) {
             float m[kAhead], s[kAhead];
             int32_t b[kAhead];
 #pragma unroll
@@ -641,12 +642,14 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
             for (uint32_t u = 0; u < kAhead; u++)
                 if (t0 + u < end) join(m[u], s[u], b[u]);
         }
+    for (uint32_t d = a.wide; d < (uint32_t)kWave; d <<= 1)
+        join(__shfl_down(top, d, kWave), __shfl_down(sum, d, kWave), __shfl_down(best, d, kWave));
     top_of[wave][lane] = top;
     sum_of[wave][lane] = sum;
     best_of[wave][lane] = best;
     __syncthreads();
-    if (wave != 0 || r >= a.rows) return;
-    for (uint32_t w = 1; w < kWaves && w * share < a.tiles; w++) join(top_of[w][lane], sum_of[w][lane], best_of[w][lane]);
+    if (wave != 0 || lane >= a.wide || r >= a.rows) return;
+    for (uint32_t w = 1; w < kWaves; w++) join(top_of[w][lane], sum_of[w][lane], best_of[w][lane]);
     const int32_t y = a.labels ? a.labels[r] : -1;
     // a label that is no class: neither a loss nor a gradient
     const float lse2 = y >= 0 && (uint64_t)y >= a.classes ? NAN : shift_of(top) + __builtin_amdgcn_logf(sum);

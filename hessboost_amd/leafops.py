@@ -57,6 +57,12 @@ class DeviceArray:
     def data_ptr(self):
         return self._ptr
 
+    def numel(self):
+        return self.shape[0] * (self.shape[1] if len(self.shape) == 2 else 1)
+
+    def is_contiguous(self):
+        return len(self.shape) == 1 or self.shape[0] <= 1 or self._stride[0] == self.shape[1]
+
     def stride(self):
         return self._stride
 
@@ -83,12 +89,12 @@ class _Call:
         if isinstance(a, DeviceArray):
             ordinal = a.ordinal
         else:
-            if a.device.type != "cuda":
+            ordinal = a.get_device()
+            if ordinal < 0:
                 raise ValueError(f"{what}: not in device memory")
-            ordinal = a.device.index
             if not self.torch:
                 _one_runtime()
-            self.torch = True
+                self.torch = True
         if self.ordinal is None:
             self.ordinal = ordinal
         elif self.ordinal != ordinal:
@@ -258,34 +264,34 @@ def clip_gradients(grads, max_norm, *, norm=None, out=None, workspace=None, stre
     grads; None: in place). The tensors are contiguous, float32 or bfloat16,
     of any shape; squares are summed in float64."""
     call = _Call()
-    out = grads if out is None else out
+    grads = list(grads)
+    out = grads if out is None else list(out)
     if len(out) != len(grads):
         raise ValueError("out: one array a gradient is needed")
-    arr = (A.Tensor * max(1, len(grads)))()
-    for i, (g, o) in enumerate(zip(grads, out)):
-        t = arr[i]
-        t.data, t.len, name = _whole(call, g, "grads")
-        t.out, n, to = _whole(call, o, "out") if o is not g else (t.data, t.len, name)
-        if n != t.len or to != name:
+    flat = []  # the records' words: data, out, len, dtype
+    for g, o in zip(grads, out):
+        data, n, name = _whole(call, g, "grads")
+        if o is g:
+            flat += (data, data, n, _CODE[name])
+            continue
+        to, m, other = _whole(call, o, "out")
+        if m != n or other != name:
             raise ValueError("out: arrays of the gradients' sizes and types are needed")
-        t.dtype = _CODE[name]
+        flat += (data, to, n, _CODE[name])
+    arr = (C.c_uint64 * max(1, len(flat)))(*flat)
     np_ = call.pointer(norm, "norm", "float32", 1)
     w, nbytes = call.memory(workspace)
     if call.ordinal is None:
         return
-    A.check(A.lib().hbr_clip_gradients(call.ordinal, arr, len(grads), float(max_norm), np_, w, nbytes,
-                                       call.stream(stream)))
+    A.check(A.lib().hbr_clip_gradients(call.ordinal, C.cast(arr, C.POINTER(A.Tensor)), len(grads), float(max_norm), np_,
+                                       w, nbytes, call.stream(stream)))
 
 
 def _whole(call, a, what):
     """A contiguous array of any shape as (address, elements, type)."""
-    n, step = 1, 1
-    st = a.stride()
-    for size, stride in zip(reversed(tuple(a.shape)), reversed(tuple(st))):
-        if size > 1 and stride != step:
-            raise ValueError(f"{what}: a contiguous array is needed")
-        step *= size
-        n *= size
+    if not a.is_contiguous():
+        raise ValueError(f"{what}: a contiguous array is needed")
+    n = a.numel()
     name = _dtype(a.dtype)
     if name not in _CODE:
         raise ValueError(f"{what}: float32 or bfloat16 is needed, not {name}")
