@@ -1173,7 +1173,7 @@ struct HeadArgs {
     const float *lse2;
     const float *weight;
     uint64_t first;               // the first class
-    float grad_scale;
+    float scale;                  // of what is written to c
     uint32_t check;               // rows of m or n may end within a chunk
     void *g;                      // [part][chunk][rows][32], g_stride columns
     uint64_t g_stride, g_chunk, g_part;
@@ -1197,7 +1197,7 @@ struct FewArgs {
     const float *weight;
     float *loss, *lse;      // or null
     int32_t *best;          // or null
-    float grad_scale;
+    float scale;            // of the gradients (the pairs are without it)
     uint32_t chunks;        // the products' shares of the rows
     void *g;                // [rows][g_stride], or null: no gradient
     uint64_t g_stride;      // a multiple of 16
@@ -1218,7 +1218,26 @@ struct FewSumsArgs {
     uint64_t dw_stride;
     uint32_t shares, waves, classes, dim;
     uint32_t dw_blocks;    // the blocks of dw's cells, those of db's behind them
-    uint32_t pad;
+    float scale;
+};
+
+// The head's gradients over short inputs (hbr_head_narrow_*): elements at
+// most, in bf16 and in f32.
+constexpr uint32_t kNarrowDim = 128;
+constexpr uint32_t kNarrowDimF32 = 64;
+struct NarrowArgs {
+    const void *x, *y;            // the held side and the walked one, in chunks
+    uint64_t x_chunk, y_chunk;    // bytes from chunk to chunk
+    uint64_t x_part, y_part;      // and from part to part
+    uint32_t nx, ny;
+    uint32_t x_tiles, splits;     // of 128 x; shares of the y
+    const float *bias;
+    const int32_t *labels;
+    const float *weight;          // or null
+    const float *lse2;
+    float *part;                  // [split][nx][dim]
+    float *part_db;               // [split][nx], or null
+    uint32_t dim, pad;
 };
 
 // src as bf16 parts in chunks of 32 columns (zeros past cols).
@@ -1255,6 +1274,8 @@ struct HeadSumArgs {
     uint64_t part_stride;
     uint32_t parts;
     uint32_t shares;  // of the parts, a wave each: 1, 4 or 16
+    float scale;
+    uint32_t pad;
 };
 
 // hbr_clip_*: up to kClipTensors tensors a launch.

@@ -363,7 +363,8 @@ struct HeadPlan {
     uint32_t score_blocks, shares;
     uint64_t g_stride;
     uint64_t parts, segments, chunks;
-    bool lay;  // h and w are laid out in chunks whatever their rows
+    bool lay;     // h and w are laid out in chunks whatever their rows
+    bool narrow;  // short inputs: no pairs are stored
     uint64_t piece, pieces;
     const HeadTiling *by_h, *by_w;  // the tiles of the products with the gradients
     uint32_t splits_h, splits_w;
@@ -391,7 +392,8 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
     q.chunks = tiles(dim, 32);
-    q.lay = dtype == HBR_F32 || n >= kLayRows;
+    q.narrow = gradient && dim <= (dtype == HBR_F32 ? kNarrowDimF32 : kNarrowDim);
+    q.lay = dtype == HBR_F32 || n >= kLayRows || q.narrow;
     const uint64_t class_tiles = tiles(classes, kTile128.tile);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
@@ -418,7 +420,17 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.lse2 = w.take<float>(n);
     q.h = w.take<char>(q.parts * q.chunks * chunk_bytes(n));
     q.w = w.take<char>(q.parts * q.chunks * chunk_bytes(classes));
-    if (gradient) {
+    if (q.narrow) {
+        // shares of the walked side, for about 1,024 workgroups of 8 steps or more
+        auto shares = [](uint64_t held, uint64_t walked) {
+            return (uint32_t)std::max<uint64_t>(1, std::min(1024 / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, 512)));
+        };
+        q.splits_h = shares(n, classes);
+        q.splits_w = shares(classes, n);
+        q.dh = w.take<float>(q.splits_h * n * dim);
+        q.dw = w.take<float>(q.splits_w * classes * dim);
+        q.part_db = w.take<float>(q.splits_w * classes);
+    } else if (gradient) {
         // the pieces as even as whole tiles allow
         const uint64_t row_bytes = std::max<uint64_t>(n, 1) * 2 * q.parts;
         q.pieces = tiles(classes, std::max<uint64_t>(256, kPieceBytes / row_bytes / 256 * 256));
@@ -468,6 +480,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     auto sum = [&](const char *kernel, const float *part, uint64_t parts, uint64_t part_stride, void *dst, uint64_t rows,
                    uint64_t cols, uint64_t dst_stride) {
         HeadSumArgs a{};
+        a.scale = p.grad_scale;
         a.part = part;
         a.parts = (uint32_t)parts;
         a.part_stride = part_stride;
@@ -502,7 +515,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         f.loss = p.loss;
         f.lse = p.lse;
         f.best = p.best;
-        f.grad_scale = p.grad_scale;
+        f.scale = p.grad_scale;
         f.chunks = q.shares;
         f.g = q.g;
         f.g_stride = q.g_stride;
@@ -529,6 +542,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             a.waves = q.score_blocks * 4;
             a.classes = (uint32_t)classes;
             a.dim = (uint32_t)dim;
+            a.scale = p.grad_scale;
             a.dw_blocks = p.dw ? (uint32_t)tiles(classes * dim, 16) : 0;
             queue.launch(("hbr_few_sums_" + suffix).c_str(), dim3(a.dw_blocks + (p.db ? (uint32_t)tiles(classes, 16) : 0)), dim3(1024), a);
         }
@@ -557,7 +571,8 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.chunks * 4), threads, a);
         return {static_cast<const char *>(to), 64, a.chunk * 2, a.part * 2, (uint32_t)(q.chunks * 32)};
     };
-    const Laid h = lay(p.h, p.h_stride, n, q.h, q.lay || p.dw, p.dw ? p.labels : nullptr);
+    const bool by_rows = p.dw || p.db || q.narrow;  // rows that take no part are read with the others
+    const Laid h = lay(p.h, p.h_stride, n, q.h, q.lay || by_rows, by_rows ? p.labels : nullptr);
     const Laid w = lay(p.w, p.w_stride, classes, q.w, q.lay, nullptr);
     auto set_a = [](HeadArgs &a, const Laid &o) { a.a = o.p, a.a_row = o.row, a.a_chunk = o.chunk, a.a_part = o.part; };
     auto set_b = [](HeadArgs &a, const Laid &o) { a.b = o.p, a.b_row = o.row, a.b_chunk = o.chunk, a.b_part = o.part; };
@@ -601,6 +616,39 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     while (f.wide > 1 && tiles(n, f.wide) < 256) f.wide /= 4;
     queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, f.wide)), dim3(1024), f);
     if (!gradient) return;
+    if (q.narrow) {
+        auto walk = [&](bool rows) {
+            const Laid &x = rows ? h : w, &y = rows ? w : h;
+            NarrowArgs a{};
+            a.x = x.p;
+            a.y = y.p;
+            a.x_chunk = x.chunk;
+            a.y_chunk = y.chunk;
+            a.x_part = x.part;
+            a.y_part = y.part;
+            a.nx = (uint32_t)(rows ? n : classes);
+            a.ny = (uint32_t)(rows ? classes : n);
+            a.x_tiles = (uint32_t)tiles(a.nx, 128);
+            a.splits = rows ? q.splits_h : q.splits_w;
+            a.bias = p.bias;
+            a.labels = p.labels;
+            a.weight = p.weight;
+            a.lse2 = q.lse2;
+            a.part = rows ? q.dh : q.dw;
+            a.part_db = rows ? nullptr : q.part_db;
+            a.dim = (uint32_t)dim;
+            queue.launch((std::string(rows ? "hbr_head_narrow_dh_" : "hbr_head_narrow_dw_") + suffix + "_" + std::to_string(q.chunks)).c_str(),
+                         dim3(a.x_tiles * a.splits), threads, a);
+        };
+        if (p.dh) {
+            walk(true);
+            sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);
+        }
+        if (p.dw || p.db) walk(false);
+        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.splits_w, classes * dim, p.dw, classes, dim, p.dw_stride);
+        if (p.db) sum("hbr_head_sum_f32", q.part_db, q.splits_w, classes, p.db, 1, classes, classes);
+        return;
+    }
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
         const uint64_t kc = std::min(q.piece, classes - k0);
         Laid wk = w;  // w from class k0 on, and its scores' gradients
@@ -619,7 +667,6 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         g.lse2 = q.lse2;
         g.weight = p.weight;
         g.first = k0;
-        g.grad_scale = p.grad_scale;
         g.g = q.g;
         g.g_stride = q.piece;
         g.g_chunk = pairs.chunk / 2;
@@ -636,6 +683,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.n = (uint32_t)dim;
             c.k = (uint32_t)n;
             c.splits = q.splits_w;
+            c.scale = q.splits_w == 1 ? p.grad_scale : 1.0f;  // else the sum's
             char *to = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
             const bool direct = q.splits_w == 1;
             c.c = direct ? (void *)to : q.dw;
@@ -652,6 +700,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.n = (uint32_t)dim;
             c.k = (uint32_t)kc;
             c.splits = q.splits_h;
+            c.scale = q.sum_h ? 1.0f : p.grad_scale;
             c.c = q.sum_h ? q.dh : p.dh;
             c.c_stride = q.sum_h ? dim : p.dh_stride;
             c.c_split = n * dim;

@@ -9,6 +9,7 @@
 #include "leaf_lookup.hip"
 #include "softmax_head.hip"
 #include "softmax_few.hip"
+#include "softmax_narrow.hip"
 #include "clip.hip"
 
 // The abi.h checksum this code object was built with (checked by the host

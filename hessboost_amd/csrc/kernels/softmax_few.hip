@@ -125,7 +125,6 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
         if (!a.g) continue;
         const uint64_t kept = __ballot(y >= 0);
         if (lane == 0) a.keep[g] = (uint32_t)kept;
-        const float by = a.grad_scale * weight;
         T *out = static_cast<T *>(a.g) + r * a.g_stride;
 #pragma unroll
         for (int t = 0; t < KT; t++)
@@ -137,7 +136,7 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
                     const int e = 4 * q + i;
                     float p = __builtin_amdgcn_exp2f(acc[t][e] - lse2);
                     if (y == (int32_t)(32 * t + row_of(e))) p -= 1.0f;
-                    p = y < 0 ? 0.0f : p * by;
+                    p = y < 0 ? 0.0f : p * weight;
                     db[t][e] += p;
                     v.v[i] = F::E::down(p);
                 }
@@ -219,7 +218,7 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
             if (d < a.dim) {
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    if (row_of(e) < m) out[row_of(e) * a.dh_stride] = F::E::down(acc[e]);
+                    if (row_of(e) < m) out[row_of(e) * a.dh_stride] = F::E::down(acc[e] * a.scale);
             }
         }
     }
@@ -253,6 +252,7 @@ __device__ __forceinline__ void few_sums(const FewSumsArgs &a) {
     __syncthreads();
     if (group || i >= cells) return;
     for (int g = 1; g < 64; g++) s += sum_of[g][lane];
+    s *= a.scale;
     if (dw) static_cast<typename E::type *>(a.dw)[i / a.dim * a.dw_stride + i % a.dim] = E::down(s);
     else a.db[i] = s;
 }

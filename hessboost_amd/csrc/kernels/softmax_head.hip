@@ -2,7 +2,12 @@
 // gradients, the scores made tile by tile and never kept.
 //
 //   z = h W^T + b; lse = log sum exp z; loss = a (lse - z_y)
-//   g = c a (exp(z - lse) - [k = y]); dh = g W; dW = g^T h; db = sum g
+//   g = a (exp(z - lse) - [k = y]); dh = c g W; dW = c g^T h; db = c sum g
+//
+// In bf16 the pairs g are rounded once to bf16 for the products, as a layer's
+// output gradient in mixed precision is: half a step each, of the size of the
+// result's own rounding. They hold no c, so that a row without a weight has
+// its label's pair near -1, which bf16 holds well, and not near -c.
 //
 // Scores are held in units of log2 (z log2 e), so that an exponential is one
 // v_exp_f32.
@@ -355,7 +360,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
         const int32_t y = r < a.m ? a.labels[r] : -1;
         const bool live = y >= 0;
         lse_of[i] = live ? a.lse2[r] : INFINITY;
-        by_of[i] = live ? a.grad_scale * (a.weight ? a.weight[r] : 1.0f) : 0.0f;
+        by_of[i] = live ? a.weight ? a.weight[r] : 1.0f : 0.0f;
         const int64_t in = (int64_t)y - (int64_t)a.first - t.n0;
         label_of[i] = live && in >= 0 && in < (int64_t)Tile::kN ? (int32_t)in : -0x10000;
     }
@@ -498,9 +503,9 @@ __device__ __forceinline__ void head_sums(const HeadArgs &a, char *lds) {
             for (int e = 0; e < 16; e++) {
                 const uint32_t to = at + (32 * i + 8 * (e / 4) + e % 4) * stride;
                 if constexpr (sizeof(T) == 4)
-                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(t.acc[i][j][e]), c, to, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(t.acc[i][j][e] * a.scale), c, to, 0, 0);
                 else
-                    __builtin_amdgcn_raw_buffer_store_b16(to_bf16(t.acc[i][j][e]), c, to, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b16(to_bf16(t.acc[i][j][e] * a.scale), c, to, 0, 0);
             }
         }
     }
@@ -532,7 +537,7 @@ __device__ __forceinline__ void head_sum(const HeadSumArgs &a) {
         }
         if (i >= cells) continue;
         const uint64_t r = i / a.cols;
-        static_cast<typename E::type *>(a.dst)[r * a.dst_stride + (i - r * a.cols)] = E::down(s);
+        static_cast<typename E::type *>(a.dst)[r * a.dst_stride + (i - r * a.cols)] = E::down(s * a.scale);
     }
 }
 
@@ -557,12 +562,12 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
             for (int k = 0; k < 8; k++)
                 if (c + k < a.cols) v.v[k] = src[k];
         }
-        // a row that takes no part may hold anything: finite, so that its
-        // gradient of zero adds nothing
+        // a row that takes no part may hold anything: finite, and far from
+        // where a score would not be, so that its gradient of zero adds nothing
         if (a.labels && a.labels[r] < 0)
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (!(__builtin_fabsf(E::up(v.v[k])) < INFINITY)) v.v[k] = (T)0;
+                if (!(__builtin_fabsf(E::up(v.v[k])) < 1e15f)) v.v[k] = (T)0;
         Vec<uint16_t, 8> out[Parts];
 #pragma unroll
         for (int k = 0; k < 8; k++) {

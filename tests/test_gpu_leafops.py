@@ -300,6 +300,15 @@ HEADS = [
     (600, 31, 1, 0.0, False, True, 0, 0),
     (2000, 3, 12, 0.1, True, True, 0, 0),
     (0, 5, 8, 0.0, True, True, 0, 0),
+    (0, 500, 300, 0.0, False, True, 0, 0),
+    (600, 200, 136, 0.1, True, True, 0, 0),   # long inputs, read where they lie
+    (600, 200, 136, 0.1, False, False, 24, 8),
+    (33, 700, 1000, 0.0, True, True, 8, 0),
+    (1030, 260, 140, 0.1, True, True, 0, 0),  # laid out first
+    (2050, 129, 129, 0.0, False, True, 1, 1),
+    (128, 4000, 64, 0.0, False, True, 0, 0),  # short inputs, classes shared out
+    (5000, 70, 9, 0.1, True, True, 0, 0),     # and rows
+    (900, 1100, 65, 0.3, False, True, 0, 0),
 ]
 
 
@@ -356,6 +365,34 @@ def test_softmax_head_and_its_gradients(case, dtype):
         assert np.array_equal(run_head(c, (k,))[k], got[k]), k
 
 
+@pytest.mark.parametrize("dtype, n, classes", [("float32", 40_000, 5_000), ("bfloat16", 90_000, 6_200)])
+def test_classes_taken_in_pieces(dtype, n, classes):
+    """More pairs than are held at once: some rows' loss and gradient against
+    all of their classes, and some classes' (the first and last of each piece
+    among them) against all rows, whose lse the first check stands for."""
+    c = head_case((n, classes, 130, 0.05, True, True, 0, 0), dtype, 9)
+    got = run_head(c, ("loss", "lse", "dh", "dw", "db"))
+    rows = np.r_[0:40, n // 2:n // 2 + 40, n - 40:n]
+    part = dict(c, h=c["h"][rows])
+    want = R.head(part["h"], c["w"], c["bias"], c["labels"][rows], c["weight"][rows], c["scale"], dtype)
+    for k in ("loss", "lse", "dh"):
+        close(got[k][rows], want[k], k)
+    some = np.r_[0:20, classes // 2 - 160:classes // 2 + 160, classes - 20:classes]
+    z = c["h"] @ c["w"][some].T + c["bias"][some]
+    p = np.exp(z - got["lse"][:, None])
+    live = c["labels"] >= 0
+    g = np.where(live[:, None], c["scale"] * c["weight"][:, None] * (p - (c["labels"][:, None] == some[None, :])), 0.0)
+    # a score's and the lse's bounds, and the pair's roundings, as in R.head
+    size = np.abs(c["h"]) @ np.abs(c["w"][some].T) + np.abs(c["bias"][some])
+    elz = want["lse"][1].max() * 2
+    eg = c["scale"] * c["weight"][:, None] * p * ((c["dim"] + 4) * R.EPS32 * size + elz + (np.abs(z - got["lse"][:, None]) + 8) * R.EPS32)
+    eg = np.where(live[:, None], eg, 0.0) + 2 * R.EPS32 * np.abs(g)
+    close(got["db"][some], (g.sum(0), eg.sum(0) + (n + 1) * R.EPS32 * np.abs(g).sum(0)), "db")
+    eg = eg + R.HALF[dtype] * np.abs(g)
+    value, err = g.T @ c["h"], eg.T @ np.abs(c["h"])
+    close(got["dw"][some], (value, err + (n + 4) * R.EPS32 * (np.abs(g).T @ np.abs(c["h"])) + R.HALF[dtype] * (np.abs(value) + err)), "dw")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n, classes, dim", [(1, 5, 16), (1, 4099, 64), (7, 1000, 33), (16, 70_000, 24), (50, 257, 512)])
 def test_rows_answered_without_labels(n, classes, dim, dtype):
@@ -381,7 +418,7 @@ def test_the_first_of_equal_classes_is_the_best(n, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n, classes, dim", [(90, 12, 20), (90, 300, 64)])
+@pytest.mark.parametrize("n, classes, dim", [(90, 12, 20), (90, 300, 64), (90, 300, 160), (1100, 300, 136)])
 def test_shut_classes_and_rows_that_take_no_part(n, classes, dim, dtype):
     """Biases of -infinity; NaN, infinities and a NaN weight in rows whose
     label is below 0: the others' results are those without them."""
@@ -406,9 +443,9 @@ def test_shut_classes_and_rows_that_take_no_part(n, classes, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("classes", [6, 200])
-def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dtype):
-    c = head_case((40, classes, 24, 0.0, False, True, 0, 0), dtype, 4)
+@pytest.mark.parametrize("classes, dim", [(6, 24), (200, 24), (200, 160)])
+def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dim, dtype):
+    c = head_case((40, classes, dim, 0.0, False, True, 0, 0), dtype, 4)
     c["bias"][0] = -np.inf
     c["labels"][:] = np.maximum(c["labels"], 1)
     c["labels"][3] = 0
@@ -420,9 +457,9 @@ def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("classes", [4, 130])
-def test_rows_with_no_open_class_and_labels_that_are_no_class(classes, dtype):
-    c = head_case((30, classes, 8, 0.0, False, True, 0, 0), dtype, 5)
+@pytest.mark.parametrize("classes, dim", [(4, 8), (130, 8), (130, 136)])
+def test_rows_with_no_open_class_and_labels_that_are_no_class(classes, dim, dtype):
+    c = head_case((30, classes, dim, 0.0, False, True, 0, 0), dtype, 5)
     shut = dict(c, bias=np.full(classes, -np.inf))
     got = run_head(shut, ("loss", "lse"))
     assert np.all(np.isneginf(got["lse"])) and np.all(np.isnan(got["loss"]))
@@ -445,7 +482,7 @@ def test_scores_far_from_zero_keep_their_loss(classes):
     check_head(got, R.head(c["h"], c["w"], c["bias"], c["labels"], None, c["scale"], "float32"))
 
 
-@pytest.mark.parametrize("n, classes, dim", [(6, 5, 8), (20, 150, 12)])
+@pytest.mark.parametrize("n, classes, dim", [(6, 5, 8), (20, 150, 12), (20, 150, 132)])
 def test_head_gradients_are_the_differences_of_the_loss(n, classes, dim):
     """A central difference along a direction in h, w and bias at once. With
     step e the difference is off by e^2/6 times the loss's third derivative
