@@ -1237,6 +1237,10 @@ struct NarrowArgs {
     const float *lse2;
     float *part;                  // [split][nx][dim]
     float *part_db;               // [split][nx], or null
+    float *part_max;              // the scores' results: [split][nx]
+    float *part_sum;
+    int32_t *part_best;           // or null
+    float *label_margin;
     uint32_t dim, pad;
 };
 

@@ -174,10 +174,19 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
                 p.table_rows / p.n_columns <= 2048 && std::max(p.out_stride, p.ids_stride) < 32768;
     if (q.columns) {
         const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
-        const uint64_t most = std::max<uint64_t>(1, q.n / (8 * p.table_rows));
-        const uint64_t fills = (1024 + p.n_columns * slices - 1) / (p.n_columns * slices);
-        uint64_t blocks = std::max((p.n_rows + kColumnBlock - 1) / kColumnBlock, std::min({most, fills, (p.n_rows + 511) / 512}));
-        if (blocks > 4) blocks = up(blocks, 8);
+        const uint64_t least = (p.n_rows + kColumnBlock - 1) / kColumnBlock;
+        const uint64_t most = std::max(least, std::min(q.n / (8 * p.table_rows), (p.n_rows + 511) / 512));
+        // 512 workgroups run at once. Beside its rows a workgroup costs about
+        // what 1,500 rows do (200,003 x 100 ids, 64 bf16: 12,500 rows in 70
+        // us), and a sum of a block what 3.5e-4 rows do.
+        uint64_t blocks = least;
+        double best = 0.0;
+        for (uint64_t b = least; b <= most + 7; b++) {
+            if (b > 4 && b % 8) continue;  // whole XCDs
+            const double rounds = (double)((b * p.n_columns * slices + 511) / 512);
+            const double cost = rounds * (double)((p.n_rows + b - 1) / b + 1500) + 3.5e-4 * (double)(b > 1 ? b * p.table_rows * p.dim : 0);
+            if (best == 0.0 || cost < best) best = cost, blocks = b;
+        }
         q.blocks = (uint32_t)blocks;
         q.block_rows = (uint32_t)((p.n_rows + blocks - 1) / blocks);
         if (blocks > 1) q.part = w.take<float>(blocks * p.table_rows * up(p.dim, 4));
@@ -191,9 +200,10 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     uint32_t bits = 1;
     while (bits < 32 && (p.table_rows >> bits)) bits++;
     q.passes = (bits + kSortBits - 1) / kSortBits;
-    // 8 to 64 entries a chunk, for about 4,096 waves of 16-byte vectors
+    // 32 or 64 entries a chunk, for about 4,096 waves of 16-byte vectors (of
+    // fewer entries, a frequent id's parts would be many)
     const uint64_t waves = (p.dim * (p.dtype == HBR_F32 ? 4 : 2) + 1023) / 1024;
-    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(8, up(q.n * waves / 4096, 8)));
+    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(32, up(q.n * waves / 4096, 8)));
     q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
     for (int b = 0; b < 2; b++) {
         q.key[b] = w.take<uint32_t>(q.n);
@@ -305,7 +315,7 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     const uint32_t groups = 256 / a.wide, slices = (a.vecs + a.wide - 1) / a.wide;
     queue.launch(("hbr_lookup_sum_" + suffix).c_str(), dim3((q.chunks + groups - 1) / groups, slices), dim3(256), a);
     a.row_blocks = (uint32_t)((p.table_rows + 4 * 63 - 1) / (4 * 63));
-    queue.launch(("hbr_lookup_finish_" + suffix).c_str(), dim3(a.row_blocks + (q.chunks + groups - 1) / groups), dim3(256), a);
+    queue.launch(("hbr_lookup_finish_" + suffix).c_str(), dim3(a.row_blocks + (q.chunks + groups - 1) / groups, slices), dim3(256), a);
 }
 
 // ---- the softmax head ------------------------------------------------------------------
@@ -367,7 +377,7 @@ struct HeadPlan {
     bool narrow;  // short inputs: no pairs are stored
     uint64_t piece, pieces;
     const HeadTiling *by_h, *by_w;  // the tiles of the products with the gradients
-    uint32_t splits_h, splits_w;
+    uint32_t splits_h, splits_w, splits_z;  // splits_z: of the classes, for the scores over short inputs
     bool sum_h;  // dh is summed from f32 parts
     float *part_max, *part_sum, *label_margin, *lse2, *part_db, *dh, *dw;
     int32_t *part_best;
@@ -394,7 +404,12 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.chunks = tiles(dim, 32);
     q.narrow = gradient && dim <= (dtype == HBR_F32 ? kNarrowDimF32 : kNarrowDim);
     q.lay = dtype == HBR_F32 || n >= kLayRows || q.narrow;
-    const uint64_t class_tiles = tiles(classes, kTile128.tile);
+    // shares of the walked side, for about 1,024 workgroups of 8 steps or more
+    auto shares = [](uint64_t held, uint64_t walked) {
+        return (uint32_t)std::max<uint64_t>(1, std::min(1024 / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, 512)));
+    };
+    q.splits_z = shares(n, classes);
+    const uint64_t class_tiles = q.narrow ? q.splits_z : tiles(classes, kTile128.tile);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
@@ -421,11 +436,7 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.h = w.take<char>(q.parts * q.chunks * chunk_bytes(n));
     q.w = w.take<char>(q.parts * q.chunks * chunk_bytes(classes));
     if (q.narrow) {
-        // shares of the walked side, for about 1,024 workgroups of 8 steps or more
-        auto shares = [](uint64_t held, uint64_t walked) {
-            return (uint32_t)std::max<uint64_t>(1, std::min(1024 / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, 512)));
-        };
-        q.splits_h = shares(n, classes);
+        q.splits_h = q.splits_z;
         q.splits_w = shares(classes, n);
         q.dh = w.take<float>(q.splits_h * n * dim);
         q.dw = w.take<float>(q.splits_w * classes * dim);
@@ -596,7 +607,34 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     z.part_sum = q.part_sum;
     z.part_best = p.best ? q.part_best : nullptr;
     z.label_margin = q.label_margin;
-    product("hbr_head_scores", kTile128, z);
+    auto walk = [&](const char *kernel, bool rows, uint32_t splits, float *part) {
+        const Laid &x = rows ? h : w, &y = rows ? w : h;
+        NarrowArgs a{};
+        a.x = x.p;
+        a.y = y.p;
+        a.x_chunk = x.chunk;
+        a.y_chunk = y.chunk;
+        a.x_part = x.part;
+        a.y_part = y.part;
+        a.nx = (uint32_t)(rows ? n : classes);
+        a.ny = (uint32_t)(rows ? classes : n);
+        a.x_tiles = (uint32_t)tiles(a.nx, 128);
+        a.splits = splits;
+        a.bias = p.bias;
+        a.labels = p.labels;
+        a.weight = p.weight;
+        a.lse2 = q.lse2;
+        a.part = part;
+        a.part_db = rows ? nullptr : q.part_db;
+        a.part_max = q.part_max;
+        a.part_sum = q.part_sum;
+        a.part_best = p.best ? q.part_best : nullptr;
+        a.label_margin = q.label_margin;
+        a.dim = (uint32_t)dim;
+        queue.launch((kernel + suffix + "_" + std::to_string(q.chunks)).c_str(), dim3(a.x_tiles * a.splits), threads, a);
+    };
+    if (q.narrow) walk("hbr_head_narrow_scores_", true, q.splits_z, nullptr);
+    else product("hbr_head_scores", kTile128, z);
     HeadFinishArgs f{};
     f.part_max = q.part_max;
     f.part_sum = q.part_sum;
@@ -610,41 +648,19 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     f.best = p.best;
     f.rows = n;
     f.classes = classes;
-    f.tiles = (uint32_t)tiles(classes, kTile128.tile);
-    // fewer rows a workgroup where they would not fill the device
+    f.tiles = (uint32_t)(q.narrow ? q.splits_z : tiles(classes, kTile128.tile));
+    // fewer rows a workgroup where they would not fill the device and a lane
+    // would have more than eight tiles
     f.wide = 64;
-    while (f.wide > 1 && tiles(n, f.wide) < 256) f.wide /= 4;
+    while (f.wide > 1 && tiles(n, f.wide) < 256 && f.tiles > 8 * 16 * (64 / f.wide)) f.wide /= 4;
     queue.launch("hbr_head_finish", dim3((uint32_t)tiles(n, f.wide)), dim3(1024), f);
     if (!gradient) return;
     if (q.narrow) {
-        auto walk = [&](bool rows) {
-            const Laid &x = rows ? h : w, &y = rows ? w : h;
-            NarrowArgs a{};
-            a.x = x.p;
-            a.y = y.p;
-            a.x_chunk = x.chunk;
-            a.y_chunk = y.chunk;
-            a.x_part = x.part;
-            a.y_part = y.part;
-            a.nx = (uint32_t)(rows ? n : classes);
-            a.ny = (uint32_t)(rows ? classes : n);
-            a.x_tiles = (uint32_t)tiles(a.nx, 128);
-            a.splits = rows ? q.splits_h : q.splits_w;
-            a.bias = p.bias;
-            a.labels = p.labels;
-            a.weight = p.weight;
-            a.lse2 = q.lse2;
-            a.part = rows ? q.dh : q.dw;
-            a.part_db = rows ? nullptr : q.part_db;
-            a.dim = (uint32_t)dim;
-            queue.launch((std::string(rows ? "hbr_head_narrow_dh_" : "hbr_head_narrow_dw_") + suffix + "_" + std::to_string(q.chunks)).c_str(),
-                         dim3(a.x_tiles * a.splits), threads, a);
-        };
         if (p.dh) {
-            walk(true);
+            walk("hbr_head_narrow_dh_", true, q.splits_h, q.dh);
             sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);
         }
-        if (p.dw || p.db) walk(false);
+        if (p.dw || p.db) walk("hbr_head_narrow_dw_", false, q.splits_w, q.dw);
         if (p.dw) sum(sum_kernel.c_str(), q.dw, q.splits_w, classes * dim, p.dw, classes, dim, p.dw_stride);
         if (p.db) sum("hbr_head_sum_f32", q.part_db, q.splits_w, classes, p.db, 1, classes, classes);
         return;

@@ -623,14 +623,15 @@ __device__ __forceinline__ uint32_t first_entry(const LookupSumArgs &a, uint64_t
 // The table rows that no chunk wrote. The first blocks write zeros where no
 // entry is: a wave finds where the entries of 64 rows begin, a search a lane,
 // and has the ends of 63. The others join the parts of runs that reach over
-// chunks, in order: a group of lanes a chunk, for the run that begins in it
-// and goes on behind it.
+// chunks, in order: a group of lanes a chunk (and 64 vectors), for the run
+// that begins in it and goes on behind it.
 template <typename E, int V>
 __device__ __forceinline__ void lookup_finish(const LookupSumArgs &a) {
     using T = typename E::type;
     const uint32_t lane = lane_id(), c0 = lane & (a.wide - 1), groups = kWave / a.wide;
     T *dtable = static_cast<T *>(a.dtable);
     if (blockIdx.x < a.row_blocks) {
+        if (blockIdx.y) return;
         const uint64_t r0 = ((uint64_t)blockIdx.x * 4 + threadIdx.x / kWave) * (kWave - 1);
         if (r0 >= a.table_rows) return;
         const uint32_t at = first_entry(a, r0 + lane);
@@ -652,23 +653,22 @@ __device__ __forceinline__ void lookup_finish(const LookupSumArgs &a) {
     if (key >= a.table_rows || a.keys[last] != key) return;
     const uint32_t start = first_entry(a, key), to = (first_entry(a, (uint64_t)key + 1) - 1) / a.chunk;
     if (start < chunk * a.chunk) return;  // it began before
-    const uint32_t slot = start != chunk * a.chunk ? 1 : 0;
-    for (uint32_t c = c0; c < a.vecs; c += a.wide) {
-        float acc[V];
-        const float *p = a.part + ((uint64_t)chunk * 2 + slot) * a.dim + c * V;
+    const uint32_t slot = start != chunk * a.chunk ? 1 : 0, c = blockIdx.y * a.wide + c0;
+    if (c >= a.vecs) return;
+    float acc[V];
+    const float *p = a.part + ((uint64_t)chunk * 2 + slot) * a.dim + c * V;
 #pragma unroll
-        for (int k = 0; k < V; k++) acc[k] = p[k];
+    for (int k = 0; k < V; k++) acc[k] = p[k];
 #pragma unroll 8
-        for (uint32_t q = chunk + 1; q <= to; q++) {
-            p = a.part + (uint64_t)q * 2 * a.dim + c * V;
+    for (uint32_t q = chunk + 1; q <= to; q++) {
+        p = a.part + (uint64_t)q * 2 * a.dim + c * V;
 #pragma unroll
-            for (int k = 0; k < V; k++) acc[k] += p[k];
-        }
-        Vec<T, V> out;
-#pragma unroll
-        for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
-        *reinterpret_cast<Vec<T, V> *>(dtable + key * a.dtable_stride + c * V) = out;
+        for (int k = 0; k < V; k++) acc[k] += p[k];
     }
+    Vec<T, V> out;
+#pragma unroll
+    for (int k = 0; k < V; k++) out.v[k] = E::down(acc[k]);
+    *reinterpret_cast<Vec<T, V> *>(dtable + key * a.dtable_stride + c * V) = out;
 }
 
 }  // namespace hbr

@@ -638,10 +638,11 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
             int32_t b[kAhead];
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; u++) {
-                const uint64_t at = min(t0 + u, end - 1) * a.rows + r;
-                m[u] = a.part_max[at];
-                s[u] = a.part_sum[at];
-                b[u] = a.part_best ? a.part_best[at] : 0;
+                const uint64_t at = (t0 + u) * a.rows + r;
+                const bool in = t0 + u < end;
+                m[u] = in ? a.part_max[at] : 0.0f;
+                s[u] = in ? a.part_sum[at] : 0.0f;
+                b[u] = in && a.part_best ? a.part_best[at] : 0;
             }
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; u++)

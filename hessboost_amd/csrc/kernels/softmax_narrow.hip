@@ -21,8 +21,13 @@ namespace hbr {
 
 constexpr int kNarrowY = 64, kNarrowWaves = 4, kNarrowX = 32 * kNarrowWaves;
 
-template <bool Rows, int Parts, int DT>
+// kScores holds rows as kRows does, and keeps each row's running maximum and
+// sum in the place of the second product.
+enum NarrowMode { kScores, kRows, kClasses };
+
+template <NarrowMode Mode, int Parts, int DT>
 __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
+    constexpr bool Rows = Mode != kClasses;
     constexpr int kChunk = kNarrowY * 64, kStage = Parts * DT * kChunk, kSteps = 2 * DT, kSegments = Parts == 1 ? 1 : 6;
     __shared__ float u_of[2][kNarrowY], weight_of[2][kNarrowY];
     __shared__ int32_t label_of[2][kNarrowY];
@@ -44,7 +49,9 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
         }
     float v_x = 0.0f, weight_x = 1.0f;
     int32_t label_x = -1;
-    if (Rows && in) {
+    if (Mode == kScores) {
+        if (in && a.labels) label_x = a.labels[x];
+    } else if (Rows && in) {
         label_x = a.labels[x];
         v_x = label_x < 0 ? -INFINITY : -a.lse2[x];
         if (a.weight && label_x >= 0) weight_x = a.weight[x];
@@ -57,6 +64,8 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
 #pragma unroll
         for (int e = 0; e < 16; e++) out[t][e] = 0.0f;
     float db = 0.0f;
+    float top = -INFINITY, total = 0.0f;  // kScores
+    int32_t best = 0x7fffffff;
     const uint32_t steps = (a.ny + kNarrowY - 1) / kNarrowY;
     const uint32_t s0 = (uint32_t)((uint64_t)steps * split / a.splits), s1 = (uint32_t)((uint64_t)steps * (split + 1) / a.splits);
     // a wave's share of a stage: 16 rows of every chunk, their 16-byte pieces
@@ -128,11 +137,37 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
                     z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, xf[pb][k], z, 0, 0, 0);
                 }
             }
+            const uint32_t y0 = s * kNarrowY + b * 32;
+            if constexpr (Mode == kScores) {
+                float most = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    z[e] = __builtin_fmaf(z[e], kLog2e, u_of[s % 2][b * 32 + row_of(e)]);
+                    most = fmaxf(most, z[e]);
+                }
+                if (__ballot((uint32_t)label_x - y0 < 32u))
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (label_x == (int32_t)(y0 + row_of(e)) && (uint32_t)label_x < a.ny) a.label_margin[x] = z[e];
+                if (a.part_best && __ballot(most > top)) {
+                    int32_t at = 0x7fffffff;
+#pragma unroll
+                    for (int e = 15; e >= 0; e--)
+                        if (z[e] == most) at = (int32_t)(y0 + row_of(e));
+                    if (most > top) best = at;
+                }
+                const float both = fmaxf(top, most), shift = shift_of(both);
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(z[e] - shift);
+                total = total * __builtin_amdgcn_exp2f(top - shift) + sum;
+                top = both;
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], kLog2e, u_of[s % 2][b * 32 + row_of(e)] + v_x));
             // one less where the row's label is the class, if that is anywhere here
-            const uint32_t y0 = s * kNarrowY + b * 32;
             if (Rows) {
                 if (__ballot((uint32_t)label_x - y0 < 32u))
 #pragma unroll
@@ -147,8 +182,10 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
                 if (a.weight)
 #pragma unroll
                     for (int e = 0; e < 16; e++) z[e] *= weight_of[s % 2][b * 32 + row_of(e)];
+                float sum = 0.0f;  // of the block alone: the running sum may be far larger
 #pragma unroll
-                for (int e = 0; e < 16; e++) db += z[e];
+                for (int e = 0; e < 16; e++) sum += z[e];
+                db += sum;
             }
             // sixteen y a fragment, of which a lane has eight: its elements
             // 8 k to 8 k + 7, y 16 k + 4 half + 0..3 and 8 more
@@ -196,6 +233,17 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (Mode == kScores) {
+        const float t = __shfl_xor(top, 32, kWave), sum = __shfl_xor(total, 32, kWave);
+        const int32_t b = __shfl_xor(best, 32, kWave);
+        const float both = fmaxf(top, t), shift = shift_of(both);
+        if (!in || half) return;
+        const uint64_t at = (uint64_t)split * a.nx + x;
+        a.part_max[at] = both;
+        a.part_sum[at] = total * __builtin_amdgcn_exp2f(top - shift) + sum * __builtin_amdgcn_exp2f(t - shift);
+        if (a.part_best) a.part_best[at] = top > t ? best : t > top ? b : min(best, b);
+        return;
+    }
     if (!Rows) db += __shfl_xor(db, 32, kWave);
     if (!in) return;
     if (!Rows && a.part_db && half == 0) a.part_db[(uint64_t)split * a.nx + x] = db;
@@ -213,15 +261,15 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
 
 using namespace hbr;
 
-#define HBR_NARROW(suffix, Parts, DT)                                                                              \
-    extern "C" __global__ __launch_bounds__(256, 2) void hbr_head_narrow_dh_##suffix(NarrowArgs a) {               \
-        __shared__ __align__(1024) char lds[2 * Parts * DT * kNarrowY * 64];                                       \
-        head_narrow<true, Parts, DT>(a, lds);                                                                      \
-    }                                                                                                              \
-    extern "C" __global__ __launch_bounds__(256, 2) void hbr_head_narrow_dw_##suffix(NarrowArgs a) {               \
-        __shared__ __align__(1024) char lds[2 * Parts * DT * kNarrowY * 64];                                       \
-        head_narrow<false, Parts, DT>(a, lds);                                                                     \
+#define HBR_NARROW_MODE(name, Mode, Parts, DT)                                      \
+    extern "C" __global__ __launch_bounds__(256, 2) void name(NarrowArgs a) {       \
+        __shared__ __align__(1024) char lds[2 * Parts * DT * kNarrowY * 64];        \
+        head_narrow<Mode, Parts, DT>(a, lds);                                       \
     }
+#define HBR_NARROW(suffix, Parts, DT)                                               \
+    HBR_NARROW_MODE(hbr_head_narrow_scores_##suffix, kScores, Parts, DT)            \
+    HBR_NARROW_MODE(hbr_head_narrow_dh_##suffix, kRows, Parts, DT)                  \
+    HBR_NARROW_MODE(hbr_head_narrow_dw_##suffix, kClasses, Parts, DT)
 HBR_NARROW(bf16_1, 1, 1)
 HBR_NARROW(bf16_2, 1, 2)
 HBR_NARROW(bf16_3, 1, 3)

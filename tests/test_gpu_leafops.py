@@ -361,8 +361,14 @@ def test_softmax_head_and_its_gradients(case, dtype):
     assert np.array_equal(got["best"][clear], want["best"][0][clear])
     again = run_head(c)
     assert all(np.array_equal(got[k], again[k]) for k in got)
-    for k in got:  # each alone
-        assert np.array_equal(run_head(c, (k,))[k], got[k]), k
+    for k in got:  # each alone: the gradients' bits, and scores within their bounds
+        alone = run_head(c, (k,))[k]
+        if k in ("dh", "dw", "db"):
+            assert np.array_equal(alone, got[k]), k
+        elif k == "best":
+            assert np.array_equal(alone[clear], got[k][clear])
+        else:
+            close(alone, want[k], k)
 
 
 @pytest.mark.parametrize("dtype, n, classes", [("float32", 40_000, 5_000), ("bfloat16", 90_000, 6_200)])

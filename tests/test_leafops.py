@@ -87,8 +87,9 @@ def test_workspaces_of_all_sizes_are_named(dtype):
     for n in (0, 1, 31, 1023, 1024, 70_000, (1 << 31) - 1):
         for classes in (1, 2, 64, 65, 128, 129, 131_072):
             for dim in (1, 7, 64, 1024, 70_000):
-                score = hb.softmax_head_workspace(n, classes, dim, dtype, gradient=False)
-                assert score <= hb.softmax_head_workspace(n, classes, dim, dtype)
+                for gradient in (False, True):
+                    need = hb.softmax_head_workspace(n, classes, dim, dtype, gradient=gradient)
+                    assert need >= 0 and need % 256 == 0
     for n in (0, 1, 16_383, 1 << 20):
         for columns in (0, 1, 3, 1000):
             for rows in (0, 1, 512, 1 << 20):
