@@ -1,6 +1,7 @@
 #include "leafops.h"
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "../abi.h"
@@ -183,7 +184,9 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
         double best = 0.0;
         for (uint64_t b = least; b <= most + 7; b++) {
             if (b > 4 && b % 8) continue;  // whole XCDs
-            const double rounds = (double)((b * p.n_columns * slices + 511) / 512);
+            // (whole rounds where they are few; later ones overlap)
+            const double groups = (double)(b * p.n_columns * slices) / 512;
+            const double rounds = groups <= 2.0 ? std::ceil(groups) : groups + 0.5;
             const double cost = rounds * (double)((p.n_rows + b - 1) / b + 1500) + 3.5e-4 * (double)(b > 1 ? b * p.table_rows * p.dim : 0);
             if (best == 0.0 || cost < best) best = cost, blocks = b;
         }
@@ -337,12 +340,13 @@ constexpr uint64_t kLayRows = 1024;
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
-// A product's tiles, and how many of them run at once on 256 CUs.
+// A product's tiles, and how many of them fill 256 CUs (of the small ones twice
+// as many run at once, at hardly more rate).
 struct HeadTiling {
     uint64_t tile, threads, slots;
     const char *name;
 };
-constexpr HeadTiling kTile256{256, 512, 256, "_256"}, kTile128{128, 256, 1024, "_128"};
+constexpr HeadTiling kTile256{256, 512, 256, "_256"}, kTile128{128, 256, 512, "_128"};
 
 // Shares of a product's steps: where its tiles are fewer than the device
 // runs at once, enough of them to fill it, of 16 steps at least.
@@ -351,21 +355,23 @@ uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, ui
     return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 16));
 }
 
-// The tiles of a product with the gradients: those that take less of the
-// device, a step of 1,024 small tiles at 1.08 times one of 256 large ones.
-// Both at their best: 16,384 x 131,072 x 1,024 products of bf16 take 3.9 ms
-// with large tiles and 4.2 with small ones, 8,191 x 32,768 x 512 ones 0.29
-// and 0.32; 4,096 x 5,003 x 256 ones of f32 70 us either way. (The scores and
-// pairs keep the small ones: four workgroups on a CU hide each other's
-// exponentials and stores. 16,384 x 32,768 pairs of 1,024 take 1.34 ms against
-// 1.35 with large ones, 4,096 x 5,003 ones of 256 in f32 84 us against 119.)
+// The tiles of a product with the gradients: those that take less time, in us:
+// a step of 256 large tiles is one (1.1 PFLOP/s), one of 512 small ones 0.54,
+// and shares' sums are read once more at 4.5 TB/s. Both at their best:
+// 16,384 x 131,072 x 1,024 products of bf16 take 3.9 ms with large tiles and
+// 4.2 with small ones, 8,191 x 32,768 x 512 ones 0.29 and 0.32, 3,229 x 2,810 x
+// 335 ones of f32 with their sums 70 us and 60. (The scores and pairs keep the
+// small ones: four workgroups on a CU hide each other's exponentials and
+// stores. 16,384 x 32,768 pairs of 1,024 take 1.34 ms against 1.35 with large
+// ones, 4,096 x 5,003 ones of 256 in f32 84 us against 119.)
 const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
     const uint64_t steps = tiles(k, kHeadK) * segments;
     auto cost = [&](const HeadTiling &t, double step) {
         const uint64_t shares = head_splits(t, m, n, k, segments);
-        return (double)(tiles(tiles(m, t.tile) * tiles(n, t.tile) * shares, t.slots) * tiles(steps, shares)) * step;
+        return (double)(tiles(tiles(m, t.tile) * tiles(n, t.tile) * shares, t.slots) * tiles(steps, shares)) * step +
+               (shares > 1 ? (double)(shares * m * n) * 4.0 / 4.5e6 : 0.0);
     };
-    return cost(kTile256, 1.0) <= cost(kTile128, 1.08) ? kTile256 : kTile128;
+    return cost(kTile256, 1.0) <= cost(kTile128, 0.54) ? kTile256 : kTile128;
 }
 
 struct HeadPlan {

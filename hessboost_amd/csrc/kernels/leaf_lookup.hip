@@ -549,7 +549,7 @@ __device__ __forceinline__ void lookup_sum(const LookupSumArgs &a) {
     constexpr uint32_t kAhead = 8, kNone = 0xffffffffu;
     const uint32_t groups = 256 / a.wide, c = blockIdx.y * a.wide + (threadIdx.x & (a.wide - 1));
     const uint32_t chunk = blockIdx.x * groups + threadIdx.x / a.wide;
-    if (chunk >= a.chunks || c >= a.vecs) return;
+    if (chunk >= a.chunks || c >= a.vecs) return;  // a chunk has an entry at least
     const uint32_t c0 = chunk * a.chunk, c1 = min(c0 + a.chunk, a.n);
     const uint32_t before = c0 ? a.keys[c0 - 1] : kNone, behind = c1 < a.n ? a.keys[c1] : kNone;
     const T *dout = static_cast<const T *>(a.dout) + c * V;
@@ -568,12 +568,15 @@ __device__ __forceinline__ void lookup_sum(const LookupSumArgs &a) {
             for (int k = 0; k < V; k++) p[k] = acc[k];
         }
     };
-    uint32_t key[kAhead], val[kAhead], next_key[kAhead], next_val[kAhead];
+    // Loads without conditions, so that none waits for another: past the
+    // chunk its last entry's again, and for an id that adds nothing (behind
+    // every other, in a run that is not written) a row like any.
+    uint32_t key[kAhead], next_key[kAhead], next_val[kAhead];
     auto entries = [&](uint32_t at) {  // the eight from `at` on, one round ahead of their rows
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; u++) {
-            next_key[u] = at + u < c1 ? a.keys[at + u] : kNone;
-            next_val[u] = at + u < c1 ? a.vals[at + u] : 0;
+            next_key[u] = a.keys[min(at + u, c1 - 1)];
+            next_val[u] = a.vals[min(at + u, c1 - 1)];
         }
     };
     entries(c0);
@@ -583,12 +586,8 @@ __device__ __forceinline__ void lookup_sum(const LookupSumArgs &a) {
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; u++) {
             key[u] = next_key[u];
-            val[u] = next_val[u];
-            v[u] = Vec<T, V>{};
-            s[u] = 1.0f;
-            if (key[u] >= a.table_rows) continue;
-            const uint32_t r = a.columns == 1 ? val[u] : val[u] / a.columns;
-            if (a.scale) s[u] = a.scale[val[u] - r * a.columns];
+            const uint32_t r = a.columns == 1 ? next_val[u] : next_val[u] / a.columns;
+            s[u] = a.scale ? a.scale[next_val[u] - r * a.columns] : 1.0f;
             v[u] = *reinterpret_cast<const Vec<T, V> *>(dout + r * a.dout_stride);
         }
         entries(i0 + kAhead);

@@ -32,19 +32,32 @@ struct FewBf16 {
     }
 };
 
-// kEach elements of a row from k on, zeros past the row's dim. Vectors need
-// no more than their elements' alignment.
+// kEach elements of a row from k on, zeros past the row's dim: a vector (of no
+// more than its elements' alignment) from where one still fits the row, so
+// that no load waits on a condition, which few_tail then shifts to its place.
+// Rows shorter than a vector are read by element.
 template <typename F>
 __device__ __forceinline__ typename F::Frag few_row(const typename F::E::type *row, uint32_t k, uint32_t dim) {
     typename F::Frag f{};
-    if (k + F::kEach <= dim) {
-        __builtin_memcpy(&f, row + k, sizeof f);
+    if (dim >= (uint32_t)F::kEach) {
+        __builtin_memcpy(&f, row + min(k, dim - F::kEach), sizeof f);
     } else {
 #pragma unroll
         for (int i = 0; i < F::kEach; i++)
             if (k + i < dim) f.v[i] = row[k + i];
     }
     return f;
+}
+template <typename F>
+__device__ __forceinline__ void few_tail(typename F::Frag &f, uint32_t k, uint32_t dim) {
+    if (dim < (uint32_t)F::kEach) return;
+    const uint32_t by = k - min(k, dim - F::kEach);
+#pragma unroll
+    for (int b = 1; b < F::kEach; b *= 2)
+        if (by & b)
+#pragma unroll
+            for (int i = 0; i < F::kEach; i++) f.v[i] = i + b < F::kEach ? f.v[i + b < F::kEach ? i + b : 0] : (typename F::E::type)0;
+    if (by >= (uint32_t)F::kEach) f = typename F::Frag{};
 }
 
 // A wave takes 32 rows at a time; a lane holds its row's classes 32 kt +
@@ -80,6 +93,15 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
                 fh[u] = few_row<F>(h, k, a.dim);
 #pragma unroll
                 for (int t = 0; t < KT; t++) fw[u][t] = few_row<F>(w[t], k, a.dim);
+            }
+            if (k0 + kAhead * F::kStep > a.dim) {
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                    const uint32_t k = k0 + u * F::kStep + lane / 32 * F::kEach;
+                    few_tail<F>(fh[u], k, a.dim);
+#pragma unroll
+                    for (int t = 0; t < KT; t++) few_tail<F>(fw[u][t], k, a.dim);
+                }
             }
 #pragma unroll
             for (int u = 0; u < kAhead; u++)
@@ -186,6 +208,8 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
         const uint32_t m = (uint32_t)min((uint64_t)32, a.rows - r0);
         const T *pairs = static_cast<const T *>(a.g) + r0 * a.g_stride;
         if (a.dw) {
+            // loads without conditions (a row past the last is the last again),
+            // and nothing of the rows that take no part
             const uint32_t kept = a.keep[g];
             const T *h = static_cast<const T *>(a.h) + r0 * a.h_stride + dd;
 #pragma unroll
@@ -193,13 +217,14 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
                 Frag fh, fg[KT];
 #pragma unroll
                 for (int i = 0; i < F::kEach; i++) {
-                    const uint32_t r = s * F::kStep + half * F::kEach + i;
-                    const bool in = (kept >> r) & 1u;  // a row past the last is not kept
-                    fh.v[i] = in ? h[r * a.h_stride] : (T)0;
+                    const uint32_t r = s * F::kStep + half * F::kEach + i, rr = min(r, m - 1);
+                    fh.v[i] = h[rr * a.h_stride];
 #pragma unroll
-                    for (int t = 0; t < KT; t++) {
-                        const uint32_t c = 32 * t + lane % 32;
-                        fg[t].v[i] = in && c < a.g_stride ? pairs[r * a.g_stride + c] : (T)0;
+                    for (int t = 0; t < KT; t++) fg[t].v[i] = pairs[rr * a.g_stride + min(32 * t + lane % 32, (uint32_t)a.g_stride - 1)];
+                    if (!((kept >> r) & 1u)) {
+                        fh.v[i] = (T)0;
+#pragma unroll
+                        for (int t = 0; t < KT; t++) fg[t].v[i] = (T)0;
                     }
                 }
 #pragma unroll
@@ -213,7 +238,7 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
             const T *row = pairs + min(lane % 32, m - 1) * a.g_stride;
 #pragma unroll
             for (int s = 0; s < kSteps; s++)
-                if ((uint32_t)(s * F::kStep) < a.g_stride) acc = F::mul(few_row<F>(row, s * F::kStep + half * F::kEach, a.g_stride), w[s], acc);
+                if ((uint32_t)(s * F::kStep) < a.g_stride) acc = F::mul(*reinterpret_cast<const Frag *>(row + s * F::kStep + half * F::kEach), w[s], acc);
             T *out = static_cast<T *>(a.dh) + r0 * a.dh_stride + d;
             if (d < a.dim) {
 #pragma unroll
