@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <vector>
 
 #include "../abi.h"
 
@@ -49,6 +50,7 @@ public:
     Queue &operator=(const Queue &) = delete;
     template <typename Args>
     void launch(const char *kernel, dim3 grid, dim3 block, const Args &args, uint32_t lds_bytes = 0) {
+        if ((uint64_t)grid.x * block.x > 0xffffffffull) fail(kRefused, std::string(kernel) + ": more than 2^32 - 1 threads");
         device_->launch_on(stream_, kernel, grid, block, args, lds_bytes);
     }
 
@@ -94,6 +96,10 @@ uint32_t vector_width(uint64_t size, std::initializer_list<uint64_t> lengths, st
     return v;
 }
 
+// Vectors and inputs are shorter, so that offsets within one fit 32 bits and
+// grids over their elements a launch.
+constexpr uint64_t kDimLimit = 1u << 20;
+
 const char *name_of(uint32_t dtype) { return dtype == HBR_F32 ? "f32" : "bf16"; }
 
 // ---- leaf vectors ------------------------------------------------------------------
@@ -101,6 +107,7 @@ const char *name_of(uint32_t dtype) { return dtype == HBR_F32 ? "f32" : "bf16"; 
 void check_lookup(const hbr_lookup &p, const char *what) {
     size_of(p.dtype, what);
     if (p.dim == 0) fail(kInvalid, std::string(what) + ": vectors of no elements");
+    if (p.dim >= kDimLimit) fail(kRefused, std::string(what) + ": vectors of 1,048,576 elements or more");
     if (p.n_rows && p.n_columns && !p.ids) fail(kInvalid, std::string(what) + ": null ids");
     if (p.n_rows > 1 && p.ids_stride < p.n_columns) fail(kInvalid, std::string(what) + ": the rows of ids overlap");
     if (p.table_rows > 1 && p.table_stride < p.dim) fail(kInvalid, std::string(what) + ": the table's rows overlap");
@@ -173,8 +180,9 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
     // (A block's rows lie within 2 GiB of dout and of the ids.)
     q.columns = q.n && p.table_rows && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows &&
                 p.table_rows / p.n_columns <= 2048 && std::max(p.out_stride, p.ids_stride) < 32768;
+    const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
+    q.columns = q.columns && p.n_columns * slices <= 1u << 18;  // of its workgroups, up to eight blocks make a launch
     if (q.columns) {
-        const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
         const uint64_t least = (p.n_rows + kColumnBlock - 1) / kColumnBlock;
         const uint64_t most = std::max(least, std::min(q.n / (8 * p.table_rows), (p.n_rows + 511) / 512));
         // 512 workgroups run at once. Beside its rows a workgroup costs about
@@ -403,7 +411,7 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     size_of(dtype, "softmax head");
     if (classes == 0 || dim == 0) fail(kInvalid, "softmax head: no classes, or inputs of no elements");
     if (classes > 0x7fffffffull || n > 0x7fffffffull) fail(kRefused, "softmax head: more than 2^31 - 1 rows or classes");
-    if (dim >= (1u << 21)) fail(kRefused, "softmax head: inputs of 2,097,152 elements or more");
+    if (dim >= kDimLimit) fail(kRefused, "softmax head: inputs of 1,048,576 elements or more");
     HeadPlan q{};
     q.parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
@@ -485,6 +493,8 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         fail(kInvalid, std::string(what) + ": rows overlap");
     if (p.dh_stride >= (1u << 21) || p.dw_stride >= (1u << 21))
         fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
+    if (!q.few && std::max(tiles(n, 128) * tiles(classes, 128), q.narrow ? tiles(n, 128) * q.splits_h : 0) >= 1u << 24)
+        fail(kRefused, std::string(what) + ": 2^24 tiles of 128 rows and 128 classes or more");
     for (const void *x : {p.h, p.w, (const void *)p.dh, (const void *)p.dw}) check_aligned(x, size, what);
     for (const void *x : {(const void *)p.bias, (const void *)p.labels, (const void *)p.weight, (const void *)p.loss,
                           (const void *)p.lse, (const void *)p.best, (const void *)p.db})
@@ -740,6 +750,32 @@ namespace {
 // The launches of one pass over the tensors: kClipTensors of them at a time.
 uint64_t clip_launches(uint64_t n) { return (n + kClipTensors - 1) / kClipTensors; }
 
+// No output may lie over another tensor or output, or over its own tensor but
+// in place: a tensor given twice would be scaled twice, or once.
+void check_apart(const hbr_tensor *tensors, uint64_t n, const char *what) {
+    struct Span {
+        uint64_t begin, end;
+        bool written;
+    };
+    std::vector<Span> spans;
+    spans.reserve(n);
+    for (uint64_t i = 0; i < n; i++) {
+        const hbr_tensor &t = tensors[i];
+        const uint64_t bytes = t.len * size_of(t.dtype, what), in = reinterpret_cast<uint64_t>(t.data),
+                       out = reinterpret_cast<uint64_t>(t.out);
+        if (!bytes) continue;
+        spans.push_back({out, out + bytes, true});
+        if (in != out) spans.push_back({in, in + bytes, false});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+    uint64_t all = 0, written = 0;  // where the spans so far end
+    for (const Span &s : spans) {
+        if (s.begin < (s.written ? all : written)) fail(kInvalid, std::string(what) + ": an output overlaps another tensor");
+        all = std::max(all, s.end);
+        if (s.written) written = std::max(written, s.end);
+    }
+}
+
 }  // namespace
 
 uint64_t clip_gradients_workspace(uint64_t n_tensors) {
@@ -764,6 +800,7 @@ void clip_gradients(int ordinal, void *stream, const hbr_tensor *tensors, uint64
         blocks = (i % kClipTensors ? blocks : 0) + (tensors[i].len + kClipElems - 1) / kClipElems;
         if (blocks > 0x7fffffffull) fail(kRefused, std::string(what) + ": too many elements");
     }
+    check_apart(tensors, n, what);
     Queue queue(ordinal, stream);
     const uint64_t launches = std::max<uint64_t>(1, clip_launches(n));
     auto fill = [&](uint64_t l, ClipArgs &a) {

@@ -5,7 +5,7 @@ classes or more is modelled on its leaves instead: every row has one leaf a
 tree (``Forest.predict_margin_device`` writes their ids on the device), each
 leaf a vector, and the sum of a row's vectors is scored against every class::
 
-    off = forest_offsets                                  # each tree's first table row
+    # off[t]: the table rows before tree t's own, ascending
     hb.leaf_embedding(table, ids, h, offset=off)          # h[r] = sum of its leaves' vectors
     ws = empty(hb.softmax_head_workspace(n, k, dim, "bfloat16"))
     hb.softmax_head(h, w, labels=y, loss=loss, dh=dh, dw=dw, grad_scale=1 / n, workspace=ws)
@@ -20,7 +20,12 @@ allocates nothing and waits for nothing, so it can be captured into a graph
 (behind a first call outside one). Outputs are written into the caller's
 arrays and must not overlap inputs, except where an argument says so. A
 workspace holds what one call needs while it runs: calls, or replayed graphs,
-that may run at the same time need one each.
+that may run at the same time need one each. The arrays have to live until
+the queued work is done: torch tensors handed to a stream other than their
+own want ``record_stream``.
+
+Vectors and inputs are shorter than 2^20 elements; strides are free as long
+as a row's elements lie side by side.
 """
 from __future__ import annotations
 
@@ -262,7 +267,7 @@ def clip_gradients(grads, max_norm, *, norm=None, out=None, workspace=None, stre
     """The set's 2-norm into ``norm`` (float32 [1]), and each tensor times
     min(1, max_norm / (norm + 1e-6)) into ``out`` (a list of arrays like the
     grads; None: in place). The tensors are contiguous, float32 or bfloat16,
-    of any shape; squares are summed in float64."""
+    of any shape, and each is given once; squares are summed in float64."""
     call = _Call()
     grads = list(grads)
     out = grads if out is None else list(out)

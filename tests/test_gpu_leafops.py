@@ -525,6 +525,110 @@ def test_head_gradients_are_the_differences_of_the_loss(n, classes, dim):
     assert abs((total[0] - total[1]) - slope / c["scale"]) <= slack
 
 
+# ---- arrays of more than 4 GiB ----------------------------------------------------------
+
+FAR = 9 << 30
+
+
+def upload(address, values):
+    A.check(A.lib().hbr_device_upload(0, C.c_void_p(address), A.ptr(values), values.nbytes))
+
+
+def far(rows, cols, dtype, stride, values=None):
+    """An array whose rows lie `stride` elements apart over more than 4 GiB,
+    with nothing known between them."""
+    size = 2 if dtype == "bfloat16" else 4
+    assert FAR > (rows - 1) * stride * size > 1 << 32
+    a = DeviceArray(hb.DeviceBuffer(FAR), dtype, (rows, cols), stride=stride)
+    if values is not None:
+        bits = R.to_bf16(values) if dtype == "bfloat16" else np.ascontiguousarray(values, np.float32)
+        for r in range(rows):
+            upload(a.data_ptr() + r * stride * size, bits[r])
+    return a
+
+
+def far_back(a):
+    size, (rows, cols) = (2 if a.dtype == "bfloat16" else 4), a.shape
+    bits = np.empty((rows, cols), _BITS[a.dtype])
+    for r in range(rows):
+        A.check(A.lib().hbr_device_download(0, A.ptr(bits[r]), C.c_void_p(a.data_ptr() + r * a.stride()[0] * size), cols * size))
+    return (R.from_bf16(bits) if a.dtype == "bfloat16" else bits.view(np.float32)).astype(np.float64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [8, 37])
+def test_lookups_over_more_than_4_gib(dim, dtype):
+    rng = np.random.default_rng(dim)
+    rows, columns, n = 8, 3, 500
+    gap = (1 << 30) // (2 if dtype == "bfloat16" else 4) + 16
+    table = R.rounded(rng.standard_normal((rows, dim)), dtype)
+    ids = rng.integers(-1, rows + 1, (n, columns)).astype(np.int32)
+    out = like((n, dim), dtype)
+    hb.leaf_embedding(far(rows, dim, dtype, gap, table), dev(ids, "int32"), out)
+    close(back(out), R.embedding(table, ids, None, None, dtype), "the table far")
+    out = far(rows, dim, dtype, gap)
+    hb.leaf_embedding(dev(table, dtype), dev(ids[:rows], "int32"), out)
+    close(far_back(out), R.embedding(table, ids[:rows], None, None, dtype), "the vectors far")
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    for t, what in ((columns, "the gradient far, by sorting"), (1, "by column")):
+        mine, dtable = ids[:, :t].copy(), far(rows, dim, dtype, gap)
+        hb.leaf_embedding_grad(dev(dout, dtype), dev(mine, "int32"), dtable,
+                               workspace=work(hb.leaf_embedding_grad_workspace(n, t, rows, dim, dtype)))
+        close(far_back(dtable), R.embedding_grad(dout, mine, None, None, rows, dtype), what)
+    dtable = like((rows, dim), dtype)
+    hb.leaf_embedding_grad(far(rows, dim, dtype, gap, dout[:rows]), dev(ids[:rows], "int32"), dtable,
+                           workspace=work(hb.leaf_embedding_grad_workspace(rows, columns, rows, dim, dtype)))
+    close(back(dtable), R.embedding_grad(dout[:rows], ids[:rows], None, None, rows, dtype), "the rows far")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, classes, dim", [(1100, 20, 24), (1100, 70, 24), (1100, 70, 136), (9, 1100, 136), (70, 1100, 40)])
+def test_a_head_over_more_than_4_gib(n, classes, dim, dtype):
+    """The longer side's rows, and their gradients, near the largest stride."""
+    c = head_case((n, classes, dim, 0.1, True, True, 0, 0), dtype, 5)
+    gap = (1 << 21) - 8
+    rows = max(n, classes)
+    by_rows = n == rows
+    x, y = (c["h"], c["w"]) if by_rows else (c["w"], c["h"])
+    x, dx = far(rows, dim, dtype, gap, x), far(rows, dim, dtype, gap)
+    y, dy = dev(y, dtype), like(y.shape, dtype)
+    h, w, dh, dw = (x, y, dx, dy) if by_rows else (y, x, dy, dx)
+    lse = like((n,), "float32")
+    hb.softmax_head(h, w, bias=dev(c["bias"], "float32"), labels=dev(c["labels"], "int32"),
+                    weight=dev(c["weight"], "float32"), grad_scale=c["scale"], lse=lse, dh=dh, dw=dw,
+                    workspace=work(hb.softmax_head_workspace(n, classes, dim, dtype)))
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    close(back(lse), want["lse"], "lse")
+    close(far_back(dx), want["dh" if by_rows else "dw"], "the far gradient")
+    close(back(dy), want["dw" if by_rows else "dh"], "the near gradient")
+
+
+def test_clipping_a_tensor_of_more_than_4_gib():
+    n = (1 << 30) + 1027
+    buf, out = hb.DeviceBuffer(4 * n), hb.DeviceBuffer(4 * n)
+    g, to = DeviceArray(buf, "float32", n), DeviceArray(out, "float32", n)
+    # zeros: the gradient of a table that no id leads to
+    hb.leaf_embedding_grad(dev(np.zeros((1, 1027)), "float32"), dev(np.full((1, 1), -1), "int32"),
+                           DeviceArray(buf, "float32", (n // 1027, 1027)),
+                           workspace=work(hb.leaf_embedding_grad_workspace(1, 1, n // 1027, 1027, "float32")))
+    at, held = [0, 5, 1 << 29, (1 << 30) - 1, 1 << 30, n - 1], np.float32([3, -1, 2, 5, -4, 6])
+    tail = n // 1027 * 1027
+    upload(g.data_ptr() + 4 * tail, np.zeros(n - tail, np.float32))
+    for i, v in zip(at, held):
+        upload(g.data_ptr() + 4 * i, np.float32([v]))
+    norm = like((1,), "float32")
+    hb.clip_gradients([g], 0.5, norm=norm, out=[to], workspace=work(hb.clip_gradients_workspace(1)))
+    true = np.sqrt(np.sum(held.astype(np.float64) ** 2))
+    assert abs(back(norm)[0] - true) <= R.EPS32 * true
+    one = np.empty(1, np.float32)
+    for i, v in zip(at, held):
+        A.check(A.lib().hbr_device_download(0, A.ptr(one), C.c_void_p(to.data_ptr() + 4 * i), 4))
+        # the factor's and the product's roundings
+        assert abs(one[0] - v * 0.5 / (true + 1e-6)) <= 2.01 * R.EPS32 * abs(v)
+    A.check(A.lib().hbr_device_download(0, A.ptr(one), C.c_void_p(to.data_ptr() + 4 * (n - 2)), 4))
+    assert one[0] == 0.0
+
+
 # ---- clipping ------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -130,6 +130,37 @@ def test_clipping_refuses_malformed_sets():
     assert L.hbr_clip_gradients_workspace((1 << 20) + 1, C.byref(n)) == A.REFUSED
 
 
+def test_clipping_refuses_sets_whose_outputs_overlap():
+    L, ok, big, n = A.lib(), 1 << 20, 1 << 40, 64
+    for pairs in ([(ok, ok), (ok, ok)], [(ok, ok), (ok + 4, ok + 4)], [(ok, ok + 4)], [(ok + 4, ok)],
+                  [(ok, 2 * ok), (3 * ok, 2 * ok + 252)], [(ok, 2 * ok), (2 * ok, 3 * ok)],
+                  [(5 * ok, 5 * ok), (ok, 3 * ok), (ok, 5 * ok - 4)]):
+        t = (A.Tensor * len(pairs))(*[A.Tensor(a, b, n, A.F32, 0) for a, b in pairs])
+        assert L.hbr_clip_gradients(0, t, len(pairs), 1.0, None, ok, big, None) == A.INVALID
+        assert "overlaps" in A.last_error(), pairs
+    # side by side, one tensor to two outputs, and empty ones anywhere, are not
+    for pairs, last in (([(ok, ok), (ok + 4 * n, ok + 4 * n)], n), ([(ok, 2 * ok), (ok, 3 * ok)], n), ([(ok, ok), (ok + 4, ok + 4)], 0)):
+        t = (A.Tensor * len(pairs))(*[A.Tensor(a, b, n, A.F32, 0) for a, b in pairs])
+        t[len(pairs) - 1].len = last
+        assert L.hbr_clip_gradients(99, t, len(pairs), 1.0, None, ok, big, None) != A.OK
+        assert "overlaps" not in A.last_error(), pairs
+
+
+def test_sizes_past_a_launch_are_refused():
+    L, ok, big, n = A.lib(), 1 << 20, 1 << 62, C.c_uint64()
+    p = lookup(dim=1 << 20, table_stride=1 << 20, out_stride=1 << 20)
+    assert L.hbr_leaf_embedding(0, C.byref(p), ok, ok, None) == A.REFUSED
+    assert L.hbr_leaf_embedding_grad(0, C.byref(p), ok, ok, ok, big, None) == A.REFUSED
+    assert L.hbr_softmax_head_workspace(3, 5, 1 << 20, A.F32, 1, C.byref(n)) == A.REFUSED
+    for rows, classes, dim in ((1 << 20, 1 << 18, 256), (1 << 20, 1 << 18, 8), ((1 << 31) - 1, 100, 8)):
+        p = softmax(n_rows=rows, n_classes=classes, dim=dim, h_stride=dim, w_stride=dim, dh_stride=dim, dw_stride=dim)
+        assert L.hbr_softmax_head(0, C.byref(p), ok, big, None) == A.REFUSED and "tiles" in A.last_error()
+    # many columns of long vectors are not summed a column at a time
+    for columns in (1 << 15, 1 << 15 | 1):
+        p = lookup(n_rows=1 << 12, n_columns=columns, ids_stride=columns, table_rows=1 << 15 | 1, dim=1024, table_stride=1024, out_stride=1024)
+        assert L.hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.OK and n.value > 1 << 30
+
+
 def test_python_arrays_are_checked():
     f, i = "float32", "int32"
     table, ids, out = arr(f, 10, 4), arr(i, 6, 3), arr(f, 6, 4)
