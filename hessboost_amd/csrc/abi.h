@@ -1077,8 +1077,9 @@ struct EmbedArgs {
     uint32_t pad;
 };
 
-// hbr_lookup_columns_*: rows of a block at most, and elements of a slice.
+// hbr_lookup_columns_*: rows of a block at most, keys of a round, and elements of a slice.
 constexpr uint32_t kColumnBlock = 16384;
+constexpr uint32_t kColumnKeys = 512;
 constexpr uint32_t kColumnSlice = 128;
 struct LookupColumnArgs {
     const int32_t *ids;
@@ -1103,7 +1104,7 @@ struct LookupColumnArgs {
 
 // The sort's digits, and the most entries that one workgroup sorts by itself.
 constexpr uint32_t kSortBits = 9;
-constexpr uint32_t kSortSmall = 4096;
+constexpr uint32_t kSortSmall = 1024;
 constexpr uint32_t kSortDigits = 1u << kSortBits;
 
 // The table gradient: the ids' entries (r, t) sorted by table row, stable.
@@ -1185,7 +1186,10 @@ struct HeadArgs {
     uint32_t pad2;
 };
 
-// The head over at most kFewClasses classes (hbr_few_*).
+// The head over at most kFewClasses classes (hbr_few_*), two tiles of 32.
+// 100,000 rows and 64 classes: of 50 f32 84 us, with the kernels for many classes
+// 163; of 256 bf16 121 and 115, of 512 197 and 173, of 64 63 and 78; 48 classes
+// of 256 bf16 114 either way; scores alone of 64 classes of 256 bf16 29 and 48.
 constexpr uint32_t kFewClasses = 64;
 struct FewArgs {
     const void *h, *w;
@@ -1222,8 +1226,10 @@ struct FewSumsArgs {
 };
 
 // The head's gradients over short inputs (hbr_head_narrow_*): elements at
-// most, in bf16 and in f32.
-constexpr uint32_t kNarrowDim = 128;
+// most, in bf16 and in f32. 16,384 rows and 8,192 classes: of 96 bf16 223 us,
+// 303 with pairs stored, of 128 343 and 346 (2,000 x 3,000 92 and 71); of 64 f32
+// 533 and 1,023. (120,000 rows and 600 classes of 96 bf16 are 215 and 193.)
+constexpr uint32_t kNarrowDim = 96;
 constexpr uint32_t kNarrowDimF32 = 64;
 struct NarrowArgs {
     const void *x, *y;            // the held side and the walked one, in chunks

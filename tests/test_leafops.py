@@ -161,6 +161,20 @@ def test_sizes_past_a_launch_are_refused():
         assert L.hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.OK and n.value > 1 << 30
 
 
+def test_a_named_workspace_serves_every_stride_and_offset():
+    """A gradient's way, and so its need, depends on them too."""
+    L, ok, n = A.lib(), 1 << 20, C.c_uint64()
+    for rows, columns, table_rows, dim in ((9, 1, 8, 37), (500, 1, 8, 37), (500, 20, 300, 16), (200_003, 100, 12_700, 64), (20_000, 1, 500, 256), (50_000, 3, 90, 1000)):
+        p = lookup(n_rows=rows, n_columns=columns, ids_stride=columns, table_rows=table_rows, dim=dim, table_stride=dim, out_stride=dim)
+        assert L.hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.OK
+        for stride in (dim, 1 << 20):
+            for offset in (None, ok):
+                p.out_stride, p.offset = stride, C.cast(offset, C.POINTER(C.c_int32)) if isinstance(p.offset, C.POINTER(C.c_int32)) else offset
+                # past the arguments' checks: the device is what there is not
+                assert L.hbr_leaf_embedding_grad(99, C.byref(p), ok, ok, ok, n.value, None) != A.OK
+                assert "workspace" not in A.last_error()
+
+
 def test_python_arrays_are_checked():
     f, i = "float32", "int32"
     table, ids, out = arr(f, 10, 4), arr(i, 6, 3), arr(f, 6, 4)
