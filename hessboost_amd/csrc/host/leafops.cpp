@@ -193,12 +193,12 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
     if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {  // up to eight blocks of them make a launch
         const uint64_t least = (p.n_rows + kColumnBlock - 1) / kColumnBlock;
-        const uint64_t most = std::max(least, std::min(q.n / (8 * p.table_rows), (p.n_rows + 511) / 512));
+        const uint64_t most = std::max(least, std::min({q.n / (8 * p.table_rows), (p.n_rows + 511) / 512, (uint64_t)4096}));
         const double keys = std::ceil((double)p.table_rows / p.n_columns), key_rounds = std::ceil(keys / kColumnKeys);
         uint64_t blocks = least;
         double best = 0.0;
-        for (uint64_t b = least; b <= most + 7; b++) {
-            if (b > 4 && b % 8) continue;  // whole XCDs
+        for (uint64_t b = least; b <= most + 7; b = b < 4 ? b + 1 : b / 8 * 8 + 8) {  // whole XCDs
+            if (b > 4 && b % 8) continue;
             // (whole rounds where they are few; later ones overlap)
             const double groups = (double)(b * p.n_columns * slices) / 512;
             const double rounds = groups <= 2.0 ? std::ceil(groups) : groups + 0.5;

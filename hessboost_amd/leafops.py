@@ -30,6 +30,7 @@ as a row's elements lie side by side.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import sys
 
 from . import _capi as A
@@ -61,6 +62,9 @@ class DeviceArray:
 
     def data_ptr(self):
         return self._ptr
+
+    def get_device(self):
+        return self.ordinal
 
     def numel(self):
         return self.shape[0] * (self.shape[1] if len(self.shape) == 2 else 1)
@@ -270,35 +274,33 @@ def clip_gradients(grads, max_norm, *, norm=None, out=None, workspace=None, stre
     of any shape, and each is given once; squares are summed in float64."""
     call = _Call()
     grads = list(grads)
-    out = grads if out is None else list(out)
+    out = grads if out is None or out is grads else list(out)
     if len(out) != len(grads):
         raise ValueError("out: one array a gradient is needed")
-    flat = []  # the records' words: data, out, len, dtype
-    for g, o in zip(grads, out):
-        data, n, name = _whole(call, g, "grads")
-        if o is g:
-            flat += (data, data, n, _CODE[name])
-            continue
-        to, m, other = _whole(call, o, "out")
-        if m != n or other != name:
+    data, sizes, codes = _whole(call, grads, "grads")
+    to = data
+    if out is not grads:
+        to, *others = _whole(call, out, "out")
+        if others != [sizes, codes]:
             raise ValueError("out: arrays of the gradients' sizes and types are needed")
-        flat += (data, to, n, _CODE[name])
-    arr = (C.c_uint64 * max(1, len(flat)))(*flat)
+    words = [w for record in zip(data, to, sizes, codes) for w in record]  # data, out, len, dtype
+    records = struct.pack(f"{len(words)}Q", *words)
     np_ = call.pointer(norm, "norm", "float32", 1)
     w, nbytes = call.memory(workspace)
     if call.ordinal is None:
         return
-    A.check(A.lib().hbr_clip_gradients(call.ordinal, C.cast(arr, C.POINTER(A.Tensor)), len(grads), float(max_norm), np_,
+    A.check(A.lib().hbr_clip_gradients(call.ordinal, C.cast(C.c_char_p(records), C.POINTER(A.Tensor)), len(grads), float(max_norm), np_,
                                        w, nbytes, call.stream(stream)))
 
 
-def _whole(call, a, what):
-    """A contiguous array of any shape as (address, elements, type)."""
-    if not a.is_contiguous():
-        raise ValueError(f"{what}: a contiguous array is needed")
-    n = a.numel()
-    name = _dtype(a.dtype)
-    if name not in _CODE:
-        raise ValueError(f"{what}: float32 or bfloat16 is needed, not {name}")
-    call.device(a, what)
-    return a.data_ptr(), n, name
+def _whole(call, arrays, what):
+    """Contiguous arrays of any shape as (addresses, elements, types' codes)."""
+    if not all([a.is_contiguous() for a in arrays]):
+        raise ValueError(f"{what}: contiguous arrays are needed")
+    codes = {d: _CODE.get(_dtype(d)) for d in {a.dtype for a in arrays}}
+    for d, code in codes.items():
+        if code is None:
+            raise ValueError(f"{what}: float32 or bfloat16 is needed, not {_dtype(d)}")
+    for a in {(a.__class__, a.get_device()): a for a in arrays}.values():  # one of each kind and device
+        call.device(a, what)
+    return [a.data_ptr() for a in arrays], [a.numel() for a in arrays], [codes[a.dtype] for a in arrays]
