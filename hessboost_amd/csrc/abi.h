@@ -1073,7 +1073,7 @@ struct EmbedArgs {
     uint32_t dim;
     uint32_t vecs;              // vectors a row
     uint32_t rows_per_block;
-    uint32_t columns_per_pass;  // a multiple of 8; with the rows at most 4,096 ids
+    uint32_t columns_per_pass;  // a multiple of 8, at most 1,024; with the rows at most 4,096 ids
     uint32_t pad;
 };
 

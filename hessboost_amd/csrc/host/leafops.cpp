@@ -146,7 +146,7 @@ void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *
     a.dim = p.dim;
     a.vecs = p.dim / v;
     a.rows_per_block = std::max(1u, 256 / a.vecs);
-    a.columns_per_pass = (uint32_t)std::min<uint64_t>(up(std::max(a.columns, 1u), 8), 4096 / a.rows_per_block / 8 * 8);
+    a.columns_per_pass = (uint32_t)std::min<uint64_t>(up(std::max(a.columns, 1u), 8), std::min(1024u, 4096 / a.rows_per_block / 8 * 8));
     const uint64_t blocks = (p.n_rows + a.rows_per_block - 1) / a.rows_per_block;
     const bool far = p.table_rows * p.table_stride * size >= (1ull << 31);
     const std::string k = std::string(far ? "hbr_leaf_embed_far_" : "hbr_leaf_embed_") + name_of(p.dtype) + "_" + std::to_string(v);

@@ -55,7 +55,8 @@ __device__ __forceinline__ uint64_t table_row(int32_t id, const int32_t *offset,
 __device__ __forceinline__ uint32_t nowhere() { return 0x80000000u; }  // past every buffer: reads as zero
 
 // A workgroup takes rows_per_block rows and places their ids in LDS as the
-// byte offsets of their table rows, kPlaces at a time; a thread then holds one
+// byte offsets of their table rows, kPlaces of them and kPlaceColumns columns
+// at a time; a thread then holds one
 // vector of one row's sum and walks the columns in order, eight look-ups in
 // flight. What an id costs (its check, its address) is paid once and not by
 // every vector of its row, and an id that adds nothing reads past the
@@ -64,43 +65,61 @@ __device__ __forceinline__ uint32_t nowhere() { return 0x80000000u; }  // past e
 //
 // Bound by the vectors that the L2 gives to the CUs and by their unpacking
 // (two instructions an element, 65 us of the following): 200,003 rows x 100 ids
-// of 64 bf16 out of 12,700 rows take 144 us, 17.8 TB/s of vectors; the ids
-// alone are 16 us of HBM. 32 rows x 100 ids of 32 f32: 12 us, latency.
-constexpr uint32_t kPlaces = 4096;
+// of 64 bf16 out of 12,700 rows take 112 us, 22.8 TB/s of vectors (143 with a
+// branch around each scale and a check in 64 bits of each id); the ids alone
+// are 16 us of HBM. 32 rows x 100 ids of 32 f32: 10 us, latency.
+constexpr uint32_t kPlaces = 4096, kPlaceColumns = 1024;
 template <typename E, int V, bool Far>
 __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
     using T = typename E::type;
     constexpr uint32_t kAhead = 8;
     __shared__ __align__(16) uint32_t place[kPlaces];
-    __shared__ __align__(16) float scale[kPlaces];
+    __shared__ __align__(16) float scale[kPlaceColumns];
+    __shared__ uint32_t first[kPlaceColumns], end[kPlaceColumns];  // the columns' table rows
     const uint64_t blocks = (a.n_rows + a.rows_per_block - 1) / a.rows_per_block;
     const uint32_t cells = a.rows_per_block * a.vecs, wide = a.columns_per_pass;
+    const uint32_t inverse = 0xffffffffu / wide + 1;  // q / wide = q inverse / 2^32 for q < kPlaces
+    const uint32_t row_bytes = (uint32_t)(a.table_stride * sizeof(T));
     __amdgpu_buffer_rsrc_t table = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(a.table), 0, 0x7fffffff, 0x00020000);
     for (uint64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         const uint64_t r0 = b * a.rows_per_block;
+        const uint32_t rows = (uint32_t)min((uint64_t)a.rows_per_block, a.n_rows - r0);
         for (uint32_t i0 = 0; i0 < cells; i0 += 256) {
             const uint32_t i = i0 + threadIdx.x, in = i / a.vecs, c = i % a.vecs * V;
-            const bool live = i < cells && r0 + in < a.n_rows;
+            const bool live = i < cells && in < rows;
             float acc[V] = {};
             for (uint32_t t0 = 0; t0 < a.columns; t0 += wide) {
                 if (t0 || i0 || b != blockIdx.x) __syncthreads();
-                for (uint32_t q = threadIdx.x; q < wide; q += 256)
-                    scale[q] = t0 + q >= a.columns ? 0.0f : a.scale ? a.scale[t0 + q] : 1.0f;
+                for (uint32_t q = threadIdx.x; q < wide; q += 256) {
+                    const uint32_t t = t0 + q;
+                    const bool is = t < a.columns;
+                    scale[q] = !is ? 0.0f : a.scale ? a.scale[t] : 1.0f;
+                    first[q] = is && a.offset ? (uint32_t)a.offset[t] : 0;
+                    int64_t to = is ? (int64_t)a.table_rows : 0;
+                    if (a.offset && t + 1 < a.columns) to = max((int64_t)0, min(to, (int64_t)a.offset[t + 1]));
+                    end[q] = (uint32_t)to;
+                }
+                __syncthreads();
                 for (uint32_t q = threadIdx.x; q < wide * a.rows_per_block; q += 256) {
-                    const uint32_t row = q / wide, t = t0 + q - row * wide;
-                    uint64_t v = a.table_rows;
-                    if (t < a.columns && r0 + row < a.n_rows)
-                        v = table_row(a.ids[(r0 + row) * a.ids_stride + t], a.offset, t, a.columns, a.table_rows);
-                    place[q] = v >= a.table_rows ? nowhere() : (uint32_t)(Far ? v : v * a.table_stride * sizeof(T));
+                    // a row below the table's is 2^31 or more here, and past
+                    // every end; one beyond 2^31 - 1 stays so
+                    const uint32_t row = __umulhi(q, inverse), t = q - row * wide;
+                    const int32_t id = a.ids[(r0 + min(row, rows - 1)) * a.ids_stride + min(t0 + t, a.columns - 1)];
+                    const uint32_t v = (uint32_t)id + first[t];
+                    place[q] = id < 0 || v >= end[t] ? nowhere() : Far ? v : v * row_bytes;
                 }
                 __syncthreads();
                 if (!live) continue;
                 const uint32_t here = min(wide, (a.columns - t0 + kAhead - 1) / kAhead * kAhead);
                 for (uint32_t t = 0; t < here; t += kAhead) {
                     uint32_t at[kAhead];
+                    float by[kAhead];
                     Vec<T, V> v[kAhead];
 #pragma unroll
-                    for (uint32_t j = 0; j < kAhead; j++) at[j] = place[in * wide + t + j];
+                    for (uint32_t j = 0; j < kAhead; j++) {
+                        at[j] = place[in * wide + t + j];
+                        by[j] = scale[t + j];
+                    }
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; j++) {
                         if constexpr (Far) {
@@ -115,7 +134,7 @@ __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
                     }
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; j++) {
-                        const float s = at[j] == nowhere() ? 0.0f : scale[t + j];
+                        const float s = at[j] == nowhere() ? 0.0f : by[j];  // whatever the column's scale
 #pragma unroll
                         for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s, E::up(v[j].v[k]), acc[k]);
                     }
