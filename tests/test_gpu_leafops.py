@@ -103,6 +103,9 @@ LOOKUPS = [
     (64, 5, 12, 3, "float32", True, True, 1.0, 0, 0),        # nothing adds
     (20_000, 4, 3, 8, "float32", True, True, 0.0, 0, 0),     # a few rows hold every id
     (9000, 1, 2, 40, "bfloat16", False, False, 0.0, 0, 0),
+    (300, 100, 9, 8, "bfloat16", True, True, 0.1, 0, 0),     # several passes over the columns
+    (9, 2100, 3, 2056, "bfloat16", True, True, 0.1, 0, 0),   # and over the vectors
+    (7, 1300, 3, 1028, "float32", True, False, 0.0, 4, 0),
     (0, 3, 4, 8, "float32", True, True, 0.0, 0, 0),
     (5, 0, 4, 8, "float32", False, False, 0.0, 0, 0),
 ]
@@ -309,6 +312,10 @@ HEADS = [
     (128, 4000, 64, 0.0, False, True, 0, 0),  # short inputs, classes shared out
     (5000, 70, 9, 0.1, True, True, 0, 0),     # and rows
     (900, 1100, 65, 0.3, False, True, 0, 0),
+    (4100, 130, 136, 0.1, True, True, 0, 0),  # enough rows to lay out the classes too
+    (300, 200, 97, 0.0, False, True, 0, 0),
+    (2000, 64, 7, 0.2, True, True, 0, 0),     # vectors shorter than a load
+    (40, 33, 515, 0.2, True, True, 5, 3),
 ]
 
 
