@@ -208,16 +208,16 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
                                                                    0x7fffffff, 0x00020000);
     const uint32_t dout_stride = (uint32_t)(a.dout_stride * sizeof(T)), ids_stride = (uint32_t)(a.ids_stride * 4);
     const uint32_t dout_at = (v0 + c) * (uint32_t)(V * sizeof(T));
-    auto write = [&](uint64_t row, const float(&acc)[V]) {
+    auto write = [&](uint64_t row, const float(&acc)[V], float by) {
         if (a.blocks == 1) {
             Vec<T, V> out;
 #pragma unroll
-            for (int k = 0; k < V; k++) out.v[k] = E::down(scale * acc[k]);
+            for (int k = 0; k < V; k++) out.v[k] = E::down(by * acc[k]);
             *reinterpret_cast<Vec<T, V> *>(static_cast<T *>(a.dtable) + row * a.dtable_stride + (v0 + c) * V) = out;
         } else {
             Vec<float, V> out;
 #pragma unroll
-            for (int k = 0; k < V; k++) out.v[k] = scale * acc[k];
+            for (int k = 0; k < V; k++) out.v[k] = by * acc[k];
             *reinterpret_cast<Vec<float, V> *>(a.part + ((uint64_t)block * a.table_rows + row) * a.part_stride + (v0 + c) * V) = out;
         }
     };
@@ -341,7 +341,7 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
                 for (int k = 0; k < V; k++) acc[k] += __shfl_xor(acc[k], d, kWave);
             if (group == 0 && live) {
                 if (s >= a0 && end <= a1) {
-                    write((uint64_t)(k0 + key), acc);
+                    write((uint64_t)(k0 + key), acc, scale);
                 } else {
 #pragma unroll
                     for (int k = 0; k < V; k++) edge[wave][s < a0 ? 0 : 1][c * V + k] = acc[k];
@@ -363,13 +363,13 @@ __device__ __forceinline__ void lookup_columns(const LookupColumnArgs &a) {
 #pragma unroll
                 for (int k = 0; k < V; k++) acc[k] += edge[w][0][c * V + k];
             }
-            write((uint64_t)(k0 + tail), acc);
+            write((uint64_t)(k0 + tail), acc, scale);
         }
         // rows that nothing leads to
         for (uint32_t k = thread / wide; k < keys; k += kColumnThreads / wide) {
             if (start[k] != start[k + 1] || !live) continue;
             const float none[V] = {};
-            write((uint64_t)(k0 + k), none);
+            write((uint64_t)(k0 + k), none, 1.0f);  // zeros, whatever the scale
         }
         __syncthreads();
     }

@@ -235,6 +235,34 @@ def test_what_no_id_leads_to_is_not_read(dtype):
     close(got[keep], (want[keep], bound[keep]))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, rows", [(3, 9), (700, 9), (3000, 900)])
+@pytest.mark.parametrize("bad", [np.inf, np.nan, -2.0])
+def test_a_scale_reaches_only_what_its_column_leads_to(bad, n, rows, dtype):
+    """By columns, in one block and several, and by sorting."""
+    rng = np.random.default_rng(n)
+    dim = 12
+    ids = rng.integers(0, rows // 2, (n, 3)).astype(np.int32)  # half of a column's rows have none
+    ids[::2, 1] = -1
+    off, s = np.arange(3, dtype=np.int32) * rows, np.float32([0.5, bad, 1.5])
+    table = R.rounded(rng.random((3 * rows, dim)) + 0.5, dtype)
+    d = dict(offset=dev(off, "int32"), scale=dev(s, "float32"))
+    out, finite = like((n, dim), dtype), np.where(np.isfinite(s), s, 1.0).astype(np.float32)
+    hb.leaf_embedding(dev(table, dtype), dev(ids, "int32"), out, **d)
+    got, want = back(out), R.embedding(table, ids, off, finite, dtype)
+    close(got[::2], (want[0][::2], want[1][::2]))
+    if not np.isfinite(bad):
+        assert not np.isfinite(got[1::2]).any()
+    dout, dtable = R.rounded(rng.random((n, dim)) + 0.5, dtype), like((3 * rows, dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable, **d,
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, 3, 3 * rows, dim, dtype)))
+    got, (want, bound) = back(dtable), R.embedding_grad(dout, ids, off, finite, 3 * rows, dtype)
+    hit = np.zeros(3 * rows, bool)
+    hit[rows + ids[1::2, 1]] = not np.isfinite(bad)
+    close(got[~hit], (want[~hit], bound[~hit]))
+    assert not np.isfinite(got[hit]).any()
+
+
 def test_an_embedding_gradient_is_the_differences_of_its_sum():
     """<out, dout> is linear in the table: a step along any direction changes
     it by <dtable, direction>, up to both sides' rounding bounds."""
