@@ -238,8 +238,14 @@ def softmax_head(h, w, *, bias=None, labels=None, weight=None, grad_scale=1.0, l
     (int32) = the first class of the largest z; ``dh``, ``dw`` (the inputs'
     type) and ``db`` (float32) = the gradients of grad_scale * sum(loss).
     Rows whose label is below 0 take no part in any gradient, whatever they
-    hold. A label of ``classes`` or more makes the row's loss and the
-    gradients NaN."""
+    hold. A label of ``classes`` or more makes the row's lse and loss, and the
+    gradients, NaN.
+
+    bfloat16 inputs: the scores' gradients (probability less one-hot, times
+    the row's weight) are rounded once to bfloat16 before the products that
+    make ``dh`` and ``dw``, half a step each beside the outputs' own rounding;
+    ``db`` is summed from the float32 values. With float32 inputs all of them
+    stay float32."""
     call = _Call()
     hp, (n, dim), hs = call.array(h, "h", 2, _FLOATS)
     dtype = _dtype(h.dtype)

@@ -706,7 +706,11 @@ int hbr_leaf_embedding_grad(int ordinal, const hbr_lookup *p, const void *dout, 
  *             labels lse[r] less the row's largest z;
  *   best[r] = the first class of the largest z;
  *   dh, dw, db = the gradients of grad_scale * (sum over r of loss[r]), in h,
- *             w and bias.
+ *             w and bias. For HBR_BF16 the scores' gradients (probability less
+ *             one-hot, times the row's weight) are rounded once to bf16 before
+ *             the products that make dh and dw, half a step of bf16 each beside
+ *             the outputs' own; db is summed from the f32 values, and for
+ *             HBR_F32 all of them stay f32.
  * (The lse of a row that takes no part counts inputs that are not finite as
  * zeros or not, as it comes.)
  * A label of n_classes or more makes its row's lse and loss, and the
