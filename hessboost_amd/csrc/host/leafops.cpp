@@ -512,7 +512,10 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     if ((n > 1 && p.h_stride < dim) || (classes > 1 && p.w_stride < dim) || (p.dh && n > 1 && p.dh_stride < dim) ||
         (p.dw && classes > 1 && p.dw_stride < dim))
         fail(kInvalid, std::string(what) + ": rows overlap");
-    if (p.dh_stride >= (1u << 21) || p.dw_stride >= (1u << 21))
+    // (a single row's stride counts nothing, and may be less than the row: the
+    // products' tiles tell the rows behind it by their place alone)
+    const uint64_t dh_stride = n > 1 ? p.dh_stride : dim, dw_stride = classes > 1 ? p.dw_stride : dim;
+    if ((p.dh && dh_stride >= (1u << 21)) || (p.dw && dw_stride >= (1u << 21)))
         fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
     if (!q.few && std::max(tiles(n, 128) * tiles(classes, 128), q.narrow ? tiles(n, 128) * q.splits_h : 0) >= 1u << 24)
         fail(kRefused, std::string(what) + ": 2^24 tiles of 128 rows and 128 classes or more");
@@ -545,7 +548,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     };
     const std::string sum_kernel = "hbr_head_sum_" + suffix;
     if (n == 0) {  // sums over no rows
-        if (p.dw) sum(sum_kernel.c_str(), nullptr, 0, 0, p.dw, classes, dim, p.dw_stride);
+        if (p.dw) sum(sum_kernel.c_str(), nullptr, 0, 0, p.dw, classes, dim, dw_stride);
         if (p.db) sum("hbr_head_sum_f32", nullptr, 0, 0, p.db, 1, classes, classes);
         return;
     }
@@ -572,7 +575,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         f.part_db = q.part_db;
         f.part_dw = q.dw;
         f.dh = p.dh;
-        f.dh_stride = p.dh_stride;
+        f.dh_stride = dh_stride;
         f.col_tiles = (uint32_t)tiles(dim, 32);
         f.dw = p.dw != nullptr;
         const std::string few = suffix + (classes > 32 ? "_2" : "_1");
@@ -586,7 +589,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             a.part_db = p.db ? q.part_db : nullptr;
             a.dw = p.dw;
             a.db = p.db;
-            a.dw_stride = p.dw_stride;
+            a.dw_stride = dw_stride;
             a.shares = q.shares;
             a.waves = q.score_blocks * 4;
             a.classes = (uint32_t)classes;
@@ -696,10 +699,10 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     if (q.narrow) {
         if (p.dh) {
             walk("hbr_head_narrow_dh_", true, q.splits_h, q.dh);
-            sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);
+            sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
         }
         if (p.dw || p.db) walk("hbr_head_narrow_dw_", false, q.splits_w, q.dw);
-        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.splits_w, classes * dim, p.dw, classes, dim, p.dw_stride);
+        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.splits_w, classes * dim, p.dw, classes, dim, dw_stride);
         if (p.db) sum("hbr_head_sum_f32", q.part_db, q.splits_w, classes, p.db, 1, classes, classes);
         return;
     }
@@ -738,13 +741,13 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.k = (uint32_t)n;
             c.splits = q.splits_w;
             c.scale = q.splits_w == 1 ? p.grad_scale : 1.0f;  // else the sum's
-            char *to = static_cast<char *>(p.dw) + k0 * p.dw_stride * size;
+            char *to = static_cast<char *>(p.dw) + k0 * dw_stride * size;
             const bool direct = q.splits_w == 1;
             c.c = direct ? (void *)to : q.dw;
-            c.c_stride = direct ? p.dw_stride : dim;
+            c.c_stride = direct ? dw_stride : dim;
             c.c_split = q.piece * dim;
             product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", *q.by_w, c);
-            if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, p.dw_stride);
+            if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, dw_stride);
         }
         if (p.dh) {
             HeadArgs c{};
@@ -756,13 +759,13 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.splits = q.splits_h;
             c.scale = q.sum_h ? 1.0f : p.grad_scale;
             c.c = q.sum_h ? q.dh : p.dh;
-            c.c_stride = q.sum_h ? dim : p.dh_stride;
+            c.c_stride = q.sum_h ? dim : dh_stride;
             c.c_split = n * dim;
             c.accumulate = k0 != 0;
             product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", *q.by_h, c);
         }
     }
-    if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, p.dh_stride);
+    if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
 }
 
 // ---- clipping ----------------------------------------------------------------------------

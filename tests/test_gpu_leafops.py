@@ -560,6 +560,39 @@ def test_head_gradients_are_the_differences_of_the_loss(n, classes, dim):
     assert abs((total[0] - total[1]) - slope / c["scale"]) <= slack
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stride", [0, 3, 1 << 40])
+def test_the_stride_of_a_single_row_counts_nothing(stride, dtype):
+    """A record of one row, or of one class or table row, may hold any stride
+    there: the results are those of its own length."""
+    L = A.lib()
+    for classes, dim in ((1, 24), (9, 128), (70, 128), (200, 128), (200, 500), (200, 40)):
+        c = head_case((1, classes, dim, 0.0, True, True, 0, 0), dtype, 12)
+        want = run_head(c)
+        out = {k: like((1,), "float32" if k != "best" else "int32") for k in ("loss", "lse", "best")}
+        out.update(dh=like((1, dim), dtype), dw=like((classes, dim), dtype), db=like((classes,), "float32"))
+        held = {k: dev(c[k], t) for k, t in (("h", dtype), ("w", dtype), ("bias", "float32"), ("labels", "int32"),
+                                             ("weight", "float32"))}
+        ws = work(hb.softmax_head_workspace(1, classes, dim, dtype))
+        one = stride if classes == 1 else dim
+        p = A.Softmax(A.F32 if dtype == "float32" else A.BF16, dim, 1, classes, c["scale"], stride, one, stride, one,
+                      *(held[k].data_ptr() for k in ("h", "w", "bias", "labels", "weight")),
+                      *(out[k].data_ptr() for k in ("loss", "lse", "best", "dh", "dw", "db")))
+        A.check(L.hbr_softmax_head(0, C.byref(p), ws.data_ptr(), ws.shape[0], None))
+        for k, v in out.items():
+            assert np.array_equal(back(v), want[k]), (classes, dim, k)
+    rng = np.random.default_rng(13)
+    table, dim = R.rounded(rng.standard_normal((1, 40)), dtype), 40
+    ids, out, dtable = dev(np.zeros((1, 3)), "int32"), like((1, dim), dtype), like((1, dim), dtype)
+    ws = work(hb.leaf_embedding_grad_workspace(1, 3, 1, dim, dtype))
+    p = A.Lookup(A.F32 if dtype == "float32" else A.BF16, dim, 1, 3, 0, 1, stride, stride, stride, ids.data_ptr(), None, None)
+    A.check(L.hbr_leaf_embedding(0, C.byref(p), dev(table, dtype).data_ptr(), out.data_ptr(), None))
+    A.check(L.hbr_leaf_embedding_grad(0, C.byref(p), dev(table, dtype).data_ptr(), dtable.data_ptr(), ws.data_ptr(), ws.shape[0], None))
+    one = R.embedding(table, np.zeros((1, 3), np.int32), None, None, dtype)
+    close(back(out), one)
+    close(back(dtable), one)
+
+
 # ---- arrays of more than 4 GiB ----------------------------------------------------------
 
 FAR = 9 << 30
