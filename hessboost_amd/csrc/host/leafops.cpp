@@ -16,13 +16,14 @@ constexpr uint32_t kWaveLanes = 64;
 uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 // A workspace handed out from its start, 256 bytes apart. Without memory it
-// only counts.
+// only counts. An array may have more room than the call at hand uses.
 struct Arena {
     char *base;
     uint64_t used = 0;
     explicit Arena(void *p) : base(static_cast<char *>(p)) {}
     template <typename T>
-    T *take(uint64_t n) {
+    T *take(uint64_t n, uint64_t used_of_it = 0) {
+        if (used_of_it > n) fail(kRefused, "a workspace has no room for the plan");
         T *p = base ? reinterpret_cast<T *>(base + used) : nullptr;
         used += up(n * sizeof(T), 256);
         return p;
@@ -167,13 +168,49 @@ struct LookupPlan {
     uint64_t bytes;
 };
 
+// A workspace named for some rows serves fewer: what fewer of them split finer
+// is counted by the most that any number of rows up to the given takes, here
+// the parts of the sort's chunks and tiles.
+constexpr uint64_t kSortLargeTiles = 600000;  // entries from which on the sort's tiles are large
+uint64_t sort_waves(const hbr_lookup &p) { return (p.dim * (p.dtype == HBR_F32 ? 4 : 2) + 1023) / 1024; }
+uint64_t sort_tiles(uint64_t n) {
+    const uint64_t small = (std::min(n, kSortLargeTiles - 1) + 511) / 512;
+    return n < kSortLargeTiles ? small : std::max(small, (n + 4095) / 4096);
+}
+uint64_t sort_chunks(const hbr_lookup &p, uint64_t n) {
+    uint64_t most = 0;
+    for (uint64_t chunk = 16; chunk <= 64; chunk += 8) {  // for each, the most entries that are chunked so
+        const uint64_t end = chunk == 64 ? n : std::min(n, ((chunk + 1) * 4096 - 1) / sort_waves(p));
+        most = std::max(most, (end + chunk - 1) / chunk);
+    }
+    return most;
+}
+// The bytes that sorting takes of the workspace.
+uint64_t sort_bytes(const hbr_lookup &p, uint64_t n) {
+    return 4 * up(n * 4, 256) + up(kSortDigits * sort_tiles(n) * 4, 256) + up(kSortDigits * 4, 256) +
+           up(sort_chunks(p, n) * 2 * p.dim * 4, 256);
+}
+// The blocks' sums of the columns are held in no more bytes than sorting
+// takes, and 16 MiB.
+uint64_t columns_limit(const hbr_lookup &p, uint64_t n) { return std::max<uint64_t>(sort_bytes(p, n), 16u << 20); }
+uint64_t columns_bytes(const hbr_lookup &p, uint64_t blocks) { return blocks > 1 ? up(blocks * p.table_rows * up(p.dim, 4) * 4, 256) : 0; }
+uint64_t columns_least(const hbr_lookup &p) { return (p.n_rows + kColumnBlock - 1) / kColumnBlock; }
+// (rounded up to whole XCDs)
+uint64_t columns_most(const hbr_lookup &p, uint64_t n) {
+    return 7 + std::max(columns_least(p), std::min({n / (8 * p.table_rows), (p.n_rows + 511) / 512, (uint64_t)4096}));
+}
+
+uint64_t lookup_ids(const hbr_lookup &p) {
+    if (p.n_columns && p.n_rows > 0x7fffffffull / p.n_columns)
+        fail(kRefused, "leaf embedding gradient: more than 2^31 - 1 ids");
+    return p.n_rows * p.n_columns;
+}
+
 // by_column: columns may be summed one at a time (they have table rows of their
 // own, and strides that allow it).
 LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     LookupPlan q{};
-    if (p.n_columns && p.n_rows > 0x7fffffffull / p.n_columns)
-        fail(kRefused, "leaf embedding gradient: more than 2^31 - 1 ids");
-    q.n = p.n_rows * p.n_columns;
+    q.n = lookup_ids(p);
     Arena w(workspace);
     uint32_t bits = 1;  // keys run from 0 to table_rows
     while (bits < 32 && (p.table_rows >> bits)) bits++;
@@ -192,22 +229,21 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     // against 38.
     const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
     if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {  // up to eight blocks of them make a launch
-        const uint64_t least = (p.n_rows + kColumnBlock - 1) / kColumnBlock;
-        const uint64_t most = std::max(least, std::min({q.n / (8 * p.table_rows), (p.n_rows + 511) / 512, (uint64_t)4096}));
+        const uint64_t least = columns_least(p), most = columns_most(p, q.n), limit = columns_limit(p, q.n);
         const double keys = std::ceil((double)p.table_rows / p.n_columns), key_rounds = std::ceil(keys / kColumnKeys);
-        uint64_t blocks = least;
+        uint64_t blocks = 0;
         double best = 0.0;
-        for (uint64_t b = least; b <= most + 7; b = b < 4 ? b + 1 : b / 8 * 8 + 8) {  // whole XCDs
+        for (uint64_t b = least; b <= most && columns_bytes(p, b) <= limit; b = b < 4 ? b + 1 : b / 8 * 8 + 8) {  // whole XCDs
             if (b > 4 && b % 8) continue;
             // (whole rounds where they are few; later ones overlap)
             const double groups = (double)(b * p.n_columns * slices) / 512;
             const double rounds = groups <= 2.0 ? std::ceil(groups) : groups + 0.5;
             const double cost = 8.0 + rounds * (5e-3 * (double)((p.n_rows + b - 1) / b) * key_rounds + 0.1 * keys) +
                                 (b > 1 ? 5.0 + 1.75e-6 * (double)(b * p.table_rows * p.dim) : 0.0);
-            if (best == 0.0 || cost < best) best = cost, blocks = b;
+            if (!blocks || cost < best) best = cost, blocks = b;
         }
         const double passes = q.n <= kSortSmall ? 1.0 : q.passes;
-        q.columns = best <= 4.0 + passes * (18.0 + 25e-6 * (double)q.n);
+        q.columns = blocks && best <= 4.0 + passes * (18.0 + 25e-6 * (double)q.n);
         if (q.columns) {
             q.blocks = (uint32_t)blocks;
             q.block_rows = (uint32_t)((p.n_rows + blocks - 1) / blocks);
@@ -218,21 +254,20 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     }
     // small tiles where large ones would be too few for the device (524,288
     // entries of 16 bf16 105 us against 111, 700,000 ones 118 against 114)
-    q.tile = q.n < 600000 ? 512 : 4096;
+    q.tile = q.n < kSortLargeTiles ? 512 : 4096;
     q.tiles = (uint32_t)((q.n + q.tile - 1) / q.tile);
     // 16 to 64 entries a chunk, for about 4,096 waves of 16-byte vectors: of
     // 20,000 ids of 256 bf16 42 us with 16, 48 with 32, 62 with 64; of 1,000,000
     // of 64 191 with 64 and 194 with 16 (a frequent id's parts are more)
-    const uint64_t waves = (p.dim * (p.dtype == HBR_F32 ? 4 : 2) + 1023) / 1024;
-    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(16, up(q.n * waves / 4096, 8)));
+    q.chunk = (uint32_t)std::min<uint64_t>(64, std::max<uint64_t>(16, up(q.n * sort_waves(p) / 4096, 8)));
     q.chunks = (uint32_t)((q.n + q.chunk - 1) / q.chunk);
     for (int b = 0; b < 2; b++) {
         q.key[b] = w.take<uint32_t>(q.n);
         q.val[b] = w.take<uint32_t>(q.n);
     }
-    q.hist = w.take<uint32_t>((uint64_t)kSortDigits * q.tiles);
+    q.hist = w.take<uint32_t>(kSortDigits * sort_tiles(q.n), (uint64_t)kSortDigits * q.tiles);
     q.total = w.take<uint32_t>(kSortDigits);
-    q.part = w.take<float>((uint64_t)q.chunks * 2 * p.dim);
+    q.part = w.take<float>(sort_chunks(p, q.n) * 2 * p.dim, (uint64_t)q.chunks * 2 * p.dim);
     q.bytes = w.used;
     return q;
 }
@@ -245,7 +280,10 @@ uint64_t leaf_embedding_grad_workspace(const hbr_lookup &p) {
     q.offset = nullptr;
     q.scale = nullptr;
     check_lookup(q, "leaf embedding gradient");
-    return std::max(lookup_plan(p, nullptr, false).bytes, lookup_plan(p, nullptr, true).bytes);  // whatever the arrays allow
+    // whatever the arrays allow, and of any number of rows up to the given
+    const uint64_t n = lookup_ids(p);
+    if (n == 0 || p.table_rows == 0) return sort_bytes(p, n);
+    return std::max(sort_bytes(p, n), std::min(columns_limit(p, n), columns_bytes(p, columns_most(p, n))));
 }
 
 void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const void *dout, void *dtable,
@@ -362,6 +400,14 @@ constexpr uint64_t kLayRows = 4096;
 
 uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
+// Scores alone over short inputs are made by rows too from this many on (and
+// from kLayRows rows): their partial results are held for a few shares of the
+// classes then, and not for every tile of 128 (200,000 rows, 20,000 classes of
+// 64 bf16: 115 MB against 407, and 1.12 ms against 1.78; 4,096 and 1,000 16.8 us
+// against 15.8, 200,000 and 70 41 against 48; in f32 17.8 us against 20.6 and 67
+// against 72).
+constexpr uint64_t kNarrowScores = 1u << 23;
+
 // A product's tiles, and how many of them fill 256 CUs (of the small ones twice
 // as many run at once, at hardly more rate).
 struct HeadTiling {
@@ -402,7 +448,7 @@ struct HeadPlan {
     uint64_t g_stride;
     uint64_t parts, segments, chunks;
     bool lay;     // h and w are laid out in chunks whatever their rows
-    bool narrow;  // short inputs: no pairs are stored
+    bool narrow;  // short inputs: no pairs are stored, and the scores are made by rows
     uint64_t piece, pieces;
     const HeadTiling *by_h, *by_w;  // the tiles of the products with the gradients
     uint32_t splits_h, splits_w, splits_z;  // splits_z: of the classes, for the scores over short inputs
@@ -421,6 +467,9 @@ bool head_in_place(const void *p, uint64_t stride, const hbr_softmax &a) {
            reinterpret_cast<uint64_t>(p) % 16 == 0;
 }
 
+// Every array has room for what any number of rows up to n takes (fewer rows
+// may be shared out finer, or taken in fewer pieces), and the arrays of a call
+// with gradients hold those of one without: a workspace serves smaller calls.
 HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, bool gradient, void *workspace) {
     size_of(dtype, "softmax head");
     if (classes == 0 || dim == 0) fail(kInvalid, "softmax head: no classes, or inputs of no elements");
@@ -430,7 +479,8 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
     q.parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
     q.chunks = tiles(dim, 32);
-    q.narrow = gradient && dim <= (dtype == HBR_F32 ? kNarrowDimF32 : kNarrowDim);
+    const bool short_inputs = dim <= (dtype == HBR_F32 ? kNarrowDimF32 : kNarrowDim);
+    q.narrow = short_inputs && (gradient || (n >= kLayRows && n * classes >= kNarrowScores));
     q.lay = dtype == HBR_F32 || n >= kLayRows || q.narrow;
     // shares of the walked side, for about 1,024 workgroups, or 512 of the
     // longest inputs, whose registers let fewer run at once (30,497 x 13,116
@@ -443,7 +493,8 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
         return (uint32_t)std::max<uint64_t>(1, std::min(groups / std::max<uint64_t>(1, tiles(held, 128)), tiles(walked, dtype == HBR_F32 ? 128 : 256)));
     };
     q.splits_z = shares(n, classes);
-    const uint64_t class_tiles = q.narrow ? q.splits_z : tiles(classes, kTile128.tile);
+    // rows times their shares of `walked`, at most (a tile of 128 rows a workgroup)
+    const uint64_t shared_rows = std::max(n, std::min(groups * 128, n * tiles(classes, dtype == HBR_F32 ? 128 : 256)));
     Arena w(workspace);
     q.few = classes <= kFewClasses;
     if (q.few) {
@@ -457,23 +508,27 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
         if (gradient) {
             q.g = w.take<char>(n * q.g_stride * (dtype == HBR_F32 ? 4 : 2));
             q.keep = w.take<uint32_t>(groups);
-            q.part_db = w.take<float>(q.score_blocks * 4ull * classes);
-            q.dw = w.take<float>(q.shares * classes * dim);
+            q.part_db = w.take<float>(tiles(std::min<uint64_t>(groups, 2048), 4) * 4 * classes, q.score_blocks * 4ull * classes);
+            q.dw = w.take<float>(std::min(groups, std::max<uint64_t>(1, 2048 / cols)) * classes * dim, q.shares * classes * dim);
         }
         q.bytes = w.used;
         return q;
     }
-    q.part_max = w.take<float>(class_tiles * n);
-    q.part_sum = w.take<float>(class_tiles * n);
-    q.part_best = w.take<int32_t>(class_tiles * n);
+    // of the rows whose scores are made in tiles, at most
+    const uint64_t tiled = short_inputs ? std::min(n, std::max(kLayRows - 1, (kNarrowScores - 1) / classes)) : n;
+    const uint64_t parts = std::max(tiled * tiles(classes, kTile128.tile), short_inputs ? shared_rows : 0);
+    const uint64_t parts_used = (q.narrow ? q.splits_z : tiles(classes, kTile128.tile)) * n;
+    q.part_max = w.take<float>(parts, parts_used);
+    q.part_sum = w.take<float>(parts, parts_used);
+    q.part_best = w.take<int32_t>(parts, parts_used);
     q.label_margin = w.take<float>(n);
     q.lse2 = w.take<float>(n);
     q.h = w.take<char>(q.parts * q.chunks * chunk_bytes(n));
     q.w = w.take<char>(q.parts * q.chunks * chunk_bytes(classes));
-    if (q.narrow) {
+    if (gradient && q.narrow) {
         q.splits_h = q.splits_z;
         q.splits_w = shares(classes, n);
-        q.dh = w.take<float>(q.splits_h * n * dim);
+        q.dh = w.take<float>(shared_rows * dim, q.splits_h * n * dim);
         q.dw = w.take<float>(q.splits_w * classes * dim);
         q.part_db = w.take<float>(q.splits_w * classes);
     } else if (gradient) {
@@ -487,10 +542,26 @@ HeadPlan head_plan(uint64_t n, uint64_t classes, uint64_t dim, uint32_t dtype, b
         q.splits_h = head_splits(*q.by_h, n, dim, q.piece, q.segments);
         q.splits_w = head_splits(*q.by_w, q.piece, dim, n, q.segments);
         q.sum_h = q.splits_h > 1 || q.pieces > 1;
-        q.g = w.take<char>(q.parts * (q.piece / 32) * chunk_bytes(n));
-        q.part_db = w.take<float>(tiles(n, kTile128.tile) * q.piece);
-        if (q.sum_h) q.dh = w.take<float>(q.splits_h * n * dim);
-        if (q.splits_w > 1) q.dw = w.take<float>(q.splits_w * q.piece * dim);
+        // The pairs: all classes at once, or one piece of at most kPieceBytes
+        // beside what the chunks' steps add to the fewest rows taken in pieces,
+        // or of 256 classes.
+        const uint64_t all = up(classes, 256), per = kPieceBytes / (2 * q.parts), row_tiles = tiles(n, kTile128.tile);
+        q.g = w.take<char>(q.parts * std::min(all / 32 * chunk_bytes(n),
+                                              std::max(8 * chunk_bytes(n), 2 * per + all / 32 * 3 * kChunkStep)),
+                           q.parts * (q.piece / 32) * chunk_bytes(n));
+        q.part_db = w.take<float>(std::min(row_tiles * all, std::max(row_tiles * 256, per / 128 + all)),
+                                  row_tiles * q.piece);
+        // the shares of a product: as many of its rows as fill the device once,
+        // of 16 steps each at least
+        const uint64_t fill = 65536 / tiles(dim, kTile256.tile);
+        static_assert(kTile256.slots * 256 == 65536 && kTile128.slots * 128 == 65536, "rows of a launch's tiles");
+        auto split = [&](uint64_t m, uint64_t k) {
+            const uint64_t most = tiles(k, kHeadK) * q.segments / 16;
+            return most > 1 ? std::min(fill, m * most) : 0;
+        };
+        const uint64_t sum_rows = std::max(split(n, all), q.pieces > 1 ? n : 0);
+        q.dh = w.take<float>(sum_rows * dim, q.sum_h ? q.splits_h * n * dim : 0);
+        q.dw = w.take<float>(split(all, n) * dim, q.splits_w > 1 ? q.splits_w * q.piece * dim : 0);
     }
     q.bytes = w.used;
     return q;
@@ -517,7 +588,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     const uint64_t dh_stride = n > 1 ? p.dh_stride : dim, dw_stride = classes > 1 ? p.dw_stride : dim;
     if ((p.dh && dh_stride >= (1u << 21)) || (p.dw && dw_stride >= (1u << 21)))
         fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
-    if (!q.few && std::max(tiles(n, 128) * tiles(classes, 128), q.narrow ? tiles(n, 128) * q.splits_h : 0) >= 1u << 24)
+    if (!q.few && std::max(tiles(n, 128) * tiles(classes, 128), q.narrow ? tiles(n, 128) * q.splits_z : 0) >= 1u << 24)
         fail(kRefused, std::string(what) + ": 2^24 tiles of 128 rows and 128 classes or more");
     for (const void *x : {p.h, p.w, (const void *)p.dh, (const void *)p.dw}) check_aligned(x, size, what);
     for (const void *x : {(const void *)p.bias, (const void *)p.labels, (const void *)p.weight, (const void *)p.loss,

@@ -19,8 +19,9 @@ of the tensors' device, the default stream for DeviceArrays) and returns; it
 allocates nothing and waits for nothing, so it can be captured into a graph
 (behind a first call outside one). Outputs are written into the caller's
 arrays and must not overlap inputs, except where an argument says so. A
-workspace holds what one call needs while it runs: calls, or replayed graphs,
-that may run at the same time need one each. The arrays have to live until
+workspace holds what one call needs while it runs: one named for the largest
+batch serves smaller ones of the same other sizes, and calls, or replayed
+graphs, that may run at the same time need one each. The arrays have to live until
 the queued work is done: torch tensors handed to a stream other than their
 own want ``record_stream``.
 
@@ -196,7 +197,8 @@ def leaf_embedding(table, ids, out, *, offset=None, scale=None, stream=None):
 
 
 def leaf_embedding_grad_workspace(n, columns, table_rows, dim, dtype):
-    """The bytes leaf_embedding_grad needs for n x columns ids."""
+    """The bytes leaf_embedding_grad needs for n x columns ids, or for fewer
+    rows of them."""
     out = C.c_uint64()
     p = A.Lookup(_CODE[_dtype(dtype)], dim, n, columns, 0, table_rows, dim, columns, dim, None, None, None)
     A.check(A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(out)))
@@ -219,7 +221,8 @@ def leaf_embedding_grad(dout, ids, dtable, *, offset=None, scale=None, workspace
 
 
 def softmax_head_workspace(n, classes, dim, dtype, gradient=True):
-    """The bytes softmax_head needs for n rows."""
+    """The bytes softmax_head needs for n rows or fewer, with gradients (that
+    serves calls without, too) or without."""
     out = C.c_uint64()
     A.check(A.lib().hbr_softmax_head_workspace(n, classes, dim, _CODE[_dtype(dtype)], int(gradient), C.byref(out)))
     return out.value
@@ -267,7 +270,7 @@ def softmax_head(h, w, *, bias=None, labels=None, weight=None, grad_scale=1.0, l
 
 
 def clip_gradients_workspace(n_tensors):
-    """The bytes clip_gradients needs for a set of n_tensors."""
+    """The bytes clip_gradients needs for a set of n_tensors or fewer."""
     out = C.c_uint64()
     A.check(A.lib().hbr_clip_gradients_workspace(n_tensors, C.byref(out)))
     return out.value

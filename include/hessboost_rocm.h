@@ -656,8 +656,10 @@ int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outp
  * Results do not depend on how the work was spread: the same call gives the
  * same bits. What a call needs meanwhile lies in the caller's workspace
  * (16-byte aligned, of at least the bytes that the operator's _workspace
- * call names for the same sizes): two calls that may run at the same time
- * need one each, and so do two graphs that may be replayed at the same time.
+ * call names for the same sizes; one named for more rows or tensors, the other
+ * sizes alike, serves too, and one named for gradients the head without): two
+ * calls that may run at the same time need one each, and so do two graphs that
+ * may be replayed at the same time.
  * Outputs overlap no input, except where said. Arrays have rows of
  * contiguous elements, `_stride` elements apart, of fewer than 2^20 (of dh
  * and dw fewer than 2^21 apart). Sizes past a launch, as of 2^24 tiles of 128

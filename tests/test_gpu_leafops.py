@@ -447,6 +447,21 @@ def test_rows_answered_without_labels(n, classes, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, classes, dim", [(4_100, 2_050, 24), (8_193, 1_030, 64), (130_000, 65, 33)])
+def test_many_rows_of_short_inputs_scored_alone(n, classes, dim, dtype):
+    """Without gradients, on a workspace that was named for them."""
+    c = head_case((n, classes, dim, 0.1, True, True, 0, 0), dtype, 17)
+    ws = work(hb.softmax_head_workspace(n, classes, dim, dtype))
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], 1.0, dtype)
+    check_head(run_head(c, ("loss", "lse"), workspace=ws), want)
+    got = run_head(c, ("loss", "lse", "best"), labels=False, workspace=ws)
+    check_head(got, R.head(c["h"], c["w"], c["bias"], None, None, 1.0, dtype))
+    z = c["h"] @ c["w"].T + c["bias"]
+    assert np.all(z[np.arange(n), got["best"]] >= z.max(1) - 2 * (dim + 4) * R.EPS32 * (
+        np.abs(c["h"]) @ np.abs(c["w"].T) + np.abs(c["bias"])).max(1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n, classes", [(70, 9), (5, 3000), (200, 700)])
 def test_the_first_of_equal_classes_is_the_best(n, classes, dtype):
     """Every class alike, and a later pair above the others."""

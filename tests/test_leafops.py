@@ -175,6 +175,61 @@ def test_a_named_workspace_serves_every_stride_and_offset():
                 assert "workspace" not in A.last_error()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_workspace_serves_fewer_rows_and_calls_without_gradients(dtype):
+    """A loop's last batch, and its evaluation, run on what its largest batch
+    was given."""
+    rng = np.random.default_rng(3)
+    counts = np.unique(np.r_[0:70, 4000:4200:7, 599_990:600_010, np.exp(rng.uniform(0, 13.5, 700)).astype(int)])
+    for classes, dim in ((10, 50), (64, 300), (65, 8), (200, 96), (5003, 64), (5003, 256), (30_000, 100), (8192, 1024),
+                         (131_072, 16), (131_072, 1024), (1_000_003, 200)):
+        held = 0
+        for n in counts.tolist():
+            need = hb.softmax_head_workspace(n, classes, dim, dtype)
+            assert need >= held, (n, classes, dim)
+            assert need >= hb.softmax_head_workspace(n, classes, dim, dtype, gradient=False), (n, classes, dim)
+            held = need
+        held = 0
+        for n in counts.tolist():
+            need = hb.softmax_head_workspace(n, classes, dim, dtype, gradient=False)
+            assert need >= held, (n, classes, dim)
+            held = need
+    for columns, rows, dim in ((1, 500, 64), (1, 131_072, 1024), (20, 10_220, 256), (100, 12_700, 64), (6, 594, 388), (3, 90, 5000)):
+        held = 0
+        for n in counts.tolist():
+            need = hb.leaf_embedding_grad_workspace(n, columns, rows, dim, dtype)
+            assert need >= held, (n, columns, rows, dim)
+            held = need
+    # 200,000 rows over all classes: scores alone do not hold a part of each tile of them
+    assert hb.softmax_head_workspace(200_000, 131_072, 16, dtype, gradient=False) < 200 << 20
+    held = [hb.clip_gradients_workspace(n) for n in range(400)]
+    assert held == sorted(held)
+
+
+def test_a_call_needs_no_more_than_was_named_for_more_rows():
+    """Past the arguments' checks on a workspace named for a larger batch: the
+    device is what there is not."""
+    L, ok, rng = A.lib(), 1 << 20, np.random.default_rng(4)
+    for dtype, code in (("float32", A.F32), ("bfloat16", A.BF16)):
+        for _ in range(300):
+            classes, dim = (int(v) for v in np.exp(rng.uniform(np.log([2, 4]), np.log([131_072, 1_024]))))
+            most = int(np.exp(rng.uniform(0, 12)))
+            need = hb.softmax_head_workspace(most, classes, dim, dtype)
+            for n in rng.integers(1, most + 1, 8).tolist():
+                p = softmax(dtype=code, dim=dim, n_rows=n, n_classes=classes, h_stride=dim, w_stride=dim, dh_stride=dim, dw_stride=dim)
+                assert L.hbr_softmax_head(99, C.byref(p), ok, need, None) != A.OK and "workspace" not in A.last_error()
+                p.labels = p.dh = p.dw = p.db = None
+                assert L.hbr_softmax_head(99, C.byref(p), ok, need, None) != A.OK and "workspace" not in A.last_error()
+            columns = int(rng.choice([1, 3, 40]))
+            rows = columns * int(np.exp(rng.uniform(0, 8)))
+            need = hb.leaf_embedding_grad_workspace(most, columns, rows, dim, dtype)
+            for n in rng.integers(1, most + 1, 8).tolist():
+                q = lookup(dtype=code, dim=dim, n_rows=n, n_columns=columns, ids_stride=columns, table_rows=rows,
+                           table_stride=dim, out_stride=dim, offset=ok if rng.random() < 0.7 else None)
+                assert L.hbr_leaf_embedding_grad(99, C.byref(q), ok, ok, ok, need, None) != A.OK
+                assert "workspace" not in A.last_error()
+
+
 def test_python_arrays_are_checked():
     f, i = "float32", "int32"
     table, ids, out = arr(f, 10, 4), arr(i, 6, 3), arr(f, 6, 4)
