@@ -1167,8 +1167,8 @@ struct HeadArgs {
     // scores (m: classes, n: rows) and pairs (m: rows, n: classes)
     const float *bias;            // of the first class
     const int32_t *labels;
-    float *part_max;              // [class tile][rows], in units of log2
-    float *part_sum;
+    float *part_max;              // [class tile][rows]
+    float *part_sum;              // of exp(z - part_max)
     int32_t *part_best;           // or null
     float *label_margin;          // [rows]
     const float *lse2;

@@ -74,7 +74,7 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
     using T = typename F::E::type;
     __shared__ __align__(16) float bias[32 * KT];
     if (threadIdx.x < 32 * KT)
-        bias[threadIdx.x] = threadIdx.x >= a.classes ? -INFINITY : a.bias ? a.bias[threadIdx.x] * kLog2e : 0.0f;
+        bias[threadIdx.x] = threadIdx.x >= a.classes ? -INFINITY : a.bias ? a.bias[threadIdx.x] : 0.0f;
     __syncthreads();
     const uint32_t lane = lane_id(), wave = blockIdx.x * 4 + threadIdx.x / kWave, waves = gridDim.x * 4;
     const uint32_t groups = (uint32_t)((a.rows + 31) / 32);
@@ -130,7 +130,7 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const uint32_t c = 32 * t + row_of(e);
-                const float z = c < a.classes ? __builtin_fmaf(acc[t][e], kLog2e, bias[c]) : -INFINITY;
+                const float z = c < a.classes ? acc[t][e] + bias[c] : -INFINITY;
                 acc[t][e] = z;
                 top = fmaxf(top, z);
                 if (y == (int32_t)c) at_label = z;
@@ -143,25 +143,27 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                sum += __builtin_amdgcn_exp2f(acc[t][e] - shift);
                 if (acc[t][e] == top) best = min(best, (int32_t)(32 * t + row_of(e)));
+                acc[t][e] = exp_of(acc[t][e] - shift);
+                sum += acc[t][e];
             }
         sum += __shfl_xor(sum, 32, kWave);
         at_label += __shfl_xor(at_label, 32, kWave);
         best = min(best, __shfl_xor(best, 32, kWave));
         // a label that is no class: neither a loss nor a gradient
         const bool no_class = y >= 0 && (uint32_t)y >= a.classes;
-        const float lse2 = no_class ? NAN : shift + __builtin_amdgcn_logf(sum);
+        const float more = no_class ? NAN : __builtin_amdgcn_logf(sum) * kLn2;
         const float weight = in && a.weight ? a.weight[r] : 1.0f;
         if (in && lane < 32) {
-            if (a.lse) a.lse[r] = lse2 * kLn2;
+            if (a.lse) a.lse[r] = shift + more;
             if (a.best) a.best[r] = best < (int32_t)a.classes ? best : 0;
             if (a.loss)
-                a.loss[r] = !a.labels ? (lse2 - top) * kLn2 : y < 0 ? 0.0f : no_class ? NAN : weight * ((lse2 - at_label) * kLn2);
+                a.loss[r] = !a.labels ? (shift - top) + more : y < 0 ? 0.0f : no_class ? NAN : weight * ((shift - at_label) + more);
         }
         if (!a.g) continue;
         const uint64_t kept = __ballot(y >= 0);
         if (lane == 0) a.keep[g] = (uint32_t)kept;
+        const float share = no_class ? NAN : 1.0f / sum;
         T *out = static_cast<T *>(a.g) + r * a.g_stride;
 #pragma unroll
         for (int t = 0; t < KT; t++)
@@ -171,7 +173,7 @@ __device__ __forceinline__ void few_scores(const FewArgs &a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int e = 4 * q + i;
-                    float p = __builtin_amdgcn_exp2f(acc[t][e] - lse2);
+                    float p = acc[t][e] * share;
                     if (y == (int32_t)(32 * t + row_of(e))) p -= 1.0f;
                     p = y < 0 ? 0.0f : p * weight;
                     db[t][e] += p;

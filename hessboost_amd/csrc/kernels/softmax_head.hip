@@ -9,8 +9,11 @@
 // result's own rounding. They hold no c, so that a row without a weight has
 // its label's pair near -1, which bf16 holds well, and not near -c.
 //
-// Scores are held in units of log2 (z log2 e), so that an exponential is one
-// v_exp_f32.
+// A row's maximum is kept in the scores' own units and the sum of its
+// exponentials relative to it: the largest score counts exactly one, two scores
+// that differ by a bit stay apart, and lse and loss are rounded at the size of
+// the scores' differences. (In units of log2 throughout an exponential has one
+// instruction less, and neighbours fall together: z log2 e rounds again.)
 //
 // 8 n K D operations with the gradients: the scores once for the sums and once
 // for the pairs (6 if they were kept, which takes 4 bytes a score), and both
@@ -41,6 +44,9 @@ __device__ __forceinline__ int32_t uniform(uint32_t v) { return __builtin_amdgcn
 
 // A running maximum's shift: a tile with no open class sums to zero.
 __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// exp of a difference of scores (-infinity: 0).
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
 __device__ __forceinline__ uint16_t to_bf16(float v) {
     const __bf16 b = (__bf16)v;
@@ -294,7 +300,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     head_place(a, t);
     for (uint32_t i = threadIdx.x; i < Tile::kM; i += Tile::kThreads) {
         const uint32_t c = t.m0 + i;
-        bias[i] = c >= a.m ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+        bias[i] = c >= a.m ? -INFINITY : a.bias ? a.bias[c] : 0.0f;
     }
     head_product<false, false>(a, lds, t);
     const uint32_t lane = lane_id(), wm = t.wave_m / Tile::kWaveM;
@@ -306,7 +312,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
         for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float z = __builtin_fmaf(t.acc[i][j][e], kLog2e, bias[t.wave_m + 32 * i + row_of(e)]);
+                const float z = t.acc[i][j][e] + bias[t.wave_m + 32 * i + row_of(e)];
                 t.acc[i][j][e] = z;
                 top = fmaxf(top, z);
             }
@@ -316,7 +322,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
 #pragma unroll
         for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(t.acc[i][j][e] - shift);
+            for (int e = 0; e < 16; e++) sum += exp_of(t.acc[i][j][e] - shift);
         sum += __shfl_xor(sum, 32, kWave);
         // the label's class, where it is one of the wave's
         const int64_t y = a.labels && r < a.n ? (int64_t)a.labels[r] - t.m0 - t.wave_m : -1;
@@ -349,7 +355,7 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     const float t0 = top_of[0][in], t1 = top_of[1][in], top = fmaxf(t0, t1), shift = shift_of(top);
     const uint64_t at = (uint64_t)(t.m0 / Tile::kM) * a.n + r;
     a.part_max[at] = top;
-    a.part_sum[at] = sum_of[0][in] * __builtin_amdgcn_exp2f(t0 - shift) + sum_of[1][in] * __builtin_amdgcn_exp2f(t1 - shift);
+    a.part_sum[at] = sum_of[0][in] * exp_of(t0 - shift) + sum_of[1][in] * exp_of(t1 - shift);
     if (a.part_best) a.part_best[at] = best_of[t1 > t0 ? 1 : 0][in];
 }
 
@@ -381,7 +387,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
 #pragma unroll
     for (int j = 0; j < Tile::kJ; j++) {
         const uint32_t c = t.n0 + t.wave_n + 32 * j + lane % 32;
-        bias[j] = c >= a.n ? -INFINITY : a.bias ? a.bias[c] * kLog2e : 0.0f;
+        bias[j] = c >= a.n ? -INFINITY : a.bias ? a.bias[c] : 0.0f;
         db[j] = 0.0f;
     }
 #pragma unroll
@@ -396,7 +402,7 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
             const float lse = lse_of[m], by = by_of[m];
 #pragma unroll
             for (int j = 0; j < Tile::kJ; j++)
-                t.acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][e], kLog2e, bias[j]) - lse) * by;
+                t.acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(t.acc[i][j][e] + bias[j], kLog2e, -lse)) * by;
         }
         if (labelled) {
 #pragma unroll
@@ -638,7 +644,7 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
     int32_t best = 0x7fffffff;
     auto join = [&](float m, float s, int32_t b) {
         const float both = fmaxf(top, m), shift = shift_of(both);
-        sum = sum * __builtin_amdgcn_exp2f(top - shift) + s * __builtin_amdgcn_exp2f(m - shift);
+        sum = sum * exp_of(top - shift) + s * exp_of(m - shift);
         best = m > top ? b : m == top ? min(best, b) : best;
         top = both;
     };
@@ -669,15 +675,16 @@ extern "C" __global__ __launch_bounds__(1024) void hbr_head_finish(HeadFinishArg
     for (uint32_t w = 1; w < kWaves; w++) join(top_of[w][lane], sum_of[w][lane], best_of[w][lane]);
     const int32_t y = a.labels ? a.labels[r] : -1;
     // a label that is no class: neither a loss nor a gradient
-    const float lse2 = y >= 0 && (uint64_t)y >= a.classes ? NAN : shift_of(top) + __builtin_amdgcn_logf(sum);
-    a.lse2[r] = lse2;
-    if (a.lse) a.lse[r] = lse2 * kLn2;
+    const bool no_class = y >= 0 && (uint64_t)y >= a.classes;
+    const float shift = shift_of(top), more2 = no_class ? NAN : __builtin_amdgcn_logf(sum), more = more2 * kLn2;
+    a.lse2[r] = __builtin_fmaf(shift, kLog2e, more2);
+    if (a.lse) a.lse[r] = shift + more;
     if (a.best) a.best[r] = best == 0x7fffffff ? 0 : best;  // a row of NaN has none
     if (!a.loss) return;
     if (!a.labels) {
-        a.loss[r] = (lse2 - top) * kLn2;
+        a.loss[r] = (shift - top) + more;
         return;
     }
     const float by = a.weight ? a.weight[r] : 1.0f;
-    a.loss[r] = y < 0 ? 0.0f : (uint64_t)y >= a.classes ? NAN : by * ((lse2 - a.label_margin[r]) * kLn2);
+    a.loss[r] = y < 0 ? 0.0f : no_class ? NAN : by * ((shift - a.label_margin[r]) + more);
 }

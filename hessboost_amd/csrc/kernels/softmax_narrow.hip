@@ -56,7 +56,7 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
         v_x = label_x < 0 ? -INFINITY : -a.lse2[x];
         if (a.weight && label_x >= 0) weight_x = a.weight[x];
     } else if (in && a.bias) {
-        v_x = a.bias[x] * kLog2e;
+        v_x = a.bias[x];
     }
     f32x16 out[DT];
 #pragma unroll
@@ -96,7 +96,7 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
             next_label = -1;
             if (threadIdx.x < left) {
                 if (Rows) {
-                    next_u = a.bias ? a.bias[y] * kLog2e : 0.0f;
+                    next_u = a.bias ? a.bias[y] : 0.0f;
                 } else {
                     next_label = a.labels[y];
                     next_u = next_label < 0 ? -INFINITY : -a.lse2[y];
@@ -142,7 +142,7 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
                 float most = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    z[e] = __builtin_fmaf(z[e], kLog2e, u_of[s % 2][b * 32 + row_of(e)]);
+                    z[e] += u_of[s % 2][b * 32 + row_of(e)];
                     most = fmaxf(most, z[e]);
                 }
                 if (__ballot((uint32_t)label_x - y0 < 32u))
@@ -159,14 +159,17 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
                 const float both = fmaxf(top, most), shift = shift_of(both);
                 float sum = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(z[e] - shift);
-                total = total * __builtin_amdgcn_exp2f(top - shift) + sum;
+                for (int e = 0; e < 16; e++) sum += exp_of(z[e] - shift);
+                total = total * exp_of(top - shift) + sum;
                 top = both;
                 continue;
             }
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], kLog2e, u_of[s % 2][b * 32 + row_of(e)] + v_x));
+            for (int e = 0; e < 16; e++) {
+                const float u = u_of[s % 2][b * 32 + row_of(e)];
+                // the class's bias and the row's -lse log2 e are one each of u and v_x
+                z[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] + (Rows ? u : v_x), kLog2e, Rows ? v_x : u));
+            }
             // one less where the row's label is the class, if that is anywhere here
             if (Rows) {
                 if (__ballot((uint32_t)label_x - y0 < 32u))
@@ -240,7 +243,7 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
         if (!in || half) return;
         const uint64_t at = (uint64_t)split * a.nx + x;
         a.part_max[at] = both;
-        a.part_sum[at] = total * __builtin_amdgcn_exp2f(top - shift) + sum * __builtin_amdgcn_exp2f(t - shift);
+        a.part_sum[at] = total * exp_of(top - shift) + sum * exp_of(t - shift);
         if (a.part_best) a.part_best[at] = top > t ? best : t > top ? b : min(best, b);
         return;
     }

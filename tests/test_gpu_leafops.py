@@ -473,6 +473,58 @@ def test_the_first_of_equal_classes_is_the_best(n, classes, dtype):
     assert np.all(run_head(c, ("best",), labels=False)["best"] == classes // 2)
 
 
+# few classes, tiles of products, short inputs (whose kernels give gradients alone)
+WAYS = [(9, 24), (60, 24), (300, 24), (300, 136)]
+
+
+def scored(values, n, dim, dtype):
+    """A case whose scores are exactly the values, whatever the types: inputs of zeros."""
+    classes = len(values)
+    return dict(n=n, classes=classes, dim=dim, w=np.ones((classes, dim)), h=np.zeros((n, dim)),
+                bias=np.asarray(values, np.float32).astype(np.float64), labels=np.zeros(n, np.int32), weight=None, gap=0,
+                lead=0, dtype=dtype, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes, dim", WAYS)
+def test_the_best_class_has_the_largest_score_to_the_last_bit(classes, dim, dtype):
+    """Scores one step of f32 apart, the larger one of the later class."""
+    rng = np.random.default_rng(classes)
+    for low in (1.4, 1.9, 0.7, 11.3, 22.9, -0.36, -1.42, -23.0, 1.2e7):
+        low = np.float32(low)
+        high = np.nextafter(low, np.float32(np.inf))
+        values = np.full(classes, low - np.float32(abs(low)) / 2 - 1, np.float32)
+        first, second = np.sort(rng.choice(classes, 2, replace=False))
+        values[first], values[second] = low, high
+        c = scored(values, 3, dim, dtype)
+        for outputs in (("best",), ("best", "dh")):
+            assert np.all(run_head(c, outputs, labels=len(outputs) > 1)["best"] == second), (low, outputs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes, dim", WAYS)
+@pytest.mark.parametrize("far", [0.0, 5e4, -3e6])
+def test_a_loss_is_made_of_differences_of_scores(far, classes, dim, dtype):
+    """Of scores held exactly, a loss is off by the rounding of their
+    differences, of the exponentials' sum and of its logarithm, however far
+    from zero they lie: (gap + classes + 16) half steps for the logarithm of
+    the sum, one of it and two of the loss. The exponentials are off by the
+    rounding of their arguments, at most (gap + 3) half steps."""
+    rng = np.random.default_rng(7)
+    values = np.float32(far) + rng.integers(-24, 25, classes).astype(np.float32) / 4
+    c = scored(values, 40, dim, dtype)
+    c["labels"] = rng.integers(0, classes, 40).astype(np.int32)
+    z = c["bias"]
+    tail = np.log(np.exp(z - z.max()).sum())
+    loss = z.max() - z[c["labels"]] + tail
+    gap = z.max() - z.min()
+    bound = (2 * gap + classes + 20 + 2 * tail + 2 * loss) * R.EPS32
+    for outputs in (("loss",), ("loss", "dh")):
+        close(run_head(c, outputs)["loss"], (loss, bound), outputs)
+    answer = run_head(c, ("loss",), labels=False)["loss"]
+    close(answer, (np.full(40, tail), (2 * gap + classes + 20 + 2 * tail) * R.EPS32), "answer")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n, classes, dim", [(90, 12, 20), (90, 300, 64), (90, 300, 160), (1100, 300, 136)])
 def test_shut_classes_and_rows_that_take_no_part(n, classes, dim, dtype):
