@@ -579,12 +579,12 @@ __device__ __forceinline__ void head_parts(const HeadPartsArgs &a) {
             for (int k = 0; k < 8; k++)
                 if (c + k < a.cols) v.v[k] = src[k];
         }
-        // a row that takes no part may hold anything: finite, and far from
-        // where a score would not be, so that its gradient of zero adds nothing
+        // a row that takes no part may hold anything: finite, so that its
+        // gradient of zero adds nothing
         if (a.labels && a.labels[r] < 0)
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (!(__builtin_fabsf(E::up(v.v[k])) < 1e15f)) v.v[k] = (T)0;
+                if (!(__builtin_fabsf(E::up(v.v[k])) < INFINITY)) v.v[k] = (T)0;
         Vec<uint16_t, 8> out[Parts];
 #pragma unroll
         for (int k = 0; k < 8; k++) {

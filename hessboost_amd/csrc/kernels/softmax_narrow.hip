@@ -185,9 +185,21 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
                 if (a.weight)
 #pragma unroll
                     for (int e = 0; e < 16; e++) z[e] *= weight_of[s % 2][b * 32 + row_of(e)];
-                float sum = 0.0f;  // of the block alone: the running sum may be far larger
+                auto sum_of = [&] {  // of the block alone: the running sum may be far larger
+                    float sum = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum += z[e];
+                    for (int e = 0; e < 16; e++) sum += z[e];
+                    return sum;
+                };
+                float sum = sum_of();
+                if (__ballot(sum != sum)) {
+                    // a row that takes no part may have any score: past f32's
+                    // range, less infinity, it is no number
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (label_of[s % 2][b * 32 + row_of(e)] < 0) z[e] = 0.0f;
+                    sum = sum_of();
+                }
                 db += sum;
             }
             // sixteen y a fragment, of which a lane has eight: its elements
@@ -256,7 +268,7 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const uint32_t d = 32 * t + row_of(e);
-            if (d < a.dim) part[d] = out[t][e] * weight_x;
+            if (d < a.dim) part[d] = Rows && label_x < 0 ? 0.0f : out[t][e] * weight_x;
         }
 }
 

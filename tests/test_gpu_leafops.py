@@ -551,6 +551,29 @@ def test_shut_classes_and_rows_that_take_no_part(n, classes, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes, dim", WAYS + [(300, 33)])
+def test_rows_that_take_no_part_keep_their_lse_and_reach_no_gradient(classes, dim, dtype):
+    """Finite inputs of any size in rows whose label is below 0: their lse is
+    that of any row, and scores past f32's range reach no gradient."""
+    c = head_case((90, classes, dim, 0.3, True, True, 0, 0), dtype, 16)
+    live = c["labels"] >= 0
+    dead = np.flatnonzero(~live)
+    c["h"][dead[0]] = R.rounded(c["h"][dead[0]] * 1e17, dtype)
+    want = R.head(c["h"], c["w"], c["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    close(run_head(c, ("lse", "dw"))["lse"], want["lse"], "lse")
+    c["h"][dead[1]] = R.rounded(np.where(c["h"][dead[1]] < 0, -3e38, 3e38), dtype)
+    c["w"][:, 2] = R.rounded(c["w"][:, 2] * 64, dtype)
+    c["h"][live, 2] = 0.0
+    want = R.head(np.where(live[:, None], c["h"], 0.0), c["w"], c["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    got = run_head(c, ("loss", "dh", "dw", "db"))
+    assert not got["dh"][dead].any() and not got["loss"][dead].any()
+    for k in ("dw", "db"):
+        close(got[k], want[k], k)
+    for k in ("loss", "dh"):
+        close(got[k][live], (want[k][0][live], want[k][1][live]), k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("classes, dim", [(6, 24), (200, 24), (200, 160)])
 def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dim, dtype):
     c = head_case((40, classes, dim, 0.0, False, True, 0, 0), dtype, 4)
