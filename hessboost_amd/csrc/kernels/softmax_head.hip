@@ -54,13 +54,19 @@ __device__ __forceinline__ uint16_t to_bf16(float v) {
 }
 
 // An f32 as the sum of three bf16 values, exactly: each takes the next eight
-// bits of what is left. One that is not finite, or rounds to infinity, is not
-// split.
+// bits of what is left. One that rounds to infinity is cut off instead. An
+// infinity is its sign's 1, 0 and infinity: of the six products with another
+// value's parts the last part meets only the first, which has the value's sign
+// and is zero only with it, so that their sum is what infinity times the value
+// is. (As the first part it would meet zeros, and be no number.)
 __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
     p[0] = to_bf16(v);
     if ((p[0] & 0x7f80u) == 0x7f80u) {
         if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) {
-            p[1] = p[2] = 0;
+            const bool none = (p[0] & 0x7fu) != 0;
+            p[2] = none ? 0 : p[0];
+            if (!none) p[0] = (p[0] & 0x8000u) | 0x3f80u;
+            p[1] = 0;
             return;
         }
         p[0] = (uint16_t)(__float_as_uint(v) >> 16);
@@ -304,6 +310,15 @@ __device__ __forceinline__ void head_scores(const HeadArgs &a, char *lds) {
     }
     head_product<false, false>(a, lds, t);
     const uint32_t lane = lane_id(), wm = t.wave_m / Tile::kWaveM;
+    if (t.m0 + Tile::kM > a.m) {  // classes past the last are zeros, which make no number of an infinite input
+#pragma unroll
+        for (int i = 0; i < Tile::kI; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (t.m0 + t.wave_m + 32 * i + row_of(e) >= a.m)
+#pragma unroll
+                    for (int j = 0; j < Tile::kJ; j++) t.acc[i][j][e] = 0.0f;
+    }
 #pragma unroll
     for (int j = 0; j < Tile::kJ; j++) {
         const uint32_t in = t.wave_n + 32 * j + lane % 32, r = t.n0 + in;
@@ -415,10 +430,30 @@ __device__ __forceinline__ void head_pairs(const HeadArgs &a, char *lds) {
                     if (at == 32 * j) t.acc[i][j][e] -= by;
             }
         }
+        // a row of zeros and an infinite weight are no number: there is none
+        // in the gradients of a row that takes no part
+        float sum[Tile::kJ] = {}, any = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; e++)
 #pragma unroll
-            for (int j = 0; j < Tile::kJ; j++) db[j] += t.acc[i][j][e];
+            for (int j = 0; j < Tile::kJ; j++) sum[j] += t.acc[i][j][e];
+#pragma unroll
+        for (int j = 0; j < Tile::kJ; j++) any += sum[j];
+        if (__ballot(any != any)) {
+#pragma unroll
+            for (int j = 0; j < Tile::kJ; j++) sum[j] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const bool dead = lse_of[t.wave_m + 32 * i + row_of(e)] == INFINITY;
+#pragma unroll
+                for (int j = 0; j < Tile::kJ; j++) {
+                    if (dead) t.acc[i][j][e] = 0.0f;
+                    sum[j] += t.acc[i][j][e];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < Tile::kJ; j++) db[j] += sum[j];
     }
 #pragma unroll
     for (int j = 0; j < Tile::kJ; j++) {

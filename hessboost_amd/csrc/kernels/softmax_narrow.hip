@@ -139,6 +139,10 @@ __device__ __forceinline__ void head_narrow(const NarrowArgs &a, char *lds) {
             }
             const uint32_t y0 = s * kNarrowY + b * 32;
             if constexpr (Mode == kScores) {
+                if (y0 + 32 > a.ny)  // past the last class: zeros, which make no number of an infinite input
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (y0 + row_of(e) >= a.ny) z[e] = 0.0f;
                 float most = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 16; e++) {

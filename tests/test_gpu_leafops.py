@@ -574,6 +574,29 @@ def test_rows_that_take_no_part_keep_their_lse_and_reach_no_gradient(classes, di
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes, dim", WAYS)
+def test_infinite_inputs_give_infinite_scores(classes, dim, dtype):
+    """An infinity in a class's weights, against inputs of one sign there:
+    a score of -infinity, which shuts the class as its bias does."""
+    c = head_case((70, classes, dim, 0.2, True, True, 0, 0), dtype, 14)
+    c["h"][:, 5] = R.rounded(np.abs(c["h"][:, 5]) + 0.25, dtype)
+    c["labels"] = np.where(c["labels"] >= 0, 1 + c["labels"] % (classes - 2), c["labels"]).astype(np.int32)
+    shut = dict(c, w=c["w"].copy(), bias=c["bias"].copy())
+    c["w"][0, 5] = c["w"][classes - 1, 5] = -np.inf
+    shut["w"][[0, classes - 1]] = 0.0
+    shut["bias"][[0, classes - 1]] = -np.inf
+    want = R.head(shut["h"], shut["w"], shut["bias"], c["labels"], c["weight"], c["scale"], dtype)
+    for outputs in (("loss", "lse"), ("loss", "lse", "dw", "db")):
+        check_head(run_head(c, outputs), want)
+    # and in an input: every score infinite, of its weight's sign
+    c = head_case((70, classes, dim, 0.0, False, True, 0, 0), dtype, 15)
+    c["w"][:, 3] = R.rounded(-np.abs(c["w"][:, 3]) - 0.25, dtype)
+    c["h"][7, 3] = np.inf
+    lse = run_head(c, ("lse",))["lse"]
+    assert np.isneginf(lse[7]) and np.isfinite(np.delete(lse, 7)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("classes, dim", [(6, 24), (200, 24), (200, 160)])
 def test_a_label_in_a_shut_class_has_an_infinite_loss(classes, dim, dtype):
     c = head_case((40, classes, dim, 0.0, False, True, 0, 0), dtype, 4)
