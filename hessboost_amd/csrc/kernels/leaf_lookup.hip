@@ -73,6 +73,9 @@ template <typename E, int V, bool Far>
 __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
     using T = typename E::type;
     constexpr uint32_t kAhead = 8;
+    // f32 sums eight columns by themselves first: a sum of 100 in order is off
+    // by 1.7e-7 of it, so by 0.9e-7. A bf16 result's own rounding is 2^-8.
+    constexpr bool kEights = sizeof(T) == 4;
     __shared__ __align__(16) uint32_t place[kPlaces];
     __shared__ __align__(16) float scale[kPlaceColumns];
     __shared__ uint32_t first[kPlaceColumns], end[kPlaceColumns];  // the columns' table rows
@@ -132,12 +135,17 @@ __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
                             v[j] = buffer_vec<T, V>(table, at[j] + c * (uint32_t)sizeof(T));
                         }
                     }
+                    float part[V];
+#pragma unroll
+                    for (int k = 0; k < V; k++) part[k] = kEights ? 0.0f : acc[k];
 #pragma unroll
                     for (uint32_t j = 0; j < kAhead; j++) {
                         const float s = at[j] == nowhere() ? 0.0f : by[j];  // whatever the column's scale
 #pragma unroll
-                        for (int k = 0; k < V; k++) acc[k] = __builtin_fmaf(s, E::up(v[j].v[k]), acc[k]);
+                        for (int k = 0; k < V; k++) part[k] = __builtin_fmaf(s, E::up(v[j].v[k]), part[k]);
                     }
+#pragma unroll
+                    for (int k = 0; k < V; k++) acc[k] = kEights ? acc[k] + part[k] : part[k];
                 }
             }
             if (!live) continue;

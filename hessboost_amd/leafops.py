@@ -187,7 +187,8 @@ def leaf_embedding(table, ids, out, *, offset=None, scale=None, stream=None):
     gives every column its own rows, up to the next column's; with None every
     column has the whole table. An id below 0, or one that leads out of its
     column's rows, adds nothing. Sums are float32, in the order of the
-    columns."""
+    columns (of float32 vectors eight columns by themselves, then the
+    eights)."""
     call = _Call()
     tp, (rows, dim), ts = call.array(table, "table", 2, _FLOATS)
     dtype = _dtype(table.dtype)

@@ -689,8 +689,8 @@ typedef struct hbr_lookup {
 } hbr_lookup;
 
 /* out[r] = sum over t of scale[t] * table[offset[t] + ids[r][t]], summed in
- * f32 in the order of the columns and rounded once. One column is a plain
- * scaled look-up. */
+ * f32 in the order of the columns (HBR_F32: eight of them by themselves, then
+ * the eights) and rounded once. One column is a plain scaled look-up. */
 int hbr_leaf_embedding(int ordinal, const hbr_lookup *p, const void *table, void *out, void *stream);
 /* dtable[v] = sum over every (r, t) that leads to row v of scale[t] *
  * dout[r], in f32, rounded once; rows that no id leads to are zeros. At most

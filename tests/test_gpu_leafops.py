@@ -157,6 +157,23 @@ def test_leaf_embedding_grad_sums_the_rows_that_lead_to_each_place(case):
     assert np.array_equal(back(dtable), got)
 
 
+def test_sums_of_many_columns_lose_no_more_than_a_few_steps():
+    """One vector of 1 and 127 of a little less than half a step of it. Eight
+    columns are summed by themselves, then added: a product and seven
+    additions, then one addition for each eight columns, each off by half a
+    step of the sum at most."""
+    columns, dim = 128, 8
+    table = np.full((2, dim), 0.9 * 2.0 ** -24)
+    table[0] = 1.0
+    table = R.rounded(table, "float32")
+    ids = np.ones((3, columns), np.int32)
+    ids[0, 0] = ids[1, columns // 2] = ids[2, 7] = 0
+    out = like((3, dim), "float32")
+    hb.leaf_embedding(dev(table, "float32"), dev(ids, "int32"), out)
+    want, _ = R.embedding(table, ids, None, None, "float32")
+    close(back(out), (want, (8 + columns / 8) * R.EPS32 * want))
+
+
 # table rows few and many against the ids, so that either way of the gradient runs
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("offsets", [None, (0, 0, 5, 6, 30, 41), (3, 9, 20, 30, 40, 50), (-7, -2, 0, 600, 1000, 1500),
