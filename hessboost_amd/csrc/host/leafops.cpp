@@ -84,6 +84,41 @@ void check_aligned(const void *p, uint64_t size, const char *what) {
         fail(kInvalid, std::string(what) + ": an array is not aligned to its elements");
 }
 
+// An array's bytes: rows of `width`, `stride` apart.
+struct Extent {
+    uint64_t begin, rows, width, stride;
+    Extent(const void *p, uint64_t n) : Extent(p, 1, n, n) {}
+    Extent(const void *p, uint64_t n_rows, uint64_t row, uint64_t step)
+        : begin(reinterpret_cast<uint64_t>(p)), rows(p && row ? n_rows : 0), width(row), stride(n_rows > 1 ? step : row) {}
+    uint64_t end() const { return begin + (rows - 1) * stride + width; }
+};
+
+// Whether two arrays share a byte. Rows of one stride may lie between each
+// other's; of two arrays with gaps of different strides it is not found out.
+bool overlap(const Extent &a, const Extent &b) {
+    if (!a.rows || !b.rows || a.begin >= b.end() || b.begin >= a.end()) return false;
+    if (a.stride == b.stride) {
+        const uint64_t by = b.begin >= a.begin ? (b.begin - a.begin) % a.stride
+                                               : (a.stride - (a.begin - b.begin) % a.stride) % a.stride;
+        return by < a.width || by + b.width > a.stride;
+    }
+    const bool a_whole = a.width == a.stride;
+    if (!a_whole && b.width != b.stride) return false;
+    const Extent &whole = a_whole ? a : b, &rows = a_whole ? b : a;
+    // the first of the rows that ends behind the whole array's begin
+    const uint64_t first = rows.begin + rows.width > whole.begin ? 0 : (whole.begin - rows.begin - rows.width) / rows.stride + 1;
+    return first < rows.rows && rows.begin + first * rows.stride < whole.end();
+}
+
+void check_apart(std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs, const char *what) {
+    for (auto o = outputs.begin(); o != outputs.end(); o++) {
+        for (auto other = outputs.begin(); other != o; other++)
+            if (overlap(*o, *other)) fail(kInvalid, std::string(what) + ": two outputs overlap");
+        for (const Extent &i : inputs)
+            if (overlap(*o, i)) fail(kInvalid, std::string(what) + ": an output overlaps an input");
+    }
+}
+
 // The widest vector (elements, at most 16 bytes) that divides every row
 // length, stride and address.
 uint32_t vector_width(uint64_t size, std::initializer_list<uint64_t> lengths, std::initializer_list<const void *> ptrs) {
@@ -120,6 +155,14 @@ void check_lookup(const hbr_lookup &p, const char *what) {
         fail(kRefused, std::string(what) + ": more than 2^31 - 1 rows");
 }
 
+// The table (or its gradient), the rows' vectors, and what leads from the one to the other.
+void check_lookup_apart(const hbr_lookup &p, const void *table, const void *vectors, bool out, const char *what) {
+    const uint64_t size = size_of(p.dtype, what);
+    const Extent t(table, p.table_rows, p.dim * size, p.table_stride * size), v(vectors, p.n_rows, p.dim * size, p.out_stride * size);
+    check_apart({out ? v : t}, {out ? t : v, Extent(p.ids, p.n_rows, p.n_columns * 4ull, p.ids_stride * 4),
+                                Extent(p.offset, p.n_columns * 4ull), Extent(p.scale, p.n_columns * 4ull)}, what);
+}
+
 }  // namespace
 
 void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *table, void *out) {
@@ -130,6 +173,7 @@ void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *
     if (!out || (!table && p.table_rows)) fail(kInvalid, std::string(what) + ": null argument");
     check_aligned(table, size, what);
     check_aligned(out, size, what);
+    check_lookup_apart(p, table, out, true, what);
     Queue queue(ordinal, stream);
     const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {table, out});
     EmbedArgs a{};
@@ -299,6 +343,7 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     const bool by_column = (p.n_columns == 1 || p.offset) && std::max(p.out_stride, p.ids_stride) < 32768;
     const LookupPlan q = lookup_plan(p, workspace, by_column);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
+    check_lookup_apart(p, dtable, dout, false, what);
     Queue queue(ordinal, stream);
     const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
     const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
@@ -595,6 +640,10 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
                           (const void *)p.lse, (const void *)p.best, (const void *)p.db})
         check_aligned(x, 4, what);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
+    check_apart({{p.loss, n * 4}, {p.lse, n * 4}, {p.best, n * 4}, {p.db, classes * 4},
+                 {p.dh, n, dim * size, dh_stride * size}, {p.dw, classes, dim * size, dw_stride * size}},
+                {{p.h, n, dim * size, p.h_stride * size}, {p.w, classes, dim * size, p.w_stride * size},
+                 {p.bias, classes * 4}, {p.labels, n * 4}, {p.weight, n * 4}}, what);
     Queue queue(ordinal, stream);
     const std::string suffix = name_of(p.dtype);
     const dim3 threads(256);
@@ -847,14 +896,16 @@ namespace {
 uint64_t clip_launches(uint64_t n) { return (n + kClipTensors - 1) / kClipTensors; }
 
 // No output may lie over another tensor or output, or over its own tensor but
-// in place: a tensor given twice would be scaled twice, or once.
-void check_apart(const hbr_tensor *tensors, uint64_t n, const char *what) {
+// in place: a tensor given twice would be scaled twice, or once. The norm lies
+// in none.
+void check_apart(const hbr_tensor *tensors, uint64_t n, const float *norm, const char *what) {
     struct Span {
         uint64_t begin, end;
         bool written;
     };
     std::vector<Span> spans;
-    spans.reserve(n);
+    spans.reserve(n + 1);
+    if (norm) spans.push_back({reinterpret_cast<uint64_t>(norm), reinterpret_cast<uint64_t>(norm) + sizeof(float), true});
     for (uint64_t i = 0; i < n; i++) {
         const hbr_tensor &t = tensors[i];
         const uint64_t bytes = t.len * size_of(t.dtype, what), in = reinterpret_cast<uint64_t>(t.data),
@@ -896,7 +947,7 @@ void clip_gradients(int ordinal, void *stream, const hbr_tensor *tensors, uint64
         blocks = (i % kClipTensors ? blocks : 0) + (tensors[i].len + kClipElems - 1) / kClipElems;
         if (blocks > 0x7fffffffull) fail(kRefused, std::string(what) + ": too many elements");
     }
-    check_apart(tensors, n, what);
+    check_apart(tensors, n, norm, what);
     Queue queue(ordinal, stream);
     const uint64_t launches = std::max<uint64_t>(1, clip_launches(n));
     auto fill = [&](uint64_t l, ClipArgs &a) {

@@ -18,7 +18,8 @@ as an int, or an object with a ``cuda_stream``; None: torch's current stream
 of the tensors' device, the default stream for DeviceArrays) and returns; it
 allocates nothing and waits for nothing, so it can be captured into a graph
 (behind a first call outside one). Outputs are written into the caller's
-arrays and must not overlap inputs, except where an argument says so. A
+arrays and must not overlap inputs or each other, except where an argument
+says so. A
 workspace holds what one call needs while it runs: one named for the largest
 batch serves smaller ones of the same other sizes, and calls, or replayed
 graphs, that may run at the same time need one each. The arrays have to live until

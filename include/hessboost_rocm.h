@@ -660,7 +660,9 @@ int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outp
  * sizes alike, serves too, and one named for gradients the head without): two
  * calls that may run at the same time need one each, and so do two graphs that
  * may be replayed at the same time.
- * Outputs overlap no input, except where said. Arrays have rows of
+ * Outputs overlap no input and no other output, except where said
+ * (HBR_INVALID; rows of one stride may lie between each other's, and arrays
+ * whose rows lie at different strides with gaps are not searched). Arrays have rows of
  * contiguous elements, `_stride` elements apart, of fewer than 2^20 (of dh
  * and dw fewer than 2^21 apart). Sizes past a launch, as of 2^24 tiles of 128
  * rows and 128 classes, are HBR_REFUSED. */
@@ -750,7 +752,8 @@ int hbr_softmax_head(int ordinal, const hbr_softmax *p, void *workspace, uint64_
  * sum of every element's square (f64, rounded to f32), out = data * min(1,
  * max_norm / (norm + 1e-6)). A norm that is no number makes every element
  * none. out may be data itself, and overlaps no other tensor or output
- * (HBR_INVALID: a tensor given twice would be scaled twice). */
+ * (HBR_INVALID: a tensor given twice would be scaled twice); norm lies in none
+ * of them. */
 typedef struct hbr_tensor {
     const void *data;
     void *out;

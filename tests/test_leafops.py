@@ -146,6 +146,54 @@ def test_clipping_refuses_sets_whose_outputs_overlap():
         assert "overlaps" not in A.last_error(), pairs
 
 
+def test_outputs_over_inputs_or_each_other_are_invalid():
+    L, big = A.lib(), 1 << 40
+    at = [(i + 1) << 20 for i in range(12)]  # arrays well apart
+
+    def said(call):  # past the arguments' checks the device is what there is not
+        assert call() != A.OK
+        return "overlap" in A.last_error()
+
+    def look(table=at[0], out=at[1], **kw):
+        p = lookup(n_rows=300, table_rows=500, dim=8, table_stride=8, out_stride=8, n_columns=3, ids_stride=3, offset=at[3], scale=at[4], **{"ids": at[2], **kw})
+        return [said(lambda: L.hbr_leaf_embedding(99, C.byref(p), table, out, None)),
+                said(lambda: L.hbr_leaf_embedding_grad(99, C.byref(p), out, table, at[5], big, None))]
+
+    assert look() == [False, False]
+    assert look(table=at[1]) == [True, True]
+    assert look(out=at[0] + 499 * 32) == [True, True] and look(out=at[0] + 500 * 32) == [False, False]
+    assert look(out=at[2] + 8) == [True, False] and look(table=at[2] + 8) == [False, True]
+    assert look(out=at[3] + 8) == [True, False] and look(table=at[4] - 8) == [False, True]
+    assert look(ids=at[1] - 300 * 12) == [False, False] and look(ids=at[1] - 300 * 12 + 4) == [True, False]
+
+    def head(**kw):
+        p = softmax(**{**dict(n_rows=40, n_classes=70, dim=16, h_stride=16, w_stride=16, dh_stride=16, dw_stride=16, h=at[0],
+                              w=at[1], bias=at[2], labels=at[3], weight=at[4], loss=at[5], lse=at[6], best=at[7], dh=at[8],
+                              dw=at[9], db=at[10]), **kw})
+        return said(lambda: L.hbr_softmax_head(99, C.byref(p), at[11], big, None))
+
+    assert not head()
+    assert head(dh=at[0]) and head(dw=at[1] + 69 * 32) and head(loss=at[3]) and head(lse=at[5] + 156) and head(best=at[4] - 4)
+    assert not head(lse=at[5] + 160) and not head(dh=at[0] + 40 * 32)
+    # rows beside each other in one buffer, and not quite beside
+    assert not head(h_stride=32, dh=at[0] + 32, dh_stride=32) and not head(dh=at[0] - 32, h_stride=32, dh_stride=32)
+    assert head(h_stride=32, dh=at[0] + 30, dh_stride=32) and head(h_stride=31, dh=at[0] + 32, dh_stride=31)
+    assert head(h_stride=32, dh=at[0] + 39 * 64 + 16, dh_stride=32) and not head(h_stride=32, dh=at[0] + 39 * 64 + 32, dh_stride=32)
+    # a vector within a row, and between two
+    assert head(h_stride=1024, db=at[0] + 5 * 2048 + 28) and not head(h_stride=1024, db=at[0] + 5 * 2048 + 32)
+    assert head(h_stride=1024, db=at[0] + 5 * 2048 - 276) and not head(h_stride=1024, db=at[0] + 5 * 2048 - 280)
+    # what takes no room overlaps nothing
+    assert not head(n_rows=0, dh=at[0], loss=at[3])
+
+    def clip(norm, *spans):
+        t = (A.Tensor * len(spans))(*[A.Tensor(a, b, 64, A.F32, 0) for a, b in spans])
+        return said(lambda: L.hbr_clip_gradients(99, t, len(spans), 1.0, norm, at[11], big, None))
+
+    assert not clip(at[2], (at[0], at[0]), (at[1], at[3]))
+    assert clip(at[0] + 252, (at[0], at[0])) and clip(at[1], (at[0], at[0]), (at[1], at[3])) and clip(at[3] + 4, (at[1], at[3]))
+    assert not clip(at[0] + 256, (at[0], at[0])) and not clip(at[0] - 4, (at[0], at[0]))
+
+
 def test_sizes_past_a_launch_are_refused():
     L, ok, big, n = A.lib(), 1 << 20, 1 << 62, C.c_uint64()
     p = lookup(dim=1 << 20, table_stride=1 << 20, out_stride=1 << 20)
