@@ -32,6 +32,7 @@ as a row's elements lie side by side.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import struct
 import sys
 
@@ -82,11 +83,26 @@ def _dtype(d):
     """A type's name: a string, or torch's or numpy's type object."""
     name = _names.get(d)
     if name is None:
-        name = str(getattr(d, "name", d)).rsplit(".", 1)[-1]
+        name = str(getattr(d, "name", None) or getattr(d, "__name__", d)).rsplit(".", 1)[-1]
         if name not in _SIZE:
             raise ValueError(f"unsupported type {d}: the operators take float32 or bfloat16 arrays and int32 ids")
         _names[d] = name
     return name
+
+
+def _code(d):
+    code = _CODE.get(_dtype(d))
+    if code is None:
+        raise ValueError(f"float32 or bfloat16 is needed, not {_dtype(d)}")
+    return code
+
+
+def _size(v, what, bits=32):
+    """A size that its field holds (the record's fields would cut it off)."""
+    v = operator.index(v)
+    if not 0 <= v < 1 << bits:
+        raise ValueError(f"{what}: {v} is not from 0 to 2^{bits} - 1")
+    return v
 
 
 class _Call:
@@ -175,7 +191,7 @@ _FLOATS = ("float32", "bfloat16")
 
 def _lookup(call, ids, offset, scale, dtype, dim, table_rows, table_stride, out_stride):
     p, (n, columns), stride = call.array(ids, "ids", 2, ("int32",))
-    return A.Lookup(_CODE[dtype], dim, n, columns, 0, table_rows, table_stride, stride, out_stride, p,
+    return A.Lookup(_CODE[dtype], _size(dim, "dim"), n, _size(columns, "columns"), 0, table_rows, table_stride, stride, out_stride, p,
                     call.pointer(offset, "offset", "int32", columns), call.pointer(scale, "scale", "float32", columns))
 
 
@@ -202,7 +218,9 @@ def leaf_embedding_grad_workspace(n, columns, table_rows, dim, dtype):
     """The bytes leaf_embedding_grad needs for n x columns ids, or for fewer
     rows of them."""
     out = C.c_uint64()
-    p = A.Lookup(_CODE[_dtype(dtype)], dim, n, columns, 0, table_rows, dim, columns, dim, None, None, None)
+    dim, columns = _size(dim, "dim"), _size(columns, "columns")
+    p = A.Lookup(_code(dtype), dim, _size(n, "n", 64), columns, 0, _size(table_rows, "table_rows", 64), dim, columns, dim,
+                 None, None, None)
     A.check(A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(out)))
     return out.value
 
@@ -226,7 +244,8 @@ def softmax_head_workspace(n, classes, dim, dtype, gradient=True):
     """The bytes softmax_head needs for n rows or fewer, with gradients (that
     serves calls without, too) or without."""
     out = C.c_uint64()
-    A.check(A.lib().hbr_softmax_head_workspace(n, classes, dim, _CODE[_dtype(dtype)], int(gradient), C.byref(out)))
+    A.check(A.lib().hbr_softmax_head_workspace(_size(n, "n", 64), _size(classes, "classes"), _size(dim, "dim"), _code(dtype),
+                                               int(bool(gradient)), C.byref(out)))
     return out.value
 
 
@@ -262,7 +281,7 @@ def softmax_head(h, w, *, bias=None, labels=None, weight=None, grad_scale=1.0, l
         hgp, _, hgs = call.array(dh, "dh", 2, (dtype,), (n, dim))
     if dw is not None:
         wgp, _, wgs = call.array(dw, "dw", 2, (dtype,), (classes, dim))
-    p = A.Softmax(_CODE[dtype], dim, n, classes, grad_scale, hs, ws, hgs, wgs, hp, wp,
+    p = A.Softmax(_CODE[dtype], _size(dim, "dim"), n, _size(classes, "classes"), grad_scale, hs, ws, hgs, wgs, hp, wp,
                   call.pointer(bias, "bias", "float32", classes), call.pointer(labels, "labels", "int32", n),
                   call.pointer(weight, "weight", "float32", n), call.pointer(loss, "loss", "float32", n),
                   call.pointer(lse, "lse", "float32", n), call.pointer(best, "best", "int32", n), hgp, wgp,
@@ -274,7 +293,7 @@ def softmax_head(h, w, *, bias=None, labels=None, weight=None, grad_scale=1.0, l
 def clip_gradients_workspace(n_tensors):
     """The bytes clip_gradients needs for a set of n_tensors or fewer."""
     out = C.c_uint64()
-    A.check(A.lib().hbr_clip_gradients_workspace(n_tensors, C.byref(out)))
+    A.check(A.lib().hbr_clip_gradients_workspace(_size(n_tensors, "n_tensors", 64), C.byref(out)))
     return out.value
 
 

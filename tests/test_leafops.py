@@ -315,6 +315,43 @@ def test_python_arrays_are_checked():
         hb.softmax_head_workspace(3, 5, 8, "float16")
 
 
+def test_sizes_past_a_record_s_fields_are_refused_and_not_cut_off():
+    far = dict(nbytes=1 << 60)
+    f, i = "float32", "int32"
+
+    def big(dtype, *shape):
+        return DeviceArray(Memory(**far), dtype, shape)
+
+    for bad in (dict(n=-1), dict(classes=(1 << 32) + 5), dict(dim=(1 << 32) + 8), dict(dim=-8), dict(n=1 << 64), dict(dtype="int32")):
+        with pytest.raises(ValueError):
+            hb.softmax_head_workspace(**{**dict(n=3, classes=70, dim=8, dtype=f), **bad})
+    for bad in (dict(n=-1), dict(columns=(1 << 32) + 1), dict(dim=(1 << 32) + 8), dict(table_rows=-5), dict(dtype="int32")):
+        with pytest.raises(ValueError):
+            hb.leaf_embedding_grad_workspace(**{**dict(n=3, columns=2, table_rows=8, dim=8, dtype=f), **bad})
+    with pytest.raises(ValueError):
+        hb.clip_gradients_workspace(-1)
+    wide = (1 << 32) + 8
+    with pytest.raises(ValueError, match="dim"):
+        hb.leaf_embedding(big(f, 1, wide), arr(i, 1, 1), big(f, 1, wide))
+    with pytest.raises(ValueError, match="columns"):
+        hb.leaf_embedding(arr(f, 5, 4), big(i, 1, wide), arr(f, 1, 4))
+    with pytest.raises(ValueError, match="dim"):
+        hb.leaf_embedding_grad(big(f, 1, wide), arr(i, 1, 1), big(f, 1, wide))
+    with pytest.raises(ValueError, match="dim"):
+        hb.softmax_head(big(f, 1, wide), big(f, 3, wide), loss=arr(f, 1))
+    with pytest.raises(ValueError, match="classes"):
+        hb.softmax_head(arr(f, 1, 4), big(f, wide, 4), loss=arr(f, 1))
+
+
+def test_types_are_named_or_given_as_type_objects():
+    for d in ("float32", np.float32, np.dtype(np.float32), "torch.float32"):
+        assert hb.softmax_head_workspace(3, 70, 8, d) == hb.softmax_head_workspace(3, 70, 8, "float32")
+    assert DeviceArray(Memory(), np.int32, 5).dtype == "int32"
+    for d in (np.float64, "float16", float):
+        with pytest.raises(ValueError):
+            hb.softmax_head_workspace(3, 70, 8, d)
+
+
 def test_a_device_array_fits_its_buffer():
     m = Memory(nbytes=100)
     DeviceArray(m, "float32", (5, 5))
