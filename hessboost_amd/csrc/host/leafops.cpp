@@ -250,9 +250,12 @@ uint64_t lookup_ids(const hbr_lookup &p) {
     return p.n_rows * p.n_columns;
 }
 
+// A slice's vectors of v elements, a lane each at most.
+uint32_t slice_vectors(uint32_t v) { return std::min<uint32_t>(kColumnSlice / v, kWaveLanes); }
+
 // by_column: columns may be summed one at a time (they have table rows of their
-// own, and strides that allow it).
-LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
+// own, and strides that allow it). v: the vectors' elements.
+LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column, uint32_t v) {
     LookupPlan q{};
     q.n = lookup_ids(p);
     Arena w(workspace);
@@ -271,7 +274,7 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column) {
     // with 1,024 164 against 105; 10,000 x 20 and 512 77 against 55; 130 x 100 and 127
     // 26 against 44; 20,000 ids of 256 f32 into 500 rows 46 against 28, 2,000 ids 30
     // against 38.
-    const uint64_t slices = (p.dim + kColumnSlice - 1) / kColumnSlice;
+    const uint64_t slices = (p.dim / v + slice_vectors(v) - 1) / slice_vectors(v);
     if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {  // up to eight blocks of them make a launch
         const uint64_t least = columns_least(p), most = columns_most(p, q.n), limit = columns_limit(p, q.n);
         const double keys = std::ceil((double)p.table_rows / p.n_columns), key_rounds = std::ceil(keys / kColumnKeys);
@@ -341,11 +344,11 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     check_aligned(dtable, size, what);
     // (a block's rows lie within 2 GiB of dout and of the ids)
     const bool by_column = (p.n_columns == 1 || p.offset) && std::max(p.out_stride, p.ids_stride) < 32768;
-    const LookupPlan q = lookup_plan(p, workspace, by_column);
+    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
+    const LookupPlan q = lookup_plan(p, workspace, by_column, v);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
     check_lookup_apart(p, dtable, dout, false, what);
     Queue queue(ordinal, stream);
-    const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
     const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
     auto blocks = [](uint64_t threads) { return dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16)); };
     if (q.columns) {
@@ -366,7 +369,7 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
         a.vecs = p.dim / v;
         a.block_rows = q.block_rows;
         a.blocks = q.blocks;
-        a.slice_vecs = std::min<uint32_t>(kColumnSlice / v, kWaveLanes);
+        a.slice_vecs = slice_vectors(v);
         a.slices = (a.vecs + a.slice_vecs - 1) / a.slice_vecs;
         queue.launch(("hbr_lookup_columns_" + suffix).c_str(), dim3(q.blocks * a.columns * a.slices), dim3(1024), a);
         if (q.blocks > 1) queue.launch(("hbr_lookup_join_" + suffix).c_str(), blocks(p.table_rows * a.vecs), dim3(256), a);

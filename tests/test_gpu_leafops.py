@@ -223,6 +223,19 @@ def test_many_ids_a_table_row(n, rows, columns, dim, few, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim", [(3_000, 65), (3_000, 127), (400, 193), (20_000, 129)])
+def test_columns_of_odd_widths_take_slices_of_single_elements(n, dim, dtype):
+    """Vectors that no wider load divides: 64 elements a slice and not 128."""
+    c = lookup_case((n, 9, 15, dim, dtype, True, True, 0.1, 0, 0), 5)
+    dout = R.rounded(c["rng"].standard_normal((n, dim)), dtype)
+    dtable = like((c["table_rows"], dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(c["ids"], "int32"), dtable, offset=dev(c["offset"], "int32"),
+                           scale=dev(c["scale"], "float32"),
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, 9, c["table_rows"], dim, dtype)))
+    close(back(dtable), R.embedding_grad(dout, c["ids"], c["offset"], c["scale"], c["table_rows"], dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_what_no_id_leads_to_is_not_read(dtype):
     """NaN and infinities in table rows, or in rows of dout, that no id leads
     to or from; a NaN that one leads to reaches its sums alone."""
