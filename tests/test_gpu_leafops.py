@@ -293,6 +293,47 @@ def test_a_scale_reaches_only_what_its_column_leads_to(bad, n, rows, dtype):
     assert not np.isfinite(got[hit]).any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, columns, rows, dim", [
+    (600_000, 1, 90_001, 4),       # the sort's large tiles, two passes
+    (300_001, 3, 1 << 18, 3),      # and three, tiles that end inside, no offsets
+    (5_000, 1, (1 << 18) + 9, 20), # three passes of small tiles
+    (1_100, 1, 1 << 19, 8)])
+def test_sorts_of_many_ids_and_of_large_tables(n, columns, rows, dim, dtype):
+    rng = np.random.default_rng(n)
+    ids = np.minimum((rng.random((n, columns)) ** 2 * rows).astype(np.int32), rows - 1)
+    ids[rng.random((n, columns)) < 0.02] = -1
+    ids[::5000] = rows - 1
+    s = (rng.random(columns) + 0.5).astype(np.float32)
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    dtable = like((rows, dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable, scale=dev(s, "float32"),
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, columns, rows, dim, dtype)))
+    got = back(dtable)
+    want = R.embedding_grad(dout, ids, None, s, rows, dtype)
+    close(got, want)
+    assert np.all(got[want[0].any(1) == 0] == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [300, 40_000])
+def test_rows_that_no_id_leads_from_are_not_read_by_columns(n, dtype):
+    """NaN in rows of dout whose ids add nothing, with columns of their own."""
+    rng = np.random.default_rng(n)
+    rows, columns, dim = 9, 3, 20
+    ids = rng.integers(0, rows, (n, columns)).astype(np.int32)
+    dead = rng.random(n) < 0.1
+    ids[dead] = np.where(rng.random((dead.sum(), columns)) < 0.5, -1, 5 * rows)
+    off = np.arange(columns, dtype=np.int32) * rows
+    dout = R.rounded(rng.standard_normal((n, dim)), dtype)
+    want = R.embedding_grad(dout, ids, off, None, rows * columns, dtype)
+    dout[dead] = np.where(rng.random((dead.sum(), dim)) < 0.5, np.nan, np.inf)
+    dtable = like((rows * columns, dim), dtype)
+    hb.leaf_embedding_grad(dev(dout, dtype), dev(ids, "int32"), dtable, offset=dev(off, "int32"),
+                           workspace=work(hb.leaf_embedding_grad_workspace(n, columns, rows * columns, dim, dtype)))
+    close(back(dtable), want)
+
+
 def test_an_embedding_gradient_is_the_differences_of_its_sum():
     """<out, dout> is linear in the table: a step along any direction changes
     it by <dtable, direction>, up to both sides' rounding bounds."""
