@@ -151,8 +151,9 @@ void check_lookup(const hbr_lookup &p, const char *what) {
     check_aligned(p.ids, 4, what);
     check_aligned(p.offset, 4, what);
     check_aligned(p.scale, 4, what);
-    if (p.table_rows > 0x7fffffffull || p.n_rows > 0x7fffffffull)
-        fail(kRefused, std::string(what) + ": more than 2^31 - 1 rows");
+    // (the kernels count columns by passes in 32 bits)
+    if (p.table_rows > 0x7fffffffull || p.n_rows > 0x7fffffffull || p.n_columns > 0x7fffffffu)
+        fail(kRefused, std::string(what) + ": more than 2^31 - 1 rows or columns");
 }
 
 // The table (or its gradient), the rows' vectors, and what leads from the one to the other.

@@ -674,7 +674,8 @@ int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outp
  * scale[t] times (a tree's weight; NULL: 1). offset (each tree's first node,
  * ascending) gives each column its own table rows, from its offset up to the
  * next column's; with NULL every column has the whole table. An id below 0,
- * or one that leads out of its column's rows, adds nothing. */
+ * or one that leads out of its column's rows, adds nothing. At most 2^31 - 1
+ * rows, columns and table rows (HBR_REFUSED beyond). */
 typedef struct hbr_lookup {
     uint32_t dtype;           /* of the table and the vectors */
     uint32_t dim;

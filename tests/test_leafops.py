@@ -61,6 +61,19 @@ def test_lookups_past_the_index_range_are_refused():
     assert A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.OK and n.value > 1 << 31
 
 
+def test_more_columns_than_the_kernels_count_are_refused():
+    """One row of 2^32 - 1 ids fits a device's memory, and no loop over them
+    in 32 bits would end."""
+    n, ok = C.c_uint64(), 1 << 20
+    for columns in (1 << 31, (1 << 32) - 1):
+        p = lookup(n_rows=1, n_columns=columns, ids_stride=columns, ids=1 << 50)
+        assert A.lib().hbr_leaf_embedding(99, C.byref(p), ok, 2 * ok, None) == A.REFUSED and "columns" in A.last_error()
+        assert A.lib().hbr_leaf_embedding_grad(99, C.byref(p), ok, 2 * ok, 3 * ok, 1 << 60, None) == A.REFUSED
+        assert A.lib().hbr_leaf_embedding_grad_workspace(C.byref(p), C.byref(n)) == A.REFUSED
+    p = lookup(n_rows=1, n_columns=(1 << 31) - 1, ids_stride=1 << 31, ids=1 << 50)
+    assert A.lib().hbr_leaf_embedding(99, C.byref(p), ok, 2 * ok, None) not in (A.OK, A.REFUSED)  # no such device
+
+
 def softmax(**kw):
     ok = 1 << 20
     p = dict(dtype=A.BF16, dim=8, n_rows=3, n_classes=5, grad_scale=1.0, h_stride=8, w_stride=8, dh_stride=8,
