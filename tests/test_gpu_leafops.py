@@ -1123,6 +1123,102 @@ print("torch ok", flush=True)
 """
 
 
+CAPTURED = """
+import sys, threading
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import hessboost_amd as hb
+
+
+class Step:
+    def __init__(self, seed, dtype, n, t, rows, dim, classes):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        r = lambda *s: torch.randn(s, generator=g, device="cuda")
+        self.table, self.w, self.b = r(rows * t, dim).to(dtype), r(classes, dim).mul_(0.2).to(dtype), r(classes)
+        self.ids = torch.randint(0, rows, (n, t), generator=g, device="cuda", dtype=torch.int32)
+        self.y = torch.randint(-1, classes, (n,), generator=g, device="cuda", dtype=torch.int32)
+        self.off = (torch.arange(t, device="cuda") * rows).int() if t > 1 else None
+        self.h, self.dh, self.dt, self.dw = (torch.empty_like(x) for x in (r(n, dim).to(dtype), r(n, dim).to(dtype), self.table, self.w))
+        self.db, self.loss, self.norm = torch.empty(classes, device="cuda"), torch.empty(n, device="cuda"), torch.empty(1, device="cuda")
+        self.best = torch.empty(n, dtype=torch.int32, device="cuda")
+        self.ws = [torch.empty(max(16, b), dtype=torch.uint8, device="cuda") for b in (
+            hb.softmax_head_workspace(n, classes, dim, dtype), hb.leaf_embedding_grad_workspace(n, t, rows * t, dim, dtype),
+            hb.clip_gradients_workspace(3))]
+
+    def run(self):
+        hb.leaf_embedding(self.table, self.ids, self.h, offset=self.off)
+        hb.softmax_head(self.h, self.w, bias=self.b, labels=self.y, loss=self.loss, dh=self.dh, dw=self.dw, db=self.db,
+                        grad_scale=0.5, workspace=self.ws[0])
+        hb.leaf_embedding_grad(self.dh, self.ids, self.dt, offset=self.off, workspace=self.ws[1])
+        hb.clip_gradients([self.dt, self.dw, self.db], 1.0, norm=self.norm, workspace=self.ws[2])
+        hb.softmax_head(self.h, self.w, bias=self.b, best=self.best, workspace=self.ws[0])
+
+    def outputs(self):
+        torch.cuda.synchronize()
+        return [x.clone() for x in (self.h, self.loss, self.dh, self.dt, self.dw, self.db, self.norm, self.best)]
+
+
+SIZES = [(torch.float32, 300, 5, 15, 24, 9), (torch.bfloat16, 500, 7, 31, 40, 60), (torch.float32, 900, 3, 63, 48, 300),
+         (torch.bfloat16, 700, 4, 31, 136, 200), (torch.float32, 400, 1, 3000, 200, 90), (torch.bfloat16, 1500, 1, 50000, 64, 2000)]
+# a first call of any operator; the steps' own kernels are met first in their captures
+one = torch.zeros(1, 4, device="cuda")
+hb.leaf_embedding(one, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.empty(1, 4, device="cuda"))
+graphs = []
+for k, size in enumerate(SIZES):
+    s = Step(k, *size)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.run()
+    graphs.append((s, graph))
+for turn in range(3):
+    for k, ((s, graph), size) in enumerate(zip(graphs, SIZES)):
+        t = Step(100 * turn + k, *size)
+        for mine, its in ((s.table, t.table), (s.w, t.w), (s.b, t.b), (s.ids, t.ids), (s.y, t.y)):
+            mine.copy_(its)
+        graph.replay()
+        got = s.outputs()
+        t.run()
+        assert all(torch.equal(a, b) for a, b in zip(got, t.outputs())), (turn, k)
+    print("replayed", turn, flush=True)
+# several threads at once, each on a stream of its own
+steps = [Step(k, *size) for k, size in enumerate(SIZES)]
+again = [Step(k, *size) for k, size in enumerate(SIZES)]
+for s in steps:
+    s.run()
+want = [s.outputs() for s in steps]
+streams, failed = [torch.cuda.Stream() for _ in again], []
+
+
+def work(s, stream):
+    try:
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                s.run()
+    except Exception as e:
+        failed.append(e)
+
+
+threads = [threading.Thread(target=work, args=a) for a in zip(again, streams)]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+assert not failed, failed
+for s, w in zip(again, want):
+    assert all(torch.equal(a, b) for a, b in zip(s.outputs(), w))
+print("captured ok", flush=True)
+"""
+
+
+def test_torch_graphs_and_threads_give_the_eager_bits():
+    """Steps of several sizes captured by torch, the first of their kernels'
+    calls, and several threads on streams of their own."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = CAPTURED.replace("{root!r}", repr(os.path.dirname(here))).replace("{tests!r}", repr(here))
+    r = subprocess.run([sys.executable, "-u", "-c", code], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "captured ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
 def test_torch_tensors_are_taken_on_their_stream():
     """In a process of its own: torch brings its own HIP runtime."""
     here = os.path.dirname(os.path.abspath(__file__))
