@@ -276,12 +276,14 @@ LookupPlan lookup_plan(const hbr_lookup &p, void *workspace, bool by_column, uin
     // 26 against 44; 20,000 ids of 256 f32 into 500 rows 46 against 28, 2,000 ids 30
     // against 38.
     const uint64_t slices = (p.dim / v + slice_vectors(v) - 1) / slice_vectors(v);
-    if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {  // up to eight blocks of them make a launch
+    constexpr uint64_t kGroups = (1u << 22) - 1;  // workgroups of 1,024 that make a launch
+    if (by_column && q.n && p.table_rows && p.n_columns * slices <= 1u << 18) {
         const uint64_t least = columns_least(p), most = columns_most(p, q.n), limit = columns_limit(p, q.n);
         const double keys = std::ceil((double)p.table_rows / p.n_columns), key_rounds = std::ceil(keys / kColumnKeys);
         uint64_t blocks = 0;
         double best = 0.0;
-        for (uint64_t b = least; b <= most && columns_bytes(p, b) <= limit; b = b < 4 ? b + 1 : b / 8 * 8 + 8) {  // whole XCDs
+        for (uint64_t b = least; b <= most && b * p.n_columns * slices <= kGroups && columns_bytes(p, b) <= limit;
+             b = b < 4 ? b + 1 : b / 8 * 8 + 8) {  // whole XCDs
             if (b > 4 && b % 8) continue;
             // (whole rounds where they are few; later ones overlap)
             const double groups = (double)(b * p.n_columns * slices) / 512;
