@@ -1226,9 +1226,9 @@ struct FewSumsArgs {
 };
 
 // The head's gradients over short inputs (hbr_head_narrow_*): elements at
-// most, in bf16 and in f32. 16,384 rows and 8,192 classes: of 96 bf16 223 us,
+// most, in bf16 and in f32. 16,384 rows and 8,192 classes: of 96 bf16 228 us,
 // 303 with pairs stored, of 128 343 and 346 (2,000 x 3,000 92 and 71); of 64 f32
-// 533 and 1,023. (120,000 rows and 600 classes of 96 bf16 are 215 and 193.)
+// 541 and 1,023. (120,000 rows and 600 classes of 96 bf16 are 215 and 193.)
 constexpr uint32_t kNarrowDim = 96;
 constexpr uint32_t kNarrowDimF32 = 64;
 struct NarrowArgs {

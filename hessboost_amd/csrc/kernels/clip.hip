@@ -9,8 +9,8 @@
 // second pass, so that the bits do not depend on the schedule and no third
 // launch joins them. The records of 96 tensors travel as the kernel's
 // argument: nothing is copied to the device. Bound by HBM: 400,000,003 bf16
-// elements take 163 us (4.9 TB/s) and 281 us (5.7, part of it out of the last
-// level's cache); 40 tensors of 300,001 f32 in all 7 and 5 us, their launches.
+// elements take 164 us (4.9 TB/s) and 279 us (5.7, part of it out of the last
+// level's cache); 40 tensors of 300,001 f32 in all 5.7 and 5.3 us, their launches.
 #include "common.h"
 
 namespace hbr {

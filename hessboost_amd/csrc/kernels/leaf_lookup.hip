@@ -169,8 +169,8 @@ __device__ __forceinline__ void leaf_embed(const EmbedArgs &a) {
 //
 // No id is written to memory, and the rows of dout that a block gathers stay
 // in the L2 of the XCD that has the block. Bound by instructions (the VALU is
-// busy 55% of the time: ranks, and two an element summed) and the gathers:
-// 200,003 x 100 ids of 64 bf16 into 12,700 rows 289 us, and 9 to join the
+// busy 57% of the time: ranks, and two an element summed) and the gathers:
+// 200,003 x 100 ids of 64 bf16 into 12,700 rows 288 us, and 9 to join the
 // blocks' sums, 8.9 TB/s of vectors; 4,000 x 20 ids of 16 f32 15 and 4 us.
 constexpr uint32_t kColumnThreads = 1024, kColumnWaves = kColumnThreads / kWave;
 constexpr uint32_t kColumnSteps = kColumnBlock / kColumnThreads;

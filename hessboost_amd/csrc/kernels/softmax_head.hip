@@ -17,13 +17,13 @@
 //
 // 8 n K D operations with the gradients: the scores once for the sums and once
 // for the pairs (6 if they were kept, which takes 4 bytes a score), and both
-// products with the pairs. Bound by the matrix cores at the clock that the
-// power limit leaves them (1.45 to 1.6 GHz while they are busy) and by the
-// exponentials between: 16,384 x 131,072 x 1,024 bf16 scores 4.5 ms (0.98
-// PFLOP/s), pairs 5.1 (0.87), dw 4.0 and dh 3.9 (1.1). f32 operands are three
-// bf16 parts, of whose nine products the six that matter are made: 4,096 x
-// 5,003 x 256 scores 69 us (152 TFLOP/s of f32, about a library product in f32),
-// pairs 82, dw 75, dh 71. One row against 131,072 classes of 1,024 bf16: 56 us,
+// products with the pairs. Bound by the products' pipeline, whose every step of
+// 32 waits for its last load (the matrix cores are busy 57% of the cycles, 45%
+// in the pairs), and by the exponentials between: 16,384 x 131,072 x 1,024 bf16
+// scores 4.4 ms (1.0 PFLOP/s), pairs 5.1 (0.86), dw 4.0 and dh 3.9 (1.1). f32
+// operands are three bf16 parts, of whose nine products the six that matter are
+// made: 4,096 x 5,003 x 256 scores 68 us (154 TFLOP/s of f32, a library product's
+// in f32), pairs 84, dw 74, dh 71. One row against 131,072 classes of 1,024 bf16: 56 us,
 // w read at 4.8 TB/s.
 #include "common.h"
 
@@ -141,6 +141,8 @@ struct Operand {
         }
 #pragma unroll
         for (int j = 0; j < kLoads; j++)
+            // (m0 is the compiler's to set before each use of its own, and nothing
+            // here keeps a value in it)
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(to + j * 1024), "v"(from[j]), "s"(r)

@@ -9,7 +9,7 @@
 // saved is the pairs' traffic, 6 bytes a score in bf16 and 30 in f32's parts
 // (written once, read twice), against 2 dim operations. Bound by the
 // exponentials and their surroundings, about ten instructions a score: 16,384 x
-// 8,192 scores of 64 bf16, made three times, take 177 us, 2.3e12 a second.
+// 8,192 scores of 64 bf16, made three times, take 184 us, 2.2e12 a second.
 //
 // The first product leaves a lane one x and, of sixteen y, the eight that the
 // second product's operand takes from it, in an order that the transposing
