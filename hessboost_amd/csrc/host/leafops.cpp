@@ -110,7 +110,10 @@ bool overlap(const Extent &a, const Extent &b) {
     return first < rows.rows && rows.begin + first * rows.stride < whole.end();
 }
 
-void check_apart(std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs, const char *what) {
+void check_apart(std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs, const Extent &workspace, const char *what) {
+    for (const auto &list : {outputs, inputs})
+        for (const Extent &a : list)
+            if (overlap(a, workspace)) fail(kInvalid, std::string(what) + ": an array lies in the memory for the call's own use");
     for (auto o = outputs.begin(); o != outputs.end(); o++) {
         for (auto other = outputs.begin(); other != o; other++)
             if (overlap(*o, *other)) fail(kInvalid, std::string(what) + ": two outputs overlap");
@@ -157,11 +160,11 @@ void check_lookup(const hbr_lookup &p, const char *what) {
 }
 
 // The table (or its gradient), the rows' vectors, and what leads from the one to the other.
-void check_lookup_apart(const hbr_lookup &p, const void *table, const void *vectors, bool out, const char *what) {
+void check_lookup_apart(const hbr_lookup &p, const void *table, const void *vectors, bool out, const Extent &workspace, const char *what) {
     const uint64_t size = size_of(p.dtype, what);
     const Extent t(table, p.table_rows, p.dim * size, p.table_stride * size), v(vectors, p.n_rows, p.dim * size, p.out_stride * size);
     check_apart({out ? v : t}, {out ? t : v, Extent(p.ids, p.n_rows, p.n_columns * 4ull, p.ids_stride * 4),
-                                Extent(p.offset, p.n_columns * 4ull), Extent(p.scale, p.n_columns * 4ull)}, what);
+                                Extent(p.offset, p.n_columns * 4ull), Extent(p.scale, p.n_columns * 4ull)}, workspace, what);
 }
 
 }  // namespace
@@ -174,7 +177,7 @@ void leaf_embedding(int ordinal, void *stream, const hbr_lookup &p, const void *
     if (!out || (!table && p.table_rows)) fail(kInvalid, std::string(what) + ": null argument");
     check_aligned(table, size, what);
     check_aligned(out, size, what);
-    check_lookup_apart(p, table, out, true, what);
+    check_lookup_apart(p, table, out, true, Extent(nullptr, 0), what);
     Queue queue(ordinal, stream);
     const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {table, out});
     EmbedArgs a{};
@@ -350,7 +353,7 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
     const uint32_t v = vector_width(size, {p.dim, p.table_stride, p.out_stride}, {dout, dtable});
     const LookupPlan q = lookup_plan(p, workspace, by_column, v);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
-    check_lookup_apart(p, dtable, dout, false, what);
+    check_lookup_apart(p, dtable, dout, false, Extent(workspace, q.bytes), what);
     Queue queue(ordinal, stream);
     const std::string suffix = std::string(name_of(p.dtype)) + "_" + std::to_string(v);
     auto blocks = [](uint64_t threads) { return dim3((uint32_t)std::min<uint64_t>((threads + 255) / 256, 1u << 16)); };
@@ -649,7 +652,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     check_apart({{p.loss, n * 4}, {p.lse, n * 4}, {p.best, n * 4}, {p.db, classes * 4},
                  {p.dh, n, dim * size, dh_stride * size}, {p.dw, classes, dim * size, dw_stride * size}},
                 {{p.h, n, dim * size, p.h_stride * size}, {p.w, classes, dim * size, p.w_stride * size},
-                 {p.bias, classes * 4}, {p.labels, n * 4}, {p.weight, n * 4}}, what);
+                 {p.bias, classes * 4}, {p.labels, n * 4}, {p.weight, n * 4}}, Extent(workspace, q.bytes), what);
     Queue queue(ordinal, stream);
     const std::string suffix = name_of(p.dtype);
     const dim3 threads(256);
@@ -954,6 +957,12 @@ void clip_gradients(int ordinal, void *stream, const hbr_tensor *tensors, uint64
         if (blocks > 0x7fffffffull) fail(kRefused, std::string(what) + ": too many elements");
     }
     check_apart(tensors, n, norm, what);
+    const Extent room(workspace, clip_gradients_workspace(n));
+    for (uint64_t i = 0; i < n; i++)
+        for (const void *x : {tensors[i].data, (const void *)tensors[i].out})
+            if (overlap(room, Extent(x, tensors[i].len * size_of(tensors[i].dtype, what))))
+                fail(kInvalid, std::string(what) + ": a tensor lies in the memory for the call's own use");
+    if (overlap(room, Extent(norm, sizeof(float)))) fail(kInvalid, std::string(what) + ": the norm lies in the memory for the call's own use");
     Queue queue(ordinal, stream);
     const uint64_t launches = std::max<uint64_t>(1, clip_launches(n));
     auto fill = [&](uint64_t l, ClipArgs &a) {

@@ -18,12 +18,11 @@ as an int, or an object with a ``cuda_stream``; None: torch's current stream
 of the tensors' device, the default stream for DeviceArrays) and returns; it
 allocates nothing and waits for nothing, so it can be captured into a graph
 (behind a first call outside one). Outputs are written into the caller's
-arrays and must not overlap inputs or each other, except where an argument
-says so. A
-workspace holds what one call needs while it runs: one named for the largest
-batch serves smaller ones of the same other sizes, and calls, or replayed
-graphs, that may run at the same time need one each. The arrays have to live until
-the queued work is done: torch tensors handed to a stream other than their
+arrays and must not overlap inputs, each other or the workspace, except where
+an argument says so. A workspace holds what one call needs while it runs: one
+named for the largest batch serves smaller ones of the same other sizes, and
+calls, or replayed graphs, that may run at the same time need one each. The
+arrays have to live until the queued work is done: torch tensors handed to a stream other than their
 own want ``record_stream``.
 
 Vectors and inputs are shorter than 2^20 elements; strides are free as long

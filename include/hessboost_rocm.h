@@ -660,12 +660,12 @@ int hbr_pred_transform(int kind, float *values, uint64_t n_rows, uint32_t n_outp
  * sizes alike, serves too, and one named for gradients the head without): two
  * calls that may run at the same time need one each, and so do two graphs that
  * may be replayed at the same time.
- * Outputs overlap no input and no other output, except where said
- * (HBR_INVALID; rows of one stride may lie between each other's, and arrays
- * whose rows lie at different strides with gaps are not searched). Arrays have rows of
- * contiguous elements, `_stride` elements apart, of fewer than 2^20 (of dh
- * and dw fewer than 2^21 apart). Sizes past a launch, as of 2^24 tiles of 128
- * rows and 128 classes, are HBR_REFUSED. */
+ * Outputs overlap no input and no other output, except where said, and the
+ * workspace none of them (HBR_INVALID; rows of one stride may lie between each
+ * other's, and arrays whose rows lie at different strides with gaps are not
+ * searched). Arrays have rows of contiguous elements, `_stride` elements
+ * apart, of fewer than 2^20 (of dh and dw fewer than 2^21 apart). Sizes past a
+ * launch, as of 2^24 tiles of 128 rows and 128 classes, are HBR_REFUSED. */
 #define HBR_F32 0
 #define HBR_BF16 1
 

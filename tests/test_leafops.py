@@ -207,6 +207,27 @@ def test_outputs_over_inputs_or_each_other_are_invalid():
     assert not clip(at[0] + 256, (at[0], at[0])) and not clip(at[0] - 4, (at[0], at[0]))
 
 
+def test_a_workspace_over_an_array_is_invalid():
+    L, big = A.lib(), 1 << 40
+    at = [(i + 1) << 24 for i in range(12)]
+
+    def lies_over(call):
+        assert call() != A.OK
+        return "the call's own use" in A.last_error()
+
+    need = hb.leaf_embedding_grad_workspace(300, 3, 500, 8, "float32")
+    p = lookup(n_rows=300, table_rows=500, dim=8, table_stride=8, out_stride=8, n_columns=3, ids_stride=3, ids=at[2], scale=at[4])
+    for w, over in ((at[8], False), (at[2] - 16, True), (at[0] + 256, True), (at[1] + 500 * 32, False), (at[4], True)):
+        assert lies_over(lambda: L.hbr_leaf_embedding_grad(99, C.byref(p), at[0], at[1], w, max(need, big), None)) == over, w
+    q = softmax(n_rows=40, n_classes=70, dim=16, h_stride=16, w_stride=16, dh_stride=16, dw_stride=16, h=at[0], w=at[1], bias=at[2],
+                labels=at[3], weight=at[4], loss=at[5], lse=at[6], best=at[7], dh=at[8], dw=at[9], db=at[10])
+    for w, over in ((at[11], False), (at[0], True), (at[9] - 256, True), (at[10] + 512, False), (at[3] - 64, True)):
+        assert lies_over(lambda: L.hbr_softmax_head(99, C.byref(q), w, big, None)) == over, w
+    t = A.Tensor(at[0], at[1], 64, A.F32, 0)
+    for w, over in ((at[3], False), (at[0] - 16, True), (at[1] + 240, True), (at[1] + 256, False), (at[2] - 16, True)):
+        assert lies_over(lambda: L.hbr_clip_gradients(99, C.byref(t), 1, 1.0, at[2], w, big, None)) == over, w
+
+
 def test_sizes_past_a_launch_are_refused():
     L, ok, big, n = A.lib(), 1 << 20, 1 << 62, C.c_uint64()
     p = lookup(dim=1 << 20, table_stride=1 << 20, out_stride=1 << 20)
