@@ -1,145 +1,13 @@
 #include "leafops.h"
 
-#include <algorithm>
 #include <cmath>
-#include <string>
 #include <vector>
 
-#include "../abi.h"
+#include "opcalls.h"
 
 namespace hbr {
 
 namespace {
-
-constexpr uint32_t kWaveLanes = 64;
-
-uint64_t up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
-
-// A workspace handed out from its start, 256 bytes apart. Without memory it
-// only counts. An array may have more room than the call at hand uses.
-struct Arena {
-    char *base;
-    uint64_t used = 0;
-    explicit Arena(void *p) : base(static_cast<char *>(p)) {}
-    template <typename T>
-    T *take(uint64_t n, uint64_t used_of_it = 0) {
-        if (used_of_it > n) fail(kRefused, "a workspace has no room for the plan");
-        T *p = base ? reinterpret_cast<T *>(base + used) : nullptr;
-        used += up(n * sizeof(T), 256);
-        return p;
-    }
-};
-
-// The caller's stream, with its device current while the call runs and the
-// thread's own device current again behind it.
-class Queue {
-public:
-    Queue(int ordinal, void *stream) : stream_(static_cast<hipStream_t>(stream)) {
-        if (hipGetDevice(&before_) != hipSuccess) before_ = -1;
-        try {
-            device_ = &device(ordinal);
-            hipDevice_t of = ordinal;
-            if (stream_) HBR_HIP(hipStreamGetDevice(stream_, &of));
-            if (of != ordinal) fail(kInvalid, "the stream is not one of device " + std::to_string(ordinal));
-        } catch (...) {
-            restore();
-            throw;
-        }
-    }
-    ~Queue() { restore(); }
-    Queue(const Queue &) = delete;
-    Queue &operator=(const Queue &) = delete;
-    template <typename Args>
-    void launch(const char *kernel, dim3 grid, dim3 block, const Args &args, uint32_t lds_bytes = 0) {
-        if ((uint64_t)grid.x * block.x > 0xffffffffull) fail(kRefused, std::string(kernel) + ": more than 2^32 - 1 threads");
-        device_->launch_on(stream_, kernel, grid, block, args, lds_bytes);
-    }
-
-private:
-    void restore() {
-        if (before_ >= 0) (void)hipSetDevice(before_);
-    }
-    int before_ = -1;
-    Device *device_ = nullptr;
-    hipStream_t stream_;
-};
-
-uint64_t size_of(uint32_t dtype, const char *what) {
-    if (dtype == HBR_F32) return 4;
-    if (dtype == HBR_BF16) return 2;
-    fail(kInvalid, std::string(what) + ": the type is neither HBR_F32 nor HBR_BF16");
-}
-
-void check_workspace(const void *p, uint64_t have, uint64_t need, const char *what) {
-    if (need == 0) return;
-    if (!p || have < need)
-        fail(kInvalid, std::string(what) + ": the workspace holds " + std::to_string(p ? have : 0) + " bytes of " +
-                           std::to_string(need));
-    if (reinterpret_cast<uint64_t>(p) % 16)
-        fail(kInvalid, std::string(what) + ": the workspace is not aligned to 16 bytes");
-}
-
-void check_aligned(const void *p, uint64_t size, const char *what) {
-    if (reinterpret_cast<uint64_t>(p) % size)
-        fail(kInvalid, std::string(what) + ": an array is not aligned to its elements");
-}
-
-// An array's bytes: rows of `width`, `stride` apart.
-struct Extent {
-    uint64_t begin, rows, width, stride;
-    Extent(const void *p, uint64_t n) : Extent(p, 1, n, n) {}
-    Extent(const void *p, uint64_t n_rows, uint64_t row, uint64_t step)
-        : begin(reinterpret_cast<uint64_t>(p)), rows(p && row ? n_rows : 0), width(row), stride(n_rows > 1 ? step : row) {}
-    uint64_t end() const { return begin + (rows - 1) * stride + width; }
-};
-
-// Whether two arrays share a byte. Rows of one stride may lie between each
-// other's; of two arrays with gaps of different strides it is not found out.
-bool overlap(const Extent &a, const Extent &b) {
-    if (!a.rows || !b.rows || a.begin >= b.end() || b.begin >= a.end()) return false;
-    if (a.stride == b.stride) {
-        const uint64_t by = b.begin >= a.begin ? (b.begin - a.begin) % a.stride
-                                               : (a.stride - (a.begin - b.begin) % a.stride) % a.stride;
-        return by < a.width || by + b.width > a.stride;
-    }
-    const bool a_whole = a.width == a.stride;
-    if (!a_whole && b.width != b.stride) return false;
-    const Extent &whole = a_whole ? a : b, &rows = a_whole ? b : a;
-    // the first of the rows that ends behind the whole array's begin
-    const uint64_t first = rows.begin + rows.width > whole.begin ? 0 : (whole.begin - rows.begin - rows.width) / rows.stride + 1;
-    return first < rows.rows && rows.begin + first * rows.stride < whole.end();
-}
-
-void check_apart(std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs, const Extent &workspace, const char *what) {
-    for (const auto &list : {outputs, inputs})
-        for (const Extent &a : list)
-            if (overlap(a, workspace)) fail(kInvalid, std::string(what) + ": an array lies in the memory for the call's own use");
-    for (auto o = outputs.begin(); o != outputs.end(); o++) {
-        for (auto other = outputs.begin(); other != o; other++)
-            if (overlap(*o, *other)) fail(kInvalid, std::string(what) + ": two outputs overlap");
-        for (const Extent &i : inputs)
-            if (overlap(*o, i)) fail(kInvalid, std::string(what) + ": an output overlaps an input");
-    }
-}
-
-// The widest vector (elements, at most 16 bytes) that divides every row
-// length, stride and address.
-uint32_t vector_width(uint64_t size, std::initializer_list<uint64_t> lengths, std::initializer_list<const void *> ptrs) {
-    uint32_t v = (uint32_t)(16 / size);
-    for (; v > 1; v /= 2) {
-        bool ok = true;
-        for (uint64_t n : lengths) ok = ok && n % v == 0;
-        for (const void *p : ptrs) ok = ok && reinterpret_cast<uint64_t>(p) % (v * size) == 0;
-        if (ok) break;
-    }
-    return v;
-}
-
-// Vectors and inputs are shorter, so that offsets within one fit 32 bits and
-// grids over their elements a launch.
-constexpr uint64_t kDimLimit = 1u << 20;
-
-const char *name_of(uint32_t dtype) { return dtype == HBR_F32 ? "f32" : "bf16"; }
 
 // ---- leaf vectors ------------------------------------------------------------------
 
@@ -440,19 +308,11 @@ namespace {
 // The scores' gradients of one piece of the classes are held at a time, in at
 // most about this many bytes.
 constexpr uint64_t kPieceBytes = 1ull << 30;
-// Bytes from one chunk of 32 bf16 columns to the next. An odd multiple of
-// 2 KiB: the chunks of a tile, whose steps of 32 rows are 2 KiB each, then
-// begin in different halves of the L2's channels.
-constexpr uint64_t kChunkStep = 2048;
-uint64_t chunk_bytes(uint64_t rows) { return ((rows * 64 + 2 * kChunkStep - 1) / (2 * kChunkStep) * 2 + 1) * kChunkStep; }
-
 // From this many rows on, w is laid out in chunks too (and h in a call that
 // only scores): 2,048 rows scored against 32,768 classes of 512 bf16 take 105 us
 // with the operands in place and 108 laid out, 4,096 rows 194 and 187; with
 // the gradients 336 and 346, 642 and 635.
 constexpr uint64_t kLayRows = 4096;
-
-uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 
 // Scores alone over short inputs are made by rows too from this many on (and
 // from kLayRows rows): their partial results are held for a few shares of the
@@ -461,40 +321,6 @@ uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 // against 15.8, 200,000 and 70 41 against 48; in f32 17.8 us against 20.6 and 67
 // against 72).
 constexpr uint64_t kNarrowScores = 1u << 23;
-
-// A product's tiles, and how many of them fill 256 CUs (of the small ones twice
-// as many run at once, at hardly more rate).
-struct HeadTiling {
-    uint64_t tile, threads, slots;
-    const char *name;
-};
-constexpr HeadTiling kTile256{256, 512, 256, "_256"}, kTile128{128, 256, 512, "_128"};
-
-// Shares of a product's steps: where its tiles are fewer than the device
-// runs at once, enough of them to fill it, of 16 steps at least.
-uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t all = tiles(m, t.tile) * tiles(n, t.tile), steps = tiles(k, kHeadK) * segments;
-    return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 16));
-}
-
-// The tiles of a product with the gradients: those that take less time, in us:
-// a step of 256 large tiles is one (1.1 PFLOP/s), one of 512 small ones 0.54,
-// and shares' sums are read once more at 4.5 TB/s. Both at their best:
-// 16,384 x 131,072 x 1,024 products of bf16 take 3.9 ms with large tiles and
-// 4.2 with small ones, 8,191 x 32,768 x 512 ones 0.29 and 0.32, 3,229 x 2,810 x
-// 335 ones of f32 with their sums 70 us and 60. (The scores and pairs keep the
-// small ones: four workgroups on a CU hide each other's exponentials and
-// stores. 16,384 x 32,768 pairs of 1,024 take 1.34 ms against 1.35 with large
-// ones, 4,096 x 5,003 ones of 256 in f32 84 us against 119.)
-const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t steps = tiles(k, kHeadK) * segments;
-    auto cost = [&](const HeadTiling &t, double step) {
-        const uint64_t shares = head_splits(t, m, n, k, segments);
-        return (double)(tiles(tiles(m, t.tile) * tiles(n, t.tile) * shares, t.slots) * tiles(steps, shares)) * step +
-               (shares > 1 ? (double)(shares * m * n) * 4.0 / 4.5e6 : 0.0);
-    };
-    return cost(kTile256, 1.0) <= cost(kTile128, 0.54) ? kTile256 : kTile128;
-}
 
 struct HeadPlan {
     bool few;  // few classes: their own kernels, and the products' shares of the rows

@@ -12,7 +12,7 @@
 // a wave's own chain of loads and exponentials), products 36 (108 MB with the
 // pairs, 3 TB/s), sums 5. 100,000 rows of 256 bf16 and ten classes 64 us in all
 // (the kernels for many classes 111).
-#include "common.h"
+#include "product.h"
 
 namespace hbr {
 

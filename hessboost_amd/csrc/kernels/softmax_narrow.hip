@@ -15,7 +15,7 @@
 // second product's operand takes from it, in an order that the transposing
 // reads of Y follow: the scores' gradients pass from the one to the other
 // without leaving the lane.
-#include "common.h"
+#include "product.h"
 
 namespace hbr {
 
