@@ -24,6 +24,7 @@ GROW_DEPTHWISE, GROW_LOSSGUIDE = 0, 1
 SCAN_EMPTY, SCAN_REPLAY, SCAN_NUMERIC, SCAN_CATEGORICAL = 0, 1, 2, 3
 FALLBACK_NUMERIC_SCORE, FALLBACK_CATEGORICAL_ORDER, FALLBACK_CATEGORICAL_SCORE, FALLBACK_NEAR_TIE = 1, 2, 3, 4
 F32, BF16 = 0, 1
+PACK_BLOCK = 32
 TRANSFORM_SIGMOID, TRANSFORM_SOFTMAX, TRANSFORM_CLASS_INDEX = 1, 2, 3
 
 P = C.POINTER
@@ -138,6 +139,47 @@ class Tensor(C.Structure):
                 ("pad", C.c_uint32)]
 
 
+class Packed(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("x_stride", C.c_uint64),
+                ("codes_stride", C.c_uint64), ("scales_stride", C.c_uint64)]
+
+
+class Norm(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("x_stride", C.c_uint64),
+                ("residual_stride", C.c_uint64), ("out_stride", C.c_uint64), ("total_stride", C.c_uint64),
+                ("codes_stride", C.c_uint64), ("scales_stride", C.c_uint64), ("x", C.c_void_p),
+                ("residual", C.c_void_p), ("weight", C.c_void_p), ("out", C.c_void_p), ("total", C.c_void_p),
+                ("inv", C.c_void_p), ("codes", C.c_void_p), ("scales", C.c_void_p), ("eps", C.c_float),
+                ("normed", C.c_uint32)]
+
+
+class NormGrad(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("dout_stride", C.c_uint64),
+                ("x_stride", C.c_uint64), ("codes_stride", C.c_uint64), ("scales_stride", C.c_uint64),
+                ("dtotal_stride", C.c_uint64), ("dx_stride", C.c_uint64), ("dout", C.c_void_p), ("x", C.c_void_p),
+                ("codes", C.c_void_p), ("scales", C.c_void_p), ("inv", C.c_void_p), ("weight", C.c_void_p),
+                ("dtotal", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("eps", C.c_float),
+                ("pad", C.c_uint32)]
+
+
+class Linear(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("n_outs", C.c_uint32),
+                ("rank", C.c_uint32), ("n_adapters", C.c_uint32), ("pad", C.c_uint32), ("x_stride", C.c_uint64),
+                ("w_stride", C.c_uint64), ("out_stride", C.c_uint64), ("down_stride", C.c_uint64),
+                ("up_stride", C.c_uint64), ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p),
+                ("down", C.c_void_p), ("up", C.c_void_p), ("ids", C.c_void_p), ("scale", C.c_void_p),
+                ("out", C.c_void_p)]
+
+
+class LinearGrad(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("dim", C.c_uint32), ("n_rows", C.c_uint64), ("n_outs", C.c_uint32),
+                ("pad", C.c_uint32), ("dout_stride", C.c_uint64), ("w_stride", C.c_uint64), ("x_stride", C.c_uint64),
+                ("codes_stride", C.c_uint64), ("scales_stride", C.c_uint64), ("dx_stride", C.c_uint64),
+                ("dw_stride", C.c_uint64), ("dout", C.c_void_p), ("w", C.c_void_p), ("x", C.c_void_p),
+                ("codes", C.c_void_p), ("scales", C.c_void_p), ("weight", C.c_void_p), ("dx", C.c_void_p),
+                ("dw", C.c_void_p), ("db", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every entry point include/hessboost_rocm.h declares
 SIGNATURES = {
     "hbr_last_error": (C.c_size_t, [C.c_char_p, C.c_size_t]),
@@ -231,6 +273,15 @@ SIGNATURES = {
     "hbr_clip_gradients_workspace": (C.c_int, [C.c_uint64, P(C.c_uint64)]),
     "hbr_clip_gradients": (C.c_int, [C.c_int, P(Tensor), C.c_uint64, C.c_double, C.c_void_p, C.c_void_p, C.c_uint64,
                                      C.c_void_p]),
+    "hbr_pack_rows": (C.c_int, [C.c_int, P(Packed), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "hbr_unpack_rows": (C.c_int, [C.c_int, P(Packed), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "hbr_rms_norm": (C.c_int, [C.c_int, P(Norm), C.c_void_p]),
+    "hbr_rms_norm_grad_workspace": (C.c_int, [C.c_uint64, C.c_uint32, C.c_uint32, P(C.c_uint64)]),
+    "hbr_rms_norm_grad": (C.c_int, [C.c_int, P(NormGrad), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "hbr_linear_workspace": (C.c_int, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, P(C.c_uint64)]),
+    "hbr_linear": (C.c_int, [C.c_int, P(Linear), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "hbr_linear_grad_workspace": (C.c_int, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, P(C.c_uint64)]),
+    "hbr_linear_grad": (C.c_int, [C.c_int, P(LinearGrad), C.c_void_p, C.c_uint64, C.c_void_p]),
     "hbr_device_alloc": (C.c_int, [C.c_int, C.c_uint64, P(C.c_void_p)]),
     "hbr_device_free": (C.c_int, [C.c_int, C.c_void_p]),
     "hbr_device_upload": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_uint64]),

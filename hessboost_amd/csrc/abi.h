@@ -1154,6 +1154,12 @@ struct LookupSumArgs {
 // of two is summed over the six pairs of parts that reach f32's precision,
 // one segment of steps each.
 constexpr uint32_t kHeadK = 32;
+// The pairs of parts of a product of two f32 operands, smallest first: (2, 0),
+// (0, 2), (1, 1), (1, 0), (0, 1), (0, 0), two bits a segment; and of one of three
+// parts with one of one.
+constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+constexpr uint32_t kPartsByOne = 2u | 1u << 2 | 0u << 4;
 struct HeadArgs {
     const void *a, *b;
     uint64_t a_row, b_row;        // bytes from row to row
@@ -1183,6 +1189,7 @@ struct HeadArgs {
     void *c;
     uint64_t c_stride, c_split;
     uint32_t accumulate;          // add to c
+    uint32_t a_order, b_order;    // the segments' parts, two bits each from the lowest
     uint32_t pad2;
 };
 
@@ -1286,6 +1293,108 @@ struct HeadSumArgs {
     uint32_t shares;  // of the parts, a wave each: 1, 4 or 16
     float scale;
     uint32_t pad;
+};
+
+// ---- operators of the layers between leaf vectors and classes ----------------------
+
+// Columns of a row in 8 bits that share a power of two.
+constexpr uint32_t kPackBlock = 32;
+
+// The rows' kernels (hbr_rms_norm_*, hbr_rms_norm_grad_*): a row on `lanes`
+// lanes, a power of two up to 64 or a whole workgroup, `vecs` vectors a row.
+struct NormArgs {
+    const void *x, *residual;   // residual or null
+    const float *weight;        // or null
+    void *out, *total;          // or null
+    float *inv;                 // or null
+    uint8_t *codes, *scales;    // or null
+    uint64_t x_stride, residual_stride, out_stride, total_stride, codes_stride, scales_stride;
+    uint64_t n_rows;
+    uint32_t dim, vecs, lanes;
+    float eps, mean;            // mean: 1 / dim
+    uint32_t normed;            // the codes hold rows before the weight
+};
+
+struct NormGradArgs {
+    const void *dout, *x, *dtotal;        // x: null where codes are given; dtotal or null
+    const uint8_t *codes, *scales;
+    const float *inv, *weight;            // or null
+    void *dx;
+    float *part;                          // [workgroup][dim], or null: dweight is not wanted
+    uint64_t dout_stride, x_stride, dtotal_stride, codes_stride, scales_stride, dx_stride;
+    uint64_t n_rows;
+    uint32_t dim, vecs, lanes;
+    float eps, mean;
+    uint32_t pad;
+};
+
+struct PackArgs {
+    void *x;                    // read by pack, written by unpack
+    uint8_t *codes, *scales;
+    const float *weight;        // unpack: of the columns, or null
+    uint64_t x_stride, codes_stride, scales_stride;
+    uint64_t n_rows;
+    uint32_t dim, vecs, lanes;
+    uint32_t each;              // vectors of a row a workgroup's lane takes
+};
+
+// A projection's products (p.c: the result, or [split] parts of its sums). Of
+// the result's columns p.weight are factors and p.bias is added; of a
+// projection's rows (hbr_linear_y_*) the first share adds the adapters.
+struct LinearArgs {
+    HeadArgs p;
+    const float *low;           // [row][rank]: the rows times their adapters' first factors and scales, or null
+    const void *up;             // [adapter][n][rank], rows up_stride apart
+    const int32_t *ids;         // of the rows
+    uint64_t up_stride;
+    uint32_t rank, adapters;
+};
+
+// dst = the sum of the parts, times the column's factor, and the column's bias.
+struct LinearJoinArgs {
+    const float *part;
+    const float *weight, *bias; // or null
+    void *dst;
+    uint64_t rows, cols, dst_stride, part_stride;
+    uint32_t parts, pad;
+};
+
+// hbr_linear_low_*: low[row][rho] = scale[a] <x[row], down[a][rho]>, a the row's adapter.
+struct LinearLowArgs {
+    const void *x, *down;
+    const int32_t *ids;
+    const float *scale;         // or null
+    float *low;
+    uint64_t x_stride, down_stride;
+    uint32_t n_rows, dim, rank, adapters;
+};
+
+// Few rows: hbr_linear_few_*.
+struct LinearFewArgs {
+    const void *x, *w;
+    const float *bias;
+    void *out;
+    const float *low;           // or null
+    const void *up;
+    const int32_t *ids;
+    uint64_t x_stride, w_stride, out_stride, up_stride;
+    uint32_t n_rows, dim, outs, rank, adapters, pad;
+};
+
+// Rows in 8 bits as bf16 in chunks of 32 columns (zeros past cols).
+struct LayCodesArgs {
+    const uint8_t *codes, *scales;
+    uint16_t *dst;
+    uint64_t rows, codes_stride, scales_stride, chunk;  // elements from chunk to chunk
+    uint32_t cols, chunks;
+};
+
+// part[share][column] = the sums of the share's rows.
+struct ColumnSumArgs {
+    const void *x;
+    float *part;
+    uint64_t rows, x_stride;
+    uint32_t cols, shares;
 };
 
 // hbr_clip_*: up to kClipTensors tensors a launch.

@@ -10,6 +10,7 @@
 #include "cuts.h"
 #include "engine.h"
 #include "forest.h"
+#include "layers.h"
 #include "leafops.h"
 #include "noalloc.h"
 #include "split_math.h"
@@ -1075,6 +1076,72 @@ int hbr_clip_gradients(int ordinal, const hbr_tensor *tensors, uint64_t n_tensor
                        void *workspace, uint64_t workspace_bytes, void *stream) {
     return guard([&] {
         clip_gradients(ordinal, stream, tensors, n_tensors, max_norm, norm, workspace, workspace_bytes);
+    });
+}
+
+// ---- operators of the layers between leaf vectors and classes -------------------------------
+
+int hbr_pack_rows(int ordinal, const hbr_packed *p, const void *x, uint8_t *codes, uint8_t *scales, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "pack rows: null argument");
+        pack_rows(ordinal, stream, *p, x, codes, scales);
+    });
+}
+
+int hbr_unpack_rows(int ordinal, const hbr_packed *p, const uint8_t *codes, const uint8_t *scales, const float *weight,
+                    void *x, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "unpack rows: null argument");
+        unpack_rows(ordinal, stream, *p, codes, scales, weight, x);
+    });
+}
+
+int hbr_rms_norm(int ordinal, const hbr_norm *p, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "rms norm: null argument");
+        rms_norm(ordinal, stream, *p);
+    });
+}
+
+int hbr_rms_norm_grad_workspace(uint64_t n_rows, uint32_t dim, uint32_t dtype, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail(kInvalid, "rms norm gradient: null argument");
+        *bytes = rms_norm_grad_workspace(n_rows, dim, dtype);
+    });
+}
+
+int hbr_rms_norm_grad(int ordinal, const hbr_norm_grad *p, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "rms norm gradient: null argument");
+        rms_norm_grad(ordinal, stream, *p, workspace, workspace_bytes);
+    });
+}
+
+int hbr_linear_workspace(uint64_t n_rows, uint32_t n_outs, uint32_t dim, uint32_t rank, uint32_t dtype, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail(kInvalid, "linear: null argument");
+        *bytes = linear_workspace(n_rows, n_outs, dim, rank, dtype);
+    });
+}
+
+int hbr_linear(int ordinal, const hbr_linear_args *p, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "linear: null argument");
+        linear(ordinal, stream, *p, workspace, workspace_bytes);
+    });
+}
+
+int hbr_linear_grad_workspace(uint64_t n_rows, uint32_t n_outs, uint32_t dim, uint32_t dtype, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) fail(kInvalid, "linear gradient: null argument");
+        *bytes = linear_grad_workspace(n_rows, n_outs, dim, dtype);
+    });
+}
+
+int hbr_linear_grad(int ordinal, const hbr_linear_grad_args *p, void *workspace, uint64_t workspace_bytes, void *stream) {
+    return guard([&] {
+        if (!p) fail(kInvalid, "linear gradient: null argument");
+        linear_grad(ordinal, stream, *p, workspace, workspace_bytes);
     });
 }
 

@@ -1,0 +1,530 @@
+#include "layers.h"
+
+#include "opcalls.h"
+
+namespace hbr {
+
+namespace {
+
+constexpr uint64_t kRowsLimit = 0x7fffffffull;
+
+void check_rows(uint64_t n, uint64_t dim, const char *what) {
+    if (dim == 0) fail(kInvalid, std::string(what) + ": rows of no elements");
+    if (dim >= kDimLimit) fail(kRefused, std::string(what) + ": rows of 1,048,576 elements or more");
+    if (n > kRowsLimit) fail(kRefused, std::string(what) + ": more than 2^31 - 1 rows");
+}
+
+// An array of rows, as its checks and its kernels see it.
+struct Rows {
+    const void *p;
+    uint64_t n, width, stride, size;  // size: of an element
+    Rows(const void *ptr, uint64_t rows, uint64_t cols, uint64_t step, uint64_t bytes, const char *what)
+        : p(ptr), n(rows), width(cols), stride(rows > 1 ? step : cols), size(bytes) {
+        if (!p) return;
+        if (stride < width) fail(kInvalid, std::string(what) + ": rows overlap");
+        check_aligned(p, size, what);
+    }
+    Extent extent() const { return {p, n, width * size, stride * size}; }
+    bool is(const Rows &o) const { return p && p == o.p && stride == o.stride && size == o.size; }
+};
+
+// The widest vector that every array's rows are made of.
+uint32_t rows_vector(uint64_t size, uint64_t dim, std::initializer_list<const Rows *> all) {
+    uint32_t v = (uint32_t)(16 / size);
+    for (; v > 1; v /= 2) {
+        bool ok = dim % v == 0;
+        for (const Rows *r : all)
+            ok = ok && (!r->p || ((r->n <= 1 || r->stride % v == 0) && reinterpret_cast<uint64_t>(r->p) % (v * r->size) == 0));
+        if (ok) break;
+    }
+    return v;
+}
+
+uint64_t scales_of(uint64_t dim) { return tiles(dim, kPackBlock); }
+
+uint32_t power_of_two(uint64_t n) {
+    uint32_t p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+// A row's lanes and its vectors a lane: a wave or less of a workgroup of 256,
+// else the whole of one; 0 vectors where the registers hold no row.
+struct RowPlan {
+    uint32_t lanes, held, threads;
+    uint64_t per() const { return threads / lanes; }  // rows a workgroup
+};
+RowPlan row_plan(uint64_t vecs, uint32_t v, bool codes) {
+    const uint32_t most = v == 8 ? 2 : 4;
+    const uint64_t least = std::max<uint64_t>(vecs, codes ? kPackBlock / v : 1);
+    if (least <= kWaveLanes) return {power_of_two(least), 1, 256};
+    for (uint32_t held = 2; held <= most; held *= 2)
+        if (vecs <= kWaveLanes * held) return {kWaveLanes, held, 256};
+    for (uint32_t threads = 256; threads <= 1024; threads *= 2)
+        for (uint32_t held = most / 2; held <= most; held *= 2)
+            if (vecs <= threads * held) return {threads, held, threads};
+    return {1024, 0, 1024};
+}
+
+std::string kernel_of(const char *name, uint32_t dtype, uint32_t v) {
+    return std::string(name) + "_" + name_of(dtype) + "_" + std::to_string(v);
+}
+
+void check_packed(const uint8_t *codes, const uint8_t *scales, const char *what) {
+    if (!codes != !scales) fail(kInvalid, std::string(what) + ": codes and scales go together");
+}
+
+}  // namespace
+
+// ---- the norm ----------------------------------------------------------------------
+
+void rms_norm(int ordinal, void *stream, const hbr_norm &p) {
+    const char *what = "rms norm";
+    const uint64_t size = size_of(p.dtype, what), n = p.n_rows, dim = p.dim;
+    check_rows(n, dim, what);
+    check_packed(p.codes, p.scales, what);
+    if (!(p.eps >= 0.0f)) fail(kInvalid, std::string(what) + ": eps is negative or no number");
+    if (n == 0) return;
+    if (!p.x) fail(kInvalid, std::string(what) + ": null argument");
+    const Rows x(p.x, n, dim, p.x_stride, size, what), residual(p.residual, n, dim, p.residual_stride, size, what),
+        out(p.out, n, dim, p.out_stride, size, what), total(p.total, n, dim, p.total_stride, size, what),
+        codes(p.codes, n, dim, p.codes_stride, 1, what), scales(p.scales, n, scales_of(dim), p.scales_stride, 1, what);
+    check_aligned(p.weight, 4, what);
+    check_aligned(p.inv, 4, what);
+    // (a row is read before it is written, so an output may be an input itself)
+    auto apart = [&](const Rows &in) { return in.is(out) || in.is(total) ? Extent(nullptr, 0) : in.extent(); };
+    check_apart({out.extent(), total.extent(), codes.extent(), scales.extent(), {p.inv, n * 4}},
+                {apart(x), apart(residual), {p.weight, dim * 4}}, Extent(nullptr, 0), what);
+    Queue queue(ordinal, stream);
+    const Rows weight(p.weight, 1, dim, dim, 4, what);
+    const uint32_t v = rows_vector(size, dim, {&x, &residual, &out, &total, &codes, &weight});
+    const RowPlan q = row_plan(dim / v, v, p.codes != nullptr);
+    NormArgs a{};
+    a.x = p.x;
+    a.residual = p.residual;
+    a.weight = p.weight;
+    a.out = p.out;
+    a.total = p.total;
+    a.inv = p.inv;
+    a.codes = p.codes;
+    a.scales = p.scales;
+    a.x_stride = x.stride;
+    a.residual_stride = residual.stride;
+    a.out_stride = out.stride;
+    a.total_stride = total.stride;
+    a.codes_stride = codes.stride;
+    a.scales_stride = scales.stride;
+    a.n_rows = n;
+    a.dim = p.dim;
+    a.vecs = p.dim / v;
+    a.lanes = q.lanes;
+    a.eps = p.eps;
+    a.mean = 1.0f / (float)p.dim;
+    a.normed = p.normed;
+    queue.launch((kernel_of("hbr_rms_norm", p.dtype, v) + "_" + std::to_string(q.held)).c_str(),
+                 dim3((uint32_t)std::min<uint64_t>(tiles(n, q.per()), 2048 * 256 / q.threads)), dim3(q.threads), a);
+}
+
+namespace {
+
+// Workgroups of the gradient at most: their sums of the weights' gradient are
+// held in the workspace.
+uint64_t norm_grad_blocks(uint64_t dim) { return std::max<uint64_t>(1, std::min<uint64_t>(1024, (1u << 22) / dim)); }
+
+}  // namespace
+
+uint64_t rms_norm_grad_workspace(uint64_t n, uint32_t dim, uint32_t dtype) {
+    size_of(dtype, "rms norm gradient");
+    check_rows(n, dim, "rms norm gradient");
+    return up(std::min(n, norm_grad_blocks(dim)) * dim * sizeof(float), 256);
+}
+
+void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *workspace, uint64_t workspace_bytes) {
+    const char *what = "rms norm gradient";
+    const uint64_t size = size_of(p.dtype, what), n = p.n_rows, dim = p.dim;
+    check_rows(n, dim, what);
+    check_packed(p.codes, p.scales, what);
+    if (n && (!p.x == !p.codes)) fail(kInvalid, std::string(what) + ": the rows, or the normed rows in 8 bits, are needed");
+    if (n && p.codes && !p.inv) fail(kInvalid, std::string(what) + ": rows in 8 bits need inv");
+    if (n && !p.dout) fail(kInvalid, std::string(what) + ": null argument");
+    if (!p.inv && !(p.eps >= 0.0f)) fail(kInvalid, std::string(what) + ": eps is negative or no number");
+    const Rows dout(p.dout, n, dim, p.dout_stride, size, what), x(p.x, n, dim, p.x_stride, size, what),
+        codes(p.codes, n, dim, p.codes_stride, 1, what), scales(p.scales, n, scales_of(dim), p.scales_stride, 1, what),
+        dtotal(p.dtotal, n, dim, p.dtotal_stride, size, what), dx(p.dx, n, dim, p.dx_stride, size, what);
+    for (const void *f : {(const void *)p.inv, (const void *)p.weight, (const void *)p.dweight}) check_aligned(f, 4, what);
+    const uint64_t need = p.dweight ? rms_norm_grad_workspace(n, p.dim, p.dtype) : 0;
+    check_workspace(workspace, workspace_bytes, need, what);
+    auto apart = [&](const Rows &in) { return in.is(dx) ? Extent(nullptr, 0) : in.extent(); };
+    check_apart({dx.extent(), {p.dweight, dim * 4}},
+                {apart(dout), apart(dtotal), x.extent(), codes.extent(), scales.extent(), {p.inv, n * 4}, {p.weight, dim * 4}},
+                Extent(need ? workspace : nullptr, need), what);
+    if (!p.dx && !p.dweight) return;
+    Queue queue(ordinal, stream);
+    uint64_t blocks = 0;
+    if (n) {
+        const Rows weight(p.weight, 1, dim, dim, 4, what);
+        const uint32_t v = rows_vector(size, dim, {&dout, &x, &codes, &dtotal, &dx, &weight});
+        const RowPlan q = row_plan(dim / v, v, false);
+        blocks = std::min(tiles(n, q.per()), norm_grad_blocks(dim));
+        NormGradArgs a{};
+        a.dout = p.dout;
+        a.x = p.x;
+        a.dtotal = p.dtotal;
+        a.codes = p.codes;
+        a.scales = p.scales;
+        a.inv = p.inv;
+        a.weight = p.weight;
+        a.dx = p.dx;
+        a.part = p.dweight ? static_cast<float *>(workspace) : nullptr;
+        a.dout_stride = dout.stride;
+        a.x_stride = x.stride;
+        a.dtotal_stride = dtotal.stride;
+        a.codes_stride = codes.stride;
+        a.scales_stride = scales.stride;
+        a.dx_stride = dx.stride;
+        a.n_rows = n;
+        a.dim = p.dim;
+        a.vecs = p.dim / v;
+        a.lanes = q.lanes;
+        a.eps = p.eps;
+        a.mean = 1.0f / (float)p.dim;
+        queue.launch((kernel_of("hbr_rms_norm_grad", p.dtype, v) + "_" + std::to_string(q.held)).c_str(), dim3((uint32_t)blocks),
+                     dim3(q.threads), a);
+    }
+    if (p.dweight) sum_parts(queue, HBR_F32, 1.0f, static_cast<const float *>(workspace), blocks, dim, p.dweight, 1, dim, dim);
+}
+
+// ---- rows in 8 bits -------------------------------------------------------------------
+
+namespace {
+
+void packed(int ordinal, void *stream, const hbr_packed &p, const void *x, const uint8_t *codes, const uint8_t *scales,
+            const float *weight, bool pack, const char *what) {
+    const uint64_t size = size_of(p.dtype, what), n = p.n_rows, dim = p.dim;
+    check_rows(n, dim, what);
+    if (n == 0) return;
+    if (!x || !codes || !scales) fail(kInvalid, std::string(what) + ": null argument");
+    const Rows rx(x, n, dim, p.x_stride, size, what), rc(codes, n, dim, p.codes_stride, 1, what),
+        rs(scales, n, scales_of(dim), p.scales_stride, 1, what), rw(weight, 1, dim, dim, 4, what);
+    if (pack) check_apart({rc.extent(), rs.extent()}, {rx.extent()}, Extent(nullptr, 0), what);
+    else check_apart({rx.extent()}, {rc.extent(), rs.extent(), rw.extent()}, Extent(nullptr, 0), what);
+    Queue queue(ordinal, stream);
+    const uint32_t v = rows_vector(size, dim, {&rx, &rc, &rw});
+    PackArgs a{};
+    a.x = const_cast<void *>(x);
+    a.codes = const_cast<uint8_t *>(codes);
+    a.scales = const_cast<uint8_t *>(scales);
+    a.weight = weight;
+    a.x_stride = rx.stride;
+    a.codes_stride = rc.stride;
+    a.scales_stride = rs.stride;
+    a.n_rows = n;
+    a.dim = p.dim;
+    a.vecs = p.dim / v;
+    a.lanes = power_of_two(std::min<uint64_t>(kWaveLanes, std::max(a.vecs, kPackBlock / v)));
+    a.each = 8;
+    queue.launch(kernel_of(pack ? "hbr_pack" : "hbr_unpack", p.dtype, v).c_str(),
+                 dim3((uint32_t)std::min<uint64_t>(tiles(n, 256 / a.lanes), 1u << 16), (uint32_t)tiles(up(a.vecs, 32), a.lanes * a.each)),
+                 dim3(256), a);
+}
+
+}  // namespace
+
+void pack_rows(int ordinal, void *stream, const hbr_packed &p, const void *x, uint8_t *codes, uint8_t *scales) {
+    packed(ordinal, stream, p, x, codes, scales, nullptr, true, "pack rows");
+}
+
+void unpack_rows(int ordinal, void *stream, const hbr_packed &p, const uint8_t *codes, const uint8_t *scales, const float *weight,
+                 void *x) {
+    packed(ordinal, stream, p, x, codes, scales, weight, false, "unpack rows");
+}
+
+// ---- projections -------------------------------------------------------------------------
+
+namespace {
+
+// A product's f32 parts, where its steps are shared out: rows of n columns, for
+// any number of rows up to m.
+uint64_t part_rows(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t most = tiles(k, kHeadK) * segments / 16;
+    return most > 1 ? std::min(65536 / tiles(n, kTile256.tile), m * most) : 0;
+}
+
+uint64_t laid_bytes(uint64_t rows, uint64_t cols, uint64_t parts) { return parts * tiles(cols, 32) * chunk_bytes(rows); }
+
+void check_product(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, const char *what) {
+    size_of(dtype, what);
+    check_rows(n, dim, what);
+    if (outs == 0) fail(kInvalid, std::string(what) + ": no outputs");
+    if (outs >= kDimLimit) fail(kRefused, std::string(what) + ": 1,048,576 outputs or more");
+}
+
+// Tiles of 128 that a launch takes.
+void check_tiles(uint64_t m, uint64_t n, const char *what) {
+    if (tiles(m, 128) * tiles(n, 128) >= 1u << 22) fail(kRefused, std::string(what) + ": 2^22 tiles of 128 x 128 or more");
+}
+
+struct LinearPlan {
+    char *x, *w;
+    float *low, *part;
+    const HeadTiling *tiling;
+    uint64_t parts, segments, splits, bytes;
+};
+LinearPlan linear_plan(uint64_t n, uint64_t outs, uint64_t dim, uint64_t rank, uint32_t dtype, void *workspace) {
+    LinearPlan q{};
+    q.parts = dtype == HBR_F32 ? 3 : 1;
+    q.segments = dtype == HBR_F32 ? 6 : 1;
+    q.tiling = &head_tiling(n, outs, dim, q.segments);
+    q.splits = head_splits(*q.tiling, n, outs, dim, q.segments);
+    Arena w(workspace);
+    q.x = w.take<char>(laid_bytes(n, dim, q.parts));
+    q.w = w.take<char>(laid_bytes(outs, dim, q.parts));
+    q.low = w.take<float>(n * rank);
+    q.part = w.take<float>(part_rows(n, outs, dim, q.segments) * outs, q.splits > 1 ? q.splits * n * outs : 0);
+    q.bytes = w.used;
+    return q;
+}
+
+}  // namespace
+
+uint64_t linear_workspace(uint64_t n, uint32_t outs, uint32_t dim, uint32_t rank, uint32_t dtype) {
+    check_product(n, outs, dim, dtype, "linear");
+    if (rank >= kDimLimit) fail(kRefused, "linear: adapters of rank 1,048,576 or more");
+    check_tiles(n, outs, "linear");
+    return linear_plan(n, outs, dim, rank, dtype, nullptr).bytes;
+}
+
+void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace, uint64_t workspace_bytes) {
+    const char *what = "linear";
+    const uint64_t n = p.n_rows, outs = p.n_outs, dim = p.dim;
+    check_product(n, outs, dim, p.dtype, what);
+    const uint64_t size = size_of(p.dtype, what), rank = p.n_adapters ? p.rank : 0;
+    if (rank >= kDimLimit) fail(kRefused, std::string(what) + ": adapters of rank 1,048,576 or more");
+    if (p.n_adapters > 0x7fffffffu) fail(kRefused, std::string(what) + ": more than 2^31 - 1 adapters");
+    check_tiles(n, outs, what);
+    if (n == 0) return;
+    if (!p.x || !p.w || !p.out) fail(kInvalid, std::string(what) + ": null argument");
+    if (rank && (!p.down || !p.up || !p.ids)) fail(kInvalid, std::string(what) + ": adapters need down, up and ids");
+    const Rows x(p.x, n, dim, p.x_stride, size, what), w(p.w, outs, dim, p.w_stride, size, what),
+        out(p.out, n, outs, p.out_stride, size, what),
+        down(rank ? p.down : nullptr, p.n_adapters * rank, dim, p.down_stride, size, what),
+        up_rows(rank ? p.up : nullptr, p.n_adapters * outs, rank, p.up_stride, size, what);
+    if (out.stride >= (1u << 21)) fail(kRefused, std::string(what) + ": results whose rows lie 2,097,152 elements or more apart");
+    for (const void *f : {(const void *)p.bias, (const void *)p.ids, (const void *)p.scale}) check_aligned(f, 4, what);
+    const LinearPlan q = linear_plan(n, outs, dim, rank, p.dtype, workspace);
+    check_workspace(workspace, workspace_bytes, q.bytes, what);
+    check_apart({out.extent()},
+                {x.extent(), w.extent(), down.extent(), up_rows.extent(), {p.bias, outs * 4}, {rank ? p.ids : nullptr, n * 4},
+                 {rank ? p.scale : nullptr, p.n_adapters * 4ull}}, Extent(workspace, q.bytes), what);
+    Queue queue(ordinal, stream);
+    const std::string type = name_of(p.dtype);
+    if (rank) {
+        LinearLowArgs a{};
+        a.x = p.x;
+        a.down = p.down;
+        a.ids = p.ids;
+        a.scale = p.scale;
+        a.low = q.low;
+        a.x_stride = x.stride;
+        a.down_stride = down.stride;
+        a.n_rows = (uint32_t)n;
+        a.dim = p.dim;
+        a.rank = p.rank;
+        a.adapters = p.n_adapters;
+        queue.launch(("hbr_linear_low_" + type).c_str(), dim3((uint32_t)std::min<uint64_t>(tiles(n, 4), 1u << 16)), dim3(256), a);
+    }
+    LinearArgs a{};
+    set_a(a.p, lay_rows(queue, p.x, x.stride, n, dim, p.dtype, q.x, false, nullptr));
+    set_b(a.p, lay_rows(queue, p.w, w.stride, outs, dim, p.dtype, q.w, false, nullptr));
+    a.p.m = a.p.rows = (uint32_t)n;
+    a.p.n = p.n_outs;
+    a.p.k = p.dim;
+    a.p.check = dim % kHeadK != 0;
+    a.p.segments = (uint32_t)q.segments;
+    if (q.segments > 1) a.p.a_order = kPartA, a.p.b_order = kPartB;
+    a.p.splits = (uint32_t)q.splits;
+    a.p.bias = p.bias;
+    a.p.m_tiles = (uint32_t)tiles(n, q.tiling->tile);
+    a.p.n_tiles = (uint32_t)tiles(outs, q.tiling->tile);
+    const bool shared = q.splits > 1;
+    a.p.c = shared ? (void *)q.part : p.out;
+    a.p.c_stride = shared ? outs : out.stride;
+    a.p.c_split = n * outs;
+    a.low = rank ? q.low : nullptr;
+    a.up = p.up;
+    a.ids = p.ids;
+    a.up_stride = up_rows.stride;
+    a.rank = p.rank;
+    a.adapters = p.n_adapters;
+    queue.launch(("hbr_linear_y_" + std::string(shared ? "part_" : "") + type + q.tiling->name).c_str(),
+                 dim3(a.p.m_tiles * a.p.n_tiles * a.p.splits), dim3((uint32_t)q.tiling->threads), a);
+    if (!shared) return;
+    LinearJoinArgs j{};
+    j.part = q.part;
+    j.bias = p.bias;
+    j.dst = p.out;
+    j.rows = n;
+    j.cols = outs;
+    j.dst_stride = out.stride;
+    j.part_stride = n * outs;
+    j.parts = a.p.splits;
+    queue.launch(("hbr_linear_join_" + type).c_str(), cells_grid(n * outs), dim3(256), j);
+}
+
+namespace {
+
+// Shares of the rows whose sums make db, at most.
+uint64_t column_shares(uint64_t outs) { return std::max<uint64_t>(1, 2048 / tiles(outs, 256)); }
+
+struct LinearGradPlan {
+    char *dout, *w, *x;
+    float *part_x, *part_w, *part_b;
+    uint64_t parts, bytes;
+    uint64_t segments_x, segments_w, splits_x, splits_w;
+    const HeadTiling *by_x, *by_w;
+};
+// held: the rows are in 8 bits, one part whatever the type
+LinearGradPlan linear_grad_plan(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, bool held, void *workspace) {
+    LinearGradPlan q{};
+    q.parts = dtype == HBR_F32 ? 3 : 1;
+    q.segments_x = dtype == HBR_F32 ? 6 : 1;
+    q.segments_w = dtype == HBR_F32 ? held ? 3 : 6 : 1;
+    q.by_x = &head_tiling(n, dim, outs, q.segments_x);
+    q.by_w = &head_tiling(outs, dim, n, q.segments_w);
+    q.splits_x = head_splits(*q.by_x, n, dim, outs, q.segments_x);
+    q.splits_w = head_splits(*q.by_w, outs, dim, n, q.segments_w);
+    Arena w(workspace);
+    q.dout = w.take<char>(laid_bytes(n, outs, q.parts));
+    q.w = w.take<char>(laid_bytes(outs, dim, q.parts));
+    q.x = w.take<char>(laid_bytes(n, dim, q.parts));
+    // (of dw whatever the tiles: a share is 16 steps at least)
+    q.part_x = w.take<float>(part_rows(n, dim, outs, q.segments_x) * dim, q.splits_x > 1 ? q.splits_x * n * dim : 0);
+    q.part_w = w.take<float>(part_rows(outs, dim, n, q.parts == 3 ? 6 : 1) * dim, q.splits_w > 1 ? q.splits_w * outs * dim : 0);
+    q.part_b = w.take<float>(column_shares(outs) * outs);
+    q.bytes = w.used;
+    return q;
+}
+
+}  // namespace
+
+uint64_t linear_grad_workspace(uint64_t n, uint32_t outs, uint32_t dim, uint32_t dtype) {
+    check_product(n, outs, dim, dtype, "linear gradient");
+    check_tiles(n, dim, "linear gradient");
+    check_tiles(outs, dim, "linear gradient");
+    return linear_grad_plan(n, outs, dim, dtype, false, nullptr).bytes;
+}
+
+void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void *workspace, uint64_t workspace_bytes) {
+    const char *what = "linear gradient";
+    const uint64_t n = p.n_rows, outs = p.n_outs, dim = p.dim;
+    check_product(n, outs, dim, p.dtype, what);
+    check_tiles(n, dim, what);
+    check_tiles(outs, dim, what);
+    check_packed(p.codes, p.scales, what);
+    const uint64_t size = size_of(p.dtype, what);
+    if (n && !p.dout) fail(kInvalid, std::string(what) + ": null argument");
+    if (p.dx && n && !p.w) fail(kInvalid, std::string(what) + ": dx needs w");
+    if (p.dw && n && (!p.x == !p.codes)) fail(kInvalid, std::string(what) + ": dw needs the rows, as they are or in 8 bits");
+    const Rows dout(p.dout, n, outs, p.dout_stride, size, what), w(p.w, outs, dim, p.w_stride, size, what),
+        x(p.x, n, dim, p.x_stride, size, what), codes(p.codes, n, dim, p.codes_stride, 1, what),
+        scales(p.scales, n, scales_of(dim), p.scales_stride, 1, what), dx(p.dx, n, dim, p.dx_stride, size, what),
+        dw(p.dw, outs, dim, p.dw_stride, size, what);
+    if ((p.dx && dx.stride >= (1u << 21)) || (p.dw && dw.stride >= (1u << 21)))
+        fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
+    check_aligned(p.weight, 4, what);
+    check_aligned(p.db, 4, what);
+    const bool held = p.codes != nullptr;
+    const LinearGradPlan q = linear_grad_plan(n, outs, dim, p.dtype, held, workspace);
+    check_workspace(workspace, workspace_bytes, q.bytes, what);
+    check_apart({dx.extent(), dw.extent(), {p.db, outs * 4}},
+                {dout.extent(), w.extent(), x.extent(), codes.extent(), scales.extent(), {p.weight, dim * 4}},
+                Extent(workspace, q.bytes), what);
+    if (!p.dw && !p.db && (!p.dx || n == 0)) return;
+    Queue queue(ordinal, stream);
+    const std::string type = name_of(p.dtype);
+    auto join = [&](const float *part, uint64_t parts, const float *weight, const Rows &to) {
+        LinearJoinArgs j{};
+        j.part = part;
+        j.weight = weight;
+        j.dst = const_cast<void *>(to.p);
+        j.rows = to.n;
+        j.cols = dim;
+        j.dst_stride = to.stride;
+        j.part_stride = to.n * dim;
+        j.parts = (uint32_t)parts;
+        queue.launch(("hbr_linear_join_" + type).c_str(), cells_grid(to.n * dim), dim3(256), j);
+    };
+    if (n == 0) {  // sums over no rows
+        if (p.dw) join(nullptr, 0, nullptr, dw);
+        if (p.db) sum_parts(queue, HBR_F32, 1.0f, nullptr, 0, 0, p.db, 1, outs, outs);
+        return;
+    }
+    if (p.db) {
+        ColumnSumArgs a{};
+        a.x = p.dout;
+        a.part = q.part_b;
+        a.rows = n;
+        a.x_stride = dout.stride;
+        a.cols = p.n_outs;
+        a.shares = (uint32_t)std::min(column_shares(outs), tiles(n, 32));
+        queue.launch(("hbr_column_sum_" + type).c_str(), dim3((uint32_t)tiles(outs, 256) * a.shares), dim3(256), a);
+        sum_parts(queue, HBR_F32, 1.0f, q.part_b, a.shares, outs, p.db, 1, outs, outs);
+    }
+    if (!p.dx && !p.dw) return;
+    const Laid by = lay_rows(queue, p.dout, dout.stride, n, outs, p.dtype, q.dout, false, nullptr);
+    auto product = [&](const char *name, const HeadTiling &t, LinearArgs &a, float *part, const Rows &to) {
+        a.p.n = p.dim;
+        a.p.rows = (uint32_t)to.n;
+        a.p.m_tiles = (uint32_t)tiles(to.n, t.tile);
+        a.p.n_tiles = (uint32_t)tiles(dim, t.tile);
+        const bool shared = a.p.splits > 1;
+        a.p.c = shared ? (void *)part : const_cast<void *>(to.p);
+        a.p.c_stride = shared ? dim : to.stride;
+        a.p.c_split = to.n * dim;
+        queue.launch((std::string(name) + (shared ? "part" : type) + t.name).c_str(), dim3(a.p.m_tiles * a.p.n_tiles * a.p.splits),
+                     dim3((uint32_t)t.threads), a);
+        if (shared) join(part, a.p.splits, a.p.weight, to);
+    };
+    if (p.dx) {
+        LinearArgs a{};
+        set_a(a.p, by);
+        set_b(a.p, lay_rows(queue, p.w, w.stride, outs, dim, p.dtype, q.w, false, nullptr));
+        a.p.m = (uint32_t)n;
+        a.p.k = p.n_outs;
+        a.p.check = outs % kHeadK != 0;
+        a.p.segments = (uint32_t)q.segments_x;
+        if (q.segments_x > 1) a.p.a_order = kPartA, a.p.b_order = kPartB;
+        a.p.splits = (uint32_t)q.splits_x;
+        product("hbr_linear_dx_", *q.by_x, a, q.part_x, dx);
+    }
+    if (p.dw) {
+        LinearArgs a{};
+        set_a(a.p, by);
+        if (held) {
+            LayCodesArgs l{};
+            l.codes = p.codes;
+            l.scales = p.scales;
+            l.dst = reinterpret_cast<uint16_t *>(q.x);
+            l.rows = n;
+            l.codes_stride = codes.stride;
+            l.scales_stride = scales.stride;
+            l.chunk = chunk_bytes(n) / 2;
+            l.cols = p.dim;
+            l.chunks = (uint32_t)tiles(dim, 32);
+            queue.launch("hbr_lay_codes", cells_grid(n * l.chunks * 4), dim3(256), l);
+            set_b(a.p, {q.x, 64, l.chunk * 2, 0, l.chunks * 32});
+        } else {
+            set_b(a.p, lay_rows(queue, p.x, x.stride, n, dim, p.dtype, q.x, false, nullptr));
+        }
+        a.p.m = by.row == 64 && by.p == q.dout ? (uint32_t)up(outs, 32) : p.n_outs;  // (to the end of a laid chunk)
+        a.p.k = (uint32_t)n;
+        a.p.segments = (uint32_t)q.segments_w;
+        if (q.segments_w == 6) a.p.a_order = kPartA, a.p.b_order = kPartB;
+        else if (q.segments_w == 3) a.p.a_order = kPartsByOne;
+        a.p.splits = (uint32_t)q.splits_w;
+        a.p.weight = p.weight;
+        product("hbr_linear_dw_", *q.by_w, a, q.part_w, dw);
+    }
+}
+
+}  // namespace hbr

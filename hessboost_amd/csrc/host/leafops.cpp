@@ -340,13 +340,6 @@ struct HeadPlan {
     uint64_t bytes;
 };
 
-// What the products can read in place: bf16 rows of whole 16-byte pieces,
-// near enough to each other for a tile's 32-bit offsets.
-bool head_in_place(const void *p, uint64_t stride, const hbr_softmax &a) {
-    return a.dtype == HBR_BF16 && a.dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 22) &&
-           reinterpret_cast<uint64_t>(p) % 16 == 0;
-}
-
 // Every array has room for what any number of rows up to n takes (fewer rows
 // may be shared out finer, or taken in fewer pieces), and the arrays of a call
 // with gradients hold those of one without: a workspace serves smaller calls.
@@ -482,29 +475,11 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     Queue queue(ordinal, stream);
     const std::string suffix = name_of(p.dtype);
     const dim3 threads(256);
-    auto cells = [](uint64_t n) { return dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 16)); };
-    auto sum = [&](const char *kernel, const float *part, uint64_t parts, uint64_t part_stride, void *dst, uint64_t rows,
-                   uint64_t cols, uint64_t dst_stride) {
-        HeadSumArgs a{};
-        a.scale = p.grad_scale;
-        a.part = part;
-        a.parts = (uint32_t)parts;
-        a.part_stride = part_stride;
-        a.dst = dst;
-        a.rows = rows;
-        a.cols = cols;
-        a.dst_stride = dst_stride;
-        // few cells of many parts: a workgroup's waves share the parts
-        a.shares = 1;
-        while (a.shares < 16 && parts >= 8 * a.shares && rows * cols * a.shares < 64 * 2048) a.shares *= 4;
-        const uint32_t waves = a.shares == 16 ? 16 : 4;
-        const uint64_t each = waves / a.shares * 64;
-        queue.launch(kernel, dim3((uint32_t)std::min<uint64_t>(tiles(rows * cols, each), 1u << 16)), dim3(waves * 64), a);
-    };
-    const std::string sum_kernel = "hbr_head_sum_" + suffix;
+    auto sum = [&](uint32_t dtype, const float *part, uint64_t parts, uint64_t part_stride, void *dst, uint64_t rows, uint64_t cols,
+                   uint64_t dst_stride) { sum_parts(queue, dtype, p.grad_scale, part, parts, part_stride, dst, rows, cols, dst_stride); };
     if (n == 0) {  // sums over no rows
-        if (p.dw) sum(sum_kernel.c_str(), nullptr, 0, 0, p.dw, classes, dim, dw_stride);
-        if (p.db) sum("hbr_head_sum_f32", nullptr, 0, 0, p.db, 1, classes, classes);
+        if (p.dw) sum(p.dtype, nullptr, 0, 0, p.dw, classes, dim, dw_stride);
+        if (p.db) sum(HBR_F32, nullptr, 0, 0, p.db, 1, classes, classes);
         return;
     }
     if (q.few) {
@@ -556,37 +531,17 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         return;
     }
     // the operands of the products
-    struct Laid {
-        const char *p;
-        uint64_t row, chunk, part;
-        uint32_t cols;
-    };
-    auto lay = [&](const void *src, uint64_t stride, uint64_t rows, char *to, bool always, const int32_t *labels) -> Laid {
-        if (rows == 1) stride = up(dim, 8);
-        if (!always && head_in_place(src, stride, p))
-            return {static_cast<const char *>(src), stride * 2, 64, 0, (uint32_t)dim};
-        HeadPartsArgs a{};
-        a.src = src;
-        a.labels = labels;
-        a.dst = reinterpret_cast<uint16_t *>(to);
-        a.rows = rows;
-        a.src_stride = stride;
-        a.chunk = chunk_bytes(rows) / 2;
-        a.part = q.chunks * a.chunk;
-        a.cols = (uint32_t)dim;
-        a.chunks = (uint32_t)q.chunks;
-        queue.launch(("hbr_head_parts_" + suffix).c_str(), cells(rows * q.chunks * 4), threads, a);
-        return {static_cast<const char *>(to), 64, a.chunk * 2, a.part * 2, (uint32_t)(q.chunks * 32)};
+    auto lay = [&](const void *src, uint64_t stride, uint64_t rows, char *to, bool always, const int32_t *labels) {
+        return lay_rows(queue, src, stride, rows, dim, p.dtype, to, always, labels);
     };
     const bool by_rows = p.dw || p.db || q.narrow;  // rows that take no part are read with the others
     const Laid h = lay(p.h, p.h_stride, n, q.h, q.lay || by_rows, by_rows ? p.labels : nullptr);
     const Laid w = lay(p.w, p.w_stride, classes, q.w, q.lay, nullptr);
-    auto set_a = [](HeadArgs &a, const Laid &o) { a.a = o.p, a.a_row = o.row, a.a_chunk = o.chunk, a.a_part = o.part; };
-    auto set_b = [](HeadArgs &a, const Laid &o) { a.b = o.p, a.b_row = o.row, a.b_chunk = o.chunk, a.b_part = o.part; };
     auto product = [&](const std::string &kernel, const HeadTiling &t, HeadArgs a) {
         a.m_tiles = (uint32_t)tiles(a.m, t.tile);
         a.n_tiles = (uint32_t)tiles(a.n, t.tile);
         a.segments = (uint32_t)q.segments;
+        if (a.segments > 1) a.a_order = kPartA, a.b_order = kPartB;
         queue.launch((kernel + t.name).c_str(), dim3(a.m_tiles * a.n_tiles * a.splits), dim3((uint32_t)t.threads), a);
     };
     HeadArgs z{};
@@ -654,11 +609,11 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
     if (q.narrow) {
         if (p.dh) {
             walk("hbr_head_narrow_dh_", true, q.splits_h, q.dh);
-            sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
+            sum(p.dtype, q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
         }
         if (p.dw || p.db) walk("hbr_head_narrow_dw_", false, q.splits_w, q.dw);
-        if (p.dw) sum(sum_kernel.c_str(), q.dw, q.splits_w, classes * dim, p.dw, classes, dim, dw_stride);
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, q.splits_w, classes, p.db, 1, classes, classes);
+        if (p.dw) sum(p.dtype, q.dw, q.splits_w, classes * dim, p.dw, classes, dim, dw_stride);
+        if (p.db) sum(HBR_F32, q.part_db, q.splits_w, classes, p.db, 1, classes, classes);
         return;
     }
     for (uint64_t k0 = 0; k0 < classes; k0 += q.piece) {
@@ -685,7 +640,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
         g.g_part = pairs.part / 2;
         g.part_db = q.part_db;
         product("hbr_head_pairs_" + suffix, kTile128, g);
-        if (p.db) sum("hbr_head_sum_f32", q.part_db, tiles(n, kTile128.tile), q.piece, p.db + k0, 1, kc, kc);
+        if (p.db) sum(HBR_F32, q.part_db, tiles(n, kTile128.tile), q.piece, p.db + k0, 1, kc, kc);
         if (p.dw) {
             HeadArgs c{};
             set_a(c, pairs);
@@ -702,7 +657,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             c.c_stride = direct ? dw_stride : dim;
             c.c_split = q.piece * dim;
             product(direct && p.dtype == HBR_BF16 ? "hbr_head_dw_bf16" : "hbr_head_dw_part", *q.by_w, c);
-            if (!direct) sum(sum_kernel.c_str(), q.dw, q.splits_w, q.piece * dim, to, kc, dim, dw_stride);
+            if (!direct) sum(p.dtype, q.dw, q.splits_w, q.piece * dim, to, kc, dim, dw_stride);
         }
         if (p.dh) {
             HeadArgs c{};
@@ -720,7 +675,7 @@ void softmax_head(int ordinal, void *stream, const hbr_softmax &p, void *workspa
             product(!q.sum_h && p.dtype == HBR_BF16 ? "hbr_head_dh_bf16" : "hbr_head_dh_part", *q.by_h, c);
         }
     }
-    if (p.dh && q.sum_h) sum(sum_kernel.c_str(), q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
+    if (p.dh && q.sum_h) sum(p.dtype, q.dh, q.splits_h, n * dim, p.dh, n, dim, dh_stride);
 }
 
 // ---- clipping ----------------------------------------------------------------------------

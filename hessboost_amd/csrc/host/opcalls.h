@@ -152,6 +152,65 @@ inline uint64_t tiles(uint64_t n, uint64_t of) { return (n + of - 1) / of; }
 constexpr uint64_t kChunkStep = 2048;
 inline uint64_t chunk_bytes(uint64_t rows) { return ((rows * 64 + 2 * kChunkStep - 1) / (2 * kChunkStep) * 2 + 1) * kChunkStep; }
 
+// What the products can read in place: bf16 rows of whole 16-byte pieces,
+// near enough to each other for a tile's 32-bit offsets.
+inline bool head_in_place(const void *p, uint64_t stride, uint64_t dim, uint32_t dtype) {
+    return dtype == HBR_BF16 && dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 22) &&
+           reinterpret_cast<uint64_t>(p) % 16 == 0;
+}
+
+// An operand of a product, in place or laid out in chunks of 32 columns.
+struct Laid {
+    const char *p;
+    uint64_t row, chunk, part;
+    uint32_t cols;
+};
+inline void set_a(HeadArgs &a, const Laid &o) { a.a = o.p, a.a_row = o.row, a.a_chunk = o.chunk, a.a_part = o.part; }
+inline void set_b(HeadArgs &a, const Laid &o) { a.b = o.p, a.b_row = o.row, a.b_chunk = o.chunk, a.b_part = o.part; }
+
+inline dim3 cells_grid(uint64_t cells) { return dim3((uint32_t)std::min<uint64_t>((cells + 255) / 256, 1u << 16)); }
+
+// Rows of `dim` elements as an operand: in place where that can be and `lay` is
+// false, else laid out at `to`. labels: rows that take no part, or null.
+inline Laid lay_rows(Queue &queue, const void *src, uint64_t stride, uint64_t rows, uint64_t dim, uint32_t dtype, void *to, bool lay,
+                     const int32_t *labels) {
+    if (rows == 1) stride = up(dim, 8);
+    if (!lay && head_in_place(src, stride, dim, dtype)) return {static_cast<const char *>(src), stride * 2, 64, 0, (uint32_t)dim};
+    HeadPartsArgs a{};
+    a.src = src;
+    a.labels = labels;
+    a.dst = static_cast<uint16_t *>(to);
+    a.rows = rows;
+    a.src_stride = stride;
+    a.chunk = chunk_bytes(rows) / 2;
+    a.cols = (uint32_t)dim;
+    a.chunks = (uint32_t)tiles(dim, 32);
+    a.part = a.chunks * a.chunk;
+    queue.launch(dtype == HBR_F32 ? "hbr_head_parts_f32" : "hbr_head_parts_bf16", cells_grid(rows * a.chunks * 4), dim3(256), a);
+    return {static_cast<const char *>(to), 64, a.chunk * 2, a.part * 2, a.chunks * 32};
+}
+
+// dst = scale times the sum of the parts.
+inline void sum_parts(Queue &queue, uint32_t dtype, float scale, const float *part, uint64_t parts, uint64_t part_stride, void *dst,
+                      uint64_t rows, uint64_t cols, uint64_t dst_stride) {
+    HeadSumArgs a{};
+    a.scale = scale;
+    a.part = part;
+    a.parts = (uint32_t)parts;
+    a.part_stride = part_stride;
+    a.dst = dst;
+    a.rows = rows;
+    a.cols = cols;
+    a.dst_stride = dst_stride;
+    // few cells of many parts: a workgroup's waves share the parts
+    a.shares = 1;
+    while (a.shares < 16 && parts >= 8 * a.shares && rows * cols * a.shares < 64 * 2048) a.shares *= 4;
+    const uint32_t waves = a.shares == 16 ? 16 : 4;
+    const uint64_t each = waves / a.shares * 64;
+    queue.launch(dtype == HBR_F32 ? "hbr_head_sum_f32" : "hbr_head_sum_bf16",
+                 dim3((uint32_t)std::min<uint64_t>(tiles(rows * cols, each), 1u << 16)), dim3(waves * 64), a);
+}
+
 // A product's tiles, and how many of them fill 256 CUs (of the small ones twice
 // as many run at once, at hardly more rate).
 struct HeadTiling {

@@ -11,6 +11,8 @@
 #include "softmax_few.hip"
 #include "softmax_narrow.hip"
 #include "clip.hip"
+#include "norm.hip"
+#include "linear.hip"
 
 // The abi.h checksum this code object was built with (checked by the host
 // library at module load).

@@ -138,11 +138,6 @@ struct Operand {
     }
 };
 
-// The pairs of parts of a product of two f32 operands, smallest first: (2, 0),
-// (0, 2), (1, 1), (1, 0), (0, 1), (0, 0), two bits a segment.
-constexpr uint32_t kPartA = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
-constexpr uint32_t kPartB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
-
 // A workgroup's tile of the product: 32 W x 32 W of W waves, 2 x W / 2, the
 // operands of two steps in LDS.
 template <int W>
@@ -203,9 +198,9 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
                    s1 = (uint32_t)((uint64_t)steps * (t.split + 1) / a.splits);
     uint32_t seg = s0 / per, at = s0 % per;
     auto seek = [&] {
-        const uint32_t of = a.segments == 1 ? 10 : 2 * min(seg, 5u);
-        oa.seek(static_cast<const char *>(a.a) + (kPartA >> of & 3u) * a.a_part, a.a_row, a.a_chunk, t.m0, at);
-        ob.seek(static_cast<const char *>(a.b) + (kPartB >> of & 3u) * a.b_part, a.b_row, a.b_chunk, t.n0, at);
+        // (past the last segment its loads read nothing)
+        oa.seek(static_cast<const char *>(a.a) + (a.a_order >> 2 * seg & 3u) * a.a_part, a.a_row, a.a_chunk, t.m0, at);
+        ob.seek(static_cast<const char *>(a.b) + (a.b_order >> 2 * seg & 3u) * a.b_part, a.b_row, a.b_chunk, t.n0, at);
     };
     seek();
     // past the last step the loads read nothing

@@ -37,7 +37,7 @@ import sys
 
 from . import _capi as A
 
-_SIZE = {"float32": 4, "bfloat16": 2, "int32": 4, "uint8": 1}
+_SIZE = {"float32": 4, "bfloat16": 2, "int32": 4, "uint8": 1, "float8_e4m3fn": 1}
 _CODE = {"float32": A.F32, "bfloat16": A.BF16}
 _names: dict = {}
 

@@ -51,6 +51,7 @@ pub const HBR_TRANSFORM_CLASS_INDEX: c_int = 3;
 
 pub const HBR_F32: u32 = 0;
 pub const HBR_BF16: u32 = 1;
+pub const HBR_PACK_BLOCK: u32 = 32;
 
 // Opaque handles.
 #[repr(C)]
@@ -297,6 +298,112 @@ pub struct hbr_tensor {
     pub pad: u32,
 }
 
+#[repr(C)]
+pub struct hbr_packed {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub x_stride: u64,
+    pub codes_stride: u64,
+    pub scales_stride: u64,
+}
+
+#[repr(C)]
+pub struct hbr_norm {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub x_stride: u64,
+    pub residual_stride: u64,
+    pub out_stride: u64,
+    pub total_stride: u64,
+    pub codes_stride: u64,
+    pub scales_stride: u64,
+    pub x: *const c_void,
+    pub residual: *const c_void,
+    pub weight: *const f32,
+    pub out: *mut c_void,
+    pub total: *mut c_void,
+    pub inv: *mut f32,
+    pub codes: *mut u8,
+    pub scales: *mut u8,
+    pub eps: f32,
+    pub normed: u32,
+}
+
+#[repr(C)]
+pub struct hbr_norm_grad {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub dout_stride: u64,
+    pub x_stride: u64,
+    pub codes_stride: u64,
+    pub scales_stride: u64,
+    pub dtotal_stride: u64,
+    pub dx_stride: u64,
+    pub dout: *const c_void,
+    pub x: *const c_void,
+    pub codes: *const u8,
+    pub scales: *const u8,
+    pub inv: *const f32,
+    pub weight: *const f32,
+    pub dtotal: *const c_void,
+    pub dx: *mut c_void,
+    pub dweight: *mut f32,
+    pub eps: f32,
+    pub pad: u32,
+}
+
+#[repr(C)]
+pub struct hbr_linear_args {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub n_outs: u32,
+    pub rank: u32,
+    pub n_adapters: u32,
+    pub pad: u32,
+    pub x_stride: u64,
+    pub w_stride: u64,
+    pub out_stride: u64,
+    pub down_stride: u64,
+    pub up_stride: u64,
+    pub x: *const c_void,
+    pub w: *const c_void,
+    pub bias: *const f32,
+    pub down: *const c_void,
+    pub up: *const c_void,
+    pub ids: *const i32,
+    pub scale: *const f32,
+    pub out: *mut c_void,
+}
+
+#[repr(C)]
+pub struct hbr_linear_grad_args {
+    pub dtype: u32,
+    pub dim: u32,
+    pub n_rows: u64,
+    pub n_outs: u32,
+    pub pad: u32,
+    pub dout_stride: u64,
+    pub w_stride: u64,
+    pub x_stride: u64,
+    pub codes_stride: u64,
+    pub scales_stride: u64,
+    pub dx_stride: u64,
+    pub dw_stride: u64,
+    pub dout: *const c_void,
+    pub w: *const c_void,
+    pub x: *const c_void,
+    pub codes: *const u8,
+    pub scales: *const u8,
+    pub weight: *const f32,
+    pub dx: *mut c_void,
+    pub dw: *mut c_void,
+    pub db: *mut f32,
+}
+
 extern "C" {
     pub fn hbr_last_error(buf: *mut c_char, len: usize) -> usize;
     pub fn hbr_device_count(count: *mut c_int) -> c_int;
@@ -416,6 +523,20 @@ extern "C" {
     pub fn hbr_clip_gradients(ordinal: c_int, tensors: *const hbr_tensor, n_tensors: u64, max_norm: f64,
                               norm: *mut f32, workspace: *mut c_void, workspace_bytes: u64,
                               stream: *mut c_void) -> c_int;
+    pub fn hbr_pack_rows(ordinal: c_int, p: *const hbr_packed, x: *const c_void, codes: *mut u8, scales: *mut u8,
+                         stream: *mut c_void) -> c_int;
+    pub fn hbr_unpack_rows(ordinal: c_int, p: *const hbr_packed, codes: *const u8, scales: *const u8,
+                           weight: *const f32, x: *mut c_void, stream: *mut c_void) -> c_int;
+    pub fn hbr_rms_norm(ordinal: c_int, p: *const hbr_norm, stream: *mut c_void) -> c_int;
+    pub fn hbr_rms_norm_grad_workspace(n_rows: u64, dim: u32, dtype: u32, bytes: *mut u64) -> c_int;
+    pub fn hbr_rms_norm_grad(ordinal: c_int, p: *const hbr_norm_grad, workspace: *mut c_void,
+                             workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub fn hbr_linear_workspace(n_rows: u64, n_outs: u32, dim: u32, rank: u32, dtype: u32, bytes: *mut u64) -> c_int;
+    pub fn hbr_linear(ordinal: c_int, p: *const hbr_linear_args, workspace: *mut c_void, workspace_bytes: u64,
+                      stream: *mut c_void) -> c_int;
+    pub fn hbr_linear_grad_workspace(n_rows: u64, n_outs: u32, dim: u32, dtype: u32, bytes: *mut u64) -> c_int;
+    pub fn hbr_linear_grad(ordinal: c_int, p: *const hbr_linear_grad_args, workspace: *mut c_void,
+                           workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub fn hbr_device_alloc(ordinal: c_int, bytes: u64, out: *mut *mut c_void) -> c_int;
     pub fn hbr_device_free(ordinal: c_int, p: *mut c_void) -> c_int;
     pub fn hbr_device_upload(ordinal: c_int, dst: *mut c_void, src: *const c_void, bytes: u64) -> c_int;

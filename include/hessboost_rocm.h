@@ -766,6 +766,155 @@ int hbr_clip_gradients_workspace(uint64_t n_tensors, uint64_t *bytes);
 int hbr_clip_gradients(int ordinal, const hbr_tensor *tensors, uint64_t n_tensors, double max_norm, float *norm,
                        void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* Operators of the layers between leaf vectors and classes, called as the
+ * operators above are: device memory, a stream, a workspace of the caller's. No
+ * counterpart in the reference.
+ *
+ * Rows in 8 bits are e4m3 codes (a sign, four bits of exponent, three behind
+ * the leading one; 0x7f and 0xff no number) and a byte for every HBR_PACK_BLOCK
+ * columns of a row: columns 32 b to 32 b + 31 stand for code * 2^(scales[b] - 127).
+ * The power is the smallest of at least 2^-109 under which none of the block's
+ * finite elements is above 448, so that nothing saturates and every value is a
+ * bf16; elements are rounded to the nearest code, ties to even. An infinite
+ * element is held as no number. */
+#define HBR_PACK_BLOCK 32
+typedef struct hbr_packed {
+    uint32_t dtype;           /* of the rows that are not in 8 bits */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint64_t x_stride;
+    uint64_t codes_stride;
+    uint64_t scales_stride;
+} hbr_packed;
+/* Rows to 8 bits, and back (times weight, one f32 a column, or NULL: 1; rounded
+ * once). */
+int hbr_pack_rows(int ordinal, const hbr_packed *p, const void *x, uint8_t *codes, uint8_t *scales, void *stream);
+int hbr_unpack_rows(int ordinal, const hbr_packed *p, const uint8_t *codes, const uint8_t *scales, const float *weight,
+                    void *x, void *stream);
+
+/* The root-mean-square norm: s = x + residual (f32), inv = 1 / sqrt(mean s^2 +
+ * eps), normed = s * inv, out = normed * weight. Outputs are rounded once, from
+ * the f32 s, and each may be NULL; total holds s; codes and scales hold out, or
+ * with `normed` the normed rows, which the gradient reads. out and total may
+ * each be x or residual itself (the same address and stride), not the same one. */
+typedef struct hbr_norm {
+    uint32_t dtype;           /* of x, residual, out and total */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint64_t x_stride;
+    uint64_t residual_stride;
+    uint64_t out_stride;
+    uint64_t total_stride;
+    uint64_t codes_stride;
+    uint64_t scales_stride;
+    const void *x;
+    const void *residual;     /* or NULL: zeros */
+    const float *weight;      /* dim, or NULL: 1 */
+    void *out;                /* the outputs, or NULL */
+    void *total;
+    float *inv;               /* n_rows */
+    uint8_t *codes;           /* both or none */
+    uint8_t *scales;
+    float eps;
+    uint32_t normed;
+} hbr_norm;
+int hbr_rms_norm(int ordinal, const hbr_norm *p, void *stream);
+
+/* Its gradient: with g = dout * weight and the rows' normed values,
+ *   dx      = inv * (g - normed * mean(g * normed)) + dtotal,
+ *   dweight = the sum over rows of dout * normed,
+ * in f32, rounded once. The rows are x as the norm saw it (its total; inv may
+ * be NULL, and is made of x and eps then), or, with x NULL, the normed rows in
+ * 8 bits (inv is needed). dtotal is the gradient that reaches total otherwise,
+ * or NULL. dx may be dout or dtotal itself (the same address and stride). */
+typedef struct hbr_norm_grad {
+    uint32_t dtype;           /* of dout, x, dtotal and dx */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint64_t dout_stride;
+    uint64_t x_stride;
+    uint64_t codes_stride;
+    uint64_t scales_stride;
+    uint64_t dtotal_stride;
+    uint64_t dx_stride;
+    const void *dout;
+    const void *x;            /* or NULL: codes and scales */
+    const uint8_t *codes;
+    const uint8_t *scales;
+    const float *inv;         /* n_rows */
+    const float *weight;      /* dim, or NULL: 1 */
+    const void *dtotal;       /* or NULL: zeros */
+    void *dx;                 /* the outputs, or NULL */
+    float *dweight;           /* dim */
+    float eps;
+    uint32_t pad;
+} hbr_norm_grad;
+int hbr_rms_norm_grad_workspace(uint64_t n_rows, uint32_t dim, uint32_t dtype, uint64_t *bytes);
+int hbr_rms_norm_grad(int ordinal, const hbr_norm_grad *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* A projection of rows beside which every row has one of n_adapters low-rank
+ * adapters, or none (an id below 0, or of n_adapters and more; rank or
+ * n_adapters 0: no row has one):
+ *   out[r] = x[r] w^T + bias + scale[a] * ((x[r] down[a]^T) up[a]^T), a = ids[r],
+ * summed in f32 and rounded once; in bf16 the `rank` values between down and up
+ * are rounded to bf16 in calls of many rows. down holds n_adapters x rank rows of dim, up
+ * n_adapters x n_outs rows of rank. Rows may come in any order; those of one
+ * adapter next to each other take the least time. */
+typedef struct hbr_linear_args {
+    uint32_t dtype;           /* of x, w, out, down and up */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint32_t n_outs;
+    uint32_t rank;
+    uint32_t n_adapters;
+    uint32_t pad;
+    uint64_t x_stride;
+    uint64_t w_stride;
+    uint64_t out_stride;
+    uint64_t down_stride;
+    uint64_t up_stride;
+    const void *x;
+    const void *w;            /* n_outs rows of dim */
+    const float *bias;        /* n_outs, or NULL: 0 */
+    const void *down;         /* the adapters, or NULL: rank is 0 */
+    const void *up;
+    const int32_t *ids;       /* n_rows */
+    const float *scale;       /* n_adapters, or NULL: 1 */
+    void *out;
+} hbr_linear_args;
+int hbr_linear_workspace(uint64_t n_rows, uint32_t n_outs, uint32_t dim, uint32_t rank, uint32_t dtype, uint64_t *bytes);
+int hbr_linear(int ordinal, const hbr_linear_args *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* The gradients of out = x w^T + bias: dx = dout w, dw = dout^T x, db = the sum
+ * of dout's rows, in f32, rounded once; each may be NULL. Only dw reads the
+ * rows: x, or with x NULL rows in 8 bits, and weight (one f32 a column, or
+ * NULL: 1) as a factor of x's columns, as of a norm whose normed rows are held. */
+typedef struct hbr_linear_grad_args {
+    uint32_t dtype;           /* of dout, w, x, dx and dw */
+    uint32_t dim;
+    uint64_t n_rows;
+    uint32_t n_outs;
+    uint32_t pad;
+    uint64_t dout_stride;
+    uint64_t w_stride;
+    uint64_t x_stride;
+    uint64_t codes_stride;
+    uint64_t scales_stride;
+    uint64_t dx_stride;
+    uint64_t dw_stride;
+    const void *dout;
+    const void *w;            /* for dx */
+    const void *x;            /* for dw: these, or codes and scales */
+    const uint8_t *codes;
+    const uint8_t *scales;
+    const float *weight;
+    void *dx;
+    void *dw;
+    float *db;
+} hbr_linear_grad_args;
+int hbr_linear_grad_workspace(uint64_t n_rows, uint32_t n_outs, uint32_t dim, uint32_t dtype, uint64_t *bytes);
+int hbr_linear_grad(int ordinal, const hbr_linear_grad_args *p, void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* Device memory for callers that keep inputs resident (bytes on device
  * `ordinal`). */
 int hbr_device_alloc(int ordinal, uint64_t bytes, void **out);
