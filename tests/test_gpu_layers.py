@@ -1,0 +1,432 @@
+"""The operators of the layers between leaf vectors and classes against their
+plain forms in 64 bits, at the sizes, masks and layouts where they can go wrong."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+import hessboost_amd as hb
+import layer_reference as L
+import leaf_reference as R
+from hessboost_amd.leafops import DeviceArray
+from test_gpu_leafops import back, close, dev, like, work
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ("float32", "bfloat16")
+
+
+def bytes_(values, pad=0, lead=0):
+    """Bytes on the device, rows `pad` apart beyond their own; the gaps hold 0xEE."""
+    v = np.asarray(values, np.uint8)
+    stride = v.shape[1] + pad
+    whole = np.full(lead + v.shape[0] * stride, 0xEE, np.uint8)
+    for r in range(v.shape[0]):
+        whole[lead + r * stride: lead + r * stride + v.shape[1]] = v[r]
+    buf = hb.DeviceBuffer(max(16, whole.nbytes))
+    if whole.nbytes:
+        buf.upload(whole)
+    a = DeviceArray(buf, "uint8", v.shape, stride=stride, byte_offset=lead)
+    a.lead, a.pad = lead, pad
+    return a
+
+
+def bytes_back(a):
+    whole = a.buffer.download(np.uint8, a.buffer.nbytes)
+    stride = a.shape[1] + a.pad
+    body = whole[a.lead: a.lead + a.shape[0] * stride].reshape(a.shape[0], stride)
+    assert np.all(whole[:a.lead] == 0xEE) and np.all(body[:, a.shape[1]:] == 0xEE), "written outside the array"
+    return np.ascontiguousarray(body[:, :a.shape[1]])
+
+
+def packed_like(n, dim, pad=0, lead=0):
+    return (bytes_(np.full((n, dim), 0xAA), pad, lead), bytes_(np.full((n, hb.packed_scales(dim)), 0xAA), pad % 3, lead % 5))
+
+
+def rows(rng, n, dim, dtype, by=1.0):
+    v = rng.standard_normal((n, dim)) * np.exp(0.7 * rng.standard_normal((n, 1))) * by
+    return R.rounded(np.where(rng.random((n, dim)) < 0.02, 20.0 * v, v), dtype)
+
+
+def f32(rng, shape, by=1.0, to=0.0):
+    return (to + by * rng.standard_normal(shape)).astype(np.float32).astype(np.float64)
+
+
+# ---- rows in 8 bits -------------------------------------------------------------------
+
+# rows, dim, stride gap, lead
+PACKS = [(1, 1, 0, 0), (3, 31, 0, 0), (5, 32, 0, 0), (4, 33, 3, 1), (7, 50, 0, 0), (2, 64, 16, 16), (9, 127, 1, 0), (300, 8, 0, 0),
+         (3, 1000, 8, 8), (2, 4100, 4, 4), (1, 70_001, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, pad, lead", PACKS)
+def test_rows_are_packed_to_the_nearest_codes(n, dim, pad, lead, dtype):
+    """Bit for bit, and unpacked to just what the codes stand for."""
+    rng = np.random.default_rng(dim)
+    v = rows(rng, n, dim, dtype, 10.0 ** rng.integers(-30, 30))
+    v[rng.random(v.shape) < 0.1] = 0.0
+    codes, scales = packed_like(n, dim, pad, lead)
+    hb.pack_rows(dev(v, dtype, pad, lead), codes, scales)
+    want = L.codes_of(v)
+    assert np.array_equal(bytes_back(scales), want[1])
+    assert np.array_equal(bytes_back(codes), want[0])
+    held = L.values_of(*want)
+    for to in DTYPES:
+        out = like((n, dim), to, pad, lead)
+        hb.unpack_rows(codes, scales, out)
+        assert np.array_equal(back(out), held)
+    weight = f32(rng, dim)
+    out = like((n, dim), dtype, pad, lead)
+    hb.unpack_rows(codes, scales, out, weight=dev(weight, "float32"))
+    close(back(out), (held * weight, (R.EPS32 + R.HALF[dtype]) * np.abs(held * weight) + 1e-40), "weighted")
+
+
+def test_packed_borders_and_values_that_are_no_numbers():
+    """Every code's value and every tie between two, powers' borders, the
+    least power, zeros of both signs, infinities and NaN beside numbers."""
+    grid = L.code_values()[:127]
+    ties = (grid[1:] + grid[:-1]) / 2
+    some = np.concatenate([grid, ties, [np.nextafter(np.float32(448), np.float32(0)), 464.0, 479.0, 480.0, 0.0]])
+    some = np.concatenate([some, -some])
+    lines = []
+    for e in (0, -3, 60, -60, -100, -109, -112, -126, 118):
+        for first in (448.0, 1.0, 449.0, 0.0):
+            line = np.zeros((-(-len(some) // 31), 32))
+            line[:, 0] = first
+            line[:, 1:].flat[:len(some)] = some
+            lines.append(line * 2.0 ** e)
+    v = np.concatenate(lines).astype(np.float32).astype(np.float64)
+    v[5, 3], v[5, 4], v[6, 0], v[7] = np.inf, -np.inf, np.nan, np.nan
+    v[8] = np.where(np.arange(32) % 2, -0.0, 0.0)
+    v = v.reshape(-1, 64) if len(v) % 2 == 0 else v[:-1].reshape(-1, 64)
+    codes, scales = packed_like(*v.shape)
+    hb.pack_rows(dev(v, "float32"), codes, scales)
+    want = L.codes_of(v)
+    assert np.array_equal(bytes_back(scales), want[1])
+    got = bytes_back(codes)
+    nan = ~np.isfinite(v)
+    assert np.all((got & 0x7F)[nan] == 0x7F) and np.array_equal(got[~nan], want[0][~nan])
+
+
+# ---- the norm ----------------------------------------------------------------------------
+
+# rows, dim, residual, weight, stride gap, lead
+NORMS = [(1, 1, False, False, 0, 0), (3, 5, True, True, 0, 0), (65, 32, True, False, 0, 0), (1000, 50, False, True, 0, 0),
+         (33, 64, True, True, 8, 8), (7, 129, True, True, 1, 1), (5, 512, False, True, 0, 0), (9, 1000, True, True, 2, 2),
+         (130, 1024, True, True, 0, 0), (4, 1500, True, False, 4, 0), (3, 2049, False, True, 0, 0), (3, 4096, True, True, 0, 0),
+         (2, 5001, True, True, 0, 3), (2, 8200, False, True, 0, 0), (2, 17_000, True, True, 0, 0), (1, 40_000, True, True, 8, 8),
+         (2, 33_333, True, True, 1, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, residual, weight, pad, lead", NORMS)
+def test_norms(n, dim, residual, weight, pad, lead, dtype):
+    rng = np.random.default_rng(n * 7 + dim)
+    x, eps = rows(rng, n, dim, dtype), np.float32(1e-5)
+    r = rows(rng, n, dim, dtype) if residual else None
+    w = f32(rng, dim, 0.3, 1.0) if weight else None
+    x[-1] = 0.0  # a padded row
+    if residual:
+        r[-1] = 0.0
+    want = L.norm(x, r, w, float(eps), dtype)
+    args = dict(weight=None if w is None else dev(w, "float32"), eps=float(eps),
+                residual=None if r is None else dev(r, dtype, pad, lead))
+    for normed in (False, True):
+        out, total, inv = like((n, dim), dtype, pad, lead), like((n, dim), dtype, pad, lead), like(n, "float32")
+        codes, scales = packed_like(n, dim, pad, lead)
+        hb.rms_norm(dev(x, dtype, pad, lead), out, total=total, inv=inv, codes=codes, scales=scales, normed=normed, **args)
+        close(back(out), want["out"], "out")
+        close(back(total), want["total"], "total")
+        close(back(inv), want["inv"], "inv")
+        c, s = bytes_back(codes), bytes_back(scales)
+        value, off = want["normed"] if normed else (want["out"][0], want["out"][1] - R.HALF[dtype] * np.abs(want["out"][0]))
+        power = np.repeat(2.0 ** (s.astype(np.float64) - 127), 32, 1)[:, :dim]
+        close(L.values_of(c, s), (value, 2.0 ** -4 * (np.abs(value) + off) + 2.0 ** -10 * power + off), "held")
+        # the power is the least, but for what the values are off by
+        top = np.stack([np.max(np.abs(value[:, b:b + 32]), 1) for b in range(0, dim, 32)], 1)
+        p = 2.0 ** (s.astype(np.float64) - 127)
+        assert np.all(top <= 448 * p * (1 + 1e-3)) and np.all((top > 224 * p * (1 - 1e-3)) | (s == 18))
+    # each output by itself, and without codes (another number of lanes)
+    out, total, inv = like((n, dim), dtype, pad, lead), like((n, dim), dtype), like(n, "float32")
+    hb.rms_norm(dev(x, dtype), out, **args)
+    hb.rms_norm(dev(x, dtype), total=total, **args)
+    hb.rms_norm(dev(x, dtype), inv=inv, **args)
+    close(back(out), want["out"], "out alone")
+    close(back(total), want["total"], "total alone")
+    close(back(inv), want["inv"], "inv alone")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [50, 1024, 40_000])
+def test_norms_in_place(dim, dtype):
+    rng = np.random.default_rng(dim)
+    n = 5
+    x, r, w = rows(rng, n, dim, dtype), rows(rng, n, dim, dtype), f32(rng, dim)
+    want = L.norm(x, r, w, 1e-6, dtype)
+    dx, dr = dev(x, dtype), dev(r, dtype)
+    hb.rms_norm(dx, dx, weight=dev(w, "float32"), residual=dr, total=dr)
+    close(back(dx), want["out"], "out over x")
+    close(back(dr), want["total"], "total over the residual")
+    dx, dr = dev(x, dtype), dev(r, dtype)
+    hb.rms_norm(dx, dr, weight=dev(w, "float32"), residual=dr, total=dx)
+    close(back(dr), want["out"], "out over the residual")
+    close(back(dx), want["total"], "total over x")
+
+
+@pytest.mark.parametrize("dim", [3, 300, 20_000])
+def test_norms_of_rows_beyond_the_range_of_f32_squares(dim):
+    """Squares past f32's range or below it, alone and beside ordinary rows."""
+    rng = np.random.default_rng(dim)
+    x = f32(rng, (8, dim))
+    x[0] *= 1e25
+    x[1] *= 1e-30
+    x[2] *= 3e36 / np.max(np.abs(x[2]))
+    x[4, 0] = 1e22
+    x = x.astype(np.float32).astype(np.float64)
+    for eps in (0.0, 1e-6):
+        want = L.norm(x, None, None, eps, "float32")
+        out, inv = like(x.shape, "float32"), like(8, "float32")
+        hb.rms_norm(dev(x, "float32"), out, eps=eps, inv=inv)
+        # (below 2^-126 inv has steps of 2^-149)
+        value, off = want["inv"]
+        close(back(inv), (value, off + 2.0 ** -149), "inv")
+        value, off = want["out"]
+        close(back(out), (value, off + np.abs(x) * 2.0 ** -149), "out")
+
+
+def test_norms_of_values_that_are_no_numbers_stay_in_their_rows():
+    rng = np.random.default_rng(5)
+    x = f32(rng, (9, 70))
+    clean = L.norm(x, None, None, 1e-6, "float32")["out"]
+    x[2, 3], x[5, 69], x[7, 0] = np.inf, np.nan, -np.inf
+    out = like(x.shape, "float32")
+    codes, scales = packed_like(*x.shape)
+    hb.rms_norm(dev(x, "float32"), out, codes=codes, scales=scales)
+    got, held = back(out), L.values_of(bytes_back(codes), bytes_back(scales))
+    others = [r for r in range(9) if r not in (2, 5, 7)]
+    close(got[others], (clean[0][others], clean[1][others]), "the other rows")
+    assert np.all(np.isnan(got[5])) and np.all(np.isnan(held[5]))
+    for r, c in ((2, 3), (7, 0)):  # 1 / infinity, and infinity times that
+        assert np.isnan(got[r, c]) and np.isnan(held[r, c])
+        rest = np.arange(70) != c
+        assert np.all(got[r, rest] == 0) and np.all(held[r, rest] == 0)
+
+
+GRADS = [(1, 1, False, False, 0, 0), (3, 5, True, True, 0, 0), (65, 32, True, False, 0, 0), (2000, 50, False, True, 0, 0),
+         (33, 64, True, True, 8, 8), (7, 129, True, True, 1, 1), (9, 1000, True, True, 2, 2), (700, 1024, True, True, 0, 0),
+         (4, 1500, True, False, 4, 0), (3, 2049, False, True, 0, 0), (3, 4096, True, True, 0, 0), (2, 9000, False, True, 0, 0),
+         (3, 40_000, True, True, 8, 8), (1030, 33_333 // 8, True, True, 1, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, dtotal, weight, pad, lead", GRADS)
+def test_norm_gradients(n, dim, dtotal, weight, pad, lead, dtype):
+    rng = np.random.default_rng(n + dim)
+    x, dout = rows(rng, n, dim, dtype), rows(rng, n, dim, dtype, 1.0 / n)
+    t = rows(rng, n, dim, dtype, 1.0 / n) if dtotal else None
+    w = f32(rng, dim, 0.3, 1.0) if weight else None
+    eps = float(np.float32(1e-5))
+    inv = (1.0 / np.sqrt(np.mean(x * x, 1) + eps)).astype(np.float32).astype(np.float64)
+    held = L.codes_of(np.asarray(x * inv[:, None], np.float32).astype(np.float64))
+    args = dict(weight=None if w is None else dev(w, "float32"), dtotal=None if t is None else dev(t, dtype, pad, lead), eps=eps)
+    ways = [("rows", dict(x=dev(x, dtype, pad, lead), inv=dev(inv, "float32")), (x, inv, False)),
+            ("rows alone", dict(x=dev(x, dtype, pad, lead)), (x, None, False)),
+            ("held", dict(codes=bytes_(held[0], pad, lead), scales=bytes_(held[1]), inv=dev(inv, "float32")),
+             (L.values_of(*held), inv, True))]
+    ws = work(hb.rms_norm_grad_workspace(n, dim, dtype))
+    for name, of, (v, by, is_held) in ways:
+        want = L.norm_grad(dout, v, by, w, t, eps, is_held, dtype)
+        dx, dweight = like((n, dim), dtype, pad, lead), like(dim, "float32")
+        hb.rms_norm_grad(dev(dout, dtype, pad, lead), dx, dweight=dweight, workspace=ws, **of, **args)
+        close(back(dx), want["dx"], f"{name}: dx")
+        close(back(dweight), want["dweight"], f"{name}: dweight")
+        dx = like((n, dim), dtype)
+        hb.rms_norm_grad(dev(dout, dtype), dx, **of, **args)
+        close(back(dx), want["dx"], f"{name}: dx alone")
+    alone = like(dim, "float32")
+    hb.rms_norm_grad(dev(dout, dtype), dweight=alone, workspace=ws, **of, **args)
+    assert np.array_equal(back(alone), back(dweight))
+    # over its inputs
+    for over in ("dout", "dtotal"):
+        if over == "dtotal" and t is None:
+            continue
+        g, d = dev(dout, dtype), None if t is None else dev(t, dtype)
+        to = g if over == "dout" else d
+        hb.rms_norm_grad(g, to, **of, **{**args, "dtotal": d})
+        close(back(to), want["dx"], f"dx over {over}")
+
+
+def test_norm_gradients_agree_with_differences():
+    """d/dt of <dout, rms_norm(x + t e)> by central differences in 64 bits."""
+    rng = np.random.default_rng(8)
+    n, dim, eps = 4, 37, 1e-5
+    x, dout, w = f32(rng, (n, dim)), f32(rng, (n, dim)), f32(rng, dim, 0.3, 1.0)
+    dx, dweight = like((n, dim), "float32"), like(dim, "float32")
+    hb.rms_norm_grad(dev(dout, "float32"), dx, x=dev(x, "float32"), weight=dev(w, "float32"), eps=eps, dweight=dweight,
+                     workspace=work(hb.rms_norm_grad_workspace(n, dim, "float32")))
+
+    def loss(x, w):
+        return np.sum(dout * x / np.sqrt(np.mean(x * x, 1, keepdims=True) + eps) * w)
+
+    for got, of in ((back(dx), "x"), (back(dweight), "w")):
+        for _ in range(10):
+            e = rng.standard_normal(got.shape)
+            h = 1e-4
+            up, down = ((x + h * e, w), (x - h * e, w)) if of == "x" else ((x, w + h * e), (x, w - h * e))
+            slope = (loss(*up) - loss(*down)) / (2 * h)
+            # differences are off by h^2 (1e-8 of third derivatives below 1e3), the gradient by f32's roundings
+            assert abs(np.sum(got * e) - slope) <= 1e-5 * np.sum(np.abs(got * e)) + 1e-5
+
+
+# ---- projections -----------------------------------------------------------------------------
+
+# rows, dim, outs, rank, adapters, order of ids, bias, scale, stride gap, lead
+LINEARS = [
+    (1, 1, 1, 0, 0, None, False, False, 0, 0),
+    (1, 8, 16, 1, 1, "one", True, True, 0, 0),
+    (3, 33, 17, 2, 3, "each", True, False, 0, 0),
+    (7, 256, 300, 16, 9, "each", True, True, 0, 0),
+    (16, 64, 64, 8, 4, "runs", False, True, 8, 8),
+    (17, 70, 130, 5, 3, "mixed", True, True, 1, 1),
+    (64, 128, 256, 64, 2, "runs", True, True, 0, 0),
+    (65, 40, 129, 7, 70, "each", True, True, 0, 0),
+    (130, 96, 257, 16, 200, "each", True, True, 0, 0),
+    (200, 512, 96, 33, 5, "mixed", False, True, 8, 0),
+    (300, 250, 515, 9, 5, "runs", True, True, 0, 0),
+    (257, 1024, 264, 16, 6, "runs", True, True, 0, 0),
+    (600, 31, 40, 3, 2, "none", True, True, 0, 0),
+    (129, 2048, 128, 0, 0, None, True, False, 0, 0),
+    (1100, 64, 1030, 24, 30, "mixed", True, True, 2, 0),
+]
+
+
+def ids_of(rng, n, adapters, order):
+    if order == "one":
+        return np.zeros(n, np.int32)
+    if order == "none":
+        return np.where(rng.random(n) < 0.5, -1, adapters + rng.integers(0, 5, n)).astype(np.int32)
+    if order == "each":
+        return (np.arange(n) * 7 % adapters).astype(np.int32)
+    if order == "mixed":
+        return rng.integers(-1, adapters + 1, n).astype(np.int32)
+    return np.sort(rng.integers(-1, adapters, n)).astype(np.int32)[::-1].copy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, outs, rank, adapters, order, bias, scale, pad, lead", LINEARS)
+def test_projections(n, dim, outs, rank, adapters, order, bias, scale, pad, lead, dtype):
+    rng = np.random.default_rng(n + dim + outs)
+    x, w = rows(rng, n, dim, dtype), R.rounded(rng.standard_normal((outs, dim)) / np.sqrt(dim), dtype)
+    b = f32(rng, outs) if bias else None
+    down = up = ids = s = None
+    args = {}
+    if rank:
+        down = R.rounded(rng.standard_normal((adapters, rank, dim)) / np.sqrt(dim), dtype)
+        up = R.rounded(rng.standard_normal((adapters, outs, rank)), dtype)
+        ids = ids_of(rng, n, adapters, order)
+        s = f32(rng, adapters, 0.5, 1.0) if scale else None
+        args = dict(down=dev(down.reshape(-1, dim), dtype, pad, lead), up=dev(up.reshape(-1, rank), dtype, pad, lead),
+                    ids=dev(ids, "int32"), scale=None if s is None else dev(s, "float32"))
+    out = like((n, outs), dtype, pad, lead)
+    hb.linear(dev(x, dtype, pad, lead), dev(w, dtype, pad, lead), out, bias=None if b is None else dev(b, "float32"),
+              workspace=work(hb.linear_workspace(n, outs, dim, dtype, rank=rank)), **args)
+    close(back(out), L.linear(x, w, b, down, up, ids, s, dtype), "out")
+
+
+def test_a_row_without_an_adapter_reads_none():
+    """NaN adapters that no row has, and NaN rows beside others."""
+    rng = np.random.default_rng(3)
+    for n in (5, 140):
+        x, w = f32(rng, (n, 48)), f32(rng, (70, 48))
+        down, up = f32(rng, (3, 4, 48)), f32(rng, (3, 70, 4))
+        down[1], up[1] = np.nan, np.nan
+        ids = np.where(np.arange(n) % 3 == 0, 0, np.where(np.arange(n) % 3 == 1, -1, 2)).astype(np.int32)
+        x[1] = np.nan
+        for dtype in DTYPES:
+            xs, ws, d, u = (R.rounded(v, dtype) for v in (x, w, down, up))
+            out = like((n, 70), dtype)
+            hb.linear(dev(xs, dtype), dev(ws, dtype), out, down=dev(d.reshape(-1, 48), dtype), up=dev(u.reshape(-1, 4), dtype),
+                      ids=dev(ids, "int32"), workspace=work(hb.linear_workspace(n, 70, 48, dtype, rank=4)))
+            got = back(out)
+            assert np.all(np.isnan(got[1]))
+            xs[1], d[1], u[1] = 0.0, 0.0, 0.0
+            value, off = L.linear(xs, ws, None, d, u, ids, None, dtype)
+            keep = np.arange(n) != 1
+            close(got[keep], (value[keep], off[keep]), dtype)
+
+
+def test_infinite_inputs_of_a_projection():
+    """An infinity reaches its row's outputs as f32 arithmetic says."""
+    rng = np.random.default_rng(4)
+    for n in (3, 150):
+        x, w = f32(rng, (n, 40)), f32(rng, (66, 40))
+        x[2, 7] = np.inf
+        w[5, 7] = 0.0
+        for dtype in DTYPES:
+            xs, ws = R.rounded(x, dtype), R.rounded(w, dtype)
+            out = like((n, 66), dtype)
+            hb.linear(dev(xs, dtype), dev(ws, dtype), out, workspace=work(hb.linear_workspace(n, 66, 40, dtype)))
+            got = back(out)
+            assert np.isnan(got[2, 5])
+            rest = np.arange(66) != 5
+            assert np.array_equal(got[2, rest], np.where(ws[rest, 7] > 0, np.inf, -np.inf))
+            xs[2] = 0.0
+            value, off = L.linear(xs, ws, None, None, None, None, None, dtype)
+            keep = np.arange(n) != 2
+            close(got[keep], (value[keep], off[keep]), dtype)
+
+
+# rows, dim, outs, weight, stride gap, lead
+LINEAR_GRADS = [(1, 1, 1, False, 0, 0), (1, 64, 40, True, 0, 0), (5, 33, 17, True, 0, 0), (64, 32, 8, False, 0, 0), (100, 50, 70, True, 1, 1),
+                (130, 256, 136, True, 8, 8), (1000, 64, 64, True, 0, 0), (515, 250, 333, False, 0, 0), (2000, 96, 300, True, 0, 0),
+                (300, 1032, 520, True, 8, 0), (3001, 40, 24, True, 0, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, outs, weight, pad, lead", LINEAR_GRADS)
+def test_projection_gradients(n, dim, outs, weight, pad, lead, dtype):
+    rng = np.random.default_rng(n + dim + outs)
+    x, dout, w = rows(rng, n, dim, dtype), rows(rng, n, outs, dtype, 1.0 / n), rows(rng, outs, dim, dtype)
+    by = f32(rng, dim, 0.3, 1.0) if weight else None
+    held = L.codes_of(x)
+    ws = work(hb.linear_grad_workspace(n, outs, dim, dtype))
+    weights = None if by is None else dev(by, "float32")
+    for name, of, v in (("rows", dict(x=dev(x, dtype, pad, lead)), x),
+                        ("held", dict(codes=bytes_(held[0], pad, lead), scales=bytes_(held[1], pad % 3)), L.values_of(*held))):
+        want = L.linear_grad(dout, w, v, by, dtype)
+        got = dict(dx=like((n, dim), dtype, pad, lead), dw=like((outs, dim), dtype, pad, lead), db=like(outs, "float32"))
+        hb.linear_grad(dev(dout, dtype, pad, lead), dev(w, dtype, pad, lead), weight=weights, workspace=ws, **of, **got)
+        whole = {k: back(a) for k, a in got.items()}
+        for k in got:
+            close(whole[k], want[k], f"{name}: {k}")
+    # each by itself
+    g = dev(dout, dtype)
+    dx, dw, db = like((n, dim), dtype), like((outs, dim), dtype), like(outs, "float32")
+    hb.linear_grad(g, dev(w, dtype), dx=dx, workspace=ws)
+    hb.linear_grad(g, weight=weights, dw=dw, workspace=ws, **of)
+    hb.linear_grad(g, dev(w, dtype), db=db, workspace=ws)
+    close(back(dx), want["dx"], "dx alone")
+    close(back(dw), want["dw"], "dw alone")
+    close(back(db), want["db"], "db alone")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_rows(dtype):
+    """Nothing is written but the gradients' sums, which are zeros."""
+    none, dim, outs = np.zeros((0, 40)), 40, 24
+    codes, scales = packed_like(0, dim)
+    hb.pack_rows(dev(none, dtype), codes, scales)
+    hb.unpack_rows(codes, scales, dev(none, dtype))
+    hb.rms_norm(dev(none, dtype), dev(none, dtype))
+    dweight, dw, db = like(dim, "float32"), like((outs, dim), dtype), like(outs, "float32")
+    hb.rms_norm_grad(dev(none, dtype), dev(none, dtype), x=dev(none, dtype), dweight=dweight,
+                     workspace=work(hb.rms_norm_grad_workspace(0, dim, dtype)))
+    w, out = dev(np.ones((outs, dim)), dtype), dev(np.zeros((0, outs)), dtype)
+    hb.linear(dev(none, dtype), w, out, workspace=work(hb.linear_workspace(0, outs, dim, dtype)))
+    hb.linear_grad(out, w, x=dev(none, dtype), dx=dev(none, dtype), dw=dw, db=db,
+                   workspace=work(hb.linear_grad_workspace(0, outs, dim, dtype)))
+    for a in (dweight, dw, db):
+        assert np.all(back(a) == 0)
