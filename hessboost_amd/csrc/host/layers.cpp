@@ -250,6 +250,12 @@ uint64_t part_rows(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
     return most > 1 ? std::min(65536 / tiles(n, kTile256.tile), m * most) : 0;
 }
 
+// Tiles that do not fill the device have a CU each, and its LDS for more steps
+// in flight.
+std::string tile_name(const HeadTiling &t, uint64_t groups) {
+    return std::string(t.name) + (t.tile == 128 && groups <= 256 ? "_deep" : "");
+}
+
 uint64_t laid_bytes(uint64_t rows, uint64_t cols, uint64_t parts) { return parts * tiles(cols, 32) * chunk_bytes(rows); }
 
 void check_product(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, const char *what) {
@@ -263,6 +269,9 @@ void check_product(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, cons
 void check_tiles(uint64_t m, uint64_t n, const char *what) {
     if (tiles(m, 128) * tiles(n, 128) >= 1u << 22) fail(kRefused, std::string(what) + ": 2^22 tiles of 128 x 128 or more");
 }
+
+// Rows up to which w is read straight into the matrix instructions' registers.
+constexpr uint64_t kFewRows = 64;
 
 struct LinearPlan {
     char *x, *w;
@@ -318,6 +327,11 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
                  {rank ? p.scale : nullptr, p.n_adapters * 4ull}}, Extent(workspace, q.bytes), what);
     Queue queue(ordinal, stream);
     const std::string type = name_of(p.dtype);
+    // rows of whole 16 bytes, or element by element
+    auto strips = [&](const char *name, std::initializer_list<const Rows *> all) {
+        const uint32_t v = rows_vector(size, dim, all);
+        return kernel_of(name, p.dtype, v == 16 / size ? v : 1);
+    };
     if (rank) {
         LinearLowArgs a{};
         a.x = p.x;
@@ -331,7 +345,32 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         a.dim = p.dim;
         a.rank = p.rank;
         a.adapters = p.n_adapters;
-        queue.launch(("hbr_linear_low_" + type).c_str(), dim3((uint32_t)std::min<uint64_t>(tiles(n, 4), 1u << 16)), dim3(256), a);
+        // 16 rows a workgroup; of few of them several for the adapters' ranks
+        const uint64_t groups = tiles(n, 16), most = tiles(std::min<uint64_t>(n, 16) * rank, 32);
+        queue.launch(strips("hbr_linear_low", {&x, &down}).c_str(), dim3((uint32_t)groups, (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups))),
+                     dim3(256), a);
+    }
+    if (n <= kFewRows) {
+        LinearFewArgs a{};
+        a.x = p.x;
+        a.w = p.w;
+        a.bias = p.bias;
+        a.out = p.out;
+        a.low = rank ? q.low : nullptr;
+        a.up = p.up;
+        a.ids = p.ids;
+        a.x_stride = x.stride;
+        a.w_stride = w.stride;
+        a.out_stride = out.stride;
+        a.up_stride = up_rows.stride;
+        a.n_rows = (uint32_t)n;
+        a.dim = p.dim;
+        a.outs = p.n_outs;
+        a.rank = p.rank;
+        a.adapters = p.n_adapters;
+        queue.launch((strips("hbr_linear_few", {&x, &w}) + (n <= 16 ? "_16" : n <= 32 ? "_32" : "_64")).c_str(), dim3((uint32_t)tiles(outs, 16)),
+                     dim3(256), a);
+        return;
     }
     LinearArgs a{};
     set_a(a.p, lay_rows(queue, p.x, x.stride, n, dim, p.dtype, q.x, false, nullptr));
@@ -356,8 +395,9 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
     a.up_stride = up_rows.stride;
     a.rank = p.rank;
     a.adapters = p.n_adapters;
-    queue.launch(("hbr_linear_y_" + std::string(shared ? "part_" : "") + type + q.tiling->name).c_str(),
-                 dim3(a.p.m_tiles * a.p.n_tiles * a.p.splits), dim3((uint32_t)q.tiling->threads), a);
+    const uint32_t groups = a.p.m_tiles * a.p.n_tiles * a.p.splits;
+    queue.launch(("hbr_linear_y_" + std::string(shared ? "part_" : "") + type + tile_name(*q.tiling, groups)).c_str(),
+                 dim3(groups), dim3((uint32_t)q.tiling->threads), a);
     if (!shared) return;
     LinearJoinArgs j{};
     j.part = q.part;
@@ -481,7 +521,8 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
         a.p.c = shared ? (void *)part : const_cast<void *>(to.p);
         a.p.c_stride = shared ? dim : to.stride;
         a.p.c_split = to.n * dim;
-        queue.launch((std::string(name) + (shared ? "part" : type) + t.name).c_str(), dim3(a.p.m_tiles * a.p.n_tiles * a.p.splits),
+        const uint32_t groups = a.p.m_tiles * a.p.n_tiles * a.p.splits;
+        queue.launch((std::string(name) + (shared ? "part" : type) + tile_name(t, groups)).c_str(), dim3(groups),
                      dim3((uint32_t)t.threads), a);
         if (shared) join(part, a.p.splits, a.p.weight, to);
     };
