@@ -1338,28 +1338,33 @@ struct PackArgs {
     uint32_t each;              // vectors of a row a workgroup's lane takes
 };
 
-// A projection's products (p.c: the result, or [split] parts of its sums). Of
-// the result's columns p.weight are factors and p.bias is added; of a
-// projection's rows (hbr_linear_y_*) the first share adds the adapters.
+// A projection's products and its gradients'. A tile lies on the result's side:
+// m are its columns, n its rows, so that a lane holds four columns of a row at a
+// time. Of the columns `weight` are factors and `bias` is added.
 struct LinearArgs {
-    HeadArgs p;
+    HeadArgs p;                 // p.m, p.n: to the end of the last chunk of a transposed operand
+    uint32_t rows, cols;        // of the result
+    void *out;
+    uint64_t out_stride;
+    const float *weight, *bias; // or null
+    // the sums of a share of the steps as the lanes hold them: [split][tile]
+    // [cell / 4 / threads][thread] of four columns; or null: the result
+    float *part;
+    float *part_b;              // dw's: [split][column tile][rows], the sums of dout's rows; or null
+    // a projection's adapters
     const float *low;           // [row][rank]: the rows times their adapters' first factors and scales, or null
-    const void *up;             // [adapter][n][rank], rows up_stride apart
-    const int32_t *ids;         // of the rows
+    const void *up;             // [adapter][cols][rank], rows up_stride apart
+    const int32_t *ids;         // of the rows (the shares' join)
+    const uint16_t *slot_of;    // of the rows: which of its tile's adapters, or kNoSlot
+    const int32_t *slot_id;     // [row tile][tile]: the tile's adapters
+    const uint32_t *slots;      // [row tile]: how many
     uint64_t up_stride;
     uint32_t rank, adapters;
 };
+constexpr uint32_t kNoSlot = 0xffff;
 
-// dst = the sum of the parts, times the column's factor, and the column's bias.
-struct LinearJoinArgs {
-    const float *part;
-    const float *weight, *bias; // or null
-    void *dst;
-    uint64_t rows, cols, dst_stride, part_stride;
-    uint32_t parts, pad;
-};
-
-// hbr_linear_low_*: low[row][rho] = scale[a] <x[row], down[a][rho]>, a the row's adapter.
+// hbr_linear_low_*: low[row][rho] = scale[a] <x[row], down[a][rho]>, a the row's
+// adapter; and which adapters a projection's tiles have.
 struct LinearLowArgs {
     const void *x, *down;
     const int32_t *ids;
@@ -1367,6 +1372,11 @@ struct LinearLowArgs {
     float *low;
     uint64_t x_stride, down_stride;
     uint32_t n_rows, dim, rank, adapters;
+    // workgroups from `groups` on: the adapters of a tile of `tile` rows
+    uint32_t groups, tile;
+    uint16_t *slot_of;
+    int32_t *slot_id;
+    uint32_t *slots;
 };
 
 // Few rows: hbr_linear_few_*.
@@ -1381,12 +1391,19 @@ struct LinearFewArgs {
     uint32_t n_rows, dim, outs, rank, adapters, pad;
 };
 
-// Rows in 8 bits as bf16 in chunks of 32 columns (zeros past cols).
-struct LayCodesArgs {
-    const uint8_t *codes, *scales;
+// hbr_lay: operands in chunks of 64 columns (zeros past cols): f32 in three bf16
+// parts, bf16 as it is, rows in 8 bits as the bf16 that they stand for.
+constexpr uint32_t kLayF32 = 0, kLayBf16 = 1, kLayCodes = 2;
+struct LayArray {
+    const void *src;
+    const uint8_t *scales;
     uint16_t *dst;
-    uint64_t rows, codes_stride, scales_stride, chunk;  // elements from chunk to chunk
-    uint32_t cols, chunks;
+    uint64_t rows, stride, scales_stride, chunk, part;  // elements from chunk to chunk, and from part to part
+    uint32_t cols, chunks, kind, blocks;                // blocks: its workgroups
+};
+struct LayArgs {
+    LayArray of[3];
+    uint32_t arrays, pad;
 };
 
 // part[share][column] = the sums of the share's rows.

@@ -243,20 +243,117 @@ void unpack_rows(int ordinal, void *stream, const hbr_packed &p, const uint8_t *
 
 namespace {
 
-// A product's f32 parts, where its steps are shared out: rows of n columns, for
-// any number of rows up to m.
-uint64_t part_rows(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
-    const uint64_t most = tiles(k, kHeadK) * segments / 16;
-    return most > 1 ? std::min(65536 / tiles(n, kTile256.tile), m * most) : 0;
+// A projection's tiles: four waves, a workgroup a CU or two, 64 products a step.
+constexpr HeadTiling kLarge{256, 256, 256, "_256"}, kSmall{128, 256, 512, "_128"};
+constexpr uint64_t kStepK = 64;
+
+// A product's tiles (m: columns, n: rows of the result) and the shares of its steps.
+struct Product {
+    const HeadTiling *t;
+    uint64_t m_tiles, n_tiles, splits;
+    uint64_t groups() const { return m_tiles * n_tiles * splits; }
+    // Tiles that do not fill the device have a CU each, and its LDS for more
+    // steps in flight.
+    std::string name() const { return std::string(t->name) + (t == &kSmall && groups() <= 256 ? "_deep" : ""); }
+};
+constexpr uint64_t kLeastSteps = 2;  // of a share
+
+uint64_t steps_of(uint64_t k, uint64_t segments) { return tiles(k, kStepK) * segments; }
+
+Product product_plan(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t steps = steps_of(k, segments);
+    Product best{};
+    double least = 0.0;
+    for (const HeadTiling *t : {&kLarge, &kSmall}) {
+        const uint64_t mt = tiles(m, t->tile), nt = tiles(n, t->tile), all = mt * nt;
+        const uint64_t most = std::max<uint64_t>(1, std::min(t->slots / std::max<uint64_t>(all, 1), steps / kLeastSteps));
+        for (uint64_t s = 1; s <= most; s++) {
+            const uint64_t groups = all * s, each = tiles(steps, s);
+            const double step = t == &kLarge ? 1.4 : groups <= 256 ? 0.5 : 0.9, more = t == &kLarge ? 9.0 : 4.0;
+            const double cost = (double)tiles(groups, t->slots) * ((double)each * step + more) +
+                                (s > 1 ? 4.0 + (double)(groups * t->tile * t->tile) * 4.0 / 4.5e6 : 0.0);
+            if (!best.t || cost < least) best = {t, mt, nt, s}, least = cost;
+        }
+    }
+    return best;
 }
 
-// Tiles that do not fill the device have a CU each, and its LDS for more steps
-// in flight.
-std::string tile_name(const HeadTiling &t, uint64_t groups) {
-    return std::string(t.name) + (t.tile == 128 && groups <= 256 ? "_deep" : "");
+// The f32 sums of its shares, for any number of rows up to those given: no more
+// tiles than run at once, nor than shares of the least steps make.
+uint64_t part_cells(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t most = steps_of(k, segments) / kLeastSteps;
+    uint64_t cells = 0;
+    if (most > 1)
+        for (const HeadTiling *t : {&kLarge, &kSmall})
+            cells = std::max(cells, std::min(t->slots, most * tiles(m, t->tile) * tiles(n, t->tile)) * t->tile * t->tile);
+    return cells;
+}
+uint64_t part_used(const Product &p) { return p.splits > 1 ? p.groups() * p.t->tile * p.t->tile : 0; }
+
+// Chunks of 64 columns: twice the head's.
+uint64_t chunk_step(uint64_t rows) { return chunk_bytes(2 * rows); }
+uint64_t laid_bytes(uint64_t rows, uint64_t cols, uint64_t parts) { return parts * tiles(cols, kStepK) * chunk_step(rows); }
+
+// A call's operands: in place, or laid out, all of them in one launch.
+struct Operands {
+    uint32_t dtype;
+    LayArgs args{};
+    explicit Operands(uint32_t type) : dtype(type) {}
+    Laid add(const Rows &r, void *to) {
+        if (head_in_place(r.p, r.n > 1 ? r.stride : up(r.width, 8), r.width, dtype))
+            return {static_cast<const char *>(r.p), r.stride * 2, kStepK * 2, 0, (uint32_t)r.width};
+        return lay(r, nullptr, dtype == HBR_F32 ? kLayF32 : kLayBf16, to);
+    }
+    Laid add(const Rows &codes, const Rows &scales, void *to) { return lay(codes, &scales, kLayCodes, to); }
+    void launch(Queue &queue) const {
+        uint32_t blocks = 0;
+        for (uint32_t i = 0; i < args.arrays; i++) blocks += args.of[i].blocks;
+        if (blocks) queue.launch("hbr_lay", dim3(blocks), dim3(256), args);
+    }
+
+private:
+    Laid lay(const Rows &r, const Rows *scales, uint32_t kind, void *to) {
+        LayArray &a = args.of[args.arrays++];
+        a.src = r.p;
+        a.dst = static_cast<uint16_t *>(to);
+        a.rows = r.n;
+        a.stride = r.stride;
+        if (scales) a.scales = static_cast<const uint8_t *>(scales->p), a.scales_stride = scales->stride;
+        a.chunk = chunk_step(r.n) / 2;
+        a.cols = (uint32_t)r.width;
+        a.chunks = (uint32_t)tiles(r.width, kStepK);
+        a.part = a.chunks * a.chunk;
+        a.kind = kind;
+        a.blocks = (uint32_t)std::min<uint64_t>(tiles(r.n * a.chunks * 8, 256), 1u << 16);
+        return {static_cast<const char *>(to), kStepK * 2, a.chunk * 2, kind == kLayF32 ? a.part * 2 : 0, a.chunks * (uint32_t)kStepK};
+    }
+};
+
+// The parts' products of two f32 operands, or of one whose rows are in 8 bits.
+void set_segments(HeadArgs &a, uint64_t segments) {
+    a.segments = (uint32_t)segments;
+    if (segments == 6) a.a_order = kPartA, a.b_order = kPartB;
+    if (segments == 3) a.b_order = kPartsByOne;
 }
 
-uint64_t laid_bytes(uint64_t rows, uint64_t cols, uint64_t parts) { return parts * tiles(cols, 32) * chunk_bytes(rows); }
+void set_product(LinearArgs &a, const Product &p, float *part) {
+    a.p.m_tiles = (uint32_t)p.m_tiles;
+    a.p.n_tiles = (uint32_t)p.n_tiles;
+    a.p.splits = (uint32_t)p.splits;
+    a.part = p.splits > 1 ? part : nullptr;
+}
+
+// A product's launch, and its shares' join.
+void run_product(Queue &queue, const char *name, uint32_t dtype, const Product &p, const LinearArgs &a) {
+    // (a workgroup of the large tiles takes several)
+    const uint64_t groups = p.t == &kLarge ? std::min(p.groups(), kLarge.slots) : p.groups();
+    queue.launch((name + p.name()).c_str(), dim3((uint32_t)groups), dim3((uint32_t)p.t->threads), a);
+    if (p.splits == 1) return;
+    // a workgroup takes four columns of every thread's rows
+    const uint64_t cells = p.t->tile * p.t->tile / p.t->threads / 4;
+    queue.launch((std::string("hbr_linear_join_") + name_of(dtype) + p.t->name).c_str(), dim3((uint32_t)(p.m_tiles * p.n_tiles * cells)),
+                 dim3((uint32_t)p.t->threads), a);
+}
 
 void check_product(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, const char *what) {
     size_of(dtype, what);
@@ -270,26 +367,39 @@ void check_tiles(uint64_t m, uint64_t n, const char *what) {
     if (tiles(m, 128) * tiles(n, 128) >= 1u << 22) fail(kRefused, std::string(what) + ": 2^22 tiles of 128 x 128 or more");
 }
 
-// Rows up to which w is read straight into the matrix instructions' registers.
-constexpr uint64_t kFewRows = 64;
+// Whether w is read straight into the matrix instructions' registers: up to 64
+// rows, which are read again with every 16 outputs. In f32 always (32 rows,
+// 4,096 x 4,096: 30 us, 71 in tiles of three parts); in bf16 while those reads
+// take less than the tiles' stages and shares (64 rows: 1,024 x 4,096 10.2 us,
+// 12.9 in tiles, 4,096 x 8,192 39.5 and 20.5; 32 rows 25.6 and 20.5).
+bool few_rows(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype) {
+    return n <= 64 && (dtype == HBR_F32 || n <= 16 || tiles(n, 16) * outs * dim * 2 <= 48u << 20);
+}
 
 struct LinearPlan {
     char *x, *w;
     float *low, *part;
-    const HeadTiling *tiling;
-    uint64_t parts, segments, splits, bytes;
+    uint16_t *slot_of;
+    int32_t *slot_id;
+    uint32_t *slots;
+    Product product;
+    uint64_t segments, bytes;
 };
 LinearPlan linear_plan(uint64_t n, uint64_t outs, uint64_t dim, uint64_t rank, uint32_t dtype, void *workspace) {
     LinearPlan q{};
-    q.parts = dtype == HBR_F32 ? 3 : 1;
+    const uint64_t parts = dtype == HBR_F32 ? 3 : 1;
     q.segments = dtype == HBR_F32 ? 6 : 1;
-    q.tiling = &head_tiling(n, outs, dim, q.segments);
-    q.splits = head_splits(*q.tiling, n, outs, dim, q.segments);
+    q.product = product_plan(outs, n, dim, q.segments);
     Arena w(workspace);
-    q.x = w.take<char>(laid_bytes(n, dim, q.parts));
-    q.w = w.take<char>(laid_bytes(outs, dim, q.parts));
+    q.x = w.take<char>(laid_bytes(n, dim, parts));
+    q.w = w.take<char>(laid_bytes(outs, dim, parts));
     q.low = w.take<float>(n * rank);
-    q.part = w.take<float>(part_rows(n, outs, dim, q.segments) * outs, q.splits > 1 ? q.splits * n * outs : 0);
+    if (rank) {
+        q.slot_of = w.take<uint16_t>(n);
+        q.slot_id = w.take<int32_t>(up(n, kLarge.tile));
+        q.slots = w.take<uint32_t>(tiles(n, kSmall.tile));
+    }
+    q.part = w.take<float>(part_cells(outs, n, dim, q.segments), part_used(q.product));
     q.bytes = w.used;
     return q;
 }
@@ -318,7 +428,6 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         out(p.out, n, outs, p.out_stride, size, what),
         down(rank ? p.down : nullptr, p.n_adapters * rank, dim, p.down_stride, size, what),
         up_rows(rank ? p.up : nullptr, p.n_adapters * outs, rank, p.up_stride, size, what);
-    if (out.stride >= (1u << 21)) fail(kRefused, std::string(what) + ": results whose rows lie 2,097,152 elements or more apart");
     for (const void *f : {(const void *)p.bias, (const void *)p.ids, (const void *)p.scale}) check_aligned(f, 4, what);
     const LinearPlan q = linear_plan(n, outs, dim, rank, p.dtype, workspace);
     check_workspace(workspace, workspace_bytes, q.bytes, what);
@@ -332,6 +441,7 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         const uint32_t v = rows_vector(size, dim, all);
         return kernel_of(name, p.dtype, v == 16 / size ? v : 1);
     };
+    const bool few = few_rows(n, outs, dim, p.dtype);
     if (rank) {
         LinearLowArgs a{};
         a.x = p.x;
@@ -347,10 +457,17 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         a.adapters = p.n_adapters;
         // 16 rows a workgroup; of few of them several for the adapters' ranks
         const uint64_t groups = tiles(n, 16), most = tiles(std::min<uint64_t>(n, 16) * rank, 32);
-        queue.launch(strips("hbr_linear_low", {&x, &down}).c_str(), dim3((uint32_t)groups, (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups))),
-                     dim3(256), a);
+        const bool slots = !few && q.product.splits == 1;
+        a.groups = (uint32_t)groups;
+        a.tile = (uint32_t)q.product.t->tile;
+        a.slot_of = q.slot_of;
+        a.slot_id = q.slot_id;
+        a.slots = q.slots;
+        const std::string name = strips("hbr_linear_low", {&x, &down}) + (few ? "_16" : "");
+        queue.launch(name.c_str(), dim3((uint32_t)(groups + (slots ? q.product.n_tiles : 0)), (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups))),
+                     dim3(few ? 1024 : 256), a);
     }
-    if (n <= kFewRows) {
+    if (few) {
         LinearFewArgs a{};
         a.x = p.x;
         a.w = p.w;
@@ -373,42 +490,28 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         return;
     }
     LinearArgs a{};
-    set_a(a.p, lay_rows(queue, p.x, x.stride, n, dim, p.dtype, q.x, false, nullptr));
-    set_b(a.p, lay_rows(queue, p.w, w.stride, outs, dim, p.dtype, q.w, false, nullptr));
-    a.p.m = a.p.rows = (uint32_t)n;
-    a.p.n = p.n_outs;
+    Operands operands(p.dtype);
+    set_a(a.p, operands.add(w, q.w));
+    set_b(a.p, operands.add(x, q.x));
+    operands.launch(queue);
+    a.p.m = a.cols = p.n_outs;
+    a.p.n = a.rows = (uint32_t)n;
     a.p.k = p.dim;
-    a.p.check = dim % kHeadK != 0;
-    a.p.segments = (uint32_t)q.segments;
-    if (q.segments > 1) a.p.a_order = kPartA, a.p.b_order = kPartB;
-    a.p.splits = (uint32_t)q.splits;
-    a.p.bias = p.bias;
-    a.p.m_tiles = (uint32_t)tiles(n, q.tiling->tile);
-    a.p.n_tiles = (uint32_t)tiles(outs, q.tiling->tile);
-    const bool shared = q.splits > 1;
-    a.p.c = shared ? (void *)q.part : p.out;
-    a.p.c_stride = shared ? outs : out.stride;
-    a.p.c_split = n * outs;
+    set_segments(a.p, q.segments);
+    set_product(a, q.product, q.part);
+    a.out = p.out;
+    a.out_stride = out.stride;
+    a.bias = p.bias;
     a.low = rank ? q.low : nullptr;
     a.up = p.up;
     a.ids = p.ids;
+    a.slot_of = q.slot_of;
+    a.slot_id = q.slot_id;
+    a.slots = q.slots;
     a.up_stride = up_rows.stride;
     a.rank = p.rank;
     a.adapters = p.n_adapters;
-    const uint32_t groups = a.p.m_tiles * a.p.n_tiles * a.p.splits;
-    queue.launch(("hbr_linear_y_" + std::string(shared ? "part_" : "") + type + tile_name(*q.tiling, groups)).c_str(),
-                 dim3(groups), dim3((uint32_t)q.tiling->threads), a);
-    if (!shared) return;
-    LinearJoinArgs j{};
-    j.part = q.part;
-    j.bias = p.bias;
-    j.dst = p.out;
-    j.rows = n;
-    j.cols = outs;
-    j.dst_stride = out.stride;
-    j.part_stride = n * outs;
-    j.parts = a.p.splits;
-    queue.launch(("hbr_linear_join_" + type).c_str(), cells_grid(n * outs), dim3(256), j);
+    run_product(queue, ("hbr_linear_y_" + (a.part ? "part" : type)).c_str(), p.dtype, q.product, a);
 }
 
 namespace {
@@ -419,28 +522,28 @@ uint64_t column_shares(uint64_t outs) { return std::max<uint64_t>(1, 2048 / tile
 struct LinearGradPlan {
     char *dout, *w, *x;
     float *part_x, *part_w, *part_b;
-    uint64_t parts, bytes;
-    uint64_t segments_x, segments_w, splits_x, splits_w;
-    const HeadTiling *by_x, *by_w;
+    uint64_t segments_x, segments_w, bytes;
+    Product by_x, by_w;
 };
 // held: the rows are in 8 bits, one part whatever the type
 LinearGradPlan linear_grad_plan(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, bool held, void *workspace) {
     LinearGradPlan q{};
-    q.parts = dtype == HBR_F32 ? 3 : 1;
-    q.segments_x = dtype == HBR_F32 ? 6 : 1;
-    q.segments_w = dtype == HBR_F32 ? held ? 3 : 6 : 1;
-    q.by_x = &head_tiling(n, dim, outs, q.segments_x);
-    q.by_w = &head_tiling(outs, dim, n, q.segments_w);
-    q.splits_x = head_splits(*q.by_x, n, dim, outs, q.segments_x);
-    q.splits_w = head_splits(*q.by_w, outs, dim, n, q.segments_w);
+    const uint64_t parts = dtype == HBR_F32 ? 3 : 1, segments = dtype == HBR_F32 ? 6 : 1;
+    q.segments_x = segments;
+    q.segments_w = dtype == HBR_F32 && held ? 3 : segments;
+    q.by_x = product_plan(dim, n, outs, q.segments_x);
+    q.by_w = product_plan(dim, outs, n, q.segments_w);
     Arena w(workspace);
-    q.dout = w.take<char>(laid_bytes(n, outs, q.parts));
-    q.w = w.take<char>(laid_bytes(outs, dim, q.parts));
-    q.x = w.take<char>(laid_bytes(n, dim, q.parts));
-    // (of dw whatever the tiles: a share is 16 steps at least)
-    q.part_x = w.take<float>(part_rows(n, dim, outs, q.segments_x) * dim, q.splits_x > 1 ? q.splits_x * n * dim : 0);
-    q.part_w = w.take<float>(part_rows(outs, dim, n, q.parts == 3 ? 6 : 1) * dim, q.splits_w > 1 ? q.splits_w * outs * dim : 0);
-    q.part_b = w.take<float>(column_shares(outs) * outs);
+    q.dout = w.take<char>(laid_bytes(n, outs, parts));
+    q.w = w.take<char>(laid_bytes(outs, dim, parts));
+    q.x = w.take<char>(laid_bytes(n, dim, parts));
+    q.part_x = w.take<float>(part_cells(dim, n, outs, segments), part_used(q.by_x));
+    q.part_w = w.take<float>(part_cells(dim, outs, n, segments), part_used(q.by_w));
+    // db: sums of the rows' shares, or of the products' shares and tiles of columns
+    // (those that run at once, by a tile's rows; or every tile's)
+    q.part_b = w.take<float>(std::max({column_shares(outs) * outs, (uint64_t)65536, tiles(dim, kSmall.tile) * outs}),
+                             std::max(column_shares(outs), q.by_w.splits * q.by_w.m_tiles) * outs);
+    static_assert(kLarge.slots * 256 == 65536 && kSmall.slots * 128 == 65536, "rows of the tiles that run at once");
     q.bytes = w.used;
     return q;
 }
@@ -469,8 +572,6 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
         x(p.x, n, dim, p.x_stride, size, what), codes(p.codes, n, dim, p.codes_stride, 1, what),
         scales(p.scales, n, scales_of(dim), p.scales_stride, 1, what), dx(p.dx, n, dim, p.dx_stride, size, what),
         dw(p.dw, outs, dim, p.dw_stride, size, what);
-    if ((p.dx && dx.stride >= (1u << 21)) || (p.dw && dw.stride >= (1u << 21)))
-        fail(kRefused, std::string(what) + ": gradients whose rows lie 2,097,152 elements or more apart");
     check_aligned(p.weight, 4, what);
     check_aligned(p.db, 4, what);
     const bool held = p.codes != nullptr;
@@ -482,24 +583,13 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
     if (!p.dw && !p.db && (!p.dx || n == 0)) return;
     Queue queue(ordinal, stream);
     const std::string type = name_of(p.dtype);
-    auto join = [&](const float *part, uint64_t parts, const float *weight, const Rows &to) {
-        LinearJoinArgs j{};
-        j.part = part;
-        j.weight = weight;
-        j.dst = const_cast<void *>(to.p);
-        j.rows = to.n;
-        j.cols = dim;
-        j.dst_stride = to.stride;
-        j.part_stride = to.n * dim;
-        j.parts = (uint32_t)parts;
-        queue.launch(("hbr_linear_join_" + type).c_str(), cells_grid(to.n * dim), dim3(256), j);
-    };
     if (n == 0) {  // sums over no rows
-        if (p.dw) join(nullptr, 0, nullptr, dw);
+        if (p.dw) sum_parts(queue, p.dtype, 1.0f, nullptr, 0, 0, p.dw, outs, dim, dw.stride);
         if (p.db) sum_parts(queue, HBR_F32, 1.0f, nullptr, 0, 0, p.db, 1, outs, outs);
         return;
     }
-    if (p.db) {
+    uint64_t sums = 0;  // of db
+    if (p.db && !p.dw) {
         ColumnSumArgs a{};
         a.x = p.dout;
         a.part = q.part_b;
@@ -507,65 +597,50 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
         a.x_stride = dout.stride;
         a.cols = p.n_outs;
         a.shares = (uint32_t)std::min(column_shares(outs), tiles(n, 32));
+        sums = a.shares;
         queue.launch(("hbr_column_sum_" + type).c_str(), dim3((uint32_t)tiles(outs, 256) * a.shares), dim3(256), a);
-        sum_parts(queue, HBR_F32, 1.0f, q.part_b, a.shares, outs, p.db, 1, outs, outs);
     }
-    if (!p.dx && !p.dw) return;
-    const Laid by = lay_rows(queue, p.dout, dout.stride, n, outs, p.dtype, q.dout, false, nullptr);
-    auto product = [&](const char *name, const HeadTiling &t, LinearArgs &a, float *part, const Rows &to) {
-        a.p.n = p.dim;
-        a.p.rows = (uint32_t)to.n;
-        a.p.m_tiles = (uint32_t)tiles(to.n, t.tile);
-        a.p.n_tiles = (uint32_t)tiles(dim, t.tile);
-        const bool shared = a.p.splits > 1;
-        a.p.c = shared ? (void *)part : const_cast<void *>(to.p);
-        a.p.c_stride = shared ? dim : to.stride;
-        a.p.c_split = to.n * dim;
-        const uint32_t groups = a.p.m_tiles * a.p.n_tiles * a.p.splits;
-        queue.launch((std::string(name) + (shared ? "part" : type) + tile_name(t, groups)).c_str(), dim3(groups),
-                     dim3((uint32_t)t.threads), a);
-        if (shared) join(part, a.p.splits, a.p.weight, to);
-    };
-    if (p.dx) {
-        LinearArgs a{};
-        set_a(a.p, by);
-        set_b(a.p, lay_rows(queue, p.w, w.stride, outs, dim, p.dtype, q.w, false, nullptr));
-        a.p.m = (uint32_t)n;
-        a.p.k = p.n_outs;
-        a.p.check = outs % kHeadK != 0;
-        a.p.segments = (uint32_t)q.segments_x;
-        if (q.segments_x > 1) a.p.a_order = kPartA, a.p.b_order = kPartB;
-        a.p.splits = (uint32_t)q.splits_x;
-        product("hbr_linear_dx_", *q.by_x, a, q.part_x, dx);
-    }
-    if (p.dw) {
-        LinearArgs a{};
-        set_a(a.p, by);
-        if (held) {
-            LayCodesArgs l{};
-            l.codes = p.codes;
-            l.scales = p.scales;
-            l.dst = reinterpret_cast<uint16_t *>(q.x);
-            l.rows = n;
-            l.codes_stride = codes.stride;
-            l.scales_stride = scales.stride;
-            l.chunk = chunk_bytes(n) / 2;
-            l.cols = p.dim;
-            l.chunks = (uint32_t)tiles(dim, 32);
-            queue.launch("hbr_lay_codes", cells_grid(n * l.chunks * 4), dim3(256), l);
-            set_b(a.p, {q.x, 64, l.chunk * 2, 0, l.chunks * 32});
-        } else {
-            set_b(a.p, lay_rows(queue, p.x, x.stride, n, dim, p.dtype, q.x, false, nullptr));
+    if (p.dx || p.dw) {
+        LinearArgs x_args{}, w_args{};
+        Operands operands(p.dtype);
+        const Laid by = operands.add(dout, q.dout);
+        if (p.dx) set_a(x_args.p, operands.add(w, q.w));
+        if (p.dw) set_a(w_args.p, held ? operands.add(codes, scales, q.x) : operands.add(x, q.x));
+        operands.launch(queue);
+        // (a transposed operand's columns are read in eights: in place there are
+        // whole ones, laid out zeros stand behind them)
+        if (p.dx) {
+            LinearArgs &a = x_args;
+            set_b(a.p, by);
+            a.p.m = (uint32_t)up(dim, 8);
+            a.p.n = a.rows = (uint32_t)n;
+            a.cols = p.dim;
+            a.p.k = p.n_outs;
+            set_segments(a.p, q.segments_x);
+            set_product(a, q.by_x, q.part_x);
+            a.out = p.dx;
+            a.out_stride = dx.stride;
+            run_product(queue, ("hbr_linear_dx_" + type).c_str(), p.dtype, q.by_x, a);
         }
-        a.p.m = by.row == 64 && by.p == q.dout ? (uint32_t)up(outs, 32) : p.n_outs;  // (to the end of a laid chunk)
-        a.p.k = (uint32_t)n;
-        a.p.segments = (uint32_t)q.segments_w;
-        if (q.segments_w == 6) a.p.a_order = kPartA, a.p.b_order = kPartB;
-        else if (q.segments_w == 3) a.p.a_order = kPartsByOne;
-        a.p.splits = (uint32_t)q.splits_w;
-        a.p.weight = p.weight;
-        product("hbr_linear_dw_", *q.by_w, a, q.part_w, dw);
+        if (p.dw) {
+            LinearArgs &a = w_args;
+            set_b(a.p, by);
+            a.p.m = (uint32_t)up(dim, 8);
+            a.p.n = (uint32_t)up(outs, 8);
+            a.cols = p.dim;
+            a.rows = p.n_outs;
+            a.p.k = (uint32_t)n;
+            set_segments(a.p, q.segments_w);
+            set_product(a, q.by_w, q.part_w);
+            a.out = p.dw;
+            a.out_stride = dw.stride;
+            a.weight = p.weight;
+            a.part_b = p.db ? q.part_b : nullptr;
+            if (p.db) sums = q.by_w.splits * q.by_w.m_tiles;
+            run_product(queue, ("hbr_linear_dw_" + type).c_str(), p.dtype, q.by_w, a);
+        }
     }
+    if (p.db) sum_parts(queue, HBR_F32, 1.0f, q.part_b, sums, outs, p.db, 1, outs, outs);
 }
 
 }  // namespace hbr

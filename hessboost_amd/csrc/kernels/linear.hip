@@ -3,125 +3,206 @@
 //   out = x w^T + bias + scale[a] (x down[a]^T) up[a]^T, a = ids[row]
 //   dx = dout w; dw = (dout^T x) weight; db = sum over rows dout
 //
-// The products are product.h's tiles. An f32 operand is three bf16 parts; rows in
+// The products are tile_product.h's. An f32 operand is three bf16 parts; rows in
 // 8 bits are one (a code times its power is a bf16), so that f32 gradients of
 // theirs take three products and not six.
 #include <type_traits>
 
-#include "product.h"
+#include "tile_product.h"
 #include "rows8.h"
 
 namespace hbr {
 
-// A tile's cells: E what c holds, f32 parts of the sums as they are, or the
-// result: times the column's factor, and its bias added.
-template <typename Tile, typename E, bool Part>
-__device__ __forceinline__ void linear_store(const HeadArgs &a, Tile &t) {
-    using T = typename E::type;
-    const uint32_t lane = lane_id();
-    const uint64_t from = reinterpret_cast<uint64_t>(static_cast<T *>(a.c) + t.split * a.c_split + t.m0 * a.c_stride + t.n0);
-    const uint32_t stride = (uint32_t)a.c_stride * sizeof(T);
-    const uint32_t rows = min(a.rows > t.m0 ? a.rows - t.m0 : 0u, (uint32_t)Tile::kM);
-    const uint32_t size = rows ? (rows - 1) * stride + min(a.n - t.n0, (uint32_t)Tile::kN) * (uint32_t)sizeof(T) : 0u;
-    // a buffer that ends with the tile's last cell
-    __amdgpu_buffer_rsrc_t c = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(from), 0, size, 0x00020000);
-#pragma unroll
-    for (int j = 0; j < Tile::kJ; j++) {
-        const uint32_t n = t.wave_n + 32 * j + lane % 32;
-        const bool in = t.n0 + n < a.n;
-        const uint32_t at = in ? (t.wave_m + lane / 32 * 4) * stride + n * (uint32_t)sizeof(T) : kNowhere;
-        const float by = !Part && in && a.weight ? a.weight[t.n0 + n] : 1.0f;
-        const float bias = !Part && in && a.bias ? a.bias[t.n0 + n] : 0.0f;
+// A lane's four columns of a row: cells e = 4 g to 4 g + 3 of acc[i][j].
+template <typename Tile>
+__device__ __forceinline__ uint32_t column_of(const Tile &t, int i, int g) { return t.m0 + t.wave_m + 32 * i + 8 * g + 4 * (lane_id() / 32); }
+
+// What a lane's columns are multiplied by (a weight) or have added (a bias), read
+// before the products and waited for behind them. Null: nothing.
+template <typename Tile>
+struct Columns {
+    float v[Tile::kI][4][4];
+    __device__ __forceinline__ void read(const Tile &t, const float *p, uint32_t cols, float otherwise) {
 #pragma unroll
         for (int i = 0; i < Tile::kI; i++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const uint32_t to = at + (32 * i + 8 * (e / 4) + e % 4) * stride;
-                const float v = Part ? t.acc[i][j][e] : __builtin_fmaf(t.acc[i][j][e], by, bias);
-                if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), c, to, 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b16(to_bf16(v), c, to, 0, 0);
-            }
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[i][g][k] = p ? p[min(column_of(t, i, g) + k, cols - 1)] : otherwise;
     }
+};
+struct NoColumns {};
+
+// The sums stay in the accumulators' registers until they are used.
+template <typename Tile>
+__device__ __forceinline__ void hold(Tile &t) {
+#pragma unroll
+    for (int i = 0; i < Tile::kI; i++)
+#pragma unroll
+        for (int j = 0; j < Tile::kJ; j++) {
+            if constexpr (Tile::kI == 4) asm volatile("" : "+a"(t.acc[i][j]));
+        }
+}
+
+// The tile's result, through LDS to stores of 16 bytes: 64 of a wave's rows by
+// 128 bytes of columns at a time, in its own 8 KiB. A row's pieces of 16 bytes are
+// exchanged by the row's bits, so that rows meet different banks.
+template <typename Tile, typename E, bool Weighted, typename More>
+__device__ __forceinline__ void linear_store(const LinearArgs &a, char *room, Tile &t, const More &more) {
+    using T = typename E::type;
+    constexpr int kSize = sizeof(T), kBlocks = 4 / kSize, kV = 16 / kSize;  // blocks of 32 columns at a time; columns a piece
+    static_assert(Tile::kI % kBlocks == 0 && Tile::kJ % 2 == 0, "whole blocks");
+    const uint32_t lane = lane_id();
+    const uint32_t own = (uint32_t)(uintptr_t)(HBR_LDS char *)room + uniform(threadIdx.x / kWave) * 8192;
+    // a lane's cells of a row lie at one piece, exchanged by constants
+    uint32_t in = own + lane % 32 * 128 + (kSize == 4 ? (lane % 8 ^ lane / 32) * 16 : lane % 8 * 16 + lane / 32 * 8);
+    uint32_t back = own + lane / 8 * 128 + (lane % 8 ^ lane / 8) * 16;
+    asm volatile("" : "+v"(in), "+v"(back));  // (no address of theirs is kept from tile to tile)
+    const bool whole = a.out_stride % kV == 0 && reinterpret_cast<uint64_t>(a.out) % 16 == 0 && t.m0 + Tile::kM <= a.cols;
+#pragma unroll
+    for (int i0 = 0; i0 < Tile::kI; i0 += kBlocks)
+#pragma unroll
+        for (int j0 = 0; j0 < Tile::kJ; j0 += 2) {
+            hold(t);
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        Vec<T, 4> v;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            float x = t.acc[i0 + b][j0 + j][4 * g + k];
+                            if constexpr (!std::is_same_v<More, NoColumns>) {
+                                if constexpr (Weighted) x *= more.v[i0 + b][g][k];
+                                else x += more.v[i0 + b][g][k];
+                            }
+                            if constexpr (kSize == 4) v.v[k] = x;
+                            else v.v[k] = to_bf16(x);
+                        }
+                        *(HBR_LDS Vec<T, 4> *)((in ^ (uint32_t)(kSize == 4 ? 2 * g : 4 * b + g) * 16) + 4096 * j) = v;
+                    }
+            const uint32_t r = t.n0 + t.wave_n + 32 * j0 + lane / 8, c = t.m0 + t.wave_m + 32 * i0 + lane % 8 * kV;
+            T *to = static_cast<T *>(a.out) + (uint64_t)r * a.out_stride + c;
+            auto piece = [&](int q) { return *(HBR_LDS const Vec<T, kV> *)(back + q * 1024); };
+            if (whole) {
+#pragma unroll
+                for (int q = 0; q < 8; q++, to += 8 * a.out_stride)
+                    if (r + 8 * q < a.rows) *reinterpret_cast<Vec<T, kV> *>(to) = piece(q);
+            } else {
+                for (int q = 0; q < 8; q++, to += 8 * a.out_stride) {
+                    const Vec<T, kV> v = piece(q);
+#pragma unroll
+                    for (int k = 0; k < kV; k++)
+                        if (r + 8 * q < a.rows && c + k < a.cols) to[k] = v.v[k];
+                }
+            }
+            asm volatile("" ::: "memory");  // the pieces are read before the next ones are written
+        }
+}
+
+// Where a tile's sums lie among the parts, in fours.
+template <typename Tile>
+__device__ __forceinline__ uint64_t part_at(const HeadArgs &p, uint64_t tile, uint32_t cell) {
+    return (tile * (Tile::kI * Tile::kJ * 4) + cell) * Tile::kThreads + threadIdx.x;
+}
+
+template <typename Tile>
+__device__ __forceinline__ void linear_store_part(const LinearArgs &a, Tile &t) {
+    const uint64_t tile = ((uint64_t)t.split * a.p.m_tiles + t.m0 / Tile::kM) * a.p.n_tiles + t.n0 / Tile::kN;
+#pragma unroll
+    for (int i = 0; i < Tile::kI; i++)
+#pragma unroll
+        for (int j = 0; j < Tile::kJ; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                Vec<float, 4> v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) v.v[k] = t.acc[i][j][4 * g + k];
+                reinterpret_cast<Vec<float, 4> *>(a.part)[part_at<Tile>(a.p, tile, (i * Tile::kJ + j) * 4 + g)] = v;
+            }
 }
 
 // The tile's adapters: more products, over the pairs (adapter of the tile, rank)
 // one behind the other. A row's low values stand at its own adapter's places and
 // zeros at the others', so that any order of the rows is right, and rows of few
-// adapters take few steps: an adapter's rows next to each other are one slot,
-// and in tiles of many slots the same adapter's are joined.
+// adapters take few steps.
 //
 // In bf16 the low values are rounded once to bf16, as any product's operand
 // is: half a step each of the adapters' part. In f32 all is in three parts.
-// id: the adapter of the thread's row of the tile, before: of the row before it
-// (none: below 0).
 template <typename Tile, typename E>
-__device__ __forceinline__ void linear_adapters(const LinearArgs &a, char *lds, Tile &t, int32_t id, int32_t before_id) {
+struct Adapters {
     using T = typename E::type;
-    constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kPairs = kParts == 3 ? 6 : 1;
-    constexpr uint32_t kM = Tile::kM, kNone = 0xffffu, kWaves = Tile::kThreads / kWave;
-    // A step is 32 products, in f32 16 of all three parts; its operands lie in
-    // front of the slots.
-    constexpr uint32_t kStep = kParts == 1 ? 32 : 16, kRow = kStep * 2, kPart = kM * kRow;
-    int32_t *slot_id = reinterpret_cast<int32_t *>(lds + 2 * kParts * kPart);    // [kM] a slot's adapter
-    uint16_t *slot_of = reinterpret_cast<uint16_t *>(slot_id + kM);              // [kM] a row's slot
-    uint16_t *joined = slot_of + kM;                                             // [kM] a slot's place among the joined
-    uint32_t *counts = reinterpret_cast<uint32_t *>(joined + kM);                // [kWaves]
-    static_assert(2 * kParts * kPart + kM * 8 + kWaves * 4 <= (uint32_t)Tile::kLds && kM <= (uint32_t)Tile::kThreads, "all fits the stages");
-    const uint32_t m = threadIdx.x, lane = lane_id(), wave = threadIdx.x / kWave;
-    const bool starts = id >= 0 && (m == 0 || before_id != id);
-    const uint64_t start = __ballot(starts);
-    if (lane == 0) counts[wave] = (uint32_t)__popcll(start);
-    __syncthreads();
-    uint32_t slots = 0, before = 0;
-    for (uint32_t w = 0; w < kWaves; w++) {
-        before += w < wave ? counts[w] : 0;
-        slots += counts[w];
-    }
-    const uint32_t slot = before + (uint32_t)__popcll(start & (~0ull >> (63 - lane))) - 1;  // of the last start up to here
-    if (m < kM) slot_of[m] = (uint16_t)(id >= 0 ? slot : kNone);
-    if (starts) slot_id[slot] = id;
-    __syncthreads();
-    slots = (uint32_t)uniform(slots);
-    if (slots > 8) {
-        // the first slot of the same adapter, and its place among the first ones
-        uint32_t first = kNone, place = 0;
-        int32_t mine = 0;
-        if (m < slots) {
-            mine = slot_id[m];
-            first = 0;
-            while (slot_id[first] != mine) first++;
-        }
-        const bool is = first == m;
-        const uint64_t some = __ballot(is);
-        __syncthreads();
-        if (lane == 0) counts[wave] = (uint32_t)__popcll(some);
-        __syncthreads();
-        slots = 0;
-        for (uint32_t w = 0; w < kWaves; w++) {
-            place += w < wave ? counts[w] : 0;
-            slots += counts[w];
-        }
-        place += (uint32_t)__popcll(some & ((1ull << lane) - 1));
-        if (is) joined[m] = (uint16_t)place, slot_id[place] = mine;  // (place <= m, and every slot_id has been read)
-        __syncthreads();
-        if (first != kNone && !is) joined[m] = joined[first];
-        __syncthreads();
-        if (m < kM && slot_of[m] != kNone) slot_of[m] = joined[slot_of[m]];
-        __syncthreads();
-        slots = (uint32_t)uniform(slots);
-    }
-    const uint32_t all = slots * a.rank;
-    const bool eights = a.rank % 8 == 0;
-    const bool wide = eights && a.up_stride % 8 == 0 && reinterpret_cast<uint64_t>(a.up) % 16 == 0;
-    // pieces of eight products of a row: of the rows' low values, and of the
-    // outputs' second factors. Every load is made, from within its array, and
-    // what does not count is zeroed.
-    constexpr uint32_t kIn = kStep / 8;  // pieces of a row
-    constexpr int kPieces = kM * kIn / Tile::kThreads;
+    static constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kPairs = kParts == 3 ? 6 : 1;
+    // A step is 32 products, in f32 16 of all three parts
+    static constexpr uint32_t kM = Tile::kM, kStep = kParts == 1 ? 32 : 16, kRow = kStep * 2, kPart = kM * kRow, kIn = kStep / 8;
+    static constexpr int kPieces = kM * kIn / Tile::kThreads;  // of eight products of a row, of either operand
     static_assert(Tile::kM == Tile::kN && kM * kIn % Tile::kThreads == 0, "as many pieces of each a thread");
+    static_assert(4 * kParts * kPart <= (uint32_t)Tile::kLds, "two steps fit the stages");
+    uint32_t all, own[kPieces];
+    const int32_t *slot_id;
+    bool eights, wide;
+
+    __device__ __forceinline__ Adapters(const LinearArgs &a, const Tile &t) {
+        all = 0;
+        if (!a.low) return;
+        const uint32_t tile = t.n0 / Tile::kN;
+        all = uniform(a.slots[tile]) * a.rank;
+        slot_id = a.slot_id + (uint64_t)tile * Tile::kN;
+        eights = a.rank % 8 == 0;
+        wide = eights && a.up_stride % 8 == 0 && reinterpret_cast<uint64_t>(a.up) % 16 == 0;
+#pragma unroll
+        for (int q = 0; q < kPieces; q++) own[q] = a.slot_of[min(t.n0 + (q * Tile::kThreads + threadIdx.x) / kIn, a.rows - 1)];
+    }
+    // Every load is made, from within its array, and what does not count is zeroed.
+    __device__ __forceinline__ void read(const LinearArgs &a, const Tile &t, uint32_t k0, float (&low)[kPieces][8], Vec<T, 8> (&up)[kPieces]) {
+#pragma unroll
+        for (int q = 0; q < kPieces; q++) {
+            const uint32_t at = q * Tile::kThreads + threadIdx.x, row = at / kIn, k = k0 + at % kIn * 8;
+            const float *lows = a.low + (uint64_t)(min(t.n0 + row, a.rows - 1)) * a.rank;
+            const uint64_t out = min(t.m0 + row, a.cols - 1);
+            const T *ups = static_cast<const T *>(a.up);
+            const uint32_t kc = min(k, all - 1);
+            uint32_t s = kc / a.rank, rho = kc - s * a.rank;
+            if (eights) {  // (a piece is one slot's)
+                rho &= ~7u;
+                const Vec<float, 4> l0 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho),
+                                    l1 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho + 4);
+                const T *from = ups + ((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + rho;
+                if (wide) {
+                    up[q] = *reinterpret_cast<const Vec<T, 8> *>(from);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) up[q].v[j] = from[j];
+                }
+                const bool some = k < all, mine = some && s == own[q];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    low[q][j] = mine ? j < 4 ? l0.v[j % 4] : l1.v[j % 4] : 0.0f;
+                    up[q].v[j] = some ? up[q].v[j] : (T)0;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const bool some = k + j < all;
+                    const float l = lows[rho];
+                    const T u = ups[((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + rho];
+                    low[q][j] = some && s == own[q] ? l : 0.0f;
+                    up[q].v[j] = some ? u : (T)0;
+                    if (++rho == a.rank) {
+                        rho = 0;
+                        s += k + j + 1 < all;
+                    }
+                }
+            }
+        }
+    }
     // a piece's place: the rows that LDS serves at once meet different banks
-    auto place = [&](uint32_t row, uint32_t piece) { return row * kRow + (piece ^ ((row >> (kIn == 4 ? 2 : 3)) & (kIn - 1))) * 16; };
-    auto put = [&](uint32_t to, const float (&v)[8]) {
+    static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
+        return row * kRow + (piece ^ ((row >> (kIn == 4 ? 2 : 3)) & (kIn - 1))) * 16;
+    }
+    static __device__ __forceinline__ void put(char *to, const float (&v)[8]) {
         Vec<uint16_t, 8> out[kParts];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -135,119 +216,301 @@ __device__ __forceinline__ void linear_adapters(const LinearArgs &a, char *lds, 
             }
         }
 #pragma unroll
-        for (int q = 0; q < kParts; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(lds + q * kPart + to) = out[q];
-    };
-    for (uint32_t k0 = 0; k0 < all; k0 += kStep) {
-        float low[kPieces][8], up[kPieces][8];
-#pragma unroll
-        for (int q = 0; q < kPieces; q++) {
-            const uint32_t at = q * Tile::kThreads + threadIdx.x, row = at / kIn, k = k0 + at % kIn * 8;
-            const uint32_t own = slot_of[row];
-            const float *lows = a.low + (uint64_t)(min(t.m0 + row, a.p.m - 1)) * a.rank;
-            const uint64_t out = min(t.n0 + row, a.p.n - 1);
-            const T *ups = static_cast<const T *>(a.up);
-            const uint32_t kc = min(k, all - 1);
-            uint32_t s = kc / a.rank, rho = kc - s * a.rank;
-            if (eights) {  // (a piece is one slot's)
-                rho &= ~7u;
-                const Vec<float, 4> l0 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho),
-                                    l1 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho + 4);
-                const T *from = ups + ((uint64_t)slot_id[s] * a.p.n + out) * a.up_stride + rho;
-                Vec<T, 8> x;
-                if (wide) {
-                    x = *reinterpret_cast<const Vec<T, 8> *>(from);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x.v[j] = from[j];
-                }
-                const bool some = k < all, mine = some && s == own;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    low[q][j] = mine ? j < 4 ? l0.v[j % 4] : l1.v[j % 4] : 0.0f;
-                    up[q][j] = some ? E::up(x.v[j]) : 0.0f;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool some = k + j < all;
-                    const float l = lows[rho], u = E::up(ups[((uint64_t)slot_id[s] * a.p.n + out) * a.up_stride + rho]);
-                    low[q][j] = some && s == own ? l : 0.0f;
-                    up[q][j] = some ? u : 0.0f;
-                    if (++rho == a.rank) rho = 0, s = min(s + 1, slots - 1);
-                }
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < kPieces; q++) {
-            const uint32_t at = q * Tile::kThreads + threadIdx.x, to = place(at / kIn, at % kIn);
-            put(to, low[q]);
-            put(to + kParts * kPart, up[q]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t kk = 0; kk < kStep / 16; kk++) {
-            const uint32_t piece = kk * 2 + lane / 32;
-            auto fragment = [&](uint32_t part, uint32_t row) {
-                return *reinterpret_cast<const bf16x8 *>(lds + part * kPart + place(row + lane % 32, piece));
-            };
-#pragma unroll
-            for (int pair = 0; pair < kPairs; pair++) {
-                const uint32_t pa = kParts == 1 ? 0 : kPartA >> 2 * pair & 3u, pb = kParts == 1 ? 0 : kPartB >> 2 * pair & 3u;
-                bf16x8 fa[Tile::kI], fb[Tile::kJ];
-#pragma unroll
-                for (int i = 0; i < Tile::kI; i++) fa[i] = fragment(pa, t.wave_m + 32 * i);
-#pragma unroll
-                for (int j = 0; j < Tile::kJ; j++) fb[j] = fragment(kParts + pb, t.wave_n + 32 * j);
-#pragma unroll
-                for (int i = 0; i < Tile::kI; i++)
-#pragma unroll
-                    for (int j = 0; j < Tile::kJ; j++)
-                        t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
-                if (kPairs > 1) __builtin_amdgcn_sched_barrier(0);  // one pair's fragments at a time in registers
-            }
-        }
-        __syncthreads();
+        for (int q = 0; q < kParts; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(to + q * kPart) = out[q];
     }
-}
+    __device__ __forceinline__ void add(const LinearArgs &a, char *stages, Tile &t) {
+        const uint32_t lane = lane_id();
+        for (uint32_t k0 = 0, turn = 0; k0 < all; k0 += kStep, turn ^= 1) {
+            char *lds = stages + turn * 2 * kParts * kPart;
+            float low[kPieces][8];
+            Vec<T, 8> up[kPieces];
+            read(a, t, k0, low, up);
+#pragma unroll
+            for (int q = 0; q < kPieces; q++) {
+                const uint32_t at = q * Tile::kThreads + threadIdx.x;
+                char *to = lds + place(at / kIn, at % kIn);
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = E::up(up[q].v[j]);
+                put(to, v);
+                put(to + kParts * kPart, low[q]);
+            }
+            __syncthreads();  // (the step before the last has been read by all that come here)
+#pragma unroll
+            for (uint32_t kk = 0; kk < kStep / 16; kk++) {
+                const uint32_t piece = kk * 2 + lane / 32;
+                auto fragment = [&](uint32_t part, uint32_t row) {
+                    return *reinterpret_cast<const bf16x8 *>(lds + part * kPart + place(row + lane % 32, piece));
+                };
+#pragma unroll
+                for (int pair = 0; pair < kPairs; pair++) {
+                    const uint32_t pa = kParts == 1 ? 0 : kPartA >> 2 * pair & 3u, pb = kParts == 1 ? 0 : kPartB >> 2 * pair & 3u;
+                    bf16x8 fa[Tile::kI], fb[Tile::kJ];
+#pragma unroll
+                    for (int i = 0; i < Tile::kI; i++) fa[i] = fragment(pa, t.wave_m + 32 * i);
+#pragma unroll
+                    for (int j = 0; j < Tile::kJ; j++) fb[j] = fragment(kParts + pb, t.wave_n + 32 * j);
+#pragma unroll
+                    for (int i = 0; i < Tile::kI; i++)
+#pragma unroll
+                        for (int j = 0; j < Tile::kJ; j++)
+                            t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
+                    if (kPairs > 1) __builtin_amdgcn_sched_barrier(0);  // one pair's fragments at a time in registers
+                }
+            }
+        }
+        if (all) __syncthreads();
+    }
+};
 
-// E: the inputs' type; Part: f32 sums of a share of the steps
-template <typename Tile, typename E, bool Part>
-__device__ __forceinline__ void linear_y(const LinearArgs &a, char *lds) {
-    Tile t;
-    head_place(a.p, t);
-    const bool adapters = a.low && (!Part || t.split == 0);
-    // (loaded here, and waited for behind the products)
+// The adapters of a tile's rows, each once, in order of their first rows.
+__device__ __forceinline__ void tile_slots(const LinearLowArgs &a, uint32_t tile) {
+    __shared__ int32_t start_id[256];
+    __shared__ uint16_t start_slot[256];
+    __shared__ uint32_t counts[4];
+    const uint32_t m = threadIdx.x, lane = lane_id(), wave = m / kWave;
+    const uint64_t r0 = (uint64_t)tile * a.tile;
     auto adapter = [&](uint32_t in) {
-        const uint32_t row = t.m0 + in;
-        const int32_t id = adapters && in < Tile::kM && row < a.p.m ? a.ids[row] : -1;
+        const int32_t id = in < a.tile && r0 + in < a.n_rows ? a.ids[r0 + in] : -1;
         return id >= 0 && (uint32_t)id < a.adapters ? id : -1;
     };
-    const int32_t id = adapter(threadIdx.x), before = threadIdx.x ? adapter(threadIdx.x - 1) : -1;
-    head_product<false, false>(a.p, lds, t);
-    if (adapters) linear_adapters<Tile, E>(a, lds, t, id, before);
-    linear_store<Tile, std::conditional_t<Part, F32, E>, Part>(a.p, t);
-}
-
-// The gradients' products: of the inputs (AT false) and of the weights. E: what c holds.
-template <typename Tile, typename E, bool AT, bool Part>
-__device__ __forceinline__ void linear_d(const LinearArgs &a, char *lds) {
-    Tile t;
-    head_place(a.p, t);
-    head_product<AT, true>(a.p, lds, t);
-    linear_store<Tile, E, Part>(a.p, t);
-}
-
-template <typename E>
-__device__ __forceinline__ void linear_join(const LinearJoinArgs &a) {
-    const uint64_t cells = a.rows * a.cols;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = i / a.cols, c = i - r * a.cols;
-        float s = 0.0f;
-#pragma unroll 8
-        for (uint32_t p = 0; p < a.parts; p++) s += a.part[p * a.part_stride + i];
-        s = __builtin_fmaf(s, a.weight ? a.weight[c] : 1.0f, a.bias ? a.bias[c] : 0.0f);
-        static_cast<typename E::type *>(a.dst)[r * a.dst_stride + c] = E::down(s);
+    // a count over the threads up to this one
+    auto place = [&](bool is, uint32_t &all) {
+        const uint64_t some = __ballot(is);
+        __syncthreads();
+        if (lane == 0) counts[wave] = (uint32_t)__popcll(some);
+        __syncthreads();
+        uint32_t before = 0;
+        all = 0;
+        for (uint32_t w = 0; w < 4; w++) {
+            before += w < wave ? counts[w] : 0;
+            all += counts[w];
+        }
+        return before + (uint32_t)__popcll(some & (~0ull >> (63 - lane)));
+    };
+    // rows of one adapter next to each other are one start
+    const int32_t id = adapter(m), before = m ? adapter(m - 1) : -1;
+    const bool starts = id >= 0 && before != id;
+    uint32_t all, slots;
+    const uint32_t start = place(starts, all) - 1;
+    if (starts) start_id[start] = id;
+    __syncthreads();
+    // the first start of the same adapter
+    uint32_t first = kNoSlot;
+    if (m < all) {
+        first = 0;
+        while (start_id[first] != start_id[m]) first++;
     }
+    const uint32_t slot = place(first == m, slots) - 1;
+    if (first == m) start_slot[m] = (uint16_t)slot;
+    __syncthreads();
+    if (m < all && first != m) start_slot[m] = start_slot[first];
+    __syncthreads();
+    if (m < a.tile && r0 + m < a.n_rows) a.slot_of[r0 + m] = id >= 0 ? start_slot[start] : (uint16_t)kNoSlot;
+    if (first == m) a.slot_id[r0 + slot] = start_id[m];
+    if (m == 0) a.slots[tile] = slots;
+}
+
+// A workgroup's tiles, one after the other: the next one's first steps are loaded
+// while the last one's cells are written. `Work` has what is done before a tile's
+// products, beside them, behind them in the stages, and with its cells.
+template <bool AT, bool BT, typename Tile, typename Work>
+__device__ __forceinline__ void linear_tiles(const LinearArgs &a, char *lds) {
+    const uint32_t all = a.p.m_tiles * a.p.n_tiles * a.p.splits;
+    char *room = lds + Tile::kRoom;
+    TileProduct<AT, BT, Tile> product(a.p, lds);
+    Tile t;
+    const uint32_t wave = uniform(threadIdx.x / kWave);
+    t.wave_m = wave / Tile::kWavesN * Tile::kWaveM;
+    t.wave_n = wave % Tile::kWavesN * Tile::kWaveN;
+    Spot next = tile_spot<Tile>(a.p, blockIdx.x, all);
+    product.prime(next);
+    for (uint32_t index = blockIdx.x;;) {
+        static_cast<Spot &>(t) = next;
+        Work work(a, t);
+        product.run(t, work.beside());
+        hold(t);
+        work.behind(a, lds, t);
+        index += gridDim.x;
+        const bool more = Tile::kSeveral && index < all;
+        if (more) {
+            next = tile_spot<Tile>(a.p, index, all);
+            product.prime(next);
+        }
+        work.store(a, room, t);
+        if (!more) return;
+    }
+}
+
+template <typename Tile, typename E>
+struct LinearY {
+    Adapters<Tile, E> adapters;
+    Columns<Tile> bias;
+    __device__ __forceinline__ LinearY(const LinearArgs &a, const Tile &t) : adapters(a, t) { bias.read(t, a.bias, a.cols, 0.0f); }
+    __device__ __forceinline__ NothingElse beside() { return {}; }
+    __device__ __forceinline__ void behind(const LinearArgs &a, char *lds, Tile &t) { adapters.add(a, lds, t); }
+    __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) { linear_store<Tile, E, false>(a, room, t, bias); }
+};
+
+// A share of a projection's steps.
+template <typename Tile>
+struct LinearPart {
+    __device__ __forceinline__ LinearPart(const LinearArgs &, const Tile &) {}
+    __device__ __forceinline__ NothingElse beside() { return {}; }
+    __device__ __forceinline__ void behind(const LinearArgs &, char *, Tile &) {}
+    __device__ __forceinline__ void store(const LinearArgs &a, char *, Tile &t) { linear_store_part(a, t); }
+};
+
+// The sums of dout's rows, out of the fragments that the products with it read:
+// of the workgroups of the same rows each takes its turn of the steps, and of
+// the waves that read the same fragments each one of them. f32 parts count with
+// the first part of what they meet, once each.
+template <typename Tile>
+struct RowSums {
+    static constexpr int kOf = Tile::kJ / Tile::kWavesM;  // a wave's fragments of each sixteenth
+    static_assert(Tile::kJ % Tile::kWavesM == 0, "the waves share the fragments evenly");
+    uint32_t per, order, m_tiles, wave;
+    uint32_t at, seg, turn;  // of the step at hand
+    bool counts = false, wanted;
+    float sum[kOf] = {};
+    __device__ __forceinline__ RowSums(const LinearArgs &a, const Tile &t) {
+        per = (a.p.k + 63) / 64;
+        const uint32_t s0 = (uint32_t)((uint64_t)per * a.p.segments * t.split / a.p.splits);
+        order = a.p.a_order;
+        m_tiles = a.p.m_tiles;
+        wave = t.wave_m / Tile::kWaveM;
+        wanted = a.part_b != nullptr;
+        at = s0 % per;
+        seg = s0 / per;
+        turn = (s0 + m_tiles - t.m0 / Tile::kM) % m_tiles;
+    }
+    __device__ __forceinline__ void operator()(const bf16x8 (&fb)[Tile::kJ], uint32_t kk) {
+        if (kk == 0) {
+            counts = wanted && turn == 0 && (order >> 2 * seg & 3u) == 0;
+            if (++turn == m_tiles) turn = 0;
+            if (++at == per) at = 0, seg++;
+        }
+        if (!counts) return;
+#pragma unroll
+        for (int q = 0; q < kOf; q++) {
+            bf16x8 f = fb[q];
+#pragma unroll
+            for (int w = 1; w < Tile::kWavesM; w++) f = wave == (uint32_t)w ? fb[w * kOf + q] : f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum[q] += (float)f[k];
+        }
+    }
+};
+
+// The gradients of the inputs and of the weights.
+template <typename Tile, typename E>
+struct LinearDx {
+    __device__ __forceinline__ LinearDx(const LinearArgs &, const Tile &) {}
+    __device__ __forceinline__ NothingElse beside() { return {}; }
+    __device__ __forceinline__ void behind(const LinearArgs &, char *, Tile &) {}
+    __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) {
+        if (a.part) linear_store_part(a, t);
+        else linear_store<Tile, E, false>(a, room, t, NoColumns{});
+    }
+};
+
+template <typename Tile, typename E>
+struct LinearDw {
+    RowSums<Tile> sums;
+    __device__ __forceinline__ LinearDw(const LinearArgs &a, const Tile &t) : sums(a, t) {}
+    __device__ __forceinline__ RowSums<Tile> &beside() { return sums; }
+    __device__ __forceinline__ void behind(const LinearArgs &a, char *, Tile &t) {
+        if (!a.part_b) return;
+#pragma unroll
+        for (int q = 0; q < RowSums<Tile>::kOf; q++) {
+            const float sum = sums.sum[q] + __shfl_xor(sums.sum[q], 32, kWave);
+            const uint32_t r = t.n0 + t.wave_n + 32 * (sums.wave * RowSums<Tile>::kOf + q) + lane_id() % 32;
+            if (lane_id() < 32 && r < a.rows) a.part_b[((uint64_t)t.split * a.p.m_tiles + t.m0 / Tile::kM) * a.rows + r] = sum;
+        }
+    }
+    __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) {
+        if (a.part) {
+            linear_store_part(a, t);
+            return;
+        }
+        Columns<Tile> weight;
+        weight.read(t, a.weight, a.cols, 1.0f);
+        linear_store<Tile, E, true>(a, room, t, weight);
+    }
+};
+
+// A row's adapter in C neighbouring outputs (of `up`'s rows), sixteen ranks of
+// loads at a time.
+template <typename E, int C>
+__device__ __forceinline__ void adapter_cells(const float *low, const typename E::type *const (&up)[C], uint32_t rank, float (&more)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; c++) more[c] = 0.0f;
+    for (uint32_t rho0 = 0; rho0 < rank; rho0 += 16) {
+        float l[16], u[C][16];
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++) {
+            const uint32_t rho = min(rho0 + k, rank - 1);
+            l[k] = low[rho];
+#pragma unroll
+            for (int c = 0; c < C; c++) u[c][k] = E::up(up[c][rho]);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++)
+#pragma unroll
+            for (int c = 0; c < C; c++) more[c] = rho0 + k < rank ? __builtin_fmaf(l[k], u[c][k], more[c]) : more[c];
+    }
+}
+
+// The shares joined: a thread takes the four columns of a row that a lane held,
+// adds the shares in order and, of a projection, the row's adapter.
+template <typename Tile, typename E>
+__device__ __forceinline__ void linear_join(const LinearArgs &a) {
+    using T = typename E::type;
+    constexpr uint32_t kCells = Tile::kI * Tile::kJ * 4;
+    const uint64_t tiles = (uint64_t)a.p.m_tiles * a.p.n_tiles, tile = blockIdx.x / kCells;
+    const uint32_t cell = blockIdx.x % kCells, g = cell % 4, j = cell / 4 % Tile::kJ, i = cell / 4 / Tile::kJ;
+    Tile t;
+    t.m0 = (uint32_t)(tile / a.p.n_tiles) * Tile::kM;
+    t.n0 = (uint32_t)(tile % a.p.n_tiles) * Tile::kN;
+    const uint32_t wave = threadIdx.x / kWave;
+    t.wave_m = wave / Tile::kWavesN * Tile::kWaveM;
+    t.wave_n = wave % Tile::kWavesN * Tile::kWaveN;
+    const uint32_t c = column_of(t, i, g), r = t.n0 + t.wave_n + 32 * j + lane_id() % 32;
+    if (r >= a.rows || c >= a.cols) return;
+    float s[4] = {};
+#pragma unroll 4
+    for (uint32_t p = 0; p < a.p.splits; p++) {
+        const Vec<float, 4> v = reinterpret_cast<const Vec<float, 4> *>(a.part)[part_at<Tile>(a.p, p * tiles + tile, cell)];
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] += v.v[k];
+    }
+    if (a.low) {
+        const int32_t id = a.ids[r];
+        if (id >= 0 && (uint32_t)id < a.adapters) {
+            const float *low = a.low + (uint64_t)r * a.rank;
+            const T *up[4];
+            float more[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) up[k] = static_cast<const T *>(a.up) + ((uint64_t)id * a.cols + min(c + k, a.cols - 1)) * a.up_stride;
+            adapter_cells<E, 4>(low, up, a.rank, more);
+#pragma unroll
+            for (int k = 0; k < 4; k++) s[k] += more[k];
+        }
+    }
+    Vec<T, 4> v;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t column = min(c + k, a.cols - 1);
+        v.v[k] = E::down((a.weight ? s[k] * a.weight[column] : s[k]) + (a.bias ? a.bias[column] : 0.0f));
+    }
+    T *to = static_cast<T *>(a.out) + (uint64_t)r * a.out_stride + c;
+    if (c + 4 <= a.cols && a.out_stride % 4 == 0 && reinterpret_cast<uint64_t>(a.out) % (4 * sizeof(T)) == 0) {
+        *reinterpret_cast<Vec<T, 4> *>(to) = v;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (c + k < a.cols) to[k] = v.v[k];
 }
 
 // ---- sixteen rows against sixteen, without LDS ------------------------------------------------
@@ -286,15 +549,20 @@ struct Strip {
 };
 
 // The rows' low values: a workgroup takes 16 rows and all ranks of their
-// adapters, each adapter once, 32 of those rows of `down` at a time; its four
-// waves share the steps. A cell counts where the row's adapter is the column's.
-template <typename E, bool Wide>
+// adapters, each adapter once, 32 of those rows of `down` at a time; its waves
+// share the steps (16 of them where few workgroups have the CUs to themselves).
+// A cell counts where the row's adapter is the column's.
+template <typename E, bool Wide, uint32_t kWaves>
 __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     using T = typename E::type;
     using S = Strip<E, Wide>;
-    constexpr uint32_t kRows = 16, kCols = 2, kWaves = 4, kAhead = 4;
+    constexpr uint32_t kRows = 16, kCols = 2, kAhead = kWaves == 4 ? 4 : 2;
     __shared__ int32_t slot_id[kRows], slot_of[kRows];
     __shared__ f32x4 part[kWaves][kCols][kWave];
+    if (blockIdx.x >= a.groups) {
+        if (blockIdx.y == 0) tile_slots(a, blockIdx.x - a.groups);
+        return;
+    }
     const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, in = lane % 16, quarter = lane / 16;
     const uint64_t r0 = (uint64_t)blockIdx.x * kRows;
     // every wave finds the slots: the rows' adapters in order of their first rows
@@ -407,41 +675,73 @@ __device__ __forceinline__ void linear_few(const LinearFewArgs &a) {
         if (a.low) {
             const int32_t id = a.ids[r];
             if (id >= 0 && (uint32_t)id < a.adapters) {
-                const T *up = static_cast<const T *>(a.up) + ((uint64_t)id * a.outs + o0 + o) * a.up_stride;
-                const float *low = a.low + (uint64_t)r * a.rank;
-                float more = 0.0f;
-#pragma unroll 4
-                for (uint32_t rho = 0; rho < a.rank; rho++) more = __builtin_fmaf(low[rho], E::up(up[rho]), more);
-                s += more;
+                const T *const up[1] = {static_cast<const T *>(a.up) + ((uint64_t)id * a.outs + o0 + o) * a.up_stride};
+                float more[1];
+                adapter_cells<E, 1>(a.low + (uint64_t)r * a.rank, up, a.rank, more);
+                s += more[0];
             }
         }
         static_cast<T *>(a.out)[(uint64_t)r * a.out_stride + o0 + o] = E::down(s + bias);
     }
 }
 
-// Eight columns of a row a thread, a wave 16 rows of a chunk.
-__device__ __forceinline__ void lay_codes(const LayCodesArgs &a) {
-    const uint64_t cells = a.rows * a.chunks * 4;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t block = i / (a.rows * 16);
-        const uint32_t wide = min(4u, a.chunks - (uint32_t)block * 4);
-        const uint64_t in = i - block * a.rows * 16, r = in / (wide * 4);
-        const uint32_t chunk = (uint32_t)block * 4 + (uint32_t)(in % (wide * 4)) / 4, c = chunk * 32 + in % 4 * 8;
-        const uint8_t *src = a.codes + r * a.codes_stride + c;
-        Vec<uint8_t, 8> codes{};
-        if (c + 8 <= a.cols) {
-            __builtin_memcpy(&codes, src, 8);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (c + k < a.cols) codes.v[k] = src[k];
-        }
-        float v[8];
-        values_of<8>(codes, exp2_of((int32_t)a.scales[r * a.scales_stride + chunk] - kPowerBias), v);
+// Operands laid out in chunks: eight columns of a row a thread, a wave eight rows
+// of a chunk. The arrays' workgroups stand one behind the other.
+template <uint32_t Kind>
+__device__ __forceinline__ void lay(const LayArray &a, uint32_t block) {
+    using E = std::conditional_t<Kind == kLayF32, F32, Bf16>;
+    using T = typename E::type;
+    const uint64_t cells = a.rows * a.chunks * 8;
+    for (uint64_t i = (uint64_t)block * 256 + threadIdx.x; i < cells; i += (uint64_t)a.blocks * 256) {
+        // two chunks of a row by neighbouring threads
+        const uint64_t group = i / (a.rows * 16);
+        const uint32_t wide = min(2u, a.chunks - (uint32_t)group * 2);
+        const uint64_t in = i - group * a.rows * 16, r = in / (wide * 8);
+        const uint32_t chunk = (uint32_t)group * 2 + (uint32_t)(in % (wide * 8)) / 8, c = chunk * 64 + in % 8 * 8;
+        uint16_t *dst = a.dst + chunk * a.chunk + r * 64 + in % 8 * 8;
         Vec<uint16_t, 8> out;
+        if constexpr (Kind == kLayCodes) {
+            const uint8_t *src = static_cast<const uint8_t *>(a.src) + r * a.stride + c;
+            Vec<uint8_t, 8> codes{};
+            if (c + 8 <= a.cols) {
+                __builtin_memcpy(&codes, src, 8);
+            } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) out.v[k] = (uint16_t)(__float_as_uint(v[k]) >> 16);
-        *reinterpret_cast<Vec<uint16_t, 8> *>(a.dst + chunk * a.chunk + r * 32 + in % 4 * 8) = out;
+                for (int k = 0; k < 8; k++)
+                    if (c + k < a.cols) codes.v[k] = src[k];
+            }
+            float v[8];
+            values_of<8>(codes, exp2_of((int32_t)a.scales[r * a.scales_stride + min(c, a.cols - 1) / kPackBlock] - kPowerBias), v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) out.v[k] = (uint16_t)(__float_as_uint(v[k]) >> 16);
+            *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
+        } else {
+            const T *src = static_cast<const T *>(a.src) + r * a.stride + c;
+            Vec<T, 8> v{};
+            if (c + 8 <= a.cols) {
+                __builtin_memcpy(&v, src, sizeof v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (c + k < a.cols) v.v[k] = src[k];
+            }
+            if constexpr (Kind == kLayBf16) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) out.v[k] = v.v[k];
+                *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
+            } else {
+                Vec<uint16_t, 8> parts[3];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    uint16_t p[3];
+                    split3(v.v[k], p);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) parts[q].v[k] = p[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(dst + q * a.part) = parts[q];
+            }
+        }
     }
 }
 
@@ -463,33 +763,34 @@ __device__ __forceinline__ void column_sum(const ColumnSumArgs &a) {
 using namespace hbr;
 
 // waves: a SIMD's, at least
-#define HBR_LINEAR(name, Tile, waves, ...)                                               \
+#define HBR_LINEAR(name, Tile, waves, AT, BT, ...)                                           \
     extern "C" __global__ __launch_bounds__(Tile::kThreads, waves) void name(LinearArgs a) { \
-        __shared__ __align__(1024) char lds[Tile::kLds];                                 \
-        __VA_ARGS__(a, lds);                                                             \
+        __shared__ __align__(1024) char lds[Tile::kLds];                                  \
+        linear_tiles<AT, BT, Tile, __VA_ARGS__>(a, lds);                                     \
     }
-#define HBR_LINEARS(suffix, Tile, waves)                                                 \
-    HBR_LINEAR(hbr_linear_y_f32_##suffix, Tile, waves, linear_y<Tile, F32, false>)       \
-    HBR_LINEAR(hbr_linear_y_bf16_##suffix, Tile, waves, linear_y<Tile, Bf16, false>)     \
-    HBR_LINEAR(hbr_linear_y_part_f32_##suffix, Tile, waves, linear_y<Tile, F32, true>)   \
-    HBR_LINEAR(hbr_linear_y_part_bf16_##suffix, Tile, waves, linear_y<Tile, Bf16, true>) \
-    HBR_LINEAR(hbr_linear_dx_f32_##suffix, Tile, waves, linear_d<Tile, F32, false, false>) \
-    HBR_LINEAR(hbr_linear_dx_bf16_##suffix, Tile, waves, linear_d<Tile, Bf16, false, false>) \
-    HBR_LINEAR(hbr_linear_dx_part_##suffix, Tile, waves, linear_d<Tile, F32, false, true>) \
-    HBR_LINEAR(hbr_linear_dw_f32_##suffix, Tile, waves, linear_d<Tile, F32, true, false>) \
-    HBR_LINEAR(hbr_linear_dw_bf16_##suffix, Tile, waves, linear_d<Tile, Bf16, true, false>) \
-    HBR_LINEAR(hbr_linear_dw_part_##suffix, Tile, waves, linear_d<Tile, F32, true, true>)
-using Tile256 = HeadTile<8>;
-using Tile128 = HeadTile<4>;
-using Tile128Deep = HeadTile<4, 8>;
-HBR_LINEARS(256, Tile256, 2)
-HBR_LINEARS(128, Tile128, 4)
+#define HBR_LINEARS(suffix, Tile, waves)                                                             \
+    HBR_LINEAR(hbr_linear_y_f32_##suffix, Tile, waves, false, false, LinearY<Tile, F32>)             \
+    HBR_LINEAR(hbr_linear_y_bf16_##suffix, Tile, waves, false, false, LinearY<Tile, Bf16>)           \
+    HBR_LINEAR(hbr_linear_y_part_##suffix, Tile, waves, false, false, LinearPart<Tile>)              \
+    HBR_LINEAR(hbr_linear_dx_f32_##suffix, Tile, waves, true, false, LinearDx<Tile, F32>)            \
+    HBR_LINEAR(hbr_linear_dx_bf16_##suffix, Tile, waves, true, false, LinearDx<Tile, Bf16>)          \
+    HBR_LINEAR(hbr_linear_dw_f32_##suffix, Tile, waves, true, true, LinearDw<Tile, F32>)             \
+    HBR_LINEAR(hbr_linear_dw_bf16_##suffix, Tile, waves, true, true, LinearDw<Tile, Bf16>)
+#define HBR_JOIN(suffix, Tile)                                                                                                         \
+    extern "C" __global__ __launch_bounds__(Tile::kThreads) void hbr_linear_join_f32_##suffix(LinearArgs a) { linear_join<Tile, F32>(a); } \
+    extern "C" __global__ __launch_bounds__(Tile::kThreads) void hbr_linear_join_bf16_##suffix(LinearArgs a) { linear_join<Tile, Bf16>(a); }
+using Tile256 = ProductTile<256, 2, true>;
+using Tile128 = ProductTile<128, 2, false>;
+using Tile128Deep = ProductTile<128, 4, false>;
+HBR_LINEARS(256, Tile256, 1)
+HBR_LINEARS(128, Tile128, 2)
 HBR_LINEARS(128_deep, Tile128Deep, 1)
+HBR_JOIN(256, Tile256)
+HBR_JOIN(128, Tile128)
 
-extern "C" __global__ __launch_bounds__(256) void hbr_linear_join_f32(LinearJoinArgs a) { linear_join<F32>(a); }
-extern "C" __global__ __launch_bounds__(256) void hbr_linear_join_bf16(LinearJoinArgs a) { linear_join<Bf16>(a); }
 #define HBR_STRIPS(t, E, v, Wide)                                                                                                   \
-    extern "C" __global__ __launch_bounds__(256) void hbr_linear_low_##t##_##v(LinearLowArgs a) { linear_low<E, Wide>(a); }         \
+    extern "C" __global__ __launch_bounds__(256) void hbr_linear_low_##t##_##v(LinearLowArgs a) { linear_low<E, Wide, 4>(a); }      \
+    extern "C" __global__ __launch_bounds__(1024) void hbr_linear_low_##t##_##v##_16(LinearLowArgs a) { linear_low<E, Wide, 16>(a); } \
     extern "C" __global__ __launch_bounds__(256) void hbr_linear_few_##t##_##v##_16(LinearFewArgs a) { linear_few<E, 1, Wide>(a); } \
     extern "C" __global__ __launch_bounds__(256) void hbr_linear_few_##t##_##v##_32(LinearFewArgs a) { linear_few<E, 2, Wide>(a); } \
     extern "C" __global__ __launch_bounds__(256) void hbr_linear_few_##t##_##v##_64(LinearFewArgs a) { linear_few<E, 4, Wide>(a); }
@@ -497,6 +798,13 @@ HBR_STRIPS(f32, F32, 1, false)
 HBR_STRIPS(f32, F32, 4, true)
 HBR_STRIPS(bf16, Bf16, 1, false)
 HBR_STRIPS(bf16, Bf16, 8, true)
-extern "C" __global__ __launch_bounds__(256) void hbr_lay_codes(LayCodesArgs a) { lay_codes(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_lay(LayArgs a) {
+    uint32_t block = blockIdx.x, i = 0;
+    while (block >= a.of[i].blocks) block -= a.of[i++].blocks;
+    const LayArray &of = a.of[i];
+    if (of.kind == kLayF32) lay<kLayF32>(of, block);
+    else if (of.kind == kLayBf16) lay<kLayBf16>(of, block);
+    else lay<kLayCodes>(of, block);
+}
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_f32(ColumnSumArgs a) { column_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_bf16(ColumnSumArgs a) { column_sum<Bf16>(a); }

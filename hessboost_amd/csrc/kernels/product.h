@@ -139,12 +139,12 @@ struct Operand {
 };
 
 // A workgroup's tile of the product: 32 W x 32 W of W waves, 2 x W / 2, the
-// operands of kStages steps in LDS.
-template <int W, int Stages = 2>
+// operands of two steps in LDS.
+template <int W>
 struct HeadTile {
-    static constexpr int kStages = Stages, kW = W, kM = 32 * W, kN = 32 * W, kWavesM = 2, kWavesN = W / 2, kThreads = W * kWave;
+    static constexpr int kW = W, kM = 32 * W, kN = 32 * W, kWavesM = 2, kWavesN = W / 2, kThreads = W * kWave;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN, kI = kWaveM / 32, kJ = kWaveN / 32;
-    static constexpr int kStage = (kM + kN) * kHeadK * 2, kLds = Stages * kStage;
+    static constexpr int kStage = (kM + kN) * kHeadK * 2, kLds = 2 * kStage;
     uint32_t m0, n0, split;  // the tile's first row and column, and its share of the steps
     // element e of acc[i][j]: row wave_m + 32 i + row_of(e), column wave_n + 32 j + lane % 32
     f32x16 acc[kI][kJ];
@@ -175,10 +175,9 @@ __device__ __forceinline__ void head_place(const HeadArgs &a, Tile &t) {
 
 // The tile's products. A step's fragments are read one sixteenth of products
 // ahead of the matrix instructions that use them, across the steps too: the
-// last sixteenth's are in registers when the waves meet, so that a later
-// step's loads may overwrite its stage and the next one's first fragments be read
-// behind the meeting, both under the last sixteenth's products. The waves wait
-// for the next step's loads alone: those of the steps behind it stay in flight.
+// last sixteenth's are in registers when the waves meet, so that the next
+// step's loads may overwrite its stage and its first fragments be read
+// behind the meeting, both under the last sixteenth's products.
 template <bool AT, bool BT, typename Tile>
 __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile &t, const int32_t *a_labels = nullptr) {
     using A = Operand<AT, Tile::kW>;
@@ -207,7 +206,7 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
     // past the last step the loads read nothing
     auto load = [&](uint32_t s) {
         const uint32_t left = s < s1 ? a.k - at * kHeadK : 0;
-        const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % Tile::kStages * Tile::kStage;
+        const uint32_t to = (uint32_t)(uintptr_t)(HBR_LDS char *)lds + s % 2 * Tile::kStage;
         oa.load(to, left, a.a_row, a.check != 0);
         ob.load(to + A::kBytes, left, a.b_row, a.check != 0);
         if (++at == per) {
@@ -217,7 +216,7 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
     };
     bf16x8 fa[2][kI], fb[2][kJ];
     auto read = [&](int set, uint32_t s, uint32_t kk) {
-        const char *from = lds + s % Tile::kStages * Tile::kStage;
+        const char *from = lds + s % 2 * Tile::kStage;
 #pragma unroll
         for (int i = 0; i < kI; i++) fa[set][i] = A::fragment(from, t.wave_m + 32 * i, kk);
 #pragma unroll
@@ -234,16 +233,14 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    constexpr int kFlight = (Tile::kStages - 2) * (A::kLoads + B::kLoads);  // loads of the steps behind the next
-    auto meet = [&] {  // the wave's loads of the next step have landed and its reads are in registers; so have all others'
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kFlight) : "memory");
+    auto meet = [&] {  // the wave's loads have landed and its reads are in registers; so have all others'
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-#pragma unroll
-    for (int s = 0; s + 1 < Tile::kStages; s++) load(s0 + s);
+    load(s0);
     meet();
-    load(s0 + Tile::kStages - 1);
+    load(s0 + 1);
     read(0, s0, 0);
     for (uint32_t s = s0; s < s1; s++) {
 #pragma unroll
@@ -252,14 +249,11 @@ __device__ __forceinline__ void head_product(const HeadArgs &a, char *lds, Tile 
             multiply(kk & 1);
         }
         meet();
-        load(s + Tile::kStages);
+        load(s + 2);
         read(kSixteenths & 1, s + 1, 0);
         multiply((kSixteenths - 1) & 1);
     }
-    // the loads ahead have landed before the LDS or the workgroup ends
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    meet();  // the loads ahead have landed before the LDS or the workgroup ends
 }
 
 }  // namespace hbr

@@ -31,6 +31,10 @@ from . import _capi as A
 from .leafops import _CODE, _FLOATS, _Call, _code, _dtype, _size
 
 _BYTES = ("uint8", "float8_e4m3fn")
+_ALIKE = {d: (d,) for d in _FLOATS}
+_UINT8, _INT32, _FLOAT32 = ("uint8",), ("int32",), ("float32",)
+_packed_record, _norm_record, _norm_grad_record, _linear_record, _linear_grad_record = (
+    A.packer(r) for r in (A.Packed, A.Norm, A.NormGrad, A.Linear, A.LinearGrad))
 
 
 def packed_scales(dim):
@@ -38,20 +42,27 @@ def packed_scales(dim):
     return -(-_size(dim, "dim") // A.PACK_BLOCK)
 
 
-def _rows(call, a, what, dtype, shape):
+def _rows(call, a, what, dtypes, shape):
     """An optional array of rows: its address and row stride."""
     if a is None:
-        return None, 0
-    p, _, stride = call.array(a, what, 2, (dtype,) if isinstance(dtype, str) else dtype, shape)
+        return 0, 0
+    p, _, stride = call.array(a, what, 2, dtypes, shape)
     return p, stride
+
+
+def _vector(call, a, what, n, dtypes=_FLOAT32):
+    """An optional vector's address."""
+    return 0 if a is None else call.array(a, what, 1, dtypes, (n,))[0]
 
 
 def _packed(call, codes, scales, shape):
     """Rows in 8 bits: (codes, stride, scales, stride)."""
     if (codes is None) != (scales is None):
         raise ValueError("codes and scales go together")
+    if codes is None:
+        return 0, 0, 0, 0
     return (*_rows(call, codes, "codes", _BYTES, shape),
-            *_rows(call, scales, "scales", "uint8", (shape[0], packed_scales(shape[1]))))
+            *_rows(call, scales, "scales", _UINT8, (shape[0], packed_scales(shape[1]))))
 
 
 def pack_rows(x, codes, scales, *, stream=None):
@@ -59,8 +70,8 @@ def pack_rows(x, codes, scales, *, stream=None):
     call = _Call()
     xp, (n, dim), xs = call.array(x, "x", 2, _FLOATS)
     cp, cs, sp, ss = _packed(call, codes, scales, (n, dim))
-    p = A.Packed(_CODE[_dtype(x.dtype)], _size(dim, "dim"), n, xs, cs, ss)
-    A.check(A.lib().hbr_pack_rows(call.ordinal, C.byref(p), xp, cp, sp, call.stream(stream)))
+    p = _packed_record(_CODE[_dtype(x.dtype)], _size(dim, "dim"), n, xs, cs, ss)
+    A.check(A.lib().hbr_pack_rows(call.ordinal, p, xp, cp, sp, call.stream(stream)))
 
 
 def unpack_rows(codes, scales, out, *, weight=None, stream=None):
@@ -69,8 +80,8 @@ def unpack_rows(codes, scales, out, *, weight=None, stream=None):
     call = _Call()
     op, (n, dim), os = call.array(out, "out", 2, _FLOATS)
     cp, cs, sp, ss = _packed(call, codes, scales, (n, dim))
-    p = A.Packed(_CODE[_dtype(out.dtype)], _size(dim, "dim"), n, os, cs, ss)
-    A.check(A.lib().hbr_unpack_rows(call.ordinal, C.byref(p), cp, sp, call.pointer(weight, "weight", "float32", dim), op,
+    p = _packed_record(_CODE[_dtype(out.dtype)], _size(dim, "dim"), n, os, cs, ss)
+    A.check(A.lib().hbr_unpack_rows(call.ordinal, p, cp, sp, _vector(call, weight, "weight", dim), op,
                                     call.stream(stream)))
 
 
@@ -89,14 +100,15 @@ def rms_norm(x, out=None, *, weight=None, eps=1e-6, residual=None, total=None, i
     call = _Call()
     xp, (n, dim), xs = call.array(x, "x", 2, _FLOATS)
     dtype, shape = _dtype(x.dtype), (n, dim)
-    rp, rs = _rows(call, residual, "residual", dtype, shape)
-    op, os = _rows(call, out, "out", dtype, shape)
-    tp, ts = _rows(call, total, "total", dtype, shape)
+    alike = _ALIKE[dtype]
+    rp, rs = _rows(call, residual, "residual", alike, shape)
+    op, os = _rows(call, out, "out", alike, shape)
+    tp, ts = _rows(call, total, "total", alike, shape)
     cp, cs, sp, ss = _packed(call, codes, scales, shape)
-    p = A.Norm(_CODE[dtype], _size(dim, "dim"), n, xs, rs, os, ts, cs, ss, xp, rp,
-               call.pointer(weight, "weight", "float32", dim), op, tp, call.pointer(inv, "inv", "float32", n), cp, sp,
+    p = _norm_record(_CODE[dtype], _size(dim, "dim"), n, xs, rs, os, ts, cs, ss, xp, rp,
+               _vector(call, weight, "weight", dim), op, tp, _vector(call, inv, "inv", n), cp, sp,
                eps, int(bool(normed)))
-    A.check(A.lib().hbr_rms_norm(call.ordinal, C.byref(p), call.stream(stream)))
+    A.check(A.lib().hbr_rms_norm(call.ordinal, p, call.stream(stream)))
 
 
 def rms_norm_grad_workspace(n, dim, dtype):
@@ -120,15 +132,16 @@ def rms_norm_grad(dout, dx=None, *, x=None, codes=None, scales=None, inv=None, w
     call = _Call()
     gp, (n, dim), gs = call.array(dout, "dout", 2, _FLOATS)
     dtype, shape = _dtype(dout.dtype), (n, dim)
-    xp, xs = _rows(call, x, "x", dtype, shape)
+    alike = _ALIKE[dtype]
+    xp, xs = _rows(call, x, "x", alike, shape)
     cp, cs, sp, ss = _packed(call, codes, scales, shape)
-    tp, ts = _rows(call, dtotal, "dtotal", dtype, shape)
-    dp, ds = _rows(call, dx, "dx", dtype, shape)
-    p = A.NormGrad(_CODE[dtype], _size(dim, "dim"), n, gs, xs, cs, ss, ts, ds, gp, xp, cp, sp,
-                   call.pointer(inv, "inv", "float32", n), call.pointer(weight, "weight", "float32", dim), tp, dp,
-                   call.pointer(dweight, "dweight", "float32", dim), eps, 0)
+    tp, ts = _rows(call, dtotal, "dtotal", alike, shape)
+    dp, ds = _rows(call, dx, "dx", alike, shape)
+    p = _norm_grad_record(_CODE[dtype], _size(dim, "dim"), n, gs, xs, cs, ss, ts, ds, gp, xp, cp, sp,
+                   _vector(call, inv, "inv", n), _vector(call, weight, "weight", dim), tp, dp,
+                   _vector(call, dweight, "dweight", dim), eps, 0)
     m, nbytes = call.memory(workspace)
-    A.check(A.lib().hbr_rms_norm_grad(call.ordinal, C.byref(p), m, nbytes, call.stream(stream)))
+    A.check(A.lib().hbr_rms_norm_grad(call.ordinal, p, m, nbytes, call.stream(stream)))
 
 
 def linear_workspace(n, outs, dim, dtype, rank=0):
@@ -140,19 +153,22 @@ def linear_workspace(n, outs, dim, dtype, rank=0):
     return out.value
 
 
-def _flat(call, a, what, dtype, rows, cols):
+def _flat(call, a, what, dtypes, rows, cols):
     """An adapters' array of ``rows`` rows an adapter, [adapters, rows, cols]
     or [adapters * rows, cols]: its address, its rows' stride and how many
     adapters there are."""
-    dims = tuple(a.shape)
+    dims = a.shape
+    if len(dims) == 3 and dims[1] == rows and dims[2] == cols and a.is_contiguous():
+        p, _, _ = call.array(a, what, 3, dtypes)
+        return p, cols, dims[0]
     if len(dims) == 3:
         if dims[1:] != (rows, cols):
-            raise ValueError(f"{what}: the shape ({dims[0]}, {rows}, {cols}) is needed, not {dims}")
-        a = a.view(dims[0] * rows, cols) if a.is_contiguous() else _joined(a, what)
-        dims = tuple(a.shape)
+            raise ValueError(f"{what}: the shape ({dims[0]}, {rows}, {cols}) is needed, not {tuple(dims)}")
+        a = _joined(a, what)
+        dims = a.shape
     if len(dims) != 2 or dims[1] != cols or (rows and dims[0] % rows):
-        raise ValueError(f"{what}: {rows} rows of {cols} an adapter are needed, not {dims}")
-    p, _, stride = call.array(a, what, 2, (dtype,))
+        raise ValueError(f"{what}: {rows} rows of {cols} an adapter are needed, not {tuple(dims)}")
+    p, _, stride = call.array(a, what, 2, dtypes)
     return p, stride, dims[0] // rows if rows else 0
 
 
@@ -180,26 +196,26 @@ def linear(x, w, out, *, bias=None, down=None, up=None, ids=None, scale=None, wo
     call = _Call()
     xp, (n, dim), xs = call.array(x, "x", 2, _FLOATS)
     dtype, outs = _dtype(x.dtype), w.shape[0]
-    wp, _, ws = call.array(w, "w", 2, (dtype,), (outs, dim))
-    op, _, os = call.array(out, "out", 2, (dtype,), (n, outs))
+    alike = _ALIKE[dtype]
+    wp, _, ws = call.array(w, "w", 2, alike, (outs, dim))
+    op, _, os = call.array(out, "out", 2, alike, (n, outs))
     if len({a is None for a in (down, up, ids)}) > 1:
         raise ValueError("down, up and ids go together")
-    dp = up_ = ip = sp = None
-    rank = adapters = ds = us = 0
+    dp = up_ = ip = sp = rank = adapters = ds = us = 0
     if down is not None:
         rank = up.shape[-1]
-        dp, ds, adapters = _flat(call, down, "down", dtype, rank, dim)
-        up_, us, more = _flat(call, up, "up", dtype, outs, rank)
+        dp, ds, adapters = _flat(call, down, "down", alike, rank, dim)
+        up_, us, more = _flat(call, up, "up", alike, outs, rank)
         if rank and more != adapters:
             raise ValueError(f"up: {adapters} adapters are needed, not {more}")
-        ip = call.pointer(ids, "ids", "int32", n)
-        sp = call.pointer(scale, "scale", "float32", adapters)
+        ip = _vector(call, ids, "ids", n, _INT32)
+        sp = _vector(call, scale, "scale", adapters)
     elif scale is not None:
         raise ValueError("scale: there are no adapters")
-    p = A.Linear(_CODE[dtype], _size(dim, "dim"), n, _size(outs, "outs"), _size(rank, "rank"), _size(adapters, "adapters"), 0,
-                 xs, ws, os, ds, us, xp, wp, call.pointer(bias, "bias", "float32", outs), dp, up_, ip, sp, op)
+    p = _linear_record(_CODE[dtype], _size(dim, "dim"), n, _size(outs, "outs"), _size(rank, "rank"), _size(adapters, "adapters"), 0,
+                 xs, ws, os, ds, us, xp, wp, _vector(call, bias, "bias", outs), dp, up_, ip, sp, op)
     m, nbytes = call.memory(workspace)
-    A.check(A.lib().hbr_linear(call.ordinal, C.byref(p), m, nbytes, call.stream(stream)))
+    A.check(A.lib().hbr_linear(call.ordinal, p, m, nbytes, call.stream(stream)))
 
 
 def linear_grad_workspace(n, outs, dim, dtype):
@@ -223,15 +239,16 @@ def linear_grad(dout, w=None, *, x=None, codes=None, scales=None, weight=None, d
     call = _Call()
     gp, (n, outs), gs = call.array(dout, "dout", 2, _FLOATS)
     dtype = _dtype(dout.dtype)
+    alike = _ALIKE[dtype]
     dim = next((a.shape[1] for a in (w, x, codes, dx, dw) if a is not None and len(a.shape) == 2), None)
     if dim is None:  # db alone
         dim = 1
-    wp, ws = _rows(call, w, "w", dtype, (outs, dim))
-    xp, xs = _rows(call, x, "x", dtype, (n, dim))
+    wp, ws = _rows(call, w, "w", alike, (outs, dim))
+    xp, xs = _rows(call, x, "x", alike, (n, dim))
     cp, cs, sp, ss = _packed(call, codes, scales, (n, dim))
-    xgp, xgs = _rows(call, dx, "dx", dtype, (n, dim))
-    wgp, wgs = _rows(call, dw, "dw", dtype, (outs, dim))
-    p = A.LinearGrad(_CODE[dtype], _size(dim, "dim"), n, _size(outs, "outs"), 0, gs, ws, xs, cs, ss, xgs, wgs, gp, wp, xp, cp, sp,
-                     call.pointer(weight, "weight", "float32", dim), xgp, wgp, call.pointer(db, "db", "float32", outs))
+    xgp, xgs = _rows(call, dx, "dx", alike, (n, dim))
+    wgp, wgs = _rows(call, dw, "dw", alike, (outs, dim))
+    p = _linear_grad_record(_CODE[dtype], _size(dim, "dim"), n, _size(outs, "outs"), 0, gs, ws, xs, cs, ss, xgs, wgs, gp, wp, xp, cp, sp,
+                     _vector(call, weight, "weight", dim), xgp, wgp, _vector(call, db, "db", outs))
     m, nbytes = call.memory(workspace)
-    A.check(A.lib().hbr_linear_grad(call.ordinal, C.byref(p), m, nbytes, call.stream(stream)))
+    A.check(A.lib().hbr_linear_grad(call.ordinal, p, m, nbytes, call.stream(stream)))

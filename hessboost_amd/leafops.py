@@ -110,6 +110,7 @@ class _Call:
     def __init__(self):
         self.ordinal = None
         self.torch = False
+        self.kind = None  # the class of the last array whose device was looked at
 
     def device(self, a, what):
         if isinstance(a, DeviceArray):
@@ -125,17 +126,19 @@ class _Call:
             self.ordinal = ordinal
         elif self.ordinal != ordinal:
             raise ValueError(f"{what}: on device {ordinal}, the others on {self.ordinal}")
+        self.kind = a.__class__
 
     def array(self, a, what, ndim, dtypes, shape=None):
         """(address, shape, row stride) of an array whose last axis is contiguous."""
-        dims = tuple(a.shape)
+        dims = a.shape
         if len(dims) != ndim:
             raise ValueError(f"{what}: {ndim} axes are needed, not {len(dims)}")
-        if _dtype(a.dtype) not in dtypes:
+        if (_names.get(a.dtype) or _dtype(a.dtype)) not in dtypes:
             raise ValueError(f"{what}: {' or '.join(dtypes)} is needed, not {_dtype(a.dtype)}")
         if shape is not None and dims != shape:
-            raise ValueError(f"{what}: the shape {shape} is needed, not {dims}")
-        self.device(a, what)
+            raise ValueError(f"{what}: the shape {shape} is needed, not {tuple(dims)}")
+        if a.__class__ is not self.kind or a.get_device() != self.ordinal:
+            self.device(a, what)
         st = a.stride()
         if dims[-1] > 1 and st[-1] != 1:
             raise ValueError(f"{what}: the elements of a row must be contiguous")
@@ -163,8 +166,20 @@ class _Call:
         if stream is None:
             if not self.torch:
                 return None
-            return sys.modules["torch"].cuda.current_stream(self.ordinal).cuda_stream
+            return _current_stream(self.ordinal)
         return getattr(stream, "cuda_stream", stream)
+
+
+_raw_stream = None
+
+
+def _current_stream(ordinal):
+    """torch's current stream, without an object for it where torch has such a call."""
+    global _raw_stream
+    if _raw_stream is None:
+        torch = sys.modules["torch"]
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda o: torch.cuda.current_stream(o).cuda_stream)
+    return _raw_stream(ordinal)
 
 
 _runtime_checked = False
