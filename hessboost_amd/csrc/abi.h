@@ -1347,6 +1347,7 @@ struct LinearArgs {
     void *out;
     uint64_t out_stride;
     const float *weight, *bias; // or null
+    uint32_t large, pad;        // tiles of 256
     // the sums of a share of the steps as the lanes hold them: [split][tile]
     // [cell / 4 / threads][thread] of four columns; or null: the result
     float *part;
@@ -1363,32 +1364,14 @@ struct LinearArgs {
 };
 constexpr uint32_t kNoSlot = 0xffff;
 
-// hbr_linear_low_*: low[row][rho] = scale[a] <x[row], down[a][rho]>, a the row's
-// adapter; and which adapters a projection's tiles have.
-struct LinearLowArgs {
-    const void *x, *down;
-    const int32_t *ids;
-    const float *scale;         // or null
-    float *low;
-    uint64_t x_stride, down_stride;
-    uint32_t n_rows, dim, rank, adapters;
-    // workgroups from `groups` on: the adapters of a tile of `tile` rows
-    uint32_t groups, tile;
-    uint16_t *slot_of;
-    int32_t *slot_id;
-    uint32_t *slots;
-};
-
-// Few rows: hbr_linear_few_*.
-struct LinearFewArgs {
-    const void *x, *w;
-    const float *bias;
-    void *out;
-    const float *low;           // or null
-    const void *up;
-    const int32_t *ids;
-    uint64_t x_stride, w_stride, out_stride, up_stride;
-    uint32_t n_rows, dim, outs, rank, adapters, pad;
+// Both gradients' products in one launch of small tiles, and all that is joined
+// behind products in one: workgroups of the first, then of the second, then of db.
+struct LinearPairArgs {
+    LinearArgs of[2];
+    uint32_t groups[2];         // 0: none
+    const float *part_b;        // [part][outs], joined to db
+    float *db;
+    uint32_t b_parts, outs;
 };
 
 // hbr_lay: operands in chunks of 64 columns (zeros past cols): f32 in three bf16
@@ -1404,6 +1387,36 @@ struct LayArray {
 struct LayArgs {
     LayArray of[3];
     uint32_t arrays, pad;
+};
+
+// hbr_linear_low_*: low[row][rho] = scale[a] <x[row], down[a][rho]>, a the row's
+// adapter; and which adapters a projection's tiles have.
+struct LinearLowArgs {
+    const void *x, *down;
+    const int32_t *ids;
+    const float *scale;         // or null
+    float *low;
+    uint64_t x_stride, down_stride;
+    uint32_t n_rows, dim, rank, adapters;
+    // workgroups: 16 rows and a share of their ranks each, then a tile's adapters
+    // each, of `tile` rows, then those that lay out the product's operands
+    uint32_t groups, shares, tile, tiles;
+    uint16_t *slot_of;
+    int32_t *slot_id;
+    uint32_t *slots;
+    LayArgs lay;
+};
+
+// Few rows: hbr_linear_few_*.
+struct LinearFewArgs {
+    const void *x, *w;
+    const float *bias;
+    void *out;
+    const float *low;           // or null
+    const void *up;
+    const int32_t *ids;
+    uint64_t x_stride, w_stride, out_stride, up_stride;
+    uint32_t n_rows, dim, outs, rank, adapters, pad;
 };
 
 // part[share][column] = the sums of the share's rows.

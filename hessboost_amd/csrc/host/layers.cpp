@@ -128,8 +128,13 @@ void rms_norm(int ordinal, void *stream, const hbr_norm &p) {
 namespace {
 
 // Workgroups of the gradient at most: their sums of the weights' gradient are
-// held in the workspace.
-uint64_t norm_grad_blocks(uint64_t dim) { return std::max<uint64_t>(1, std::min<uint64_t>(1024, (1u << 22) / dim)); }
+// held in the workspace, 4 MiB of them where that leaves 512 workgroups, and read
+// once more (200,003 rows of 50: 2,048 of them 31.7 us, 1,024 38.3; 65,537 rows of
+// 1,024: 119 and 110).
+uint64_t norm_grad_blocks(uint64_t dim) {
+    const uint64_t by_sums = std::max<uint64_t>(512, std::min<uint64_t>(2048, (1u << 20) / dim));
+    return std::max<uint64_t>(1, std::min<uint64_t>(by_sums, (1u << 22) / dim));
+}
 
 }  // namespace
 
@@ -305,10 +310,13 @@ struct Operands {
         return lay(r, nullptr, dtype == HBR_F32 ? kLayF32 : kLayBf16, to);
     }
     Laid add(const Rows &codes, const Rows &scales, void *to) { return lay(codes, &scales, kLayCodes, to); }
+    uint32_t blocks() const {
+        uint32_t n = 0;
+        for (uint32_t i = 0; i < args.arrays; i++) n += args.of[i].blocks;
+        return n;
+    }
     void launch(Queue &queue) const {
-        uint32_t blocks = 0;
-        for (uint32_t i = 0; i < args.arrays; i++) blocks += args.of[i].blocks;
-        if (blocks) queue.launch("hbr_lay", dim3(blocks), dim3(256), args);
+        if (blocks()) queue.launch("hbr_lay", dim3(blocks()), dim3(256), args);
     }
 
 private:
@@ -340,20 +348,31 @@ void set_product(LinearArgs &a, const Product &p, float *part) {
     a.p.m_tiles = (uint32_t)p.m_tiles;
     a.p.n_tiles = (uint32_t)p.n_tiles;
     a.p.splits = (uint32_t)p.splits;
+    a.large = p.t == &kLarge;
     a.part = p.splits > 1 ? part : nullptr;
 }
 
-// A product's launch, and its shares' join.
-void run_product(Queue &queue, const char *name, uint32_t dtype, const Product &p, const LinearArgs &a) {
+void run_product(Queue &queue, const std::string &name, const Product &p, const LinearArgs &a) {
     // (a workgroup of the large tiles takes several)
     const uint64_t groups = p.t == &kLarge ? std::min(p.groups(), kLarge.slots) : p.groups();
     queue.launch((name + p.name()).c_str(), dim3((uint32_t)groups), dim3((uint32_t)p.t->threads), a);
-    if (p.splits == 1) return;
-    // a workgroup takes four columns of every thread's rows
-    const uint64_t cells = p.t->tile * p.t->tile / p.t->threads / 4;
-    queue.launch((std::string("hbr_linear_join_") + name_of(dtype) + p.t->name).c_str(), dim3((uint32_t)(p.m_tiles * p.n_tiles * cells)),
-                 dim3((uint32_t)p.t->threads), a);
 }
+
+// What is joined behind products: shares (a workgroup takes four columns of
+// every thread's rows of a tile), and db.
+struct Joins {
+    LinearPairArgs args{};
+    uint32_t products = 0;
+    void add(const Product &p, const LinearArgs &a) {
+        if (p.splits == 1) return;
+        args.of[products] = a;
+        args.groups[products++] = (uint32_t)(p.m_tiles * p.n_tiles * (p.t->tile * p.t->tile / p.t->threads / 4));
+    }
+    void launch(Queue &queue, const std::string &type) const {
+        const uint32_t groups = args.groups[0] + args.groups[1] + (args.db ? (uint32_t)tiles(args.outs, 16) : 0);
+        if (groups) queue.launch(("hbr_linear_joins_" + type).c_str(), dim3(groups), dim3(256), args);
+    }
+};
 
 void check_product(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype, const char *what) {
     size_of(dtype, what);
@@ -421,6 +440,7 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
     if (rank >= kDimLimit) fail(kRefused, std::string(what) + ": adapters of rank 1,048,576 or more");
     if (p.n_adapters > 0x7fffffffu) fail(kRefused, std::string(what) + ": more than 2^31 - 1 adapters");
     check_tiles(n, outs, what);
+    if (rank && n >= 1u << 28) fail(kRefused, std::string(what) + ": adapters of 2^28 rows or more");
     if (n == 0) return;
     if (!p.x || !p.w || !p.out) fail(kInvalid, std::string(what) + ": null argument");
     if (rank && (!p.down || !p.up || !p.ids)) fail(kInvalid, std::string(what) + ": adapters need down, up and ids");
@@ -442,58 +462,62 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         return kernel_of(name, p.dtype, v == 16 / size ? v : 1);
     };
     const bool few = few_rows(n, outs, dim, p.dtype);
-    if (rank) {
-        LinearLowArgs a{};
-        a.x = p.x;
-        a.down = p.down;
-        a.ids = p.ids;
-        a.scale = p.scale;
-        a.low = q.low;
-        a.x_stride = x.stride;
-        a.down_stride = down.stride;
-        a.n_rows = (uint32_t)n;
-        a.dim = p.dim;
-        a.rank = p.rank;
-        a.adapters = p.n_adapters;
-        // 16 rows a workgroup; of few of them several for the adapters' ranks
-        const uint64_t groups = tiles(n, 16), most = tiles(std::min<uint64_t>(n, 16) * rank, 32);
-        const bool slots = !few && q.product.splits == 1;
-        a.groups = (uint32_t)groups;
-        a.tile = (uint32_t)q.product.t->tile;
-        a.slot_of = q.slot_of;
-        a.slot_id = q.slot_id;
-        a.slots = q.slots;
-        const std::string name = strips("hbr_linear_low", {&x, &down}) + (few ? "_16" : "");
-        queue.launch(name.c_str(), dim3((uint32_t)(groups + (slots ? q.product.n_tiles : 0)), (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups))),
-                     dim3(few ? 1024 : 256), a);
-    }
-    if (few) {
-        LinearFewArgs a{};
-        a.x = p.x;
-        a.w = p.w;
-        a.bias = p.bias;
-        a.out = p.out;
-        a.low = rank ? q.low : nullptr;
-        a.up = p.up;
-        a.ids = p.ids;
-        a.x_stride = x.stride;
-        a.w_stride = w.stride;
-        a.out_stride = out.stride;
-        a.up_stride = up_rows.stride;
-        a.n_rows = (uint32_t)n;
-        a.dim = p.dim;
-        a.outs = p.n_outs;
-        a.rank = p.rank;
-        a.adapters = p.n_adapters;
-        queue.launch((strips("hbr_linear_few", {&x, &w}) + (n <= 16 ? "_16" : n <= 32 ? "_32" : "_64")).c_str(), dim3((uint32_t)tiles(outs, 16)),
-                     dim3(256), a);
-        return;
-    }
     LinearArgs a{};
     Operands operands(p.dtype);
-    set_a(a.p, operands.add(w, q.w));
-    set_b(a.p, operands.add(x, q.x));
-    operands.launch(queue);
+    if (!few) {
+        set_a(a.p, operands.add(w, q.w));
+        set_b(a.p, operands.add(x, q.x));
+    }
+    if (rank) {
+        LinearLowArgs l{};
+        l.x = p.x;
+        l.down = p.down;
+        l.ids = p.ids;
+        l.scale = p.scale;
+        l.low = q.low;
+        l.x_stride = x.stride;
+        l.down_stride = down.stride;
+        l.n_rows = (uint32_t)n;
+        l.dim = p.dim;
+        l.rank = p.rank;
+        l.adapters = p.n_adapters;
+        // 16 rows a workgroup; of few of them several for the adapters' ranks
+        const uint64_t groups = tiles(n, 16), most = tiles(std::min<uint64_t>(n, 16) * rank, 32);
+        l.groups = (uint32_t)groups;
+        l.shares = (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups));
+        l.tile = (uint32_t)q.product.t->tile;
+        l.tiles = !few && q.product.splits == 1 ? (uint32_t)q.product.n_tiles : 0;
+        l.slot_of = q.slot_of;
+        l.slot_id = q.slot_id;
+        l.slots = q.slots;
+        l.lay = operands.args;
+        queue.launch((strips("hbr_linear_low", {&x, &down}) + (few ? "_16" : "")).c_str(),
+                     dim3(l.groups * l.shares + l.tiles + operands.blocks()), dim3(few ? 1024 : 256), l);
+    } else {
+        operands.launch(queue);
+    }
+    if (few) {
+        LinearFewArgs f{};
+        f.x = p.x;
+        f.w = p.w;
+        f.bias = p.bias;
+        f.out = p.out;
+        f.low = rank ? q.low : nullptr;
+        f.up = p.up;
+        f.ids = p.ids;
+        f.x_stride = x.stride;
+        f.w_stride = w.stride;
+        f.out_stride = out.stride;
+        f.up_stride = up_rows.stride;
+        f.n_rows = (uint32_t)n;
+        f.dim = p.dim;
+        f.outs = p.n_outs;
+        f.rank = p.rank;
+        f.adapters = p.n_adapters;
+        queue.launch((strips("hbr_linear_few", {&x, &w}) + (n <= 16 ? "_16" : n <= 32 ? "_32" : "_64")).c_str(), dim3((uint32_t)tiles(outs, 16)),
+                     dim3(256), f);
+        return;
+    }
     a.p.m = a.cols = p.n_outs;
     a.p.n = a.rows = (uint32_t)n;
     a.p.k = p.dim;
@@ -511,7 +535,10 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
     a.up_stride = up_rows.stride;
     a.rank = p.rank;
     a.adapters = p.n_adapters;
-    run_product(queue, ("hbr_linear_y_" + (a.part ? "part" : type)).c_str(), p.dtype, q.product, a);
+    run_product(queue, "hbr_linear_y_" + (a.part ? "part" : type), q.product, a);
+    Joins joins;
+    joins.add(q.product, a);
+    joins.launch(queue, type);
 }
 
 namespace {
@@ -589,6 +616,7 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
         return;
     }
     uint64_t sums = 0;  // of db
+    Joins joins;
     if (p.db && !p.dw) {
         ColumnSumArgs a{};
         a.x = p.dout;
@@ -620,7 +648,6 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
             set_product(a, q.by_x, q.part_x);
             a.out = p.dx;
             a.out_stride = dx.stride;
-            run_product(queue, ("hbr_linear_dx_" + type).c_str(), p.dtype, q.by_x, a);
         }
         if (p.dw) {
             LinearArgs &a = w_args;
@@ -637,10 +664,28 @@ void linear_grad(int ordinal, void *stream, const hbr_linear_grad_args &p, void 
             a.weight = p.weight;
             a.part_b = p.db ? q.part_b : nullptr;
             if (p.db) sums = q.by_w.splits * q.by_w.m_tiles;
-            run_product(queue, ("hbr_linear_dw_" + type).c_str(), p.dtype, q.by_w, a);
         }
+        // both in one launch where both have small tiles that run at once (4,001 x
+        // 250 x 333 in f32: 26 us in two launches)
+        if (p.dx && p.dw && q.by_x.t == &kSmall && q.by_w.t == &kSmall && q.by_x.groups() + q.by_w.groups() <= kSmall.slots) {
+            LinearPairArgs pair{};
+            pair.of[0] = x_args;
+            pair.of[1] = w_args;
+            pair.groups[0] = (uint32_t)q.by_x.groups();
+            pair.groups[1] = (uint32_t)q.by_w.groups();
+            queue.launch(("hbr_linear_pair_" + type).c_str(), dim3(pair.groups[0] + pair.groups[1]), dim3(256), pair);
+        } else {
+            if (p.dx) run_product(queue, "hbr_linear_dx_" + type, q.by_x, x_args);
+            if (p.dw) run_product(queue, "hbr_linear_dw_" + type, q.by_w, w_args);
+        }
+        if (p.dx) joins.add(q.by_x, x_args);
+        if (p.dw) joins.add(q.by_w, w_args);
     }
-    if (p.db) sum_parts(queue, HBR_F32, 1.0f, q.part_b, sums, outs, p.db, 1, outs, outs);
+    joins.args.part_b = q.part_b;
+    joins.args.db = p.db;
+    joins.args.b_parts = (uint32_t)sums;
+    joins.args.outs = p.n_outs;
+    joins.launch(queue, type);
 }
 
 }  // namespace hbr

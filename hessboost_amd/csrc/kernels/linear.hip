@@ -315,7 +315,7 @@ __device__ __forceinline__ void tile_slots(const LinearLowArgs &a, uint32_t tile
 // while the last one's cells are written. `Work` has what is done before a tile's
 // products, beside them, behind them in the stages, and with its cells.
 template <bool AT, bool BT, typename Tile, typename Work>
-__device__ __forceinline__ void linear_tiles(const LinearArgs &a, char *lds) {
+__device__ __forceinline__ void linear_tiles(const LinearArgs &a, char *lds, uint32_t first, uint32_t groups) {
     const uint32_t all = a.p.m_tiles * a.p.n_tiles * a.p.splits;
     char *room = lds + Tile::kRoom;
     TileProduct<AT, BT, Tile> product(a.p, lds);
@@ -323,15 +323,15 @@ __device__ __forceinline__ void linear_tiles(const LinearArgs &a, char *lds) {
     const uint32_t wave = uniform(threadIdx.x / kWave);
     t.wave_m = wave / Tile::kWavesN * Tile::kWaveM;
     t.wave_n = wave % Tile::kWavesN * Tile::kWaveN;
-    Spot next = tile_spot<Tile>(a.p, blockIdx.x, all);
+    Spot next = tile_spot<Tile>(a.p, first, all);
     product.prime(next);
-    for (uint32_t index = blockIdx.x;;) {
+    for (uint32_t index = first;;) {
         static_cast<Spot &>(t) = next;
         Work work(a, t);
         product.run(t, work.beside());
         hold(t);
         work.behind(a, lds, t);
-        index += gridDim.x;
+        index += groups;
         const bool more = Tile::kSeveral && index < all;
         if (more) {
             next = tile_spot<Tile>(a.p, index, all);
@@ -464,11 +464,11 @@ __device__ __forceinline__ void adapter_cells(const float *low, const typename E
 // The shares joined: a thread takes the four columns of a row that a lane held,
 // adds the shares in order and, of a projection, the row's adapter.
 template <typename Tile, typename E>
-__device__ __forceinline__ void linear_join(const LinearArgs &a) {
+__device__ __forceinline__ void linear_join(const LinearArgs &a, uint32_t block) {
     using T = typename E::type;
     constexpr uint32_t kCells = Tile::kI * Tile::kJ * 4;
-    const uint64_t tiles = (uint64_t)a.p.m_tiles * a.p.n_tiles, tile = blockIdx.x / kCells;
-    const uint32_t cell = blockIdx.x % kCells, g = cell % 4, j = cell / 4 % Tile::kJ, i = cell / 4 / Tile::kJ;
+    const uint64_t tiles = (uint64_t)a.p.m_tiles * a.p.n_tiles, tile = block / kCells;
+    const uint32_t cell = block % kCells, g = cell % 4, j = cell / 4 % Tile::kJ, i = cell / 4 / Tile::kJ;
     Tile t;
     t.m0 = (uint32_t)(tile / a.p.n_tiles) * Tile::kM;
     t.n0 = (uint32_t)(tile % a.p.n_tiles) * Tile::kN;
@@ -511,6 +511,114 @@ __device__ __forceinline__ void linear_join(const LinearArgs &a) {
 #pragma unroll
     for (int k = 0; k < 4; k++)
         if (c + k < a.cols) to[k] = v.v[k];
+}
+
+// db's parts joined: 16 columns a workgroup, a thread a column and a sixteenth of the parts.
+__device__ __forceinline__ void linear_join_db(const LinearPairArgs &a, uint32_t block) {
+    __shared__ float sum_of[16][16];
+    const uint32_t in = threadIdx.x % 16, share = threadIdx.x / 16, c = block * 16 + in;
+    float s = 0.0f;
+    if (c < a.outs) {
+#pragma unroll 4
+        for (uint32_t p = share; p < a.b_parts; p += 16) s += a.part_b[(uint64_t)p * a.outs + c];
+    }
+    sum_of[share][in] = s;
+    __syncthreads();
+    if (share || c >= a.outs) return;
+    for (uint32_t w = 1; w < 16; w++) s += sum_of[w][in];
+    a.db[c] = s;
+}
+
+// Either product's shares, by its tile, and db.
+template <typename E>
+__device__ __forceinline__ void linear_joins(const LinearPairArgs &a) {
+    uint32_t block = blockIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (block < a.groups[i]) {
+            if (a.of[i].large) linear_join<ProductTile<256, 2, true>, E>(a.of[i], block);
+            else linear_join<ProductTile<128, 2, false>, E>(a.of[i], block);
+            return;
+        }
+        block -= a.groups[i];
+    }
+    linear_join_db(a, block);
+}
+
+// Operands laid out in chunks: eight columns of a row a thread, a wave eight rows
+// of a chunk. The arrays' workgroups stand one behind the other.
+template <uint32_t Kind>
+__device__ __forceinline__ void lay(const LayArray &a, uint32_t block) {
+    using E = std::conditional_t<Kind == kLayF32, F32, Bf16>;
+    using T = typename E::type;
+    const uint64_t cells = a.rows * a.chunks * 8;
+    for (uint64_t i = (uint64_t)block * 256 + threadIdx.x; i < cells; i += (uint64_t)a.blocks * 256) {
+        // two chunks of a row by neighbouring threads
+        const uint64_t group = i / (a.rows * 16);
+        const uint32_t wide = min(2u, a.chunks - (uint32_t)group * 2);
+        const uint64_t in = i - group * a.rows * 16, r = in / (wide * 8);
+        const uint32_t chunk = (uint32_t)group * 2 + (uint32_t)(in % (wide * 8)) / 8, c = chunk * 64 + in % 8 * 8;
+        uint16_t *dst = a.dst + chunk * a.chunk + r * 64 + in % 8 * 8;
+        Vec<uint16_t, 8> out;
+        if constexpr (Kind == kLayCodes) {
+            const uint8_t *src = static_cast<const uint8_t *>(a.src) + r * a.stride + c;
+            Vec<uint8_t, 8> codes{};
+            if (c + 8 <= a.cols) {
+                __builtin_memcpy(&codes, src, 8);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (c + k < a.cols) codes.v[k] = src[k];
+            }
+            float v[8];
+            values_of<8>(codes, exp2_of((int32_t)a.scales[r * a.scales_stride + min(c, a.cols - 1) / kPackBlock] - kPowerBias), v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) out.v[k] = (uint16_t)(__float_as_uint(v[k]) >> 16);
+            *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
+        } else {
+            const T *src = static_cast<const T *>(a.src) + r * a.stride + c;
+            Vec<T, 8> v{};
+            if (c + 8 <= a.cols) {
+                __builtin_memcpy(&v, src, sizeof v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (c + k < a.cols) v.v[k] = src[k];
+            }
+            if constexpr (Kind == kLayBf16) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) out.v[k] = v.v[k];
+                *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
+            } else {
+                Vec<uint16_t, 8> parts[3];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    uint16_t p[3];
+                    split3(v.v[k], p);
+#pragma unroll
+                    for (int q = 0; q < 3; q++) parts[q].v[k] = p[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(dst + q * a.part) = parts[q];
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void lay_all(const LayArgs &a, uint32_t block) {
+    // (by constant places: an argument read at a variable one goes through memory)
+    LayArray of = a.of[0];
+    if (block >= of.blocks) {
+        block -= of.blocks;
+        of = a.of[1];
+        if (block >= of.blocks) {
+            block -= of.blocks;
+            of = a.of[2];
+        }
+    }
+    if (of.kind == kLayF32) lay<kLayF32>(of, block);
+    else if (of.kind == kLayBf16) lay<kLayBf16>(of, block);
+    else lay<kLayCodes>(of, block);
 }
 
 // ---- sixteen rows against sixteen, without LDS ------------------------------------------------
@@ -559,12 +667,17 @@ __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     constexpr uint32_t kRows = 16, kCols = 2, kAhead = kWaves == 4 ? 4 : 2;
     __shared__ int32_t slot_id[kRows], slot_of[kRows];
     __shared__ f32x4 part[kWaves][kCols][kWave];
-    if (blockIdx.x >= a.groups) {
-        if (blockIdx.y == 0) tile_slots(a, blockIdx.x - a.groups);
+    if (blockIdx.x >= a.groups * a.shares) {
+        const uint32_t block = blockIdx.x - a.groups * a.shares;
+        if constexpr (kWaves == 4) {
+            if (block < a.tiles) tile_slots(a, block);
+            else lay_all(a.lay, block - a.tiles);
+        }
         return;
     }
+    const uint32_t share = blockIdx.x / a.groups;
     const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, in = lane % 16, quarter = lane / 16;
-    const uint64_t r0 = (uint64_t)blockIdx.x * kRows;
+    const uint64_t r0 = (uint64_t)(blockIdx.x % a.groups) * kRows;
     // every wave finds the slots: the rows' adapters in order of their first rows
     int32_t id = r0 + in < a.n_rows ? a.ids[r0 + in] : -1;
     if (id < 0 || (uint32_t)id >= a.adapters) id = -1;
@@ -581,7 +694,7 @@ __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     __syncthreads();
     const uint32_t all = slots * a.rank;
     const T *x = static_cast<const T *>(a.x) + min(r0 + in, (uint64_t)a.n_rows - 1) * a.x_stride;
-    for (uint32_t v0 = blockIdx.y * kCols * 16; v0 < all; v0 += gridDim.y * kCols * 16) {
+    for (uint32_t v0 = share * kCols * 16; v0 < all; v0 += a.shares * kCols * 16) {
         const T *down[kCols];
 #pragma unroll
         for (uint32_t q = 0; q < kCols; q++) {
@@ -685,66 +798,6 @@ __device__ __forceinline__ void linear_few(const LinearFewArgs &a) {
     }
 }
 
-// Operands laid out in chunks: eight columns of a row a thread, a wave eight rows
-// of a chunk. The arrays' workgroups stand one behind the other.
-template <uint32_t Kind>
-__device__ __forceinline__ void lay(const LayArray &a, uint32_t block) {
-    using E = std::conditional_t<Kind == kLayF32, F32, Bf16>;
-    using T = typename E::type;
-    const uint64_t cells = a.rows * a.chunks * 8;
-    for (uint64_t i = (uint64_t)block * 256 + threadIdx.x; i < cells; i += (uint64_t)a.blocks * 256) {
-        // two chunks of a row by neighbouring threads
-        const uint64_t group = i / (a.rows * 16);
-        const uint32_t wide = min(2u, a.chunks - (uint32_t)group * 2);
-        const uint64_t in = i - group * a.rows * 16, r = in / (wide * 8);
-        const uint32_t chunk = (uint32_t)group * 2 + (uint32_t)(in % (wide * 8)) / 8, c = chunk * 64 + in % 8 * 8;
-        uint16_t *dst = a.dst + chunk * a.chunk + r * 64 + in % 8 * 8;
-        Vec<uint16_t, 8> out;
-        if constexpr (Kind == kLayCodes) {
-            const uint8_t *src = static_cast<const uint8_t *>(a.src) + r * a.stride + c;
-            Vec<uint8_t, 8> codes{};
-            if (c + 8 <= a.cols) {
-                __builtin_memcpy(&codes, src, 8);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (c + k < a.cols) codes.v[k] = src[k];
-            }
-            float v[8];
-            values_of<8>(codes, exp2_of((int32_t)a.scales[r * a.scales_stride + min(c, a.cols - 1) / kPackBlock] - kPowerBias), v);
-#pragma unroll
-            for (int k = 0; k < 8; k++) out.v[k] = (uint16_t)(__float_as_uint(v[k]) >> 16);
-            *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
-        } else {
-            const T *src = static_cast<const T *>(a.src) + r * a.stride + c;
-            Vec<T, 8> v{};
-            if (c + 8 <= a.cols) {
-                __builtin_memcpy(&v, src, sizeof v);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (c + k < a.cols) v.v[k] = src[k];
-            }
-            if constexpr (Kind == kLayBf16) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) out.v[k] = v.v[k];
-                *reinterpret_cast<Vec<uint16_t, 8> *>(dst) = out;
-            } else {
-                Vec<uint16_t, 8> parts[3];
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    uint16_t p[3];
-                    split3(v.v[k], p);
-#pragma unroll
-                    for (int q = 0; q < 3; q++) parts[q].v[k] = p[q];
-                }
-#pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(dst + q * a.part) = parts[q];
-            }
-        }
-    }
-}
-
 // A column a thread, a share of the rows a workgroup.
 template <typename E>
 __device__ __forceinline__ void column_sum(const ColumnSumArgs &a) {
@@ -766,7 +819,7 @@ using namespace hbr;
 #define HBR_LINEAR(name, Tile, waves, AT, BT, ...)                                           \
     extern "C" __global__ __launch_bounds__(Tile::kThreads, waves) void name(LinearArgs a) { \
         __shared__ __align__(1024) char lds[Tile::kLds];                                  \
-        linear_tiles<AT, BT, Tile, __VA_ARGS__>(a, lds);                                     \
+        linear_tiles<AT, BT, Tile, __VA_ARGS__>(a, lds, blockIdx.x, gridDim.x);              \
     }
 #define HBR_LINEARS(suffix, Tile, waves)                                                             \
     HBR_LINEAR(hbr_linear_y_f32_##suffix, Tile, waves, false, false, LinearY<Tile, F32>)             \
@@ -776,17 +829,22 @@ using namespace hbr;
     HBR_LINEAR(hbr_linear_dx_bf16_##suffix, Tile, waves, true, false, LinearDx<Tile, Bf16>)          \
     HBR_LINEAR(hbr_linear_dw_f32_##suffix, Tile, waves, true, true, LinearDw<Tile, F32>)             \
     HBR_LINEAR(hbr_linear_dw_bf16_##suffix, Tile, waves, true, true, LinearDw<Tile, Bf16>)
-#define HBR_JOIN(suffix, Tile)                                                                                                         \
-    extern "C" __global__ __launch_bounds__(Tile::kThreads) void hbr_linear_join_f32_##suffix(LinearArgs a) { linear_join<Tile, F32>(a); } \
-    extern "C" __global__ __launch_bounds__(Tile::kThreads) void hbr_linear_join_bf16_##suffix(LinearArgs a) { linear_join<Tile, Bf16>(a); }
 using Tile256 = ProductTile<256, 2, true>;
 using Tile128 = ProductTile<128, 2, false>;
 using Tile128Deep = ProductTile<128, 4, false>;
 HBR_LINEARS(256, Tile256, 1)
 HBR_LINEARS(128, Tile128, 2)
 HBR_LINEARS(128_deep, Tile128Deep, 1)
-HBR_JOIN(256, Tile256)
-HBR_JOIN(128, Tile128)
+
+#define HBR_PAIR(t, E)                                                                                                \
+    extern "C" __global__ __launch_bounds__(256, 2) void hbr_linear_pair_##t(LinearPairArgs a) {                      \
+        __shared__ __align__(1024) char lds[Tile128::kLds];                                                           \
+        if (blockIdx.x < a.groups[0]) linear_tiles<true, false, Tile128, LinearDx<Tile128, E>>(a.of[0], lds, blockIdx.x, 1); \
+        else linear_tiles<true, true, Tile128, LinearDw<Tile128, E>>(a.of[1], lds, blockIdx.x - a.groups[0], 1);      \
+    }                                                                                                                 \
+    extern "C" __global__ __launch_bounds__(256) void hbr_linear_joins_##t(LinearPairArgs a) { linear_joins<E>(a); }
+HBR_PAIR(f32, F32)
+HBR_PAIR(bf16, Bf16)
 
 #define HBR_STRIPS(t, E, v, Wide)                                                                                                   \
     extern "C" __global__ __launch_bounds__(256) void hbr_linear_low_##t##_##v(LinearLowArgs a) { linear_low<E, Wide, 4>(a); }      \
@@ -798,13 +856,6 @@ HBR_STRIPS(f32, F32, 1, false)
 HBR_STRIPS(f32, F32, 4, true)
 HBR_STRIPS(bf16, Bf16, 1, false)
 HBR_STRIPS(bf16, Bf16, 8, true)
-extern "C" __global__ __launch_bounds__(256) void hbr_lay(LayArgs a) {
-    uint32_t block = blockIdx.x, i = 0;
-    while (block >= a.of[i].blocks) block -= a.of[i++].blocks;
-    const LayArray &of = a.of[i];
-    if (of.kind == kLayF32) lay<kLayF32>(of, block);
-    else if (of.kind == kLayBf16) lay<kLayBf16>(of, block);
-    else lay<kLayCodes>(of, block);
-}
+extern "C" __global__ __launch_bounds__(256) void hbr_lay(LayArgs a) { lay_all(a, blockIdx.x); }
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_f32(ColumnSumArgs a) { column_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_bf16(ColumnSumArgs a) { column_sum<Bf16>(a); }
