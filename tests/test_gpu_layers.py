@@ -1,5 +1,6 @@
 """The operators of the layers between leaf vectors and classes against their
 plain forms in 64 bits, at the sizes, masks and layouts where they can go wrong."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -11,7 +12,7 @@ import hessboost_amd as hb
 import layer_reference as L
 import leaf_reference as R
 from hessboost_amd.leafops import DeviceArray
-from test_gpu_leafops import back, close, dev, like, work
+from test_gpu_leafops import back, close, dev, far, far_back, hip, like, ok, work
 
 pytestmark = pytest.mark.gpu
 
@@ -430,3 +431,315 @@ def test_no_rows(dtype):
                    workspace=work(hb.linear_grad_workspace(0, outs, dim, dtype)))
     for a in (dweight, dw, db):
         assert np.all(back(a) == 0)
+
+
+# ---- arrays of more than 4 GiB, and other places ------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layers_over_more_than_4_gib(dtype):
+    """Rows far apart: 8 of them 2 GiB or so, and 70 of them 128 MiB."""
+    rng = np.random.default_rng(9)
+    size = 2 if dtype == "bfloat16" else 4
+    for n, dim, gap in ((8, 40, (1 << 30) // size + 16), (70, 200, (1 << 27) // size + 8)):
+        x, r, w = rows(rng, n, dim, dtype), rows(rng, n, dim, dtype), rows(rng, 24, dim, dtype)
+        want = L.norm(x, r, None, 1e-6, dtype)
+        held = far(n, dim, dtype, gap, x)
+        out = like((n, dim), dtype)
+        hb.rms_norm(held, out, residual=dev(r, dtype))
+        close(back(out), want["out"], "x far")
+        codes, scales = packed_like(n, dim)
+        hb.pack_rows(held, codes, scales)
+        assert np.array_equal(bytes_back(codes), L.codes_of(x)[0])
+        dout = rows(rng, n, dim, dtype)
+        dx = like((n, dim), dtype)
+        hb.rms_norm_grad(dev(dout, dtype), dx, x=held)
+        close(back(dx), L.norm_grad(dout, x, None, None, None, 1e-6, False, dtype)["dx"], "x of the gradient far")
+        g = rows(rng, n, 24, dtype)
+        y = like((n, 24), dtype)
+        hb.linear(held, dev(w, dtype), y, workspace=work(hb.linear_workspace(n, 24, dim, dtype)))
+        close(back(y), L.linear(x, w, None, None, None, None, None, dtype), "x of a projection far")
+        dw = like((24, dim), dtype)
+        hb.linear_grad(dev(g, dtype), x=held, dw=dw, workspace=work(hb.linear_grad_workspace(n, 24, dim, dtype)))
+        close(back(dw), L.linear_grad(g, None, x, None, dtype)["dw"], "x of dw far")
+        del held
+        for call, value in ((lambda a: hb.rms_norm(dev(x, dtype), a, residual=dev(r, dtype)), want["out"]),
+                            (lambda a: hb.unpack_rows(codes, scales, a), (L.values_of(*L.codes_of(x)), 1e-40 + 0 * x)),
+                            (lambda a: hb.linear_grad(dev(g, dtype), dev(w, dtype), dx=a, workspace=work(hb.linear_grad_workspace(n, 24, dim, dtype))),
+                             L.linear_grad(g, w, None, None, dtype)["dx"])):
+            a = far(n, dim, dtype, gap)
+            call(a)
+            close(far_back(a), value, "an output far")
+            del a
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows(dtype):
+    """More rows than a launch has workgroups, tiles of several rounds, shares
+    of long sums: against sums in 64 bits of what the operators were given."""
+    rng = np.random.default_rng(12)
+    n, dim, outs = 70_001, 40, 72
+    x, w = rows(rng, n, dim, dtype), rows(rng, outs, dim, dtype, 0.2)
+    out, codes, scales = like((n, dim), dtype), *packed_like(n, dim)
+    inv = like(n, "float32")
+    hb.rms_norm(dev(x, dtype), out, inv=inv, codes=codes, scales=scales, normed=True)
+    want = L.norm(x, None, None, 1e-6, dtype)
+    close(back(out), want["out"], "out")
+    dout = rows(rng, n, dim, dtype, 1.0 / n)
+    v = L.values_of(bytes_back(codes), bytes_back(scales))
+    by = back(inv)
+    dx, dweight = like((n, dim), dtype), like(dim, "float32")
+    hb.rms_norm_grad(dev(dout, dtype), dx, codes=codes, scales=scales, inv=inv, dweight=dweight,
+                     workspace=work(hb.rms_norm_grad_workspace(n, dim, dtype)))
+    want = L.norm_grad(dout, v, by, None, None, 0.0, True, dtype)
+    close(back(dx), want["dx"], "dx")
+    close(back(dweight), want["dweight"], "dweight")
+    ids = ids_of(rng, n, 5, "runs")
+    down, up = rows(rng, 5 * 8, dim, dtype, 0.2), rows(rng, 5 * outs, 8, dtype)
+    y = like((n, outs), dtype)
+    hb.linear(dev(x, dtype), dev(w, dtype), y, down=dev(down, dtype), up=dev(up, dtype), ids=dev(ids, "int32"),
+              workspace=work(hb.linear_workspace(n, outs, dim, dtype, rank=8)))
+    got = back(y)
+    some = np.unique(np.r_[0:300, n - 300:n, rng.integers(0, n, 500)])
+    value, off = L.linear(x[some], w, None, down.reshape(5, 8, dim), up.reshape(5, outs, 8), ids[some], None, dtype)
+    close(got[some], (value, off), "y")
+    g = rows(rng, n, outs, dtype, 1.0 / n)
+    dw, db, dx = like((outs, dim), dtype), like(outs, "float32"), like((n, dim), dtype)
+    hb.linear_grad(dev(g, dtype), dev(w, dtype), codes=codes, scales=scales, dw=dw, db=db, dx=dx,
+                   workspace=work(hb.linear_grad_workspace(n, outs, dim, dtype)))
+    want = L.linear_grad(g, w, v, None, dtype)
+    for name, a in (("dw", dw), ("db", db), ("dx", dx)):
+        close(back(a), want[name], name)
+
+
+@pytest.mark.parametrize("n, dim, outs", [(600, 256, 2560), (1500, 2000, 300), (5000, 520, 1030), (130, 70, 9000), (16_500, 64, 1024),
+                                          (8191, 1000, 4096), (8191, 4096, 1000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_projections_of_large_and_small_tiles(n, dim, outs, dtype):
+    """Sizes at which a product has tiles of either size, several a workgroup,
+    or shares of its steps: a sample of the cells, in 64 bits."""
+    rng = np.random.default_rng(n + outs)
+    x, w, g = rows(rng, n, dim, dtype), rows(rng, outs, dim, dtype, 0.1), rows(rng, n, outs, dtype, 1.0 / n)
+    b = f32(rng, outs)
+    y, dx, dw, db = like((n, outs), dtype), like((n, dim), dtype), like((outs, dim), dtype), like(outs, "float32")
+    hb.linear(dev(x, dtype), dev(w, dtype), y, bias=dev(b, "float32"), workspace=work(hb.linear_workspace(n, outs, dim, dtype)))
+    hb.linear_grad(dev(g, dtype), dev(w, dtype), x=dev(x, dtype), dx=dx, dw=dw, db=db, workspace=work(hb.linear_grad_workspace(n, outs, dim, dtype)))
+    some = np.unique(np.r_[0, n - 1, rng.integers(0, n, 40)])
+    value, off = L.linear(x[some], w, b, None, None, None, None, dtype)
+    close(back(y)[some], (value, off), "y")
+    value, off = L.linear_grad(g[some], w, None, None, dtype)["dx"]
+    close(back(dx)[some], (value, off), "dx")
+    few = np.unique(np.r_[0, outs - 1, rng.integers(0, outs, 40)])
+    want = L.linear_grad(np.ascontiguousarray(g[:, few]), None, x, None, dtype)
+    close(back(dw)[few], want["dw"], "dw")
+    close(back(db), L.linear_grad(g, None, None, None, dtype)["db"], "db")
+
+
+# ---- a training step of all of them ----------------------------------------------------------
+
+
+class Layers:
+    """One step of a model on leaves with a layer in its middle: look-up, norm
+    with its checkpoint, projection, head, and all gradients back to the table."""
+
+    def __init__(self, dtype, seed, n=500, columns=6, table=31, dim=40, outs=72, classes=130):
+        rng = np.random.default_rng(seed)
+        self.dtype, self.n = dtype, n
+        self.v = dict(ids=rng.integers(0, table, (n, columns)).astype(np.int32), off=(np.arange(columns) * table).astype(np.int32),
+                      table=rows(rng, table * columns, dim, dtype, 0.3), residual=rows(rng, n, dim, dtype), weight=f32(rng, dim, 0.2, 1.0),
+                      w=rows(rng, outs, dim, dtype, 0.15), bias=f32(rng, outs, 0.1), head=rows(rng, classes, outs, dtype, 0.2),
+                      y=rng.integers(-1, classes, n).astype(np.int32))
+        kinds = dict(ids="int32", off="int32", y="int32", weight="float32", bias="float32")
+        self.inputs = {k: dev(a, kinds.get(k, dtype)) for k, a in self.v.items()}
+        new = lambda *s: like(s, dtype)
+        self.h, self.total, self.out, self.z = new(n, dim), new(n, dim), new(n, dim), new(n, outs)
+        self.inv, self.loss = like(n, "float32"), like(n, "float32")
+        self.codes, self.scales = packed_like(n, dim)
+        self.dz, self.dhead, self.dout, self.dw, self.dh, self.dtable = new(n, outs), new(classes, outs), new(n, dim), new(outs, dim), new(n, dim), new(table * columns, dim)
+        self.db, self.dweight, self.norm = like(outs, "float32"), like(dim, "float32"), like(1, "float32")
+        self.ws = [work(b) for b in (hb.linear_workspace(n, outs, dim, dtype), hb.softmax_head_workspace(n, classes, outs, dtype),
+                                     hb.linear_grad_workspace(n, outs, dim, dtype), hb.rms_norm_grad_workspace(n, dim, dtype),
+                                     hb.leaf_embedding_grad_workspace(n, columns, table * columns, dim, dtype), hb.clip_gradients_workspace(5))]
+
+    def run(self, stream=None):
+        i, kw = self.inputs, dict(stream=stream)
+        hb.leaf_embedding(i["table"], i["ids"], self.h, offset=i["off"], **kw)
+        hb.rms_norm(self.h, self.out, weight=i["weight"], residual=i["residual"], total=self.total, inv=self.inv, codes=self.codes,
+                    scales=self.scales, normed=True, **kw)
+        hb.linear(self.out, i["w"], self.z, bias=i["bias"], workspace=self.ws[0], **kw)
+        hb.softmax_head(self.z, i["head"], labels=i["y"], loss=self.loss, dh=self.dz, dw=self.dhead, grad_scale=1.0 / self.n,
+                        workspace=self.ws[1], **kw)
+        hb.linear_grad(self.dz, i["w"], codes=self.codes, scales=self.scales, weight=i["weight"], dx=self.dout, dw=self.dw, db=self.db,
+                       workspace=self.ws[2], **kw)
+        hb.rms_norm_grad(self.dout, self.dh, codes=self.codes, scales=self.scales, inv=self.inv, weight=i["weight"], dweight=self.dweight,
+                         workspace=self.ws[3], **kw)
+        hb.leaf_embedding_grad(self.dh, i["ids"], self.dtable, offset=i["off"], workspace=self.ws[4], **kw)
+        hb.clip_gradients([self.dtable, self.dw, self.db, self.dweight, self.dhead], 0.01, norm=self.norm, workspace=self.ws[5], **kw)
+
+    def outputs(self):
+        return [back(a) for a in (self.total, self.z, self.loss, self.dw, self.db, self.dweight, self.dhead, self.dtable, self.norm)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_of_layers_runs_through_all_of_them(dtype):
+    """Every call against its plain form on what the call before it gave."""
+    s = Layers(dtype, 3)
+    s.run()
+    v = s.v
+    h = back(s.h)
+    close(h, R.embedding(v["table"], v["ids"], v["off"], None, dtype), "h")
+    want = L.norm(h, v["residual"], v["weight"], float(np.float32(1e-6)), dtype)
+    for name, a in (("out", s.out), ("total", s.total), ("inv", s.inv)):
+        close(back(a), want[name], name)
+    close(back(s.z), L.linear(back(s.out), v["w"], v["bias"], None, None, None, None, dtype), "z")
+    want = R.head(back(s.z), v["head"], None, v["y"], None, float(np.float32(1 / s.n)), dtype)
+    close(back(s.loss), want["loss"], "loss")
+    close(back(s.dz), want["dh"], "dz")
+    held = L.values_of(bytes_back(s.codes), bytes_back(s.scales))
+    want = L.linear_grad(back(s.dz), v["w"], held, v["weight"], dtype)
+    close(back(s.dout), want["dx"], "dout")
+    last = L.norm_grad(back(s.dout), held, back(s.inv), v["weight"], None, 0.0, True, dtype)
+    close(back(s.dh), last["dx"], "dh")
+    table = R.embedding_grad(back(s.dh), v["ids"], v["off"], None, len(v["table"]), dtype)
+    full = [table, want["dw"], want["db"], last["dweight"], R.head(back(s.z), v["head"], None, v["y"], None, float(np.float32(1 / s.n)), dtype)["dw"]]
+    true = np.sqrt(sum(np.sum(a * a) for a, _ in full))
+    slack = np.sqrt(sum(np.sum(e * e) for _, e in full))
+    assert true > 0.01 and abs(back(s.norm)[0] - true) <= slack + 2 * R.EPS32 * true
+    by = 0.01 / (true + 1e-6)
+    for a, (x, e), t in zip((s.dtable, s.dw, s.db, s.dweight, s.dhead), full, (dtype, dtype, "float32", "float32", dtype)):
+        close(back(a), (x * by, (e + np.abs(x) * (slack / true + 6 * R.EPS32)) * by * 1.01 + R.HALF[t] * 1.01 * (np.abs(x) + e) * by + 1e-38))
+
+
+def test_layers_on_several_streams_give_the_same_bits():
+    H = hip()
+    sizes = [("bfloat16", 21, {}), ("bfloat16", 22, dict(n=900, dim=264, outs=300)), ("float32", 23, {}), ("float32", 24, dict(n=30, dim=33, outs=17))]
+    want = []
+    for dtype, seed, kw in sizes:
+        s = Layers(dtype, seed, **kw)
+        s.run()
+        want.append(s.outputs())
+    again, streams = [Layers(dtype, seed, **kw) for dtype, seed, kw in sizes], []
+    for _ in again:
+        st = C.c_void_p()
+        ok(H.hipStreamCreateWithFlags(C.byref(st), 1))
+        streams.append(st)
+    for _ in range(3):
+        for s, st in zip(again, streams):
+            s.run(st.value)
+    ok(H.hipDeviceSynchronize())
+    for s, w in zip(again, want):
+        for a, b in zip(s.outputs(), w):
+            assert np.array_equal(a, b)
+    for st in streams:
+        ok(H.hipStreamDestroy(st))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_captured_layers_replay_with_the_eager_bits(dtype):
+    """Captured once; replayed on other inputs with eager work between."""
+    H = hip()
+    st = C.c_void_p()
+    ok(H.hipStreamCreateWithFlags(C.byref(st), 1))
+    s, other = Layers(dtype, 31), Layers(dtype, 32)
+    other.run()
+    ok(H.hipStreamBeginCapture(st, 2))
+    s.run(st.value)
+    graph, run = C.c_void_p(), C.c_void_p()
+    ok(H.hipStreamEndCapture(st, C.byref(graph)))
+    ok(H.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)))
+    for seed in (31, 41, 42, 31):
+        t = Layers(dtype, seed)
+        for k, a in s.inputs.items():
+            a.buffer.copy_from(t.inputs[k].buffer)
+        ok(H.hipDeviceSynchronize())
+        ok(H.hipGraphLaunch(run, st))
+        ok(H.hipStreamSynchronize(st))
+        got = s.outputs()
+        t.run()
+        for a, b in zip(got, t.outputs()):
+            assert np.array_equal(a, b)
+        other.run()
+    ok(H.hipGraphExecDestroy(run))
+    ok(H.hipGraphDestroy(graph))
+    ok(H.hipStreamDestroy(st))
+
+
+TORCH = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import hessboost_amd as hb
+
+torch.manual_seed(0)
+n, dim, outs, rank, adapters = 300, 96, 200, 8, 5
+for dtype in (torch.float32, torch.bfloat16):
+    r = lambda *s: torch.randn(*s, device="cuda").to(dtype)
+    x, res, w, dout = r(n, dim), r(n, dim), r(outs, dim), r(n, outs)
+    weight, bias, scale = torch.rand(dim, device="cuda") + 0.5, torch.randn(outs, device="cuda"), torch.rand(adapters, device="cuda")
+    down, up = r(adapters, rank, dim), r(adapters, outs, rank)
+    ids = torch.randint(-1, adapters, (n,), device="cuda", dtype=torch.int32)
+    names = ("out", "total", "y", "dx", "dw", "db", "dres", "dweight", "held")
+
+    def step():
+        got = dict(out=torch.empty_like(x), total=torch.empty_like(x), y=torch.empty(n, outs, device="cuda", dtype=dtype), dx=torch.empty_like(x),
+                   dw=torch.empty_like(w), db=torch.empty(outs, device="cuda"), dres=torch.empty_like(x), dweight=torch.empty_like(weight),
+                   held=torch.empty(n, dim, device="cuda", dtype=torch.bfloat16))
+        inv = torch.empty(n, device="cuda")
+        codes = torch.empty(n, dim, device="cuda", dtype=torch.float8_e4m3fn)
+        scales = torch.empty(n, hb.packed_scales(dim), device="cuda", dtype=torch.uint8)
+        ws = lambda b: torch.empty(max(16, b), dtype=torch.uint8, device="cuda")
+        hb.rms_norm(x, got["out"], weight=weight, residual=res, total=got["total"], inv=inv, codes=codes, scales=scales, normed=True)
+        hb.unpack_rows(codes, scales, got["held"])
+        hb.linear(got["out"], w, got["y"], bias=bias, down=down, up=up, ids=ids, scale=scale, workspace=ws(hb.linear_workspace(n, outs, dim, dtype, rank=rank)))
+        hb.linear_grad(dout, w, codes=codes.view(torch.uint8), scales=scales, weight=weight, dx=got["dx"], dw=got["dw"], db=got["db"],
+                       workspace=ws(hb.linear_grad_workspace(n, outs, dim, dtype)))
+        hb.rms_norm_grad(got["dx"], got["dres"], codes=codes, scales=scales, inv=inv, weight=weight, dtotal=res, dweight=got["dweight"],
+                         workspace=ws(hb.rms_norm_grad_workspace(n, dim, dtype)))
+        return got
+
+    eager = step()
+    torch.cuda.synchronize()
+    t = (x.double() + res.double())
+    nn = t * (t.square().mean(1, keepdim=True) + 1e-6).rsqrt()
+    assert (eager["out"].double() - nn * weight.double()).abs().max() < 0.05
+    assert ((eager["held"].double() - nn).abs() <= nn.abs() / 16 + 0.01).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # the tensors' stream by default: torch's current one
+        there = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(there[k], eager[k]) for k in names)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    for seed in range(3):
+        for a in (x, res, dout, down):
+            a.copy_(r(*a.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        mine = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(kept[k], mine[k]) for k in names), seed
+    # rows of views, and adapters whose rows lie apart
+    wide = torch.full((n, 2 * outs), float("nan"), device="cuda", dtype=dtype)
+    spread = torch.zeros(adapters, rank, 2 * dim, device="cuda", dtype=dtype)
+    spread[:, :, :dim] = down
+    hb.linear(kept["out"], w, wide[:, :outs], bias=bias, down=spread[:, :, :dim], up=up, ids=ids, scale=scale,
+              workspace=torch.empty(hb.linear_workspace(n, outs, dim, dtype, rank=rank), dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(wide[:, :outs], kept["y"]) and torch.isnan(wide[:, outs:]).all()
+    try:
+        hb.linear(x, w, kept["y"], down=down.transpose(0, 1).contiguous().transpose(0, 1), up=up, ids=ids)
+        raise SystemExit("adapters of two strides were taken")
+    except ValueError:
+        pass
+print("torch layers ok", flush=True)
+"""
+
+
+def test_torch_tensors_of_layers_are_taken_on_their_stream():
+    """In a process of its own: torch brings its own HIP runtime."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = TORCH.replace("{root!r}", repr(os.path.dirname(here))).replace("{tests!r}", repr(here))
+    r = subprocess.run([sys.executable, "-u", "-c", code], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "torch layers ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
