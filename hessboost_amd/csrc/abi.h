@@ -1419,6 +1419,13 @@ struct LinearFewArgs {
     uint32_t n_rows, dim, outs, rank, adapters, pad;
 };
 
+// dst[column] = the sum of part[.][column], in order within shares and over them.
+struct ColumnJoinArgs {
+    const float *part;
+    float *dst;
+    uint32_t parts, cols;
+};
+
 // part[share][column] = the sums of the share's rows.
 struct ColumnSumArgs {
     const void *x;

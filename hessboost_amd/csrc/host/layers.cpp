@@ -196,7 +196,13 @@ void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *work
         queue.launch((kernel_of("hbr_rms_norm_grad", p.dtype, v) + "_" + std::to_string(q.held)).c_str(), dim3((uint32_t)blocks),
                      dim3(q.threads), a);
     }
-    if (p.dweight) sum_parts(queue, HBR_F32, 1.0f, static_cast<const float *>(workspace), blocks, dim, p.dweight, 1, dim, dim);
+    if (!p.dweight) return;
+    ColumnJoinArgs j{};
+    j.part = static_cast<const float *>(workspace);
+    j.dst = p.dweight;
+    j.parts = (uint32_t)blocks;
+    j.cols = p.dim;
+    queue.launch("hbr_column_join", dim3((uint32_t)tiles(dim, 16)), dim3(1024), j);
 }
 
 // ---- rows in 8 bits -------------------------------------------------------------------
@@ -535,7 +541,7 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
     a.up_stride = up_rows.stride;
     a.rank = p.rank;
     a.adapters = p.n_adapters;
-    run_product(queue, "hbr_linear_y_" + (a.part ? "part" : type), q.product, a);
+    run_product(queue, a.part ? "hbr_linear_y_part" : (rank ? "hbr_linear_ya_" : "hbr_linear_y_") + type, q.product, a);
     Joins joins;
     joins.add(q.product, a);
     joins.launch(queue, type);

@@ -145,8 +145,6 @@ struct Adapters {
     bool eights, wide;
 
     __device__ __forceinline__ Adapters(const LinearArgs &a, const Tile &t) {
-        all = 0;
-        if (!a.low) return;
         const uint32_t tile = t.n0 / Tile::kN;
         all = uniform(a.slots[tile]) * a.rank;
         slot_id = a.slot_id + (uint64_t)tile * Tile::kN;
@@ -344,11 +342,26 @@ __device__ __forceinline__ void linear_tiles(const LinearArgs &a, char *lds, uin
 
 template <typename Tile, typename E>
 struct LinearY {
+    Columns<Tile> bias;
+    __device__ __forceinline__ LinearY(const LinearArgs &a, const Tile &t) { bias.read(t, a.bias, a.cols, 0.0f); }
+    __device__ __forceinline__ NothingElse beside() { return {}; }
+    __device__ __forceinline__ void behind(const LinearArgs &, char *, Tile &) {}
+    __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) { linear_store<Tile, E, false>(a, room, t, bias); }
+};
+
+// With adapters, whose operands take the registers that fragments had: the biases
+// are read with them, behind the products. (The first step's operands read before
+// the products spilled: 98 us against 83, 8,191 rows of 1,024 by 4,096.)
+template <typename Tile, typename E>
+struct LinearYa {
     Adapters<Tile, E> adapters;
     Columns<Tile> bias;
-    __device__ __forceinline__ LinearY(const LinearArgs &a, const Tile &t) : adapters(a, t) { bias.read(t, a.bias, a.cols, 0.0f); }
+    __device__ __forceinline__ LinearYa(const LinearArgs &a, const Tile &t) : adapters(a, t) {}
     __device__ __forceinline__ NothingElse beside() { return {}; }
-    __device__ __forceinline__ void behind(const LinearArgs &a, char *lds, Tile &t) { adapters.add(a, lds, t); }
+    __device__ __forceinline__ void behind(const LinearArgs &a, char *lds, Tile &t) {
+        bias.read(t, a.bias, a.cols, 0.0f);
+        adapters.add(a, lds, t);
+    }
     __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) { linear_store<Tile, E, false>(a, room, t, bias); }
 };
 
@@ -513,20 +526,21 @@ __device__ __forceinline__ void linear_join(const LinearArgs &a, uint32_t block)
         if (c + k < a.cols) to[k] = v.v[k];
 }
 
-// db's parts joined: 16 columns a workgroup, a thread a column and a sixteenth of the parts.
-__device__ __forceinline__ void linear_join_db(const LinearPairArgs &a, uint32_t block) {
-    __shared__ float sum_of[16][16];
+// Columns' parts joined: 16 columns a workgroup, a thread a column and a share of the parts.
+template <uint32_t Shares>
+__device__ __forceinline__ void column_join(const float *part, uint32_t parts, uint32_t cols, float *dst, uint32_t block) {
+    __shared__ float sum_of[Shares][16];
     const uint32_t in = threadIdx.x % 16, share = threadIdx.x / 16, c = block * 16 + in;
     float s = 0.0f;
-    if (c < a.outs) {
-#pragma unroll 4
-        for (uint32_t p = share; p < a.b_parts; p += 16) s += a.part_b[(uint64_t)p * a.outs + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (uint32_t p = share; p < parts; p += Shares) s += part[(uint64_t)p * cols + c];
     }
     sum_of[share][in] = s;
     __syncthreads();
-    if (share || c >= a.outs) return;
-    for (uint32_t w = 1; w < 16; w++) s += sum_of[w][in];
-    a.db[c] = s;
+    if (share || c >= cols) return;
+    for (uint32_t w = 1; w < Shares; w++) s += sum_of[w][in];
+    dst[c] = s;
 }
 
 // Either product's shares, by its tile, and db.
@@ -542,7 +556,7 @@ __device__ __forceinline__ void linear_joins(const LinearPairArgs &a) {
         }
         block -= a.groups[i];
     }
-    linear_join_db(a, block);
+    column_join<16>(a.part_b, a.b_parts, a.outs, a.db, block);
 }
 
 // Operands laid out in chunks: eight columns of a row a thread, a wave eight rows
@@ -664,7 +678,7 @@ template <typename E, bool Wide, uint32_t kWaves>
 __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     using T = typename E::type;
     using S = Strip<E, Wide>;
-    constexpr uint32_t kRows = 16, kCols = 2, kAhead = kWaves == 4 ? 4 : 2;
+    constexpr uint32_t kRows = 16, kCols = 2, kAhead = kWaves == 4 ? sizeof(T) == 2 && Wide ? 8 : 4 : 2;
     __shared__ int32_t slot_id[kRows], slot_of[kRows];
     __shared__ f32x4 part[kWaves][kCols][kWave];
     if (blockIdx.x >= a.groups * a.shares) {
@@ -678,13 +692,20 @@ __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     const uint32_t share = blockIdx.x / a.groups;
     const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, in = lane % 16, quarter = lane / 16;
     const uint64_t r0 = (uint64_t)(blockIdx.x % a.groups) * kRows;
-    // every wave finds the slots: the rows' adapters in order of their first rows
+    const T *x = static_cast<const T *>(a.x) + min(r0 + in, (uint64_t)a.n_rows - 1) * a.x_stride;
     int32_t id = r0 + in < a.n_rows ? a.ids[r0 + in] : -1;
+    Vec<T, S::kV> fx[kAhead];  // of the rows' first steps, which wait for no id
+    auto read_x = [&](uint32_t c0) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) fx[k] = S::load(x, c0 + k * S::kStep + quarter * S::kV, a.dim);
+    };
+    read_x(wave * kAhead * S::kStep);
+    // every wave finds the slots: the rows' adapters in order of their first rows
     if (id < 0 || (uint32_t)id >= a.adapters) id = -1;
     uint32_t first = in;
 #pragma unroll
     for (int o = kRows - 1; o >= 0; o--)
-        if (__shfl(id, o, kWave) == id) first = min(first, (uint32_t)o);
+        if (__builtin_amdgcn_readlane(id, o) == id) first = min(first, (uint32_t)o);
     const uint64_t firsts = __ballot(lane < kRows && id >= 0 && first == in);
     const uint32_t slots = (uint32_t)__popcll(firsts), slot = (uint32_t)__popcll(firsts & ((1ull << first) - 1));
     if (wave == 0 && lane < kRows) {
@@ -693,7 +714,7 @@ __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
     }
     __syncthreads();
     const uint32_t all = slots * a.rank;
-    const T *x = static_cast<const T *>(a.x) + min(r0 + in, (uint64_t)a.n_rows - 1) * a.x_stride;
+    bool fresh = true;  // fx holds the wave's first steps
     for (uint32_t v0 = share * kCols * 16; v0 < all; v0 += a.shares * kCols * 16) {
         const T *down[kCols];
 #pragma unroll
@@ -703,11 +724,12 @@ __device__ __forceinline__ void linear_low(const LinearLowArgs &a) {
         }
         f32x4 acc[kCols] = {};
         for (uint32_t c0 = wave * kAhead * S::kStep; c0 < a.dim; c0 += kWaves * kAhead * S::kStep) {
-            Vec<T, S::kV> fx[kAhead], fd[kAhead][kCols];
+            Vec<T, S::kV> fd[kAhead][kCols];
+            if (!fresh) read_x(c0);
+            fresh = false;
 #pragma unroll
             for (uint32_t k = 0; k < kAhead; k++) {
                 const uint32_t c = c0 + k * S::kStep + quarter * S::kV;
-                fx[k] = S::load(x, c, a.dim);
 #pragma unroll
                 for (uint32_t q = 0; q < kCols; q++) fd[k][q] = S::load(down[q], c, a.dim);
             }
@@ -824,6 +846,8 @@ using namespace hbr;
 #define HBR_LINEARS(suffix, Tile, waves)                                                             \
     HBR_LINEAR(hbr_linear_y_f32_##suffix, Tile, waves, false, false, LinearY<Tile, F32>)             \
     HBR_LINEAR(hbr_linear_y_bf16_##suffix, Tile, waves, false, false, LinearY<Tile, Bf16>)           \
+    HBR_LINEAR(hbr_linear_ya_f32_##suffix, Tile, waves, false, false, LinearYa<Tile, F32>)           \
+    HBR_LINEAR(hbr_linear_ya_bf16_##suffix, Tile, waves, false, false, LinearYa<Tile, Bf16>)         \
     HBR_LINEAR(hbr_linear_y_part_##suffix, Tile, waves, false, false, LinearPart<Tile>)              \
     HBR_LINEAR(hbr_linear_dx_f32_##suffix, Tile, waves, true, false, LinearDx<Tile, F32>)            \
     HBR_LINEAR(hbr_linear_dx_bf16_##suffix, Tile, waves, true, false, LinearDx<Tile, Bf16>)          \
@@ -857,5 +881,6 @@ HBR_STRIPS(f32, F32, 4, true)
 HBR_STRIPS(bf16, Bf16, 1, false)
 HBR_STRIPS(bf16, Bf16, 8, true)
 extern "C" __global__ __launch_bounds__(256) void hbr_lay(LayArgs a) { lay_all(a, blockIdx.x); }
+extern "C" __global__ __launch_bounds__(1024) void hbr_column_join(ColumnJoinArgs a) { column_join<64>(a.part, a.parts, a.cols, a.dst, blockIdx.x); }
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_f32(ColumnSumArgs a) { column_sum<F32>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_column_sum_bf16(ColumnSumArgs a) { column_sum<Bf16>(a); }
