@@ -40,6 +40,15 @@ uint32_t rows_vector(uint64_t size, uint64_t dim, std::initializer_list<const Ro
     return v;
 }
 
+// The rows' kernels take vectors of 16 bytes wherever they lie and let a row's
+// last one reach back (65,537 rows of 1,023 bf16: norm 203 us and its gradient
+// 183, element by element 542 and 444), and rows shorter than a vector element
+// by element.
+uint32_t row_vector(uint64_t size, uint64_t dim) { return dim >= 16 / size ? (uint32_t)(16 / size) : 1; }
+// Rows of f32 that are whole vectors of 8 bytes only: 161,579 rows of 310 took
+// 174 us, and 197 by vectors of 16 that reach back.
+uint32_t norm_vector(uint64_t size, uint64_t dim) { return size == 4 && dim % 4 == 2 ? 2 : row_vector(size, dim); }
+
 uint64_t scales_of(uint64_t dim) { return tiles(dim, kPackBlock); }
 
 uint32_t power_of_two(uint64_t n) {
@@ -49,21 +58,26 @@ uint32_t power_of_two(uint64_t n) {
 }
 
 // A row's lanes and its vectors a lane: a wave or less of a workgroup of 256,
-// else the whole of one; 0 vectors where the registers hold no row.
+// else the whole of one; 0 vectors where the registers hold no row. `most`
+// vectors a lane: what 128 registers hold of the kernel's arrays.
 struct RowPlan {
     uint32_t lanes, held, threads;
     uint64_t per() const { return threads / lanes; }  // rows a workgroup
+    std::string name() const { return "_" + std::to_string(held); }
 };
-RowPlan row_plan(uint64_t vecs, uint32_t v, bool codes) {
-    const uint32_t most = v == 8 ? 2 : 4;
+RowPlan row_plan(uint64_t vecs, uint32_t v, uint32_t most, bool codes) {
     const uint64_t least = std::max<uint64_t>(vecs, codes ? kPackBlock / v : 1);
     if (least <= kWaveLanes) return {power_of_two(least), 1, 256};
     for (uint32_t held = 2; held <= most; held *= 2)
         if (vecs <= kWaveLanes * held) return {kWaveLanes, held, 256};
-    for (uint32_t threads = 256; threads <= 1024; threads *= 2)
-        for (uint32_t held = most / 2; held <= most; held *= 2)
-            if (vecs <= threads * held) return {threads, held, threads};
+    for (uint32_t threads = most == 2 ? 128 : 256; threads <= 1024; threads *= 2)
+        if (vecs <= threads * 2) return {threads, 2, threads};
     return {1024, 0, 1024};
+}
+
+// (rows of other than whole vectors have kernels of their own)
+std::string rows_kernel(const char *name, uint32_t dtype, uint32_t v, uint64_t dim) {
+    return std::string(name) + "_" + name_of(dtype) + "_" + std::to_string(v) + (dim % v ? "r" : "");
 }
 
 std::string kernel_of(const char *name, uint32_t dtype, uint32_t v) {
@@ -96,9 +110,8 @@ void rms_norm(int ordinal, void *stream, const hbr_norm &p) {
     check_apart({out.extent(), total.extent(), codes.extent(), scales.extent(), {p.inv, n * 4}},
                 {apart(x), apart(residual), {p.weight, dim * 4}}, Extent(nullptr, 0), what);
     Queue queue(ordinal, stream);
-    const Rows weight(p.weight, 1, dim, dim, 4, what);
-    const uint32_t v = rows_vector(size, dim, {&x, &residual, &out, &total, &codes, &weight});
-    const RowPlan q = row_plan(dim / v, v, p.codes != nullptr);
+    const uint32_t v = norm_vector(size, dim);
+    const RowPlan q = row_plan(tiles(dim, v), v, v == 8 ? 2 : 4, p.codes != nullptr);
     NormArgs a{};
     a.x = p.x;
     a.residual = p.residual;
@@ -116,12 +129,12 @@ void rms_norm(int ordinal, void *stream, const hbr_norm &p) {
     a.scales_stride = scales.stride;
     a.n_rows = n;
     a.dim = p.dim;
-    a.vecs = p.dim / v;
+    a.vecs = (uint32_t)tiles(dim, v);
     a.lanes = q.lanes;
     a.eps = p.eps;
     a.mean = 1.0f / (float)p.dim;
     a.normed = p.normed;
-    queue.launch((kernel_of("hbr_rms_norm", p.dtype, v) + "_" + std::to_string(q.held)).c_str(),
+    queue.launch((rows_kernel("hbr_rms_norm", p.dtype, v, dim) + q.name()).c_str(),
                  dim3((uint32_t)std::min<uint64_t>(tiles(n, q.per()), 2048 * 256 / q.threads)), dim3(q.threads), a);
 }
 
@@ -167,9 +180,9 @@ void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *work
     Queue queue(ordinal, stream);
     uint64_t blocks = 0;
     if (n) {
-        const Rows weight(p.weight, 1, dim, dim, 4, what);
-        const uint32_t v = rows_vector(size, dim, {&dout, &x, &codes, &dtotal, &dx, &weight});
-        const RowPlan q = row_plan(dim / v, v, false);
+        const uint32_t v = norm_vector(size, dim);
+        // (4 that reach back spill: 65,537 rows of 1,023 f32 356 us, with 2 326)
+        const RowPlan q = row_plan(tiles(dim, v), v, v == 8 || dim % v ? 2 : 4, false);
         blocks = std::min(tiles(n, q.per()), norm_grad_blocks(dim));
         NormGradArgs a{};
         a.dout = p.dout;
@@ -189,11 +202,11 @@ void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *work
         a.dx_stride = dx.stride;
         a.n_rows = n;
         a.dim = p.dim;
-        a.vecs = p.dim / v;
+        a.vecs = (uint32_t)tiles(dim, v);
         a.lanes = q.lanes;
         a.eps = p.eps;
         a.mean = 1.0f / (float)p.dim;
-        queue.launch((kernel_of("hbr_rms_norm_grad", p.dtype, v) + "_" + std::to_string(q.held)).c_str(), dim3((uint32_t)blocks),
+        queue.launch((rows_kernel("hbr_rms_norm_grad", p.dtype, v, dim) + q.name()).c_str(), dim3((uint32_t)blocks),
                      dim3(q.threads), a);
     }
     if (!p.dweight) return;
@@ -220,7 +233,7 @@ void packed(int ordinal, void *stream, const hbr_packed &p, const void *x, const
     if (pack) check_apart({rc.extent(), rs.extent()}, {rx.extent()}, Extent(nullptr, 0), what);
     else check_apart({rx.extent()}, {rc.extent(), rs.extent(), rw.extent()}, Extent(nullptr, 0), what);
     Queue queue(ordinal, stream);
-    const uint32_t v = rows_vector(size, dim, {&rx, &rc, &rw});
+    const uint32_t v = row_vector(size, dim);
     PackArgs a{};
     a.x = const_cast<void *>(x);
     a.codes = const_cast<uint8_t *>(codes);
@@ -231,10 +244,10 @@ void packed(int ordinal, void *stream, const hbr_packed &p, const void *x, const
     a.scales_stride = rs.stride;
     a.n_rows = n;
     a.dim = p.dim;
-    a.vecs = p.dim / v;
+    a.vecs = (uint32_t)tiles(dim, v);
     a.lanes = power_of_two(std::min<uint64_t>(kWaveLanes, std::max(a.vecs, kPackBlock / v)));
     a.each = 8;
-    queue.launch(kernel_of(pack ? "hbr_pack" : "hbr_unpack", p.dtype, v).c_str(),
+    queue.launch(rows_kernel(pack ? "hbr_pack" : "hbr_unpack", p.dtype, v, dim).c_str(),
                  dim3((uint32_t)std::min<uint64_t>(tiles(n, 256 / a.lanes), 1u << 16), (uint32_t)tiles(up(a.vecs, 32), a.lanes * a.each)),
                  dim3(256), a);
 }
