@@ -119,7 +119,7 @@ NORMS = [(1, 1, False, False, 0, 0), (3, 5, True, True, 0, 0), (65, 32, True, Fa
          (33, 64, True, True, 8, 8), (7, 129, True, True, 1, 1), (5, 512, False, True, 0, 0), (9, 1000, True, True, 2, 2),
          (130, 1024, True, True, 0, 0), (4, 1500, True, False, 4, 0), (3, 2049, False, True, 0, 0), (3, 4096, True, True, 0, 0),
          (2, 5001, True, True, 0, 3), (2, 8200, False, True, 0, 0), (2, 17_000, True, True, 0, 0), (1, 40_000, True, True, 8, 8),
-         (2, 33_333, True, True, 1, 0)]
+         (2, 33_333, True, True, 1, 0), (40, 310, True, True, 1, 1), (6, 10, True, True, 1, 1), (4, 1022, True, True, 1, 1)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -161,7 +161,7 @@ def test_norms(n, dim, residual, weight, pad, lead, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("dim", [50, 1024, 40_000])
+@pytest.mark.parametrize("dim", [50, 1003, 1024, 9001, 40_000, 40_003])
 def test_norms_in_place(dim, dtype):
     rng = np.random.default_rng(dim)
     n = 5
@@ -219,7 +219,8 @@ def test_norms_of_values_that_are_no_numbers_stay_in_their_rows():
 GRADS = [(1, 1, False, False, 0, 0), (3, 5, True, True, 0, 0), (65, 32, True, False, 0, 0), (2000, 50, False, True, 0, 0),
          (33, 64, True, True, 8, 8), (7, 129, True, True, 1, 1), (9, 1000, True, True, 2, 2), (700, 1024, True, True, 0, 0),
          (4, 1500, True, False, 4, 0), (3, 2049, False, True, 0, 0), (3, 4096, True, True, 0, 0), (2, 9000, False, True, 0, 0),
-         (3, 40_000, True, True, 8, 8), (1030, 33_333 // 8, True, True, 1, 0)]
+         (3, 40_000, True, True, 8, 8), (1030, 33_333 // 8, True, True, 1, 0),
+         (5, 10, True, True, 1, 1), (40, 310, True, True, 1, 1), (2, 8193, True, True, 1, 0), (3, 20_003, True, True, 3, 1)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
