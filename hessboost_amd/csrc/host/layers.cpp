@@ -459,7 +459,7 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
     if (rank >= kDimLimit) fail(kRefused, std::string(what) + ": adapters of rank 1,048,576 or more");
     if (p.n_adapters > 0x7fffffffu) fail(kRefused, std::string(what) + ": more than 2^31 - 1 adapters");
     check_tiles(n, outs, what);
-    if (rank && n >= 1u << 28) fail(kRefused, std::string(what) + ": adapters of 2^28 rows or more");
+    if (rank && n >= 1u << 27) fail(kRefused, std::string(what) + ": adapters of 2^27 rows or more");
     if (n == 0) return;
     if (!p.x || !p.w || !p.out) fail(kInvalid, std::string(what) + ": null argument");
     if (rank && (!p.down || !p.up || !p.ids)) fail(kInvalid, std::string(what) + ": adapters need down, up and ids");

@@ -131,6 +131,12 @@ __device__ __forceinline__ void linear_store_part(const LinearArgs &a, Tile &t) 
 //
 // In bf16 the low values are rounded once to bf16, as any product's operand
 // is: half a step each of the adapters' part. In f32 all is in three parts.
+//
+// An adapter is its own rows' alone: an element of `up` that is no finite number
+// would make no number of the others' zeros, so it is taken as zero, and a tile
+// that met one goes over its adapters twice more, with a product of the largest
+// numbers where a row's own adapter has such an element, added and taken off:
+// infinity less infinity there, zero everywhere else.
 template <typename Tile, typename E>
 struct Adapters {
     using T = typename E::type;
@@ -140,6 +146,7 @@ struct Adapters {
     static constexpr int kPieces = kM * kIn / Tile::kThreads;  // of eight products of a row, of either operand
     static_assert(Tile::kM == Tile::kN && kM * kIn % Tile::kThreads == 0, "as many pieces of each a thread");
     static_assert(4 * kParts * kPart <= (uint32_t)Tile::kLds, "two steps fit the stages");
+    static_assert(Tile::kThreads == 4 * kWave, "four waves' flags");
     uint32_t all, own[kPieces];
     const int32_t *slot_id;
     bool eights, wide;
@@ -153,6 +160,17 @@ struct Adapters {
 #pragma unroll
         for (int q = 0; q < kPieces; q++) own[q] = a.slot_of[min(t.n0 + (q * Tile::kThreads + threadIdx.x) / kIn, a.rows - 1)];
     }
+    // Whether any of eight elements is no finite number: their exponents, two at a
+    // time in 16 bits, carried into the sign's place.
+    static __device__ __forceinline__ bool not_finite(const Vec<T, 8> &v) {
+        constexpr uint32_t kExponents = sizeof(T) == 4 ? 0x7f800000u : 0x7f807f80u, kOne = sizeof(T) == 4 ? 0x00800000u : 0x00800080u;
+        const auto words = __builtin_bit_cast(Vec<uint32_t, 2 * sizeof(T)>, v);
+        uint32_t carried = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 2 * sizeof(T); i++) carried |= (words.v[i] & kExponents) + kOne;
+        return (carried & ~kExponents & (kExponents << 1)) != 0;
+    }
+    static __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
     // Every load is made, from within its array, and what does not count is zeroed.
     __device__ __forceinline__ void read(const LinearArgs &a, const Tile &t, uint32_t k0, float (&low)[kPieces][8], Vec<T, 8> (&up)[kPieces]) {
 #pragma unroll
@@ -216,20 +234,45 @@ struct Adapters {
 #pragma unroll
         for (int q = 0; q < kParts; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(to + q * kPart) = out[q];
     }
-    __device__ __forceinline__ void add(const LinearArgs &a, char *stages, Tile &t) {
+    // What stands in the operands' places of the passes behind the first: the
+    // largest bf16, whose square f32 does not hold.
+    static constexpr float kLargest = 0x1.fep127f;
+    __device__ __forceinline__ void mark(const LinearArgs &a, const Tile &t, uint32_t k0, int q, float sign, float (&low)[8], float (&up)[8]) {
+        const uint32_t at = q * Tile::kThreads + threadIdx.x, row = at / kIn;
+        const uint64_t out = min(t.m0 + row, a.cols - 1);
+        for (int j = 0; j < 8; j++) {
+            const uint32_t k = k0 + at % kIn * 8 + j, kc = min(k, all - 1), s = kc / a.rank;
+            const T u = static_cast<const T *>(a.up)[((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + (kc - s * a.rank)];
+            low[j] = k < all && s == own[q] ? kLargest : 0.0f;
+            up[j] = k < all && !finite(E::up(u)) ? sign : 0.0f;
+        }
+    }
+    // a pass over the adapters; whether a thread's elements are all finite
+    template <bool First>
+    __device__ __forceinline__ bool pass(const LinearArgs &a, char *stages, Tile &t, float sign) {
         const uint32_t lane = lane_id();
+        bool all_finite = true;
         for (uint32_t k0 = 0, turn = 0; k0 < all; k0 += kStep, turn ^= 1) {
             char *lds = stages + turn * 2 * kParts * kPart;
             float low[kPieces][8];
             Vec<T, 8> up[kPieces];
-            read(a, t, k0, low, up);
+            if constexpr (First) read(a, t, k0, low, up);
 #pragma unroll
             for (int q = 0; q < kPieces; q++) {
                 const uint32_t at = q * Tile::kThreads + threadIdx.x;
                 char *to = lds + place(at / kIn, at % kIn);
                 float v[8];
+                if constexpr (First) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = E::up(up[q].v[j]);
+                    for (int j = 0; j < 8; j++) v[j] = E::up(up[q].v[j]);
+                    if (not_finite(up[q])) {
+                        all_finite = false;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[j] = finite(v[j]) ? v[j] : 0.0f;
+                    }
+                } else {
+                    mark(a, t, k0, q, sign, low[q], v);
+                }
                 put(to, v);
                 put(to + kParts * kPart, low[q]);
             }
@@ -257,7 +300,22 @@ struct Adapters {
                 }
             }
         }
-        if (all) __syncthreads();
+        __syncthreads();
+        return all_finite;
+    }
+    __device__ __forceinline__ void add(const LinearArgs &a, char *stages, Tile &t) {
+        if (all == 0) return;
+        const uint64_t some = __ballot(!pass<true>(a, stages, t, 0.0f));
+        uint32_t *met = reinterpret_cast<uint32_t *>(stages);
+        if (lane_id() == 0) met[threadIdx.x / kWave] = some != 0;
+        __syncthreads();
+        const uint32_t any = uniform(met[0] | met[1] | met[2] | met[3]);
+        __syncthreads();
+        if (!any) return;
+        for (float sign = kLargest;; sign = -kLargest) {
+            pass<false>(a, stages, t, sign);
+            if (sign < 0.0f) return;
+        }
     }
 };
 

@@ -189,6 +189,8 @@ def linear(x, w, out, *, bias=None, down=None, up=None, ids=None, scale=None, wo
     ``bias`` [outs] and ``scale`` [adapters] float32 (None: 0 and 1), ``ids``
     [n] int32. A row whose id is below 0, or no adapter's, has none. Rows come
     in any order; those of one adapter take the least time next to each other.
+    Elements of an adapter that are no finite numbers reach its own rows alone,
+    whose outputs are then infinite or NaN.
 
     Sums are float32 and rounded once. In bfloat16 calls of many rows round
     the ``rank`` values between down and up (the scale in them) to bfloat16,

@@ -338,6 +338,35 @@ def test_projections(n, dim, outs, rank, adapters, order, bias, scale, pad, lead
     close(back(out), L.linear(x, w, b, down, up, ids, s, dtype), "out")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, outs, rank", [(12, 64, 80, 8), (200, 40, 300, 16), (200, 40, 300, 5), (1500, 64, 1100, 8), (2100, 64, 2100, 3), (2100, 512, 4100, 8)])
+def test_an_adapter_that_is_no_number_is_its_own_rows_alone(n, dim, outs, rank, dtype):
+    """Elements of adapters that are infinite or NaN, its rows among others'."""
+    rng = np.random.default_rng(rank + n)
+    adapters = 5
+    x, w = rows(rng, n, dim, dtype), R.rounded(rng.standard_normal((outs, dim)) / np.sqrt(dim), dtype)
+    down = R.rounded(rng.standard_normal((adapters, rank, dim)) / np.sqrt(dim), dtype)
+    up = R.rounded(rng.standard_normal((adapters, outs, rank)), dtype)
+    ids = rng.integers(-1, adapters, n).astype(np.int32)
+    value, off = L.linear(x, w, None, down, up, ids, None, dtype)
+    for array, of in (("up", 1), ("up", 3), ("down", 2)):
+        d, u = down.copy(), up.copy()
+        bad = np.zeros((n, outs), bool)
+        if array == "up":
+            cells = rng.choice(outs, 9, replace=False)
+            u[of, cells, rng.integers(0, rank, 9)] = np.array([np.inf, -np.inf, np.nan])[np.arange(9) % 3]
+            bad[np.ix_(ids == of, cells)] = True
+        else:
+            d[of, rank - 1, dim // 2] = np.nan
+            bad[ids == of] = True
+        out = like((n, outs), dtype)
+        hb.linear(dev(x, dtype), dev(w, dtype), out, down=dev(d.reshape(-1, dim), dtype), up=dev(u.reshape(-1, rank), dtype),
+                  ids=dev(ids, "int32"), workspace=work(hb.linear_workspace(n, outs, dim, dtype, rank=rank)))
+        got = back(out)
+        assert not np.any(np.isfinite(got[bad])), array
+        close(got[~bad], (value[~bad], off[~bad]), array)
+
+
 def test_a_row_without_an_adapter_reads_none():
     """NaN adapters that no row has, and NaN rows beside others."""
     rng = np.random.default_rng(3)
