@@ -171,47 +171,73 @@ struct Adapters {
         return (carried & ~kExponents & (kExponents << 1)) != 0;
     }
     static __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-    // Every load is made, from within its array, and what does not count is zeroed.
-    __device__ __forceinline__ void read(const LinearArgs &a, const Tile &t, uint32_t k0, float (&low)[kPieces][8], Vec<T, 8> (&up)[kPieces]) {
+    // A step's operands as they are read, beside the products of the step before
+    // (8,191 rows of 1,024 by 4,096, 64 adapters of rank 16 in random order: 262 us,
+    // read behind them 298), and which pieces of `low` and `up` count: nothing waits
+    // for them before they are put into LDS.
+    struct Step {
+        float low[kPieces][8];
+        Vec<T, 8> up[kPieces];
+        bool mine[kPieces], some[kPieces];
+        uint32_t slot, rho;  // of the next read, whose adapter is known by then
+        int32_t id;
+    };
+    // (a piece of eight is one slot's, and all of a thread's pieces are the same one's)
+    __device__ __forceinline__ void look(const LinearArgs &a, uint32_t k0, Step &to) {
+        const uint32_t kc = min(k0 + threadIdx.x % kIn * 8, all - 1);
+        to.slot = kc / a.rank;
+        to.rho = (kc - to.slot * a.rank) & ~7u;
+        to.id = slot_id[to.slot];
+    }
+    // Every load is made, from within its array.
+    __device__ __forceinline__ void read(const LinearArgs &a, const Tile &t, uint32_t k0, Step &to) {
+        const T *ups = static_cast<const T *>(a.up);
+        auto lows = [&](int q) { return a.low + (uint64_t)(min(t.n0 + (q * Tile::kThreads + threadIdx.x) / kIn, a.rows - 1)) * a.rank; };
+        auto from = [&](int q, int32_t id) {
+            const uint64_t out = min(t.m0 + (q * Tile::kThreads + threadIdx.x) / kIn, a.cols - 1);
+            return ups + ((uint64_t)id * a.cols + out) * a.up_stride;
+        };
+        if (eights) {
+            const uint32_t k = k0 + threadIdx.x % kIn * 8, s = to.slot, rho = to.rho;
+            const int32_t id = to.id;
+            look(a, k0 + kStep, to);
 #pragma unroll
-        for (int q = 0; q < kPieces; q++) {
-            const uint32_t at = q * Tile::kThreads + threadIdx.x, row = at / kIn, k = k0 + at % kIn * 8;
-            const float *lows = a.low + (uint64_t)(min(t.n0 + row, a.rows - 1)) * a.rank;
-            const uint64_t out = min(t.m0 + row, a.cols - 1);
-            const T *ups = static_cast<const T *>(a.up);
-            const uint32_t kc = min(k, all - 1);
-            uint32_t s = kc / a.rank, rho = kc - s * a.rank;
-            if (eights) {  // (a piece is one slot's)
-                rho &= ~7u;
-                const Vec<float, 4> l0 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho),
-                                    l1 = *reinterpret_cast<const Vec<float, 4> *>(lows + rho + 4);
-                const T *from = ups + ((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + rho;
-                if (wide) {
-                    up[q] = *reinterpret_cast<const Vec<T, 8> *>(from);
-                } else {
+            for (int q = 0; q < kPieces; q++) {
+                const Vec<float, 4> l0 = *reinterpret_cast<const Vec<float, 4> *>(lows(q) + rho),
+                                    l1 = *reinterpret_cast<const Vec<float, 4> *>(lows(q) + rho + 4);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) up[q].v[j] = from[j];
-                }
-                const bool some = k < all, mine = some && s == own[q];
+                for (int j = 0; j < 8; j++) to.low[q][j] = j < 4 ? l0.v[j % 4] : l1.v[j % 4];
+                to.some[q] = k < all;
+                to.mine[q] = k < all && s == own[q];
+            }
+            if (wide) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    low[q][j] = mine ? j < 4 ? l0.v[j % 4] : l1.v[j % 4] : 0.0f;
-                    up[q].v[j] = some ? up[q].v[j] : (T)0;
-                }
+                for (int q = 0; q < kPieces; q++) to.up[q] = *reinterpret_cast<const Vec<T, 8> *>(from(q, id) + rho);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool some = k + j < all;
-                    const float l = lows[rho];
-                    const T u = ups[((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + rho];
-                    low[q][j] = some && s == own[q] ? l : 0.0f;
-                    up[q].v[j] = some ? u : (T)0;
-                    if (++rho == a.rank) {
-                        rho = 0;
-                        s += k + j + 1 < all;
-                    }
+                for (int q = 0; q < kPieces; q++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) to.up[q].v[j] = from(q, id)[rho + j];
+            }
+            return;
+        }
+#pragma unroll
+        for (int q = 0; q < kPieces; q++) {
+            const uint32_t k = k0 + threadIdx.x % kIn * 8, kc = min(k, all - 1);
+            uint32_t s = kc / a.rank, rho = kc - s * a.rank;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const bool some = k + j < all;
+                const float l = lows(q)[rho];
+                const T u = from(q, slot_id[s])[rho];
+                to.low[q][j] = some && s == own[q] ? l : 0.0f;
+                to.up[q].v[j] = some ? u : (T)0;
+                if (++rho == a.rank) {
+                    rho = 0;
+                    s += k + j + 1 < all;
                 }
             }
+            to.some[q] = to.mine[q] = true;
         }
     }
     // a piece's place: the rows that LDS serves at once meet different banks
@@ -252,31 +278,46 @@ struct Adapters {
     __device__ __forceinline__ bool pass(const LinearArgs &a, char *stages, Tile &t, float sign) {
         const uint32_t lane = lane_id();
         bool all_finite = true;
+        Step step;
+        if constexpr (First) {
+            look(a, 0, step);
+            read(a, t, 0, step);
+        }
         for (uint32_t k0 = 0, turn = 0; k0 < all; k0 += kStep, turn ^= 1) {
             char *lds = stages + turn * 2 * kParts * kPart;
-            float low[kPieces][8];
-            Vec<T, 8> up[kPieces];
-            if constexpr (First) read(a, t, k0, low, up);
 #pragma unroll
             for (int q = 0; q < kPieces; q++) {
                 const uint32_t at = q * Tile::kThreads + threadIdx.x;
                 char *to = lds + place(at / kIn, at % kIn);
-                float v[8];
+                float v[8], low[8];
                 if constexpr (First) {
+                    Vec<T, 8> &u = step.up[q];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = E::up(up[q].v[j]);
-                    if (not_finite(up[q])) {
+                    for (int j = 0; j < 8; j++) {
+                        low[j] = step.mine[q] ? step.low[q][j] : 0.0f;
+                        u.v[j] = step.some[q] ? u.v[j] : (T)0;
+                    }
+                    if (not_finite(u)) {
                         all_finite = false;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) v[j] = finite(v[j]) ? v[j] : 0.0f;
+                        for (int j = 0; j < 8; j++) u.v[j] = finite(E::up(u.v[j])) ? u.v[j] : (T)0;
+                    }
+                    if constexpr (kParts == 1) {
+                        *reinterpret_cast<Vec<T, 8> *>(to) = u;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[j] = u.v[j];
+                        put(to, v);
                     }
                 } else {
-                    mark(a, t, k0, q, sign, low[q], v);
+                    mark(a, t, k0, q, sign, low, v);
+                    put(to, v);
                 }
-                put(to, v);
-                put(to + kParts * kPart, low[q]);
+                put(to + kParts * kPart, low);
             }
             __syncthreads();  // (the step before the last has been read by all that come here)
+            if constexpr (First)
+                if (k0 + kStep < all) read(a, t, k0 + kStep, step);  // beside the products
 #pragma unroll
             for (uint32_t kk = 0; kk < kStep / 16; kk++) {
                 const uint32_t piece = kk * 2 + lane / 32;
