@@ -8,7 +8,9 @@
 // sixteenth where eight waves of 128 x 64 read 48), and a row's 64 products are
 // one line of 128 bytes (with 32 the L2 answered twice as many requests). One wave
 // a SIMD has no other to fill its gaps: whatever feeds the matrix instructions
-// is put between them.
+// is put between them. The matrix cores are busy 63 to 68% of a large product's
+// cycles, and power holds their clock: matrix instructions alone, nothing loaded,
+// take 76% of the time (8,192 x 4,096 x 4,096: 214 us of 281).
 #pragma once
 #include "product.h"
 
