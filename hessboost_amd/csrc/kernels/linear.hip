@@ -136,8 +136,11 @@ __device__ __forceinline__ void linear_store_part(const LinearArgs &a, Tile &t) 
 // zeros at the others', so that any order of the rows is right, and rows of few
 // adapters take few steps.
 //
-// In bf16 the low values are rounded once to bf16, as any product's operand
-// is: half a step each of the adapters' part. In f32 all is in three parts.
+// The low values are f32 sums and stay so, in three bf16 parts; `up` is one part in
+// bf16 and three in f32. (As one bf16 each they took less time, 8,191 rows of 1,024
+// by 4,096 with 64 adapters in 50 runs 94 us and now 99, in random order 256 and
+// 308; but few rows and shares' joins add f32 values, and a row's outputs depended
+// on how many rows stood beside it.)
 //
 // An adapter is its own rows' alone: an element of `up` that is no finite number
 // would make no number of the others' zeros, so it is taken as zero, and a tile
@@ -147,12 +150,13 @@ __device__ __forceinline__ void linear_store_part(const LinearArgs &a, Tile &t) 
 template <typename Tile, typename E>
 struct Adapters {
     using T = typename E::type;
-    static constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kPairs = kParts == 3 ? 6 : 1;
-    // A step is 32 products, in f32 16 of all three parts
-    static constexpr uint32_t kM = Tile::kM, kStep = kParts == 1 ? 32 : 16, kRow = kStep * 2, kPart = kM * kRow, kIn = kStep / 8;
+    static constexpr int kUps = sizeof(T) == 4 ? 3 : 1, kLows = 3, kPairs = kUps == 3 ? 6 : 3;
+    // A step is 32 products, in f32 16, of all their parts
+    static constexpr uint32_t kM = Tile::kM, kStep = kUps == 1 ? 32 : 16, kRow = kStep * 2, kPart = kM * kRow, kIn = kStep / 8;
+    static constexpr uint32_t kStage = (kUps + kLows) * kPart;
     static constexpr int kPieces = kM * kIn / Tile::kThreads;  // of eight products of a row, of either operand
     static_assert(Tile::kM == Tile::kN && kM * kIn % Tile::kThreads == 0, "as many pieces of each a thread");
-    static_assert(4 * kParts * kPart <= (uint32_t)Tile::kLds, "two steps fit the stages");
+    static_assert(2 * kStage <= (uint32_t)Tile::kLds, "two steps fit the stages");
     static_assert(Tile::kThreads == 4 * kWave, "four waves' flags");
     uint32_t all, own[kPieces];
     const int32_t *slot_id;
@@ -169,18 +173,19 @@ struct Adapters {
     }
     // Whether any of eight elements is no finite number: their exponents, two at a
     // time in 16 bits, carried into the sign's place.
-    static __device__ __forceinline__ bool not_finite(const Vec<T, 8> &v) {
-        constexpr uint32_t kExponents = sizeof(T) == 4 ? 0x7f800000u : 0x7f807f80u, kOne = sizeof(T) == 4 ? 0x00800000u : 0x00800080u;
-        const auto words = __builtin_bit_cast(Vec<uint32_t, 2 * sizeof(T)>, v);
+    template <typename B>
+    static __device__ __forceinline__ bool not_finite(const Vec<B, 8> &v) {
+        constexpr uint32_t kExponents = sizeof(B) == 4 ? 0x7f800000u : 0x7f807f80u, kOne = sizeof(B) == 4 ? 0x00800000u : 0x00800080u;
+        const auto words = __builtin_bit_cast(Vec<uint32_t, 2 * sizeof(B)>, v);
         uint32_t carried = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 2 * sizeof(T); i++) carried |= (words.v[i] & kExponents) + kOne;
+        for (uint32_t i = 0; i < 2 * sizeof(B); i++) carried |= (words.v[i] & kExponents) + kOne;
         return (carried & ~kExponents & (kExponents << 1)) != 0;
     }
     static __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
     // A step's operands as they are read, beside the products of the step before
-    // (8,191 rows of 1,024 by 4,096, 64 adapters of rank 16 in random order: 262 us,
-    // read behind them 298), and which pieces of `low` and `up` count: nothing waits
+    // (64 adapters in random order took an eighth less time so than read behind
+    // them), and which pieces of `low` and `up` count: nothing waits
     // for them before they are put into LDS.
     struct Step {
         float low[kPieces][8];
@@ -251,21 +256,31 @@ struct Adapters {
     static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t piece) {
         return row * kRow + (piece ^ ((row >> (kIn == 4 ? 2 : 3)) & (kIn - 1))) * 16;
     }
+    template <int Parts>
     static __device__ __forceinline__ void put(char *to, const float (&v)[8]) {
-        Vec<uint16_t, 8> out[kParts];
+        Vec<uint16_t, 8> out[Parts];
+        float rest[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if constexpr (kParts == 1) {
-                out[0].v[j] = to_bf16(v[j]);
-            } else {
+        for (int j = 0; j < 8; j++) rest[j] = v[j];
+#pragma unroll
+        for (int q = 0; q < Parts; q++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                out[q].v[j] = to_bf16(rest[j]);
+                rest[j] -= bf16_f32(out[q].v[j]);
+            }
+        // (what does not round to a finite number is split by itself)
+        if (Parts == 3 && not_finite(out[0])) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
                 uint16_t p[3];
                 split3(v[j], p);
 #pragma unroll
-                for (int q = 0; q < kParts; q++) out[q].v[j] = p[q];
+                for (int q = 0; q < Parts; q++) out[q].v[j] = p[q];
             }
         }
 #pragma unroll
-        for (int q = 0; q < kParts; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(to + q * kPart) = out[q];
+        for (int q = 0; q < Parts; q++) *reinterpret_cast<Vec<uint16_t, 8> *>(to + q * kPart) = out[q];
     }
     // What stands in the operands' places of the passes behind the first: the
     // largest bf16, whose square f32 does not hold.
@@ -291,7 +306,7 @@ struct Adapters {
             read(a, t, 0, step);
         }
         for (uint32_t k0 = 0, turn = 0; k0 < all; k0 += kStep, turn ^= 1) {
-            char *lds = stages + turn * 2 * kParts * kPart;
+            char *lds = stages + turn * kStage;
 #pragma unroll
             for (int q = 0; q < kPieces; q++) {
                 const uint32_t at = q * Tile::kThreads + threadIdx.x;
@@ -309,18 +324,24 @@ struct Adapters {
 #pragma unroll
                         for (int j = 0; j < 8; j++) u.v[j] = finite(E::up(u.v[j])) ? u.v[j] : (T)0;
                     }
-                    if constexpr (kParts == 1) {
+                    if constexpr (kUps == 1) {
                         *reinterpret_cast<Vec<T, 8> *>(to) = u;
                     } else {
 #pragma unroll
                         for (int j = 0; j < 8; j++) v[j] = u.v[j];
-                        put(to, v);
+                        put<kUps>(to, v);
                     }
                 } else {
                     mark(a, t, k0, q, sign, low, v);
-                    put(to, v);
+                    put<kUps>(to, v);
                 }
-                put(to + kParts * kPart, low);
+                if (!First || __ballot(step.mine[q])) {
+                    put<kLows>(to + kUps * kPart, low);
+                } else {  // zeros need no parts
+#pragma unroll
+                    for (int part = 0; part < kLows; part++) *reinterpret_cast<Vec<uint16_t, 8> *>(to + (kUps + part) * kPart) = {};
+                }
+                __builtin_amdgcn_sched_barrier(0);  // and one piece's parts
             }
             __syncthreads();  // (the step before the last has been read by all that come here)
             if constexpr (First)
@@ -331,20 +352,28 @@ struct Adapters {
                 auto fragment = [&](uint32_t part, uint32_t row) {
                     return *reinterpret_cast<const bf16x8 *>(lds + part * kPart + place(row + lane % 32, piece));
                 };
+                bf16x8 fa[kUps][Tile::kI], first[Tile::kJ];
 #pragma unroll
-                for (int pair = 0; pair < kPairs; pair++) {
-                    const uint32_t pa = kParts == 1 ? 0 : kPartA >> 2 * pair & 3u, pb = kParts == 1 ? 0 : kPartB >> 2 * pair & 3u;
-                    bf16x8 fa[Tile::kI], fb[Tile::kJ];
+                for (int j = 0; j < Tile::kJ; j++) first[j] = fragment(kUps, t.wave_n + 32 * j);
 #pragma unroll
-                    for (int i = 0; i < Tile::kI; i++) fa[i] = fragment(pa, t.wave_m + 32 * i);
+                for (int part = 0; part < kUps; part++)
 #pragma unroll
-                    for (int j = 0; j < Tile::kJ; j++) fb[j] = fragment(kParts + pb, t.wave_n + 32 * j);
+                    for (int i = 0; i < Tile::kI; i++) fa[part][i] = fragment(part, t.wave_m + 32 * i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int i = 0; i < Tile::kI; i++)
+                for (int j = 0; j < Tile::kJ; j++) {
+                    // (where none of the 32 rows has the adapters of these products nothing is added)
+                    const auto words = __builtin_bit_cast(i32x4, first[j]);
+                    if (!__ballot((words[0] | words[1] | words[2] | words[3]) != 0)) continue;
+                    // the other parts are read under the products with the first
+                    const bf16x8 fb[kLows] = {first[j], fragment(kUps + 1, t.wave_n + 32 * j), fragment(kUps + 2, t.wave_n + 32 * j)};
 #pragma unroll
-                        for (int j = 0; j < Tile::kJ; j++)
-                            t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], t.acc[i][j], 0, 0, 0);
-                    if (kPairs > 1) __builtin_amdgcn_sched_barrier(0);  // one pair's fragments at a time in registers
+                    for (int pair = kPairs - 1; pair >= 0; pair--) {
+                        const uint32_t pa = kUps == 1 ? 0 : kPartB >> 2 * pair & 3u, pb = (kUps == 1 ? kPartsByOne : kPartA) >> 2 * pair & 3u;
+#pragma unroll
+                        for (int i = 0; i < Tile::kI; i++)
+                            t.acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[pa][i], fb[pb], t.acc[i][j], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -456,8 +485,9 @@ struct LinearY {
 };
 
 // With adapters, whose operands take the registers that fragments had: the biases
-// are read with them, behind the products. (The first step's operands read before
-// the products spilled: 98 us against 83, 8,191 rows of 1,024 by 4,096.)
+// are read with them, behind the products, and of small tiles, of which a SIMD has
+// two waves, behind theirs too. (The first step's operands read before the products
+// spilled: 98 us against 83, 8,191 rows of 1,024 by 4,096.)
 template <typename Tile, typename E>
 struct LinearYa {
     Adapters<Tile, E> adapters;
@@ -465,8 +495,9 @@ struct LinearYa {
     __device__ __forceinline__ LinearYa(const LinearArgs &a, const Tile &t) : adapters(a, t) {}
     __device__ __forceinline__ NothingElse beside() { return {}; }
     __device__ __forceinline__ void behind(const LinearArgs &a, char *lds, Tile &t) {
-        bias.read(t, a.bias, a.cols, 0.0f);
+        if constexpr (Tile::kI == 4) bias.read(t, a.bias, a.cols, 0.0f);
         adapters.add(a, lds, t);
+        if constexpr (Tile::kI != 4) bias.read(t, a.bias, a.cols, 0.0f);
     }
     __device__ __forceinline__ void store(const LinearArgs &a, char *room, Tile &t) { linear_store<Tile, E, false>(a, room, t, bias); }
 };

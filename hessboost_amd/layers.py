@@ -192,9 +192,8 @@ def linear(x, w, out, *, bias=None, down=None, up=None, ids=None, scale=None, wo
     Elements of an adapter that are no finite numbers reach its own rows alone,
     whose outputs are then infinite or NaN.
 
-    Sums are float32 and rounded once. In bfloat16 calls of many rows round
-    the ``rank`` values between down and up (the scale in them) to bfloat16,
-    as any product's operand is: half a step each of the adapter's part."""
+    Sums are float32, the ``rank`` values between down and up (the scale in
+    them) too, and the outputs are rounded once."""
     call = _Call()
     xp, (n, dim), xs = call.array(x, "x", 2, _FLOATS)
     dtype, outs = _dtype(x.dtype), w.shape[0]

@@ -856,11 +856,11 @@ int hbr_rms_norm_grad(int ordinal, const hbr_norm_grad *p, void *workspace, uint
  * adapters, or none (an id below 0, or of n_adapters and more; rank or
  * n_adapters 0: no row has one):
  *   out[r] = x[r] w^T + bias + scale[a] * ((x[r] down[a]^T) up[a]^T), a = ids[r],
- * summed in f32 and rounded once; in bf16 the `rank` values between down and up
- * are rounded to bf16 in calls of many rows. down holds n_adapters x rank rows of dim, up
- * n_adapters x n_outs rows of rank. Rows may come in any order; those of one
- * adapter next to each other take the least time. Elements of an adapter that
- * are no finite numbers reach its own rows alone (outputs infinite or NaN). */
+ * summed in f32, the `rank` values between down and up too, and rounded once.
+ * down holds n_adapters x rank rows of dim, up n_adapters x n_outs rows of rank.
+ * Rows may come in any order; those of one adapter next to each other take the
+ * least time. Elements of an adapter that are no finite numbers reach its own
+ * rows alone (outputs infinite or NaN). */
 typedef struct hbr_linear_args {
     uint32_t dtype;           /* of x, w, out, down and up */
     uint32_t dim;

@@ -773,3 +773,25 @@ def test_torch_tensors_of_layers_are_taken_on_their_stream():
     code = TORCH.replace("{root!r}", repr(os.path.dirname(here))).replace("{tests!r}", repr(here))
     r = subprocess.run([sys.executable, "-u", "-c", code], capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "torch layers ok" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("n, dim, outs, rank", [(1, 64, 80, 8), (12, 64, 80, 8), (40, 200, 96, 4), (200, 64, 300, 16), (200, 40, 300, 6), (300, 2048, 130, 8),
+                                                (1500, 64, 1100, 8), (2100, 64, 2100, 32), (2100, 512, 4100, 8)])
+def test_the_low_values_of_adapters_are_f32_sums_for_any_number_of_rows(n, dim, outs, rank):
+    """Ranks in pairs that take each other off but for their last bits: in
+    bfloat16 the outputs are those of float32 low values, rounded once."""
+    rng = np.random.default_rng(n + rank)
+    adapters = 3
+    x = rows(rng, n, dim, "bfloat16")
+    down = R.rounded(rng.standard_normal((adapters, rank, dim)) / np.sqrt(dim), "bfloat16")
+    down[:, 1::2] = R.rounded(down[:, ::2] * (1 + 2.0 ** -7 * rng.integers(-1, 2, down[:, ::2].shape)), "bfloat16")
+    up = R.rounded(rng.standard_normal((adapters, outs, rank)), "bfloat16")
+    up[:, :, 1::2] = -up[:, :, ::2]
+    ids, scale = rng.integers(-1, adapters, n).astype(np.int32), f32(rng, adapters, 0.5, 1.0)
+    ids[0] = 1
+    out = like((n, outs), "bfloat16")
+    hb.linear(dev(x, "bfloat16"), dev(np.zeros((outs, dim)), "bfloat16"), out, down=dev(down.reshape(-1, dim), "bfloat16"),
+              up=dev(up.reshape(-1, rank), "bfloat16"), ids=dev(ids, "int32"), scale=dev(scale, "float32"),
+              workspace=work(hb.linear_workspace(n, outs, dim, "bfloat16", rank=rank)))
+    value, off = L.linear(x, np.zeros((outs, dim)), None, down, up, ids, scale, "float32")
+    close(back(out), (value, off + R.HALF["bfloat16"] * (np.abs(value) + off)), "out")
