@@ -143,10 +143,12 @@ __device__ __forceinline__ void linear_store_part(const LinearArgs &a, Tile &t) 
 // on how many rows stood beside it.)
 //
 // An adapter is its own rows' alone: an element of `up` that is no finite number
-// would make no number of the others' zeros, so it is taken as zero, and a tile
-// that met one goes over its adapters twice more, with a product of the largest
-// numbers where a row's own adapter has such an element, added and taken off:
-// infinity less infinity there, zero everywhere else.
+// would make no number of the others' zeros, so a one of its sign stands in its
+// place (so that an infinite low value stays infinite), and a tile that met one
+// goes over its adapters four times more, once for either sign of low values and
+// of such elements, with a product of the largest numbers, infinite, where a row's
+// own adapter has the pair. What is zero or no number counts for both signs:
+// infinity less infinity, no number, as the formula has it.
 template <typename Tile, typename E>
 struct Adapters {
     using T = typename E::type;
@@ -285,19 +287,21 @@ struct Adapters {
     // What stands in the operands' places of the passes behind the first: the
     // largest bf16, whose square f32 does not hold.
     static constexpr float kLargest = 0x1.fep127f;
-    __device__ __forceinline__ void mark(const LinearArgs &a, const Tile &t, uint32_t k0, int q, float sign, float (&low)[8], float (&up)[8]) {
+    __device__ __forceinline__ void mark(const LinearArgs &a, const Tile &t, uint32_t k0, int q, float sign_low, float sign_up, float (&low)[8],
+                                         float (&up)[8]) {
         const uint32_t at = q * Tile::kThreads + threadIdx.x, row = at / kIn;
-        const uint64_t out = min(t.m0 + row, a.cols - 1);
+        const uint64_t out = min(t.m0 + row, a.cols - 1), in = min(t.n0 + row, a.rows - 1);
         for (int j = 0; j < 8; j++) {
-            const uint32_t k = k0 + at % kIn * 8 + j, kc = min(k, all - 1), s = kc / a.rank;
-            const T u = static_cast<const T *>(a.up)[((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + (kc - s * a.rank)];
-            low[j] = k < all && s == own[q] ? kLargest : 0.0f;
-            up[j] = k < all && !finite(E::up(u)) ? sign : 0.0f;
+            const uint32_t k = k0 + at % kIn * 8 + j, kc = min(k, all - 1), s = kc / a.rank, rho = kc - s * a.rank;
+            const float u = E::up(static_cast<const T *>(a.up)[((uint64_t)slot_id[s] * a.cols + out) * a.up_stride + rho]);
+            const bool mine = k < all && s == own[q];
+            low[j] = mine && !(a.low[in * a.rank + rho] * sign_low < 0.0f) ? kLargest : 0.0f;
+            up[j] = k < all && !finite(u) && !(u * sign_up < 0.0f) ? kLargest * sign_low * sign_up : 0.0f;
         }
     }
     // a pass over the adapters; whether a thread's elements are all finite
     template <bool First>
-    __device__ __forceinline__ bool pass(const LinearArgs &a, char *stages, Tile &t, float sign) {
+    __device__ __forceinline__ bool pass(const LinearArgs &a, char *stages, Tile &t, float sign_low = 0.0f, float sign_up = 0.0f) {
         const uint32_t lane = lane_id();
         bool all_finite = true;
         Step step;
@@ -322,7 +326,7 @@ struct Adapters {
                     if (not_finite(u)) {
                         all_finite = false;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) u.v[j] = finite(E::up(u.v[j])) ? u.v[j] : (T)0;
+                        for (int j = 0; j < 8; j++) u.v[j] = finite(E::up(u.v[j])) ? u.v[j] : E::down(__builtin_copysignf(1.0f, E::up(u.v[j])));
                     }
                     if constexpr (kUps == 1) {
                         *reinterpret_cast<Vec<T, 8> *>(to) = u;
@@ -332,7 +336,7 @@ struct Adapters {
                         put<kUps>(to, v);
                     }
                 } else {
-                    mark(a, t, k0, q, sign, low, v);
+                    mark(a, t, k0, q, sign_low, sign_up, low, v);
                     put<kUps>(to, v);
                 }
                 if (!First || __ballot(step.mine[q])) {
@@ -382,17 +386,14 @@ struct Adapters {
     }
     __device__ __forceinline__ void add(const LinearArgs &a, char *stages, Tile &t) {
         if (all == 0) return;
-        const uint64_t some = __ballot(!pass<true>(a, stages, t, 0.0f));
+        const uint64_t some = __ballot(!pass<true>(a, stages, t));
         uint32_t *met = reinterpret_cast<uint32_t *>(stages);
         if (lane_id() == 0) met[threadIdx.x / kWave] = some != 0;
         __syncthreads();
         const uint32_t any = uniform(met[0] | met[1] | met[2] | met[3]);
         __syncthreads();
         if (!any) return;
-        for (float sign = kLargest;; sign = -kLargest) {
-            pass<false>(a, stages, t, sign);
-            if (sign < 0.0f) return;
-        }
+        for (uint32_t signs = 0; signs < 4; signs++) pass<false>(a, stages, t, signs & 1 ? -1.0f : 1.0f, signs & 2 ? -1.0f : 1.0f);
     }
 };
 

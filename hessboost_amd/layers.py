@@ -190,7 +190,8 @@ def linear(x, w, out, *, bias=None, down=None, up=None, ids=None, scale=None, wo
     [n] int32. A row whose id is below 0, or no adapter's, has none. Rows come
     in any order; those of one adapter take the least time next to each other.
     Elements of an adapter that are no finite numbers reach its own rows alone,
-    whose outputs are then infinite or NaN.
+    whose outputs are then infinite or NaN, as the formula has it for any number
+    of rows.
 
     Sums are float32, the ``rank`` values between down and up (the scale in
     them) too, and the outputs are rounded once."""

@@ -860,7 +860,7 @@ int hbr_rms_norm_grad(int ordinal, const hbr_norm_grad *p, void *workspace, uint
  * down holds n_adapters x rank rows of dim, up n_adapters x n_outs rows of rank.
  * Rows may come in any order; those of one adapter next to each other take the
  * least time. Elements of an adapter that are no finite numbers reach its own
- * rows alone (outputs infinite or NaN). */
+ * rows alone (outputs infinite or NaN, as the formula has it). */
 typedef struct hbr_linear_args {
     uint32_t dtype;           /* of x, w, out, down and up */
     uint32_t dim;

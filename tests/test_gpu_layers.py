@@ -795,3 +795,53 @@ def test_the_low_values_of_adapters_are_f32_sums_for_any_number_of_rows(n, dim, 
               workspace=work(hb.linear_workspace(n, outs, dim, "bfloat16", rank=rank)))
     value, off = L.linear(x, np.zeros((outs, dim)), None, down, up, ids, scale, "float32")
     close(back(out), (value, off + R.HALF["bfloat16"] * (np.abs(value) + off)), "out")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim, outs, rank", [(12, 64, 80, 8), (200, 40, 300, 16), (200, 40, 300, 5), (300, 2048, 130, 8), (1500, 64, 1100, 8),
+                                                (2100, 64, 2100, 3), (2100, 512, 4100, 8)])
+def test_infinite_adapters_give_what_their_formula_does(n, dim, outs, rank, dtype):
+    """Infinities of either sign and NaN in either factor and in the scales, for
+    low values of either sign, zeros and infinities among them: the same outputs
+    for any number of rows, infinite with their sign or no numbers. All is whole
+    numbers, so that no low value's sign is a matter of roundings."""
+    rng = np.random.default_rng(rank + n)
+    adapters = 4
+    x, w = rng.integers(-2, 3, (n, dim)).astype(float), rng.integers(-1, 2, (outs, dim)).astype(float)
+    x[::7] = 0.0
+    down, up = rng.integers(-1, 2, (adapters, rank, dim)).astype(float), rng.integers(-2, 3, (adapters, outs, rank)).astype(float)
+    ids, scale = rng.integers(-1, adapters, n).astype(np.int32), np.array([1.0, -2.0, 0.5, 1.0])
+    ids[:4] = 0, 1, 2, 3
+    off = L.linear(x, w, None, down, up, ids, scale, dtype)[1]
+    cells = rng.permutation(outs)[:18].reshape(2, 9)
+    for a in (0, 1):
+        up[a, cells[a], rng.integers(0, rank, 9)] = np.array([np.inf, -np.inf, np.inf, -np.inf, np.nan, np.inf, -np.inf, np.inf, -np.inf])
+        up[a, cells[a][:3], rng.integers(0, rank, 3)] = np.inf  # two of a sum, of one sign or of both
+    down[1, 0, dim // 2], scale[3] = -np.inf, np.inf
+    out = like((n, outs), dtype)
+    hb.linear(dev(x, dtype), dev(w, dtype), out, down=dev(down.reshape(-1, dim), dtype), up=dev(up.reshape(-1, rank), dtype), ids=dev(ids, "int32"),
+              scale=dev(scale, "float32"), workspace=work(hb.linear_workspace(n, outs, dim, dtype, rank=rank)))
+    got, want = back(out), x @ w.T
+    with np.errstate(invalid="ignore"):
+        for r in np.flatnonzero(ids >= 0):
+            low = np.sum(x[r] * down[ids[r]], 1) * scale[ids[r]]
+            want[r] += np.sum(low * up[ids[r]], 1)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    some = np.isinf(want)
+    assert np.array_equal(got[some], want[some]) and np.any(want[some] > 0) and np.any(want[some] < 0)
+    rest = np.isfinite(want)
+    close(got[rest], (want[rest], off[rest]), "finite outputs")
+
+
+@pytest.mark.parametrize("n", [10, 130, 2000])
+def test_low_values_past_bfloat16_stay_finite(n):
+    """A low value of more than bfloat16's largest, and less than float32's."""
+    outs, dim = 1100, 64
+    x, down, up = np.ones((n, dim)), np.zeros((1, 1, dim)), np.full((1, outs, 1), 2.0 ** -20)
+    down[0, 0, 0] = 1.0
+    out = like((n, outs), "bfloat16")
+    scale = float(np.float32(3.4e38))
+    hb.linear(dev(x, "bfloat16"), dev(np.zeros((outs, dim)), "bfloat16"), out, down=dev(down[0], "bfloat16"), up=dev(up[0], "bfloat16"),
+              ids=dev(np.zeros(n), "int32"), scale=dev(np.array([scale]), "float32"), workspace=work(hb.linear_workspace(n, outs, dim, "bfloat16", rank=1)))
+    value = np.full((n, outs), scale * 2.0 ** -20)
+    close(back(out), (value, (R.HALF["bfloat16"] + 10 * R.EPS32) * value), "out")
