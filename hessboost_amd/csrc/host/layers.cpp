@@ -415,6 +415,7 @@ bool few_rows(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype) {
 }
 
 struct LinearPlan {
+    bool few;
     char *x, *w;
     float *low, *part;
     uint16_t *slot_of;
@@ -426,9 +427,16 @@ struct LinearPlan {
 LinearPlan linear_plan(uint64_t n, uint64_t outs, uint64_t dim, uint64_t rank, uint32_t dtype, void *workspace) {
     LinearPlan q{};
     const uint64_t parts = dtype == HBR_F32 ? 3 : 1;
+    Arena w(workspace);
+    // (a number of rows is few with every smaller one: room for more serves them)
+    q.few = few_rows(n, outs, dim, dtype);
+    if (q.few) {
+        q.low = w.take<float>(n * rank);
+        q.bytes = w.used;
+        return q;
+    }
     q.segments = dtype == HBR_F32 ? 6 : 1;
     q.product = product_plan(outs, n, dim, q.segments);
-    Arena w(workspace);
     q.x = w.take<char>(laid_bytes(n, dim, parts));
     q.w = w.take<char>(laid_bytes(outs, dim, parts));
     q.low = w.take<float>(n * rank);
@@ -480,7 +488,7 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         const uint32_t v = rows_vector(size, dim, all);
         return kernel_of(name, p.dtype, v == 16 / size ? v : 1);
     };
-    const bool few = few_rows(n, outs, dim, p.dtype);
+    const bool few = q.few;
     LinearArgs a{};
     Operands operands(p.dtype);
     if (!few) {
@@ -504,8 +512,10 @@ void linear(int ordinal, void *stream, const hbr_linear_args &p, void *workspace
         const uint64_t groups = tiles(n, 16), most = tiles(std::min<uint64_t>(n, 16) * rank, 32);
         l.groups = (uint32_t)groups;
         l.shares = (uint32_t)std::max<uint64_t>(1, std::min(most, 256 / groups));
-        l.tile = (uint32_t)q.product.t->tile;
-        l.tiles = !few && q.product.splits == 1 ? (uint32_t)q.product.n_tiles : 0;
+        if (!few && q.product.splits == 1) {
+            l.tile = (uint32_t)q.product.t->tile;
+            l.tiles = (uint32_t)q.product.n_tiles;
+        }
         l.slot_of = q.slot_of;
         l.slot_id = q.slot_id;
         l.slots = q.slots;

@@ -845,3 +845,13 @@ def test_low_values_past_bfloat16_stay_finite(n):
               ids=dev(np.zeros(n), "int32"), scale=dev(np.array([scale]), "float32"), workspace=work(hb.linear_workspace(n, outs, dim, "bfloat16", rank=1)))
     value = np.full((n, outs), scale * 2.0 ** -20)
     close(back(out), (value, (R.HALF["bfloat16"] + 10 * R.EPS32) * value), "out")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_without_adapters_need_no_workspace(dtype):
+    rng = np.random.default_rng(6)
+    for n, dim, outs in ((1, 1024, 700), (16, 96, 33), (64, 72, 64)):
+        x, w = rows(rng, n, dim, dtype), rows(rng, outs, dim, dtype, 0.2)
+        out = like((n, outs), dtype)
+        hb.linear(dev(x, dtype), dev(w, dtype), out)
+        close(back(out), L.linear(x, w, None, None, None, None, None, dtype), "out")

@@ -260,3 +260,19 @@ def test_the_codes_of_the_plain_form_are_the_nearest():
                 assert np.abs(held[r, c] - v[r, c]) == best
             else:
                 assert np.isnan(held[r, c])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_few_rows_need_room_for_their_low_values_alone(dtype):
+    """Up to 64 rows (in bfloat16 16, and more where w is small) read x and w in
+    place: without adapters no workspace is needed, with them f32 values."""
+    code = A.F32 if dtype == "float32" else A.BF16
+    far = [(i + 1) << 40 for i in range(12)]
+    for n, outs, dim in ((1, 8192, 8192), (16, 14_336, 4096), (64, 512, 256), (3, 7, 5)):
+        assert hb.linear_workspace(n, outs, dim, dtype) == 0
+        assert 4 * n * 16 <= hb.linear_workspace(n, outs, dim, dtype, rank=16) <= 4 * n * 16 + 255
+        kw = dict(dtype=code, dim=dim, n_rows=n, n_outs=outs, x_stride=dim, w_stride=dim, out_stride=outs, x=far[0], w=far[1], bias=far[2], out=far[7])
+        assert checked(linear(workspace=(None, 0), rank=0, down=None, up=None, ids=None, scale=None, **kw)), A.last_error()
+        kw.update(rank=16, down_stride=dim, up_stride=16, down=far[3], up=far[4], ids=far[5], scale=far[6])
+        assert checked(linear(workspace=(far[11], hb.linear_workspace(n, outs, dim, dtype, rank=16)), **kw)), A.last_error()
+        assert linear(workspace=(far[11], 4 * n * 16 - 1), **kw) == A.INVALID
