@@ -181,8 +181,12 @@ void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *work
     uint64_t blocks = 0;
     if (n) {
         const uint32_t v = norm_vector(size, dim);
-        // (4 that reach back spill: 65,537 rows of 1,023 f32 356 us, with 2 326)
-        const RowPlan q = row_plan(tiles(dim, v), v, v == 8 || dim % v ? 2 : 4, false);
+        // Two vectors a lane. Four of f32 take 150 registers, which leave a SIMD three
+        // waves: 65,429 rows of 1,024 177 us (153 held to 128 registers, ten of them
+        // put away), 129,844 of 516 197, 216,129 of 310 212; by two on twice the lanes
+        // 147, 168 and 194. Rows that reach back take 206 to 273 us of four and 226 to
+        // 256 of two (515 to 1,023 columns, 67,000,000 elements).
+        const RowPlan q = row_plan(tiles(dim, v), v, 2, false);
         blocks = std::min(tiles(n, q.per()), norm_grad_blocks(dim));
         NormGradArgs a{};
         a.dout = p.dout;

@@ -486,8 +486,9 @@ HBR_NORMS(f32_4, F32, 4, false)
 HBR_NORMS(f32_4r, F32, 4, true)
 HBR_NORMS(bf16_8, Bf16, 8, false)
 HBR_NORMS(bf16_8r, Bf16, 8, true)
-HBR_NORM(f32_2_4, F32, 2, 4, false)
-HBR_NORM(f32_4_4, F32, 4, 4, false)
+// (four vectors a lane: the norm's alone, by workgroups of 256)
+extern "C" __global__ __launch_bounds__(256) void hbr_rms_norm_f32_2_4(NormArgs a) { rms_norm<F32, 2, 4, false>(a); }
+extern "C" __global__ __launch_bounds__(256) void hbr_rms_norm_f32_4_4(NormArgs a) { rms_norm<F32, 4, 4, false>(a); }
 extern "C" __global__ __launch_bounds__(256) void hbr_rms_norm_f32_4r_4(NormArgs a) { rms_norm<F32, 4, 4, true>(a); }
 HBR_PACK(f32_1, F32, 1, false)
 HBR_PACK(f32_4, F32, 4, false)

@@ -1,6 +1,9 @@
 """The operators of the layers between leaf vectors and classes refuse what
 they cannot run, before they touch a device."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -276,3 +279,19 @@ def test_few_rows_need_room_for_their_low_values_alone(dtype):
         kw.update(rank=16, down_stride=dim, up_stride=16, down=far[3], up=far[4], ids=far[5], scale=far[6])
         assert checked(linear(workspace=(far[11], hb.linear_workspace(n, outs, dim, dtype, rank=16)), **kw)), A.last_error()
         assert linear(workspace=(far[11], 4 * n * 16 - 1), **kw) == A.INVALID
+
+
+def test_the_layers_kernels_keep_their_registers(tmp_path):
+    """Rows and tiles that are held in registers are not put away in scratch
+    memory: by the built code object's own counts."""
+    readelf = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "llvm-readelf")
+    if not os.path.exists(readelf):
+        pytest.skip("no llvm-readelf")
+    with open(os.path.join(os.path.dirname(hb.__file__), "lib", "hbrocm_gfx950.hsaco"), "rb") as f:
+        bundle = f.read()
+    code = tmp_path / "code"
+    code.write_bytes(bundle[bundle.index(b"\x7fELF"):])
+    notes = subprocess.run([readelf, "--notes", str(code)], capture_output=True, text=True, check=True).stdout
+    spilled = dict(re.findall(r"\.name: +(hbr_\w+)\n(?:.*\n)*?.*\.vgpr_spill_count: +(\d+)", notes))
+    held = {k: int(v) for k, v in spilled.items() if re.match(r"hbr_(rms_norm|pack|unpack|linear_(y|ya|dx|dw|pair))_", k)}
+    assert len(held) > 60 and not any(held.values()), {k: v for k, v in held.items() if v}
