@@ -45,9 +45,15 @@ uint32_t rows_vector(uint64_t size, uint64_t dim, std::initializer_list<const Ro
 // 183, element by element 542 and 444), and rows shorter than a vector element
 // by element.
 uint32_t row_vector(uint64_t size, uint64_t dim) { return dim >= 16 / size ? (uint32_t)(16 / size) : 1; }
-// Rows of f32 that are whole vectors of 8 bytes only: 161,579 rows of 310 took
-// 174 us, and 197 by vectors of 16 that reach back.
-uint32_t norm_vector(uint64_t size, uint64_t dim) { return size == 4 && dim % 4 == 2 ? 2 : row_vector(size, dim); }
+// Rows of f32 that are whole vectors of 8 bytes only take those up to `most`
+// columns, and beyond vectors of 16 that reach back (67,000,000 elements, us, 8
+// bytes and 16): norm 310 columns 120 and 142, 510 115 and 127, 514 207 and 120,
+// 2,046 135 and 119; gradient 50 162 and 221, 510 176 and 183, 2,046 151 and 247,
+// 2,050 272 and 230, 3,582 206 and 184.
+constexpr uint64_t kNormNarrow = 512, kNormGradNarrow = 2048;
+uint32_t norm_vector(uint64_t size, uint64_t dim, uint64_t most) {
+    return size == 4 && dim % 4 == 2 && dim <= most ? 2 : row_vector(size, dim);
+}
 
 uint64_t scales_of(uint64_t dim) { return tiles(dim, kPackBlock); }
 
@@ -110,7 +116,7 @@ void rms_norm(int ordinal, void *stream, const hbr_norm &p) {
     check_apart({out.extent(), total.extent(), codes.extent(), scales.extent(), {p.inv, n * 4}},
                 {apart(x), apart(residual), {p.weight, dim * 4}}, Extent(nullptr, 0), what);
     Queue queue(ordinal, stream);
-    const uint32_t v = norm_vector(size, dim);
+    const uint32_t v = norm_vector(size, dim, kNormNarrow);
     const RowPlan q = row_plan(tiles(dim, v), v, v == 8 ? 2 : 4, p.codes != nullptr);
     NormArgs a{};
     a.x = p.x;
@@ -180,7 +186,7 @@ void rms_norm_grad(int ordinal, void *stream, const hbr_norm_grad &p, void *work
     Queue queue(ordinal, stream);
     uint64_t blocks = 0;
     if (n) {
-        const uint32_t v = norm_vector(size, dim);
+        const uint32_t v = norm_vector(size, dim, kNormGradNarrow);
         // Two vectors a lane. Four of f32 take 150 registers, which leave a SIMD three
         // waves: 65,429 rows of 1,024 177 us (153 held to 128 registers, ten of them
         // put away), 129,844 of 516 197, 216,129 of 310 212; by two on twice the lanes

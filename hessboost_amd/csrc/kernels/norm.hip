@@ -467,7 +467,7 @@ __device__ __forceinline__ void unpack_rows(const PackArgs &a) {
 
 using namespace hbr;
 
-// V: 16 bytes, or 8 for rows of f32 of whole such, or one element for rows
+// V: 16 bytes, or 8 for short rows of f32 of whole such, or one element for rows
 // shorter than a vector; R: rows of other than whole vectors
 #define HBR_NORM(suffix, E, V, U, R)                                                                                   \
     extern "C" __global__ __launch_bounds__(1024) void hbr_rms_norm_##suffix(NormArgs a) { rms_norm<E, V, U, R>(a); }  \
@@ -481,7 +481,8 @@ using namespace hbr;
     HBR_NORM(suffix##_0, E, V, 0, R)
 HBR_NORM(f32_1_1, F32, 1, 1, false)
 HBR_NORM(bf16_1_1, Bf16, 1, 1, false)
-HBR_NORMS(f32_2, F32, 2, false)
+HBR_NORM(f32_2_1, F32, 2, 1, false)
+HBR_NORM(f32_2_2, F32, 2, 2, false)
 HBR_NORMS(f32_4, F32, 4, false)
 HBR_NORMS(f32_4r, F32, 4, true)
 HBR_NORMS(bf16_8, Bf16, 8, false)

@@ -855,3 +855,34 @@ def test_few_rows_without_adapters_need_no_workspace(dtype):
         out = like((n, outs), dtype)
         hb.linear(dev(x, dtype), dev(w, dtype), out)
         close(back(out), L.linear(x, w, None, None, None, None, None, dtype), "out")
+
+
+# rows, dim: either side of what rows of 8 bytes are taken by, and of what a
+# workgroup's registers hold, by vectors of 8 bytes and of 16
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, dim", [(5, 2), (70, 126), (33, 130), (9, 258), (7, 510), (5, 514), (300, 514), (5, 600), (3, 1018), (3, 1026), (5, 2046),
+                                    (5, 2050), (3, 4094), (3, 4098), (300, 4098), (4, 6002), (3, 8190), (3, 8194), (2, 16_382), (2, 16_386)])
+def test_norms_of_every_width(n, dim, dtype):
+    """And their gradients, from the rows and from 8 bits, in views too."""
+    rng = np.random.default_rng(n + dim)
+    x, r, dout, w = rows(rng, n, dim, dtype), rows(rng, n, dim, dtype), rows(rng, n, dim, dtype, 1.0 / n), f32(rng, dim, 0.3, 1.0)
+    eps, weight = float(np.float32(1e-5)), dev(w, "float32")
+    for pad, lead in ((0, 0), (3, 1)):
+        want = L.norm(x, r, w, eps, dtype)
+        out, total, inv, (codes, scales) = like((n, dim), dtype, pad, lead), like((n, dim), dtype, pad, lead), like(n, "float32"), packed_like(n, dim, pad, lead)
+        hb.rms_norm(dev(x, dtype, pad, lead), out, weight=weight, eps=eps, residual=dev(r, dtype, pad, lead), total=total, inv=inv, codes=codes,
+                    scales=scales, normed=True)
+        close(back(out), want["out"], "out")
+        close(back(total), want["total"], "total")
+        close(back(inv), want["inv"], "inv")
+        held, by = L.values_of(bytes_back(codes), bytes_back(scales)), back(inv)
+        value, off = want["normed"]
+        power = np.repeat(2.0 ** (bytes_back(scales).astype(np.float64) - 127), 32, 1)[:, :dim]
+        close(held, (value, 2.0 ** -4 * (np.abs(value) + off) + 2.0 ** -10 * power + off), "held")
+        ws = work(hb.rms_norm_grad_workspace(n, dim, dtype))
+        for of, args in (((x, None, False), dict(x=dev(x, dtype, pad, lead))), ((held, by, True), dict(codes=codes, scales=scales, inv=inv))):
+            want = L.norm_grad(dout, of[0], of[1], w, r, eps, of[2], dtype)
+            dx, dweight = like((n, dim), dtype, pad, lead), like(dim, "float32")
+            hb.rms_norm_grad(dev(dout, dtype, pad, lead), dx, weight=weight, eps=eps, dtotal=dev(r, dtype, pad, lead), dweight=dweight, workspace=ws, **args)
+            close(back(dx), want["dx"], "dx")
+            close(back(dweight), want["dweight"], "dweight")
