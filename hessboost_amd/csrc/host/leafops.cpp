@@ -9,6 +9,19 @@ namespace hbr {
 
 namespace {
 
+// The widest vector (elements, at most 16 bytes) that divides every row
+// length, stride and address.
+uint32_t vector_width(uint64_t size, std::initializer_list<uint64_t> lengths, std::initializer_list<const void *> ptrs) {
+    uint32_t v = (uint32_t)(16 / size);
+    for (; v > 1; v /= 2) {
+        bool ok = true;
+        for (uint64_t n : lengths) ok = ok && n % v == 0;
+        for (const void *p : ptrs) ok = ok && reinterpret_cast<uint64_t>(p) % (v * size) == 0;
+        if (ok) break;
+    }
+    return v;
+}
+
 // ---- leaf vectors ------------------------------------------------------------------
 
 void check_lookup(const hbr_lookup &p, const char *what) {
@@ -304,6 +317,57 @@ void leaf_embedding_grad(int ordinal, void *stream, const hbr_lookup &p, const v
 // ---- the softmax head ------------------------------------------------------------------
 
 namespace {
+
+dim3 cells_grid(uint64_t cells) { return dim3((uint32_t)std::min<uint64_t>((cells + 255) / 256, 1u << 16)); }
+
+// Rows of `dim` elements as an operand: in place where that can be and `lay` is
+// false, else laid out at `to`. labels: rows that take no part, or null.
+Laid lay_rows(Queue &queue, const void *src, uint64_t stride, uint64_t rows, uint64_t dim, uint32_t dtype, void *to, bool lay,
+              const int32_t *labels) {
+    if (rows == 1) stride = up(dim, 8);
+    if (!lay && head_in_place(src, stride, dim, dtype)) return {static_cast<const char *>(src), stride * 2, 64, 0, (uint32_t)dim};
+    HeadPartsArgs a{};
+    a.src = src;
+    a.labels = labels;
+    a.dst = static_cast<uint16_t *>(to);
+    a.rows = rows;
+    a.src_stride = stride;
+    a.chunk = chunk_bytes(rows) / 2;
+    a.cols = (uint32_t)dim;
+    a.chunks = (uint32_t)tiles(dim, 32);
+    a.part = a.chunks * a.chunk;
+    queue.launch(dtype == HBR_F32 ? "hbr_head_parts_f32" : "hbr_head_parts_bf16", cells_grid(rows * a.chunks * 4), dim3(256), a);
+    return {static_cast<const char *>(to), 64, a.chunk * 2, a.part * 2, a.chunks * 32};
+}
+
+// The head's tiles.
+constexpr HeadTiling kTile256{256, 512, 256, "_256"}, kTile128{128, 256, 512, "_128"};
+
+// Shares of a product's steps: where its tiles are fewer than the device
+// runs at once, enough of them to fill it, of 16 steps at least.
+uint32_t head_splits(const HeadTiling &t, uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t all = tiles(m, t.tile) * tiles(n, t.tile), steps = tiles(k, kHeadK) * segments;
+    return (uint32_t)std::max<uint64_t>(1, std::min(t.slots / std::max<uint64_t>(all, 1), steps / 16));
+}
+
+// The tiles of a product with the gradients: those that take less time, in us:
+// a step of 256 large tiles is one (1.1 PFLOP/s), one of 512 small ones 0.54,
+// and shares' sums are read once more at 4.5 TB/s. Both at their best:
+// 16,384 x 131,072 x 1,024 products of bf16 take 3.9 ms with large tiles and
+// 4.2 with small ones, 8,191 x 32,768 x 512 ones 0.29 and 0.32, 3,229 x 2,810 x
+// 335 ones of f32 with their sums 70 us and 60. (The scores and pairs keep the
+// small ones: four workgroups on a CU hide each other's exponentials and
+// stores. 16,384 x 32,768 pairs of 1,024 take 1.34 ms against 1.35 with large
+// ones, 4,096 x 5,003 ones of 256 in f32 84 us against 119.)
+const HeadTiling &head_tiling(uint64_t m, uint64_t n, uint64_t k, uint64_t segments) {
+    const uint64_t steps = tiles(k, kHeadK) * segments;
+    auto cost = [&](const HeadTiling &t, double step) {
+        const uint64_t shares = head_splits(t, m, n, k, segments);
+        return (double)(tiles(tiles(m, t.tile) * tiles(n, t.tile) * shares, t.slots) * tiles(steps, shares)) * step +
+               (shares > 1 ? (double)(shares * m * n) * 4.0 / 4.5e6 : 0.0);
+    };
+    return cost(kTile256, 1.0) <= cost(kTile128, 0.54) ? kTile256 : kTile128;
+}
 
 // The scores' gradients of one piece of the classes are held at a time, in at
 // most about this many bytes.
