@@ -424,9 +424,13 @@ void check_tiles(uint64_t m, uint64_t n, const char *what) {
 
 // Whether w is read straight into the matrix instructions' registers: up to 64
 // rows, which are read again with every 16 outputs. In f32 always (32 rows,
-// 4,096 x 4,096: 30 us, 71 in tiles of three parts); in bf16 while those reads
-// take less than the tiles' stages and shares (64 rows: 1,024 x 4,096 10.2 us,
-// 12.9 in tiles, 4,096 x 8,192 39.5 and 20.5; 32 rows 25.6 and 20.5).
+// 4,096 x 4,096: 29 us, 60 in tiles of three parts); in bf16 while those reads
+// take less than the tiles' stages and shares (64 rows: 1,024 x 4,096 7.4 us,
+// 11.9 in tiles, 4,096 x 8,192 38.7 and 20.9; 32 rows 25.2 and 20.2). Of 40 cases
+// each of 1 to 64 rows, 512 to 8,192 columns and 1,024 to 16,384 outputs that is the
+// slower way in seven of bf16 and three of f32, most of them long rows by few outputs,
+// whose workgroups leave CUs idle (32 rows of 8,192 by 1,024 bf16 23.1 us and 14.6, 64
+// of f32 74.8 and 43.0).
 bool few_rows(uint64_t n, uint64_t outs, uint64_t dim, uint32_t dtype) {
     return n <= 64 && (dtype == HBR_F32 || n <= 16 || tiles(n, 16) * outs * dim * 2 <= 48u << 20);
 }

@@ -8,11 +8,11 @@
 // theirs take three products and not six.
 //
 // Measured (us, and what a large product's 1,361 TFLOP/s would take): 65,536 rows of
-// 1,024 by 4,096 bf16, both gradients out of rows in 8 bits 944 to 972 (808), of
-// which dx 457 to 506, dw 469 to 528, codes laid out 45, shares joined 20; 8,191 rows
-// forward 72 (50), with 64 adapters of rank 16 in 50 runs 90 (52); 7 rows, each its
-// own adapter, 15 for the call, 5 a kernel; 4,001 x 250 by 333 f32, both gradients,
-// 35 in three short kernels.
+// 1,024 by 4,096 bf16, both gradients out of rows in 8 bits 944 to 990 (808), of
+// which dx 446 to 511, dw 459 to 535, codes laid out 46 to 51, shares joined 20 to 22;
+// 8,191 rows forward 73 to 78 (50), with 64 adapters of rank 16 in 50 runs 94 to 99
+// (52), in random order 297 to 308; 7 rows, each its own adapter, 15 for the call, 5 a
+// kernel; 4,001 x 250 by 333 f32, both gradients, 36 in three short kernels.
 #include <type_traits>
 
 #include "tile_product.h"

@@ -4,16 +4,18 @@
 //   g = dout weight; dx = inv (g - n mean(g n)) + dtotal; dweight = sum over rows dout n
 //
 // A row lies on `lanes` lanes and stays in their registers between its sum and
-// its results: it is read once and written once. A lane's columns are the same
+// its results: up to 16,384 columns of bf16 and 8,192 of f32 it is read once and
+// written once, beyond it is read again for every use. A lane's columns are the same
 // in every row, so that the weights are loaded once and the weights' gradient is
 // summed in registers, joined in LDS and over the workgroups in order.
 //
 // Memory bounds all of it. Measured, against a large copy's 5.15 TB/s: 65,537 rows
-// of 1,024 bf16 with a residual, their sum and codes written too, 167 us (157 at
-// the copy's rate); their gradient 109 us (104); 262,144 x 1,024 bf16 into codes
-// and back 289 us (317: some of the codes come out of a cache); one row 9 us, all
-// of it the launch. Rows of other than whole vectors: 10,058 x 6,661 bf16 226 us
-// (157), gradient 148 (104).
+// of 1,024 bf16 with a residual, their sum and codes written too and the codes read
+// back, 167 us (157 at the copy's rate); the gradient out of the codes, with dtotal,
+// 108 us (92); 262,144 x 1,024 bf16 into codes and back 287 us (317: some of the codes
+// come out of a cache); one row 9 us, all of it the launch. Rows of other than whole
+// vectors: 10,058 x 6,661 bf16 the same 226 us (157), the gradient out of the rows
+// 149 (104).
 #include "rows8.h"
 
 namespace hbr {

@@ -146,7 +146,7 @@ def rms_norm_grad(dout, dx=None, *, x=None, codes=None, scales=None, inv=None, w
 
 def linear_workspace(n, outs, dim, dtype, rank=0):
     """The bytes linear needs for n rows or fewer, with adapters of the rank
-    or less."""
+    or less (a few rows without adapters need none)."""
     out = C.c_uint64()
     A.check(A.lib().hbr_linear_workspace(_size(n, "n", 64), _size(outs, "outs"), _size(dim, "dim"), _size(rank, "rank"),
                                          _code(dtype), C.byref(out)))
